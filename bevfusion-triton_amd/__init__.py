@@ -22,6 +22,7 @@ The directory name is not a Python identifier; load it with
 """
 from . import legacy
 from ._lib import BevPoolError, LibraryNotBuilt, library
+from .attention import attend_packed, axis_frequencies, norm_rotate
 from .bev_pool import BevPoolFunction, BevPoolIndexExport, bev_pool, check_errors
 from .vtransform import (BevPoolTransform, CameraIndex, LSSIndexExport, create_frustum, gen_dx_bx, host_grid, lss_bev_pool, lss_bev_pool_depth,
                          lss_index_cameras)
@@ -34,6 +35,8 @@ __all__ = [
     'CameraIndex',
     'LSSIndexExport',
     'LibraryNotBuilt',
+    'attend_packed',
+    'axis_frequencies',
     'bev_pool',
     'check_errors',
     'create_frustum',
@@ -44,4 +47,5 @@ __all__ = [
     'lss_bev_pool',
     'lss_bev_pool_depth',
     'lss_index_cameras',
+    'norm_rotate',
 ]

@@ -41,6 +41,8 @@ _i64 = ctypes.c_int64
 _sz = ctypes.c_size_t
 _f3 = ctypes.c_float * 3
 _i3 = ctypes.c_int32 * 3
+_i32p = ctypes.POINTER(ctypes.c_int32)
+_f32 = ctypes.c_float
 
 _SIGNATURES = {
     'bevpool_abi_version': ([], ctypes.c_int),
@@ -125,6 +127,23 @@ _SIGNATURES = {
     ),
     'bevpool_planar_kept_rows': (
         [_vp, _i64, _i64, _i32, _i32, _i64, _vp, _vp, _vp], ctypes.c_int,
+    ),
+    'bevpool_norm_rotate_forward': (
+        [_vp, _i64, _i64, _i32, _vp, _i64, _i64, _i32, _i32, _i64, _i32, _vp, _i32, _i64, _vp,
+         _i32p, _i32, _i32, _vp, _vp, _f32, _vp, _vp, _vp],
+        ctypes.c_int,
+    ),
+    'bevpool_norm_rotate_backward_scratch_bytes': ([_i32], _sz),
+    'bevpool_norm_rotate_backward': (
+        [_vp, _i64, _i64, _i32, _vp, _i64, _i64, _i32, _vp, _i64, _i64, _vp, _i64, _i64, _i32,
+         _i64, _i32, _vp, _i32, _i64, _vp, _i32p, _i32, _i32, _vp, _vp, _f32, _vp, _vp, _vp, _vp,
+         _vp, _sz, _vp],
+        ctypes.c_int,
+    ),
+    'bevpool_attention_forward': (
+        [_vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _i32, _i64, _i64, _i32, _i32, _i32,
+         _vp, _vp, _i32, _i32, _f32, _vp, _vp, _vp],
+        ctypes.c_int,
     ),
     'bevpool_timing_enable': ([ctypes.c_int], ctypes.c_int),
     'bevpool_timing_reset': ([], ctypes.c_int),

@@ -1,0 +1,279 @@
+"""Token operators on MI355X: norm and rotation of queries and keys, and
+attention over packed sequences.
+
+What a transformer over camera and BEV tokens needs after the pooling, as HIP
+kernels behind the same C ABI (``include/bevpool.h``); the reference has no
+counterpart.
+
+  * :func:`norm_rotate`      RMS norm of each head and rotary positions with
+                             several axes (frame, row, column), one pass
+  * :func:`axis_frequencies` the usual frequency ladders for it
+  * :func:`attend_packed`    attention over packed sequences of different
+                             lengths, causal or not, grouped heads
+
+Both operators have gradients.  Operands are fp32, fp16 or bf16 (rows, heads,
+dim) tensors; any strides are taken, so parts of one projection's output need
+no copy (attention copies an operand whose rows or heads do not start at
+multiples of 16 bytes).  Calls run on torch's current stream, allocate with
+torch's allocator and never wait for the device.
+"""
+from __future__ import annotations
+
+import ctypes
+
+import torch
+
+from . import _lib as L
+from . import _pipeline as P
+
+_POSITION_KINDS = {torch.int32: 0, torch.int64: 1, torch.float32: 2}
+MAX_AXES = 4
+
+
+def axis_frequencies(pairs, base=10000.0, *, shared=False, device=None):
+    """Frequencies (radians per unit of position) of ``sum(pairs)`` rotated
+    pairs, ``pairs[i]`` of them turned by axis i: ``base ** (-j / n)``.  Each
+    axis has a ladder of its own (j, n within the axis), or, with ``shared``,
+    all share one over all the pairs in order."""
+    pairs = [int(n) for n in pairs]
+    if any(n < 0 for n in pairs):
+        raise ValueError('pairs must not be negative')
+    ladders = [sum(pairs)] if shared else pairs
+    parts = [float(base) ** (-torch.arange(n, dtype=torch.float64) / max(n, 1)) for n in ladders]
+    return torch.cat(parts).to(device, torch.float32)
+
+
+def _check_rows(name, x, dims=3):
+    if x.dim() != dims:
+        raise ValueError(f'{name} must have {dims} dimensions (..., heads, dim).')
+    if x.dtype not in L.DTYPE_CODES:
+        raise TypeError(f'{name} must have dtype torch.float16, torch.float32, or torch.bfloat16.')
+
+
+def _check_same(name, x, like):
+    if x.dtype != like.dtype:
+        raise TypeError(f'{name} must have the dtype of q ({like.dtype}).')
+    if x.device != like.device:
+        raise ValueError(f'{name} must be on the device of q ({like.device}).')
+
+
+def _unit(x):
+    """x with unit stride along its last dimension."""
+    return x if x.stride(-1) == 1 or x.shape[-1] == 1 else x.contiguous()
+
+
+def _strides(x):
+    return (L.ptr(x), x.stride(0), x.stride(1)) if x is not None else (0, 0, 0)
+
+
+def _run(call, device, what):
+    with torch.cuda.device(device):
+        L.check(call(L.library(), L.stream_handle(device)), what)
+
+
+# ---- norm and rotation -----------------------------------------------------
+
+class _NormRotate(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, q_weight, k_weight, positions, frequencies, pairs, eps, interleaved):
+        q = _unit(q)
+        k = _unit(k) if k is not None else None
+        tokens, q_heads, dim = q.shape
+        k_heads = k.shape[1] if k is not None else 0
+        q_out = torch.empty((tokens, q_heads, dim), dtype=q.dtype, device=q.device)
+        k_out = None if k is None else torch.empty((tokens, k_heads, dim), dtype=q.dtype,
+                                                   device=q.device)
+        ctx.call = (tokens, q_heads, k_heads, dim, q.dtype, pairs, eps, interleaved)
+        # (a rotation alone needs no input for its gradient)
+        ctx.save_for_backward(q if q_weight is not None else None,
+                              k if k_weight is not None else None, q_weight, k_weight, positions,
+                              frequencies)
+        _run(lambda lib, s: lib.bevpool_norm_rotate_forward(
+            *_strides(q), q_heads, *_strides(k), k_heads, L.DTYPE_CODES[q.dtype], tokens, dim,
+            *_rotation(positions, frequencies, pairs, interleaved), L.ptr(q_weight),
+            L.ptr(k_weight), eps, L.ptr(q_out), L.ptr(k_out), s), q.device,
+            'bevpool_norm_rotate_forward')
+        return q_out, k_out
+
+    @staticmethod
+    def backward(ctx, dq_out, dk_out):
+        q, k, q_weight, k_weight, positions, frequencies = ctx.saved_tensors
+        tokens, q_heads, k_heads, dim, dtype, pairs, eps, interleaved = ctx.call
+        dev = positions.device
+
+        def grad_rows(g, heads):
+            if heads == 0:
+                return None
+            if g is None:  # an output that nothing was computed from
+                return torch.zeros((tokens, heads, dim), dtype=dtype, device=dev)
+            return _unit(g.to(dtype))
+
+        dq_out, dk_out = grad_rows(dq_out, q_heads), grad_rows(dk_out, k_heads)
+        dq = torch.empty((tokens, q_heads, dim), dtype=dtype, device=dev)
+        dk = torch.empty((tokens, k_heads, dim), dtype=dtype, device=dev) if k_heads else None
+        dqw = torch.empty_like(q_weight) if q_weight is not None else None
+        dkw = torch.empty_like(k_weight) if k_weight is not None else None
+        lib = L.library()
+        nbytes = lib.bevpool_norm_rotate_backward_scratch_bytes(dim)
+        normed = dqw is not None or dkw is not None
+        scratch = torch.empty(nbytes, dtype=torch.uint8, device=dev) if normed else None
+        _run(lambda lib, s: lib.bevpool_norm_rotate_backward(
+            *_strides(q), q_heads, *_strides(k), k_heads, *_strides(dq_out), *_strides(dk_out),
+            L.DTYPE_CODES[dtype], tokens, dim,
+            *_rotation(positions, frequencies, pairs, interleaved), L.ptr(q_weight),
+            L.ptr(k_weight), eps, L.ptr(dq), L.ptr(dk), L.ptr(dqw), L.ptr(dkw), L.ptr(scratch),
+            nbytes if normed else 0, s), dev, 'bevpool_norm_rotate_backward')
+        return dq, dk, dqw, dkw, None, None, None, None, None
+
+
+def _rotation(positions, frequencies, pairs, interleaved):
+    return (L.ptr(positions), _POSITION_KINDS[positions.dtype],
+            positions.stride(0) if positions.shape[0] else 0, L.ptr(frequencies),
+            (ctypes.c_int32 * max(1, len(pairs)))(*pairs), len(pairs), int(interleaved))
+
+
+def norm_rotate(q, k, positions, frequencies, pairs=None, *, q_weight=None, k_weight=None,
+                eps=1e-6, interleaved=False):
+    """RMS norm of queries and keys for each head (where a weight is given),
+    then rotation by positions with several axes; returns (q, k) contiguous.
+
+    q (tokens, q_heads, dim) and k (tokens, k_heads, dim) or None, dim even and
+    at most 256.  positions (tokens,) or (tokens, axes), int32, int64 or
+    float32.  frequencies (P,) fp32, 2 P <= dim; ``pairs[i]`` of them (in
+    order, ``sum(pairs) == P``; default: all, one axis) turn by axis i.  Pair p
+    is the elements (p, P + p) of a head, or (2p, 2p + 1) with
+    ``interleaved``; the elements from 2 P on are not turned.  q_weight,
+    k_weight (dim,): n = x / sqrt(mean(x^2) + eps) * weight in fp32.
+    Gradients flow to q, k and the weights."""
+    _check_rows('q', q)
+    tokens, _, dim = q.shape
+    if k is not None:
+        _check_rows('k', k)
+        _check_same('k', k, q)
+        if k.shape[0] != tokens or k.shape[2] != dim:
+            raise ValueError('q and k must agree on tokens and dim.')
+    elif k_weight is not None:
+        raise ValueError('k_weight without k.')
+    if dim % 2 or not 2 <= dim <= 256:
+        raise ValueError('dim must be even and at most 256.')
+    if positions.dim() == 1:
+        positions = positions.unsqueeze(1)
+    if positions.dim() != 2 or positions.shape[0] != tokens:
+        raise ValueError('positions must have shape [tokens] or [tokens, axes].')
+    if positions.dtype not in _POSITION_KINDS:
+        raise TypeError('positions must have dtype torch.int32, torch.int64 or torch.float32.')
+    if frequencies.dim() != 1 or frequencies.dtype != torch.float32:
+        raise ValueError('frequencies must be a 1-d float32 tensor.')
+    pairs = (frequencies.shape[0],) if pairs is None else tuple(int(n) for n in pairs)
+    if len(pairs) > MAX_AXES or any(n < 0 for n in pairs):
+        raise ValueError(f'pairs must be at most {MAX_AXES} numbers, none negative.')
+    if sum(pairs) != frequencies.shape[0] or 2 * sum(pairs) > dim:
+        raise ValueError('pairs must sum to the number of frequencies, at most dim / 2.')
+    if positions.shape[1] < len(pairs):
+        raise ValueError('positions must have a column for each axis.')
+    if not eps >= 0:
+        raise ValueError('eps must not be negative.')
+    for name, w in (('q_weight', q_weight), ('k_weight', k_weight)):
+        if w is not None:
+            if tuple(w.shape) != (dim,):
+                raise ValueError(f'{name} must have shape [dim].')
+            _check_same(name, w, q)
+    P.require_gpu(q, positions, frequencies, *[t for t in (k, q_weight, k_weight) if t is not None])
+    for name, t in (('positions', positions), ('frequencies', frequencies)):
+        if t.device != q.device:
+            raise ValueError(f'{name} must be on the device of q ({q.device}).')
+    weights = [w if w is None else w.contiguous() for w in (q_weight, k_weight)]
+    return _NormRotate.apply(q, k, *weights, _unit(positions), frequencies.contiguous(), pairs,
+                             float(eps), bool(interleaved))
+
+
+# ---- attention over packed sequences ---------------------------------------
+
+def _aligned(x):
+    """x with unit stride along dim and every row and head at a multiple of 16
+    bytes, as the kernels' 16-byte accesses need: itself, or a copy."""
+    per = 16 // x.element_size()
+    if x.stride(-1) == 1 and x.data_ptr() % 16 == 0 and all(s % per == 0 for s in x.stride()[:-1]):
+        return x
+    return x.contiguous() if not x.is_contiguous() else x.clone()
+
+
+def _check_heads(q, k, v):
+    _check_rows('q', q, q.dim())
+    for name, x in (('k', k), ('v', v)):
+        _check_rows(name, x, x.dim())
+        _check_same(name, x, q)
+    if k.shape != v.shape:
+        raise ValueError('k and v must have the same shape.')
+    dim = q.shape[-1]
+    if k.shape[-1] != dim:
+        raise ValueError('q and k must have the same dim.')
+    if dim % 8 or not 8 <= dim <= 128:
+        raise ValueError('dim must be a multiple of 8, at most 128.')
+    if q.shape[-2] < 1 or k.shape[-2] < 1 or q.shape[-2] % k.shape[-2]:
+        raise ValueError('the number of query heads must be a multiple of that of key heads.')
+
+
+def _check_scale(scale, dim):
+    scale = dim ** -0.5 if scale is None else float(scale)
+    if not 0.0 < scale < float('inf'):
+        raise ValueError('scale must be positive and finite.')
+    return scale
+
+
+def _check_starts(name, starts, like):
+    if starts.dim() != 1 or starts.shape[0] < 1:
+        raise ValueError(f'{name} must have shape [sequences + 1].')
+    if starts.dtype not in (torch.int32, torch.int64):
+        raise TypeError(f'{name} must have dtype torch.int32 or torch.int64.')
+    if starts.device != like.device:
+        raise ValueError(f'{name} must be on the device of q ({like.device}).')
+    return starts.to(torch.int32).contiguous()
+
+
+class _AttendPacked(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, q_starts, k_starts, causal, scale):
+        q, k, v = _aligned(q), _aligned(k), _aligned(v)
+        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        lse = torch.empty(q.shape[:2], dtype=torch.float32, device=q.device)
+        _run(lambda lib, s: lib.bevpool_attention_forward(
+            *_strides(q), *_strides(k), *_strides(v), L.DTYPE_CODES[q.dtype], q.shape[0],
+            k.shape[0], q.shape[1], k.shape[1], q.shape[2], L.ptr(q_starts), L.ptr(k_starts),
+            q_starts.shape[0] - 1, int(causal), scale, L.ptr(out), L.ptr(lse), s), q.device,
+            'bevpool_attention_forward')
+        ctx.mark_non_differentiable(lse)
+        return out, lse
+
+
+def attend_packed(q, k, v, q_starts, k_starts=None, *, causal=False, scale=None,
+                  return_lse=False):
+    """Attention within packed sequences of different lengths.
+
+    q (q_total, q_heads, dim), k and v (k_total, k_heads, dim), q_heads a
+    multiple of k_heads (query head h reads key head h // (q_heads /
+    k_heads)), dim a multiple of 8 up to 128.  Sequence i has the queries
+    [q_starts[i], q_starts[i + 1]) and the keys [k_starts[i], k_starts[i + 1])
+    (default: as the queries); both are int32 or int64 tensors on the device,
+    ascending from 0, and are never read back.  With ``causal``, query j of a
+    sequence sees its keys up to j + (keys - queries): the last query sees
+    all.  out = softmax(scale * q k) v (scale: dim ** -0.5); a query that sees
+    no key or is in no sequence gives zeros and passes no gradient.  With
+    ``return_lse`` also the logarithm of each query's sum of exponentials,
+    (q_total, q_heads) fp32 (-inf without keys, no gradient)."""
+    for name, x in (('q', q), ('k', k), ('v', v)):
+        _check_rows(name, x)
+    _check_heads(q, k, v)
+    scale = _check_scale(scale, q.shape[2])
+    P.require_gpu(q, k, v)
+    q_starts = _check_starts('q_starts', q_starts, q)
+    if k_starts is None:
+        if k.shape[0] != q.shape[0]:
+            raise ValueError('without k_starts, q and k must have the same number of tokens.')
+        k_starts = q_starts
+    else:
+        k_starts = _check_starts('k_starts', k_starts, q)
+    if k_starts.shape != q_starts.shape:
+        raise ValueError('q_starts and k_starts must have the same length.')
+    out, lse = _AttendPacked.apply(q, k, v, q_starts, k_starts, bool(causal), scale)
+    return (out, lse) if return_lse else out

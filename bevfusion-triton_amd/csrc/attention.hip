@@ -1,0 +1,267 @@
+// attention.hip -- attention over packed sequences, forward (gfx950).
+//
+//   s_ij = scale q_i k_j over the keys j that query i sees,
+//   L_i = log sum_j exp(s_ij),  o_i = sum_j exp(s_ij - L_i) v_j
+// for sequences of nq queries and nk keys; causal: j <= i + nk - nq.  A
+// query that sees no key has o = 0 and L = -inf.
+#include "attention_tiles.h"
+#include "host_calls.h"
+
+namespace {
+
+using namespace attention;
+using bevpool_host::check_grid;
+using bevpool_host::check_launch;
+using bevpool_host::fail;
+using bevpool_host::LaunchScope;
+
+// Running softmax of one row: a lane and lane ^ 32 share it, with half of a
+// block's keys each.
+struct Softmax {
+  float top = -kInf;  // the maximum that the weights are relative to
+  float sum = 0.f;    // of this lane's half of the keys
+};
+
+// Takes kN scores of this lane's row (raw products, -inf where masked):
+// they become weights exp2(scale_log2 (s - top)).  top follows the maximum
+// only where the row's new maximum is more than kSlack above it (in log2),
+// so most blocks leave the sums as they are: weights stay below 2^kSlack,
+// far from the types' largest values, and relative to each other as exact.
+constexpr float kSlack = 8.f;
+template <int kN, int kB>
+__device__ __forceinline__ void softmax_step(float (&s)[kN], Softmax &x, f32x16 (&out)[kB],
+                                             float scale_log2) {
+  float most = s[0];
+#pragma unroll
+  for (int i = 1; i < kN; ++i) most = fmaxf(most, s[i]);
+  most = max_halves(most);
+  // (no comparison is true for a row that has seen nothing but -inf)
+  if (__ballot((most - x.top) * scale_log2 > kSlack)) {
+    const float top = fmaxf(most, x.top);
+    const float by = top == -kInf ? 1.f : exp2_fast((x.top - top) * scale_log2);
+    x.top = top;
+    x.sum *= by;
+#pragma unroll
+    for (int b = 0; b < kB; ++b)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) out[b][r] *= by;
+  }
+  const float shift = x.top == -kInf ? 0.f : x.top * scale_log2;
+  float sum = 0.f;
+#pragma unroll
+  for (int i = 0; i < kN; ++i) {
+    s[i] = exp2_fast(fmaf(s[i], scale_log2, -shift));
+    sum += s[i];
+  }
+  x.sum += sum;
+}
+
+// Rows of a tile are pairs (query, head of the group), the group's heads next
+// to each other: the heads that share keys share their tiles, and short
+// sequences still fill rows.  A wave has 32 rows and all of the tile's keys;
+// K and V tiles are staged in two buffers, the next one's loads in flight
+// while one is used.
+template <typename T, int DP, int kKeys>
+__global__ __launch_bounds__(kThreads, sizeof(T) == 4 && DP > 64 ? 1 : 2) void packed_forward_kernel(
+    PackedArgs A) {
+  using S = Shape<T, DP>;
+  extern __shared__ __attribute__((aligned(16))) char lds[];
+  constexpr int kTile = S::tile_bytes(kKeys);  // buffers: K0 V0 K1 V1
+  constexpr int kRows = kWaves * kWaveRows;
+  const int head = blockIdx.x % A.k_heads;
+  // late tiles, the long ones of a causal sequence, start first
+  const int index = A.tiles - 1 - int(blockIdx.x / A.k_heads);
+  int first;
+  const int which = find_sequence(A.q_starts, A.sequences, A.q_total, A.group.size, kRows, index,
+                                  &first);
+  Sequence seq = sequence_at(A.q_starts, A.k_starts, which, A.sequences, A.q_total, A.k_total);
+  if (which == A.sequences) seq.nq = A.q_total - seq.q0;  // rows of no sequence: no keys
+  const int rows = seq.nq * A.group.size;
+  const int r0 = (index - first) * kRows;
+  if (r0 >= rows) return;
+
+  const int lane = lane_id(), wave = wave_id(), c = lane & 31, h = lane >> 5;
+  const int row = r0 + wave * kWaveRows + c;
+  const bool valid = row < rows;
+  const int row_in = valid ? row : rows - 1;
+  const int query = A.group.div(row_in);
+  const int q_head = head * A.group.size + row_in - query * A.group.size;
+  const int64_t token = seq.q0 + query;
+  const int ahead = seq.nk - seq.nq;  // causal: query i sees keys up to i + ahead
+  // keys [0, limit) are this row's; keys of the block's last row
+  const int limit = A.causal ? min(seq.nk, query + ahead + 1) : seq.nk;
+  const int last_query = A.group.div(min(r0 + kRows, rows) - 1);
+  const int keys = A.causal ? max(0, min(seq.nk, last_query + ahead + 1)) : seq.nk;
+  const int tiles = (keys + kKeys - 1) / kKeys;
+  // the wave's least limit (no mask below it) and its greatest (nothing above)
+  const int w0 = r0 + wave * kWaveRows;
+  const int low = A.causal ? min(seq.nk, A.group.div(min(w0, rows - 1)) + ahead + 1) : seq.nk;
+  const int high = A.causal
+                       ? min(seq.nk, A.group.div(min(w0 + kWaveRows, rows) - 1) + ahead + 1)
+                       : seq.nk;
+  const bool wave_on = w0 < rows;
+
+  Frags<T, DP> q;
+  row_frags<T, DP>(q, A.q.at + token * A.q.row + q_head * A.q.head, A.chunks, true);
+  const char *k_at = A.k.at + seq.k0 * A.k.row + head * A.k.head;
+  const char *v_at = A.v.at + seq.k0 * A.v.row + head * A.v.head;
+  auto load_tile = [&](int t) {
+    char *to = lds + (t & 1) * 2 * kTile;
+    const int k0 = t * kKeys, most = seq.nk - 1;
+    stage<T, DP, kKeys, kThreads>(to, threadIdx.x, A.chunks, [&](int r) {
+      return k_at + int64_t(min(k0 + r, most)) * A.k.row;
+    });
+    stage<T, DP, kKeys, kThreads>(to + kTile, threadIdx.x, A.chunks, [&](int r) {
+      return v_at + int64_t(min(k0 + r, most)) * A.v.row;
+    });
+  };
+  clear_rest<T, DP>(lds, 4 * kKeys, threadIdx.x, kThreads, A.chunks);
+
+  Sums<T, DP> out = {};
+  Softmax x;
+  if (tiles > 0) load_tile(0);
+  for (int t = 0; t < tiles; ++t) {
+    wait_loads<0>();
+    __syncthreads();  // tile t is there, and tile t - 1 has been read
+    if (t + 1 < tiles) load_tile(t + 1);
+    const char *k_tile = lds + (t & 1) * 2 * kTile, *v_tile = k_tile + kTile;
+    const int k0 = t * kKeys;
+    if (!wave_on || k0 >= high) continue;
+    float s[kKeys / 2];
+#pragma unroll
+    for (int b = 0; b < kKeys / 32; ++b) {
+      const f32x16 dots = dot_rows<T, DP>(k_tile, 32 * b, q);
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s[16 * b + r] = dots[r];
+    }
+    if (k0 + kKeys > low) {
+#pragma unroll
+      for (int b = 0; b < kKeys / 32; ++b)
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          if (k0 + 32 * b + c_row(r, h) >= limit) s[16 * b + r] = -kInf;
+    }
+    softmax_step(s, x, out, A.scale_log2);
+#pragma unroll
+    for (int b = 0; b < kKeys / 32; ++b) {
+      float p[16];
+#pragma unroll
+      for (int r = 0; r < 16; ++r) p[r] = s[16 * b + r];
+      Weights<T> w;
+      w.set(p);
+      add_transposed<T, DP>(out, v_tile, 32 * b, w);
+    }
+  }
+
+  const float sum = sum_halves(x.sum);
+  const bool any = x.top > -kInf || sum != 0.f;
+  store_row<T, DP>(A.out.at + token * A.out.row + q_head * A.out.head, out,
+                   any ? 1.f / sum : 0.f, A.dim, valid);
+  if (valid && h == 0 && A.lse)
+    A.lse[token * A.q_heads + q_head] =
+        any ? (x.top * A.scale_log2 + __builtin_amdgcn_logf(sum)) / kLog2e : -kInf;
+}
+
+template <typename T, int DP>
+int launch_forward(const PackedArgs &A, hipStream_t s) {
+  constexpr int kKeys = sizeof(T) == 4 ? 32 : 64;
+  constexpr int kLds = 4 * Shape<T, DP>::tile_bytes(kKeys);
+  static_assert(kLds <= 160 * 1024, "LDS of a CU");
+  const int64_t blocks = int64_t(A.tiles) * A.k_heads;
+  int st = check_grid(blocks, kThreads, "attention forward");
+  if (st) return st;
+  LaunchScope scope("attention_forward", s);
+  hipLaunchKernelGGL((packed_forward_kernel<T, DP, kKeys>), dim3(unsigned(blocks)),
+                     dim3(kThreads), kLds, s, A);
+  return check_launch("attention forward");
+}
+
+}  // namespace
+
+namespace attention {
+
+// Shared by forward and backward: sizes and operands of a packed call.
+int check_packed(PackedArgs &A, int dtype, int64_t q_total, int64_t k_total, int sequences,
+                 int q_heads, int k_heads, int dim, const void *q_starts, const void *k_starts,
+                 int causal, float scale) {
+  if (dtype < BEVPOOL_F32 || dtype > BEVPOOL_BF16)
+    return fail(BEVPOOL_EINVAL, "unsupported dtype code %d", dtype);
+  if (q_total < 0 || k_total < 0 || sequences < 0)
+    return fail(BEVPOOL_EINVAL, "negative number of tokens or sequences");
+  if (q_heads < 1 || k_heads < 1 || q_heads % k_heads)
+    return fail(BEVPOOL_EINVAL, "%d query heads are no multiple of %d key heads", q_heads,
+                k_heads);
+  if (dim < 8 || dim > 128 || dim % 8)
+    return fail(BEVPOOL_EINVAL, "head size %d: must be a multiple of 8 up to 128", dim);
+  if (!(scale > 0.f) || !(scale < 3e38f))
+    return fail(BEVPOOL_EINVAL, "scale must be positive and finite");
+  const int64_t group = q_heads / k_heads;
+  if (q_total * group * group >= (int64_t(1) << 31) || k_total >= (int64_t(1) << 31) - 256)
+    return fail(BEVPOOL_EINVAL, "too many tokens (%lld queries in groups of %lld, %lld keys)",
+                (long long)q_total, (long long)group, (long long)k_total);
+  if ((q_total > 0 || k_total > 0) && (!q_starts || !k_starts))
+    return fail(BEVPOOL_EINVAL, "null starts");
+  A.q_starts = static_cast<const int32_t *>(q_starts);
+  A.k_starts = static_cast<const int32_t *>(k_starts);
+  A.sequences = sequences;
+  A.q_total = int(q_total);
+  A.k_total = int(k_total);
+  A.q_heads = q_heads;
+  A.k_heads = k_heads;
+  A.group = make_group(int(group));
+  A.dim = dim;
+  A.chunks = dim * (dtype == BEVPOOL_F32 ? 4 : 2) / 16;
+  A.causal = causal != 0;
+  A.scale = scale;
+  A.scale_log2 = scale * kLog2e;
+  return BEVPOOL_OK;
+}
+
+int set_operand(Operand &o, const char *what, const void *at, int64_t row, int64_t head, int elem,
+                int64_t total) {
+  o.at = static_cast<char *>(const_cast<void *>(at));
+  o.row = row * elem;
+  o.head = head * elem;
+  if (total > 0 && !at) return fail(BEVPOOL_EINVAL, "%s: null", what);
+  if (total > 0 && (reinterpret_cast<uintptr_t>(at) % 16 || o.row % 16 || o.head % 16))
+    return fail(BEVPOOL_EINVAL, "%s: rows and heads must start at multiples of 16 bytes", what);
+  return BEVPOOL_OK;
+}
+
+}  // namespace attention
+
+#define ATTENTION_DIM(T, FN, ...)                                                   \
+  dim <= 32   ? FN<T, 32>(__VA_ARGS__)                                              \
+  : dim <= 64 ? FN<T, 64>(__VA_ARGS__)                                              \
+  : dim <= 80 ? FN<T, 80>(__VA_ARGS__)                                              \
+  : dim <= 96 ? FN<T, 96>(__VA_ARGS__)                                              \
+              : FN<T, 128>(__VA_ARGS__)
+
+extern "C" {
+
+int bevpool_attention_forward(const void *q, int64_t q_row, int64_t q_head, const void *k,
+                              int64_t k_row, int64_t k_head, const void *v, int64_t v_row,
+                              int64_t v_head, int32_t dtype, int64_t q_total, int64_t k_total,
+                              int32_t q_heads, int32_t k_heads, int32_t dim,
+                              const int32_t *q_starts, const int32_t *k_starts, int32_t sequences,
+                              int32_t causal, float scale, void *out, float *lse, void *stream) {
+  bevpool_host::clear_error();
+  PackedArgs A = {};
+  const int elem = dtype == BEVPOOL_F32 ? 4 : 2;
+  int st = check_packed(A, dtype, q_total, k_total, sequences, q_heads, k_heads, dim, q_starts,
+                        k_starts, causal, scale);
+  if (!st) st = set_operand(A.q, "q", q, q_row, q_head, elem, q_total);
+  if (!st) st = set_operand(A.k, "k", k, k_row, k_head, elem, k_total);
+  if (!st) st = set_operand(A.v, "v", v, v_row, v_head, elem, k_total);
+  if (!st) st = set_operand(A.out, "out", out, int64_t(q_heads) * dim, dim, elem, q_total);
+  if (st) return st;
+  if (q_total == 0) return BEVPOOL_OK;
+  A.lse = lse;
+  A.tiles = int(q_total * A.group.size / (kWaves * kWaveRows)) + sequences + 1;
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  return dtype == BEVPOOL_BF16  ? (ATTENTION_DIM(__bf16, launch_forward, A, s))
+         : dtype == BEVPOOL_F16 ? (ATTENTION_DIM(_Float16, launch_forward, A, s))
+                                : (ATTENTION_DIM(float, launch_forward, A, s));
+}
+
+}  // extern "C"

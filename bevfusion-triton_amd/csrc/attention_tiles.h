@@ -1,0 +1,392 @@
+// Tiles, fragments and work lists shared by the attention kernels (gfx950).
+//
+// Everything is built on the 32 x 32 matrix instructions, one tile a wave.
+// With lane = 32 h + c:
+//   A (32 x K): lane holds row c, B (K x 32): lane holds column c, both 16
+//     bytes of consecutive contraction indices, the half h the later ones;
+//   C (32 x 32): lane holds column c; register r holds row
+//     8 (r / 4) + 4 h + r % 4.
+// A product's contraction index may be permuted as long as both operands
+// are.  So the scores are formed with the softmax's rows as columns of C
+// (keys x rows, or rows x keys in the key gradients): a lane holds 16 or 32
+// scores of ONE row, its maximum and sum need one exchange with lane ^ 32,
+// and the weights go back into the next product as B straight from the
+// registers they are in, with the rows of C as the contraction index in the
+// order above.  The A of that product is the transpose of a row-major tile
+// and comes from LDS by the transposing read (16-bit types) or one element a
+// lane (float).
+//
+// Tiles lie in LDS as rows of kPitch 16-byte chunks, chunk c of row r at
+// c ^ (r & 7): eight consecutive rows of one chunk, which a fragment read
+// takes at once, are in eight different bank groups.  They are filled by
+// loads from global memory straight to LDS; since such a load writes its
+// lanes' 16 bytes in lane order, the swizzle is on the side of the global
+// address.
+#pragma once
+
+#include <hip/hip_runtime.h>
+
+#include <stdint.h>
+
+#include "bevpool.h"
+
+namespace attention {
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef short i16x4 __attribute__((ext_vector_type(4)));
+typedef short i16x8 __attribute__((ext_vector_type(8)));
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
+
+constexpr int kThreads = 256;  // four waves
+constexpr int kWaves = 4;
+constexpr int kWaveRows = 32;  // rows (or keys) that a wave owns
+constexpr float kLog2e = 1.44269504088896340736f;
+constexpr float kInf = __builtin_inff();
+
+#define ATTENTION_LDS __attribute__((address_space(3)))
+#define ATTENTION_GLOBAL __attribute__((address_space(1)))
+
+template <typename T>
+struct Mat;
+template <>
+struct Mat<__bf16> {
+  typedef bf16x8 Frag;
+  static __device__ __forceinline__ f32x16 mma(Frag a, Frag b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+  }
+};
+template <>
+struct Mat<_Float16> {
+  typedef f16x8 Frag;
+  static __device__ __forceinline__ f32x16 mma(Frag a, Frag b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+  }
+};
+template <>
+struct Mat<float> {
+  typedef f32x4 Frag;
+  // four products of two contraction indices, element i of each half
+  static __device__ __forceinline__ f32x16 mma(Frag a, Frag b, f32x16 c) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[i], b[i], c, 0, 0, 0);
+    return c;
+  }
+};
+
+// A head of up to DP elements of T.
+template <typename T, int DP>
+struct Shape {
+  static constexpr int kSteps = DP * int(sizeof(T)) / 32;        // fragments of a row (2 chunks)
+  static constexpr int kChunks = 2 * kSteps;
+  static constexpr int kPitch = (kChunks + 7) / 8 * 8;           // chunks of a row in LDS
+  static constexpr int kBlocks = (DP + 31) / 32;                 // blocks of 32 elements
+  static constexpr int tile_bytes(int rows) { return rows * kPitch * 16; }
+};
+
+template <typename T, int DP>
+using Frags = typename Mat<T>::Frag[Shape<T, DP>::kSteps];  // of one row
+template <typename T, int DP>
+using Sums = f32x16[Shape<T, DP>::kBlocks];  // 32 columns of elements
+
+__device__ __forceinline__ int lane_id() { return threadIdx.x & 63; }
+__device__ __forceinline__ int wave_id() {
+  return __builtin_amdgcn_readfirstlane(int(threadIdx.x >> 6));
+}
+
+// The row of C that register r of this lane holds.
+__device__ __forceinline__ int c_row(int r, int h) { return 8 * (r >> 2) + 4 * h + (r & 3); }
+
+// The low half's value and the high half's, each in both halves.  (Elements
+// are copied out before the cast: hipcc 7.2 takes __builtin_bit_cast of any
+// element of a vector for that of its first.)
+struct Halves {
+  float low, high;
+};
+__device__ __forceinline__ Halves halves_of(float v) {
+  const unsigned a = __builtin_bit_cast(unsigned, v);
+  const auto x = __builtin_amdgcn_permlane32_swap(a, a, false, false);
+  const unsigned low = x[0], high = x[1];
+  return {__builtin_bit_cast(float, low), __builtin_bit_cast(float, high)};
+}
+__device__ __forceinline__ float max_halves(float v) {
+  const Halves x = halves_of(v);
+  return fmaxf(x.low, x.high);
+}
+__device__ __forceinline__ float sum_halves(float v) {
+  const Halves x = halves_of(v);
+  return x.low + x.high;
+}
+
+__device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// Waits until this wave's loads to LDS, all but the newest `left` of them,
+// have arrived.
+template <int kLeft>
+__device__ __forceinline__ void wait_loads() {
+  static_assert(kLeft >= 0 && kLeft < 64, "vmcnt has 6 bits");
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kLeft) : "memory");
+}
+
+// Fills kRows rows of a tile with kLanes lanes; row(i) gives the address of
+// row i's first byte.  Chunks past the head's `chunks` are left as they are.
+template <typename T, int DP, int kRows, int kLanes, typename Row>
+__device__ __forceinline__ void stage(char *tile, int thread, int chunks, Row row) {
+  constexpr int kPitch = Shape<T, DP>::kPitch;
+  static_assert(kRows * kPitch % kLanes == 0, "whole rounds");
+#pragma unroll
+  for (int i = 0; i < kRows * kPitch / kLanes; ++i) {
+    const int slot = i * kLanes + thread;
+    const int r = slot / kPitch, c = (slot % kPitch) ^ (r & 7);
+    if (c < chunks) {
+      char *to = tile + (i * kLanes + (thread & ~63)) * 16;  // (the wave's; a lane adds 16 each)
+      __builtin_amdgcn_global_load_lds(
+          (const ATTENTION_GLOBAL void *)(row(r) + c * 16),
+          (ATTENTION_LDS void *)(uintptr_t)(unsigned)(__builtin_amdgcn_readfirstlane(
+              int((uintptr_t)(ATTENTION_LDS char *)to))),
+          16, 0, 0);
+    }
+  }
+}
+
+// Chunks [chunks, kChunks) of a tile's rows, which no load fills but a
+// product reads: zeros.
+template <typename T, int DP>
+__device__ __forceinline__ void clear_rest(char *tile, int rows, int thread, int lanes,
+                                           int chunks) {
+  constexpr int kPitch = Shape<T, DP>::kPitch, kChunks = Shape<T, DP>::kChunks;
+  if (chunks >= kChunks) return;
+  for (int i = thread; i < rows * kPitch; i += lanes) {
+    const int r = i / kPitch, c = (i % kPitch) ^ (r & 7);
+    if (c >= chunks) *reinterpret_cast<u32x4 *>(tile + i * 16) = u32x4{0, 0, 0, 0};
+  }
+}
+
+// Fragment s of row r0 + c of a tile (r0 a multiple of 8).
+template <typename T, int DP>
+__device__ __forceinline__ typename Mat<T>::Frag tile_frag(const char *tile, int r0, int s) {
+  const int lane = lane_id(), c = lane & 31, h = lane >> 5;
+  const int chunk = (2 * s + h) ^ (c & 7);
+  return *reinterpret_cast<const typename Mat<T>::Frag *>(
+      tile + (r0 + c) * (Shape<T, DP>::kPitch * 16) + chunk * 16);
+}
+
+// Fragments of one row in global memory (chunks past the head's: zeros).
+template <typename T, int DP>
+__device__ __forceinline__ void row_frags(Frags<T, DP> &f, const char *row, int chunks, bool valid) {
+  const int h = lane_id() >> 5;
+#pragma unroll
+  for (int s = 0; s < Shape<T, DP>::kSteps; ++s) {
+    typename Mat<T>::Frag z = {};
+    if (valid && 2 * s + h < chunks)
+      z = *reinterpret_cast<const typename Mat<T>::Frag *>(row + (2 * s + h) * 16);
+    f[s] = z;
+  }
+}
+
+// C = (tile rows r0 .. r0 + 31) x (the fragments' rows): scores.
+template <typename T, int DP>
+__device__ __forceinline__ f32x16 dot_rows(const char *tile, int r0,
+                                           const Frags<T, DP> &f) {
+  f32x16 c = {};
+#pragma unroll
+  for (int s = 0; s < Shape<T, DP>::kSteps; ++s)
+    c = Mat<T>::mma(tile_frag<T, DP>(tile, r0, s), f[s], c);
+  return c;
+}
+
+// The weights of a 32 x 32 block of scores as B of the next product.
+template <typename T>
+struct Weights {
+  typename Mat<T>::Frag f[2];
+  __device__ __forceinline__ void set(const float (&p)[16]) {
+#pragma unroll
+    for (int r = 0; r < 16; ++r) f[r >> 3][r & 7] = T(p[r]);
+  }
+};
+template <>
+struct Weights<float> {
+  float f[16];
+  __device__ __forceinline__ void set(const float (&p)[16]) {
+#pragma unroll
+    for (int r = 0; r < 16; ++r) f[r] = p[r];
+  }
+};
+
+// acc[b] += (rows r0 .. r0 + 31 of the tile, elements 32 b .. 32 b + 31)^T x
+// weights.
+template <typename T, int DP>
+__device__ __forceinline__ void add_transposed(Sums<T, DP> &acc, const char *tile, int r0,
+                                               const Weights<T> &w) {
+  constexpr int kRow = Shape<T, DP>::kPitch * 16;
+  const int lane = lane_id(), h = lane >> 5;
+  if constexpr (sizeof(T) == 4) {
+    // register r's row, one element a lane
+    const int c = lane & 31;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      const int row = c_row(r, h);
+      const char *at = tile + (r0 + row) * kRow + (c & 3) * 4;
+#pragma unroll
+      for (int b = 0; b < Shape<T, DP>::kBlocks; ++b) {
+        const float a =
+            *reinterpret_cast<const float *>(at + ((8 * b + (c >> 2)) ^ (row & 7)) * 16);
+        acc[b] = __builtin_amdgcn_mfma_f32_32x32x2f32(a, w.f[r], acc[b], 0, 0, 0);
+      }
+    }
+  } else {
+    // the transposing read gives lane i (of 16) element i of four rows; it
+    // reads row i / 4, elements 4 (i % 4) .. + 3
+    const int row = 4 * h + ((lane & 15) >> 2);
+    const int chunk = 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
+    const char *at = tile + (r0 + row) * kRow + (lane & 1) * 8;
+#pragma unroll
+    for (int b = 0; b < Shape<T, DP>::kBlocks; ++b) {
+      const char *col = at + ((4 * b + chunk) ^ row) * 16;
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const i16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+            (ATTENTION_LDS i16x4 *)(col + 16 * j * kRow));
+        const i16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+            (ATTENTION_LDS i16x4 *)(col + (16 * j + 8) * kRow));
+        const i16x8 a = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+        acc[b] = Mat<T>::mma(__builtin_bit_cast(typename Mat<T>::Frag, a), w.f[j], acc[b]);
+      }
+    }
+  }
+}
+
+// Writes a lane's column of acc times `by`, rounded to T once, as a row.
+template <typename T, int DP>
+__device__ __forceinline__ void store_row(char *row, const Sums<T, DP> &acc, float by,
+                                          int dim, bool valid) {
+  const int h = lane_id() >> 5;
+#pragma unroll
+  for (int b = 0; b < (DP + 31) / 32; ++b) {
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const int d = 32 * b + 8 * g + 4 * h;
+        if (valid && d < dim)
+          *reinterpret_cast<f32x4 *>(row + d * 4) =
+              f32x4{acc[b][4 * g] * by, acc[b][4 * g + 1] * by, acc[b][4 * g + 2] * by,
+                    acc[b][4 * g + 3] * by};
+      }
+    } else {
+      // four neighbours a lane; the halves trade so that each has eight
+#pragma unroll
+      for (int p = 0; p < 2; ++p) {
+        typedef T Pair __attribute__((ext_vector_type(2)));
+        unsigned x[2], y[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          x[i] = __builtin_bit_cast(unsigned, Pair{T(acc[b][8 * p + 2 * i] * by),
+                                                   T(acc[b][8 * p + 2 * i + 1] * by)});
+          y[i] = __builtin_bit_cast(unsigned, Pair{T(acc[b][8 * p + 4 + 2 * i] * by),
+                                                   T(acc[b][8 * p + 5 + 2 * i] * by)});
+        }
+        const auto a = __builtin_amdgcn_permlane32_swap(x[0], y[0], false, false);
+        const auto c = __builtin_amdgcn_permlane32_swap(x[1], y[1], false, false);
+        const int d = 32 * b + 16 * p + 8 * h;
+        if (valid && d < dim)
+          *reinterpret_cast<u32x4 *>(row + d * 2) = u32x4{a[0], c[0], a[1], c[1]};
+      }
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// packed sequences
+// ---------------------------------------------------------------------------
+
+// n / group for n < 2^32 / group.
+struct Group {
+  int size;
+  uint32_t magic;  // ceil(2^32 / size); 0 for 1
+  __device__ __forceinline__ int div(int n) const {
+    return magic ? int(__umulhi(uint32_t(n), magic)) : n;
+  }
+};
+
+inline Group make_group(int size) {
+  return {size, size == 1 ? 0u : uint32_t(((uint64_t(1) << 32) + size - 1) / size)};
+}
+
+struct Sequence {
+  int q0, nq, k0, nk;
+};
+
+// starts[i] kept within the rows there are, whatever the array holds.
+__device__ __forceinline__ int start_at(const int32_t *starts, int i, int total) {
+  if (i <= 0) return 0;
+  const int v = starts[i];
+  return v < 0 ? 0 : v > total ? total : v;
+}
+
+__device__ __forceinline__ Sequence sequence_at(const int32_t *q_starts, const int32_t *k_starts,
+                                                int i, int n, int tq, int tk) {
+  Sequence s;
+  s.q0 = start_at(q_starts, i, tq);
+  s.k0 = start_at(k_starts, i, tk);
+  s.nq = i < n ? start_at(q_starts, i + 1, tq) - s.q0 : 0;
+  s.nk = i < n ? start_at(k_starts, i + 1, tk) - s.k0 : 0;
+  if (s.nq < 0) s.nq = 0;
+  if (s.nk < 0) s.nk = 0;
+  return s;
+}
+
+// Tiles of `tile` rows over sequences of starts[i + 1] - starts[i] tokens of
+// `per` rows each, without a plan: sequence i's tiles are numbered from
+// starts[i] * per / tile + i.  No two sequences' numbers meet, since
+// floor(a) + ceil(b) <= floor(a + b) + 1, and all are below
+// total * per / tile + n + 1, which the host knows.  Sequence n stands for
+// the rows after the last one, which belong to none.  Finds the sequence
+// whose numbers `index` is among; its first number goes to `first`.  Each
+// round narrows the range 64 times, so that any number of sequences takes a
+// few loads.  The whole wave calls it.
+__device__ __forceinline__ int find_sequence(const int32_t *starts, int n, int total, int per,
+                                             int tile, int index, int *first) {
+  int low = 0, count = n + 1;
+  for (;;) {
+    const int step = (count + 63) / 64;
+    const int at = low + lane_id() * step;
+    const bool ok = lane_id() * step < count &&
+                    int(int64_t(start_at(starts, at, total)) * per / tile) + at <= index;
+    const int taken = __popcll(__ballot(ok));
+    const int i = taken > 0 ? taken - 1 : 0;
+    low += i * step;
+    count = count - i * step < step ? count - i * step : step;
+    if (step == 1) break;
+  }
+  low = __builtin_amdgcn_readfirstlane(low);
+  *first = int(int64_t(start_at(starts, low, total)) * per / tile) + low;
+  return low;
+}
+
+// ---------------------------------------------------------------------------
+// arguments
+// ---------------------------------------------------------------------------
+
+struct Operand {  // (rows, heads, dim), unit stride along dim; strides in bytes
+  char *at;
+  int64_t row, head;
+};
+
+struct PackedArgs {
+  Operand q, k, v, out, dout, dq, dk, dv;
+  float *lse;          // (tokens, heads): log of the sum of exponentials
+  const float *delta;  // backward: (tokens, heads), sum of dout * out
+  const int32_t *q_starts, *k_starts;  // sequences + 1
+  int sequences, q_total, k_total;
+  int q_heads, k_heads;
+  Group group;
+  int dim, chunks;     // elements and 16-byte chunks of a head
+  int causal;
+  float scale, scale_log2;
+  int tiles;
+};
+
+}  // namespace attention

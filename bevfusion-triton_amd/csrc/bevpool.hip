@@ -65,6 +65,7 @@
 #include <stdio.h>
 
 #include <mutex>
+#include <new>
 #include <type_traits>
 #include <string>
 #include <unordered_map>
@@ -72,6 +73,7 @@
 
 #include "bevpool.h"
 #include "channel_blocks.h"
+#include "host_calls.h"
 
 namespace {
 
@@ -225,6 +227,27 @@ struct LaunchTimer {
     g_timing_pending.push_back({name, start, stop});
   }
 };
+
+}  // namespace
+
+// What the other source files use of the two sections above (host_calls.h).
+namespace bevpool_host {
+
+void clear_error() { g_last_error.clear(); }
+
+int set_error(int code, const char *text) {
+  g_last_error = text;
+  return code;
+}
+
+LaunchScope::LaunchScope(const char *name, hipStream_t stream)
+    : timer_(new (std::nothrow) LaunchTimer(name, stream)) {}
+
+LaunchScope::~LaunchScope() { delete static_cast<LaunchTimer *>(timer_); }
+
+}  // namespace bevpool_host
+
+namespace {
 
 // ---------------------------------------------------------------------------
 // device helpers

@@ -521,6 +521,80 @@ int bevpool_runs(const void *ranks, int32_t rank_bytes, int64_t n, int32_t *star
                  int32_t *lengths, int32_t *meta, void *workspace, size_t workspace_bytes,
                  void *stream);
 
+/* -------------------------------------------------------------------------
+ * Token operators: what a transformer over camera and BEV tokens needs after
+ * the pooling.  No counterpart in the reference.  Operands are (rows, heads,
+ * dim) views with unit stride along dim; row and head strides are counted in
+ * elements.  All sums are held in fp32; each result is rounded once to the
+ * operands' type.
+ * ---------------------------------------------------------------------- */
+
+/*
+ * RMS norm of queries and keys for each head and rotation by positions with
+ * several axes, in one pass:
+ *   n = x / sqrt(mean(x^2) + eps) * weight      (weight NULL: n = x)
+ *   pair p of n turned by the angle pos[token, axis(p)] * frequencies[p]
+ * where axis i has axis_pairs[i] pairs, in order.  Pair p is the elements
+ * (p, P + p), P = sum of axis_pairs, or (2p, 2p + 1) with `interleaved`;
+ * elements from 2P on are not turned.  The angle is formed in double and
+ * reduced to one turn, so it is as good at position 10^6 as at 1.
+ *   q, k         (tokens, heads, dim), fp32 / fp16 / bf16; k_heads may be 0
+ *   dim          even, at most 256
+ *   positions    [tokens][>= n_axes], row stride pos_stride, of pos_kind
+ *                0 int32, 1 int64, 2 float32
+ *   frequencies  fp32 [P], radians per unit of position
+ *   axis_pairs   host array of n_axes (0 .. 4) counts
+ *   q_weight, k_weight   [dim] in the operands' type, or NULL
+ *   q_out, k_out contiguous
+ */
+int bevpool_norm_rotate_forward(const void *q, int64_t q_token, int64_t q_head, int32_t q_heads,
+                                const void *k, int64_t k_token, int64_t k_head, int32_t k_heads,
+                                int32_t dtype, int64_t tokens, int32_t dim, const void *positions,
+                                int32_t pos_kind, int64_t pos_stride, const float *frequencies,
+                                const int32_t *axis_pairs, int32_t n_axes, int32_t interleaved,
+                                const void *q_weight, const void *k_weight, float eps, void *q_out,
+                                void *k_out, void *stream);
+
+/*
+ * Its gradients: dq, dk contiguous; dq_weight, dk_weight [dim] (with the
+ * weights), summed in an order that does not depend on the launch.  q and k
+ * may be NULL when there are no weights (a rotation needs no input).
+ *   scratch   >= bevpool_norm_rotate_backward_scratch_bytes(dim) (with the
+ *             weights; else it may be NULL)
+ */
+size_t bevpool_norm_rotate_backward_scratch_bytes(int32_t dim);
+
+int bevpool_norm_rotate_backward(
+    const void *q, int64_t q_token, int64_t q_head, int32_t q_heads, const void *k,
+    int64_t k_token, int64_t k_head, int32_t k_heads, const void *dq_out, int64_t dq_token,
+    int64_t dq_head, const void *dk_out, int64_t dk_token, int64_t dk_head, int32_t dtype,
+    int64_t tokens, int32_t dim, const void *positions, int32_t pos_kind, int64_t pos_stride,
+    const float *frequencies, const int32_t *axis_pairs, int32_t n_axes, int32_t interleaved,
+    const void *q_weight, const void *k_weight, float eps, void *dq, void *dk, void *dq_weight,
+    void *dk_weight, void *scratch, size_t scratch_bytes, void *stream);
+
+/*
+ * Attention over packed sequences.  Sequence i has queries
+ * [q_starts[i], q_starts[i + 1]) and keys [k_starts[i], k_starts[i + 1]);
+ * query head h reads key head h / (q_heads / k_heads).  With `causal`, query
+ * j of a sequence of nq queries and nk keys sees its keys up to
+ * j + nk - nq.  out = softmax(scale q k) v; a query that sees no key, or is
+ * in no sequence, gets zeros (and lse -inf).
+ *   dim          a multiple of 8, at most 128; rows and heads of every
+ *                operand start at multiples of 16 bytes
+ *   q_starts, k_starts   device int32 [sequences + 1], ascending from 0
+ *                (values are clamped to the rows there are)
+ *   out          (q_total, q_heads, dim) contiguous
+ *   lse          (q_total, q_heads) fp32, log of the sum of exponentials,
+ *                or NULL
+ */
+int bevpool_attention_forward(const void *q, int64_t q_row, int64_t q_head, const void *k,
+                              int64_t k_row, int64_t k_head, const void *v, int64_t v_row,
+                              int64_t v_head, int32_t dtype, int64_t q_total, int64_t k_total,
+                              int32_t q_heads, int32_t k_heads, int32_t dim,
+                              const int32_t *q_starts, const int32_t *k_starts, int32_t sequences,
+                              int32_t causal, float scale, void *out, float *lse, void *stream);
+
 /*
  * Optional per-kernel timing.  When enabled, every kernel launch is bracketed
  * by HIP events on the launch stream; bevpool_timing_read() synchronises
