@@ -242,8 +242,26 @@ class _AttendPacked(torch.autograd.Function):
             k.shape[0], q.shape[1], k.shape[1], q.shape[2], L.ptr(q_starts), L.ptr(k_starts),
             q_starts.shape[0] - 1, int(causal), scale, L.ptr(out), L.ptr(lse), s), q.device,
             'bevpool_attention_forward')
+        ctx.save_for_backward(q, k, v, out, lse, q_starts, k_starts)
+        ctx.call = (causal, scale)
         ctx.mark_non_differentiable(lse)
         return out, lse
+
+    @staticmethod
+    def backward(ctx, dout, _):
+        q, k, v, out, lse, q_starts, k_starts = ctx.saved_tensors
+        causal, scale = ctx.call
+        dout = _aligned(dout.to(q.dtype))
+        dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
+        nbytes = L.library().bevpool_attention_backward_scratch_bytes(q.shape[0], q.shape[1])
+        scratch = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
+        _run(lambda lib, s: lib.bevpool_attention_backward(
+            *_strides(q), *_strides(k), *_strides(v), L.ptr(out), *_strides(dout), L.ptr(lse),
+            L.DTYPE_CODES[q.dtype], q.shape[0], k.shape[0], q.shape[1], k.shape[1], q.shape[2],
+            L.ptr(q_starts), L.ptr(k_starts), q_starts.shape[0] - 1, int(causal), scale, L.ptr(dq),
+            L.ptr(dk), L.ptr(dv), L.ptr(scratch), nbytes, s), q.device,
+            'bevpool_attention_backward')
+        return dq, dk, dv, None, None, None, None
 
 
 def attend_packed(q, k, v, q_starts, k_starts=None, *, causal=False, scale=None,

@@ -196,7 +196,9 @@ int check_packed(PackedArgs &A, int dtype, int64_t q_total, int64_t k_total, int
   if (!(scale > 0.f) || !(scale < 3e38f))
     return fail(BEVPOOL_EINVAL, "scale must be positive and finite");
   const int64_t group = q_heads / k_heads;
-  if (q_total * group * group >= (int64_t(1) << 31) || k_total >= (int64_t(1) << 31) - 256)
+  // (packed row numbers, and their quotients by the group, in 32 bits)
+  if (q_total * group * group >= (int64_t(1) << 31) ||
+      (k_total + 256) * group >= (int64_t(1) << 31))
     return fail(BEVPOOL_EINVAL, "too many tokens (%lld queries in groups of %lld, %lld keys)",
                 (long long)q_total, (long long)group, (long long)k_total);
   if ((q_total > 0 || k_total > 0) && (!q_starts || !k_starts))
@@ -229,13 +231,6 @@ int set_operand(Operand &o, const char *what, const void *at, int64_t row, int64
 }
 
 }  // namespace attention
-
-#define ATTENTION_DIM(T, FN, ...)                                                   \
-  dim <= 32   ? FN<T, 32>(__VA_ARGS__)                                              \
-  : dim <= 64 ? FN<T, 64>(__VA_ARGS__)                                              \
-  : dim <= 80 ? FN<T, 80>(__VA_ARGS__)                                              \
-  : dim <= 96 ? FN<T, 96>(__VA_ARGS__)                                              \
-              : FN<T, 128>(__VA_ARGS__)
 
 extern "C" {
 

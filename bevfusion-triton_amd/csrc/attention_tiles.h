@@ -389,4 +389,20 @@ struct PackedArgs {
   int tiles;
 };
 
+// Host side (attention.hip): sizes and operands of a packed call.
+__attribute__((visibility("hidden"))) int check_packed(
+    PackedArgs &A, int dtype, int64_t q_total, int64_t k_total, int sequences, int q_heads,
+    int k_heads, int dim, const void *q_starts, const void *k_starts, int causal, float scale);
+__attribute__((visibility("hidden"))) int set_operand(Operand &o, const char *what, const void *at,
+                                                      int64_t row, int64_t head, int elem,
+                                                      int64_t total);
+
 }  // namespace attention
+
+// FN of the smallest instance that holds a head of `dim` elements.
+#define ATTENTION_DIM(T, FN, ...)                                                   \
+  dim <= 32   ? FN<T, 32>(__VA_ARGS__)                                              \
+  : dim <= 64 ? FN<T, 64>(__VA_ARGS__)                                              \
+  : dim <= 80 ? FN<T, 80>(__VA_ARGS__)                                              \
+  : dim <= 96 ? FN<T, 96>(__VA_ARGS__)                                              \
+              : FN<T, 128>(__VA_ARGS__)

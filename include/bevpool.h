@@ -596,6 +596,25 @@ int bevpool_attention_forward(const void *q, int64_t q_row, int64_t q_head, cons
                               int32_t causal, float scale, void *out, float *lse, void *stream);
 
 /*
+ * Its gradients, from the forward's out and lse: dq (q_total, q_heads, dim),
+ * dk and dv (k_total, k_heads, dim), contiguous, every row written (zeros for
+ * queries that see no key and keys that no query sees).  dout has strides of
+ * its own, out is contiguous.  No atomics: the same call gives the same bits.
+ *   scratch   >= bevpool_attention_backward_scratch_bytes(q_total, q_heads)
+ */
+size_t bevpool_attention_backward_scratch_bytes(int64_t q_total, int32_t q_heads);
+
+int bevpool_attention_backward(const void *q, int64_t q_row, int64_t q_head, const void *k,
+                               int64_t k_row, int64_t k_head, const void *v, int64_t v_row,
+                               int64_t v_head, const void *out, const void *dout,
+                               int64_t dout_row, int64_t dout_head, const float *lse,
+                               int32_t dtype, int64_t q_total, int64_t k_total, int32_t q_heads,
+                               int32_t k_heads, int32_t dim, const int32_t *q_starts,
+                               const int32_t *k_starts, int32_t sequences, int32_t causal,
+                               float scale, void *dq, void *dk, void *dv, void *scratch,
+                               size_t scratch_bytes, void *stream);
+
+/*
  * Optional per-kernel timing.  When enabled, every kernel launch is bracketed
  * by HIP events on the launch stream; bevpool_timing_read() synchronises
  * those events and returns, per kernel name, the summed milliseconds and

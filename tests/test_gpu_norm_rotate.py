@@ -279,33 +279,6 @@ def test_refusals(pkg):
         pkg.norm_rotate(x, None, pos, freq)
 
 
-def test_refusals_of_the_c_entry(pkg):
-    """Argument checks return before any HIP call."""
-    import ctypes
-
-    lib = pkg.library()
-    i32 = lambda *v: (ctypes.c_int32 * max(1, len(v)))(*v)
-
-    def forward(dtype=0, tokens=4, dim=64, kind=0, pairs=(32,), eps=1e-6, k_heads=0, kw=None):
-        return lib.bevpool_norm_rotate_forward(1, 64, 64, 1, None, 0, 0, k_heads, dtype, tokens,
-                                               dim, 1, kind, 1, 1, i32(*pairs), len(pairs), 0,
-                                               None, kw, eps, 1, None, None)
-
-    for bad, text in ((dict(dtype=5), b'dtype'), (dict(tokens=-1), b'negative'),
-                      (dict(dim=63), b'even'), (dict(dim=258), b'256'),
-                      (dict(pairs=(33,)), b'fit'), (dict(pairs=(20, 20)), b'fit'),
-                      (dict(kind=3), b'position type'), (dict(eps=float('nan')), b'eps'),
-                      (dict(k_heads=2), b'null'), (dict(kw=1), b'no heads')):
-        assert forward(**bad) == -1, bad
-        assert text in lib.bevpool_last_error(), bad
-    assert lib.bevpool_norm_rotate_backward(
-        None, 0, 0, 1, None, 0, 0, 0, 1, 64, 64, None, 0, 0, 0, 4, 64, 1, 0, 1, 1, i32(32), 1, 0,
-        1, None, 1e-6, 1, None, 1, None, None, 0, None) == -1  # a weight, but no rows
-    assert lib.bevpool_norm_rotate_backward(
-        1, 64, 64, 1, None, 0, 0, 0, 1, 64, 64, None, 0, 0, 0, 4, 64, 1, 0, 1, 1, i32(32), 1, 0,
-        1, None, 1e-6, 1, None, 1, None, 1, 16, None) == -3
-
-
 def test_frequencies(pkg):
     f = pkg.axis_frequencies((2, 4))
     assert f.dtype == torch.float32 and f.shape == (6,)

@@ -1,0 +1,56 @@
+"""Argument checks of the token operators' C entries: they return the
+documented status and message before any HIP call, so no GPU is needed."""
+from __future__ import annotations
+
+import ctypes
+
+
+def test_norm_rotate(pkg):
+    """Argument checks return before any HIP call."""
+    lib = pkg.library()
+    i32 = lambda *v: (ctypes.c_int32 * max(1, len(v)))(*v)
+
+    def forward(dtype=0, tokens=4, dim=64, kind=0, pairs=(32,), eps=1e-6, k_heads=0, kw=None):
+        return lib.bevpool_norm_rotate_forward(1, 64, 64, 1, None, 0, 0, k_heads, dtype, tokens,
+                                               dim, 1, kind, 1, 1, i32(*pairs), len(pairs), 0,
+                                               None, kw, eps, 1, None, None)
+
+    for bad, text in ((dict(dtype=5), b'dtype'), (dict(tokens=-1), b'negative'),
+                      (dict(dim=63), b'even'), (dict(dim=258), b'256'),
+                      (dict(pairs=(33,)), b'fit'), (dict(pairs=(20, 20)), b'fit'),
+                      (dict(kind=3), b'position type'), (dict(eps=float('nan')), b'eps'),
+                      (dict(k_heads=2), b'null'), (dict(kw=1), b'no heads')):
+        assert forward(**bad) == -1, bad
+        assert text in lib.bevpool_last_error(), bad
+    assert lib.bevpool_norm_rotate_backward(
+        None, 0, 0, 1, None, 0, 0, 0, 1, 64, 64, None, 0, 0, 0, 4, 64, 1, 0, 1, 1, i32(32), 1, 0,
+        1, None, 1e-6, 1, None, 1, None, None, 0, None) == -1  # a weight, but no rows
+    assert lib.bevpool_norm_rotate_backward(
+        1, 64, 64, 1, None, 0, 0, 0, 1, 64, 64, None, 0, 0, 0, 4, 64, 1, 0, 1, 1, i32(32), 1, 0,
+        1, None, 1e-6, 1, None, 1, None, 1, 16, None) == -3
+
+
+def test_attention(pkg):
+    """Argument checks return before any HIP call."""
+    lib = pkg.library()
+
+    def forward(dtype=2, q_total=4, k_total=4, q_heads=4, k_heads=2, dim=64, scale=0.125, q=16,
+                row=256, starts=16):
+        return lib.bevpool_attention_forward(q, row, dim, 16, 128, dim, 16, 128, dim, dtype,
+                                             q_total, k_total, q_heads, k_heads, dim, starts,
+                                             starts, 1, 0, scale, 16, None, None)
+
+    for bad, text in ((dict(dtype=3), b'dtype'), (dict(q_total=-1), b'negative'),
+                      (dict(q_heads=3), b'no multiple'), (dict(k_heads=0), b'no multiple'),
+                      (dict(dim=60), b'multiple of 8'), (dict(dim=256), b'multiple of 8'),
+                      (dict(scale=-1.0), b'scale'), (dict(scale=float('nan')), b'scale'),
+                      (dict(q_total=1 << 30), b'too many'), (dict(k_total=1 << 30), b'too many'),
+                      (dict(q=None), b'q: null'), (dict(q=8), b'16 bytes'),
+                      (dict(row=255), b'16 bytes'), (dict(starts=None), b'null starts')):
+        assert forward(**bad) == -1, bad
+        assert text in lib.bevpool_last_error(), bad
+    args = (16, 256, 64, 16, 128, 64, 16, 128, 64, 16, 16, 256, 64, 16, 2, 4, 4, 4, 2, 64, 16, 16,
+            1, 0, 0.125, 16, 16, 16)
+    assert lib.bevpool_attention_backward_scratch_bytes(4, 4) == 4 * 4 * 2 * 4
+    assert lib.bevpool_attention_backward(*args, None, 0, None) == -3
+    assert b'scratch' in lib.bevpool_last_error()
