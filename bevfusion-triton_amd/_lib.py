@@ -151,6 +151,13 @@ _SIGNATURES = {
          _i64, _i64, _i32, _i32, _i32, _vp, _vp, _i32, _i32, _f32, _vp, _vp, _vp, _vp, _sz, _vp],
         ctypes.c_int,
     ),
+    'bevpool_attention_cached_scratch_bytes': ([_i32] * 7, _sz),
+    'bevpool_attention_cached': (
+        [_vp, _i64, _i64, _vp, _i64, _i64, _i64, _vp, _i64, _i64, _i64, _vp, _i64, _i64, _vp,
+         _i64, _i64, _vp, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _f32, _vp, _vp, _sz,
+         _vp],
+        ctypes.c_int,
+    ),
     'bevpool_timing_enable': ([ctypes.c_int], ctypes.c_int),
     'bevpool_timing_reset': ([], ctypes.c_int),
     'bevpool_timing_read': (

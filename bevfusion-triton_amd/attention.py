@@ -10,11 +10,13 @@ counterpart.
   * :func:`axis_frequencies` the usual frequency ladders for it
   * :func:`attend_packed`    attention over packed sequences of different
                              lengths, causal or not, grouped heads
+  * :func:`attend_cached`    its form for serving: new tokens of many requests
+                             over their caches and a prefix that all share
 
-Both operators have gradients.  Operands are fp32, fp16 or bf16 (rows, heads,
+The first two have gradients.  Operands are fp32, fp16 or bf16 (rows, heads,
 dim) tensors; any strides are taken, so parts of one projection's output need
 no copy (attention copies an operand whose rows or heads do not start at
-multiples of 16 bytes).  Calls run on torch's current stream, allocate with
+multiples of 16 bytes; a cache that does not is refused).  Calls run on torch's current stream, allocate with
 torch's allocator and never wait for the device.
 """
 from __future__ import annotations
@@ -199,9 +201,7 @@ def _aligned(x):
 
 
 def _check_heads(q, k, v):
-    _check_rows('q', q, q.dim())
     for name, x in (('k', k), ('v', v)):
-        _check_rows(name, x, x.dim())
         _check_same(name, x, q)
     if k.shape != v.shape:
         raise ValueError('k and v must have the same shape.')
@@ -295,3 +295,73 @@ def attend_packed(q, k, v, q_starts, k_starts=None, *, causal=False, scale=None,
         raise ValueError('q_starts and k_starts must have the same length.')
     out, lse = _AttendPacked.apply(q, k, v, q_starts, k_starts, bool(causal), scale)
     return (out, lse) if return_lse else out
+
+
+# ---- new tokens over caches ------------------------------------------------
+
+def _cache(name, x, dims):
+    _check_rows(name, x, dims)
+    per = 16 // x.element_size()
+    if x.numel() and (x.stride(-1) != 1 or x.data_ptr() % 16
+                      or any(s % per for s in x.stride()[:-1])):
+        raise ValueError(f'{name}: rows and heads must start at multiples of 16 bytes.')
+    return x
+
+
+def attend_cached(q, k, v, lengths, prefix_k=None, prefix_v=None, *, scale=None):
+    """Attention of new tokens over caches, with a prefix that all requests
+    share.
+
+    q (requests, tokens, q_heads, dim), or (requests, q_heads, dim) for single
+    tokens; k, v (requests, capacity, k_heads, dim): each request's own cache,
+    its new tokens' keys and values already in it.  lengths (requests,), int32
+    or int64 on the device: the keys in use, the new tokens' among them (taken
+    as within [0, capacity]).  prefix_k, prefix_v (prefix, k_heads, dim) or
+    None.  New token i sees the whole prefix and the first lengths - (tokens -
+    1 - i) keys of its request's cache; what lies past a length is never read.
+    A row that sees nothing gives zeros.  Returns q's shape, contiguous.  Heads
+    and scale are as in :func:`attend_packed`.  No gradient."""
+    single = q.dim() == 3
+    if single:
+        q = q.unsqueeze(1)
+    _check_rows('q', q, 4)
+    k, v = _cache('k', k, 4), _cache('v', v, 4)
+    _check_heads(q, k, v)
+    requests, tokens, q_heads, dim = q.shape
+    capacity, k_heads = k.shape[1:3]
+    if k.shape[0] != requests:
+        raise ValueError('q and k must have the same number of requests.')
+    if tokens < 1:
+        raise ValueError('q must hold at least one token of each request.')
+    if (prefix_k is None) != (prefix_v is None):
+        raise ValueError('prefix_k and prefix_v go together.')
+    if prefix_k is not None:
+        prefix_k, prefix_v = _cache('prefix_k', prefix_k, 3), _cache('prefix_v', prefix_v, 3)
+        for name, x in (('prefix_k', prefix_k), ('prefix_v', prefix_v)):
+            _check_same(name, x, q)
+            if x.shape[1:] != k.shape[2:] or x.shape != prefix_k.shape:
+                raise ValueError(f'{name} must have shape [prefix, k_heads, dim].')
+    scale = _check_scale(scale, dim)
+    if lengths.dim() != 1 or lengths.shape[0] != requests:
+        raise ValueError('lengths must have shape [requests].')
+    if lengths.dtype not in (torch.int32, torch.int64):
+        raise TypeError('lengths must have dtype torch.int32 or torch.int64.')
+    P.require_gpu(q, k, v, lengths)
+    if lengths.device != q.device:
+        raise ValueError(f'lengths must be on the device of q ({q.device}).')
+    for t in (q, k, v, prefix_k, prefix_v):
+        if t is not None and t.requires_grad and torch.is_grad_enabled():
+            raise RuntimeError('attend_cached has no gradient; call it under torch.no_grad()')
+    rows = _aligned(q.reshape(requests * tokens, q_heads, dim))
+    lengths = lengths.to(torch.int32).contiguous()
+    prefix = prefix_k.shape[0] if prefix_k is not None else 0
+    out = torch.empty((requests, tokens, q_heads, dim), dtype=q.dtype, device=q.device)
+    nbytes = L.library().bevpool_attention_cached_scratch_bytes(
+        requests, tokens, capacity, prefix, q_heads, k_heads, dim)
+    scratch = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
+    _run(lambda lib, s: lib.bevpool_attention_cached(
+        *_strides(rows), L.ptr(k), *k.stride()[:3], L.ptr(v), *v.stride()[:3],
+        *_strides(prefix_k), *_strides(prefix_v), L.ptr(lengths), L.DTYPE_CODES[q.dtype],
+        requests, tokens, capacity, prefix, q_heads, k_heads, dim, scale, L.ptr(out),
+        L.ptr(scratch), nbytes, s), q.device, 'bevpool_attention_cached')
+    return out[:, 0] if single else out

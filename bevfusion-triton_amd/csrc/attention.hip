@@ -15,47 +15,6 @@ using bevpool_host::check_launch;
 using bevpool_host::fail;
 using bevpool_host::LaunchScope;
 
-// Running softmax of one row: a lane and lane ^ 32 share it, with half of a
-// block's keys each.
-struct Softmax {
-  float top = -kInf;  // the maximum that the weights are relative to
-  float sum = 0.f;    // of this lane's half of the keys
-};
-
-// Takes kN scores of this lane's row (raw products, -inf where masked):
-// they become weights exp2(scale_log2 (s - top)).  top follows the maximum
-// only where the row's new maximum is more than kSlack above it (in log2),
-// so most blocks leave the sums as they are: weights stay below 2^kSlack,
-// far from the types' largest values, and relative to each other as exact.
-constexpr float kSlack = 8.f;
-template <int kN, int kB>
-__device__ __forceinline__ void softmax_step(float (&s)[kN], Softmax &x, f32x16 (&out)[kB],
-                                             float scale_log2) {
-  float most = s[0];
-#pragma unroll
-  for (int i = 1; i < kN; ++i) most = fmaxf(most, s[i]);
-  most = max_halves(most);
-  // (no comparison is true for a row that has seen nothing but -inf)
-  if (__ballot((most - x.top) * scale_log2 > kSlack)) {
-    const float top = fmaxf(most, x.top);
-    const float by = top == -kInf ? 1.f : exp2_fast((x.top - top) * scale_log2);
-    x.top = top;
-    x.sum *= by;
-#pragma unroll
-    for (int b = 0; b < kB; ++b)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) out[b][r] *= by;
-  }
-  const float shift = x.top == -kInf ? 0.f : x.top * scale_log2;
-  float sum = 0.f;
-#pragma unroll
-  for (int i = 0; i < kN; ++i) {
-    s[i] = exp2_fast(fmaf(s[i], scale_log2, -shift));
-    sum += s[i];
-  }
-  x.sum += sum;
-}
-
 // Rows of a tile are pairs (query, head of the group), the group's heads next
 // to each other: the heads that share keys share their tiles, and short
 // sequences still fill rows.  A wave has 32 rows and all of the tile's keys;
@@ -64,9 +23,7 @@ __device__ __forceinline__ void softmax_step(float (&s)[kN], Softmax &x, f32x16 
 template <typename T, int DP, int kKeys>
 __global__ __launch_bounds__(kThreads, sizeof(T) == 4 && DP > 64 ? 1 : 2) void packed_forward_kernel(
     PackedArgs A) {
-  using S = Shape<T, DP>;
   extern __shared__ __attribute__((aligned(16))) char lds[];
-  constexpr int kTile = S::tile_bytes(kKeys);  // buffers: K0 V0 K1 V1
   constexpr int kRows = kWaves * kWaveRows;
   const int head = blockIdx.x % A.k_heads;
   // late tiles, the long ones of a causal sequence, start first
@@ -80,7 +37,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 4 && DP > 64 ? 1 : 2) void p
   const int r0 = (index - first) * kRows;
   if (r0 >= rows) return;
 
-  const int lane = lane_id(), wave = wave_id(), c = lane & 31, h = lane >> 5;
+  const int wave = wave_id(), c = lane_id() & 31, h = lane_id() >> 5;
   const int row = r0 + wave * kWaveRows + c;
   const bool valid = row < rows;
   const int row_in = valid ? row : rows - 1;
@@ -92,7 +49,6 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 4 && DP > 64 ? 1 : 2) void p
   const int limit = A.causal ? min(seq.nk, query + ahead + 1) : seq.nk;
   const int last_query = A.group.div(min(r0 + kRows, rows) - 1);
   const int keys = A.causal ? max(0, min(seq.nk, last_query + ahead + 1)) : seq.nk;
-  const int tiles = (keys + kKeys - 1) / kKeys;
   // the wave's least limit (no mask below it) and its greatest (nothing above)
   const int w0 = r0 + wave * kWaveRows;
   const int low = A.causal ? min(seq.nk, A.group.div(min(w0, rows - 1)) + ahead + 1) : seq.nk;
@@ -103,55 +59,11 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 4 && DP > 64 ? 1 : 2) void p
 
   Frags<T, DP> q;
   row_frags<T, DP>(q, A.q.at + token * A.q.row + q_head * A.q.head, A.chunks, true);
-  const char *k_at = A.k.at + seq.k0 * A.k.row + head * A.k.head;
-  const char *v_at = A.v.at + seq.k0 * A.v.row + head * A.v.head;
-  auto load_tile = [&](int t) {
-    char *to = lds + (t & 1) * 2 * kTile;
-    const int k0 = t * kKeys, most = seq.nk - 1;
-    stage<T, DP, kKeys, kThreads>(to, threadIdx.x, A.chunks, [&](int r) {
-      return k_at + int64_t(min(k0 + r, most)) * A.k.row;
-    });
-    stage<T, DP, kKeys, kThreads>(to + kTile, threadIdx.x, A.chunks, [&](int r) {
-      return v_at + int64_t(min(k0 + r, most)) * A.v.row;
-    });
-  };
-  clear_rest<T, DP>(lds, 4 * kKeys, threadIdx.x, kThreads, A.chunks);
-
   Sums<T, DP> out = {};
   Softmax x;
-  if (tiles > 0) load_tile(0);
-  for (int t = 0; t < tiles; ++t) {
-    wait_loads<0>();
-    __syncthreads();  // tile t is there, and tile t - 1 has been read
-    if (t + 1 < tiles) load_tile(t + 1);
-    const char *k_tile = lds + (t & 1) * 2 * kTile, *v_tile = k_tile + kTile;
-    const int k0 = t * kKeys;
-    if (!wave_on || k0 >= high) continue;
-    float s[kKeys / 2];
-#pragma unroll
-    for (int b = 0; b < kKeys / 32; ++b) {
-      const f32x16 dots = dot_rows<T, DP>(k_tile, 32 * b, q);
-#pragma unroll
-      for (int r = 0; r < 16; ++r) s[16 * b + r] = dots[r];
-    }
-    if (k0 + kKeys > low) {
-#pragma unroll
-      for (int b = 0; b < kKeys / 32; ++b)
-#pragma unroll
-        for (int r = 0; r < 16; ++r)
-          if (k0 + 32 * b + c_row(r, h) >= limit) s[16 * b + r] = -kInf;
-    }
-    softmax_step(s, x, out, A.scale_log2);
-#pragma unroll
-    for (int b = 0; b < kKeys / 32; ++b) {
-      float p[16];
-#pragma unroll
-      for (int r = 0; r < 16; ++r) p[r] = s[16 * b + r];
-      Weights<T> w;
-      w.set(p);
-      add_transposed<T, DP>(out, v_tile, 32 * b, w);
-    }
-  }
+  attend_tiles<T, DP, kKeys>(lds, q, A.k.at + seq.k0 * A.k.row + head * A.k.head, A.k.row,
+                             A.v.at + seq.k0 * A.v.row + head * A.v.head, A.v.row, A.chunks, 0,
+                             keys, seq.nk, limit, low, wave_on ? high : 0, A.scale_log2, x, out);
 
   const float sum = sum_halves(x.sum);
   const bool any = x.top > -kInf || sum != 0.f;

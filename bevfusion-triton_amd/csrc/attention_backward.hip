@@ -200,8 +200,7 @@ __global__ __launch_bounds__(kThreads, DP * sizeof(T) > 128 ? 1 : 2) void key_gr
       const int row = min(r0 + lane, rows - 1), i = A.group.div(row);
       const float *at = (wave ? A.delta : A.lse2) + stat0 + int64_t(i) * A.q_heads + row - i * group;
       float *put = stats + ((t & 1) * 2 + wave) * kRows;
-      __builtin_amdgcn_global_load_lds((const ATTENTION_GLOBAL void *)at,
-                                       (ATTENTION_LDS void *)put, 4, 0, 0);
+      load_to_lds4(reinterpret_cast<const char *>(at), reinterpret_cast<const char *>(put));
     }
   };
   clear_rest<T, DP>(lds, 4 * kRows, threadIdx.x, kThreads, A.chunks);

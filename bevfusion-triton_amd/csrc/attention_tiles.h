@@ -48,7 +48,6 @@ constexpr float kLog2e = 1.44269504088896340736f;
 constexpr float kInf = __builtin_inff();
 
 #define ATTENTION_LDS __attribute__((address_space(3)))
-#define ATTENTION_GLOBAL __attribute__((address_space(1)))
 
 template <typename T>
 struct Mat;
@@ -123,6 +122,10 @@ __device__ __forceinline__ float sum_halves(float v) {
 
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 
+// Waits until this wave's reads of LDS are done (before a load overwrites
+// what they read).
+__device__ __forceinline__ void wait_reads() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
+
 // Waits until this wave's loads to LDS, all but the newest `left` of them,
 // have arrived.
 template <int kLeft>
@@ -131,8 +134,35 @@ __device__ __forceinline__ void wait_loads() {
   asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kLeft) : "memory");
 }
 
+// One load of 16 bytes a lane from `from` to LDS, lane i's at `to` (the same
+// for the wave) + 16 i; lanes that are off load nothing.  As asm, for the
+// compiler would make the next read of LDS, of whatever buffer, wait for it:
+// wait_loads() and a barrier stand before the reads that need it.  It writes
+// no register.
+__device__ __forceinline__ void load_to_lds(const char *from, const char *to) {
+  const unsigned at = unsigned(uintptr_t((const ATTENTION_LDS char *)to));
+  asm volatile(
+      "s_mov_b32 m0, %0\n\t"
+      "s_nop 0\n\t"
+      "global_load_lds_dwordx4 %1, off" ::"s"(__builtin_amdgcn_readfirstlane(int(at))),
+      "v"(from)
+      : "memory");
+}
+
+// The same of 4 bytes a lane.
+__device__ __forceinline__ void load_to_lds4(const char *from, const char *to) {
+  const unsigned at = unsigned(uintptr_t((const ATTENTION_LDS char *)to));
+  asm volatile(
+      "s_mov_b32 m0, %0\n\t"
+      "s_nop 0\n\t"
+      "global_load_lds_dword %1, off" ::"s"(__builtin_amdgcn_readfirstlane(int(at))),
+      "v"(from)
+      : "memory");
+}
+
 // Fills kRows rows of a tile with kLanes lanes; row(i) gives the address of
 // row i's first byte.  Chunks past the head's `chunks` are left as they are.
+// Every wave issues kRows * kPitch / kLanes loads (each round has a chunk 0).
 template <typename T, int DP, int kRows, int kLanes, typename Row>
 __device__ __forceinline__ void stage(char *tile, int thread, int chunks, Row row) {
   constexpr int kPitch = Shape<T, DP>::kPitch;
@@ -141,14 +171,7 @@ __device__ __forceinline__ void stage(char *tile, int thread, int chunks, Row ro
   for (int i = 0; i < kRows * kPitch / kLanes; ++i) {
     const int slot = i * kLanes + thread;
     const int r = slot / kPitch, c = (slot % kPitch) ^ (r & 7);
-    if (c < chunks) {
-      char *to = tile + (i * kLanes + (thread & ~63)) * 16;  // (the wave's; a lane adds 16 each)
-      __builtin_amdgcn_global_load_lds(
-          (const ATTENTION_GLOBAL void *)(row(r) + c * 16),
-          (ATTENTION_LDS void *)(uintptr_t)(unsigned)(__builtin_amdgcn_readfirstlane(
-              int((uintptr_t)(ATTENTION_LDS char *)to))),
-          16, 0, 0);
-    }
+    if (c < chunks) load_to_lds(row(r) + c * 16, tile + (i * kLanes + (thread & ~63)) * 16);
   }
 }
 
@@ -255,6 +278,106 @@ __device__ __forceinline__ void add_transposed(Sums<T, DP> &acc, const char *til
         const i16x8 a = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
         acc[b] = Mat<T>::mma(__builtin_bit_cast(typename Mat<T>::Frag, a), w.f[j], acc[b]);
       }
+    }
+  }
+}
+
+// Running softmax of one row: a lane and lane ^ 32 share it, with half of a
+// block's keys each.
+struct Softmax {
+  float top = -kInf;  // the maximum that the weights are relative to
+  float sum = 0.f;    // of this lane's half of the keys
+};
+
+// Takes kN scores of this lane's row (raw products, -inf where masked):
+// they become weights exp2(scale_log2 (s - top)).  top follows the maximum
+// only where the row's new maximum is more than kSlack above it (in log2),
+// so most blocks leave the sums as they are: weights stay below 2^kSlack,
+// far from the types' largest values, and relative to each other as exact.
+constexpr float kSlack = 8.f;
+template <int kN, int kB>
+__device__ __forceinline__ void softmax_step(float (&s)[kN], Softmax &x, f32x16 (&out)[kB],
+                                             float scale_log2) {
+  float most = s[0];
+#pragma unroll
+  for (int i = 1; i < kN; ++i) most = fmaxf(most, s[i]);
+  most = max_halves(most);
+  // (no comparison is true for a row that has seen nothing but -inf)
+  if (__ballot((most - x.top) * scale_log2 > kSlack)) {
+    const float top = fmaxf(most, x.top);
+    const float by = top == -kInf ? 1.f : exp2_fast((x.top - top) * scale_log2);
+    x.top = top;
+    x.sum *= by;
+#pragma unroll
+    for (int b = 0; b < kB; ++b)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) out[b][r] *= by;
+  }
+  const float shift = x.top == -kInf ? 0.f : x.top * scale_log2;
+  float sum = 0.f;
+#pragma unroll
+  for (int i = 0; i < kN; ++i) {
+    s[i] = exp2_fast(fmaf(s[i], scale_log2, -shift));
+    sum += s[i];
+  }
+  x.sum += sum;
+}
+
+// A wave's 32 rows (fragments q) against the keys [begin, end) of one head,
+// in tiles of kKeys keys staged by the whole block in two buffers (K0 V0 K1
+// V1), the next tile's loads in flight while one is used.  This lane's row
+// sees the keys below `limit`; every row of the wave those below `low` (no
+// mask there), none those from `high` on.  Keys from `stored` on are not
+// read.  The block calls it together, with the same begin and end.
+template <typename T, int DP, int kKeys>
+__device__ __forceinline__ void attend_tiles(char *lds, const Frags<T, DP> &q, const char *k_at,
+                                             int64_t k_row, const char *v_at, int64_t v_row,
+                                             int chunks, int begin, int end, int stored, int limit,
+                                             int low, int high, float scale_log2, Softmax &x,
+                                             Sums<T, DP> &out) {
+  constexpr int kTile = Shape<T, DP>::tile_bytes(kKeys);
+  const int h = lane_id() >> 5;
+  auto load_tile = [&](int k0, int buffer) {
+    char *to = lds + buffer * 2 * kTile;
+    stage<T, DP, kKeys, kThreads>(to, threadIdx.x, chunks, [&](int r) {
+      return k_at + int64_t(min(k0 + r, stored - 1)) * k_row;
+    });
+    stage<T, DP, kKeys, kThreads>(to + kTile, threadIdx.x, chunks, [&](int r) {
+      return v_at + int64_t(min(k0 + r, stored - 1)) * v_row;
+    });
+  };
+  clear_rest<T, DP>(lds, 4 * kKeys, threadIdx.x, kThreads, chunks);
+  if (begin < end) load_tile(begin, 0);
+  int buffer = 0;
+  for (int k0 = begin; k0 < end; k0 += kKeys, buffer ^= 1) {
+    wait_loads<0>();
+    __syncthreads();  // this tile is there, and the last one has been read
+    if (k0 + kKeys < end) load_tile(k0 + kKeys, buffer ^ 1);
+    const char *k_tile = lds + buffer * 2 * kTile, *v_tile = k_tile + kTile;
+    if (k0 >= high) continue;
+    float s[kKeys / 2];
+#pragma unroll
+    for (int b = 0; b < kKeys / 32; ++b) {
+      const f32x16 dots = dot_rows<T, DP>(k_tile, 32 * b, q);
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s[16 * b + r] = dots[r];
+    }
+    if (k0 + kKeys > low) {
+#pragma unroll
+      for (int b = 0; b < kKeys / 32; ++b)
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          if (k0 + 32 * b + c_row(r, h) >= limit) s[16 * b + r] = -kInf;
+    }
+    softmax_step(s, x, out, scale_log2);
+#pragma unroll
+    for (int b = 0; b < kKeys / 32; ++b) {
+      float p[16];
+#pragma unroll
+      for (int r = 0; r < 16; ++r) p[r] = s[16 * b + r];
+      Weights<T> w;
+      w.set(p);
+      add_transposed<T, DP>(out, v_tile, 32 * b, w);
     }
   }
 }

@@ -615,6 +615,37 @@ int bevpool_attention_backward(const void *q, int64_t q_row, int64_t q_head, con
                                size_t scratch_bytes, void *stream);
 
 /*
+ * Attention of new tokens over caches, with a prefix that all requests share
+ * and that is read once for all of them.  Request b's cache holds
+ * lengths[b] keys (clamped to [0, capacity]), the newest `tokens` of them its
+ * new tokens' own; new token i sees the whole prefix and the cache's first
+ * lengths[b] - (tokens - 1 - i) keys.  A row that sees nothing gets zeros.
+ *   q            (requests * tokens, q_heads, dim)
+ *   k, v         (requests, capacity, k_heads, dim); slots past a request's
+ *                length are never read
+ *   prefix_k, prefix_v   (prefix, k_heads, dim), or prefix 0
+ *   lengths      device int32 [requests]
+ *   dim          a multiple of 8, at most 128; requests, rows and heads start
+ *                at multiples of 16 bytes
+ *   out          (requests * tokens, q_heads, dim) contiguous
+ *   scratch      >= bevpool_attention_cached_scratch_bytes(...) (may be 0:
+ *                then NULL)
+ */
+size_t bevpool_attention_cached_scratch_bytes(int32_t requests, int32_t tokens, int32_t capacity,
+                                              int32_t prefix, int32_t q_heads, int32_t k_heads,
+                                              int32_t dim);
+
+int bevpool_attention_cached(const void *q, int64_t q_row, int64_t q_head, const void *k,
+                             int64_t k_request, int64_t k_row, int64_t k_head, const void *v,
+                             int64_t v_request, int64_t v_row, int64_t v_head,
+                             const void *prefix_k, int64_t prefix_k_row, int64_t prefix_k_head,
+                             const void *prefix_v, int64_t prefix_v_row, int64_t prefix_v_head,
+                             const int32_t *lengths, int32_t dtype, int32_t requests,
+                             int32_t tokens, int32_t capacity, int32_t prefix, int32_t q_heads,
+                             int32_t k_heads, int32_t dim, float scale, void *out, void *scratch,
+                             size_t scratch_bytes, void *stream);
+
+/*
  * Optional per-kernel timing.  When enabled, every kernel launch is bracketed
  * by HIP events on the launch stream; bevpool_timing_read() synchronises
  * those events and returns, per kernel name, the summed milliseconds and

@@ -140,3 +140,22 @@ def attend_packed(q, k, v, q_starts, k_starts, causal, scale, dout=None, dtype=t
         value, bound = res[n]
         bound += u * value.abs() + tiny
     return res
+
+
+def attend_cached(q, k, v, lengths, prefix_k, prefix_v, scale, dtype):
+    """(value, bound) of out (requests, tokens, heads, dim): every row as a
+    packed sequence of one query over its prefix and its own keys."""
+    B, n, heads, dim = q.shape
+    value, bound = torch.zeros(q.shape).double(), torch.zeros(q.shape).double()
+    for b in range(B):
+        for i in range(n):
+            own = min(max(int(lengths[b]), 0), k.shape[1]) - (n - 1 - i)
+            own = max(own, 0)
+            kk, vv = k[b, :own], v[b, :own]
+            if prefix_k is not None:
+                kk, vv = torch.cat((prefix_k, kk)), torch.cat((prefix_v, vv))
+            res = attend_packed(q[b, i][None], kk, vv, torch.tensor([0, 1]),
+                                torch.tensor([0, kk.shape[0]]), False, scale, dtype=dtype)
+            value[b, i], bound[b, i] = (t[0] for t in res['out'])
+    # the parts' weights: two exponentials and products more
+    return value, bound + 16 * F * bound / U[dtype]

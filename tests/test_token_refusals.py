@@ -54,3 +54,27 @@ def test_attention(pkg):
     assert lib.bevpool_attention_backward_scratch_bytes(4, 4) == 4 * 4 * 2 * 4
     assert lib.bevpool_attention_backward(*args, None, 0, None) == -3
     assert b'scratch' in lib.bevpool_last_error()
+
+
+def test_cached_attention(pkg):
+    lib = pkg.library()
+
+    def call(dtype=2, requests=2, tokens=1, capacity=64, prefix=0, q_heads=4, k_heads=2, dim=64,
+             scale=0.125, q=16, k=16, request=64 * 128, pk=None, lengths=16, scratch=None, nbytes=0):
+        return lib.bevpool_attention_cached(
+            q, 256, 64, k, request, 128, 64, 16, request, 128, 64, pk, 128, 64, pk, 128, 64,
+            lengths, dtype, requests, tokens, capacity, prefix, q_heads, k_heads, dim, scale, 16,
+            scratch, nbytes, None)
+
+    for bad, text in ((dict(dtype=3), b'dtype'), (dict(tokens=0), b'bad sizes'),
+                      (dict(capacity=-1), b'bad sizes'), (dict(q_heads=3), b'bad sizes'),
+                      (dict(requests=1 << 30), b'bad sizes'), (dict(dim=20), b'multiple of 8'),
+                      (dict(scale=0.0), b'scale'), (dict(lengths=None), b'lengths'),
+                      (dict(q=None), b'q: null'), (dict(k=8), b'16 bytes'),
+                      (dict(request=64 * 128 + 4), b'16 bytes'), (dict(prefix=9), b'prefix_k')):
+        assert call(**bad) == -1, bad
+        assert text in lib.bevpool_last_error(), bad
+    need = lib.bevpool_attention_cached_scratch_bytes(2, 1, 5000, 0, 4, 2, 64)
+    assert need > 0 and need % ((64 + 2) * 4 * 2 * 4) == 0
+    assert call(capacity=5000, scratch=16, nbytes=need - 1) == -3
+    assert lib.bevpool_attention_cached_scratch_bytes(2, 1, 64, 0, 4, 2, 64) == 0
