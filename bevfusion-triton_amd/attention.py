@@ -191,11 +191,14 @@ def norm_rotate(q, k, positions, frequencies, pairs=None, *, q_weight=None, k_we
 
 # ---- attention over packed sequences ---------------------------------------
 
-def _aligned(x):
-    """x with unit stride along dim and every row and head at a multiple of 16
-    bytes, as the kernels' 16-byte accesses need: itself, or a copy."""
-    per = 16 // x.element_size()
-    if x.stride(-1) == 1 and x.data_ptr() % 16 == 0 and all(s % per == 0 for s in x.stride()[:-1]):
+def _aligned(x, group=1):
+    """x (rows, heads, dim) with unit stride along dim, every row and head at a
+    multiple of 16 bytes, and strides whose multiples over a tile (64 rows,
+    the heads of a group) the kernels form in 32 bits: itself, or a copy."""
+    size = x.element_size()
+    row, head = x.stride(0) * size, x.stride(1) * size
+    if (x.stride(-1) == 1 and x.data_ptr() % 16 == 0 and row % 16 == 0 and head % 16 == 0
+            and row < 1 << 24 and head * group < 1 << 30):
         return x
     return x.contiguous() if not x.is_contiguous() else x.clone()
 
@@ -234,7 +237,8 @@ def _check_starts(name, starts, like):
 class _AttendPacked(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, q_starts, k_starts, causal, scale):
-        q, k, v = _aligned(q), _aligned(k), _aligned(v)
+        group = q.shape[1] // k.shape[1]
+        q, k, v = _aligned(q, group), _aligned(k), _aligned(v)
         out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
         lse = torch.empty(q.shape[:2], dtype=torch.float32, device=q.device)
         _run(lambda lib, s: lib.bevpool_attention_forward(
@@ -251,7 +255,7 @@ class _AttendPacked(torch.autograd.Function):
     def backward(ctx, dout, _):
         q, k, v, out, lse, q_starts, k_starts = ctx.saved_tensors
         causal, scale = ctx.call
-        dout = _aligned(dout.to(q.dtype))
+        dout = _aligned(dout.to(q.dtype), q.shape[1] // k.shape[1])
         dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
         nbytes = L.library().bevpool_attention_backward_scratch_bytes(q.shape[0], q.shape[1])
         scratch = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
@@ -303,8 +307,10 @@ def _cache(name, x, dims):
     _check_rows(name, x, dims)
     per = 16 // x.element_size()
     if x.numel() and (x.stride(-1) != 1 or x.data_ptr() % 16
-                      or any(s % per for s in x.stride()[:-1])):
-        raise ValueError(f'{name}: rows and heads must start at multiples of 16 bytes.')
+                      or any(s % per for s in x.stride()[:-1])
+                      or x.stride(-3) >= per << 20):
+        raise ValueError(f'{name}: rows and heads must start at multiples of 16 bytes, rows less '
+                         'than 16 MiB apart.')
     return x
 
 

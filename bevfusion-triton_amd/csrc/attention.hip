@@ -137,6 +137,9 @@ int set_operand(Operand &o, const char *what, const void *at, int64_t row, int64
   o.row = row * elem;
   o.head = head * elem;
   if (total > 0 && !at) return fail(BEVPOOL_EINVAL, "%s: null", what);
+  // (the offsets of 64 rows are 32-bit)
+  if (total > 0 && (o.row < 0 || o.head < 0 || o.row >= (1 << 24)))
+    return fail(BEVPOOL_EINVAL, "%s: strides must be positive, a row's below 2^24 bytes", what);
   if (total > 0 && (reinterpret_cast<uintptr_t>(at) % 16 || o.row % 16 || o.head % 16))
     return fail(BEVPOOL_EINVAL, "%s: rows and heads must start at multiples of 16 bytes", what);
   return BEVPOOL_OK;

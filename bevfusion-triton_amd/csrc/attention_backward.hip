@@ -24,13 +24,13 @@ using bevpool_host::fail;
 using bevpool_host::LaunchScope;
 
 struct BackwardArgs : PackedArgs {
-  const float *lse2;  // (tokens, heads): L in units of log 2
+  const float2 *stats;  // (tokens, heads): L in units of log 2, and D
 };
 
 // D and L / log 2 of every (token, head): a row's 16-byte chunks on kLanes
 // lanes.
 template <typename T, int kLanes>
-__global__ __launch_bounds__(kThreads) void delta_kernel(PackedArgs A, float *lse2, float *delta) {
+__global__ __launch_bounds__(kThreads) void stats_kernel(PackedArgs A, float2 *stats) {
   constexpr int kPer = 16 / sizeof(T);
   const int64_t row = int64_t(blockIdx.x) * (kThreads / kLanes) + threadIdx.x / kLanes;
   const int chunk = threadIdx.x % kLanes;
@@ -48,10 +48,7 @@ __global__ __launch_bounds__(kThreads) void delta_kernel(PackedArgs A, float *ls
   }
 #pragma unroll
   for (int m = 1; m < kLanes; m <<= 1) sum += __shfl_xor(sum, m, 64);
-  if (chunk == 0) {
-    delta[row] = sum;
-    lse2[row] = A.lse[row] * kLog2e;
-  }
+  if (chunk == 0) stats[row] = make_float2(A.lse[row] * kLog2e, sum);
 }
 
 // dq: rows and tiles as in the forward.
@@ -95,19 +92,20 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 4 && DP > 64 ? 1 : 2) void q
   Frags<T, DP> q, g;
   row_frags<T, DP>(q, A.q.at + token * A.q.row + q_head * A.q.head, A.chunks, true);
   row_frags<T, DP>(g, A.dout.at + token * A.dout.row + q_head * A.dout.head, A.chunks, true);
-  const float lse2 = A.lse2[token * A.q_heads + q_head];
-  const float delta = A.delta[token * A.q_heads + q_head];
+  const float2 both = A.stats[token * A.q_heads + q_head];
+  float stat[2] = {both.x, both.y};
+  settle(stat);
+  const float lse2 = stat[0], delta = stat[1];
   const char *k_at = A.k.at + seq.k0 * A.k.row + head * A.k.head;
   const char *v_at = A.v.at + seq.k0 * A.v.row + head * A.v.head;
+  const unsigned lds0 = lds_address(lds);
+  Stage<T, DP, kKeys, kThreads> k_stage, v_stage;
+  k_stage.set(A.chunks, [&](int r) { return r * int(A.k.row); });
+  v_stage.set(A.chunks, [&](int r) { return r * int(A.v.row); });
   auto load_tile = [&](int t) {
-    char *to = lds + (t & 1) * 2 * kTile;
-    const int k0 = t * kKeys, most = seq.nk - 1;
-    stage<T, DP, kKeys, kThreads>(to, threadIdx.x, A.chunks, [&](int r) {
-      return k_at + int64_t(min(k0 + r, most)) * A.k.row;
-    });
-    stage<T, DP, kKeys, kThreads>(to + kTile, threadIdx.x, A.chunks, [&](int r) {
-      return v_at + int64_t(min(k0 + r, most)) * A.v.row;
-    });
+    const unsigned to = lds0 + (t & 1) * 2 * kTile;
+    load_rows(k_stage, k_at, A.k.row, t * kKeys, seq.nk, to);
+    load_rows(v_stage, v_at, A.v.row, t * kKeys, seq.nk, to + kTile);
   };
   clear_rest<T, DP>(lds, 4 * kKeys, threadIdx.x, kThreads, A.chunks);
 
@@ -123,8 +121,15 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 4 && DP > 64 ? 1 : 2) void q
     const bool masked = k0 + kKeys > low;
 #pragma unroll
     for (int b = 0; b < kKeys / 32; ++b) {
-      const f32x16 dots = dot_rows<T, DP>(k_tile, 32 * b, q);
-      const f32x16 dp = dot_rows<T, DP>(v_tile, 32 * b, g);
+      Frags<T, DP> k, v;
+      read_rows<T, DP>(k, k_tile, 32 * b);
+      read_rows<T, DP>(v, v_tile, 32 * b);
+      pin_reads();
+      const f32x16 dots = dot_rows<T, DP>(k, q);
+      const f32x16 dp = dot_rows<T, DP>(v, g);
+      Columns<T, DP> kt;
+      kt.read(k_tile, 32 * b);
+      pin_reads();
       float p[16];
 #pragma unroll
       for (int r = 0; r < 16; ++r)
@@ -136,22 +141,52 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 4 && DP > 64 ? 1 : 2) void q
       }
       Weights<T> w;
       w.set(p);
-      add_transposed<T, DP>(dq, k_tile, 32 * b, w);
+      kt.add(dq, w);
     }
   }
   store_row<T, DP>(A.dq.at + token * A.dq.row + q_head * A.dq.head, dq, A.scale, A.dim, valid);
 }
 
+// How the keys' kernel keeps a wave's 32 keys: their K and V fragments and
+// both sums take 6 DP / 4 registers a lane in the 16-bit types (twice that in
+// float).  Up to 6 * 128 bytes / 4 that leaves room for two waves a SIMD,
+// which hide each other's waits; for heads of more than 192 bytes it does so
+// with V in LDS, read again for every 32 rows.
+template <typename T, int DP>
+struct KeyPlan {
+  static constexpr bool kTwoWaves = DP * sizeof(T) <= 256;
+  static constexpr bool kValuesInLds = kTwoWaves && DP * sizeof(T) > 192;
+  // Two groups of four waves with the same keys take the rows' tiles in
+  // turn: a sequence's first keys are seen by all its rows, and the longest
+  // walk is what the launch ends with.
+  static constexpr int kGroups = kTwoWaves ? 2 : 1;
+  static constexpr int kThreads = 256 * kGroups;
+  static constexpr int kRows = 32;  // of a tile
+  static constexpr int kTile = Shape<T, DP>::tile_bytes(kRows);
+  // Three buffers of Q and dout rows: a tile's loads are given the time of
+  // two tiles, as many rows come from beyond L2.  Behind them the rows' L and
+  // D, in pairs.
+  static constexpr int kBuffers = 3;
+  static constexpr int kGroupLds = kBuffers * (2 * kTile + 8 * kRows);
+  static constexpr int kValues =
+      kValuesInLds ? Shape<T, DP>::tile_bytes(kWaves * kWaveRows) : 0;
+  // (the second group's sums pass through LDS at the end)
+  static constexpr int kSums = kGroups > 1 ? 256 * 64 * Shape<T, DP>::kBlocks : 0;
+  static constexpr int kTiles = kGroups * kGroupLds + kValues;
+  static constexpr int kLds = kTiles > kSums ? kTiles : kSums;
+  static_assert(kLds <= 160 * 1024, "LDS of a CU");
+};
+
 // dk and dv: a wave owns 32 keys and walks the sequence's rows (query, head
-// of the group), kRows at a time, in two buffers.
-template <typename T, int DP, int kRows>
-__global__ __launch_bounds__(kThreads, DP * sizeof(T) > 128 ? 1 : 2) void key_grad_kernel(
-    BackwardArgs A) {
-  using S = Shape<T, DP>;
+// of the group) in tiles of 32, from the last to the first that sees one of
+// its keys: blocks of one sequence start together there, and find each
+// other's rows in L2.
+template <typename T, int DP>
+__global__ __launch_bounds__((KeyPlan<T, DP>::kThreads), 1) void key_grad_kernel(BackwardArgs A) {
+  using Plan = KeyPlan<T, DP>;
+  constexpr int kRows = Plan::kRows, kTile = Plan::kTile, kGroups = Plan::kGroups;
+  constexpr int kSteps = Shape<T, DP>::kSteps, kBlocks = Shape<T, DP>::kBlocks;
   extern __shared__ __attribute__((aligned(16))) char lds[];
-  // buffers: Q0 G0 Q1 G1, then L0 D0 L1 D1 of kRows floats
-  constexpr int kTile = S::tile_bytes(kRows);
-  float *stats = reinterpret_cast<float *>(lds + 4 * kTile);
   constexpr int kKeys = kWaves * kWaveRows;
   const int head = blockIdx.x % A.k_heads;
   const int index = int(blockIdx.x / A.k_heads);
@@ -163,107 +198,233 @@ __global__ __launch_bounds__(kThreads, DP * sizeof(T) > 128 ? 1 : 2) void key_gr
   const int kb = (index - first) * kKeys;
   if (kb >= seq.nk) return;
 
-  const int lane = lane_id(), wave = wave_id(), c = lane & 31, h = lane >> 5;
+  const int lane = lane_id(), c = lane & 31, h = lane >> 5;
+  const int group_of = kGroups == 1 ? 0 : wave_id() / kWaves, wave = wave_id() % kWaves;
+  char *tiles_at = lds + group_of * Plan::kGroupLds;
+  constexpr int kBuffers = Plan::kBuffers;
+  const float *stats = reinterpret_cast<const float *>(tiles_at + kBuffers * 2 * kTile);
+  char *values = lds + kGroups * Plan::kGroupLds;
   const int key0 = kb + wave * kWaveRows, key = key0 + c;
   const bool valid = key < seq.nk;
   const int64_t k_row = seq.k0 + (valid ? key : seq.nk - 1);
-  const int group = A.group.size, rows = seq.nq * group;
+  const int heads = A.group.size, rows = seq.nq * heads;
   const int ahead = seq.nk - seq.nq;
   // key j is seen by the queries from j - ahead on: packed rows from
-  // (j - ahead) * group; first for the block, for this key, for the wave's
+  // (j - ahead) * heads; first for the block, for this key, for the wave's
   // last key and its first
-  const int begin = A.causal ? max(0, min(kb - ahead, seq.nq)) * group : 0;
-  const int from = A.causal ? (key - ahead) * group : 0;
-  const int from_last = A.causal ? (key0 + kWaveRows - 1 - ahead) * group : 0;
-  const int from_first = A.causal ? (key0 - ahead) * group : 0;
+  const int begin = A.causal ? max(0, min(kb - ahead, seq.nq)) * heads : 0;
+  const int from = A.causal ? (key - ahead) * heads : 0;
+  const int from_last = A.causal ? (key0 + kWaveRows - 1 - ahead) * heads : 0;
+  const int from_first = A.causal ? (key0 - ahead) * heads : 0;
   const int tiles = (rows - begin + kRows - 1) / kRows;
 
   Frags<T, DP> k, v;
   row_frags<T, DP>(k, A.k.at + k_row * A.k.row + head * A.k.head, A.chunks, true);
-  row_frags<T, DP>(v, A.v.at + k_row * A.v.row + head * A.v.head, A.chunks, true);
-  const char *q_at = A.q.at + seq.q0 * A.q.row + int64_t(head) * group * A.q.head;
-  const char *g_at = A.dout.at + seq.q0 * A.dout.row + int64_t(head) * group * A.dout.head;
-  const int64_t stat0 = int64_t(seq.q0) * A.q_heads + head * group;
-  auto load_tile = [&](int t) {
-    char *to = lds + (t & 1) * 2 * kTile;
-    const int r0 = begin + t * kRows;
-    stage<T, DP, kRows, kThreads>(to, threadIdx.x, A.chunks, [&](int r) {
-      const int row = min(r0 + r, rows - 1), i = A.group.div(row);
-      return q_at + i * A.q.row + (row - i * group) * A.q.head;
-    });
-    stage<T, DP, kRows, kThreads>(to + kTile, threadIdx.x, A.chunks, [&](int r) {
-      const int row = min(r0 + r, rows - 1), i = A.group.div(row);
-      return g_at + i * A.dout.row + (row - i * group) * A.dout.head;
-    });
-    // wave 0: L of the rows, wave 1: D
-    if (wave < 2 && lane < kRows) {
-      const int row = min(r0 + lane, rows - 1), i = A.group.div(row);
-      const float *at = (wave ? A.delta : A.lse2) + stat0 + int64_t(i) * A.q_heads + row - i * group;
-      float *put = stats + ((t & 1) * 2 + wave) * kRows;
-      load_to_lds4(reinterpret_cast<const char *>(at), reinterpret_cast<const char *>(put));
-    }
+  if constexpr (Plan::kValuesInLds) {
+    Stage<T, DP, kKeys, Plan::kThreads> v_stage;
+    v_stage.set(A.chunks, [&](int r) { return r * int(A.v.row); });
+    load_rows(v_stage, A.v.at + seq.k0 * A.v.row + head * A.v.head, A.v.row, kb, seq.nk,
+              lds_address(values));
+    clear_rest<T, DP>(values, kKeys, threadIdx.x, Plan::kThreads, A.chunks);
+  } else {
+    row_frags<T, DP>(v, A.v.at + k_row * A.v.row + head * A.v.head, A.chunks, true);
+  }
+  const char *q_at = A.q.at + seq.q0 * A.q.row + int64_t(head) * heads * A.q.head;
+  const char *g_at = A.dout.at + seq.q0 * A.dout.row + int64_t(head) * heads * A.dout.head;
+  const int64_t stat0 = int64_t(seq.q0) * A.q_heads + head * heads;
+  const unsigned tiles0 = lds_address(lds) + group_of * Plan::kGroupLds;
+  // Where kRows is a multiple of the group's heads, a tile's rows lie alike
+  // in every tile (the first one starts with a query), but for the last's.
+  const bool alike = kRows % heads == 0;
+  Stage<T, DP, kRows, 256> q_stage, g_stage;
+  auto place = [&](int row, const Operand &o) {
+    const int i = A.group.div(row);
+    return i * int(o.row) + (row - i * heads) * int(o.head);
   };
-  clear_rest<T, DP>(lds, 4 * kRows, threadIdx.x, kThreads, A.chunks);
+  q_stage.set(A.chunks, [&](int r) { return alike ? place(r, A.q) : 0; });
+  g_stage.set(A.chunks, [&](int r) { return alike ? place(r, A.dout) : 0; });
+  auto load_tile = [&](int t, int buffer) {
+    const unsigned to = tiles0 + buffer * 2 * kTile;
+    const int r0 = begin + (tiles - 1 - t) * kRows, i0 = A.group.div(r0);
+    // rows from r0 on, as rows from the query that r0 belongs to on
+    const int skip = r0 - i0 * heads, last = rows - 1 - i0 * heads;
+    const char *q_base = q_at + i0 * A.q.row, *g_base = g_at + i0 * A.dout.row;
+    if (alike && r0 + kRows <= rows) {
+      q_stage.load(q_base, to);
+      g_stage.load(g_base, to + kTile);
+    } else {
+      q_stage.load(q_base, to, [&](int r) { return place(min(skip + r, last), A.q); });
+      g_stage.load(g_base, to + kTile, [&](int r) { return place(min(skip + r, last), A.dout); });
+    }
+    // L and D of 32 rows, a lane each (by every wave: all count the same loads)
+    const int row = min(skip + (lane >> 1), last), i = A.group.div(row);
+    load_to_lds4(reinterpret_cast<const char *>(A.stats + stat0 + int64_t(i0) * A.q_heads),
+                 unsigned((i * A.q_heads + row - i * heads) * 2 + (lane & 1)) * 4,
+                 tiles0 + kBuffers * 2 * kTile + buffer * kRows * 8);
+  };
+  constexpr int kTileLoads = 2 * Stage<T, DP, kRows, 256>::kLoads + 1;
+  clear_rest<T, DP>(tiles_at, kBuffers * 2 * kRows, threadIdx.x % 256, 256, A.chunks);
 
   Sums<T, DP> dk = {}, dv = {};
-  if (tiles > 0) load_tile(0);
-  for (int t = 0; t < tiles; ++t) {
-    wait_loads<0>();
-    __syncthreads();  // tile t is there, and tile t - 1 has been read
-    if (t + 1 < tiles) load_tile(t + 1);
-    const char *q_tile = lds + (t & 1) * 2 * kTile, *g_tile = q_tile + kTile;
-    const float *l_row = stats + (t & 1) * 2 * kRows, *d_row = l_row + kRows;
-    const int r0 = begin + t * kRows;
-    if (key0 >= seq.nk || r0 + kRows <= from_first) continue;
+  if (group_of < tiles) load_tile(group_of, 0);
+  if (group_of + kGroups < tiles) load_tile(group_of + kGroups, 1);
+  int buffer = 0;
+  // (both groups go round as often: they share the barrier)
+  for (int t0 = 0; t0 < tiles; t0 += kGroups, buffer = buffer == kBuffers - 1 ? 0 : buffer + 1) {
+    const int t = t0 + group_of;
+    if (t + kGroups < tiles)
+      wait_loads<kTileLoads>();  // all but the next tile's
+    else
+      wait_loads<0>();
+    tile_barrier();  // tile t is there, and the last one has been read
+    if (t + 2 * kGroups < tiles)
+      load_tile(t + 2 * kGroups, buffer == 0 ? kBuffers - 1 : buffer - 1);
+    const char *q_tile = tiles_at + buffer * 2 * kTile, *g_tile = q_tile + kTile;
+    const float *stat_row = stats + buffer * 2 * kRows;
+    const int r0 = begin + (tiles - 1 - t) * kRows;
+    if (t >= tiles || key0 >= seq.nk || r0 + kRows <= from_first) continue;
     const bool masked = r0 < from_last || r0 + kRows > rows;
+    // (hides that the addresses of the reads are the same in every round: to
+    // keep them all takes more registers than there are)
+    int at_lane = lane;
+    if constexpr (DP * sizeof(T) > 192) asm volatile("" : "+v"(at_lane));
+    // Four fragments are read while four are in use.
+    f32x16 dots = {}, dp = {};
+    Piece<T> x[2];
+    read_piece<T, DP, 4>(x[0], q_tile, 0, 0, at_lane);
+    constexpr int kDotPieces = (kSteps + 3) / 4;
 #pragma unroll
-    for (int b = 0; b < kRows / 32; ++b) {
-      const f32x16 dots = dot_rows<T, DP>(q_tile, 32 * b, k);
-      const f32x16 dp = dot_rows<T, DP>(g_tile, 32 * b, v);
-      float p[16], ds[16];
+    for (int n = 0; n < kDotPieces; ++n) {
+      if (n + 1 < kDotPieces) {
+        read_piece<T, DP, 4>(x[(n + 1) & 1], q_tile, 0, 4 * n + 4, at_lane);
+      } else if constexpr (Plan::kValuesInLds) {
+        read_piece<T, DP, 2>(x[(n + 1) & 1], g_tile, 0, 0, at_lane);
+        read_piece<T, DP, 2, 2>(x[(n + 1) & 1], values, wave * kWaveRows, 0, at_lane);
+      } else {
+        read_piece<T, DP, 4>(x[(n + 1) & 1], g_tile, 0, 0, at_lane);
+      }
+      pin_reads();
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const f32x4 l = *reinterpret_cast<const f32x4 *>(l_row + 32 * b + 8 * i + 4 * h);
-        const f32x4 d = *reinterpret_cast<const f32x4 *>(d_row + 32 * b + 8 * i + 4 * h);
+      for (int i = 0; i < 4; ++i)
+        if (4 * n + i < kSteps) dots = Mat<T>::mma(x[n & 1][i], k[4 * n + i], dots);
+      pin_reads();
+    }
+    constexpr int kPer = Plan::kValuesInLds ? 2 : 4;
+    constexpr int kGradPieces = (kSteps + kPer - 1) / kPer;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int r = 4 * i + j;
-          p[r] = exp2_fast(fmaf(dots[r], A.scale_log2, -l[j]));
-          ds[r] = p[r] * (dp[r] - d[j]);
-          if (masked) {
-            const int at = r0 + 32 * b + c_row(r, h);
-            if (at < from || at >= rows) p[r] = ds[r] = 0.f;
-          }
+    for (int n = 0; n < kGradPieces; ++n) {
+      Piece<T> &now = x[(kDotPieces + n) & 1], &next = x[(kDotPieces + n + 1) & 1];
+      if (n + 1 < kGradPieces) {
+        if constexpr (Plan::kValuesInLds) {
+          read_piece<T, DP, 2>(next, g_tile, 0, 2 * n + 2, at_lane);
+          read_piece<T, DP, 2, 2>(next, values, wave * kWaveRows, 2 * n + 2, at_lane);
+        } else {
+          read_piece<T, DP, 4>(next, g_tile, 0, 4 * n + 4, at_lane);
         }
       }
-      Weights<T> w;
-      w.set(p);
-      add_transposed<T, DP>(dv, g_tile, 32 * b, w);
-      w.set(ds);
-      add_transposed<T, DP>(dk, q_tile, 32 * b, w);
+      pin_reads();
+#pragma unroll
+      for (int i = 0; i < kPer; ++i)
+        if (kPer * n + i < kSteps) {
+          if constexpr (Plan::kValuesInLds)
+            dp = Mat<T>::mma(now[i], now[2 + i], dp);
+          else
+            dp = Mat<T>::mma(now[i], v[kPer * n + i], dp);
+        }
+      pin_reads();
     }
+    float p[16], ds[16];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      // L and D of four rows
+      const f32x4 s01 = *reinterpret_cast<const f32x4 *>(stat_row + 16 * i + 8 * h);
+      const f32x4 s23 = *reinterpret_cast<const f32x4 *>(stat_row + 16 * i + 8 * h + 4);
+      const float l[4] = {s01[0], s01[2], s23[0], s23[2]};
+      const float d[4] = {s01[1], s01[3], s23[1], s23[3]};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int r = 4 * i + j;
+        p[r] = exp2_fast(fmaf(dots[r], A.scale_log2, -l[j]));
+        ds[r] = p[r] * (dp[r] - d[j]);
+        if (masked) {
+          const int at = r0 + c_row(r, h);
+          if (at < from || at >= rows) p[r] = ds[r] = 0.f;
+        }
+      }
+    }
+    Weights<T> w, u;
+    w.set(p);
+    u.set(ds);
+    if constexpr (sizeof(T) == 4) {
+      Columns<T, DP> g, q;
+      g.read(g_tile, 0);
+      q.read(q_tile, 0);
+      g.add(dv, w, at_lane);
+      q.add(dk, u, at_lane);
+    } else {
+      constexpr int kAt = kDotPieces + kGradPieces, kPieces = (kBlocks + 1) / 2;
+      pin_reads();
+      read_column_piece<T, DP>(x[kAt & 1], g_tile, 0, 0, at_lane);
+#pragma unroll
+      for (int n = 0; n < 2 * kPieces; ++n) {
+        Piece<T> &now = x[(kAt + n) & 1], &next = x[(kAt + n + 1) & 1];
+        if (n + 1 < 2 * kPieces)
+          read_column_piece<T, DP>(next, n + 1 < kPieces ? g_tile : q_tile, 0,
+                                   2 * ((n + 1) % kPieces), at_lane);
+        pin_reads();
+        if (n < kPieces)
+          add_column_piece<T, DP>(dv, now, w, 2 * n);
+        else
+          add_column_piece<T, DP>(dk, now, u, 2 * (n - kPieces));
+        pin_reads();
+      }
+    }
+  }
+
+  if constexpr (kGroups > 1) {
+    // the second group hands its sums over, dk and then dv
+    float *sums = reinterpret_cast<float *>(lds) + wave * (kBlocks * 16 * 64) + lane;
+#pragma unroll
+    for (int n = 0; n < 2; ++n) {
+      Sums<T, DP> &mine = n == 0 ? dk : dv;
+      __syncthreads();
+      if (group_of == 1) {
+#pragma unroll
+        for (int b = 0; b < kBlocks; ++b)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) sums[(b * 16 + r) * 64] = mine[b][r];
+      }
+      __syncthreads();
+      if (group_of == 0) {
+#pragma unroll
+        for (int b = 0; b < kBlocks; ++b)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) mine[b][r] += sums[(b * 16 + r) * 64];
+      }
+    }
+    if (group_of == 1) return;
   }
   store_row<T, DP>(A.dk.at + k_row * A.dk.row + head * A.dk.head, dk, A.scale, A.dim, valid);
   store_row<T, DP>(A.dv.at + k_row * A.dv.row + head * A.dv.head, dv, 1.f, A.dim, valid);
 }
 
 template <typename T, int DP>
-int launch_backward(BackwardArgs &A, float *lse2, float *delta, hipStream_t s) {
+int launch_backward(BackwardArgs &A, float2 *stats, hipStream_t s) {
   constexpr int kLanes = sizeof(T) == 4 ? 32 : 16;
-  constexpr int kKeys = sizeof(T) == 4 ? 32 : 64;  // rows of a tile, too
+  constexpr int kKeys = sizeof(T) == 4 ? 32 : 64;
   constexpr int kLds = 4 * Shape<T, DP>::tile_bytes(kKeys);
-  static_assert(kLds + 16 * kKeys <= 160 * 1024, "LDS of a CU");
+  static_assert(kLds <= 160 * 1024, "LDS of a CU");
   int st = BEVPOOL_OK;
   if (A.q_total > 0) {
     const int64_t rows = int64_t(A.q_total) * A.q_heads, per = kThreads / kLanes;
-    st = check_grid((rows + per - 1) / per, kThreads, "attention delta");
+    st = check_grid((rows + per - 1) / per, kThreads, "attention row sums");
     if (st) return st;
     {
-      LaunchScope scope("attention_delta", s);
-      hipLaunchKernelGGL((delta_kernel<T, kLanes>), dim3(unsigned((rows + per - 1) / per)),
-                         dim3(kThreads), 0, s, static_cast<const PackedArgs &>(A), lse2, delta);
+      LaunchScope scope("attention_stats", s);
+      hipLaunchKernelGGL((stats_kernel<T, kLanes>), dim3(unsigned((rows + per - 1) / per)),
+                         dim3(kThreads), 0, s, static_cast<const PackedArgs &>(A), stats);
     }
-    st = check_launch("attention delta");
+    st = check_launch("attention row sums");
     if (st) return st;
     A.tiles = int(int64_t(A.q_total) * A.group.size / (kWaves * kWaveRows)) + A.sequences + 1;
     const int64_t blocks = int64_t(A.tiles) * A.k_heads;
@@ -279,12 +440,13 @@ int launch_backward(BackwardArgs &A, float *lse2, float *delta, hipStream_t s) {
   }
   if (A.k_total > 0) {
     A.tiles = A.k_total / (kWaves * kWaveRows) + A.sequences + 1;
+    using Plan = KeyPlan<T, DP>;
     const int64_t blocks = int64_t(A.tiles) * A.k_heads;
-    st = check_grid(blocks, kThreads, "attention key gradient");
+    st = check_grid(blocks, Plan::kThreads, "attention key gradient");
     if (st) return st;
     LaunchScope scope("attention_key_grad", s);
-    hipLaunchKernelGGL((key_grad_kernel<T, DP, kKeys>), dim3(unsigned(blocks)), dim3(kThreads),
-                       kLds + 16 * kKeys, s, A);
+    hipLaunchKernelGGL((key_grad_kernel<T, DP>), dim3(unsigned(blocks)), dim3(Plan::kThreads),
+                       Plan::kLds, s, A);
     st = check_launch("attention key gradient");
   }
   return st;
@@ -324,19 +486,21 @@ int bevpool_attention_backward(const void *q, int64_t q_row, int64_t q_head, con
   if (!st) st = set_operand(A.dv, "dv", dv, k_dense, dim, elem, k_total);
   if (st) return st;
   if (q_total > 0 && !lse) return fail(BEVPOOL_EINVAL, "lse: null");
+  // (as are those of a tile's rows, heads of a group among them)
+  const int64_t heads = A.group.size < 64 ? A.group.size : 64;
+  if (A.q.head * heads >= (1 << 30) || A.dout.head * heads >= (1 << 30))
+    return fail(BEVPOOL_EINVAL, "q, dout: the heads of a group must lie within 2^30 bytes");
   const size_t need = bevpool_attention_backward_scratch_bytes(q_total, q_heads);
   if (scratch_bytes < need || (need > 0 && !scratch))
     return fail(BEVPOOL_ESPACE, "attention backward scratch: %zu bytes, %zu needed",
                 scratch_bytes, need);
   A.lse = const_cast<float *>(lse);
-  float *lse2 = static_cast<float *>(scratch);
-  float *delta = lse2 + q_total * q_heads;
-  A.lse2 = lse2;
-  A.delta = delta;
+  float2 *stats = static_cast<float2 *>(scratch);
+  A.stats = stats;
   hipStream_t s = static_cast<hipStream_t>(stream);
-  return dtype == BEVPOOL_BF16  ? (ATTENTION_DIM(__bf16, launch_backward, A, lse2, delta, s))
-         : dtype == BEVPOOL_F16 ? (ATTENTION_DIM(_Float16, launch_backward, A, lse2, delta, s))
-                                : (ATTENTION_DIM(float, launch_backward, A, lse2, delta, s));
+  return dtype == BEVPOOL_BF16  ? (ATTENTION_DIM(__bf16, launch_backward, A, stats, s))
+         : dtype == BEVPOOL_F16 ? (ATTENTION_DIM(_Float16, launch_backward, A, stats, s))
+                                : (ATTENTION_DIM(float, launch_backward, A, stats, s));
 }
 
 }  // extern "C"

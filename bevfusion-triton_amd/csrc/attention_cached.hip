@@ -87,14 +87,14 @@ __global__ __launch_bounds__(kThreads, 1) void cached_part_kernel(CachedArgs A) 
   const char *k_at = A.k.at + request * A.k.request + head * A.k.head;
   const char *v_at = A.v.at + request * A.v.request + head * A.v.head;
   char *mine = lds + wave * kMine;
+  const unsigned mine0 = lds_address(lds) + wave * kMine;
+  Stage<T, DP, 32, 64> k_stage, v_stage;
+  k_stage.set(A.chunks, [&](int r) { return r * int(A.k.row); });
+  v_stage.set(A.chunks, [&](int r) { return r * int(A.v.row); });
   auto load_tile = [&](int k0, int buffer) {
-    char *to = mine + buffer * 2 * kTile;
-    stage<T, DP, 32, 64>(to, lane, A.chunks, [&](int r) {
-      return k_at + int64_t(min(k0 + r, length - 1)) * A.k.row;
-    });
-    stage<T, DP, 32, 64>(to + kTile, lane, A.chunks, [&](int r) {
-      return v_at + int64_t(min(k0 + r, length - 1)) * A.v.row;
-    });
+    const unsigned to = mine0 + buffer * 2 * kTile;
+    load_rows(k_stage, k_at, A.k.row, k0, length, to);
+    load_rows(v_stage, v_at, A.v.row, k0, length, to + kTile);
   };
   clear_rest<T, DP>(mine, kBuffers * 64, lane, 64, A.chunks);
 
@@ -114,13 +114,19 @@ __global__ __launch_bounds__(kThreads, 1) void cached_part_kernel(CachedArgs A) 
     }
     const char *k_tile = mine + buffer * 2 * kTile;
     float s[16];
-    const f32x16 dots = dot_rows<T, DP>(k_tile, 0, q);
+    Frags<T, DP> k;
+    read_rows<T, DP>(k, k_tile, 0);
+    pin_reads();
+    const f32x16 dots = dot_rows<T, DP>(k, q);
 #pragma unroll
     for (int r = 0; r < 16; ++r) s[r] = k0 + c_row(r, h) < limit ? dots[r] : -kInf;
     softmax_step(s, x, out, A.scale_log2);
     Weights<T> w;
     w.set(s);
-    add_transposed<T, DP>(out, k_tile + kTile, 0, w);
+    Columns<T, DP> v;
+    v.read(k_tile + kTile, 0);
+    pin_reads();
+    v.add(out, w);
     if (kBuffers == 2) {
       buffer ^= 1;
     } else if (k0 + kStep < end) {

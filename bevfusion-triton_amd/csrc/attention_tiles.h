@@ -16,9 +16,8 @@
 // and comes from LDS by the transposing read (16-bit types) or one element a
 // lane (float).
 //
-// Tiles lie in LDS as rows of kPitch 16-byte chunks, chunk c of row r at
-// c ^ (r & 7): eight consecutive rows of one chunk, which a fragment read
-// takes at once, are in eight different bank groups.  They are filled by
+// Tiles lie in LDS as rows of kPitch 16-byte chunks, swizzled so that reads
+// spread over the banks (see swizzle()).  They are filled by
 // loads from global memory straight to LDS; since such a load writes its
 // lanes' 16 bytes in lane order, the swizzle is on the side of the global
 // address.
@@ -134,45 +133,111 @@ __device__ __forceinline__ void wait_loads() {
   asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kLeft) : "memory");
 }
 
-// One load of 16 bytes a lane from `from` to LDS, lane i's at `to` (the same
-// for the wave) + 16 i; lanes that are off load nothing.  As asm, for the
-// compiler would make the next read of LDS, of whatever buffer, wait for it:
-// wait_loads() and a barrier stand before the reads that need it.  It writes
-// no register.
-__device__ __forceinline__ void load_to_lds(const char *from, const char *to) {
-  const unsigned at = unsigned(uintptr_t((const ATTENTION_LDS char *)to));
-  asm volatile(
-      "s_mov_b32 m0, %0\n\t"
-      "s_nop 0\n\t"
-      "global_load_lds_dwordx4 %1, off" ::"s"(__builtin_amdgcn_readfirstlane(int(at))),
-      "v"(from)
-      : "memory");
+// A barrier behind this wave's reads of LDS.  Unlike __syncthreads() it does
+// not wait for loads to LDS that are still on their way to other buffers.
+__device__ __forceinline__ void tile_barrier() {
+  asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
 }
 
+// One load of 16 bytes a lane from `base` + `offset` to LDS, lane i's at `to`
+// (the same for the wave) + 16 i; lanes that are off load nothing.  As asm,
+// for the compiler would make the next read of LDS, of whatever buffer, wait
+// for it: wait_loads() and a barrier stand before the reads that need it.  It
+// writes no register.  The compiler does not see a memory access here, so the
+// block itself keeps the five wait states that one needs behind a vector
+// instruction that wrote its scalar base (a reload of a spilled one, say),
+// and the one behind a write of m0.
+__device__ __forceinline__ void load_to_lds(const char *base, unsigned offset, unsigned to) {
+  asm volatile(
+      "s_mov_b32 m0, %0\n\t"
+      "s_nop 3\n\t"
+      "global_load_lds_dwordx4 %1, %2" ::"s"(__builtin_amdgcn_readfirstlane(int(to))),
+      "v"(offset), "s"(base)
+      : "memory");
+}
 // The same of 4 bytes a lane.
-__device__ __forceinline__ void load_to_lds4(const char *from, const char *to) {
-  const unsigned at = unsigned(uintptr_t((const ATTENTION_LDS char *)to));
+__device__ __forceinline__ void load_to_lds4(const char *base, unsigned offset, unsigned to) {
   asm volatile(
       "s_mov_b32 m0, %0\n\t"
-      "s_nop 0\n\t"
-      "global_load_lds_dword %1, off" ::"s"(__builtin_amdgcn_readfirstlane(int(at))),
-      "v"(from)
+      "s_nop 3\n\t"
+      "global_load_lds_dword %1, %2" ::"s"(__builtin_amdgcn_readfirstlane(int(to))),
+      "v"(offset), "s"(base)
       : "memory");
 }
 
-// Fills kRows rows of a tile with kLanes lanes; row(i) gives the address of
-// row i's first byte.  Chunks past the head's `chunks` are left as they are.
-// Every wave issues kRows * kPitch / kLanes loads (each round has a chunk 0).
-template <typename T, int DP, int kRows, int kLanes, typename Row>
-__device__ __forceinline__ void stage(char *tile, int thread, int chunks, Row row) {
-  constexpr int kPitch = Shape<T, DP>::kPitch;
+__device__ __forceinline__ unsigned lds_address(const char *p) {
+  return unsigned(uintptr_t((const ATTENTION_LDS char *)p));
+}
+
+// Where chunk c of row r lies in its row: at c ^ swizzle(r).  LDS gives 256
+// bytes a cycle, 16 chunks.  A fragment read takes one chunk of 16 rows at
+// once, a transposing read four chunks of four rows: with rows of a multiple
+// of 256 bytes the four low bits of r, those of r % 4 first, put either into
+// 16 different places; with rows of an odd number of 128 bytes, neighbours
+// are in different halves by themselves and the next bits do the rest.  For
+// float the second kind of read is 8 chunks of the rows r and r + 4.
+template <typename T, int DP>
+__device__ __forceinline__ int swizzle(int r) {
+  if constexpr (Shape<T, DP>::kPitch % 16 != 0) return (r & 2) << 1 | ((r >> 2) & 3);
+  if constexpr (sizeof(T) == 4) return (r & 4) << 1 | (r & 3) << 1 | ((r >> 3) & 1);
+  return (r & 3) << 2 | ((r >> 2) & 3);
+}
+
+// Fills tiles of kRows rows with kLanes lanes: this lane's 16-byte pieces of
+// a tile, as offsets that stay the same from tile to tile.  Chunks past the
+// head's `chunks` are left as they are.  Every wave issues kLoads loads for a
+// tile (each of its rounds has a chunk 0).
+template <typename T, int DP, int kRows, int kLanes>
+struct Stage {
+  static constexpr int kPitch = Shape<T, DP>::kPitch;
+  static constexpr int kLoads = kRows * kPitch / kLanes;
   static_assert(kRows * kPitch % kLanes == 0, "whole rounds");
-#pragma unroll
-  for (int i = 0; i < kRows * kPitch / kLanes; ++i) {
-    const int slot = i * kLanes + thread;
-    const int r = slot / kPitch, c = (slot % kPitch) ^ (r & 7);
-    if (c < chunks) load_to_lds(row(r) + c * 16, tile + (i * kLanes + (thread & ~63)) * 16);
+  unsigned at[kLoads];
+  bool on[kLoads];
+  __device__ __forceinline__ static int row(int i) {
+    return (i * kLanes + int(threadIdx.x) % kLanes) / kPitch;
   }
+  __device__ __forceinline__ static int chunk(int i) {
+    return (i * kLanes + int(threadIdx.x) % kLanes) % kPitch ^ swizzle<T, DP>(row(i));
+  }
+  // place(r): bytes from a tile's base to its row r
+  template <typename Place>
+  __device__ __forceinline__ void set(int chunks, Place place) {
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) {
+      at[i] = unsigned(place(row(i))) + chunk(i) * 16;
+      on[i] = chunk(i) < chunks;
+    }
+  }
+  __device__ __forceinline__ void load(const char *base, unsigned tile) const {
+    const unsigned wave = wave_id() % (kLanes / 64) * 1024;
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i)
+      if (on[i]) load_to_lds(base, at[i], tile + i * kLanes * 16 + wave);
+  }
+  // the same with rows placed for this tile alone
+  template <typename Place>
+  __device__ __forceinline__ void load(const char *base, unsigned tile, Place place) const {
+    const unsigned wave = wave_id() % (kLanes / 64) * 1024;
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i)
+      if (on[i])
+        load_to_lds(base, unsigned(place(row(i))) + chunk(i) * 16,
+                    tile + i * kLanes * 16 + wave);
+  }
+};
+
+// Rows [k0, k0 + kRows) of an operand into a tile, rows from `stored` on as
+// the last one there is.  (Offsets within a tile fit 32 bits: strides are
+// checked.)
+template <typename T, int DP, int kRows, int kLanes>
+__device__ __forceinline__ void load_rows(const Stage<T, DP, kRows, kLanes> &stage, const char *at,
+                                          int64_t stride, int k0, int stored, unsigned tile) {
+  const char *base = at + k0 * stride;
+  if (k0 + kRows <= stored)
+    stage.load(base, tile);
+  else
+    stage.load(base, tile, [&](int r) { return min(r, stored - 1 - k0) * int(stride); });
 }
 
 // Chunks [chunks, kChunks) of a tile's rows, which no load fills but a
@@ -183,18 +248,34 @@ __device__ __forceinline__ void clear_rest(char *tile, int rows, int thread, int
   constexpr int kPitch = Shape<T, DP>::kPitch, kChunks = Shape<T, DP>::kChunks;
   if (chunks >= kChunks) return;
   for (int i = thread; i < rows * kPitch; i += lanes) {
-    const int r = i / kPitch, c = (i % kPitch) ^ (r & 7);
+    const int r = i / kPitch, c = (i % kPitch) ^ swizzle<T, DP>(r);
     if (c >= chunks) *reinterpret_cast<u32x4 *>(tile + i * 16) = u32x4{0, 0, 0, 0};
   }
 }
 
-// Fragment s of row r0 + c of a tile (r0 a multiple of 8).
+// Keeps reads of LDS and matrix products above it above and those below it
+// below; all else may cross.  hipcc 7.2 otherwise puts each read right before
+// the product that needs it, and every product waits for LDS.
+__device__ __forceinline__ void pin_reads() { __builtin_amdgcn_sched_barrier(0x476); }
+
+// The fragments of rows r0 .. r0 + 31 of a tile (r0 a multiple of 32).
 template <typename T, int DP>
-__device__ __forceinline__ typename Mat<T>::Frag tile_frag(const char *tile, int r0, int s) {
+__device__ __forceinline__ void read_rows(Frags<T, DP> &f, const char *tile, int r0) {
   const int lane = lane_id(), c = lane & 31, h = lane >> 5;
-  const int chunk = (2 * s + h) ^ (c & 7);
-  return *reinterpret_cast<const typename Mat<T>::Frag *>(
-      tile + (r0 + c) * (Shape<T, DP>::kPitch * 16) + chunk * 16);
+#pragma unroll
+  for (int s = 0; s < Shape<T, DP>::kSteps; ++s) {
+    const int chunk = (2 * s + h) ^ swizzle<T, DP>(c);
+    f[s] = *reinterpret_cast<const typename Mat<T>::Frag *>(
+        tile + (r0 + c) * (Shape<T, DP>::kPitch * 16) + chunk * 16);
+  }
+}
+
+// Has the compiler's own loads into these registers arrive here: in a loop
+// behind loads to LDS that it does not count, it would wait for all of them.
+template <typename F, int kN>
+__device__ __forceinline__ void settle(F (&f)[kN]) {
+#pragma unroll
+  for (int i = 0; i < kN; ++i) asm volatile("" : "+v"(f[i]));
 }
 
 // Fragments of one row in global memory (chunks past the head's: zeros).
@@ -208,16 +289,15 @@ __device__ __forceinline__ void row_frags(Frags<T, DP> &f, const char *row, int 
       z = *reinterpret_cast<const typename Mat<T>::Frag *>(row + (2 * s + h) * 16);
     f[s] = z;
   }
+  settle(f);
 }
 
-// C = (tile rows r0 .. r0 + 31) x (the fragments' rows): scores.
+// C = (rows of a) x (rows of b): scores.
 template <typename T, int DP>
-__device__ __forceinline__ f32x16 dot_rows(const char *tile, int r0,
-                                           const Frags<T, DP> &f) {
+__device__ __forceinline__ f32x16 dot_rows(const Frags<T, DP> &a, const Frags<T, DP> &b) {
   f32x16 c = {};
 #pragma unroll
-  for (int s = 0; s < Shape<T, DP>::kSteps; ++s)
-    c = Mat<T>::mma(tile_frag<T, DP>(tile, r0, s), f[s], c);
+  for (int s = 0; s < Shape<T, DP>::kSteps; ++s) c = Mat<T>::mma(a[s], b[s], c);
   return c;
 }
 
@@ -239,47 +319,119 @@ struct Weights<float> {
   }
 };
 
-// acc[b] += (rows r0 .. r0 + 31 of the tile, elements 32 b .. 32 b + 31)^T x
-// weights.
+// Rows r0 .. r0 + 31 of a tile, transposed: A of a product over the rows, in
+// the order in which Weights holds them.
 template <typename T, int DP>
-__device__ __forceinline__ void add_transposed(Sums<T, DP> &acc, const char *tile, int r0,
-                                               const Weights<T> &w) {
-  constexpr int kRow = Shape<T, DP>::kPitch * 16;
-  const int lane = lane_id(), h = lane >> 5;
-  if constexpr (sizeof(T) == 4) {
-    // register r's row, one element a lane
-    const int c = lane & 31;
-#pragma unroll
-    for (int r = 0; r < 16; ++r) {
-      const int row = c_row(r, h);
-      const char *at = tile + (r0 + row) * kRow + (c & 3) * 4;
-#pragma unroll
-      for (int b = 0; b < Shape<T, DP>::kBlocks; ++b) {
-        const float a =
-            *reinterpret_cast<const float *>(at + ((8 * b + (c >> 2)) ^ (row & 7)) * 16);
-        acc[b] = __builtin_amdgcn_mfma_f32_32x32x2f32(a, w.f[r], acc[b], 0, 0, 0);
-      }
-    }
-  } else {
+struct Columns {
+  static constexpr int kBlocks = Shape<T, DP>::kBlocks;
+  typename Mat<T>::Frag f[kBlocks][2];
+  __device__ __forceinline__ void read(const char *tile, int r0) {
     // the transposing read gives lane i (of 16) element i of four rows; it
     // reads row i / 4, elements 4 (i % 4) .. + 3
+    constexpr int kRow = Shape<T, DP>::kPitch * 16;
+    const int lane = lane_id(), h = lane >> 5;
     const int row = 4 * h + ((lane & 15) >> 2);
     const int chunk = 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
     const char *at = tile + (r0 + row) * kRow + (lane & 1) * 8;
 #pragma unroll
-    for (int b = 0; b < Shape<T, DP>::kBlocks; ++b) {
-      const char *col = at + ((4 * b + chunk) ^ row) * 16;
+    for (int b = 0; b < kBlocks; ++b) {
+      const char *low = at + ((4 * b + chunk) ^ swizzle<T, DP>(row)) * 16;
+      const char *high = at + 8 * kRow + ((4 * b + chunk) ^ swizzle<T, DP>(row + 8)) * 16;
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
         const i16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-            (ATTENTION_LDS i16x4 *)(col + 16 * j * kRow));
+            (ATTENTION_LDS i16x4 *)(low + 16 * j * kRow));
         const i16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-            (ATTENTION_LDS i16x4 *)(col + (16 * j + 8) * kRow));
+            (ATTENTION_LDS i16x4 *)(high + 16 * j * kRow));
         const i16x8 a = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
-        acc[b] = Mat<T>::mma(__builtin_bit_cast(typename Mat<T>::Frag, a), w.f[j], acc[b]);
+        f[b][j] = __builtin_bit_cast(typename Mat<T>::Frag, a);
       }
     }
   }
+  // acc[b] += (columns 32 b .. 32 b + 31)^T x weights
+  __device__ __forceinline__ void add(Sums<T, DP> &acc, const Weights<T> &w) const {
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int b = 0; b < kBlocks; ++b)
+        acc[b] = Mat<T>::mma(f[b][j], w.f[j], acc[b]);
+  }
+};
+// float: one element a lane of register r's row, read as they are used.
+template <int DP>
+struct Columns<float, DP> {
+  static constexpr int kBlocks = Shape<float, DP>::kBlocks;
+  const char *at;
+  __device__ __forceinline__ void read(const char *tile, int r0) {
+    at = tile + r0 * (Shape<float, DP>::kPitch * 16);
+  }
+  __device__ __forceinline__ void add(Sums<float, DP> &acc, const Weights<float> &w,
+                                      int lane = lane_id()) const {
+    constexpr int kRow = Shape<float, DP>::kPitch * 16;
+    const int h = lane >> 5, c = lane & 31;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      const int row = c_row(r, h);
+#pragma unroll
+      for (int b = 0; b < kBlocks; ++b) {
+        const float a = *reinterpret_cast<const float *>(
+            at + row * kRow + ((8 * b + (c >> 2)) ^ swizzle<float, DP>(row)) * 16 + (c & 3) * 4);
+        acc[b] = __builtin_amdgcn_mfma_f32_32x32x2f32(a, w.f[r], acc[b], 0, 0, 0);
+      }
+    }
+  }
+};
+
+// Pieces of the above, four fragments at a time, for kernels that are short of
+// registers: rows' fragments s0 .. s0 + kN - 1 into f[kAt ..], and column
+// blocks b0, b0 + 1.
+template <typename T>
+using Piece = typename Mat<T>::Frag[4];
+
+template <typename T, int DP, int kN, int kAt = 0>
+__device__ __forceinline__ void read_piece(Piece<T> &f, const char *tile, int r0, int s0,
+                                           int lane) {
+  const int c = lane & 31, h = lane >> 5;
+#pragma unroll
+  for (int i = 0; i < kN; ++i)
+    if (s0 + i < Shape<T, DP>::kSteps)
+      f[kAt + i] = *reinterpret_cast<const typename Mat<T>::Frag *>(
+          tile + (r0 + c) * (Shape<T, DP>::kPitch * 16) +
+          ((2 * (s0 + i) + h) ^ swizzle<T, DP>(c)) * 16);
+}
+template <typename T, int DP>
+__device__ __forceinline__ void read_column_piece(Piece<T> &f, const char *tile, int r0, int b0,
+                                                  int lane) {
+  constexpr int kRow = Shape<T, DP>::kPitch * 16;
+  const int h = lane >> 5;
+  const int row = 4 * h + ((lane & 15) >> 2);
+  const int chunk = 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
+  const char *at = tile + (r0 + row) * kRow + (lane & 1) * 8;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    if (b0 + i >= Shape<T, DP>::kBlocks) continue;
+    const char *low = at + ((4 * (b0 + i) + chunk) ^ swizzle<T, DP>(row)) * 16;
+    const char *high = at + 8 * kRow + ((4 * (b0 + i) + chunk) ^ swizzle<T, DP>(row + 8)) * 16;
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const i16x4 lo =
+          __builtin_amdgcn_ds_read_tr16_b64_v4i16((ATTENTION_LDS i16x4 *)(low + 16 * j * kRow));
+      const i16x4 hi =
+          __builtin_amdgcn_ds_read_tr16_b64_v4i16((ATTENTION_LDS i16x4 *)(high + 16 * j * kRow));
+      const i16x8 a = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+      f[2 * i + j] = __builtin_bit_cast(typename Mat<T>::Frag, a);
+    }
+  }
+}
+template <typename T, int DP>
+__device__ __forceinline__ void add_column_piece(Sums<T, DP> &acc, const Piece<T> &f,
+                                                 const Weights<T> &w, int b0) {
+#pragma unroll
+  for (int j = 0; j < 2; ++j)
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      if (b0 + i < Shape<T, DP>::kBlocks)
+        acc[b0 + i] = Mat<T>::mma(f[2 * i + j], w.f[j], acc[b0 + i]);
 }
 
 // Running softmax of one row: a lane and lane ^ 32 share it, with half of a
@@ -337,14 +489,14 @@ __device__ __forceinline__ void attend_tiles(char *lds, const Frags<T, DP> &q, c
                                              Sums<T, DP> &out) {
   constexpr int kTile = Shape<T, DP>::tile_bytes(kKeys);
   const int h = lane_id() >> 5;
+  const unsigned lds0 = lds_address(lds);
+  Stage<T, DP, kKeys, kThreads> k_stage, v_stage;
+  k_stage.set(chunks, [&](int r) { return r * int(k_row); });
+  v_stage.set(chunks, [&](int r) { return r * int(v_row); });
   auto load_tile = [&](int k0, int buffer) {
-    char *to = lds + buffer * 2 * kTile;
-    stage<T, DP, kKeys, kThreads>(to, threadIdx.x, chunks, [&](int r) {
-      return k_at + int64_t(min(k0 + r, stored - 1)) * k_row;
-    });
-    stage<T, DP, kKeys, kThreads>(to + kTile, threadIdx.x, chunks, [&](int r) {
-      return v_at + int64_t(min(k0 + r, stored - 1)) * v_row;
-    });
+    const unsigned to = lds0 + buffer * 2 * kTile;
+    load_rows(k_stage, k_at, k_row, k0, stored, to);
+    load_rows(v_stage, v_at, v_row, k0, stored, to + kTile);
   };
   clear_rest<T, DP>(lds, 4 * kKeys, threadIdx.x, kThreads, chunks);
   if (begin < end) load_tile(begin, 0);
@@ -358,7 +510,10 @@ __device__ __forceinline__ void attend_tiles(char *lds, const Frags<T, DP> &q, c
     float s[kKeys / 2];
 #pragma unroll
     for (int b = 0; b < kKeys / 32; ++b) {
-      const f32x16 dots = dot_rows<T, DP>(k_tile, 32 * b, q);
+      Frags<T, DP> k;
+      read_rows<T, DP>(k, k_tile, 32 * b);
+      pin_reads();
+      const f32x16 dots = dot_rows<T, DP>(k, q);
 #pragma unroll
       for (int r = 0; r < 16; ++r) s[16 * b + r] = dots[r];
     }
@@ -377,7 +532,10 @@ __device__ __forceinline__ void attend_tiles(char *lds, const Frags<T, DP> &q, c
       for (int r = 0; r < 16; ++r) p[r] = s[16 * b + r];
       Weights<T> w;
       w.set(p);
-      add_transposed<T, DP>(out, v_tile, 32 * b, w);
+      Columns<T, DP> v;
+      v.read(v_tile, 32 * b);
+      pin_reads();
+      v.add(out, w);
     }
   }
 }
@@ -501,7 +659,6 @@ struct Operand {  // (rows, heads, dim), unit stride along dim; strides in bytes
 struct PackedArgs {
   Operand q, k, v, out, dout, dq, dk, dv;
   float *lse;          // (tokens, heads): log of the sum of exponentials
-  const float *delta;  // backward: (tokens, heads), sum of dout * out
   const int32_t *q_starts, *k_starts;  // sequences + 1
   int sequences, q_total, k_total;
   int q_heads, k_heads;
