@@ -149,94 +149,106 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 4 && DP > 64 ? 1 : 2) void q
 
 // How the keys' kernel keeps a wave's 32 keys: their K and V fragments and
 // both sums take 6 DP / 4 registers a lane in the 16-bit types (twice that in
-// float).  Up to 6 * 128 bytes / 4 that leaves room for two waves a SIMD,
-// which hide each other's waits; for heads of more than 192 bytes it does so
-// with V in LDS, read again for every 32 rows.
+// float).  For heads of up to 192 bytes that leaves room for two blocks a CU,
+// which hide each other's waits.  For longer heads dk and dv are two launches
+// of half the sums each: five products in place of four, but 10 MFLOP a
+// microsecond and CU at two blocks in place of 4 at one (heads of 128, bf16).
 template <typename T, int DP>
 struct KeyPlan {
-  static constexpr bool kTwoWaves = DP * sizeof(T) <= 256;
-  static constexpr bool kValuesInLds = kTwoWaves && DP * sizeof(T) > 192;
-  // Two groups of four waves with the same keys take the rows' tiles in
-  // turn: a sequence's first keys are seen by all its rows, and the longest
-  // walk is what the launch ends with.
-  static constexpr int kGroups = kTwoWaves ? 2 : 1;
-  static constexpr int kThreads = 256 * kGroups;
-  static constexpr int kRows = 32;  // of a tile
+  static constexpr bool kApart = DP * sizeof(T) > 192;
+  static constexpr int kBlocksPerCu = DP * sizeof(T) > 320 ? 1 : 2;
+  // Buffers of Q and dout rows, and behind them the rows' L and D in pairs.
+  static constexpr int kRows = sizeof(T) == 4 ? 32 : 64;  // of a tile
   static constexpr int kTile = Shape<T, DP>::tile_bytes(kRows);
-  // Three buffers of Q and dout rows: a tile's loads are given the time of
-  // two tiles, as many rows come from beyond L2.  Behind them the rows' L and
-  // D, in pairs.
-  static constexpr int kBuffers = 3;
-  static constexpr int kGroupLds = kBuffers * (2 * kTile + 8 * kRows);
-  static constexpr int kValues =
-      kValuesInLds ? Shape<T, DP>::tile_bytes(kWaves * kWaveRows) : 0;
-  // (the second group's sums pass through LDS at the end)
-  static constexpr int kSums = kGroups > 1 ? 256 * 64 * Shape<T, DP>::kBlocks : 0;
-  static constexpr int kTiles = kGroups * kGroupLds + kValues;
-  static constexpr int kLds = kTiles > kSums ? kTiles : kSums;
-  static_assert(kLds <= 160 * 1024, "LDS of a CU");
+  static constexpr int kBuffers = sizeof(T) == 4 ? 3 : 2;
+  static constexpr int kLds = kBuffers * (2 * kTile + 8 * kRows);
+  static_assert(kLds <= 160 * 1024 / kBlocksPerCu, "LDS of a CU");
+  static constexpr int kSums = 16 * Shape<T, DP>::kBlocks;  // registers of dk, and of dv
 };
+
+// Walks over the rows are cut where there are few of them: `splits` blocks a
+// key tile at most, each with about `steps` tiles of rows or more.
+struct Splits {
+  int most, steps;
+  float *sums;  // [key tile, head][split][dk, dv][wave][register][lane]
+  __device__ __forceinline__ int of(int tiles) const {
+    return max(1, min(most, (tiles + steps - 1) / steps));
+  }
+};
+
+// The key tile that a block works on.
+struct KeyTile {
+  Sequence seq;
+  int kb;        // first key
+  int begin;     // first row that sees one of its keys
+  int rows, tiles;
+};
+__device__ __forceinline__ bool key_tile_at(const BackwardArgs &A, int index, int tile_rows,
+                                            KeyTile &t) {
+  constexpr int kKeys = kWaves * kWaveRows;
+  int first;
+  const int which = find_sequence(A.k_starts, A.sequences, A.k_total, 1, kKeys, index, &first);
+  t.seq = sequence_at(A.q_starts, A.k_starts, which, A.sequences, A.q_total, A.k_total);
+  if (which == A.sequences) t.seq.nk = A.k_total - t.seq.k0;  // keys of no sequence: no queries
+  t.kb = (index - first) * kKeys;
+  t.rows = t.seq.nq * A.group.size;
+  // key j is seen by the queries from j - (nk - nq) on
+  t.begin = A.causal
+                ? max(0, min(t.kb - (t.seq.nk - t.seq.nq), t.seq.nq)) * A.group.size
+                : 0;
+  t.tiles = (t.rows - t.begin + tile_rows - 1) / tile_rows;
+  return t.kb < t.seq.nk;
+}
 
 // dk and dv: a wave owns 32 keys and walks the sequence's rows (query, head
 // of the group) in tiles of 32, from the last to the first that sees one of
 // its keys: blocks of one sequence start together there, and find each
 // other's rows in L2.
-template <typename T, int DP>
-__global__ __launch_bounds__((KeyPlan<T, DP>::kThreads), 1) void key_grad_kernel(BackwardArgs A) {
+template <typename T, int DP, bool kDk, bool kDv>
+__global__ __launch_bounds__(kThreads, (KeyPlan<T, DP>::kBlocksPerCu)) void key_grad_kernel(
+    BackwardArgs A, Splits splits) {
   using Plan = KeyPlan<T, DP>;
-  constexpr int kRows = Plan::kRows, kTile = Plan::kTile, kGroups = Plan::kGroups;
+  constexpr int kRows = Plan::kRows, kTile = Plan::kTile, kBuffers = Plan::kBuffers;
   constexpr int kSteps = Shape<T, DP>::kSteps, kBlocks = Shape<T, DP>::kBlocks;
   extern __shared__ __attribute__((aligned(16))) char lds[];
-  constexpr int kKeys = kWaves * kWaveRows;
   const int head = blockIdx.x % A.k_heads;
-  const int index = int(blockIdx.x / A.k_heads);
-  int first;
-  const int which =
-      find_sequence(A.k_starts, A.sequences, A.k_total, 1, kKeys, index, &first);
-  Sequence seq = sequence_at(A.q_starts, A.k_starts, which, A.sequences, A.q_total, A.k_total);
-  if (which == A.sequences) seq.nk = A.k_total - seq.k0;  // keys of no sequence: no queries
-  const int kb = (index - first) * kKeys;
-  if (kb >= seq.nk) return;
+  // the cuts of the long walks first
+  const int index = int(blockIdx.x / A.k_heads) % A.tiles;
+  const int split = splits.most - 1 - int(blockIdx.x / A.k_heads) / A.tiles;
+  KeyTile tile;
+  if (!key_tile_at(A, index, kRows, tile)) return;
+  const int n_splits = splits.of(tile.tiles);
+  if (split >= n_splits) return;
+  const Sequence seq = tile.seq;
+  const int kb = tile.kb, begin = tile.begin, rows = tile.rows;
+  // this block's tiles of rows, counted from the last
+  const int per_split = (tile.tiles + n_splits - 1) / n_splits;
+  const int t_begin = split * per_split, t_end = min(tile.tiles, t_begin + per_split);
 
-  const int lane = lane_id(), c = lane & 31, h = lane >> 5;
-  const int group_of = kGroups == 1 ? 0 : wave_id() / kWaves, wave = wave_id() % kWaves;
-  char *tiles_at = lds + group_of * Plan::kGroupLds;
-  constexpr int kBuffers = Plan::kBuffers;
-  const float *stats = reinterpret_cast<const float *>(tiles_at + kBuffers * 2 * kTile);
-  char *values = lds + kGroups * Plan::kGroupLds;
+  const int lane = lane_id(), wave = wave_id(), c = lane & 31, h = lane >> 5;
+  const float *stats = reinterpret_cast<const float *>(lds + kBuffers * 2 * kTile);
   const int key0 = kb + wave * kWaveRows, key = key0 + c;
   const bool valid = key < seq.nk;
   const int64_t k_row = seq.k0 + (valid ? key : seq.nk - 1);
-  const int heads = A.group.size, rows = seq.nq * heads;
+  const int heads = A.group.size;
   const int ahead = seq.nk - seq.nq;
-  // key j is seen by the queries from j - ahead on: packed rows from
-  // (j - ahead) * heads; first for the block, for this key, for the wave's
-  // last key and its first
-  const int begin = A.causal ? max(0, min(kb - ahead, seq.nq)) * heads : 0;
+  // the first packed row that sees this key, the wave's last key, its first
   const int from = A.causal ? (key - ahead) * heads : 0;
   const int from_last = A.causal ? (key0 + kWaveRows - 1 - ahead) * heads : 0;
   const int from_first = A.causal ? (key0 - ahead) * heads : 0;
-  const int tiles = (rows - begin + kRows - 1) / kRows;
 
   Frags<T, DP> k, v;
   row_frags<T, DP>(k, A.k.at + k_row * A.k.row + head * A.k.head, A.chunks, true);
-  if constexpr (Plan::kValuesInLds) {
-    Stage<T, DP, kKeys, Plan::kThreads> v_stage;
-    v_stage.set(A.chunks, [&](int r) { return r * int(A.v.row); });
-    load_rows(v_stage, A.v.at + seq.k0 * A.v.row + head * A.v.head, A.v.row, kb, seq.nk,
-              lds_address(values));
-    clear_rest<T, DP>(values, kKeys, threadIdx.x, Plan::kThreads, A.chunks);
-  } else {
+  if constexpr (kDk)
     row_frags<T, DP>(v, A.v.at + k_row * A.v.row + head * A.v.head, A.chunks, true);
-  }
   const char *q_at = A.q.at + seq.q0 * A.q.row + int64_t(head) * heads * A.q.head;
   const char *g_at = A.dout.at + seq.q0 * A.dout.row + int64_t(head) * heads * A.dout.head;
   const int64_t stat0 = int64_t(seq.q0) * A.q_heads + head * heads;
-  const unsigned tiles0 = lds_address(lds) + group_of * Plan::kGroupLds;
+  const unsigned tiles0 = lds_address(lds);
   // Where kRows is a multiple of the group's heads, a tile's rows lie alike
   // in every tile (the first one starts with a query), but for the last's.
   const bool alike = kRows % heads == 0;
-  Stage<T, DP, kRows, 256> q_stage, g_stage;
+  Stage<T, DP, kRows, kThreads> q_stage, g_stage;
   auto place = [&](int row, const Operand &o) {
     const int i = A.group.div(row);
     return i * int(o.row) + (row - i * heads) * int(o.head);
@@ -245,7 +257,7 @@ __global__ __launch_bounds__((KeyPlan<T, DP>::kThreads), 1) void key_grad_kernel
   g_stage.set(A.chunks, [&](int r) { return alike ? place(r, A.dout) : 0; });
   auto load_tile = [&](int t, int buffer) {
     const unsigned to = tiles0 + buffer * 2 * kTile;
-    const int r0 = begin + (tiles - 1 - t) * kRows, i0 = A.group.div(r0);
+    const int r0 = begin + (tile.tiles - 1 - t) * kRows, i0 = A.group.div(r0);
     // rows from r0 on, as rows from the query that r0 belongs to on
     const int skip = r0 - i0 * heads, last = rows - 1 - i0 * heads;
     const char *q_base = q_at + i0 * A.q.row, *g_base = g_at + i0 * A.dout.row;
@@ -257,159 +269,200 @@ __global__ __launch_bounds__((KeyPlan<T, DP>::kThreads), 1) void key_grad_kernel
       g_stage.load(g_base, to + kTile, [&](int r) { return place(min(skip + r, last), A.dout); });
     }
     // L and D of 32 rows, a lane each (by every wave: all count the same loads)
-    const int row = min(skip + (lane >> 1), last), i = A.group.div(row);
-    load_to_lds4(reinterpret_cast<const char *>(A.stats + stat0 + int64_t(i0) * A.q_heads),
-                 unsigned((i * A.q_heads + row - i * heads) * 2 + (lane & 1)) * 4,
-                 tiles0 + kBuffers * 2 * kTile + buffer * kRows * 8);
+#pragma unroll
+    for (int j = 0; j < kRows / 32; ++j) {
+      const int row = min(skip + 32 * j + (lane >> 1), last), i = A.group.div(row);
+      load_to_lds4(reinterpret_cast<const char *>(A.stats + stat0 + int64_t(i0) * A.q_heads),
+                   unsigned((i * A.q_heads + row - i * heads) * 2 + (lane & 1)) * 4,
+                   tiles0 + kBuffers * 2 * kTile + (buffer * kRows + 32 * j) * 8);
+    }
   };
-  constexpr int kTileLoads = 2 * Stage<T, DP, kRows, 256>::kLoads + 1;
-  clear_rest<T, DP>(tiles_at, kBuffers * 2 * kRows, threadIdx.x % 256, 256, A.chunks);
+  constexpr int kTileLoads = 2 * Stage<T, DP, kRows, kThreads>::kLoads + kRows / 32;
+  clear_rest<T, DP>(lds, kBuffers * 2 * kRows, threadIdx.x, kThreads, A.chunks);
 
   Sums<T, DP> dk = {}, dv = {};
-  if (group_of < tiles) load_tile(group_of, 0);
-  if (group_of + kGroups < tiles) load_tile(group_of + kGroups, 1);
+#pragma unroll
+  for (int i = 0; i < kBuffers - 1; ++i)
+    if (t_begin + i < t_end) load_tile(t_begin + i, i);
   int buffer = 0;
-  // (both groups go round as often: they share the barrier)
-  for (int t0 = 0; t0 < tiles; t0 += kGroups, buffer = buffer == kBuffers - 1 ? 0 : buffer + 1) {
-    const int t = t0 + group_of;
-    if (t + kGroups < tiles)
+  for (int t = t_begin; t < t_end; ++t, buffer = buffer == kBuffers - 1 ? 0 : buffer + 1) {
+    if (kBuffers == 3 && t + 1 < t_end)
       wait_loads<kTileLoads>();  // all but the next tile's
     else
       wait_loads<0>();
     tile_barrier();  // tile t is there, and the last one has been read
-    if (t + 2 * kGroups < tiles)
-      load_tile(t + 2 * kGroups, buffer == 0 ? kBuffers - 1 : buffer - 1);
-    const char *q_tile = tiles_at + buffer * 2 * kTile, *g_tile = q_tile + kTile;
+    if (t + kBuffers - 1 < t_end)
+      load_tile(t + kBuffers - 1, buffer == 0 ? kBuffers - 1 : buffer - 1);
+    const char *q_tile = lds + buffer * 2 * kTile, *g_tile = q_tile + kTile;
     const float *stat_row = stats + buffer * 2 * kRows;
-    const int r0 = begin + (tiles - 1 - t) * kRows;
-    if (t >= tiles || key0 >= seq.nk || r0 + kRows <= from_first) continue;
+    const int r0 = begin + (tile.tiles - 1 - t) * kRows;
+    if (key0 >= seq.nk || r0 + kRows <= from_first) continue;
     const bool masked = r0 < from_last || r0 + kRows > rows;
-    // (hides that the addresses of the reads are the same in every round: to
-    // keep them all takes more registers than there are)
+    // (hides that the addresses of the reads are the same in every round: kept,
+    // they take more registers than there are)
     int at_lane = lane;
-    if constexpr (DP * sizeof(T) > 192) asm volatile("" : "+v"(at_lane));
-    // Four fragments are read while four are in use.
-    f32x16 dots = {}, dp = {};
-    Piece<T> x[2];
-    read_piece<T, DP, 4>(x[0], q_tile, 0, 0, at_lane);
-    constexpr int kDotPieces = (kSteps + 3) / 4;
+    if constexpr ((kDk && kDv && DP > 80) || (sizeof(T) == 4 && DP > 64))
+      asm volatile("" : "+v"(at_lane));
 #pragma unroll
-    for (int n = 0; n < kDotPieces; ++n) {
-      if (n + 1 < kDotPieces) {
-        read_piece<T, DP, 4>(x[(n + 1) & 1], q_tile, 0, 4 * n + 4, at_lane);
-      } else if constexpr (Plan::kValuesInLds) {
-        read_piece<T, DP, 2>(x[(n + 1) & 1], g_tile, 0, 0, at_lane);
-        read_piece<T, DP, 2, 2>(x[(n + 1) & 1], values, wave * kWaveRows, 0, at_lane);
+    for (int b = 0; b < kRows / 32; ++b) {
+      // Four fragments are read while four are in use.
+      f32x16 dots = {}, dp = {};
+      Piece<T> x[2];
+      constexpr int kPieces = (kSteps + 3) / 4;  // of a row's fragments
+      read_piece<T, DP, 4>(x[0], q_tile, 32 * b, 0, at_lane);
+#pragma unroll
+      for (int n = 0; n < (kDk ? 2 : 1) * kPieces; ++n) {
+        Piece<T> &now = x[n & 1], &next = x[(n + 1) & 1];
+        const int s0 = n % kPieces * 4, s1 = (n + 1) % kPieces * 4;
+        if (n + 1 < kPieces)
+          read_piece<T, DP, 4>(next, q_tile, 32 * b, s1, at_lane);
+        else if (kDk && n + 1 < 2 * kPieces)
+          read_piece<T, DP, 4>(next, g_tile, 32 * b, s1, at_lane);
+        pin_reads();
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (s0 + i < kSteps) {
+            if (n < kPieces)
+              dots = Mat<T>::mma(now[i], k[s0 + i], dots);
+            else
+              dp = Mat<T>::mma(now[i], v[s0 + i], dp);
+          }
+        pin_reads();
+      }
+      float p[16], ds[16];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        // L and D of four rows
+        const f32x4 s01 = *reinterpret_cast<const f32x4 *>(stat_row + 64 * b + 16 * i + 8 * h);
+        const f32x4 s23 = *reinterpret_cast<const f32x4 *>(stat_row + 64 * b + 16 * i + 8 * h + 4);
+        const float l[4] = {s01[0], s01[2], s23[0], s23[2]};
+        const float d[4] = {s01[1], s01[3], s23[1], s23[3]};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int r = 4 * i + j;
+          p[r] = exp2_fast(fmaf(dots[r], A.scale_log2, -l[j]));
+          ds[r] = kDk ? p[r] * (dp[r] - d[j]) : 0.f;
+          if (masked) {
+            const int at = r0 + 32 * b + c_row(r, h);
+            if (at < from || at >= rows) p[r] = ds[r] = 0.f;
+          }
+        }
+      }
+      Weights<T> w, u;
+      if constexpr (kDv) w.set(p);
+      if constexpr (kDk) u.set(ds);
+      if constexpr (sizeof(T) == 4) {
+        Columns<T, DP> g, q;
+        g.read(g_tile, 32 * b);
+        q.read(q_tile, 32 * b);
+        if constexpr (kDv) g.add(dv, w, at_lane);
+        if constexpr (kDk) q.add(dk, u, at_lane);
       } else {
-        read_piece<T, DP, 4>(x[(n + 1) & 1], g_tile, 0, 0, at_lane);
-      }
-      pin_reads();
+        constexpr int kHalves = (kBlocks + 1) / 2;  // pieces of 64 columns
+        constexpr int kFirst = kDv ? 0 : kHalves, kLast = kDk ? 2 * kHalves : kHalves;
+        pin_reads();
+        read_column_piece<T, DP>(x[0], kDv ? g_tile : q_tile, 32 * b, 0, at_lane);
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (4 * n + i < kSteps) dots = Mat<T>::mma(x[n & 1][i], k[4 * n + i], dots);
-      pin_reads();
-    }
-    constexpr int kPer = Plan::kValuesInLds ? 2 : 4;
-    constexpr int kGradPieces = (kSteps + kPer - 1) / kPer;
-#pragma unroll
-    for (int n = 0; n < kGradPieces; ++n) {
-      Piece<T> &now = x[(kDotPieces + n) & 1], &next = x[(kDotPieces + n + 1) & 1];
-      if (n + 1 < kGradPieces) {
-        if constexpr (Plan::kValuesInLds) {
-          read_piece<T, DP, 2>(next, g_tile, 0, 2 * n + 2, at_lane);
-          read_piece<T, DP, 2, 2>(next, values, wave * kWaveRows, 2 * n + 2, at_lane);
-        } else {
-          read_piece<T, DP, 4>(next, g_tile, 0, 4 * n + 4, at_lane);
-        }
-      }
-      pin_reads();
-#pragma unroll
-      for (int i = 0; i < kPer; ++i)
-        if (kPer * n + i < kSteps) {
-          if constexpr (Plan::kValuesInLds)
-            dp = Mat<T>::mma(now[i], now[2 + i], dp);
+        for (int n = kFirst; n < kLast; ++n) {
+          Piece<T> &now = x[(n - kFirst) & 1], &next = x[(n - kFirst + 1) & 1];
+          if (n + 1 < kLast)
+            read_column_piece<T, DP>(next, n + 1 < kHalves ? g_tile : q_tile, 32 * b,
+                                     2 * ((n + 1) % kHalves), at_lane);
+          pin_reads();
+          if (n < kHalves)
+            add_column_piece<T, DP>(dv, now, w, 2 * n);
           else
-            dp = Mat<T>::mma(now[i], v[kPer * n + i], dp);
+            add_column_piece<T, DP>(dk, now, u, 2 * (n - kHalves));
+          pin_reads();
         }
-      pin_reads();
-    }
-    float p[16], ds[16];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      // L and D of four rows
-      const f32x4 s01 = *reinterpret_cast<const f32x4 *>(stat_row + 16 * i + 8 * h);
-      const f32x4 s23 = *reinterpret_cast<const f32x4 *>(stat_row + 16 * i + 8 * h + 4);
-      const float l[4] = {s01[0], s01[2], s23[0], s23[2]};
-      const float d[4] = {s01[1], s01[3], s23[1], s23[3]};
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int r = 4 * i + j;
-        p[r] = exp2_fast(fmaf(dots[r], A.scale_log2, -l[j]));
-        ds[r] = p[r] * (dp[r] - d[j]);
-        if (masked) {
-          const int at = r0 + c_row(r, h);
-          if (at < from || at >= rows) p[r] = ds[r] = 0.f;
-        }
-      }
-    }
-    Weights<T> w, u;
-    w.set(p);
-    u.set(ds);
-    if constexpr (sizeof(T) == 4) {
-      Columns<T, DP> g, q;
-      g.read(g_tile, 0);
-      q.read(q_tile, 0);
-      g.add(dv, w, at_lane);
-      q.add(dk, u, at_lane);
-    } else {
-      constexpr int kAt = kDotPieces + kGradPieces, kPieces = (kBlocks + 1) / 2;
-      pin_reads();
-      read_column_piece<T, DP>(x[kAt & 1], g_tile, 0, 0, at_lane);
-#pragma unroll
-      for (int n = 0; n < 2 * kPieces; ++n) {
-        Piece<T> &now = x[(kAt + n) & 1], &next = x[(kAt + n + 1) & 1];
-        if (n + 1 < 2 * kPieces)
-          read_column_piece<T, DP>(next, n + 1 < kPieces ? g_tile : q_tile, 0,
-                                   2 * ((n + 1) % kPieces), at_lane);
-        pin_reads();
-        if (n < kPieces)
-          add_column_piece<T, DP>(dv, now, w, 2 * n);
-        else
-          add_column_piece<T, DP>(dk, now, u, 2 * (n - kPieces));
-        pin_reads();
       }
     }
   }
 
-  if constexpr (kGroups > 1) {
-    // the second group hands its sums over, dk and then dv
-    float *sums = reinterpret_cast<float *>(lds) + wave * (kBlocks * 16 * 64) + lane;
+  if (n_splits > 1) {
+    float *put = splits.sums +
+                 ((int64_t(index) * A.k_heads + head) * splits.most + split) *
+                     (2 * kWaves * Plan::kSums * 64) +
+                 wave * Plan::kSums * 64 + lane;
 #pragma unroll
-    for (int n = 0; n < 2; ++n) {
-      Sums<T, DP> &mine = n == 0 ? dk : dv;
-      __syncthreads();
-      if (group_of == 1) {
+    for (int b = 0; b < kBlocks; ++b)
 #pragma unroll
-        for (int b = 0; b < kBlocks; ++b)
-#pragma unroll
-          for (int r = 0; r < 16; ++r) sums[(b * 16 + r) * 64] = mine[b][r];
+      for (int r = 0; r < 16; ++r) {
+        if constexpr (kDk) put[(b * 16 + r) * 64] = dk[b][r];
+        if constexpr (kDv) put[(kWaves * Plan::kSums + b * 16 + r) * 64] = dv[b][r];
       }
-      __syncthreads();
-      if (group_of == 0) {
-#pragma unroll
-        for (int b = 0; b < kBlocks; ++b)
-#pragma unroll
-          for (int r = 0; r < 16; ++r) mine[b][r] += sums[(b * 16 + r) * 64];
-      }
-    }
-    if (group_of == 1) return;
+    return;
   }
-  store_row<T, DP>(A.dk.at + k_row * A.dk.row + head * A.dk.head, dk, A.scale, A.dim, valid);
-  store_row<T, DP>(A.dv.at + k_row * A.dv.row + head * A.dv.head, dv, 1.f, A.dim, valid);
+  if constexpr (kDk)
+    store_row<T, DP>(A.dk.at + k_row * A.dk.row + head * A.dk.head, dk, A.scale, A.dim, valid);
+  if constexpr (kDv)
+    store_row<T, DP>(A.dv.at + k_row * A.dv.row + head * A.dv.head, dv, 1.f, A.dim, valid);
+}
+
+// Adds the sums of a key tile whose walk was cut, in the order of the cuts: a
+// wave for 32 keys' dk, and one for their dv.
+template <typename T, int DP>
+__global__ __launch_bounds__(64) void key_sum_kernel(BackwardArgs A, Splits splits) {
+  using Plan = KeyPlan<T, DP>;
+  const int n = blockIdx.x & 1, wave = (blockIdx.x >> 1) % kWaves;
+  const int head = blockIdx.x / (2 * kWaves) % A.k_heads;
+  const int index = blockIdx.x / (2 * kWaves) / A.k_heads;
+  KeyTile tile;
+  if (!key_tile_at(A, index, Plan::kRows, tile)) return;
+  const int n_splits = splits.of(tile.tiles);
+  if (n_splits == 1) return;
+  const int lane = lane_id();
+  const int key = tile.kb + wave * kWaveRows + (lane & 31);
+  const bool valid = key < tile.seq.nk;
+  const int64_t k_row = tile.seq.k0 + (valid ? key : tile.seq.nk - 1);
+  Sums<T, DP> sum = {};
+  const float *from =
+      splits.sums +
+      (int64_t(index) * A.k_heads + head) * splits.most * (2 * kWaves * Plan::kSums * 64) +
+      (n * kWaves + wave) * Plan::kSums * 64 + lane;
+  for (int i = 0; i < n_splits; ++i, from += 2 * kWaves * Plan::kSums * 64)
+#pragma unroll
+    for (int b = 0; b < Shape<T, DP>::kBlocks; ++b)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) sum[b][r] += from[(b * 16 + r) * 64];
+  const Operand &to = n == 0 ? A.dk : A.dv;
+  store_row<T, DP>(to.at + k_row * to.row + head * to.head, sum, n == 0 ? A.scale : 1.f, A.dim,
+                   valid);
+}
+
+// Cuts of the keys' kernel, from what the host knows.  Blocks of one wave
+// each of about 512 (two a CU) last as long as their longest walk, so there
+// are to be about 2048; a cut below 1024 rows would not pay for its sums.  The
+// steps are a block's share if the sequences are alike.
+Splits plan_splits(int64_t q_total, int64_t k_total, int group, int k_heads, int sequences,
+                   int causal, int tile_rows) {
+  Splits s = {1, 1 << 30, nullptr};
+  const int64_t tiles = k_total / (kWaves * kWaveRows) + sequences + 1;
+  const int64_t walk = q_total * group / tile_rows + 1;  // of one sequence of all
+  const int64_t most = (2048 + tiles * k_heads - 1) / (tiles * k_heads);
+  // (`most` decides the scratch, and so goes by the rows alone)
+  const int64_t limit = q_total * group / 1024;
+  s.most = int(most < limit ? most : limit);
+  if (s.most < 2) {
+    s.most = 1;
+    return s;
+  }
+  if (s.most > 16) s.most = 16;
+  const int64_t share =
+      walk * tiles * k_heads / (sequences > 0 ? sequences : 1) / 512 / (causal ? 2 : 1);
+  s.steps = int(share < 1024 / tile_rows ? 1024 / tile_rows : share > (1 << 20) ? (1 << 20) : share);
+  return s;
+}
+
+size_t split_bytes(const Splits &s, int64_t k_total, int k_heads, int sequences, int dim) {
+  if (s.most == 1) return 0;
+  const int64_t tiles = k_total / (kWaves * kWaveRows) + sequences + 1;
+  const int width = dim <= 32 ? 32 : dim <= 64 ? 64 : dim <= 96 ? 96 : 128;
+  return size_t(tiles) * k_heads * s.most * 2 * kWaves * 32 * width * sizeof(float);
 }
 
 template <typename T, int DP>
-int launch_backward(BackwardArgs &A, float2 *stats, hipStream_t s) {
+int launch_backward(BackwardArgs &A, float2 *stats, const Splits &splits, hipStream_t s) {
   constexpr int kLanes = sizeof(T) == 4 ? 32 : 16;
   constexpr int kKeys = sizeof(T) == 4 ? 32 : 64;
   constexpr int kLds = 4 * Shape<T, DP>::tile_bytes(kKeys);
@@ -440,14 +493,33 @@ int launch_backward(BackwardArgs &A, float2 *stats, hipStream_t s) {
   }
   if (A.k_total > 0) {
     A.tiles = A.k_total / (kWaves * kWaveRows) + A.sequences + 1;
-    using Plan = KeyPlan<T, DP>;
     const int64_t blocks = int64_t(A.tiles) * A.k_heads;
-    st = check_grid(blocks, Plan::kThreads, "attention key gradient");
+    st = check_grid(blocks * splits.most, kThreads, "attention key gradient");
     if (st) return st;
-    LaunchScope scope("attention_key_grad", s);
-    hipLaunchKernelGGL((key_grad_kernel<T, DP>), dim3(unsigned(blocks)), dim3(Plan::kThreads),
-                       Plan::kLds, s, A);
+    const dim3 grid(unsigned(blocks * splits.most));
+    constexpr int kKeyLds = KeyPlan<T, DP>::kLds;
+    if constexpr (KeyPlan<T, DP>::kApart) {
+      {
+        LaunchScope scope("attention_key_grad", s);
+        hipLaunchKernelGGL((key_grad_kernel<T, DP, true, false>), grid, dim3(kThreads), kKeyLds, s,
+                           A, splits);
+      }
+      LaunchScope scope("attention_value_grad", s);
+      hipLaunchKernelGGL((key_grad_kernel<T, DP, false, true>), grid, dim3(kThreads), kKeyLds, s,
+                         A, splits);
+    } else {
+      LaunchScope scope("attention_key_grad", s);
+      hipLaunchKernelGGL((key_grad_kernel<T, DP, true, true>), grid, dim3(kThreads), kKeyLds, s, A,
+                         splits);
+    }
     st = check_launch("attention key gradient");
+    if (st || splits.most == 1) return st;
+    st = check_grid(blocks * 2 * kWaves, 64, "attention key sums");
+    if (st) return st;
+    LaunchScope scope("attention_key_sum", s);
+    hipLaunchKernelGGL((key_sum_kernel<T, DP>), dim3(unsigned(blocks * 2 * kWaves)), dim3(64), 0, s,
+                       A, splits);
+    st = check_launch("attention key sums");
   }
   return st;
 }
@@ -456,9 +528,13 @@ int launch_backward(BackwardArgs &A, float2 *stats, hipStream_t s) {
 
 extern "C" {
 
-size_t bevpool_attention_backward_scratch_bytes(int64_t q_total, int32_t q_heads) {
-  if (q_total < 1 || q_heads < 1) return 0;
-  return size_t(q_total) * size_t(q_heads) * 2 * sizeof(float);
+size_t bevpool_attention_backward_scratch_bytes(int64_t q_total, int64_t k_total, int32_t q_heads,
+                                                int32_t k_heads, int32_t dim, int32_t sequences) {
+  if (q_total < 1 || q_heads < 1 || k_heads < 1 || k_total < 0 || sequences < 0) return 0;
+  const size_t stats = size_t(q_total) * size_t(q_heads) * sizeof(float2);
+  // (causal walks are cut as often or more)
+  const Splits s = plan_splits(q_total, k_total, q_heads / k_heads, k_heads, sequences, 1, 32);
+  return (stats + 255) / 256 * 256 + split_bytes(s, k_total, k_heads, sequences, dim);
 }
 
 int bevpool_attention_backward(const void *q, int64_t q_row, int64_t q_head, const void *k,
@@ -490,17 +566,22 @@ int bevpool_attention_backward(const void *q, int64_t q_row, int64_t q_head, con
   const int64_t heads = A.group.size < 64 ? A.group.size : 64;
   if (A.q.head * heads >= (1 << 30) || A.dout.head * heads >= (1 << 30))
     return fail(BEVPOOL_EINVAL, "q, dout: the heads of a group must lie within 2^30 bytes");
-  const size_t need = bevpool_attention_backward_scratch_bytes(q_total, q_heads);
+  const size_t need = bevpool_attention_backward_scratch_bytes(q_total, k_total, q_heads, k_heads,
+                                                               dim, sequences);
   if (scratch_bytes < need || (need > 0 && !scratch))
     return fail(BEVPOOL_ESPACE, "attention backward scratch: %zu bytes, %zu needed",
                 scratch_bytes, need);
   A.lse = const_cast<float *>(lse);
   float2 *stats = static_cast<float2 *>(scratch);
   A.stats = stats;
+  Splits splits =
+      plan_splits(q_total, k_total, A.group.size, k_heads, sequences, A.causal, elem == 4 ? 32 : 64);
+  const size_t stats_bytes = (size_t(q_total) * q_heads * sizeof(float2) + 255) / 256 * 256;
+  splits.sums = reinterpret_cast<float *>(static_cast<char *>(scratch) + stats_bytes);
   hipStream_t s = static_cast<hipStream_t>(stream);
-  return dtype == BEVPOOL_BF16  ? (ATTENTION_DIM(__bf16, launch_backward, A, stats, s))
-         : dtype == BEVPOOL_F16 ? (ATTENTION_DIM(_Float16, launch_backward, A, stats, s))
-                                : (ATTENTION_DIM(float, launch_backward, A, stats, s));
+  return dtype == BEVPOOL_BF16  ? (ATTENTION_DIM(__bf16, launch_backward, A, stats, splits, s))
+         : dtype == BEVPOOL_F16 ? (ATTENTION_DIM(_Float16, launch_backward, A, stats, splits, s))
+                                : (ATTENTION_DIM(float, launch_backward, A, stats, splits, s));
 }
 
 }  // extern "C"

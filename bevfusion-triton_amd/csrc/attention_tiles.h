@@ -383,19 +383,18 @@ struct Columns<float, DP> {
 };
 
 // Pieces of the above, four fragments at a time, for kernels that are short of
-// registers: rows' fragments s0 .. s0 + kN - 1 into f[kAt ..], and column
-// blocks b0, b0 + 1.
+// registers: rows' fragments s0 .. s0 + kN - 1, and column blocks b0, b0 + 1.
 template <typename T>
 using Piece = typename Mat<T>::Frag[4];
 
-template <typename T, int DP, int kN, int kAt = 0>
+template <typename T, int DP, int kN>
 __device__ __forceinline__ void read_piece(Piece<T> &f, const char *tile, int r0, int s0,
                                            int lane) {
   const int c = lane & 31, h = lane >> 5;
 #pragma unroll
   for (int i = 0; i < kN; ++i)
     if (s0 + i < Shape<T, DP>::kSteps)
-      f[kAt + i] = *reinterpret_cast<const typename Mat<T>::Frag *>(
+      f[i] = *reinterpret_cast<const typename Mat<T>::Frag *>(
           tile + (r0 + c) * (Shape<T, DP>::kPitch * 16) +
           ((2 * (s0 + i) + h) ^ swizzle<T, DP>(c)) * 16);
 }

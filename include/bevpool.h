@@ -600,9 +600,10 @@ int bevpool_attention_forward(const void *q, int64_t q_row, int64_t q_head, cons
  * dk and dv (k_total, k_heads, dim), contiguous, every row written (zeros for
  * queries that see no key and keys that no query sees).  dout has strides of
  * its own, out is contiguous.  No atomics: the same call gives the same bits.
- *   scratch   >= bevpool_attention_backward_scratch_bytes(q_total, q_heads)
+ *   scratch   >= bevpool_attention_backward_scratch_bytes(...)
  */
-size_t bevpool_attention_backward_scratch_bytes(int64_t q_total, int32_t q_heads);
+size_t bevpool_attention_backward_scratch_bytes(int64_t q_total, int64_t k_total, int32_t q_heads,
+                                                int32_t k_heads, int32_t dim, int32_t sequences);
 
 int bevpool_attention_backward(const void *q, int64_t q_row, int64_t q_head, const void *k,
                                int64_t k_row, int64_t k_head, const void *v, int64_t v_row,
