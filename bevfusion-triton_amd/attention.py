@@ -69,33 +69,47 @@ def _strides(x):
 
 
 def _run(call, device, what):
-    with torch.cuda.device(device):
-        L.check(call(L.library(), L.stream_handle(device)), what)
+    """call(library, stream) on the device's current stream.  (Where the device
+    is current already, as it mostly is, without the context manager.)"""
+    if device.index == torch._C._cuda_getDevice():
+        status = call(L.library(), torch._C._cuda_getCurrentRawStream(device.index))
+    else:
+        with torch.cuda.device(device):
+            status = call(L.library(), L.stream_handle(device))
+    L.check(status, what)
+
+
+def _wants_grad(*tensors):
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
 
 
 # ---- norm and rotation -----------------------------------------------------
 
+def _norm_rotate(q, k, q_weight, k_weight, positions, frequencies, pairs, eps, interleaved):
+    tokens, q_heads, dim = q.shape
+    k_heads = k.shape[1] if k is not None else 0
+    q_out = torch.empty((tokens, q_heads, dim), dtype=q.dtype, device=q.device)
+    k_out = None if k is None else torch.empty((tokens, k_heads, dim), dtype=q.dtype,
+                                               device=q.device)
+    _run(lambda lib, s: lib.bevpool_norm_rotate_forward(
+        *_strides(q), q_heads, *_strides(k), k_heads, L.DTYPE_CODES[q.dtype], tokens, dim,
+        *_rotation(positions, frequencies, pairs, interleaved), L.ptr(q_weight), L.ptr(k_weight),
+        eps, L.ptr(q_out), L.ptr(k_out), s), q.device, 'bevpool_norm_rotate_forward')
+    return q_out, k_out
+
+
 class _NormRotate(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, q_weight, k_weight, positions, frequencies, pairs, eps, interleaved):
-        q = _unit(q)
-        k = _unit(k) if k is not None else None
         tokens, q_heads, dim = q.shape
         k_heads = k.shape[1] if k is not None else 0
-        q_out = torch.empty((tokens, q_heads, dim), dtype=q.dtype, device=q.device)
-        k_out = None if k is None else torch.empty((tokens, k_heads, dim), dtype=q.dtype,
-                                                   device=q.device)
         ctx.call = (tokens, q_heads, k_heads, dim, q.dtype, pairs, eps, interleaved)
         # (a rotation alone needs no input for its gradient)
         ctx.save_for_backward(q if q_weight is not None else None,
                               k if k_weight is not None else None, q_weight, k_weight, positions,
                               frequencies)
-        _run(lambda lib, s: lib.bevpool_norm_rotate_forward(
-            *_strides(q), q_heads, *_strides(k), k_heads, L.DTYPE_CODES[q.dtype], tokens, dim,
-            *_rotation(positions, frequencies, pairs, interleaved), L.ptr(q_weight),
-            L.ptr(k_weight), eps, L.ptr(q_out), L.ptr(k_out), s), q.device,
-            'bevpool_norm_rotate_forward')
-        return q_out, k_out
+        return _norm_rotate(q, k, q_weight, k_weight, positions, frequencies, pairs, eps,
+                            interleaved)
 
     @staticmethod
     def backward(ctx, dq_out, dk_out):
@@ -185,8 +199,9 @@ def norm_rotate(q, k, positions, frequencies, pairs=None, *, q_weight=None, k_we
         if t.device != q.device:
             raise ValueError(f'{name} must be on the device of q ({q.device}).')
     weights = [w if w is None else w.contiguous() for w in (q_weight, k_weight)]
-    return _NormRotate.apply(q, k, *weights, _unit(positions), frequencies.contiguous(), pairs,
-                             float(eps), bool(interleaved))
+    run = _NormRotate.apply if _wants_grad(q, k, *weights) else _norm_rotate
+    return run(_unit(q), _unit(k) if k is not None else None, *weights, _unit(positions),
+               frequencies.contiguous(), pairs, float(eps), bool(interleaved))
 
 
 # ---- attention over packed sequences ---------------------------------------
@@ -234,18 +249,21 @@ def _check_starts(name, starts, like):
     return starts.to(torch.int32).contiguous()
 
 
+def _attend_packed(q, k, v, q_starts, k_starts, causal, scale):
+    out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    lse = torch.empty(q.shape[:2], dtype=torch.float32, device=q.device)
+    _run(lambda lib, s: lib.bevpool_attention_forward(
+        *_strides(q), *_strides(k), *_strides(v), L.DTYPE_CODES[q.dtype], q.shape[0], k.shape[0],
+        q.shape[1], k.shape[1], q.shape[2], L.ptr(q_starts), L.ptr(k_starts),
+        q_starts.shape[0] - 1, int(causal), scale, L.ptr(out), L.ptr(lse), s), q.device,
+        'bevpool_attention_forward')
+    return out, lse
+
+
 class _AttendPacked(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, q_starts, k_starts, causal, scale):
-        group = q.shape[1] // k.shape[1]
-        q, k, v = _aligned(q, group), _aligned(k), _aligned(v)
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        lse = torch.empty(q.shape[:2], dtype=torch.float32, device=q.device)
-        _run(lambda lib, s: lib.bevpool_attention_forward(
-            *_strides(q), *_strides(k), *_strides(v), L.DTYPE_CODES[q.dtype], q.shape[0],
-            k.shape[0], q.shape[1], k.shape[1], q.shape[2], L.ptr(q_starts), L.ptr(k_starts),
-            q_starts.shape[0] - 1, int(causal), scale, L.ptr(out), L.ptr(lse), s), q.device,
-            'bevpool_attention_forward')
+        out, lse = _attend_packed(q, k, v, q_starts, k_starts, causal, scale)
         ctx.save_for_backward(q, k, v, out, lse, q_starts, k_starts)
         ctx.call = (causal, scale)
         ctx.mark_non_differentiable(lse)
@@ -298,7 +316,9 @@ def attend_packed(q, k, v, q_starts, k_starts=None, *, causal=False, scale=None,
         k_starts = _check_starts('k_starts', k_starts, q)
     if k_starts.shape != q_starts.shape:
         raise ValueError('q_starts and k_starts must have the same length.')
-    out, lse = _AttendPacked.apply(q, k, v, q_starts, k_starts, bool(causal), scale)
+    run = _AttendPacked.apply if _wants_grad(q, k, v) else _attend_packed
+    out, lse = run(_aligned(q, q.shape[1] // k.shape[1]), _aligned(k), _aligned(v), q_starts,
+                   k_starts, bool(causal), scale)
     return (out, lse) if return_lse else out
 
 
@@ -356,9 +376,8 @@ def attend_cached(q, k, v, lengths, prefix_k=None, prefix_v=None, *, scale=None)
     P.require_gpu(q, k, v, lengths)
     if lengths.device != q.device:
         raise ValueError(f'lengths must be on the device of q ({q.device}).')
-    for t in (q, k, v, prefix_k, prefix_v):
-        if t is not None and t.requires_grad and torch.is_grad_enabled():
-            raise RuntimeError('attend_cached has no gradient; call it under torch.no_grad()')
+    if _wants_grad(q, k, v, prefix_k, prefix_v):
+        raise RuntimeError('attend_cached has no gradient; call it under torch.no_grad()')
     rows = _aligned(q.reshape(requests * tokens, q_heads, dim))
     lengths = lengths.to(torch.int32).contiguous()
     prefix = prefix_k.shape[0] if prefix_k is not None else 0

@@ -54,15 +54,28 @@ __device__ __forceinline__ int length_of(const CachedArgs &A, int request) {
 // Rows of one request and key head (token, head of the group), 32 of them a
 // block, against one range of its keys.  The waves take 32 keys each in
 // turn, every wave with buffers of its own and no barrier in the loop; their
-// sums are joined at the end.  kBuffers 2: the next keys' loads are in flight
-// while 32 are used.  kFinal: the only part, written as the result.
-template <typename T, int DP, int kBuffers, bool kFinal>
-__global__ __launch_bounds__(kThreads, 1) void cached_part_kernel(CachedArgs A) {
+// sums are joined at the end.  kFinal: the only part, written as the result.
+//
+// LDS for two blocks a CU: where a wave's two buffers of 32 keys fit half of
+// it (rows of up to 128 bytes), the next keys' loads are in flight while 32
+// are used; longer rows have one buffer, and the CU's other block loads
+// meanwhile.
+template <typename T, int DP>
+struct PartPlan {
+  static constexpr int kTile = Shape<T, DP>::tile_bytes(32);
+  static constexpr int kBuffers = kTile > 4096 ? 1 : 2;
+  static constexpr int kOut = DP + 4;  // floats of a row of sums (4: other banks for the next)
+  // a wave's: K0 V0 K1 V1, and its sums at the end
+  static constexpr int kMine =
+      kBuffers * 2 * kTile > 128 * kOut ? kBuffers * 2 * kTile : 128 * kOut;
+  static constexpr int kLds = kWaves * kMine + kWaves * 32 * 8;
+  static_assert(kLds <= 160 * 1024, "LDS of a CU");
+};
+template <typename T, int DP, bool kFinal>
+__device__ __forceinline__ void cached_part(const CachedArgs &A, char *lds, int at) {
   using S = Shape<T, DP>;
-  extern __shared__ __attribute__((aligned(16))) char lds[];
-  constexpr int kTile = S::tile_bytes(32);
-  constexpr int kMine = kBuffers * 2 * kTile;  // a wave's: K0 V0 K1 V1
-  int at = blockIdx.x;
+  constexpr int kTile = PartPlan<T, DP>::kTile, kBuffers = PartPlan<T, DP>::kBuffers;
+  constexpr int kMine = PartPlan<T, DP>::kMine;
   const int part = at % A.parts;
   at /= A.parts;
   const int head = at % A.k_heads;
@@ -136,8 +149,7 @@ __global__ __launch_bounds__(kThreads, 1) void cached_part_kernel(CachedArgs A) 
   }
 
   // Join the waves: outputs as rows of floats over each wave's buffers.
-  constexpr int kOut = DP + 4;  // floats of a row (4: other banks for the next)
-  static_assert(32 * kOut * 4 <= kMine, "a wave's sums fit its buffers");
+  constexpr int kOut = PartPlan<T, DP>::kOut;
   float2 *tops = reinterpret_cast<float2 *>(lds + kWaves * kMine);
   const float sum = sum_halves(x.sum);
   if (h == 0) tops[wave * 32 + c] = make_float2(x.top * A.scale_log2, sum);
@@ -191,10 +203,7 @@ __global__ __launch_bounds__(kThreads, 1) void cached_part_kernel(CachedArgs A) 
 // Rows of all requests (128 a block, 32 a wave) against one range of the
 // prefix, as in attention over a packed sequence.
 template <typename T, int DP, int kKeys>
-__global__ __launch_bounds__(kThreads, sizeof(T) == 4 && DP > 64 ? 1 : 2) void prefix_part_kernel(
-    CachedArgs A) {
-  extern __shared__ __attribute__((aligned(16))) char lds[];
-  int at = blockIdx.x;
+__device__ __forceinline__ void prefix_part(const CachedArgs &A, char *lds, int at) {
   const int head = at % A.k_heads;
   at /= A.k_heads;
   const int tile = at % A.row_tiles, part = at / A.row_tiles;
@@ -230,35 +239,64 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 4 && DP > 64 ? 1 : 2) void p
     }
 }
 
-// Joins the parts of a row: a wave a row, two neighbouring elements a lane.
-// `shared` parts are every row's, the rest as many as the request's length
-// has ranges.
+// All parts of a call in one launch: the prefix' are bound by the matrix
+// instructions where many rows share it, the own caches' by memory, and side
+// by side on a CU they hide each other.  The blocks of the one are spread
+// evenly among those of the other.
+template <typename T, int DP, bool kByRows, bool kFinal>
+__global__ __launch_bounds__(kThreads, DP * sizeof(T) > 256 ? 1 : 2) void parts_kernel(
+    CachedArgs own, CachedArgs shared, int shared_blocks) {
+  extern __shared__ __attribute__((aligned(16))) char lds[];
+  const int64_t i = blockIdx.x, n = gridDim.x;
+  const int before = int(i * shared_blocks / n);
+  if (int((i + 1) * shared_blocks / n) == before) {
+    cached_part<T, DP, kFinal>(own, lds, int(i) - before);
+  } else if constexpr (kByRows) {
+    prefix_part<T, DP, sizeof(T) == 4 ? 32 : 64>(shared, lds, before);
+  } else if constexpr (!kFinal) {
+    cached_part<T, DP, false>(shared, lds, before);
+  }
+}
+
+// Joins the parts of a row, a block a row: a wave takes every fourth part, two
+// neighbouring elements a lane.  `shared` parts are every row's, the rest as
+// many as the request's length has ranges.
 template <typename T>
 __global__ __launch_bounds__(kThreads) void join_kernel(CachedArgs A, int shared) {
-  const int64_t row = int64_t(blockIdx.x) * kWaves + wave_id();
-  if (row >= A.rows) return;
-  const int lane = lane_id();
+  __shared__ float2 sums[kWaves][64];
+  __shared__ float totals[kWaves];
+  const int64_t row = blockIdx.x;
+  const int lane = lane_id(), wave = wave_id();
   const int token = int(row / A.q_heads);
   const int parts = shared + (length_of(A, token / A.tokens) + A.range - 1) / A.range;
   float top = -kInf;
   for (int p = lane; p < parts; p += 64) top = fmaxf(top, A.part_top[p * A.rows + row].x);
 #pragma unroll
   for (int m = 1; m < 64; m <<= 1) top = fmaxf(top, __shfl_xor(top, m, 64));
+  const int d = 2 * lane < A.dim ? 2 * lane : A.dim - 2;  // (the lanes past dim read along)
   float total = 0.f, a = 0.f, b = 0.f;
-  const int d = 2 * lane;
-  for (int p = 0; p < parts; ++p) {
+#pragma unroll 8
+  for (int p = wave; p < parts; p += kWaves) {
     const float2 t = A.part_top[p * A.rows + row];
+    const float2 v =
+        *reinterpret_cast<const float2 *>(A.part_out + (p * A.rows + row) * A.dim + d);
     const float by = t.x == -kInf ? 0.f : exp2_fast(t.x - top);
     total += by * t.y;
-    if (d < A.dim) {
-      const float2 v =
-          *reinterpret_cast<const float2 *>(A.part_out + (p * A.rows + row) * A.dim + d);
-      a += by * v.x;
-      b += by * v.y;
-    }
+    a += by * v.x;
+    b += by * v.y;
+  }
+  sums[wave][lane] = make_float2(a, b);
+  if (lane == 0) totals[wave] = total;
+  __syncthreads();
+  if (wave > 0) return;
+#pragma unroll
+  for (int w = 1; w < kWaves; ++w) {
+    total += totals[w];
+    a += sums[w][lane].x;
+    b += sums[w][lane].y;
   }
   const float norm = total > 0.f || total != total ? 1.f / total : 0.f;
-  if (d < A.dim) {
+  if (2 * lane < A.dim) {
     typedef T Pair __attribute__((ext_vector_type(2)));
     *reinterpret_cast<Pair *>(A.out.at + token * A.out.row +
                               (row - int64_t(token) * A.q_heads) * A.out.head + d * sizeof(T)) =
@@ -270,17 +308,18 @@ __global__ __launch_bounds__(kThreads) void join_kernel(CachedArgs A, int shared
 // host side
 // ---------------------------------------------------------------------------
 
-// Keys of a part: a multiple of 128 (what a block takes at once) such that
-// `blocks` row tiles and heads times the parts come to about `target` blocks.
-int range_for(int64_t blocks, int keys, int64_t target) {
-  const int64_t range = (blocks * keys / target + 127) / 128 * 128;
-  return int(range < 128 ? 128 : range);
+// Keys of a part: the least multiple of `step` such that `blocks` row tiles
+// and heads times the parts are no more than `target` blocks.
+int range_for(int64_t blocks, int keys, int64_t target, int step) {
+  const int64_t parts = target / blocks > 1 ? target / blocks : 1;
+  const int64_t range = ((keys + parts - 1) / parts + step - 1) / step * step;
+  return int(range < step ? step : range);
 }
 
 struct CachedPlan {
   int own_range, own_parts, own_tiles;
   int shared_range, shared_parts, shared_tiles;
-  bool by_rows;  // the prefix by prefix_part_kernel
+  bool by_rows;  // the prefix by prefix_part
   bool final;    // one part: no join
 };
 
@@ -289,13 +328,23 @@ CachedPlan plan_cached(int requests, int tokens, int capacity, int prefix, int q
   CachedPlan p = {};
   const int64_t group = q_heads / k_heads;
   p.own_tiles = int((tokens * group + 31) / 32);
-  p.own_range = range_for(int64_t(requests) * k_heads * p.own_tiles, capacity, 2048);
+  // About 4096 blocks even out caches of different lengths (24 requests of up
+  // to 16,384 keys: 93 us, at 1024 blocks 101), but a part below 512 keys
+  // costs more than it evens out (64 requests of up to 1,024 keys: 62 us at
+  // 512, 73 at 256), unless the card would not be full.
+  const int64_t own_blocks = int64_t(requests) * k_heads * p.own_tiles;
+  p.own_range = own_blocks > 0 ? range_for(own_blocks, capacity, 4096, 128) : 128;
+  if (p.own_range < 512) {
+    const int full = own_blocks > 0 ? range_for(own_blocks, capacity, 512, 128) : 128;
+    if (p.own_range < full) p.own_range = full < 512 ? full : 512;
+  }
   p.own_parts = (capacity + p.own_range - 1) / p.own_range;
   if (prefix > 0) {
     const int64_t rows = requests * tokens * group;
     p.by_rows = rows > 64;
     p.shared_tiles = int(p.by_rows ? (rows + 127) / 128 : (rows + 31) / 32);
-    p.shared_range = range_for(int64_t(k_heads) * p.shared_tiles, prefix, 512);
+    p.shared_range = range_for(int64_t(k_heads) * p.shared_tiles, prefix, p.by_rows ? 256 : 512,
+                               p.by_rows ? 64 : 128);
     p.shared_parts = (prefix + p.shared_range - 1) / p.shared_range;
   }
   p.final = p.shared_parts == 0 && p.own_parts <= 1;
@@ -303,50 +352,36 @@ CachedPlan plan_cached(int requests, int tokens, int capacity, int prefix, int q
 }
 
 template <typename T, int DP>
-int launch_parts(const CachedArgs &A, bool final, const char *name, hipStream_t s) {
-  const int64_t blocks = int64_t(A.requests) * A.row_tiles * A.k_heads * A.parts;
-  if (blocks == 0) return BEVPOOL_OK;
-  const int st = check_grid(blocks, kThreads, name);
-  if (st) return st;
-  constexpr int kBuffers = Shape<T, DP>::tile_bytes(32) > 8192 ? 1 : 2;
-  constexpr int kLds = kWaves * kBuffers * 2 * Shape<T, DP>::tile_bytes(32) + kWaves * 32 * 8;
-  static_assert(kLds <= 160 * 1024, "LDS of a CU");
-  LaunchScope scope(name, s);
-  if (final)
-    hipLaunchKernelGGL((cached_part_kernel<T, DP, kBuffers, true>), dim3(unsigned(blocks)),
-                       dim3(kThreads), kLds, s, A);
-  else
-    hipLaunchKernelGGL((cached_part_kernel<T, DP, kBuffers, false>), dim3(unsigned(blocks)),
-                       dim3(kThreads), kLds, s, A);
-  return check_launch(name);
-}
-
-template <typename T, int DP>
 int launch_cached(const CachedArgs &own, const CachedArgs &shared, const CachedPlan &p,
                   hipStream_t s) {
-  int st = BEVPOOL_OK;
-  if (p.shared_parts > 0) {
-    if (p.by_rows) {
-      constexpr int kKeys = sizeof(T) == 4 ? 32 : 64;
-      const int64_t blocks = int64_t(shared.row_tiles) * shared.k_heads * shared.parts;
-      st = check_grid(blocks, kThreads, "attention prefix");
-      if (st) return st;
-      LaunchScope scope("attention_prefix", s);
-      hipLaunchKernelGGL((prefix_part_kernel<T, DP, kKeys>), dim3(unsigned(blocks)),
-                         dim3(kThreads), 4 * (Shape<T, DP>::tile_bytes(kKeys)), s, shared);
-      st = check_launch("attention prefix");
-    } else {
-      st = launch_parts<T, DP>(shared, false, "attention_prefix", s);
-    }
-    if (st) return st;
+  const int64_t shared_blocks =
+      p.shared_parts > 0 ? int64_t(shared.row_tiles) * shared.k_heads * shared.parts : 0;
+  const int64_t blocks =
+      shared_blocks + int64_t(own.requests) * own.row_tiles * own.k_heads * own.parts;
+  int st = check_grid(blocks, kThreads, "attention parts");
+  if (st) return st;
+  constexpr int kPrefixLds = 4 * Shape<T, DP>::tile_bytes(sizeof(T) == 4 ? 32 : 64);
+  constexpr int kOwnLds = PartPlan<T, DP>::kLds;
+  constexpr int kBothLds = kPrefixLds > kOwnLds ? kPrefixLds : kOwnLds;
+  if (blocks > 0) {
+    LaunchScope scope("attention_parts", s);
+    const dim3 grid{unsigned(blocks)}, block{kThreads};
+    if (p.final)
+      hipLaunchKernelGGL((parts_kernel<T, DP, false, true>), grid, block, kOwnLds, s, own, shared,
+                         0);
+    else if (p.by_rows)
+      hipLaunchKernelGGL((parts_kernel<T, DP, true, false>), grid, block, kBothLds, s, own, shared,
+                         int(shared_blocks));
+    else
+      hipLaunchKernelGGL((parts_kernel<T, DP, false, false>), grid, block, kOwnLds, s, own,
+                         shared, int(shared_blocks));
   }
-  st = launch_parts<T, DP>(own, p.final, "attention_cached", s);
+  st = check_launch("attention parts");
   if (st || p.final) return st;
-  const int64_t blocks = (own.rows + kWaves - 1) / kWaves;
-  st = check_grid(blocks, kThreads, "attention join");
+  st = check_grid(own.rows, kThreads, "attention join");
   if (st) return st;
   LaunchScope scope("attention_join", s);
-  hipLaunchKernelGGL((join_kernel<T>), dim3(unsigned(blocks)), dim3(kThreads), 0, s, own,
+  hipLaunchKernelGGL((join_kernel<T>), dim3(unsigned(own.rows)), dim3(kThreads), 0, s, own,
                      p.shared_parts);
   return check_launch("attention join");
 }

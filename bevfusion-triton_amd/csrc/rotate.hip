@@ -72,10 +72,33 @@ __device__ __forceinline__ void store(T *to, const float (&from)[V]) {
   *reinterpret_cast<Pack<T, V> *>(to) = p;
 }
 
-// Sum over groups of `lanes` (a power of two) consecutive lanes.
+// Where a thread stands: rows are worked on by groups of `lanes` consecutive
+// lanes of a wave, as many as fit it; the lanes left over have a group past
+// all rows and a lane past all units.
+struct Place {
+  int lane, group, groups;
+};
+__device__ __forceinline__ Place place_of(int lanes) {
+  const int in_wave = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int per_wave = 64 / lanes, g = in_wave / lanes;
+  if (g >= per_wave) return {1 << 20, 1 << 30, 1 << 30};
+  return {in_wave - g * lanes, wave * per_wave + g, per_wave * (kThreads / 64)};
+}
+
+// Sum over a group's lanes, in all of them.
 __device__ __forceinline__ float group_sum(float v, int lanes) {
-  for (int m = 1; m < lanes; m <<= 1) v += __shfl_xor(v, m, 64);
-  return v;
+  if ((lanes & (lanes - 1)) == 0) {
+    for (int m = 1; m < lanes; m <<= 1) v += __shfl_xor(v, m, 64);
+    return v;
+  }
+  // lane i collects the lanes i .. i + 2 m - 1 that there are; the first has
+  // all in the end
+  const int in_wave = threadIdx.x & 63, first = in_wave / lanes * lanes, lane = in_wave - first;
+  for (int m = 1; m < lanes; m <<= 1) {
+    const float other = __shfl(v, in_wave + m, 64);
+    if (lane + m < lanes) v += other;
+  }
+  return __shfl(v, first, 64);
 }
 
 // cos and sin of pos * frequency.  The product in double (an angle of 10^5
@@ -157,7 +180,8 @@ __global__ __launch_bounds__(kThreads) void norm_rotate_kernel(RotateArgs A, int
     cs[i] = turn(A, t0 + t, i - t * A.pairs);
   }
   __syncthreads();
-  const int lane = threadIdx.x % lanes, group = threadIdx.x / lanes, groups = kThreads / lanes;
+  const Place place = place_of(lanes);
+  const int lane = place.lane, group = place.group, groups = place.groups;
   const int heads = A.q.heads + A.k.heads;
   // group-uniform: the lanes of one sum leave the loop together
   for (int row = group; row < n_tokens * heads; row += groups) {
@@ -203,41 +227,68 @@ __global__ __launch_bounds__(kThreads) void norm_rotate_kernel(RotateArgs A, int
   }
 }
 
+// One row's elements of this lane, as they lie in memory.
+template <typename T, int V, int kUnits>
+struct RowData {
+  Pack<T, V> xa[kUnits], xb[kUnits], ga[kUnits], gb[kUnits];
+};
+
 // Backward of one operand's rows of a tile; dwa, dwb collect this lane's part
-// of the weight's gradient (a lane keeps its units over all its rows).
+// of the weight's gradient (a lane keeps its units over all its rows, and
+// their weights wa, wb).  The next row's loads are in flight while one is
+// worked on.
 template <typename T, int V, int kUnits>
 __device__ __forceinline__ void backward_rows(const RotateArgs &A, const Heads &X, int64_t t0,
                                               int n_tokens, int lanes, const float2 *cs,
+                                              const Pack<T, V> (&wa)[kUnits],
+                                              const Pack<T, V> (&wb)[kUnits],
                                               float (&dwa)[kUnits][V], float (&dwb)[kUnits][V]) {
-  const int lane = threadIdx.x % lanes, group = threadIdx.x / lanes, groups = kThreads / lanes;
-  const T *w = static_cast<const T *>(X.weight);
-  for (int row = group; row < n_tokens * X.heads; row += groups) {
+  const Place place = place_of(lanes);
+  const int lane = place.lane, group = place.group, groups = place.groups;
+  const bool w = X.weight != nullptr;
+  const int rows = n_tokens * X.heads;
+  auto fetch = [&](int row, RowData<T, V, kUnits> &d) {
     const int t = row / X.heads, head = row - t * X.heads;
     const T *x = static_cast<const T *>(X.x) + (t0 + t) * X.x_token + head * X.x_head;
     const T *dy = static_cast<const T *>(X.dy) + (t0 + t) * X.dy_token + head * X.dy_head;
-    T *dx = static_cast<T *>(X.y) + (t0 + t) * X.y_token + head * X.y_head;
-    float a[kUnits][V], b[kUnits][V], ga[kUnits][V], gb[kUnits][V];
-    float sum = 0.f, dot = 0.f;
 #pragma unroll
     for (int j = 0; j < kUnits; ++j) {
       const int u = lane + j * lanes;
       if (u >= A.units) continue;
       const Unit at = unit_at<V>(A, u);
-      load<T, V>(ga[j], dy + at.a);
-      load<T, V>(gb[j], dy + at.b);
+      d.ga[j] = *reinterpret_cast<const Pack<T, V> *>(dy + at.a);
+      d.gb[j] = *reinterpret_cast<const Pack<T, V> *>(dy + at.b);
       if (w) {
-        load<T, V>(a[j], x + at.a);
-        load<T, V>(b[j], x + at.b);
+        d.xa[j] = *reinterpret_cast<const Pack<T, V> *>(x + at.a);
+        d.xb[j] = *reinterpret_cast<const Pack<T, V> *>(x + at.b);
       }
-      turn_unit<V>(ga[j], gb[j], cs + t * A.pairs, A, at, true);
+    }
+  };
+  RowData<T, V, kUnits> next;
+  if (group < rows) fetch(group, next);
+  for (int row = group; row < rows; row += groups) {
+    const RowData<T, V, kUnits> d = next;
+    if (row + groups < rows) fetch(row + groups, next);
+    const int t = row / X.heads, head = row - t * X.heads;
+    T *dx = static_cast<T *>(X.y) + (t0 + t) * X.y_token + head * X.y_head;
+    float ga[kUnits][V], gb[kUnits][V];
+    float sum = 0.f, dot = 0.f;
+#pragma unroll
+    for (int j = 0; j < kUnits; ++j) {
+      const int u = lane + j * lanes;
+      if (u >= A.units) continue;
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        ga[j][i] = float(d.ga[j].v[i]);
+        gb[j][i] = float(d.gb[j].v[i]);
+      }
+      turn_unit<V>(ga[j], gb[j], cs + t * A.pairs, A, unit_at<V>(A, u), true);
       if (w) {
-        float wa[V], wb[V];
-        load<T, V>(wa, w + at.a);
-        load<T, V>(wb, w + at.b);
 #pragma unroll
         for (int i = 0; i < V; ++i) {
-          sum += a[j][i] * a[j][i] + b[j][i] * b[j][i];
-          dot += ga[j][i] * wa[i] * a[j][i] + gb[j][i] * wb[i] * b[j][i];
+          const float a = float(d.xa[j].v[i]), b = float(d.xb[j].v[i]);
+          sum += a * a + b * b;
+          dot += ga[j][i] * float(wa[j].v[i]) * a + gb[j][i] * float(wb[j].v[i]) * b;
         }
       }
     }
@@ -252,15 +303,13 @@ __device__ __forceinline__ void backward_rows(const RotateArgs &A, const Heads &
       if (u >= A.units) continue;
       const Unit at = unit_at<V>(A, u);
       if (w) {
-        float wa[V], wb[V];
-        load<T, V>(wa, w + at.a);
-        load<T, V>(wb, w + at.b);
 #pragma unroll
         for (int i = 0; i < V; ++i) {
-          dwa[j][i] += ga[j][i] * (a[j][i] * r);
-          dwb[j][i] += gb[j][i] * (b[j][i] * r);
-          ga[j][i] = r * (ga[j][i] * wa[i] - a[j][i] * back);
-          gb[j][i] = r * (gb[j][i] * wb[i] - b[j][i] * back);
+          const float a = float(d.xa[j].v[i]), b = float(d.xb[j].v[i]);
+          dwa[j][i] += ga[j][i] * (a * r);
+          dwb[j][i] += gb[j][i] * (b * r);
+          ga[j][i] = r * (ga[j][i] * float(wa[j].v[i]) - a * back);
+          gb[j][i] = r * (gb[j][i] * float(wb[j].v[i]) - b * back);
         }
       }
       store<T, V>(dx + at.a, ga[j]);
@@ -269,15 +318,31 @@ __device__ __forceinline__ void backward_rows(const RotateArgs &A, const Heads &
   }
 }
 
+// This lane's weights.
+template <typename T, int V, int kUnits>
+__device__ __forceinline__ void load_weights(const RotateArgs &A, const Heads &X, int lanes,
+                                             Pack<T, V> (&wa)[kUnits], Pack<T, V> (&wb)[kUnits]) {
+  const T *w = static_cast<const T *>(X.weight);
+  const int lane = place_of(lanes).lane;
+#pragma unroll
+  for (int j = 0; j < kUnits; ++j) {
+    const int u = lane + j * lanes;
+    if (!w || u >= A.units) continue;
+    const Unit at = unit_at<V>(A, u);
+    wa[j] = *reinterpret_cast<const Pack<T, V> *>(w + at.a);
+    wb[j] = *reinterpret_cast<const Pack<T, V> *>(w + at.b);
+  }
+}
+
 // The groups' parts of a weight's gradient, added in the groups' order.
 template <int V, int kUnits>
-__device__ __forceinline__ void flush_weight(const RotateArgs &A, const Heads &X, int lanes,
-                                             float *sums, const float (&dwa)[kUnits][V],
+__device__ __forceinline__ void flush_weight(const RotateArgs &A, const Heads &X, int block,
+                                             int lanes, float *sums, const float (&dwa)[kUnits][V],
                                              const float (&dwb)[kUnits][V]) {
-  if (!X.weight || X.heads == 0) return;
-  const int lane = threadIdx.x % lanes, group = threadIdx.x / lanes, groups = kThreads / lanes;
-  __syncthreads();
-  for (int i = threadIdx.x; i < groups * A.dim; i += kThreads) sums[i] = 0.f;
+  if (!X.weight) return;
+  const Place place = place_of(lanes);
+  const int lane = place.lane, group = place.group;
+  const int all = 64 / lanes * (kThreads / 64);
   __syncthreads();
 #pragma unroll
   for (int j = 0; j < kUnits; ++j) {
@@ -293,33 +358,38 @@ __device__ __forceinline__ void flush_weight(const RotateArgs &A, const Heads &X
   __syncthreads();
   for (int d = threadIdx.x; d < A.dim; d += kThreads) {
     float s = 0.f;
-    for (int g = 0; g < groups; ++g) s += sums[g * A.dim + d];
-    X.partial[int64_t(blockIdx.x) * A.dim + d] = s;
+    for (int g = 0; g < all; ++g) s += sums[g * A.dim + d];
+    X.partial[int64_t(block) * A.dim + d] = s;
   }
 }
 
-// As the forward, but a block walks tiles (grid stride), so that the weight's
-// gradient leaves it once.
+// As the forward, but a block walks an equal share of one operand's tokens, so
+// that its weight's gradient leaves it once, and holds one weight and one
+// gradient of it: in 128 registers, four blocks a CU.
 template <typename T, int V, int kUnits>
-__global__ __launch_bounds__(kThreads) void norm_rotate_backward_kernel(RotateArgs A, int tile,
-                                                                        int lanes) {
+__global__ __launch_bounds__(kThreads, (kUnits == 1 ? 4 : 2)) void norm_rotate_backward_kernel(
+    RotateArgs A, int tile, int lanes, int q_blocks) {
   extern __shared__ float2 cs[];
-  float dqa[kUnits][V] = {}, dqb[kUnits][V] = {}, dka[kUnits][V] = {}, dkb[kUnits][V] = {};
-  for (int64_t t0 = int64_t(blockIdx.x) * tile; t0 < A.tokens;
-       t0 += int64_t(gridDim.x) * tile) {
-    const int n_tokens = int(A.tokens - t0 < tile ? A.tokens - t0 : tile);
+  const bool is_q = int(blockIdx.x) < q_blocks;
+  const Heads &X = is_q ? A.q : A.k;
+  const int block = is_q ? blockIdx.x : blockIdx.x - q_blocks;
+  const int blocks = is_q ? q_blocks : gridDim.x - q_blocks;
+  float dwa[kUnits][V] = {}, dwb[kUnits][V] = {};
+  Pack<T, V> wa[kUnits], wb[kUnits];
+  load_weights<T, V, kUnits>(A, X, lanes, wa, wb);
+  const int64_t share = (A.tokens + blocks - 1) / blocks;
+  const int64_t end = A.tokens < (block + 1) * share ? A.tokens : (block + 1) * share;
+  for (int64_t t0 = block * share; t0 < end; t0 += tile) {
+    const int n_tokens = int(end - t0 < tile ? end - t0 : tile);
     __syncthreads();  // the last tile's angles have been read
     for (int i = threadIdx.x; i < n_tokens * A.pairs; i += kThreads) {
       const int t = i / A.pairs;
       cs[i] = turn(A, t0 + t, i - t * A.pairs);
     }
     __syncthreads();
-    backward_rows<T, V, kUnits>(A, A.q, t0, n_tokens, lanes, cs, dqa, dqb);
-    backward_rows<T, V, kUnits>(A, A.k, t0, n_tokens, lanes, cs, dka, dkb);
+    backward_rows<T, V, kUnits>(A, X, t0, n_tokens, lanes, cs, wa, wb, dwa, dwb);
   }
-  float *sums = reinterpret_cast<float *>(cs);
-  flush_weight<V, kUnits>(A, A.q, lanes, sums, dqa, dqb);
-  flush_weight<V, kUnits>(A, A.k, lanes, sums, dka, dkb);
+  flush_weight<V, kUnits>(A, X, block, lanes, reinterpret_cast<float *>(cs), dwa, dwb);
 }
 
 // Column sums of the blocks' parts: a wave an element, lanes along the
@@ -327,11 +397,12 @@ __global__ __launch_bounds__(kThreads) void norm_rotate_backward_kernel(RotateAr
 template <typename T>
 __global__ __launch_bounds__(64) void weight_sum_kernel(const float *q_partial, T *dq_weight,
                                                         const float *k_partial, T *dk_weight,
-                                                        int blocks, int dim) {
+                                                        int q_blocks, int k_blocks, int dim) {
   const bool is_q = int(blockIdx.x) < dim;
   const int d = is_q ? blockIdx.x : blockIdx.x - dim;
   const float *from = is_q ? q_partial : k_partial;
   T *to = is_q ? dq_weight : dk_weight;
+  const int blocks = is_q ? q_blocks : k_blocks;
   if (!to) return;
   float s = 0.f;
   for (int b = threadIdx.x; b < blocks; b += 64) s += from[int64_t(b) * dim + d];
@@ -361,8 +432,12 @@ Plan plan_for(int elem, int dim, int pairs, int interleaved, int heads,
       break;
   }
   p.units = dim / (2 * p.vec);
+  // A power of two, whose sums take fewer steps, unless that leaves a fifth of
+  // the lanes without a unit (5 units of a head of 80 on 8 lanes: backward of
+  // 16,896 x 32 rows 76 us, on 5 lanes 64).
   p.lanes = 1;
   while (p.lanes < p.units && p.lanes < 64) p.lanes *= 2;
+  if (p.units * 5 < p.lanes * 4) p.lanes = p.units;
   // enough rows for four rounds of the block's groups, at most 16 tokens,
   // and no fewer blocks than CUs
   p.tile = 1;
@@ -419,11 +494,18 @@ int fill_args(RotateArgs &A, int dtype, int64_t tokens, int dim, const void *pos
   return BEVPOOL_OK;
 }
 
-// Blocks of the backward: as many as the card holds at once (256 CUs, 4
-// each), or as there are tiles.
-int64_t backward_blocks(int64_t tokens, const Plan &p) {
-  const int64_t tiles = (tokens + p.tile - 1) / p.tile;
-  return tiles < 1024 ? tiles : 1024;
+// Blocks of the backward, of both operands by their heads: as many as the card
+// holds at once (256 CUs, 4 each), or as there are tiles.
+constexpr int kBackwardBlocks = 1024;
+void backward_blocks(int64_t tokens, const Plan &p, int q_heads, int k_heads, int *q_blocks,
+                     int *k_blocks) {
+  const int64_t tiles = (tokens + p.tile - 1) / p.tile, heads = q_heads + k_heads;
+  auto share = [&](int64_t n) {
+    const int64_t part = heads > 0 ? (kBackwardBlocks * n + heads - 1) / heads : 0;
+    return int(tiles < part ? tiles : part);
+  };
+  *q_blocks = share(q_heads);
+  *k_blocks = share(k_heads);
 }
 
 template <typename T, int V>
@@ -439,17 +521,19 @@ void launch_forward(const RotateArgs &A, const Plan &p, unsigned grid, hipStream
 }
 
 template <typename T, int V>
-void launch_backward(const RotateArgs &A, const Plan &p, unsigned grid, hipStream_t s) {
+void launch_backward(const RotateArgs &A, const Plan &p, int q_blocks, int k_blocks,
+                     hipStream_t s) {
+  const unsigned grid = q_blocks + k_blocks;
   const size_t angles = sizeof(float2) * size_t(p.tile) * A.pairs;
   const size_t sums = sizeof(float) * size_t(kThreads / p.lanes) * A.dim;
   const size_t lds = angles > sums ? angles : sums;
   const int per_lane = (A.units + p.lanes - 1) / p.lanes;
   if (per_lane == 1)
     hipLaunchKernelGGL((norm_rotate_backward_kernel<T, V, 1>), dim3(grid), dim3(kThreads), lds, s,
-                       A, p.tile, p.lanes);
+                       A, p.tile, p.lanes, q_blocks);
   else
     hipLaunchKernelGGL((norm_rotate_backward_kernel<T, V, 2>), dim3(grid), dim3(kThreads), lds, s,
-                       A, p.tile, p.lanes);
+                       A, p.tile, p.lanes, q_blocks);
 }
 
 #define ROTATE_VEC(T, FN, ...)                       \
@@ -508,7 +592,7 @@ int bevpool_norm_rotate_forward(const void *q, int64_t q_token, int64_t q_head, 
 }
 
 size_t bevpool_norm_rotate_backward_scratch_bytes(int32_t dim) {
-  return dim < 1 ? 0 : size_t(2) * 1024 * size_t(dim) * sizeof(float);
+  return dim < 1 ? 0 : size_t(2) * kBackwardBlocks * size_t(dim) * sizeof(float);
 }
 
 int bevpool_norm_rotate_backward(
@@ -538,34 +622,40 @@ int bevpool_norm_rotate_backward(
   float *parts = static_cast<float *>(scratch);
   A.q = {q, dq_out, dq, q_weight, parts, q_token, q_head, dq_token, dq_head, q_heads * d, d,
          q_heads};
-  A.k = {k, dk_out, dk, k_weight, parts + (q_weight || k_weight ? 1024 * d : 0), k_token, k_head,
+  A.k = {k, dk_out, dk, k_weight, parts + (q_weight || k_weight ? kBackwardBlocks * d : 0), k_token, k_head,
          dk_token, dk_head, k_heads * d, d, k_heads};
-  const Plan p = plan_for(dtype == BEVPOOL_F32 ? 4 : 2, dim, A.pairs, A.interleaved,
-                          heads > 0 ? heads : 1, tokens);
+  Plan p = plan_for(dtype == BEVPOOL_F32 ? 4 : 2, dim, A.pairs, A.interleaved,
+                    heads > 0 ? heads : 1, tokens);
+  // (a block walks tiles here, and each begins with two barriers: up to 16
+  // tokens while that leaves the blocks a tile each)
+  while (p.tile < 16 && tokens >= p.tile * 2 * int64_t(kBackwardBlocks) / 2) p.tile *= 2;
   A.units = p.units;
-  const int64_t grid = heads > 0 ? backward_blocks(tokens, p) : 0;
+  int q_blocks, k_blocks;
+  backward_blocks(tokens, p, q_heads, k_heads, &q_blocks, &k_blocks);
   hipStream_t s = static_cast<hipStream_t>(stream);
-  if (grid > 0) {
+  if (q_blocks + k_blocks > 0) {
     LaunchScope scope("norm_rotate_backward", s);
-    ROTATE_TYPE(launch_backward, A, p, unsigned(grid), s)
+    ROTATE_TYPE(launch_backward, A, p, q_blocks, k_blocks, s)
     st = check_launch("norm_rotate_backward");
     if (st) return st;
   }
   if (!q_weight && !k_weight) return BEVPOOL_OK;
   // (no tokens: the sums of nothing, zeros)
   void *wq = q_weight ? dq_weight : nullptr, *wk = k_weight ? dk_weight : nullptr;
-  const int blocks = int(grid);
   LaunchScope scope("norm_rotate_weight_sum", s);
   const float *pk = A.k.partial;
   if (dtype == BEVPOOL_F32)
     hipLaunchKernelGGL((weight_sum_kernel<float>), dim3(2 * dim), dim3(64), 0, s, parts,
-                       static_cast<float *>(wq), pk, static_cast<float *>(wk), blocks, dim);
+                       static_cast<float *>(wq), pk, static_cast<float *>(wk), q_blocks, k_blocks,
+                       dim);
   else if (dtype == BEVPOOL_F16)
     hipLaunchKernelGGL((weight_sum_kernel<_Float16>), dim3(2 * dim), dim3(64), 0, s, parts,
-                       static_cast<_Float16 *>(wq), pk, static_cast<_Float16 *>(wk), blocks, dim);
+                       static_cast<_Float16 *>(wq), pk, static_cast<_Float16 *>(wk), q_blocks,
+                       k_blocks, dim);
   else
     hipLaunchKernelGGL((weight_sum_kernel<__bf16>), dim3(2 * dim), dim3(64), 0, s, parts,
-                       static_cast<__bf16 *>(wq), pk, static_cast<__bf16 *>(wk), blocks, dim);
+                       static_cast<__bf16 *>(wq), pk, static_cast<__bf16 *>(wk), q_blocks,
+                       k_blocks, dim);
   return check_launch("norm_rotate_weight_sum");
 }
 
