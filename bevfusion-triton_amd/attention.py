@@ -249,13 +249,13 @@ def _check_starts(name, starts, like):
     return starts.to(torch.int32).contiguous()
 
 
-def _attend_packed(q, k, v, q_starts, k_starts, causal, scale):
+def _attend_packed(q, k, v, q_starts, k_starts, causal, scale, rest=None):
     out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
     lse = torch.empty(q.shape[:2], dtype=torch.float32, device=q.device)
     _run(lambda lib, s: lib.bevpool_attention_forward(
         *_strides(q), *_strides(k), *_strides(v), L.DTYPE_CODES[q.dtype], q.shape[0], k.shape[0],
         q.shape[1], k.shape[1], q.shape[2], L.ptr(q_starts), L.ptr(k_starts),
-        q_starts.shape[0] - 1, int(causal), scale, L.ptr(out), L.ptr(lse), s), q.device,
+        q_starts.shape[0] - 1, int(causal), scale, L.ptr(out), L.ptr(rest), L.ptr(lse), s), q.device,
         'bevpool_attention_forward')
     return out, lse
 
@@ -263,15 +263,18 @@ def _attend_packed(q, k, v, q_starts, k_starts, causal, scale):
 class _AttendPacked(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, q_starts, k_starts, causal, scale):
-        out, lse = _attend_packed(q, k, v, q_starts, k_starts, causal, scale)
-        ctx.save_for_backward(q, k, v, out, lse, q_starts, k_starts)
+        # (16-bit types: the output's rounding, for the gradients)
+        rest = torch.empty_like(q, memory_format=torch.contiguous_format) \
+            if q.element_size() == 2 else None
+        out, lse = _attend_packed(q, k, v, q_starts, k_starts, causal, scale, rest)
+        ctx.save_for_backward(q, k, v, out, rest, lse, q_starts, k_starts)
         ctx.call = (causal, scale)
         ctx.mark_non_differentiable(lse)
         return out, lse
 
     @staticmethod
     def backward(ctx, dout, _):
-        q, k, v, out, lse, q_starts, k_starts = ctx.saved_tensors
+        q, k, v, out, rest, lse, q_starts, k_starts = ctx.saved_tensors
         causal, scale = ctx.call
         dout = _aligned(dout.to(q.dtype), q.shape[1] // k.shape[1])
         dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
@@ -279,7 +282,7 @@ class _AttendPacked(torch.autograd.Function):
             q.shape[0], k.shape[0], q.shape[1], k.shape[1], q.shape[2], q_starts.shape[0] - 1)
         scratch = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
         _run(lambda lib, s: lib.bevpool_attention_backward(
-            *_strides(q), *_strides(k), *_strides(v), L.ptr(out), *_strides(dout), L.ptr(lse),
+            *_strides(q), *_strides(k), *_strides(v), L.ptr(out), L.ptr(rest), *_strides(dout), L.ptr(lse),
             L.DTYPE_CODES[q.dtype], q.shape[0], k.shape[0], q.shape[1], k.shape[1], q.shape[2],
             L.ptr(q_starts), L.ptr(k_starts), q_starts.shape[0] - 1, int(causal), scale, L.ptr(dq),
             L.ptr(dk), L.ptr(dv), L.ptr(scratch), nbytes, s), q.device,

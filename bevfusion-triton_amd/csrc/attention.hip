@@ -67,8 +67,12 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 4 && DP > 64 ? 1 : 2) void p
 
   const float sum = sum_halves(x.sum);
   const bool any = x.top > -kInf || sum != 0.f;
-  store_row<T, DP>(A.out.at + token * A.out.row + q_head * A.out.head, out,
-                   any ? 1.f / sum : 0.f, A.dim, valid);
+  const float by = any ? 1.f / sum : 0.f;
+  const int64_t at = token * A.out.row + q_head * A.out.head;
+  if (sizeof(T) == 2 && A.rest)
+    store_row<T, DP, true>(A.out.at + at, out, by, A.dim, valid, A.rest + at);
+  else
+    store_row<T, DP>(A.out.at + at, out, by, A.dim, valid);
   if (valid && h == 0 && A.lse)
     A.lse[token * A.q_heads + q_head] =
         any ? (x.top * A.scale_log2 + __builtin_amdgcn_logf(sum)) / kLog2e : -kInf;
@@ -154,7 +158,8 @@ int bevpool_attention_forward(const void *q, int64_t q_row, int64_t q_head, cons
                               int64_t v_head, int32_t dtype, int64_t q_total, int64_t k_total,
                               int32_t q_heads, int32_t k_heads, int32_t dim,
                               const int32_t *q_starts, const int32_t *k_starts, int32_t sequences,
-                              int32_t causal, float scale, void *out, float *lse, void *stream) {
+                              int32_t causal, float scale, void *out, void *out_rest, float *lse,
+                              void *stream) {
   bevpool_host::clear_error();
   PackedArgs A = {};
   const int elem = dtype == BEVPOOL_F32 ? 4 : 2;
@@ -165,8 +170,11 @@ int bevpool_attention_forward(const void *q, int64_t q_row, int64_t q_head, cons
   if (!st) st = set_operand(A.v, "v", v, v_row, v_head, elem, k_total);
   if (!st) st = set_operand(A.out, "out", out, int64_t(q_heads) * dim, dim, elem, q_total);
   if (st) return st;
+  if (reinterpret_cast<uintptr_t>(out_rest) % 16)
+    return fail(BEVPOOL_EINVAL, "out_rest must start at a multiple of 16 bytes");
   if (q_total == 0) return BEVPOOL_OK;
   A.lse = lse;
+  A.rest = static_cast<char *>(out_rest);
   A.tiles = int(q_total * A.group.size / (kWaves * kWaveRows)) + sequences + 1;
   hipStream_t s = static_cast<hipStream_t>(stream);
   return dtype == BEVPOOL_BF16  ? (ATTENTION_DIM(__bf16, launch_forward, A, s))

@@ -28,7 +28,9 @@ struct BackwardArgs : PackedArgs {
 };
 
 // D and L / log 2 of every (token, head): a row's 16-byte chunks on kLanes
-// lanes.
+// lanes.  D is a small difference of what dS subtracts it from where a row
+// sees few keys, so it is formed from the output before its rounding (out and
+// its rest): with out alone the error of dq and dk grew by a fifth.
 template <typename T, int kLanes>
 __global__ __launch_bounds__(kThreads) void stats_kernel(PackedArgs A, float2 *stats) {
   constexpr int kPer = 16 / sizeof(T);
@@ -45,6 +47,12 @@ __global__ __launch_bounds__(kThreads) void stats_kernel(PackedArgs A, float2 *s
                                                      head * A.dout.head + chunk * 16);
 #pragma unroll
     for (int i = 0; i < kPer; ++i) sum += float(o[i]) * float(g[i]);
+    if (sizeof(T) == 2 && A.rest) {
+      const Chunk r = *reinterpret_cast<const Chunk *>(A.rest + token * A.out.row +
+                                                       head * A.out.head + chunk * 16);
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) sum += float(r[i]) * float(g[i]);
+    }
   }
 #pragma unroll
   for (int m = 1; m < kLanes; m <<= 1) sum += __shfl_xor(sum, m, 64);
@@ -539,7 +547,7 @@ size_t bevpool_attention_backward_scratch_bytes(int64_t q_total, int64_t k_total
 
 int bevpool_attention_backward(const void *q, int64_t q_row, int64_t q_head, const void *k,
                                int64_t k_row, int64_t k_head, const void *v, int64_t v_row,
-                               int64_t v_head, const void *out, const void *dout,
+                               int64_t v_head, const void *out, const void *out_rest, const void *dout,
                                int64_t dout_row, int64_t dout_head, const float *lse,
                                int32_t dtype, int64_t q_total, int64_t k_total, int32_t q_heads,
                                int32_t k_heads, int32_t dim, const int32_t *q_starts,
@@ -571,6 +579,9 @@ int bevpool_attention_backward(const void *q, int64_t q_row, int64_t q_head, con
   if (scratch_bytes < need || (need > 0 && !scratch))
     return fail(BEVPOOL_ESPACE, "attention backward scratch: %zu bytes, %zu needed",
                 scratch_bytes, need);
+  if (reinterpret_cast<uintptr_t>(out_rest) % 16)
+    return fail(BEVPOOL_EINVAL, "out_rest must start at a multiple of 16 bytes");
+  A.rest = static_cast<char *>(const_cast<void *>(out_rest));
   A.lse = const_cast<float *>(lse);
   float2 *stats = static_cast<float2 *>(scratch);
   A.stats = stats;

@@ -539,13 +539,14 @@ __device__ __forceinline__ void attend_tiles(char *lds, const Frags<T, DP> &q, c
   }
 }
 
-// Writes a lane's column of acc times `by`, rounded to T once, as a row.
-template <typename T, int DP>
-__device__ __forceinline__ void store_row(char *row, const Sums<T, DP> &acc, float by,
-                                          int dim, bool valid) {
+// Writes a lane's column of acc times `by`, rounded to T once, as a row; with
+// kRest what the rounding took off, rounded to T itself, to another.
+template <typename T, int DP, bool kRest = false>
+__device__ __forceinline__ void store_row(char *row, const Sums<T, DP> &acc, float by, int dim,
+                                          bool valid, char *rest = nullptr) {
   const int h = lane_id() >> 5;
 #pragma unroll
-  for (int b = 0; b < (DP + 31) / 32; ++b) {
+  for (int b = 0; b < Shape<T, DP>::kBlocks; ++b) {
     if constexpr (sizeof(T) == 4) {
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
@@ -560,19 +561,28 @@ __device__ __forceinline__ void store_row(char *row, const Sums<T, DP> &acc, flo
 #pragma unroll
       for (int p = 0; p < 2; ++p) {
         typedef T Pair __attribute__((ext_vector_type(2)));
-        unsigned x[2], y[2];
+        float v[8];
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          x[i] = __builtin_bit_cast(unsigned, Pair{T(acc[b][8 * p + 2 * i] * by),
-                                                   T(acc[b][8 * p + 2 * i + 1] * by)});
-          y[i] = __builtin_bit_cast(unsigned, Pair{T(acc[b][8 * p + 4 + 2 * i] * by),
-                                                   T(acc[b][8 * p + 5 + 2 * i] * by)});
-        }
-        const auto a = __builtin_amdgcn_permlane32_swap(x[0], y[0], false, false);
-        const auto c = __builtin_amdgcn_permlane32_swap(x[1], y[1], false, false);
+        for (int i = 0; i < 8; ++i) v[i] = acc[b][8 * p + i] * by;
         const int d = 32 * b + 16 * p + 8 * h;
-        if (valid && d < dim)
-          *reinterpret_cast<u32x4 *>(row + d * 2) = u32x4{a[0], c[0], a[1], c[1]};
+#pragma unroll
+        for (int n = 0; n < (kRest ? 2 : 1); ++n) {
+          unsigned x[4];  // v[0..1], v[2..3], v[4..5], v[6..7]
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const Pair pair{T(v[2 * i]), T(v[2 * i + 1])};
+            x[i] = __builtin_bit_cast(unsigned, pair);
+            if (kRest) {
+              v[2 * i] -= float(pair[0]);
+              v[2 * i + 1] -= float(pair[1]);
+            }
+          }
+          const auto a = __builtin_amdgcn_permlane32_swap(x[0], x[2], false, false);
+          const auto c = __builtin_amdgcn_permlane32_swap(x[1], x[3], false, false);
+          if (valid && d < dim)
+            *reinterpret_cast<u32x4 *>((n == 0 ? row : rest) + d * 2) =
+                u32x4{a[0], c[0], a[1], c[1]};
+        }
       }
     }
   }
@@ -657,6 +667,7 @@ struct Operand {  // (rows, heads, dim), unit stride along dim; strides in bytes
 
 struct PackedArgs {
   Operand q, k, v, out, dout, dq, dk, dv;
+  char *rest;          // as out: what out's rounding took off, or null
   float *lse;          // (tokens, heads): log of the sum of exponentials
   const int32_t *q_starts, *k_starts;  // sequences + 1
   int sequences, q_total, k_total;

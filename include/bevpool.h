@@ -585,6 +585,8 @@ int bevpool_norm_rotate_backward(
  *   q_starts, k_starts   device int32 [sequences + 1], ascending from 0
  *                (values are clamped to the rows there are)
  *   out          (q_total, q_heads, dim) contiguous
+ *   out_rest     as out: what rounding took off out, rounded itself (fp32:
+ *                not written), for the gradients; or NULL
  *   lse          (q_total, q_heads) fp32, log of the sum of exponentials,
  *                or NULL
  */
@@ -593,10 +595,12 @@ int bevpool_attention_forward(const void *q, int64_t q_row, int64_t q_head, cons
                               int64_t v_head, int32_t dtype, int64_t q_total, int64_t k_total,
                               int32_t q_heads, int32_t k_heads, int32_t dim,
                               const int32_t *q_starts, const int32_t *k_starts, int32_t sequences,
-                              int32_t causal, float scale, void *out, float *lse, void *stream);
+                              int32_t causal, float scale, void *out, void *out_rest, float *lse,
+                              void *stream);
 
 /*
- * Its gradients, from the forward's out and lse: dq (q_total, q_heads, dim),
+ * Its gradients, from the forward's out, out_rest (or NULL: dq and dk are a
+ * little less exact) and lse: dq (q_total, q_heads, dim),
  * dk and dv (k_total, k_heads, dim), contiguous, every row written (zeros for
  * queries that see no key and keys that no query sees).  dout has strides of
  * its own, out is contiguous.  No atomics: the same call gives the same bits.
@@ -607,7 +611,7 @@ size_t bevpool_attention_backward_scratch_bytes(int64_t q_total, int64_t k_total
 
 int bevpool_attention_backward(const void *q, int64_t q_row, int64_t q_head, const void *k,
                                int64_t k_row, int64_t k_head, const void *v, int64_t v_row,
-                               int64_t v_head, const void *out, const void *dout,
+                               int64_t v_head, const void *out, const void *out_rest, const void *dout,
                                int64_t dout_row, int64_t dout_head, const float *lse,
                                int32_t dtype, int64_t q_total, int64_t k_total, int32_t q_heads,
                                int32_t k_heads, int32_t dim, const int32_t *q_starts,

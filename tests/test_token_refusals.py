@@ -35,10 +35,10 @@ def test_attention(pkg):
     lib = pkg.library()
 
     def forward(dtype=2, q_total=4, k_total=4, q_heads=4, k_heads=2, dim=64, scale=0.125, q=16,
-                row=256, starts=16):
+                row=256, starts=16, rest=None):
         return lib.bevpool_attention_forward(q, row, dim, 16, 128, dim, 16, 128, dim, dtype,
                                              q_total, k_total, q_heads, k_heads, dim, starts,
-                                             starts, 1, 0, scale, 16, None, None)
+                                             starts, 1, 0, scale, 16, rest, None, None)
 
     for bad, text in ((dict(dtype=3), b'dtype'), (dict(q_total=-1), b'negative'),
                       (dict(q_heads=3), b'no multiple'), (dict(k_heads=0), b'no multiple'),
@@ -46,10 +46,10 @@ def test_attention(pkg):
                       (dict(scale=-1.0), b'scale'), (dict(scale=float('nan')), b'scale'),
                       (dict(q_total=1 << 30), b'too many'), (dict(k_total=1 << 30), b'too many'),
                       (dict(q=None), b'q: null'), (dict(q=8), b'16 bytes'),
-                      (dict(row=255), b'16 bytes'), (dict(starts=None), b'null starts')):
+                      (dict(row=255), b'16 bytes'), (dict(rest=8), b'out_rest'), (dict(starts=None), b'null starts')):
         assert forward(**bad) == -1, bad
         assert text in lib.bevpool_last_error(), bad
-    args = (16, 256, 64, 16, 128, 64, 16, 128, 64, 16, 16, 256, 64, 16, 2, 4, 4, 4, 2, 64, 16, 16,
+    args = (16, 256, 64, 16, 128, 64, 16, 128, 64, 16, 16, 16, 256, 64, 16, 2, 4, 4, 4, 2, 64, 16, 16,
             1, 0, 0.125, 16, 16, 16)
     assert lib.bevpool_attention_backward_scratch_bytes(4, 4, 4, 2, 64, 1) == 256
     assert lib.bevpool_attention_backward(*args, None, 0, None) == -3
