@@ -24,42 +24,25 @@ using bevpool_host::fail;
 using bevpool_host::LaunchScope;
 
 struct BackwardArgs : PackedArgs {
-  const float2 *stats;  // (tokens, heads): L in units of log 2, and D
+  float2 *stats;  // (tokens, heads): L in units of log 2, and D
 };
 
-// D and L / log 2 of every (token, head): a row's 16-byte chunks on kLanes
-// lanes.  D is a small difference of what dS subtracts it from where a row
-// sees few keys, so it is formed from the output before its rounding (out and
-// its rest): with out alone the error of dq and dk grew by a fifth.
-template <typename T, int kLanes>
-__global__ __launch_bounds__(kThreads) void stats_kernel(PackedArgs A, float2 *stats) {
-  constexpr int kPer = 16 / sizeof(T);
-  const int64_t row = int64_t(blockIdx.x) * (kThreads / kLanes) + threadIdx.x / kLanes;
-  const int chunk = threadIdx.x % kLanes;
-  if (row >= int64_t(A.q_total) * A.q_heads) return;
-  const int64_t token = row / A.q_heads, head = row - token * A.q_heads;
+// A lane's part of the dot product of two rows.
+template <typename T, int DP>
+__device__ __forceinline__ float row_dot(const Frags<T, DP> &a, const Frags<T, DP> &b) {
   float sum = 0.f;
-  if (chunk < A.chunks) {
-    typedef T Chunk __attribute__((ext_vector_type(16 / sizeof(T))));
-    const Chunk o = *reinterpret_cast<const Chunk *>(A.out.at + token * A.out.row +
-                                                     head * A.out.head + chunk * 16);
-    const Chunk g = *reinterpret_cast<const Chunk *>(A.dout.at + token * A.dout.row +
-                                                     head * A.dout.head + chunk * 16);
 #pragma unroll
-    for (int i = 0; i < kPer; ++i) sum += float(o[i]) * float(g[i]);
-    if (sizeof(T) == 2 && A.rest) {
-      const Chunk r = *reinterpret_cast<const Chunk *>(A.rest + token * A.out.row +
-                                                       head * A.out.head + chunk * 16);
+  for (int s = 0; s < Shape<T, DP>::kSteps; ++s)
 #pragma unroll
-      for (int i = 0; i < kPer; ++i) sum += float(r[i]) * float(g[i]);
-    }
-  }
-#pragma unroll
-  for (int m = 1; m < kLanes; m <<= 1) sum += __shfl_xor(sum, m, 64);
-  if (chunk == 0) stats[row] = make_float2(A.lse[row] * kLog2e, sum);
+    for (int i = 0; i < int(16 / sizeof(T)); ++i) sum = fmaf(float(a[s][i]), float(b[s][i]), sum);
+  return sum;
 }
 
-// dq: rows and tiles as in the forward.
+// dq: rows and tiles as in the forward.  Also writes L / log 2 and D of its
+// rows, for the keys' kernels.  D is a small difference of what dS subtracts
+// it from where a row sees few keys, so it is formed from the output before
+// its rounding (out and its rest): with out alone the error of dq and dk grew
+// by a fifth.
 template <typename T, int DP, int kKeys>
 __global__ __launch_bounds__(kThreads, sizeof(T) == 4 && DP > 64 ? 1 : 2) void query_grad_kernel(
     BackwardArgs A) {
@@ -100,10 +83,22 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 4 && DP > 64 ? 1 : 2) void q
   Frags<T, DP> q, g;
   row_frags<T, DP>(q, A.q.at + token * A.q.row + q_head * A.q.head, A.chunks, true);
   row_frags<T, DP>(g, A.dout.at + token * A.dout.row + q_head * A.dout.head, A.chunks, true);
-  const float2 both = A.stats[token * A.q_heads + q_head];
-  float stat[2] = {both.x, both.y};
+  const int64_t stat_at = token * A.q_heads + q_head;
+  float stat[2] = {A.lse[stat_at] * kLog2e, 0.f};
+  {
+    const int64_t at = token * A.out.row + q_head * A.out.head;
+    Frags<T, DP> o;
+    row_frags<T, DP>(o, A.out.at + at, A.chunks, true);
+    stat[1] = row_dot<T, DP>(o, g);
+    if (sizeof(T) == 2 && A.rest) {
+      row_frags<T, DP>(o, A.rest + at, A.chunks, true);
+      stat[1] += row_dot<T, DP>(o, g);
+    }
+    stat[1] = sum_halves(stat[1]);
+  }
   settle(stat);
   const float lse2 = stat[0], delta = stat[1];
+  if (valid && h == 0) A.stats[stat_at] = make_float2(lse2, delta);
   const char *k_at = A.k.at + seq.k0 * A.k.row + head * A.k.head;
   const char *v_at = A.v.at + seq.k0 * A.v.row + head * A.v.head;
   const unsigned lds0 = lds_address(lds);
@@ -127,17 +122,37 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 4 && DP > 64 ? 1 : 2) void q
     const int k0 = t * kKeys;
     if (!wave_on || k0 >= high) continue;
     const bool masked = k0 + kKeys > low;
+    // (hides that the addresses of the reads are the same in every round: kept,
+    // they take more registers than there are)
+    int at_lane = lane;
+    if constexpr (DP * sizeof(T) > 192) asm volatile("" : "+v"(at_lane));
 #pragma unroll
     for (int b = 0; b < kKeys / 32; ++b) {
-      Frags<T, DP> k, v;
-      read_rows<T, DP>(k, k_tile, 32 * b);
-      read_rows<T, DP>(v, v_tile, 32 * b);
-      pin_reads();
-      const f32x16 dots = dot_rows<T, DP>(k, q);
-      const f32x16 dp = dot_rows<T, DP>(v, g);
-      Columns<T, DP> kt;
-      kt.read(k_tile, 32 * b);
-      pin_reads();
+      // Four fragments are read while four are in use.
+      constexpr int kSteps = S::kSteps, kPieces = (kSteps + 3) / 4;
+      constexpr int kHalves = (S::kBlocks + 1) / 2;
+      f32x16 dots = {}, dp = {};
+      Piece<T> x[2];
+      read_piece<T, DP, 4>(x[0], k_tile, 32 * b, 0, at_lane);
+#pragma unroll
+      for (int n = 0; n < 2 * kPieces; ++n) {
+        Piece<T> &now = x[n & 1], &next = x[(n + 1) & 1];
+        const int s0 = n % kPieces * 4, s1 = (n + 1) % kPieces * 4;
+        if (n + 1 < 2 * kPieces)
+          read_piece<T, DP, 4>(next, n + 1 < kPieces ? k_tile : v_tile, 32 * b, s1, at_lane);
+        else if constexpr (sizeof(T) == 2)
+          read_column_piece<T, DP>(next, k_tile, 32 * b, 0, at_lane);
+        pin_reads();
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (s0 + i < kSteps) {
+            if (n < kPieces)
+              dots = Mat<T>::mma(now[i], q[s0 + i], dots);
+            else
+              dp = Mat<T>::mma(now[i], g[s0 + i], dp);
+          }
+        pin_reads();
+      }
       float p[16];
 #pragma unroll
       for (int r = 0; r < 16; ++r)
@@ -149,7 +164,20 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 4 && DP > 64 ? 1 : 2) void q
       }
       Weights<T> w;
       w.set(p);
-      kt.add(dq, w);
+      if constexpr (sizeof(T) == 4) {
+        Columns<T, DP> kt;
+        kt.read(k_tile, 32 * b);
+        kt.add(dq, w, at_lane);
+      } else {
+#pragma unroll
+        for (int n = 0; n < kHalves; ++n) {
+          Piece<T> &now = x[n & 1], &next = x[(n + 1) & 1];
+          if (n + 1 < kHalves) read_column_piece<T, DP>(next, k_tile, 32 * b, 2 * n + 2, at_lane);
+          pin_reads();
+          add_column_piece<T, DP>(dq, now, w, 2 * n);
+          pin_reads();
+        }
+      }
     }
   }
   store_row<T, DP>(A.dq.at + token * A.dq.row + q_head * A.dq.head, dq, A.scale, A.dim, valid);
@@ -470,23 +498,12 @@ size_t split_bytes(const Splits &s, int64_t k_total, int k_heads, int sequences,
 }
 
 template <typename T, int DP>
-int launch_backward(BackwardArgs &A, float2 *stats, const Splits &splits, hipStream_t s) {
-  constexpr int kLanes = sizeof(T) == 4 ? 32 : 16;
+int launch_backward(BackwardArgs &A, const Splits &splits, hipStream_t s) {
   constexpr int kKeys = sizeof(T) == 4 ? 32 : 64;
   constexpr int kLds = 4 * Shape<T, DP>::tile_bytes(kKeys);
   static_assert(kLds <= 160 * 1024, "LDS of a CU");
   int st = BEVPOOL_OK;
   if (A.q_total > 0) {
-    const int64_t rows = int64_t(A.q_total) * A.q_heads, per = kThreads / kLanes;
-    st = check_grid((rows + per - 1) / per, kThreads, "attention row sums");
-    if (st) return st;
-    {
-      LaunchScope scope("attention_stats", s);
-      hipLaunchKernelGGL((stats_kernel<T, kLanes>), dim3(unsigned((rows + per - 1) / per)),
-                         dim3(kThreads), 0, s, static_cast<const PackedArgs &>(A), stats);
-    }
-    st = check_launch("attention row sums");
-    if (st) return st;
     A.tiles = int(int64_t(A.q_total) * A.group.size / (kWaves * kWaveRows)) + A.sequences + 1;
     const int64_t blocks = int64_t(A.tiles) * A.k_heads;
     st = check_grid(blocks, kThreads, "attention query gradient");
@@ -583,16 +600,15 @@ int bevpool_attention_backward(const void *q, int64_t q_row, int64_t q_head, con
     return fail(BEVPOOL_EINVAL, "out_rest must start at a multiple of 16 bytes");
   A.rest = static_cast<char *>(const_cast<void *>(out_rest));
   A.lse = const_cast<float *>(lse);
-  float2 *stats = static_cast<float2 *>(scratch);
-  A.stats = stats;
+  A.stats = static_cast<float2 *>(scratch);
   Splits splits =
       plan_splits(q_total, k_total, A.group.size, k_heads, sequences, A.causal, elem == 4 ? 32 : 64);
   const size_t stats_bytes = (size_t(q_total) * q_heads * sizeof(float2) + 255) / 256 * 256;
   splits.sums = reinterpret_cast<float *>(static_cast<char *>(scratch) + stats_bytes);
   hipStream_t s = static_cast<hipStream_t>(stream);
-  return dtype == BEVPOOL_BF16  ? (ATTENTION_DIM(__bf16, launch_backward, A, stats, splits, s))
-         : dtype == BEVPOOL_F16 ? (ATTENTION_DIM(_Float16, launch_backward, A, stats, splits, s))
-                                : (ATTENTION_DIM(float, launch_backward, A, stats, splits, s));
+  return dtype == BEVPOOL_BF16  ? (ATTENTION_DIM(__bf16, launch_backward, A, splits, s))
+         : dtype == BEVPOOL_F16 ? (ATTENTION_DIM(_Float16, launch_backward, A, splits, s))
+                                : (ATTENTION_DIM(float, launch_backward, A, splits, s));
 }
 
 }  // extern "C"
