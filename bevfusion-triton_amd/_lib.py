@@ -145,7 +145,7 @@ _SIGNATURES = {
          _vp, _vp, _i32, _i32, _f32, _vp, _vp, _vp, _vp],
         ctypes.c_int,
     ),
-    'bevpool_attention_backward_scratch_bytes': ([_i64, _i64, _i32, _i32, _i32, _i32], _sz),
+    'bevpool_attention_backward_scratch_bytes': ([_i64, _i64, _i32, _i32, _i32, _i32, _i32], _sz),
     'bevpool_attention_backward': (
         [_vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _vp, _i64, _i64, _vp, _i32,
          _i64, _i64, _i32, _i32, _i32, _vp, _vp, _i32, _i32, _f32, _vp, _vp, _vp, _vp, _sz, _vp],

@@ -279,7 +279,8 @@ class _AttendPacked(torch.autograd.Function):
         dout = _aligned(dout.to(q.dtype), q.shape[1] // k.shape[1])
         dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
         nbytes = L.library().bevpool_attention_backward_scratch_bytes(
-            q.shape[0], k.shape[0], q.shape[1], k.shape[1], q.shape[2], q_starts.shape[0] - 1)
+            q.shape[0], k.shape[0], q.shape[1], k.shape[1], q.shape[2], L.DTYPE_CODES[q.dtype],
+            q_starts.shape[0] - 1)
         scratch = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
         _run(lambda lib, s: lib.bevpool_attention_backward(
             *_strides(q), *_strides(k), *_strides(v), L.ptr(out), L.ptr(rest), *_strides(dout), L.ptr(lse),

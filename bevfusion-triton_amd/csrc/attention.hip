@@ -17,14 +17,14 @@ using bevpool_host::LaunchScope;
 
 // Rows of a tile are pairs (query, head of the group), the group's heads next
 // to each other: the heads that share keys share their tiles, and short
-// sequences still fill rows.  A wave has 32 rows and all of the tile's keys;
-// K and V tiles are staged in two buffers, the next one's loads in flight
-// while one is used.
-template <typename T, int DP, int kKeys>
+// sequences still fill rows.  A wave has 32 rows and all of the tile's keys
+// (kHalves: half of them); K and V tiles are staged in two buffers, the next
+// one's loads in flight while one is used.
+template <typename T, int DP, int kKeys, bool kHalves>
 __global__ __launch_bounds__(kThreads, sizeof(T) == 4 && DP > 64 ? 1 : 2) void packed_forward_kernel(
     PackedArgs A) {
   extern __shared__ __attribute__((aligned(16))) char lds[];
-  constexpr int kRows = kWaves * kWaveRows;
+  constexpr int kRows = (kHalves ? 2 : 4) * kWaveRows;
   const int head = blockIdx.x % A.k_heads;
   // late tiles, the long ones of a causal sequence, start first
   const int index = A.tiles - 1 - int(blockIdx.x / A.k_heads);
@@ -37,7 +37,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 4 && DP > 64 ? 1 : 2) void p
   const int r0 = (index - first) * kRows;
   if (r0 >= rows) return;
 
-  const int wave = wave_id(), c = lane_id() & 31, h = lane_id() >> 5;
+  const int wave = wave_id() / (kHalves ? 2 : 1), c = lane_id() & 31, h = lane_id() >> 5;
   const int row = r0 + wave * kWaveRows + c;
   const bool valid = row < rows;
   const int row_in = valid ? row : rows - 1;
@@ -61,11 +61,36 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 4 && DP > 64 ? 1 : 2) void p
   row_frags<T, DP>(q, A.q.at + token * A.q.row + q_head * A.q.head, A.chunks, true);
   Sums<T, DP> out = {};
   Softmax x;
-  attend_tiles<T, DP, kKeys>(lds, q, A.k.at + seq.k0 * A.k.row + head * A.k.head, A.k.row,
+  const int half = kHalves ? wave_id() % 2 : 0;
+  attend_tiles<T, DP, kKeys, kHalves>(lds, q, A.k.at + seq.k0 * A.k.row + head * A.k.head, A.k.row,
                              A.v.at + seq.k0 * A.v.row + head * A.v.head, A.v.row, A.chunks, 0,
-                             keys, seq.nk, limit, low, wave_on ? high : 0, A.scale_log2, x, out);
+                             keys, seq.nk, limit, low, wave_on ? high : 0, A.scale_log2, x, out, half);
 
-  const float sum = sum_halves(x.sum);
+  float sum = sum_halves(x.sum);
+  if constexpr (kHalves) {
+    constexpr int kSums = 64 * 16 * Shape<T, DP>::kBlocks;
+    float *sums = reinterpret_cast<float *>(lds) + wave * (kSums + 128);
+    float2 *tops = reinterpret_cast<float2 *>(sums + kSums);
+    __syncthreads();  // the tiles have been read
+    if (half == 1) {
+      put_sums<T, DP>(sums, out);
+      tops[lane_id()] = make_float2(x.top, sum);
+    }
+    __syncthreads();
+    if (half == 1) return;
+    const float2 other = tops[lane_id()];
+    const float top = fmaxf(x.top, other.x);
+    // (a half that saw nothing has -inf, and -inf less -inf is no number)
+    const float mine = x.top == -kInf ? 1.f : exp2_fast((x.top - top) * A.scale_log2);
+    const float by = other.x == -kInf ? 1.f : exp2_fast((other.x - top) * A.scale_log2);
+    x.top = top;
+    sum = mine * sum + by * other.y;
+#pragma unroll
+    for (int b = 0; b < Shape<T, DP>::kBlocks; ++b)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) out[b][r] *= mine;
+    add_sums<T, DP>(out, sums, by);
+  }
   const bool any = x.top > -kInf || sum != 0.f;
   const float by = any ? 1.f / sum : 0.f;
   const int64_t at = token * A.out.row + q_head * A.out.head;
@@ -78,18 +103,28 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 4 && DP > 64 ? 1 : 2) void p
         any ? (x.top * A.scale_log2 + __builtin_amdgcn_logf(sum)) / kLog2e : -kInf;
 }
 
-template <typename T, int DP>
-int launch_forward(const PackedArgs &A, hipStream_t s) {
-  constexpr int kKeys = sizeof(T) == 4 ? 32 : 64;
-  constexpr int kLds = 4 * Shape<T, DP>::tile_bytes(kKeys);
+template <typename T, int DP, bool kHalves>
+int launch_rows(PackedArgs &A, hipStream_t s) {
+  constexpr int kKeys = sizeof(T) == 4 && !kHalves ? 32 : 64;
+  constexpr int kTiles = 4 * Shape<T, DP>::tile_bytes(kKeys);
+  constexpr int kSums = kHalves ? 2 * (64 * 16 * Shape<T, DP>::kBlocks + 128) * 4 : 0;
+  constexpr int kLds = kTiles > kSums ? kTiles : kSums;
   static_assert(kLds <= 160 * 1024, "LDS of a CU");
+  A.tiles = int(int64_t(A.q_total) * A.group.size / (kHalves ? 64 : 128)) + A.sequences + 1;
   const int64_t blocks = int64_t(A.tiles) * A.k_heads;
   int st = check_grid(blocks, kThreads, "attention forward");
   if (st) return st;
   LaunchScope scope("attention_forward", s);
-  hipLaunchKernelGGL((packed_forward_kernel<T, DP, kKeys>), dim3(unsigned(blocks)),
+  hipLaunchKernelGGL((packed_forward_kernel<T, DP, kKeys, kHalves>), dim3(unsigned(blocks)),
                      dim3(kThreads), kLds, s, A);
   return check_launch("attention forward");
+}
+
+template <typename T, int DP>
+int launch_forward(PackedArgs &A, hipStream_t s) {
+  if constexpr (kMayHalve<T, DP>)
+    if (row_blocks(A) < kFullBlocks) return launch_rows<T, DP, true>(A, s);
+  return launch_rows<T, DP, false>(A, s);
 }
 
 }  // namespace
@@ -175,7 +210,6 @@ int bevpool_attention_forward(const void *q, int64_t q_row, int64_t q_head, cons
   if (q_total == 0) return BEVPOOL_OK;
   A.lse = lse;
   A.rest = static_cast<char *>(out_rest);
-  A.tiles = int(q_total * A.group.size / (kWaves * kWaveRows)) + sequences + 1;
   hipStream_t s = static_cast<hipStream_t>(stream);
   return dtype == BEVPOOL_BF16  ? (ATTENTION_DIM(__bf16, launch_forward, A, s))
          : dtype == BEVPOOL_F16 ? (ATTENTION_DIM(_Float16, launch_forward, A, s))

@@ -43,13 +43,14 @@ __device__ __forceinline__ float row_dot(const Frags<T, DP> &a, const Frags<T, D
 // it from where a row sees few keys, so it is formed from the output before
 // its rounding (out and its rest): with out alone the error of dq and dk grew
 // by a fifth.
-template <typename T, int DP, int kKeys>
+template <typename T, int DP, int kKeys, bool kHalves>
 __global__ __launch_bounds__(kThreads, sizeof(T) == 4 && DP > 64 ? 1 : 2) void query_grad_kernel(
     BackwardArgs A) {
   using S = Shape<T, DP>;
   extern __shared__ __attribute__((aligned(16))) char lds[];
   constexpr int kTile = S::tile_bytes(kKeys);  // buffers: K0 V0 K1 V1
-  constexpr int kRows = kWaves * kWaveRows;
+  constexpr int kRows = (kHalves ? 2 : 4) * kWaveRows;
+  constexpr int kMine = kHalves ? 1 : kKeys / 32;  // blocks of 32 keys a wave takes of a tile
   const int head = blockIdx.x % A.k_heads;
   const int index = A.tiles - 1 - int(blockIdx.x / A.k_heads);
   int first;
@@ -61,7 +62,9 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 4 && DP > 64 ? 1 : 2) void q
   const int r0 = (index - first) * kRows;
   if (r0 >= rows) return;
 
-  const int lane = lane_id(), wave = wave_id(), c = lane & 31, h = lane >> 5;
+  const int lane = lane_id(), c = lane & 31, h = lane >> 5;
+  const int wave = wave_id() / (kHalves ? 2 : 1), half = kHalves ? wave_id() % 2 : 0;
+  const int mine = 32 * half;
   const int row = r0 + wave * kWaveRows + c;
   const bool valid = row < rows;
   const int row_in = valid ? row : rows - 1;
@@ -98,7 +101,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 4 && DP > 64 ? 1 : 2) void q
   }
   settle(stat);
   const float lse2 = stat[0], delta = stat[1];
-  if (valid && h == 0) A.stats[stat_at] = make_float2(lse2, delta);
+  if (valid && h == 0 && half == 0) A.stats[stat_at] = make_float2(lse2, delta);
   const char *k_at = A.k.at + seq.k0 * A.k.row + head * A.k.head;
   const char *v_at = A.v.at + seq.k0 * A.v.row + head * A.v.head;
   const unsigned lds0 = lds_address(lds);
@@ -120,28 +123,28 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 4 && DP > 64 ? 1 : 2) void q
     if (t + 1 < tiles) load_tile(t + 1);
     const char *k_tile = lds + (t & 1) * 2 * kTile, *v_tile = k_tile + kTile;
     const int k0 = t * kKeys;
-    if (!wave_on || k0 >= high) continue;
-    const bool masked = k0 + kKeys > low;
+    if (!wave_on || k0 + mine >= high) continue;
+    const bool masked = k0 + mine + 32 * kMine > low;
     // (hides that the addresses of the reads are the same in every round: kept,
     // they take more registers than there are)
     int at_lane = lane;
     if constexpr (DP * sizeof(T) > 192) asm volatile("" : "+v"(at_lane));
 #pragma unroll
-    for (int b = 0; b < kKeys / 32; ++b) {
+    for (int b = 0; b < kMine; ++b) {
       // Four fragments are read while four are in use.
       constexpr int kSteps = S::kSteps, kPieces = (kSteps + 3) / 4;
-      constexpr int kHalves = (S::kBlocks + 1) / 2;
+      constexpr int kColumns = (S::kBlocks + 1) / 2;  // pieces of 64
       f32x16 dots = {}, dp = {};
       Piece<T> x[2];
-      read_piece<T, DP, 4>(x[0], k_tile, 32 * b, 0, at_lane);
+      read_piece<T, DP, 4>(x[0], k_tile, mine + 32 * b, 0, at_lane);
 #pragma unroll
       for (int n = 0; n < 2 * kPieces; ++n) {
         Piece<T> &now = x[n & 1], &next = x[(n + 1) & 1];
         const int s0 = n % kPieces * 4, s1 = (n + 1) % kPieces * 4;
         if (n + 1 < 2 * kPieces)
-          read_piece<T, DP, 4>(next, n + 1 < kPieces ? k_tile : v_tile, 32 * b, s1, at_lane);
+          read_piece<T, DP, 4>(next, n + 1 < kPieces ? k_tile : v_tile, mine + 32 * b, s1, at_lane);
         else if constexpr (sizeof(T) == 2)
-          read_column_piece<T, DP>(next, k_tile, 32 * b, 0, at_lane);
+          read_column_piece<T, DP>(next, k_tile, mine + 32 * b, 0, at_lane);
         pin_reads();
 #pragma unroll
         for (int i = 0; i < 4; ++i)
@@ -160,25 +163,33 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 4 && DP > 64 ? 1 : 2) void q
       if (masked) {
 #pragma unroll
         for (int r = 0; r < 16; ++r)
-          if (k0 + 32 * b + c_row(r, h) >= limit) p[r] = 0.f;
+          if (k0 + mine + 32 * b + c_row(r, h) >= limit) p[r] = 0.f;
       }
       Weights<T> w;
       w.set(p);
       if constexpr (sizeof(T) == 4) {
         Columns<T, DP> kt;
-        kt.read(k_tile, 32 * b);
+        kt.read(k_tile, mine + 32 * b);
         kt.add(dq, w, at_lane);
       } else {
 #pragma unroll
-        for (int n = 0; n < kHalves; ++n) {
+        for (int n = 0; n < kColumns; ++n) {
           Piece<T> &now = x[n & 1], &next = x[(n + 1) & 1];
-          if (n + 1 < kHalves) read_column_piece<T, DP>(next, k_tile, 32 * b, 2 * n + 2, at_lane);
+          if (n + 1 < kColumns) read_column_piece<T, DP>(next, k_tile, mine + 32 * b, 2 * n + 2, at_lane);
           pin_reads();
           add_column_piece<T, DP>(dq, now, w, 2 * n);
           pin_reads();
         }
       }
     }
+  }
+  if constexpr (kHalves) {
+    float *sums = reinterpret_cast<float *>(lds) + wave * (64 * 16 * S::kBlocks);
+    __syncthreads();  // the tiles have been read
+    if (half == 1) put_sums<T, DP>(sums, dq);
+    __syncthreads();
+    if (half == 1) return;
+    add_sums<T, DP>(dq, sums);
   }
   store_row<T, DP>(A.dq.at + token * A.dq.row + q_head * A.dq.head, dq, A.scale, A.dim, valid);
 }
@@ -189,15 +200,18 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 4 && DP > 64 ? 1 : 2) void q
 // which hide each other's waits.  For longer heads dk and dv are two launches
 // of half the sums each: five products in place of four, but 10 MFLOP a
 // microsecond and CU at two blocks in place of 4 at one (heads of 128, bf16).
-template <typename T, int DP>
+template <typename T, int DP, bool kHalves>
 struct KeyPlan {
+  static constexpr int kKeys = (kHalves ? 2 : 4) * kWaveRows;
   static constexpr bool kApart = DP * sizeof(T) > 192;
   static constexpr int kBlocksPerCu = DP * sizeof(T) > 320 ? 1 : 2;
   // Buffers of Q and dout rows, and behind them the rows' L and D in pairs.
-  static constexpr int kRows = sizeof(T) == 4 ? 32 : 64;  // of a tile
+  static constexpr int kRows = sizeof(T) == 4 && !kHalves ? 32 : 64;  // of a tile
   static constexpr int kTile = Shape<T, DP>::tile_bytes(kRows);
-  static constexpr int kBuffers = sizeof(T) == 4 ? 3 : 2;
-  static constexpr int kLds = kBuffers * (2 * kTile + 8 * kRows);
+  static constexpr int kBuffers = kRows == 32 ? 3 : 2;
+  static constexpr int kTiles = kBuffers * (2 * kTile + 8 * kRows);
+  static constexpr int kHanded = kHalves ? 2 * 64 * 16 * Shape<T, DP>::kBlocks * 4 : 0;
+  static constexpr int kLds = kTiles > kHanded ? kTiles : kHanded;
   static_assert(kLds <= 160 * 1024 / kBlocksPerCu, "LDS of a CU");
   static constexpr int kSums = 16 * Shape<T, DP>::kBlocks;  // registers of dk, and of dv
 };
@@ -206,7 +220,7 @@ struct KeyPlan {
 // key tile at most, each with about `steps` tiles of rows or more.
 struct Splits {
   int most, steps;
-  float *sums;  // [key tile, head][split][dk, dv][wave][register][lane]
+  float *sums;  // [key tile, head][split][dk, dv][32 keys][register][lane]
   __device__ __forceinline__ int of(int tiles) const {
     return max(1, min(most, (tiles + steps - 1) / steps));
   }
@@ -219,9 +233,9 @@ struct KeyTile {
   int begin;     // first row that sees one of its keys
   int rows, tiles;
 };
+template <int kKeys>
 __device__ __forceinline__ bool key_tile_at(const BackwardArgs &A, int index, int tile_rows,
                                             KeyTile &t) {
-  constexpr int kKeys = kWaves * kWaveRows;
   int first;
   const int which = find_sequence(A.k_starts, A.sequences, A.k_total, 1, kKeys, index, &first);
   t.seq = sequence_at(A.q_starts, A.k_starts, which, A.sequences, A.q_total, A.k_total);
@@ -240,10 +254,11 @@ __device__ __forceinline__ bool key_tile_at(const BackwardArgs &A, int index, in
 // of the group) in tiles of 32, from the last to the first that sees one of
 // its keys: blocks of one sequence start together there, and find each
 // other's rows in L2.
-template <typename T, int DP, bool kDk, bool kDv>
-__global__ __launch_bounds__(kThreads, (KeyPlan<T, DP>::kBlocksPerCu)) void key_grad_kernel(
-    BackwardArgs A, Splits splits) {
-  using Plan = KeyPlan<T, DP>;
+template <typename T, int DP, bool kHalves, bool kDk, bool kDv>
+__global__ __launch_bounds__(kThreads, (KeyPlan<T, DP, kHalves>::kBlocksPerCu)) void
+key_grad_kernel(BackwardArgs A, Splits splits) {
+  using Plan = KeyPlan<T, DP, kHalves>;
+  constexpr int kMine = kHalves ? 1 : Plan::kRows / 32;  // blocks of 32 rows a wave takes
   constexpr int kRows = Plan::kRows, kTile = Plan::kTile, kBuffers = Plan::kBuffers;
   constexpr int kSteps = Shape<T, DP>::kSteps, kBlocks = Shape<T, DP>::kBlocks;
   extern __shared__ __attribute__((aligned(16))) char lds[];
@@ -252,7 +267,7 @@ __global__ __launch_bounds__(kThreads, (KeyPlan<T, DP>::kBlocksPerCu)) void key_
   const int index = int(blockIdx.x / A.k_heads) % A.tiles;
   const int split = splits.most - 1 - int(blockIdx.x / A.k_heads) / A.tiles;
   KeyTile tile;
-  if (!key_tile_at(A, index, kRows, tile)) return;
+  if (!key_tile_at<Plan::kKeys>(A, index, kRows, tile)) return;
   const int n_splits = splits.of(tile.tiles);
   if (split >= n_splits) return;
   const Sequence seq = tile.seq;
@@ -261,7 +276,9 @@ __global__ __launch_bounds__(kThreads, (KeyPlan<T, DP>::kBlocksPerCu)) void key_
   const int per_split = (tile.tiles + n_splits - 1) / n_splits;
   const int t_begin = split * per_split, t_end = min(tile.tiles, t_begin + per_split);
 
-  const int lane = lane_id(), wave = wave_id(), c = lane & 31, h = lane >> 5;
+  const int lane = lane_id(), c = lane & 31, h = lane >> 5;
+  const int wave = wave_id() / (kHalves ? 2 : 1), half = kHalves ? wave_id() % 2 : 0;
+  const int mine = 32 * half;
   const float *stats = reinterpret_cast<const float *>(lds + kBuffers * 2 * kTile);
   const int key0 = kb + wave * kWaveRows, key = key0 + c;
   const bool valid = key < seq.nk;
@@ -332,28 +349,29 @@ __global__ __launch_bounds__(kThreads, (KeyPlan<T, DP>::kBlocksPerCu)) void key_
     const char *q_tile = lds + buffer * 2 * kTile, *g_tile = q_tile + kTile;
     const float *stat_row = stats + buffer * 2 * kRows;
     const int r0 = begin + (tile.tiles - 1 - t) * kRows;
-    if (key0 >= seq.nk || r0 + kRows <= from_first) continue;
-    const bool masked = r0 < from_last || r0 + kRows > rows;
+    const int r_mine = r0 + mine, r_end = r_mine + 32 * kMine;
+    if (key0 >= seq.nk || r_end <= from_first || r_mine >= rows) continue;
+    const bool masked = r_mine < from_last || r_end > rows;
     // (hides that the addresses of the reads are the same in every round: kept,
     // they take more registers than there are)
     int at_lane = lane;
     if constexpr ((kDk && kDv && DP > 80) || (sizeof(T) == 4 && DP > 64))
       asm volatile("" : "+v"(at_lane));
 #pragma unroll
-    for (int b = 0; b < kRows / 32; ++b) {
+    for (int b = 0; b < kMine; ++b) {
       // Four fragments are read while four are in use.
       f32x16 dots = {}, dp = {};
       Piece<T> x[2];
       constexpr int kPieces = (kSteps + 3) / 4;  // of a row's fragments
-      read_piece<T, DP, 4>(x[0], q_tile, 32 * b, 0, at_lane);
+      read_piece<T, DP, 4>(x[0], q_tile, mine + 32 * b, 0, at_lane);
 #pragma unroll
       for (int n = 0; n < (kDk ? 2 : 1) * kPieces; ++n) {
         Piece<T> &now = x[n & 1], &next = x[(n + 1) & 1];
         const int s0 = n % kPieces * 4, s1 = (n + 1) % kPieces * 4;
         if (n + 1 < kPieces)
-          read_piece<T, DP, 4>(next, q_tile, 32 * b, s1, at_lane);
+          read_piece<T, DP, 4>(next, q_tile, mine + 32 * b, s1, at_lane);
         else if (kDk && n + 1 < 2 * kPieces)
-          read_piece<T, DP, 4>(next, g_tile, 32 * b, s1, at_lane);
+          read_piece<T, DP, 4>(next, g_tile, mine + 32 * b, s1, at_lane);
         pin_reads();
 #pragma unroll
         for (int i = 0; i < 4; ++i)
@@ -369,8 +387,8 @@ __global__ __launch_bounds__(kThreads, (KeyPlan<T, DP>::kBlocksPerCu)) void key_
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         // L and D of four rows
-        const f32x4 s01 = *reinterpret_cast<const f32x4 *>(stat_row + 64 * b + 16 * i + 8 * h);
-        const f32x4 s23 = *reinterpret_cast<const f32x4 *>(stat_row + 64 * b + 16 * i + 8 * h + 4);
+        const f32x4 s01 = *reinterpret_cast<const f32x4 *>(stat_row + 2 * mine + 64 * b + 16 * i + 8 * h);
+        const f32x4 s23 = *reinterpret_cast<const f32x4 *>(stat_row + 2 * mine + 64 * b + 16 * i + 8 * h + 4);
         const float l[4] = {s01[0], s01[2], s23[0], s23[2]};
         const float d[4] = {s01[1], s01[3], s23[1], s23[3]};
 #pragma unroll
@@ -379,7 +397,7 @@ __global__ __launch_bounds__(kThreads, (KeyPlan<T, DP>::kBlocksPerCu)) void key_
           p[r] = exp2_fast(fmaf(dots[r], A.scale_log2, -l[j]));
           ds[r] = kDk ? p[r] * (dp[r] - d[j]) : 0.f;
           if (masked) {
-            const int at = r0 + 32 * b + c_row(r, h);
+            const int at = r_mine + 32 * b + c_row(r, h);
             if (at < from || at >= rows) p[r] = ds[r] = 0.f;
           }
         }
@@ -389,43 +407,54 @@ __global__ __launch_bounds__(kThreads, (KeyPlan<T, DP>::kBlocksPerCu)) void key_
       if constexpr (kDk) u.set(ds);
       if constexpr (sizeof(T) == 4) {
         Columns<T, DP> g, q;
-        g.read(g_tile, 32 * b);
-        q.read(q_tile, 32 * b);
+        g.read(g_tile, mine + 32 * b);
+        q.read(q_tile, mine + 32 * b);
         if constexpr (kDv) g.add(dv, w, at_lane);
         if constexpr (kDk) q.add(dk, u, at_lane);
       } else {
-        constexpr int kHalves = (kBlocks + 1) / 2;  // pieces of 64 columns
-        constexpr int kFirst = kDv ? 0 : kHalves, kLast = kDk ? 2 * kHalves : kHalves;
+        constexpr int kColumns = (kBlocks + 1) / 2;  // pieces of 64 columns
+        constexpr int kFirst = kDv ? 0 : kColumns, kLast = kDk ? 2 * kColumns : kColumns;
         pin_reads();
-        read_column_piece<T, DP>(x[0], kDv ? g_tile : q_tile, 32 * b, 0, at_lane);
+        read_column_piece<T, DP>(x[0], kDv ? g_tile : q_tile, mine + 32 * b, 0, at_lane);
 #pragma unroll
         for (int n = kFirst; n < kLast; ++n) {
           Piece<T> &now = x[(n - kFirst) & 1], &next = x[(n - kFirst + 1) & 1];
           if (n + 1 < kLast)
-            read_column_piece<T, DP>(next, n + 1 < kHalves ? g_tile : q_tile, 32 * b,
-                                     2 * ((n + 1) % kHalves), at_lane);
+            read_column_piece<T, DP>(next, n + 1 < kColumns ? g_tile : q_tile, mine + 32 * b,
+                                     2 * ((n + 1) % kColumns), at_lane);
           pin_reads();
-          if (n < kHalves)
+          if (n < kColumns)
             add_column_piece<T, DP>(dv, now, w, 2 * n);
           else
-            add_column_piece<T, DP>(dk, now, u, 2 * (n - kHalves));
+            add_column_piece<T, DP>(dk, now, u, 2 * (n - kColumns));
           pin_reads();
         }
       }
     }
   }
 
+  if constexpr (kHalves) {
+    float *sums = reinterpret_cast<float *>(lds) + wave * (64 * 16 * kBlocks);
+#pragma unroll
+    for (int n = kDk ? 0 : 1; n < (kDv ? 2 : 1); ++n) {
+      __syncthreads();  // the tiles, or dk's sums, have been read
+      if (half == 1) put_sums<T, DP>(sums, n == 0 ? dk : dv);
+      __syncthreads();
+      if (half == 0) add_sums<T, DP>(n == 0 ? dk : dv, sums);
+    }
+    if (half == 1) return;
+  }
   if (n_splits > 1) {
     float *put = splits.sums +
                  ((int64_t(index) * A.k_heads + head) * splits.most + split) *
-                     (2 * kWaves * Plan::kSums * 64) +
+                     (2 * (Plan::kKeys / 32) * Plan::kSums * 64) +
                  wave * Plan::kSums * 64 + lane;
 #pragma unroll
     for (int b = 0; b < kBlocks; ++b)
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
         if constexpr (kDk) put[(b * 16 + r) * 64] = dk[b][r];
-        if constexpr (kDv) put[(kWaves * Plan::kSums + b * 16 + r) * 64] = dv[b][r];
+        if constexpr (kDv) put[(Plan::kKeys / 32 * Plan::kSums + b * 16 + r) * 64] = dv[b][r];
       }
     return;
   }
@@ -437,14 +466,15 @@ __global__ __launch_bounds__(kThreads, (KeyPlan<T, DP>::kBlocksPerCu)) void key_
 
 // Adds the sums of a key tile whose walk was cut, in the order of the cuts: a
 // wave for 32 keys' dk, and one for their dv.
-template <typename T, int DP>
+template <typename T, int DP, bool kHalves>
 __global__ __launch_bounds__(64) void key_sum_kernel(BackwardArgs A, Splits splits) {
-  using Plan = KeyPlan<T, DP>;
-  const int n = blockIdx.x & 1, wave = (blockIdx.x >> 1) % kWaves;
-  const int head = blockIdx.x / (2 * kWaves) % A.k_heads;
-  const int index = blockIdx.x / (2 * kWaves) / A.k_heads;
+  using Plan = KeyPlan<T, DP, kHalves>;
+  constexpr int kParts = Plan::kKeys / 32;
+  const int n = blockIdx.x & 1, wave = (blockIdx.x >> 1) % kParts;
+  const int head = blockIdx.x / (2 * kParts) % A.k_heads;
+  const int index = blockIdx.x / (2 * kParts) / A.k_heads;
   KeyTile tile;
-  if (!key_tile_at(A, index, Plan::kRows, tile)) return;
+  if (!key_tile_at<Plan::kKeys>(A, index, Plan::kRows, tile)) return;
   const int n_splits = splits.of(tile.tiles);
   if (n_splits == 1) return;
   const int lane = lane_id();
@@ -454,9 +484,9 @@ __global__ __launch_bounds__(64) void key_sum_kernel(BackwardArgs A, Splits spli
   Sums<T, DP> sum = {};
   const float *from =
       splits.sums +
-      (int64_t(index) * A.k_heads + head) * splits.most * (2 * kWaves * Plan::kSums * 64) +
-      (n * kWaves + wave) * Plan::kSums * 64 + lane;
-  for (int i = 0; i < n_splits; ++i, from += 2 * kWaves * Plan::kSums * 64)
+      (int64_t(index) * A.k_heads + head) * splits.most * (2 * kParts * Plan::kSums * 64) +
+      (n * kParts + wave) * Plan::kSums * 64 + lane;
+  for (int i = 0; i < n_splits; ++i, from += 2 * kParts * Plan::kSums * 64)
 #pragma unroll
     for (int b = 0; b < Shape<T, DP>::kBlocks; ++b)
 #pragma unroll
@@ -471,9 +501,9 @@ __global__ __launch_bounds__(64) void key_sum_kernel(BackwardArgs A, Splits spli
 // are to be about 2048; a cut below 1024 rows would not pay for its sums.  The
 // steps are a block's share if the sequences are alike.
 Splits plan_splits(int64_t q_total, int64_t k_total, int group, int k_heads, int sequences,
-                   int causal, int tile_rows) {
+                   int causal, int tile_keys, int tile_rows) {
   Splits s = {1, 1 << 30, nullptr};
-  const int64_t tiles = k_total / (kWaves * kWaveRows) + sequences + 1;
+  const int64_t tiles = k_total / tile_keys + sequences + 1;
   const int64_t walk = q_total * group / tile_rows + 1;  // of one sequence of all
   const int64_t most = (2048 + tiles * k_heads - 1) / (tiles * k_heads);
   // (`most` decides the scratch, and so goes by the rows alone)
@@ -490,63 +520,94 @@ Splits plan_splits(int64_t q_total, int64_t k_total, int group, int k_heads, int
   return s;
 }
 
-size_t split_bytes(const Splits &s, int64_t k_total, int k_heads, int sequences, int dim) {
+// Whether the keys' kernel takes 64 keys a block.
+bool halve_keys(int64_t k_total, int k_heads, int sequences, int dim, int elem) {
+  return (k_total / 128 + sequences + 1) * k_heads < kFullBlocks && (elem == 2 || dim <= 64);
+}
+
+Splits plan_for(int64_t q_total, int64_t k_total, int q_heads, int k_heads, int dim, int elem,
+                int sequences, int causal) {
+  const bool halves = halve_keys(k_total, k_heads, sequences, dim, elem);
+  return plan_splits(q_total, k_total, q_heads / k_heads, k_heads, sequences, causal,
+                     halves ? 64 : 128, elem == 4 && !halves ? 32 : 64);
+}
+
+size_t split_bytes(const Splits &s, int64_t k_total, int k_heads, int dim, int elem,
+                   int sequences) {
   if (s.most == 1) return 0;
-  const int64_t tiles = k_total / (kWaves * kWaveRows) + sequences + 1;
+  const int keys = halve_keys(k_total, k_heads, sequences, dim, elem) ? 64 : 128;
+  const int64_t tiles = k_total / keys + sequences + 1;
   const int width = dim <= 32 ? 32 : dim <= 64 ? 64 : dim <= 96 ? 96 : 128;
-  return size_t(tiles) * k_heads * s.most * 2 * kWaves * 32 * width * sizeof(float);
+  return size_t(tiles) * k_heads * s.most * 2 * keys * width * sizeof(float);
+}
+
+template <typename T, int DP, bool kHalves>
+int launch_query(BackwardArgs &A, hipStream_t s) {
+  constexpr int kKeys = sizeof(T) == 4 && !kHalves ? 32 : 64;
+  constexpr int kTiles = 4 * Shape<T, DP>::tile_bytes(kKeys);
+  constexpr int kSums = kHalves ? 2 * 64 * 16 * Shape<T, DP>::kBlocks * 4 : 0;
+  constexpr int kLds = kTiles > kSums ? kTiles : kSums;
+  static_assert(kLds <= 160 * 1024, "LDS of a CU");
+  A.tiles = int(int64_t(A.q_total) * A.group.size / (kHalves ? 64 : 128)) + A.sequences + 1;
+  const int64_t blocks = int64_t(A.tiles) * A.k_heads;
+  int st = check_grid(blocks, kThreads, "attention query gradient");
+  if (st) return st;
+  LaunchScope scope("attention_query_grad", s);
+  hipLaunchKernelGGL((query_grad_kernel<T, DP, kKeys, kHalves>), dim3(unsigned(blocks)),
+                     dim3(kThreads), kLds, s, A);
+  return check_launch("attention query gradient");
+}
+
+template <typename T, int DP, bool kHalves>
+int launch_keys(BackwardArgs &A, const Splits &splits, hipStream_t s) {
+  using Plan = KeyPlan<T, DP, kHalves>;
+  A.tiles = A.k_total / Plan::kKeys + A.sequences + 1;
+  const int64_t blocks = int64_t(A.tiles) * A.k_heads;
+  int st = check_grid(blocks * splits.most, kThreads, "attention key gradient");
+  if (st) return st;
+  const dim3 grid(unsigned(blocks * splits.most));
+  if constexpr (Plan::kApart) {
+    {
+      LaunchScope scope("attention_key_grad", s);
+      hipLaunchKernelGGL((key_grad_kernel<T, DP, kHalves, true, false>), grid, dim3(kThreads),
+                         Plan::kLds, s, A, splits);
+    }
+    LaunchScope scope("attention_value_grad", s);
+    hipLaunchKernelGGL((key_grad_kernel<T, DP, kHalves, false, true>), grid, dim3(kThreads),
+                       Plan::kLds, s, A, splits);
+  } else {
+    LaunchScope scope("attention_key_grad", s);
+    hipLaunchKernelGGL((key_grad_kernel<T, DP, kHalves, true, true>), grid, dim3(kThreads),
+                       Plan::kLds, s, A, splits);
+  }
+  st = check_launch("attention key gradient");
+  if (st || splits.most == 1) return st;
+  const int64_t sums = blocks * 2 * (Plan::kKeys / 32);
+  st = check_grid(sums, 64, "attention key sums");
+  if (st) return st;
+  LaunchScope scope("attention_key_sum", s);
+  hipLaunchKernelGGL((key_sum_kernel<T, DP, kHalves>), dim3(unsigned(sums)), dim3(64), 0, s, A,
+                     splits);
+  return check_launch("attention key sums");
 }
 
 template <typename T, int DP>
 int launch_backward(BackwardArgs &A, const Splits &splits, hipStream_t s) {
-  constexpr int kKeys = sizeof(T) == 4 ? 32 : 64;
-  constexpr int kLds = 4 * Shape<T, DP>::tile_bytes(kKeys);
-  static_assert(kLds <= 160 * 1024, "LDS of a CU");
   int st = BEVPOOL_OK;
   if (A.q_total > 0) {
-    A.tiles = int(int64_t(A.q_total) * A.group.size / (kWaves * kWaveRows)) + A.sequences + 1;
-    const int64_t blocks = int64_t(A.tiles) * A.k_heads;
-    st = check_grid(blocks, kThreads, "attention query gradient");
-    if (st) return st;
-    {
-      LaunchScope scope("attention_query_grad", s);
-      hipLaunchKernelGGL((query_grad_kernel<T, DP, kKeys>), dim3(unsigned(blocks)),
-                         dim3(kThreads), kLds, s, A);
+    bool halves = false;
+    if constexpr (kMayHalve<T, DP>) {
+      halves = row_blocks(A) < kFullBlocks;
+      if (halves) st = launch_query<T, DP, true>(A, s);
     }
-    st = check_launch("attention query gradient");
+    if (!halves) st = launch_query<T, DP, false>(A, s);
     if (st) return st;
   }
-  if (A.k_total > 0) {
-    A.tiles = A.k_total / (kWaves * kWaveRows) + A.sequences + 1;
-    const int64_t blocks = int64_t(A.tiles) * A.k_heads;
-    st = check_grid(blocks * splits.most, kThreads, "attention key gradient");
-    if (st) return st;
-    const dim3 grid(unsigned(blocks * splits.most));
-    constexpr int kKeyLds = KeyPlan<T, DP>::kLds;
-    if constexpr (KeyPlan<T, DP>::kApart) {
-      {
-        LaunchScope scope("attention_key_grad", s);
-        hipLaunchKernelGGL((key_grad_kernel<T, DP, true, false>), grid, dim3(kThreads), kKeyLds, s,
-                           A, splits);
-      }
-      LaunchScope scope("attention_value_grad", s);
-      hipLaunchKernelGGL((key_grad_kernel<T, DP, false, true>), grid, dim3(kThreads), kKeyLds, s,
-                         A, splits);
-    } else {
-      LaunchScope scope("attention_key_grad", s);
-      hipLaunchKernelGGL((key_grad_kernel<T, DP, true, true>), grid, dim3(kThreads), kKeyLds, s, A,
-                         splits);
-    }
-    st = check_launch("attention key gradient");
-    if (st || splits.most == 1) return st;
-    st = check_grid(blocks * 2 * kWaves, 64, "attention key sums");
-    if (st) return st;
-    LaunchScope scope("attention_key_sum", s);
-    hipLaunchKernelGGL((key_sum_kernel<T, DP>), dim3(unsigned(blocks * 2 * kWaves)), dim3(64), 0, s,
-                       A, splits);
-    st = check_launch("attention key sums");
-  }
-  return st;
+  if (A.k_total == 0) return st;
+  if constexpr (kMayHalve<T, DP>)
+    if (halve_keys(A.k_total, A.k_heads, A.sequences, A.dim, sizeof(T)))
+      return launch_keys<T, DP, true>(A, splits, s);
+  return launch_keys<T, DP, false>(A, splits, s);
 }
 
 }  // namespace
@@ -554,12 +615,13 @@ int launch_backward(BackwardArgs &A, const Splits &splits, hipStream_t s) {
 extern "C" {
 
 size_t bevpool_attention_backward_scratch_bytes(int64_t q_total, int64_t k_total, int32_t q_heads,
-                                                int32_t k_heads, int32_t dim, int32_t sequences) {
+                                                int32_t k_heads, int32_t dim, int32_t dtype,
+                                                int32_t sequences) {
   if (q_total < 1 || q_heads < 1 || k_heads < 1 || k_total < 0 || sequences < 0) return 0;
+  const int elem = dtype == BEVPOOL_F32 ? 4 : 2;
   const size_t stats = size_t(q_total) * size_t(q_heads) * sizeof(float2);
-  // (causal walks are cut as often or more)
-  const Splits s = plan_splits(q_total, k_total, q_heads / k_heads, k_heads, sequences, 1, 32);
-  return (stats + 255) / 256 * 256 + split_bytes(s, k_total, k_heads, sequences, dim);
+  const Splits s = plan_for(q_total, k_total, q_heads, k_heads, dim, elem, sequences, 1);
+  return (stats + 255) / 256 * 256 + split_bytes(s, k_total, k_heads, dim, elem, sequences);
 }
 
 int bevpool_attention_backward(const void *q, int64_t q_row, int64_t q_head, const void *k,
@@ -592,7 +654,7 @@ int bevpool_attention_backward(const void *q, int64_t q_row, int64_t q_head, con
   if (A.q.head * heads >= (1 << 30) || A.dout.head * heads >= (1 << 30))
     return fail(BEVPOOL_EINVAL, "q, dout: the heads of a group must lie within 2^30 bytes");
   const size_t need = bevpool_attention_backward_scratch_bytes(q_total, k_total, q_heads, k_heads,
-                                                               dim, sequences);
+                                                               dim, dtype, sequences);
   if (scratch_bytes < need || (need > 0 && !scratch))
     return fail(BEVPOOL_ESPACE, "attention backward scratch: %zu bytes, %zu needed",
                 scratch_bytes, need);
@@ -601,8 +663,7 @@ int bevpool_attention_backward(const void *q, int64_t q_row, int64_t q_head, con
   A.rest = static_cast<char *>(const_cast<void *>(out_rest));
   A.lse = const_cast<float *>(lse);
   A.stats = static_cast<float2 *>(scratch);
-  Splits splits =
-      plan_splits(q_total, k_total, A.group.size, k_heads, sequences, A.causal, elem == 4 ? 32 : 64);
+  Splits splits = plan_for(q_total, k_total, q_heads, k_heads, dim, elem, sequences, A.causal);
   const size_t stats_bytes = (size_t(q_total) * q_heads * sizeof(float2) + 255) / 256 * 256;
   splits.sums = reinterpret_cast<float *>(static_cast<char *>(scratch) + stats_bytes);
   hipStream_t s = static_cast<hipStream_t>(stream);

@@ -479,14 +479,18 @@ __device__ __forceinline__ void softmax_step(float (&s)[kN], Softmax &x, f32x16 
 // V1), the next tile's loads in flight while one is used.  This lane's row
 // sees the keys below `limit`; every row of the wave those below `low` (no
 // mask there), none those from `high` on.  Keys from `stored` on are not
-// read.  The block calls it together, with the same begin and end.
-template <typename T, int DP, int kKeys>
+// read.  The block calls it together, with the same begin and end.  With
+// kHalves the wave takes 32 keys of each tile of 64, those from 32 * half on.
+template <typename T, int DP, int kKeys, bool kHalves = false>
 __device__ __forceinline__ void attend_tiles(char *lds, const Frags<T, DP> &q, const char *k_at,
                                              int64_t k_row, const char *v_at, int64_t v_row,
                                              int chunks, int begin, int end, int stored, int limit,
                                              int low, int high, float scale_log2, Softmax &x,
-                                             Sums<T, DP> &out) {
+                                             Sums<T, DP> &out, int half = 0) {
   constexpr int kTile = Shape<T, DP>::tile_bytes(kKeys);
+  constexpr int kMine = kHalves ? 1 : kKeys / 32;  // blocks of 32 keys
+  static_assert(!kHalves || kKeys == 64, "two halves of 32");
+  const int mine = kHalves ? 32 * half : 0;
   const int h = lane_id() >> 5;
   const unsigned lds0 = lds_address(lds);
   Stage<T, DP, kKeys, kThreads> k_stage, v_stage;
@@ -505,34 +509,34 @@ __device__ __forceinline__ void attend_tiles(char *lds, const Frags<T, DP> &q, c
     __syncthreads();  // this tile is there, and the last one has been read
     if (k0 + kKeys < end) load_tile(k0 + kKeys, buffer ^ 1);
     const char *k_tile = lds + buffer * 2 * kTile, *v_tile = k_tile + kTile;
-    if (k0 >= high) continue;
-    float s[kKeys / 2];
+    if (k0 + mine >= high) continue;
+    float s[16 * kMine];
 #pragma unroll
-    for (int b = 0; b < kKeys / 32; ++b) {
+    for (int b = 0; b < kMine; ++b) {
       Frags<T, DP> k;
-      read_rows<T, DP>(k, k_tile, 32 * b);
+      read_rows<T, DP>(k, k_tile, mine + 32 * b);
       pin_reads();
       const f32x16 dots = dot_rows<T, DP>(k, q);
 #pragma unroll
       for (int r = 0; r < 16; ++r) s[16 * b + r] = dots[r];
     }
-    if (k0 + kKeys > low) {
+    if (k0 + mine + 32 * kMine > low) {
 #pragma unroll
-      for (int b = 0; b < kKeys / 32; ++b)
+      for (int b = 0; b < kMine; ++b)
 #pragma unroll
         for (int r = 0; r < 16; ++r)
-          if (k0 + 32 * b + c_row(r, h) >= limit) s[16 * b + r] = -kInf;
+          if (k0 + mine + 32 * b + c_row(r, h) >= limit) s[16 * b + r] = -kInf;
     }
     softmax_step(s, x, out, scale_log2);
 #pragma unroll
-    for (int b = 0; b < kKeys / 32; ++b) {
+    for (int b = 0; b < kMine; ++b) {
       float p[16];
 #pragma unroll
       for (int r = 0; r < 16; ++r) p[r] = s[16 * b + r];
       Weights<T> w;
       w.set(p);
       Columns<T, DP> v;
-      v.read(v_tile, 32 * b);
+      v.read(v_tile, mine + 32 * b);
       pin_reads();
       v.add(out, w);
     }
@@ -588,9 +592,33 @@ __device__ __forceinline__ void store_row(char *row, const Sums<T, DP> &acc, flo
   }
 }
 
+// A lane's sums pass from the waves of one half to those of the other through
+// LDS, at `at` (the pair's, 64 * 16 * kBlocks floats).
+template <typename T, int DP>
+__device__ __forceinline__ void put_sums(float *at, const Sums<T, DP> &acc) {
+#pragma unroll
+  for (int b = 0; b < Shape<T, DP>::kBlocks; ++b)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) at[(b * 16 + r) * 64 + lane_id()] = acc[b][r];
+}
+template <typename T, int DP>
+__device__ __forceinline__ void add_sums(Sums<T, DP> &acc, const float *at, float by = 1.f) {
+#pragma unroll
+  for (int b = 0; b < Shape<T, DP>::kBlocks; ++b)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) acc[b][r] += by * at[(b * 16 + r) * 64 + lane_id()];
+}
+
 // ---------------------------------------------------------------------------
 // packed sequences
 // ---------------------------------------------------------------------------
+
+// Blocks of four waves take 128 rows (or keys), 32 a wave, where that fills
+// the card: two blocks a CU.  Below that they take 64, and two waves halve
+// the walk over the other side, whose length is then the time of the launch.
+constexpr int kFullBlocks = 512;
+template <typename T, int DP>
+constexpr bool kMayHalve = DP * int(sizeof(T)) <= 256;  // (a tile of 64 in LDS, twice)
 
 // n / group for n < 2^32 / group.
 struct Group {
@@ -678,6 +706,11 @@ struct PackedArgs {
   float scale, scale_log2;
   int tiles;
 };
+
+// Blocks of 128 rows that a call has.
+inline int64_t row_blocks(const PackedArgs &A) {
+  return (int64_t(A.q_total) * A.group.size / 128 + A.sequences + 1) * A.k_heads;
+}
 
 // Host side (attention.hip): sizes and operands of a packed call.
 __attribute__((visibility("hidden"))) int check_packed(

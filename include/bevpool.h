@@ -607,7 +607,8 @@ int bevpool_attention_forward(const void *q, int64_t q_row, int64_t q_head, cons
  *   scratch   >= bevpool_attention_backward_scratch_bytes(...)
  */
 size_t bevpool_attention_backward_scratch_bytes(int64_t q_total, int64_t k_total, int32_t q_heads,
-                                                int32_t k_heads, int32_t dim, int32_t sequences);
+                                                int32_t k_heads, int32_t dim, int32_t dtype,
+                                                int32_t sequences);
 
 int bevpool_attention_backward(const void *q, int64_t q_row, int64_t q_head, const void *k,
                                int64_t k_row, int64_t k_head, const void *v, int64_t v_row,

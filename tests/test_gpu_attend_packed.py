@@ -98,6 +98,30 @@ def test_many_sequences(pkg, cuda):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize('causal', [False, True])
+@pytest.mark.parametrize('dtype', DTYPES)
+@pytest.mark.parametrize('dim', [32, 64, 80, 96, 128])
+def test_full_card(pkg, cuda, dim, dtype, causal):
+    """Enough blocks for the form that takes 128 rows a block (the smaller
+    cases take 64)."""
+    g = torch.Generator().manual_seed(dim)
+    lengths = torch.randint(0, 3, (600,), generator=g).tolist()
+    lengths[5], lengths[300], lengths[599] = 150, 260, 70
+    keys = list(lengths)
+    keys[300], keys[599] = 200, 130
+    check(pkg, cuda, make(lengths, keys, 2, 1, dim, dtype), causal)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('dtype', DTYPES)
+@pytest.mark.parametrize('dim', [32, 80, 128])
+def test_long_walks(pkg, cuda, dim, dtype):
+    """Few keys that very many rows see: the walk over them is cut."""
+    check(pkg, cuda, make([1100, 900], [70, 140], 8, 1, dim, dtype), False)
+    check(pkg, cuda, make([700], [700], 6, 1, dim, dtype), True)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize('dtype', DTYPES)
 def test_parts_of_one_projection(pkg, cuda, dtype):
     """Operands as slices of one matrix, aligned and not, and a gradient with

@@ -51,7 +51,7 @@ def test_attention(pkg):
         assert text in lib.bevpool_last_error(), bad
     args = (16, 256, 64, 16, 128, 64, 16, 128, 64, 16, 16, 16, 256, 64, 16, 2, 4, 4, 4, 2, 64, 16, 16,
             1, 0, 0.125, 16, 16, 16)
-    assert lib.bevpool_attention_backward_scratch_bytes(4, 4, 4, 2, 64, 1) == 256
+    assert lib.bevpool_attention_backward_scratch_bytes(4, 4, 4, 2, 64, 2, 1) == 256
     assert lib.bevpool_attention_backward(*args, None, 0, None) == -3
     assert b'scratch' in lib.bevpool_last_error()
 
