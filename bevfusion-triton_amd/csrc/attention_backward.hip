@@ -520,22 +520,29 @@ Splits plan_splits(int64_t q_total, int64_t k_total, int group, int k_heads, int
   return s;
 }
 
-// Whether the keys' kernel takes 64 keys a block.
-bool halve_keys(int64_t k_total, int k_heads, int sequences, int dim, int elem) {
-  return (k_total / 128 + sequences + 1) * k_heads < kFullBlocks && (elem == 2 || dim <= 64);
+// Whether the keys' kernel takes 64 keys a block: where key tiles of 128, with
+// the cuts that sequences of the mean length have, do not fill the card.
+bool halve_keys(int64_t q_total, int64_t k_total, int group, int k_heads, int sequences, int dim,
+                int elem) {
+  if (elem == 4 && dim > 64) return false;
+  const Splits s = plan_splits(q_total, k_total, group, k_heads, sequences, 1, 128, 64);
+  const int64_t mean = q_total * group / 1024 / (sequences > 0 ? sequences : 1);
+  const int64_t cuts = mean < 1 ? 1 : mean < s.most ? mean : s.most;
+  return (k_total / 128 + sequences + 1) * k_heads * cuts < kFullBlocks;
 }
 
-Splits plan_for(int64_t q_total, int64_t k_total, int q_heads, int k_heads, int dim, int elem,
+Splits plan_for(int64_t q_total, int64_t k_total, int group, int k_heads, int dim, int elem,
                 int sequences, int causal) {
-  const bool halves = halve_keys(k_total, k_heads, sequences, dim, elem);
-  return plan_splits(q_total, k_total, q_heads / k_heads, k_heads, sequences, causal,
-                     halves ? 64 : 128, elem == 4 && !halves ? 32 : 64);
+  const bool halves = halve_keys(q_total, k_total, group, k_heads, sequences, dim, elem);
+  return plan_splits(q_total, k_total, group, k_heads, sequences, causal, halves ? 64 : 128,
+                     elem == 4 && !halves ? 32 : 64);
 }
 
-size_t split_bytes(const Splits &s, int64_t k_total, int k_heads, int dim, int elem,
-                   int sequences) {
+size_t split_bytes(const Splits &s, int64_t q_total, int64_t k_total, int group, int k_heads,
+                   int dim, int elem, int sequences) {
   if (s.most == 1) return 0;
-  const int keys = halve_keys(k_total, k_heads, sequences, dim, elem) ? 64 : 128;
+  const int keys =
+      halve_keys(q_total, k_total, group, k_heads, sequences, dim, elem) ? 64 : 128;
   const int64_t tiles = k_total / keys + sequences + 1;
   const int width = dim <= 32 ? 32 : dim <= 64 ? 64 : dim <= 96 ? 96 : 128;
   return size_t(tiles) * k_heads * s.most * 2 * keys * width * sizeof(float);
@@ -605,7 +612,7 @@ int launch_backward(BackwardArgs &A, const Splits &splits, hipStream_t s) {
   }
   if (A.k_total == 0) return st;
   if constexpr (kMayHalve<T, DP>)
-    if (halve_keys(A.k_total, A.k_heads, A.sequences, A.dim, sizeof(T)))
+    if (halve_keys(A.q_total, A.k_total, A.group.size, A.k_heads, A.sequences, A.dim, sizeof(T)))
       return launch_keys<T, DP, true>(A, splits, s);
   return launch_keys<T, DP, false>(A, splits, s);
 }
@@ -620,8 +627,10 @@ size_t bevpool_attention_backward_scratch_bytes(int64_t q_total, int64_t k_total
   if (q_total < 1 || q_heads < 1 || k_heads < 1 || k_total < 0 || sequences < 0) return 0;
   const int elem = dtype == BEVPOOL_F32 ? 4 : 2;
   const size_t stats = size_t(q_total) * size_t(q_heads) * sizeof(float2);
-  const Splits s = plan_for(q_total, k_total, q_heads, k_heads, dim, elem, sequences, 1);
-  return (stats + 255) / 256 * 256 + split_bytes(s, k_total, k_heads, dim, elem, sequences);
+  const int group = q_heads / k_heads;
+  const Splits s = plan_for(q_total, k_total, group, k_heads, dim, elem, sequences, 1);
+  return (stats + 255) / 256 * 256 +
+         split_bytes(s, q_total, k_total, group, k_heads, dim, elem, sequences);
 }
 
 int bevpool_attention_backward(const void *q, int64_t q_row, int64_t q_head, const void *k,
@@ -663,7 +672,8 @@ int bevpool_attention_backward(const void *q, int64_t q_row, int64_t q_head, con
   A.rest = static_cast<char *>(const_cast<void *>(out_rest));
   A.lse = const_cast<float *>(lse);
   A.stats = static_cast<float2 *>(scratch);
-  Splits splits = plan_for(q_total, k_total, q_heads, k_heads, dim, elem, sequences, A.causal);
+  Splits splits =
+      plan_for(q_total, k_total, A.group.size, k_heads, dim, elem, sequences, A.causal);
   const size_t stats_bytes = (size_t(q_total) * q_heads * sizeof(float2) + 255) / 256 * 256;
   splits.sums = reinterpret_cast<float *>(static_cast<char *>(scratch) + stats_bytes);
   hipStream_t s = static_cast<hipStream_t>(stream);
