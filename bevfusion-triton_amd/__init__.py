@@ -13,7 +13,8 @@ ziyangyeh/bevfusion-triton behind the reference's own Python surface:
                                             quantisation (cacheable for static cameras)
   legacy.bev_pool / legacy.QuickCumsumCuda  ops/bev_pool/bev_pool_legacy.py:53-108
   norm_rotate, attend_packed, attend_cached  operators of a transformer over camera and BEV
-                                            tokens (no counterpart in the reference)
+                                            tokens, and TokenAttention, the layer that
+                                            runs them (no counterpart in the reference)
 
 The kernels live in ``csrc/`` and are reached through the C ABI of
 ``include/bevpool.h`` (``libbevpool_amd.so``, loaded by ``_lib``).  There is no
@@ -26,6 +27,7 @@ from . import legacy
 from ._lib import BevPoolError, LibraryNotBuilt, library
 from .attention import attend_cached, attend_packed, axis_frequencies, norm_rotate
 from .bev_pool import BevPoolFunction, BevPoolIndexExport, bev_pool, check_errors
+from .tokens import TokenAttention
 from .vtransform import (BevPoolTransform, CameraIndex, LSSIndexExport, create_frustum, gen_dx_bx, host_grid, lss_bev_pool, lss_bev_pool_depth,
                          lss_index_cameras)
 
@@ -37,6 +39,7 @@ __all__ = [
     'CameraIndex',
     'LSSIndexExport',
     'LibraryNotBuilt',
+    'TokenAttention',
     'attend_cached',
     'attend_packed',
     'axis_frequencies',
