@@ -22,6 +22,7 @@ torch's allocator and never wait for the device.
 from __future__ import annotations
 
 import ctypes
+import functools
 
 import torch
 
@@ -65,7 +66,7 @@ def _unit(x):
 
 
 def _strides(x):
-    return (L.ptr(x), x.stride(0), x.stride(1)) if x is not None else (0, 0, 0)
+    return (x.data_ptr(), *x.stride()[:2]) if x is not None else (0, 0, 0)
 
 
 def _run(call, device, what):
@@ -88,9 +89,8 @@ def _wants_grad(*tensors):
 def _norm_rotate(q, k, q_weight, k_weight, positions, frequencies, pairs, eps, interleaved):
     tokens, q_heads, dim = q.shape
     k_heads = k.shape[1] if k is not None else 0
-    q_out = torch.empty((tokens, q_heads, dim), dtype=q.dtype, device=q.device)
-    k_out = None if k is None else torch.empty((tokens, k_heads, dim), dtype=q.dtype,
-                                               device=q.device)
+    q_out = q.new_empty(q.shape)
+    k_out = None if k is None else k.new_empty(k.shape)
     _run(lambda lib, s: lib.bevpool_norm_rotate_forward(
         *_strides(q), q_heads, *_strides(k), k_heads, L.DTYPE_CODES[q.dtype], tokens, dim,
         *_rotation(positions, frequencies, pairs, interleaved), L.ptr(q_weight), L.ptr(k_weight),
@@ -122,11 +122,11 @@ class _NormRotate(torch.autograd.Function):
                 return None
             if g is None:  # an output that nothing was computed from
                 return torch.zeros((tokens, heads, dim), dtype=dtype, device=dev)
-            return _unit(g.to(dtype))
+            return _unit(g if g.dtype == dtype else g.to(dtype))
 
         dq_out, dk_out = grad_rows(dq_out, q_heads), grad_rows(dk_out, k_heads)
-        dq = torch.empty((tokens, q_heads, dim), dtype=dtype, device=dev)
-        dk = torch.empty((tokens, k_heads, dim), dtype=dtype, device=dev) if k_heads else None
+        dq = dq_out.new_empty(dq_out.shape)
+        dk = dk_out.new_empty(dk_out.shape) if k_heads else None
         dqw = torch.empty_like(q_weight) if q_weight is not None else None
         dkw = torch.empty_like(k_weight) if k_weight is not None else None
         lib = L.library()
@@ -145,7 +145,12 @@ class _NormRotate(torch.autograd.Function):
 def _rotation(positions, frequencies, pairs, interleaved):
     return (L.ptr(positions), _POSITION_KINDS[positions.dtype],
             positions.stride(0) if positions.shape[0] else 0, L.ptr(frequencies),
-            (ctypes.c_int32 * max(1, len(pairs)))(*pairs), len(pairs), int(interleaved))
+            _counts(pairs), len(pairs), int(interleaved))
+
+
+@functools.lru_cache(maxsize=64)
+def _counts(pairs):
+    return (ctypes.c_int32 * max(1, len(pairs)))(*pairs)
 
 
 def norm_rotate(q, k, positions, frequencies, pairs=None, *, q_weight=None, k_weight=None,
@@ -211,9 +216,10 @@ def _aligned(x, group=1):
     multiple of 16 bytes, and strides whose multiples over a tile (64 rows,
     the heads of a group) the kernels form in 32 bits: itself, or a copy."""
     size = x.element_size()
-    row, head = x.stride(0) * size, x.stride(1) * size
-    if (x.stride(-1) == 1 and x.data_ptr() % 16 == 0 and row % 16 == 0 and head % 16 == 0
-            and row < 1 << 24 and head * group < 1 << 30):
+    row, head, one = x.stride()
+    row, head = row * size, head * size
+    if (one == 1 and row % 16 == 0 and head % 16 == 0 and row < 1 << 24
+            and head * group < 1 << 30 and x.data_ptr() % 16 == 0):
         return x
     return x.contiguous() if not x.is_contiguous() else x.clone()
 
@@ -246,12 +252,14 @@ def _check_starts(name, starts, like):
         raise TypeError(f'{name} must have dtype torch.int32 or torch.int64.')
     if starts.device != like.device:
         raise ValueError(f'{name} must be on the device of q ({like.device}).')
+    if starts.dtype == torch.int32 and starts.is_contiguous():
+        return starts
     return starts.to(torch.int32).contiguous()
 
 
 def _attend_packed(q, k, v, q_starts, k_starts, causal, scale, rest=None):
-    out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    lse = torch.empty(q.shape[:2], dtype=torch.float32, device=q.device)
+    out = q.new_empty(q.shape)
+    lse = q.new_empty(q.shape[:2], dtype=torch.float32)
     _run(lambda lib, s: lib.bevpool_attention_forward(
         *_strides(q), *_strides(k), *_strides(v), L.DTYPE_CODES[q.dtype], q.shape[0], k.shape[0],
         q.shape[1], k.shape[1], q.shape[2], L.ptr(q_starts), L.ptr(k_starts),
@@ -264,8 +272,7 @@ class _AttendPacked(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, q_starts, k_starts, causal, scale):
         # (16-bit types: the output's rounding, for the gradients)
-        rest = torch.empty_like(q, memory_format=torch.contiguous_format) \
-            if q.element_size() == 2 else None
+        rest = q.new_empty(q.shape) if q.element_size() == 2 else None
         out, lse = _attend_packed(q, k, v, q_starts, k_starts, causal, scale, rest)
         ctx.save_for_backward(q, k, v, out, rest, lse, q_starts, k_starts)
         ctx.call = (causal, scale)
@@ -276,12 +283,14 @@ class _AttendPacked(torch.autograd.Function):
     def backward(ctx, dout, _):
         q, k, v, out, rest, lse, q_starts, k_starts = ctx.saved_tensors
         causal, scale = ctx.call
-        dout = _aligned(dout.to(q.dtype), q.shape[1] // k.shape[1])
-        dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
+        if dout.dtype != q.dtype:
+            dout = dout.to(q.dtype)
+        dout = _aligned(dout, q.shape[1] // k.shape[1])
+        dq, dk, dv = q.new_empty(q.shape), k.new_empty(k.shape), v.new_empty(v.shape)
         nbytes = L.library().bevpool_attention_backward_scratch_bytes(
             q.shape[0], k.shape[0], q.shape[1], k.shape[1], q.shape[2], L.DTYPE_CODES[q.dtype],
             q_starts.shape[0] - 1)
-        scratch = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
+        scratch = q.new_empty(nbytes, dtype=torch.uint8)
         _run(lambda lib, s: lib.bevpool_attention_backward(
             *_strides(q), *_strides(k), *_strides(v), L.ptr(out), L.ptr(rest), *_strides(dout), L.ptr(lse),
             L.DTYPE_CODES[q.dtype], q.shape[0], k.shape[0], q.shape[1], k.shape[1], q.shape[2],
@@ -383,12 +392,13 @@ def attend_cached(q, k, v, lengths, prefix_k=None, prefix_v=None, *, scale=None)
     if _wants_grad(q, k, v, prefix_k, prefix_v):
         raise RuntimeError('attend_cached has no gradient; call it under torch.no_grad()')
     rows = _aligned(q.reshape(requests * tokens, q_heads, dim))
-    lengths = lengths.to(torch.int32).contiguous()
+    if lengths.dtype != torch.int32 or not lengths.is_contiguous():
+        lengths = lengths.to(torch.int32).contiguous()
     prefix = prefix_k.shape[0] if prefix_k is not None else 0
-    out = torch.empty((requests, tokens, q_heads, dim), dtype=q.dtype, device=q.device)
+    out = q.new_empty(q.shape)
     nbytes = L.library().bevpool_attention_cached_scratch_bytes(
         requests, tokens, capacity, prefix, q_heads, k_heads, dim)
-    scratch = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
+    scratch = q.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
     _run(lambda lib, s: lib.bevpool_attention_cached(
         *_strides(rows), L.ptr(k), *k.stride()[:3], L.ptr(v), *v.stride()[:3],
         *_strides(prefix_k), *_strides(prefix_v), L.ptr(lengths), L.DTYPE_CODES[q.dtype],
