@@ -80,7 +80,9 @@ template <typename T, int DP>
 struct Shape {
   static constexpr int kSteps = DP * int(sizeof(T)) / 32;        // fragments of a row (2 chunks)
   static constexpr int kChunks = 2 * kSteps;
-  static constexpr int kPitch = (kChunks + 7) / 8 * 8;           // chunks of a row in LDS
+  // chunks of a row in LDS: whole groups of four (float: eight), see swizzle()
+  static constexpr int kPitch =
+      sizeof(T) == 2 ? (kChunks + 3) / 4 * 4 : (kChunks + 7) / 8 * 8;
   static constexpr int kBlocks = (DP + 31) / 32;                 // blocks of 32 elements
   static constexpr int tile_bytes(int rows) { return rows * kPitch * 16; }
 };
@@ -171,14 +173,17 @@ __device__ __forceinline__ unsigned lds_address(const char *p) {
 
 // Where chunk c of row r lies in its row: at c ^ swizzle(r).  LDS gives 256
 // bytes a cycle, 16 chunks.  A fragment read takes one chunk of 16 rows at
-// once, a transposing read four chunks of four rows: with rows of a multiple
-// of 256 bytes the four low bits of r, those of r % 4 first, put either into
-// 16 different places; with rows of an odd number of 128 bytes, neighbours
-// are in different halves by themselves and the next bits do the rest.  For
-// float the second kind of read is 8 chunks of the rows r and r + 4.
+// once, a transposing read four chunks, a group, of four rows.  With rows of
+// a multiple of 256 bytes all four low bits of r have to tell the places
+// apart, those of r % 4 by whole groups; rows of an odd number of 128 or 64
+// bytes already start in different halves or quarters, and the bits left do
+// the rest.  For float the second kind of read is 8 chunks of the rows r and
+// r + 4.
 template <typename T, int DP>
 __device__ __forceinline__ int swizzle(int r) {
-  if constexpr (Shape<T, DP>::kPitch % 16 != 0) return (r & 2) << 1 | ((r >> 2) & 3);
+  constexpr int kPitch = Shape<T, DP>::kPitch;
+  if constexpr (kPitch % 8 != 0) return (r >> 2) & 3;
+  if constexpr (kPitch % 16 != 0) return (r & 2) << 1 | ((r >> 2) & 3);
   if constexpr (sizeof(T) == 4) return (r & 4) << 1 | (r & 3) << 1 | ((r >> 3) & 1);
   return (r & 3) << 2 | ((r >> 2) & 3);
 }
