@@ -58,8 +58,8 @@ __device__ __forceinline__ int length_of(const CachedArgs &A, int request) {
 //
 // LDS for two blocks a CU: where a wave's two buffers of 32 keys fit half of
 // it (rows of up to 128 bytes), the next keys' loads are in flight while 32
-// are used; longer rows have one buffer, and the CU's other block loads
-// meanwhile.
+// are used; longer rows have one buffer, whose keys are loaded again as soon
+// as the scores are formed, and its values once they are added.
 template <typename T, int DP>
 struct PartPlan {
   static constexpr int kTile = Shape<T, DP>::tile_bytes(32);
@@ -104,26 +104,32 @@ __device__ __forceinline__ void cached_part(const CachedArgs &A, char *lds, int 
   Stage<T, DP, 32, 64> k_stage, v_stage;
   k_stage.set(A.chunks, [&](int r) { return r * int(A.k.row); });
   v_stage.set(A.chunks, [&](int r) { return r * int(A.v.row); });
-  auto load_tile = [&](int k0, int buffer) {
-    const unsigned to = mine0 + buffer * 2 * kTile;
-    load_rows(k_stage, k_at, A.k.row, k0, length, to);
-    load_rows(v_stage, v_at, A.v.row, k0, length, to + kTile);
+  auto load_keys = [&](int k0, int buffer) {
+    load_rows(k_stage, k_at, A.k.row, k0, length, mine0 + buffer * 2 * kTile);
+  };
+  auto load_values = [&](int k0, int buffer) {
+    load_rows(v_stage, v_at, A.v.row, k0, length, mine0 + buffer * 2 * kTile + kTile);
   };
   clear_rest<T, DP>(mine, kBuffers * 64, lane, 64, A.chunks);
 
   Sums<T, DP> out = {};
   Softmax x;
-  constexpr int kStep = kWaves * 32;
+  constexpr int kStep = kWaves * 32, kLoads = Stage<T, DP, 32, 64>::kLoads;
   const int first = begin + wave * 32;
-  if (first < end) load_tile(first, 0);
+  if (first < end) {
+    load_keys(first, 0);
+    load_values(first, 0);
+  }
   int buffer = 0;
   for (int k0 = first; k0 < end; k0 += kStep) {
-    if (kBuffers == 2 && k0 + kStep < end) {
+    const bool more = k0 + kStep < end;
+    if (kBuffers == 2 && more) {
       wait_reads();  // of the last round, from the buffer that is filled now
-      load_tile(k0 + kStep, buffer ^ 1);
-      wait_loads<S::kPitch>();  // all but the loads just issued
+      load_keys(k0 + kStep, buffer ^ 1);
+      load_values(k0 + kStep, buffer ^ 1);
+      wait_loads<2 * kLoads>();  // all but the loads just issued
     } else {
-      wait_loads<0>();
+      wait_loads<kBuffers == 2 ? 0 : kLoads>();  // (one buffer: the keys, not yet the values)
     }
     const char *k_tile = mine + buffer * 2 * kTile;
     float s[16];
@@ -131,20 +137,30 @@ __device__ __forceinline__ void cached_part(const CachedArgs &A, char *lds, int 
     read_rows<T, DP>(k, k_tile, 0);
     pin_reads();
     const f32x16 dots = dot_rows<T, DP>(k, q);
+    if (kBuffers == 1 && more) {
+      wait_reads();
+      load_keys(k0 + kStep, 0);
+    }
 #pragma unroll
     for (int r = 0; r < 16; ++r) s[r] = k0 + c_row(r, h) < limit ? dots[r] : -kInf;
     softmax_step(s, x, out, A.scale_log2);
     Weights<T> w;
     w.set(s);
+    if (kBuffers == 1) {
+      if (more)
+        wait_loads<kLoads>();  // the values: all but the next keys
+      else
+        wait_loads<0>();
+    }
     Columns<T, DP> v;
     v.read(k_tile + kTile, 0);
     pin_reads();
     v.add(out, w);
     if (kBuffers == 2) {
       buffer ^= 1;
-    } else if (k0 + kStep < end) {
+    } else if (more) {
       wait_reads();
-      load_tile(k0 + kStep, 0);
+      load_values(k0 + kStep, 0);
     }
   }
 
