@@ -218,7 +218,7 @@ __device__ __forceinline__ void cached_part(const CachedArgs &A, char *lds, int 
 
 // Rows of all requests (128 a block, 32 a wave) against one range of the
 // prefix, as in attention over a packed sequence.
-template <typename T, int DP, int kKeys>
+template <typename T, int DP>
 __device__ __forceinline__ void prefix_part(const CachedArgs &A, char *lds, int at) {
   const int head = at % A.k_heads;
   at /= A.k_heads;
@@ -236,7 +236,7 @@ __device__ __forceinline__ void prefix_part(const CachedArgs &A, char *lds, int 
   const int begin = part * A.range, end = min(A.capacity, begin + A.range);
   Sums<T, DP> out = {};
   Softmax x;
-  attend_tiles<T, DP, kKeys>(lds, q, A.k.at + head * A.k.head, A.k.row, A.v.at + head * A.v.head,
+  attend_tiles<T, DP, 64>(lds, q, A.k.at + head * A.k.head, A.k.row, A.v.at + head * A.v.head,
                              A.v.row, A.chunks, begin, end, A.capacity, end, end,
                              w0 < rows ? end : begin, A.scale_log2, x, out);
   const float sum = sum_halves(x.sum);
@@ -268,7 +268,7 @@ __global__ __launch_bounds__(kThreads, DP * sizeof(T) > 256 ? 1 : 2) void parts_
   if (int((i + 1) * shared_blocks / n) == before) {
     cached_part<T, DP, kFinal>(own, lds, int(i) - before);
   } else if constexpr (kByRows) {
-    prefix_part<T, DP, sizeof(T) == 4 ? 32 : 64>(shared, lds, before);
+    prefix_part<T, DP>(shared, lds, before);
   } else if constexpr (!kFinal) {
     cached_part<T, DP, false>(shared, lds, before);
   }
@@ -339,7 +339,7 @@ struct CachedPlan {
   bool final;    // one part: no join
 };
 
-CachedPlan plan_cached(int requests, int tokens, int capacity, int prefix, int q_heads,
+CachedPlan plan_cached(bool f32, int requests, int tokens, int capacity, int prefix, int q_heads,
                        int k_heads) {
   CachedPlan p = {};
   const int64_t group = q_heads / k_heads;
@@ -357,7 +357,14 @@ CachedPlan plan_cached(int requests, int tokens, int capacity, int prefix, int q
   p.own_parts = (capacity + p.own_range - 1) / p.own_range;
   if (prefix > 0) {
     const int64_t rows = requests * tokens * group;
-    p.by_rows = rows > 64;
+    // The prefix by rows reads it once for 128 of them, by keys for 32, but by
+    // rows most waves have none where there are few.  16,896 keys, own caches
+    // of 100, us by rows and by keys: 8 heads of 128 in bf16 32 and 31 at 64
+    // rows, 35 and 39 at 96, 54 and 97 at 256; 8 heads of 64 in f16 26 and 24,
+    // 27 and 28, 41 and 52.  Float is bound by its matrix instructions, and
+    // its tiles by rows hold half the keys: 4 heads of 64, 56 and 31 at 64
+    // rows, 94 and 76 at 256, 312 and 264 at 1024.
+    p.by_rows = !f32 && rows > 64;
     p.shared_tiles = int(p.by_rows ? (rows + 127) / 128 : (rows + 31) / 32);
     p.shared_range = range_for(int64_t(k_heads) * p.shared_tiles, prefix, p.by_rows ? 256 : 512,
                                p.by_rows ? 64 : 128);
@@ -376,7 +383,7 @@ int launch_cached(const CachedArgs &own, const CachedArgs &shared, const CachedP
       shared_blocks + int64_t(own.requests) * own.row_tiles * own.k_heads * own.parts;
   int st = check_grid(blocks, kThreads, "attention parts");
   if (st) return st;
-  constexpr int kPrefixLds = 4 * Shape<T, DP>::tile_bytes(sizeof(T) == 4 ? 32 : 64);
+  constexpr int kPrefixLds = 4 * Shape<T, DP>::tile_bytes(64);
   constexpr int kOwnLds = PartPlan<T, DP>::kLds;
   constexpr int kBothLds = kPrefixLds > kOwnLds ? kPrefixLds : kOwnLds;
   if (blocks > 0) {
@@ -385,8 +392,8 @@ int launch_cached(const CachedArgs &own, const CachedArgs &shared, const CachedP
     if (p.final)
       hipLaunchKernelGGL((parts_kernel<T, DP, false, true>), grid, block, kOwnLds, s, own, shared,
                          0);
-    else if (p.by_rows)
-      hipLaunchKernelGGL((parts_kernel<T, DP, true, false>), grid, block, kBothLds, s, own, shared,
+    else if (sizeof(T) == 2 && p.by_rows)
+      hipLaunchKernelGGL((parts_kernel<T, DP, sizeof(T) == 2, false>), grid, block, kBothLds, s, own, shared,
                          int(shared_blocks));
     else
       hipLaunchKernelGGL((parts_kernel<T, DP, false, false>), grid, block, kOwnLds, s, own,
@@ -423,8 +430,14 @@ size_t bevpool_attention_cached_scratch_bytes(int32_t requests, int32_t tokens, 
                                               int32_t prefix, int32_t q_heads, int32_t k_heads,
                                               int32_t dim) {
   if (!cached_sizes_ok(requests, tokens, capacity, prefix, q_heads, k_heads) || dim < 1) return 0;
-  return scratch_for(plan_cached(requests, tokens, capacity, prefix, q_heads, k_heads),
-                     int64_t(requests) * tokens * q_heads, dim);
+  size_t most = 0;  // of the types' plans
+  for (const bool f32 : {false, true}) {
+    const size_t need =
+        scratch_for(plan_cached(f32, requests, tokens, capacity, prefix, q_heads, k_heads),
+                    int64_t(requests) * tokens * q_heads, dim);
+    if (need > most) most = need;
+  }
+  return most;
 }
 
 int bevpool_attention_cached(const void *q, int64_t q_row, int64_t q_head, const void *k,
@@ -462,7 +475,7 @@ int bevpool_attention_cached(const void *q, int64_t q_row, int64_t q_head, const
   if (st) return st;
   if (capacity > 0 && (k_request * elem % 16 || v_request * elem % 16))
     return fail(BEVPOOL_EINVAL, "caches of requests must start at multiples of 16 bytes");
-  const CachedPlan p = plan_cached(requests, tokens, capacity, prefix, q_heads, k_heads);
+  const CachedPlan p = plan_cached(dtype == BEVPOOL_F32, requests, tokens, capacity, prefix, q_heads, k_heads);
   const size_t need = scratch_for(p, rows * q_heads, dim);
   if (scratch_bytes < need || (need > 0 && !scratch))
     return fail(BEVPOOL_ESPACE, "attention scratch: %zu bytes, %zu needed", scratch_bytes, need);
