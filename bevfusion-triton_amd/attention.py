@@ -25,6 +25,7 @@ import ctypes
 import functools
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import _lib as L
 from . import _pipeline as P
@@ -112,6 +113,7 @@ class _NormRotate(torch.autograd.Function):
                             interleaved)
 
     @staticmethod
+    @once_differentiable  # (the gradients are no functions of the graph's)
     def backward(ctx, dq_out, dk_out):
         q, k, q_weight, k_weight, positions, frequencies = ctx.saved_tensors
         tokens, q_heads, k_heads, dim, dtype, pairs, eps, interleaved = ctx.call
@@ -280,6 +282,7 @@ class _AttendPacked(torch.autograd.Function):
         return out, lse
 
     @staticmethod
+    @once_differentiable  # (the gradients are no functions of the graph's)
     def backward(ctx, dout, _):
         q, k, v, out, rest, lse, q_starts, k_starts = ctx.saved_tensors
         causal, scale = ctx.call
@@ -312,7 +315,10 @@ def attend_packed(q, k, v, q_starts, k_starts=None, *, causal=False, scale=None,
     ascending from 0, and are never read back.  With ``causal``, query j of a
     sequence sees its keys up to j + (keys - queries): the last query sees
     all.  out = softmax(scale * q k) v (scale: dim ** -0.5); a query that sees
-    no key or is in no sequence gives zeros and passes no gradient.  With
+    no key or is in no sequence gives zeros and passes no gradient.  Values of
+    other sequences and of rows of none never matter, but a key or value that is
+    not finite may reach the queries of its own sequence that do not see it
+    (weights of zero times infinity, as where all keys are multiplied).  With
     ``return_lse`` also the logarithm of each query's sum of exponentials,
     (q_total, q_heads) fp32 (-inf without keys, no gradient)."""
     for name, x in (('q', q), ('k', k), ('v', v)):

@@ -66,7 +66,7 @@ class TokenAttention(nn.Module):
         """New tokens x (requests, new, dim) at positions (requests, new, axes):
         their keys and values go into the caches (requests, capacity, k_heads,
         head_dim) behind the ``lengths`` (requests,) that are there, which
-        grow by ``new``; then the tokens attend to ``prefix``, to what their
+        grow by ``new`` (up to the capacity, which is not checked here); then the tokens attend to ``prefix``, to what their
         request's cache held and to themselves.  Returns (requests, new, dim)."""
         requests, new = x.shape[:2]
         q, k, v = self.project(x.flatten(0, 1), positions.flatten(0, 1))

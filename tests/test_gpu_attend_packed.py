@@ -333,3 +333,14 @@ def test_starts_out_of_range_stay_inside(pkg, cuda):
     want = run(pkg, cuda, case, True)
     for n in got:
         assert torch.equal(got[n], want[n]), n
+
+
+@pytest.mark.gpu
+def test_no_second_derivative(pkg, cuda):
+    """A second derivative is refused, not silently left out."""
+    q = torch.randn((6, 2, 32), device=cuda, requires_grad=True)
+    starts = torch.tensor([0, 6], device=cuda)
+    out = pkg.attend_packed(q, q, q, starts)
+    grad, = torch.autograd.grad(out.square().sum(), q, create_graph=True)
+    with pytest.raises(RuntimeError, match='once_differentiable'):
+        grad.sum().backward()

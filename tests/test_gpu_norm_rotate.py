@@ -292,3 +292,15 @@ def test_frequencies(pkg):
         index, partner, first = ref.pair_of(12, pairs, inter)
         assert sorted(i for i in index if i >= 0) == sorted(2 * list(range(sum(pairs))))
         assert all(partner[partner[d]] == d for d in range(12))
+
+
+@pytest.mark.gpu
+def test_no_second_derivative(pkg, cuda):
+    """A second derivative is refused, not silently left out."""
+    q = torch.randn((6, 2, 32), device=cuda, requires_grad=True)
+    pos = torch.arange(6, device=cuda, dtype=torch.int32)[:, None]
+    out, _ = pkg.norm_rotate(q, None, pos, pkg.axis_frequencies((16,), device=cuda),
+                             q_weight=torch.ones(32, device=cuda))
+    grad, = torch.autograd.grad(out.square().sum(), q, create_graph=True)
+    with pytest.raises(RuntimeError, match='once_differentiable'):
+        grad.sum().backward()
