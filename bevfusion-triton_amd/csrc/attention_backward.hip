@@ -43,6 +43,13 @@ __device__ __forceinline__ float row_dot(const Frags<T, DP> &a, const Frags<T, D
 // it from where a row sees few keys, so it is formed from the output before
 // its rounding (out and its rest): with out alone the error of dq and dk grew
 // by a fifth.
+//
+// Three products of 2 dim operations a pair: bound by the matrix instructions
+// and, of each tile, by the exponentials that stand between the second and the
+// third.  In bf16, 11 causal prompts of up to 4,096 over heads of 128: 336 us,
+// 930 TFLOP/s; six cameras of 2,816 tokens, heads of 80: 455 us, 800 TFLOP/s
+// (of 80 of the 96 columns that it computes).  fp32, 9 windows of 900, heads
+// of 32: 84 us.
 template <typename T, int DP, int kKeys, bool kHalves>
 __global__ __launch_bounds__(kThreads, sizeof(T) == 4 && DP > 64 ? 1 : 2) void query_grad_kernel(
     BackwardArgs A) {
@@ -197,9 +204,10 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 4 && DP > 64 ? 1 : 2) void q
 // How the keys' kernel keeps a wave's 32 keys: their K and V fragments and
 // both sums take 6 DP / 4 registers a lane in the 16-bit types (twice that in
 // float).  For heads of up to 192 bytes that leaves room for two blocks a CU,
-// which hide each other's waits.  For longer heads dk and dv are two launches
-// of half the sums each: five products in place of four, but 10 MFLOP a
-// microsecond and CU at two blocks in place of 4 at one (heads of 128, bf16).
+// which hide each other's waits; for longer heads dk and dv are two launches
+// of half the sums each: five products in place of four, at two blocks in
+// place of one.  In bf16, together and apart: heads of 128, 1,150 us and 431 +
+// 341; heads of 80, 700 us and 568 + 458.
 template <typename T, int DP, bool kHalves>
 struct KeyPlan {
   static constexpr int kKeys = (kHalves ? 2 : 4) * kWaveRows;
@@ -217,7 +225,10 @@ struct KeyPlan {
 };
 
 // Walks over the rows are cut where there are few of them: `splits` blocks a
-// key tile at most, each with about `steps` tiles of rows or more.
+// key tile at most, each with about `steps` tiles of rows or more.  Backward in
+// bf16, uncut and cut: 11 causal prompts of up to 4,096, 16 heads over 4 of
+// 128 (forward too) 1,657 and 1,409 us; one of 8,192, 8 heads over 1 of 128,
+// 2,813 and 843 us; one of 4,096 without a mask, 8 over 2 of 64, 359 and 165.
 struct Splits {
   int most, steps;
   float *sums;  // [key tile, head][split][dk, dv][32 keys][register][lane]
@@ -254,6 +265,13 @@ __device__ __forceinline__ bool key_tile_at(const BackwardArgs &A, int index, in
 // of the group) in tiles of 32, from the last to the first that sees one of
 // its keys: blocks of one sequence start together there, and find each
 // other's rows in L2.
+//
+// Bound by the matrix instructions, with the reads of Q and dout from LDS (as
+// rows for one product, as columns for the next) next to them.  In bf16, six
+// cameras of 2,816 tokens, heads of 80, dk and dv together: 700 us, 700
+// TFLOP/s; 11 causal prompts of up to 4,096, 16 heads over 4 of 128: dk 431 us,
+// 725 TFLOP/s, dv 341 us, 610 TFLOP/s, sums of the cuts 26 us.  fp32, 9
+// windows of 900, heads of 32: 112 us.
 template <typename T, int DP, bool kHalves, bool kDk, bool kDv>
 __global__ __launch_bounds__(kThreads, (KeyPlan<T, DP, kHalves>::kBlocksPerCu)) void
 key_grad_kernel(BackwardArgs A, Splits splits) {

