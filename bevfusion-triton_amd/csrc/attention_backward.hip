@@ -44,9 +44,9 @@ __device__ __forceinline__ float row_dot(const Frags<T, DP> &a, const Frags<T, D
 // its rounding (out and its rest): with out alone the error of dq and dk grew
 // by a fifth.
 //
-// Three products of 2 dim operations a pair: bound by the matrix instructions
-// and, of each tile, by the exponentials that stand between the second and the
-// third.  In bf16, 11 causal prompts of up to 4,096 over heads of 128: 336 us,
+// Three products of 2 dim operations a pair.  The matrix instructions are busy
+// in half of the cycles: two waves a SIMD, and of each block of 32 keys the
+// exponentials stand between the second product and the third.  In bf16, 11 causal prompts of up to 4,096 over heads of 128: 336 us,
 // 930 TFLOP/s; six cameras of 2,816 tokens, heads of 80: 455 us, 800 TFLOP/s
 // (of 80 of the 96 columns that it computes).  fp32, 9 windows of 900, heads
 // of 32: 84 us.
@@ -266,8 +266,10 @@ __device__ __forceinline__ bool key_tile_at(const BackwardArgs &A, int index, in
 // its keys: blocks of one sequence start together there, and find each
 // other's rows in L2.
 //
-// Bound by the matrix instructions, with the reads of Q and dout from LDS (as
-// rows for one product, as columns for the next) next to them.  In bf16, six
+// The matrix instructions are busy in 35 to 45% of the cycles: two waves a
+// SIMD, each a chain from product to exponential to product, with Q and dout
+// read from LDS twice (as rows for one product, as columns for the next) and a
+// barrier a tile.  In bf16, six
 // cameras of 2,816 tokens, heads of 80, dk and dv together: 700 us, 700
 // TFLOP/s; 11 causal prompts of up to 4,096, 16 heads over 4 of 128: dk 431 us,
 // 725 TFLOP/s, dv 341 us, 610 TFLOP/s, sums of the cuts 26 us.  fp32, 9
