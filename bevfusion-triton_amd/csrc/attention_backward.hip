@@ -24,7 +24,7 @@ using bevpool_host::fail;
 using bevpool_host::LaunchScope;
 
 struct BackwardArgs : PackedArgs {
-  float2 *stats;  // (tokens, heads): L in units of log 2, and D
+  float2 *stats;  // (tokens, heads): L in units of log 2, and -D
 };
 
 // A lane's part of the dot product of two rows.
@@ -108,7 +108,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 4 && DP > 64 ? 1 : 2) void q
   }
   settle(stat);
   const float lse2 = stat[0], delta = stat[1];
-  if (valid && h == 0 && half == 0) A.stats[stat_at] = make_float2(lse2, delta);
+  if (valid && h == 0 && half == 0) A.stats[stat_at] = make_float2(lse2, -delta);
   const char *k_at = A.k.at + seq.k0 * A.k.row + head * A.k.head;
   const char *v_at = A.v.at + seq.k0 * A.v.row + head * A.v.head;
   const unsigned lds0 = lds_address(lds);
@@ -213,7 +213,7 @@ struct KeyPlan {
   static constexpr int kKeys = (kHalves ? 2 : 4) * kWaveRows;
   static constexpr bool kApart = DP * sizeof(T) > 192;
   static constexpr int kBlocksPerCu = DP * sizeof(T) > 320 ? 1 : 2;
-  // Buffers of Q and dout rows, and behind them the rows' L and D in pairs.
+  // Buffers of Q and dout rows, and behind them L of 32 rows and their -D.
   static constexpr int kRows = sizeof(T) == 4 && !kHalves ? 32 : 64;  // of a tile
   static constexpr int kTile = Shape<T, DP>::tile_bytes(kRows);
   static constexpr int kBuffers = kRows == 32 ? 3 : 2;
@@ -341,12 +341,13 @@ key_grad_kernel(BackwardArgs A, Splits splits) {
       q_stage.load(q_base, to, [&](int r) { return place(min(skip + r, last), A.q); });
       g_stage.load(g_base, to + kTile, [&](int r) { return place(min(skip + r, last), A.dout); });
     }
-    // L and D of 32 rows, a lane each (by every wave: all count the same loads)
+    // L of 32 rows and their -D, a lane each (by every wave: all count the same
+    // loads)
 #pragma unroll
     for (int j = 0; j < kRows / 32; ++j) {
-      const int row = min(skip + 32 * j + (lane >> 1), last), i = A.group.div(row);
+      const int row = min(skip + 32 * j + c, last), i = A.group.div(row);
       load_to_lds4(reinterpret_cast<const char *>(A.stats + stat0 + int64_t(i0) * A.q_heads),
-                   unsigned((i * A.q_heads + row - i * heads) * 2 + (lane & 1)) * 4,
+                   unsigned((i * A.q_heads + row - i * heads) * 2 + h) * 4,
                    tiles0 + kBuffers * 2 * kTile + (buffer * kRows + 32 * j) * 8);
     }
   };
@@ -380,18 +381,33 @@ key_grad_kernel(BackwardArgs A, Splits splits) {
 #pragma unroll
     for (int b = 0; b < kMine; ++b) {
       // Four fragments are read while four are in use.
-      f32x16 dots = {}, dp = {};
+      f32x16 dots = {}, dp;
+      const float *stat = stat_row + 2 * mine + 64 * b + 4 * h;  // of rows 8 i + 4 h on: 8 i more
       Piece<T> x[2];
       constexpr int kPieces = (kSteps + 3) / 4;  // of a row's fragments
+      // the first columns are read before the exponentials (dk alone, of long
+      // heads, has no registers for them)
+      constexpr bool kEarly = sizeof(T) == 2 && kDv;
+      constexpr int kProducts = (kDk ? 2 : 1) * kPieces;
       read_piece<T, DP, 4>(x[0], q_tile, mine + 32 * b, 0, at_lane);
 #pragma unroll
-      for (int n = 0; n < (kDk ? 2 : 1) * kPieces; ++n) {
+      for (int n = 0; n < kProducts; ++n) {
         Piece<T> &now = x[n & 1], &next = x[(n + 1) & 1];
         const int s0 = n % kPieces * 4, s1 = (n + 1) % kPieces * 4;
         if (n + 1 < kPieces)
           read_piece<T, DP, 4>(next, q_tile, mine + 32 * b, s1, at_lane);
         else if (kDk && n + 1 < 2 * kPieces)
           read_piece<T, DP, 4>(next, g_tile, mine + 32 * b, s1, at_lane);
+        else if constexpr (kEarly)
+          read_column_piece<T, DP>(next, g_tile, mine + 32 * b, 0, at_lane);
+        if (kDk && n == kPieces - 1) {  // the sums of dP begin at -D
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const f32x4 d = *reinterpret_cast<const f32x4 *>(stat + 32 + 8 * i);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) dp[4 * i + j] = d[j];
+          }
+        }
         pin_reads();
 #pragma unroll
         for (int i = 0; i < 4; ++i)
@@ -406,16 +422,12 @@ key_grad_kernel(BackwardArgs A, Splits splits) {
       float p[16], ds[16];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        // L and D of four rows
-        const f32x4 s01 = *reinterpret_cast<const f32x4 *>(stat_row + 2 * mine + 64 * b + 16 * i + 8 * h);
-        const f32x4 s23 = *reinterpret_cast<const f32x4 *>(stat_row + 2 * mine + 64 * b + 16 * i + 8 * h + 4);
-        const float l[4] = {s01[0], s01[2], s23[0], s23[2]};
-        const float d[4] = {s01[1], s01[3], s23[1], s23[3]};
+        const f32x4 l = *reinterpret_cast<const f32x4 *>(stat + 8 * i);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           const int r = 4 * i + j;
           p[r] = exp2_fast(fmaf(dots[r], A.scale_log2, -l[j]));
-          ds[r] = kDk ? p[r] * (dp[r] - d[j]) : 0.f;
+          ds[r] = kDk ? p[r] * dp[r] : 0.f;
           if (masked) {
             const int at = r_mine + 32 * b + c_row(r, h);
             if (at < from || at >= rows) p[r] = ds[r] = 0.f;
@@ -434,11 +446,13 @@ key_grad_kernel(BackwardArgs A, Splits splits) {
       } else {
         constexpr int kColumns = (kBlocks + 1) / 2;  // pieces of 64 columns
         constexpr int kFirst = kDv ? 0 : kColumns, kLast = kDk ? 2 * kColumns : kColumns;
-        pin_reads();
-        read_column_piece<T, DP>(x[0], kDv ? g_tile : q_tile, mine + 32 * b, 0, at_lane);
+        if constexpr (!kEarly) {
+          pin_reads();
+          read_column_piece<T, DP>(x[kProducts & 1], q_tile, mine + 32 * b, 0, at_lane);
+        }
 #pragma unroll
         for (int n = kFirst; n < kLast; ++n) {
-          Piece<T> &now = x[(n - kFirst) & 1], &next = x[(n - kFirst + 1) & 1];
+          Piece<T> &now = x[(kProducts + n - kFirst) & 1], &next = x[(kProducts + n - kFirst + 1) & 1];
           if (n + 1 < kLast)
             read_column_piece<T, DP>(next, n + 1 < kColumns ? g_tile : q_tile, mine + 32 * b,
                                      2 * ((n + 1) % kColumns), at_lane);
