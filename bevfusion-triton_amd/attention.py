@@ -242,8 +242,8 @@ def _check_heads(q, k, v):
 
 def _check_scale(scale, dim):
     scale = dim ** -0.5 if scale is None else float(scale)
-    if not 0.0 < scale < float('inf'):
-        raise ValueError('scale must be positive and finite.')
+    if not 1e-30 <= scale < float('inf'):
+        raise ValueError('scale must be positive (1e-30 or more) and finite.')
     return scale
 
 

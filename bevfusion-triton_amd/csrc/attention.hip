@@ -155,8 +155,9 @@ int check_packed(PackedArgs &A, int dtype, int64_t q_total, int64_t k_total, int
                 k_heads);
   if (dim < 8 || dim > 128 || dim % 8)
     return fail(BEVPOOL_EINVAL, "head size %d: must be a multiple of 8 up to 128", dim);
-  if (!(scale > 0.f) || !(scale < 3e38f))
-    return fail(BEVPOOL_EINVAL, "scale must be positive and finite");
+  // (the gradients divide L by the scale)
+  if (!(scale >= 1e-30f) || !(scale < 3e38f))
+    return fail(BEVPOOL_EINVAL, "scale must be positive (1e-30 or more) and finite");
   const int64_t group = q_heads / k_heads;
   // (packed row numbers, and their quotients by the group, in 32 bits)
   if (q_total * group * group >= (int64_t(1) << 31) ||

@@ -24,7 +24,7 @@ using bevpool_host::fail;
 using bevpool_host::LaunchScope;
 
 struct BackwardArgs : PackedArgs {
-  float2 *stats;  // (tokens, heads): L in units of log 2, and -D
+  float2 *stats;  // (tokens, heads): -L / scale, where the sums of q k begin, and -D
 };
 
 // A lane's part of the dot product of two rows.
@@ -38,7 +38,7 @@ __device__ __forceinline__ float row_dot(const Frags<T, DP> &a, const Frags<T, D
   return sum;
 }
 
-// dq: rows and tiles as in the forward.  Also writes L / log 2 and D of its
+// dq: rows and tiles as in the forward.  Also writes -L / scale and -D of its
 // rows, for the keys' kernels.  D is a small difference of what dS subtracts
 // it from where a row sees few keys, so it is formed from the output before
 // its rounding (out and its rest): with out alone the error of dq and dk grew
@@ -108,7 +108,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 4 && DP > 64 ? 1 : 2) void q
   }
   settle(stat);
   const float lse2 = stat[0], delta = stat[1];
-  if (valid && h == 0 && half == 0) A.stats[stat_at] = make_float2(lse2, -delta);
+  if (valid && h == 0 && half == 0) A.stats[stat_at] = make_float2(-lse2 / A.scale_log2, -delta);
   const char *k_at = A.k.at + seq.k0 * A.k.row + head * A.k.head;
   const char *v_at = A.v.at + seq.k0 * A.v.row + head * A.v.head;
   const unsigned lds0 = lds_address(lds);
@@ -206,14 +206,16 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 4 && DP > 64 ? 1 : 2) void q
 // float).  For heads of up to 192 bytes that leaves room for two blocks a CU,
 // which hide each other's waits; for longer heads dk and dv are two launches
 // of half the sums each: five products in place of four, at two blocks in
-// place of one.  In bf16, together and apart: heads of 128, 1,150 us and 431 +
-// 341; heads of 80, 700 us and 568 + 458.
+// place of one.  In bf16, together and apart, before the exponentials ran
+// beside products: heads of 128, 1,150 us and 431 + 341; heads of 80, 700 us
+// and 568 + 458.
 template <typename T, int DP, bool kHalves>
 struct KeyPlan {
   static constexpr int kKeys = (kHalves ? 2 : 4) * kWaveRows;
   static constexpr bool kApart = DP * sizeof(T) > 192;
   static constexpr int kBlocksPerCu = DP * sizeof(T) > 320 ? 1 : 2;
-  // Buffers of Q and dout rows, and behind them L of 32 rows and their -D.
+  // Buffers of Q and dout rows, and behind them the first statistic of 32 rows
+  // and their second.
   static constexpr int kRows = sizeof(T) == 4 && !kHalves ? 32 : 64;  // of a tile
   static constexpr int kTile = Shape<T, DP>::tile_bytes(kRows);
   static constexpr int kBuffers = kRows == 32 ? 3 : 2;
@@ -266,14 +268,15 @@ __device__ __forceinline__ bool key_tile_at(const BackwardArgs &A, int index, in
 // its keys: blocks of one sequence start together there, and find each
 // other's rows in L2.
 //
-// The matrix instructions are busy in 35 to 45% of the cycles: two waves a
-// SIMD, each a chain from product to exponential to product, with Q and dout
-// read from LDS twice (as rows for one product, as columns for the next) and a
-// barrier a tile.  In bf16, six
-// cameras of 2,816 tokens, heads of 80, dk and dv together: 700 us, 700
-// TFLOP/s; 11 causal prompts of up to 4,096, 16 heads over 4 of 128: dk 431 us,
-// 725 TFLOP/s, dv 341 us, 610 TFLOP/s, sums of the cuts 26 us.  fp32, 9
-// windows of 900, heads of 32: 112 us.
+// Two waves a SIMD, each a chain from product to exponential to product, with Q
+// and dout read from LDS twice (as rows for one product, as columns for the
+// next) and a barrier a tile.  The exponentials run beside the products of dP:
+// with the sums of q k begun at -L / scale they wait for no read, and the mask
+// is apart from them, with one branch for all.  In bf16, six cameras of 2,816
+// tokens, heads of 80, dk and dv together: 600 us, 810 TFLOP/s (before, 719);
+// 11 causal prompts of up to 4,096, 16 heads over 4 of 128: dk 375 us, 830
+// TFLOP/s, dv 295 us, 700 TFLOP/s (446 and 351), sums of the cuts 26 us.  fp32,
+// 9 windows of 900, heads of 32: 108 us.
 template <typename T, int DP, bool kHalves, bool kDk, bool kDv>
 __global__ __launch_bounds__(kThreads, (KeyPlan<T, DP, kHalves>::kBlocksPerCu)) void
 key_grad_kernel(BackwardArgs A, Splits splits) {
@@ -341,8 +344,8 @@ key_grad_kernel(BackwardArgs A, Splits splits) {
       q_stage.load(q_base, to, [&](int r) { return place(min(skip + r, last), A.q); });
       g_stage.load(g_base, to + kTile, [&](int r) { return place(min(skip + r, last), A.dout); });
     }
-    // L of 32 rows and their -D, a lane each (by every wave: all count the same
-    // loads)
+    // both statistics of 32 rows, a lane each (by every wave: all count the
+    // same loads)
 #pragma unroll
     for (int j = 0; j < kRows / 32; ++j) {
       const int row = min(skip + 32 * j + c, last), i = A.group.div(row);
@@ -381,14 +384,24 @@ key_grad_kernel(BackwardArgs A, Splits splits) {
 #pragma unroll
     for (int b = 0; b < kMine; ++b) {
       // Four fragments are read while four are in use.
-      f32x16 dots = {}, dp;
+      f32x16 dots, dp;
       const float *stat = stat_row + 2 * mine + 64 * b + 4 * h;  // of rows 8 i + 4 h on: 8 i more
+      // q k - L / scale and dP - D: the sums begin at what is taken off
+      auto begin_at = [&](f32x16 &sums, const float *from) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const f32x4 s = *reinterpret_cast<const f32x4 *>(from + 8 * i);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) sums[4 * i + j] = s[j];
+        }
+      };
       Piece<T> x[2];
       constexpr int kPieces = (kSteps + 3) / 4;  // of a row's fragments
       // the first columns are read before the exponentials (dk alone, of long
       // heads, has no registers for them)
       constexpr bool kEarly = sizeof(T) == 2 && kDv;
       constexpr int kProducts = (kDk ? 2 : 1) * kPieces;
+      begin_at(dots, stat);
       read_piece<T, DP, 4>(x[0], q_tile, mine + 32 * b, 0, at_lane);
 #pragma unroll
       for (int n = 0; n < kProducts; ++n) {
@@ -400,14 +413,7 @@ key_grad_kernel(BackwardArgs A, Splits splits) {
           read_piece<T, DP, 4>(next, g_tile, mine + 32 * b, s1, at_lane);
         else if constexpr (kEarly)
           read_column_piece<T, DP>(next, g_tile, mine + 32 * b, 0, at_lane);
-        if (kDk && n == kPieces - 1) {  // the sums of dP begin at -D
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const f32x4 d = *reinterpret_cast<const f32x4 *>(stat + 32 + 8 * i);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) dp[4 * i + j] = d[j];
-          }
-        }
+        if (kDk && n == kPieces - 1) begin_at(dp, stat + 32);
         pin_reads();
 #pragma unroll
         for (int i = 0; i < 4; ++i)
@@ -421,17 +427,15 @@ key_grad_kernel(BackwardArgs A, Splits splits) {
       }
       float p[16], ds[16];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const f32x4 l = *reinterpret_cast<const f32x4 *>(stat + 8 * i);
+      for (int r = 0; r < 16; ++r) {
+        p[r] = exp2_fast(dots[r] * A.scale_log2);
+        ds[r] = kDk ? p[r] * dp[r] : 0.f;
+      }
+      if (masked) {  // (apart from the exponentials, which so run beside the products of dP)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int r = 4 * i + j;
-          p[r] = exp2_fast(fmaf(dots[r], A.scale_log2, -l[j]));
-          ds[r] = kDk ? p[r] * dp[r] : 0.f;
-          if (masked) {
-            const int at = r_mine + 32 * b + c_row(r, h);
-            if (at < from || at >= rows) p[r] = ds[r] = 0.f;
-          }
+        for (int r = 0; r < 16; ++r) {
+          const int at = r_mine + 32 * b + c_row(r, h);
+          if (at < from || at >= rows) p[r] = ds[r] = 0.f;
         }
       }
       Weights<T> w, u;

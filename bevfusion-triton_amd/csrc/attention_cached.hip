@@ -467,8 +467,8 @@ int bevpool_attention_cached(const void *q, int64_t q_row, int64_t q_head, const
                 requests, tokens, capacity, prefix, q_heads, k_heads);
   if (dim < 8 || dim > 128 || dim % 8)
     return fail(BEVPOOL_EINVAL, "head size %d: must be a multiple of 8 up to 128", dim);
-  if (!(scale > 0.f) || !(scale < 3e38f))
-    return fail(BEVPOOL_EINVAL, "scale must be positive and finite");
+  if (!(scale >= 1e-30f) || !(scale < 3e38f))
+    return fail(BEVPOOL_EINVAL, "scale must be positive (1e-30 or more) and finite");
   if (requests == 0) return BEVPOOL_OK;
   if (!lengths) return fail(BEVPOOL_EINVAL, "lengths: null");
   const int elem = dtype == BEVPOOL_F32 ? 4 : 2;
