@@ -24,7 +24,9 @@ using bevpool_host::fail;
 using bevpool_host::LaunchScope;
 
 struct BackwardArgs : PackedArgs {
-  float2 *stats;  // (tokens, heads): -L / scale, where the sums of q k begin, and -D
+  // (tokens, heads): -L / scale, where the sums of q k begin, and -D.  In fp32
+  // -L in units of log 2: sums begun so far from zero lose a bit there.
+  float2 *stats;
 };
 
 // A lane's part of the dot product of two rows.
@@ -39,7 +41,7 @@ __device__ __forceinline__ float row_dot(const Frags<T, DP> &a, const Frags<T, D
 }
 
 // dq: rows and tiles as in the forward.  Also writes -L / scale and -D of its
-// rows, for the keys' kernels.  D is a small difference of what dS subtracts
+// rows (in fp32 -L), for the keys' kernels.  D is a small difference of what dS subtracts
 // it from where a row sees few keys, so it is formed from the output before
 // its rounding (out and its rest): with out alone the error of dq and dk grew
 // by a fifth.
@@ -58,6 +60,10 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 4 && DP > 64 ? 1 : 2) void q
   constexpr int kTile = S::tile_bytes(kKeys);  // buffers: K0 V0 K1 V1
   constexpr int kRows = (kHalves ? 2 : 4) * kWaveRows;
   constexpr int kMine = kHalves ? 1 : kKeys / 32;  // blocks of 32 keys a wave takes of a tile
+  // dP's sums begin at -D (16 registers of it) but for the longest heads, which
+  // have none left: whole backward in 16 bits 474 us begun at zero and 461 at
+  // -D for heads of 32, 1,064 and 1,053 for 96, but 945 and 957 for 128.
+  constexpr bool kBegin = DP * sizeof(T) <= 192;
   const int head = blockIdx.x % A.k_heads;
   const int index = A.tiles - 1 - int(blockIdx.x / A.k_heads);
   int first;
@@ -108,7 +114,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 4 && DP > 64 ? 1 : 2) void q
   }
   settle(stat);
   const float lse2 = stat[0], delta = stat[1];
-  if (valid && h == 0 && half == 0) A.stats[stat_at] = make_float2(-lse2 / A.scale_log2, -delta);
+  if (valid && h == 0 && half == 0) A.stats[stat_at] = make_float2(sizeof(T) == 4 ? -lse2 : -lse2 / A.scale_log2, -delta);
   const char *k_at = A.k.at + seq.k0 * A.k.row + head * A.k.head;
   const char *v_at = A.v.at + seq.k0 * A.v.row + head * A.v.head;
   const unsigned lds0 = lds_address(lds);
@@ -141,7 +147,9 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 4 && DP > 64 ? 1 : 2) void q
       // Four fragments are read while four are in use.
       constexpr int kSteps = S::kSteps, kPieces = (kSteps + 3) / 4;
       constexpr int kColumns = (S::kBlocks + 1) / 2;  // pieces of 64
-      f32x16 dots = {}, dp = {};
+      f32x16 dots = {}, dp;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) dp[r] = kBegin ? -delta : 0.f;
       Piece<T> x[2];
       read_piece<T, DP, 4>(x[0], k_tile, mine + 32 * b, 0, at_lane);
 #pragma unroll
@@ -166,7 +174,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 4 && DP > 64 ? 1 : 2) void q
       float p[16];
 #pragma unroll
       for (int r = 0; r < 16; ++r)
-        p[r] = exp2_fast(fmaf(dots[r], A.scale_log2, -lse2)) * (dp[r] - delta);
+        p[r] = exp2_fast(fmaf(dots[r], A.scale_log2, -lse2)) * (kBegin ? dp[r] : dp[r] - delta);
       if (masked) {
 #pragma unroll
         for (int r = 0; r < 16; ++r)
@@ -401,7 +409,14 @@ key_grad_kernel(BackwardArgs A, Splits splits) {
       // heads, has no registers for them)
       constexpr bool kEarly = sizeof(T) == 2 && kDv;
       constexpr int kProducts = (kDk ? 2 : 1) * kPieces;
-      begin_at(dots, stat);
+      float l[16];
+      if constexpr (sizeof(T) == 4) {
+        dots = {};
+#pragma unroll
+        for (int i = 0; i < 16; ++i) l[i] = stat[i / 4 * 8 + i % 4];
+      } else {
+        begin_at(dots, stat);
+      }
       read_piece<T, DP, 4>(x[0], q_tile, mine + 32 * b, 0, at_lane);
 #pragma unroll
       for (int n = 0; n < kProducts; ++n) {
@@ -428,7 +443,8 @@ key_grad_kernel(BackwardArgs A, Splits splits) {
       float p[16], ds[16];
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
-        p[r] = exp2_fast(dots[r] * A.scale_log2);
+        p[r] = exp2_fast(sizeof(T) == 4 ? fmaf(dots[r], A.scale_log2, l[r])
+                                        : dots[r] * A.scale_log2);
         ds[r] = kDk ? p[r] * dp[r] : 0.f;
       }
       if (masked) {  // (apart from the exponentials, which so run beside the products of dP)
