@@ -49,9 +49,9 @@ __device__ __forceinline__ float row_dot(const Frags<T, DP> &a, const Frags<T, D
 // Three products of 2 dim operations a pair.  The matrix instructions are busy
 // in half of the cycles: two waves a SIMD, and of each block of 32 keys the
 // exponentials stand between the second product and the third.  In bf16, 11 causal prompts of up to 4,096 over heads of 128: 336 us,
-// 930 TFLOP/s; six cameras of 2,816 tokens, heads of 80: 455 us, 800 TFLOP/s
+// 930 TFLOP/s; six cameras of 2,816 tokens, heads of 80: 465 us, 790 TFLOP/s
 // (of 80 of the 96 columns that it computes).  fp32, 9 windows of 900, heads
-// of 32: 84 us.
+// of 32: 81 us.
 template <typename T, int DP, int kKeys, bool kHalves>
 __global__ __launch_bounds__(kThreads, sizeof(T) == 4 && DP > 64 ? 1 : 2) void query_grad_kernel(
     BackwardArgs A) {
