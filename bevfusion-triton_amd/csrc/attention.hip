@@ -39,14 +39,11 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 4 && DP > 64 ? 1 : 2) void p
   const int head = blockIdx.x % A.k_heads;
   // late tiles, the long ones of a causal sequence, start first
   const int index = A.tiles - 1 - int(blockIdx.x / A.k_heads);
-  int first;
-  const int which = find_sequence(A.q_starts, A.sequences, A.q_total, A.group.size, kRows, index,
-                                  &first);
-  Sequence seq = sequence_at(A.q_starts, A.k_starts, which, A.sequences, A.q_total, A.k_total);
-  if (which == A.sequences) seq.nq = A.q_total - seq.q0;  // rows of no sequence: no keys
-  const int rows = seq.nq * A.group.size;
-  const int r0 = (index - first) * kRows;
-  if (r0 >= rows) return;
+  const sequences::RowTile at_rows =
+      sequences::row_tile(starts_of(A), A.group.size, kRows, index, Wave{});
+  if (!at_rows.on) return;
+  const Sequence seq = at_rows.seq;
+  const int rows = at_rows.rows, r0 = at_rows.r0;
 
   const int wave = wave_id() / (kHalves ? 2 : 1), c = lane_id() & 31, h = lane_id() >> 5;
   const int row = r0 + wave * kWaveRows + c;

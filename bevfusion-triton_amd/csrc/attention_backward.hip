@@ -66,14 +66,11 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 4 && DP > 64 ? 1 : 2) void q
   constexpr bool kBegin = DP * sizeof(T) <= 192;
   const int head = blockIdx.x % A.k_heads;
   const int index = A.tiles - 1 - int(blockIdx.x / A.k_heads);
-  int first;
-  const int which = find_sequence(A.q_starts, A.sequences, A.q_total, A.group.size, kRows, index,
-                                  &first);
-  Sequence seq = sequence_at(A.q_starts, A.k_starts, which, A.sequences, A.q_total, A.k_total);
-  if (which == A.sequences) seq.nq = A.q_total - seq.q0;  // rows of no sequence: no keys
-  const int rows = seq.nq * A.group.size;
-  const int r0 = (index - first) * kRows;
-  if (r0 >= rows) return;
+  const sequences::RowTile at_rows =
+      sequences::row_tile(starts_of(A), A.group.size, kRows, index, Wave{});
+  if (!at_rows.on) return;
+  const Sequence seq = at_rows.seq;
+  const int rows = at_rows.rows, r0 = at_rows.r0;
 
   const int lane = lane_id(), c = lane & 31, h = lane >> 5;
   const int wave = wave_id() / (kHalves ? 2 : 1), half = kHalves ? wave_id() % 2 : 0;
@@ -247,30 +244,6 @@ struct Splits {
   }
 };
 
-// The key tile that a block works on.
-struct KeyTile {
-  Sequence seq;
-  int kb;        // first key
-  int begin;     // first row that sees one of its keys
-  int rows, tiles;
-};
-template <int kKeys>
-__device__ __forceinline__ bool key_tile_at(const BackwardArgs &A, int index, int tile_rows,
-                                            KeyTile &t) {
-  int first;
-  const int which = find_sequence(A.k_starts, A.sequences, A.k_total, 1, kKeys, index, &first);
-  t.seq = sequence_at(A.q_starts, A.k_starts, which, A.sequences, A.q_total, A.k_total);
-  if (which == A.sequences) t.seq.nk = A.k_total - t.seq.k0;  // keys of no sequence: no queries
-  t.kb = (index - first) * kKeys;
-  t.rows = t.seq.nq * A.group.size;
-  // key j is seen by the queries from j - (nk - nq) on
-  t.begin = A.causal
-                ? max(0, min(t.kb - (t.seq.nk - t.seq.nq), t.seq.nq)) * A.group.size
-                : 0;
-  t.tiles = (t.rows - t.begin + tile_rows - 1) / tile_rows;
-  return t.kb < t.seq.nk;
-}
-
 // dk and dv: a wave owns 32 keys and walks the sequence's rows (query, head
 // of the group) in tiles of 32, from the last to the first that sees one of
 // its keys: blocks of one sequence start together there, and find each
@@ -297,8 +270,9 @@ key_grad_kernel(BackwardArgs A, Splits splits) {
   // the cuts of the long walks first
   const int index = int(blockIdx.x / A.k_heads) % A.tiles;
   const int split = splits.most - 1 - int(blockIdx.x / A.k_heads) / A.tiles;
-  KeyTile tile;
-  if (!key_tile_at<Plan::kKeys>(A, index, kRows, tile)) return;
+  const sequences::KeyTile tile = sequences::key_tile(starts_of(A), A.group.size, A.causal,
+                                                      Plan::kKeys, kRows, index, Wave{});
+  if (!tile.on) return;
   const int n_splits = splits.of(tile.tiles);
   if (split >= n_splits) return;
   const Sequence seq = tile.seq;
@@ -527,8 +501,9 @@ __global__ __launch_bounds__(64) void key_sum_kernel(BackwardArgs A, Splits spli
   const int n = blockIdx.x & 1, wave = (blockIdx.x >> 1) % kParts;
   const int head = blockIdx.x / (2 * kParts) % A.k_heads;
   const int index = blockIdx.x / (2 * kParts) / A.k_heads;
-  KeyTile tile;
-  if (!key_tile_at<Plan::kKeys>(A, index, Plan::kRows, tile)) return;
+  const sequences::KeyTile tile = sequences::key_tile(starts_of(A), A.group.size, A.causal,
+                                                      Plan::kKeys, Plan::kRows, index, Wave{});
+  if (!tile.on) return;
   const int n_splits = splits.of(tile.tiles);
   if (n_splits == 1) return;
   const int lane = lane_id();

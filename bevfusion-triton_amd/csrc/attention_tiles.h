@@ -28,6 +28,7 @@
 #include <stdint.h>
 
 #include "bevpool.h"
+#include "sequences.h"
 
 namespace attention {
 
@@ -629,69 +630,18 @@ constexpr int kFullBlocks = 512;
 template <typename T, int DP>
 constexpr bool kMayHalve = DP * int(sizeof(T)) <= 256;  // (a tile of 64 in LDS, twice)
 
-// n / group for n < 2^32 / group.
-struct Group {
-  int size;
-  uint32_t magic;  // ceil(2^32 / size); 0 for 1
-  __device__ __forceinline__ int div(int n) const {
-    return magic ? int(__umulhi(uint32_t(n), magic)) : n;
+// The wave's side of the search over the starts (sequences.h).
+struct Wave {
+  template <typename Ok>
+  __device__ __forceinline__ int count(Ok ok) const {
+    return __popcll(__ballot(ok(lane_id())));
   }
+  __device__ __forceinline__ int uniform(int v) const { return __builtin_amdgcn_readfirstlane(v); }
 };
 
-inline Group make_group(int size) {
-  return {size, size == 1 ? 0u : uint32_t(((uint64_t(1) << 32) + size - 1) / size)};
-}
-
-struct Sequence {
-  int q0, nq, k0, nk;
-};
-
-// starts[i] kept within the rows there are, whatever the array holds.
-__device__ __forceinline__ int start_at(const int32_t *starts, int i, int total) {
-  if (i <= 0) return 0;
-  const int v = starts[i];
-  return v < 0 ? 0 : v > total ? total : v;
-}
-
-__device__ __forceinline__ Sequence sequence_at(const int32_t *q_starts, const int32_t *k_starts,
-                                                int i, int n, int tq, int tk) {
-  Sequence s;
-  s.q0 = start_at(q_starts, i, tq);
-  s.k0 = start_at(k_starts, i, tk);
-  s.nq = i < n ? start_at(q_starts, i + 1, tq) - s.q0 : 0;
-  s.nk = i < n ? start_at(k_starts, i + 1, tk) - s.k0 : 0;
-  if (s.nq < 0) s.nq = 0;
-  if (s.nk < 0) s.nk = 0;
-  return s;
-}
-
-// Tiles of `tile` rows over sequences of starts[i + 1] - starts[i] tokens of
-// `per` rows each, without a plan: sequence i's tiles are numbered from
-// starts[i] * per / tile + i.  No two sequences' numbers meet, since
-// floor(a) + ceil(b) <= floor(a + b) + 1, and all are below
-// total * per / tile + n + 1, which the host knows.  Sequence n stands for
-// the rows after the last one, which belong to none.  Finds the sequence
-// whose numbers `index` is among; its first number goes to `first`.  Each
-// round narrows the range 64 times, so that any number of sequences takes a
-// few loads.  The whole wave calls it.
-__device__ __forceinline__ int find_sequence(const int32_t *starts, int n, int total, int per,
-                                             int tile, int index, int *first) {
-  int low = 0, count = n + 1;
-  for (;;) {
-    const int step = (count + 63) / 64;
-    const int at = low + lane_id() * step;
-    const bool ok = lane_id() * step < count &&
-                    int(int64_t(start_at(starts, at, total)) * per / tile) + at <= index;
-    const int taken = __popcll(__ballot(ok));
-    const int i = taken > 0 ? taken - 1 : 0;
-    low += i * step;
-    count = count - i * step < step ? count - i * step : step;
-    if (step == 1) break;
-  }
-  low = __builtin_amdgcn_readfirstlane(low);
-  *first = int(int64_t(start_at(starts, low, total)) * per / tile) + low;
-  return low;
-}
+using sequences::Group;
+using sequences::make_group;
+using sequences::Sequence;
 
 // ---------------------------------------------------------------------------
 // arguments
@@ -715,6 +665,10 @@ struct PackedArgs {
   float scale, scale_log2;
   int tiles;
 };
+
+__device__ __forceinline__ sequences::Starts starts_of(const PackedArgs &A) {
+  return {A.q_starts, A.k_starts, A.sequences, A.q_total, A.k_total};
+}
 
 // Blocks of 128 rows that a call has.
 inline int64_t row_blocks(const PackedArgs &A) {

@@ -583,7 +583,9 @@ int bevpool_norm_rotate_backward(
  *   dim          a multiple of 8, at most 128; rows and heads of every
  *                operand start at multiples of 16 bytes
  *   q_starts, k_starts   device int32 [sequences + 1], ascending from 0
- *                (values are clamped to the rows there are)
+ *                (values are clamped to the rows there are; starts that do
+ *                not ascend give results of no meaning, and rows that are not
+ *                written, but lead to no access outside the operands)
  *   out          (q_total, q_heads, dim) contiguous
  *   out_rest     as out: what rounding took off out, rounded itself (fp32:
  *                not written), for the gradients; or NULL
