@@ -25,6 +25,7 @@ import ctypes
 import functools
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _lib as L
@@ -83,6 +84,14 @@ def _run(call, device, what):
 
 def _wants_grad(*tensors):
     return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+
+
+def _recorded():
+    """Whether something other than a gradient follows the calls: tangents,
+    which the autograd functions refuse (a result without one would stand for
+    a derivative of zero), or a trace, which records the functions as they are
+    (it does not see the library's calls)."""
+    return forward_ad._current_level >= 0 or torch._C._get_tracing_state() is not None
 
 
 # ---- norm and rotation -----------------------------------------------------
@@ -187,7 +196,7 @@ def norm_rotate(q, k, positions, frequencies, pairs=None, *, q_weight=None, k_we
         raise TypeError('positions must have dtype torch.int32, torch.int64 or torch.float32.')
     if frequencies.dim() != 1 or frequencies.dtype != torch.float32:
         raise ValueError('frequencies must be a 1-d float32 tensor.')
-    pairs = (frequencies.shape[0],) if pairs is None else tuple(int(n) for n in pairs)
+    pairs = (int(frequencies.shape[0]),) if pairs is None else tuple(int(n) for n in pairs)
     if len(pairs) > MAX_AXES or any(n < 0 for n in pairs):
         raise ValueError(f'pairs must be at most {MAX_AXES} numbers, none negative.')
     if sum(pairs) != frequencies.shape[0] or 2 * sum(pairs) > dim:
@@ -206,7 +215,7 @@ def norm_rotate(q, k, positions, frequencies, pairs=None, *, q_weight=None, k_we
         if t.device != q.device:
             raise ValueError(f'{name} must be on the device of q ({q.device}).')
     weights = [w if w is None else w.contiguous() for w in (q_weight, k_weight)]
-    run = _NormRotate.apply if _wants_grad(q, k, *weights) else _norm_rotate
+    run = _NormRotate.apply if _wants_grad(q, k, *weights) or _recorded() else _norm_rotate
     return run(_unit(q), _unit(k) if k is not None else None, *weights, _unit(positions),
                frequencies.contiguous(), pairs, float(eps), bool(interleaved))
 
@@ -241,7 +250,7 @@ def _check_heads(q, k, v):
 
 
 def _check_scale(scale, dim):
-    scale = dim ** -0.5 if scale is None else float(scale)
+    scale = float(dim) ** -0.5 if scale is None else float(scale)
     if not 1e-30 <= scale < float('inf'):
         raise ValueError('scale must be positive (1e-30 or more) and finite.')
     return scale
@@ -335,7 +344,7 @@ def attend_packed(q, k, v, q_starts, k_starts=None, *, causal=False, scale=None,
         k_starts = _check_starts('k_starts', k_starts, q)
     if k_starts.shape != q_starts.shape:
         raise ValueError('q_starts and k_starts must have the same length.')
-    run = _AttendPacked.apply if _wants_grad(q, k, v) else _attend_packed
+    run = _AttendPacked.apply if _wants_grad(q, k, v) or _recorded() else _attend_packed
     out, lse = run(_aligned(q, q.shape[1] // k.shape[1]), _aligned(k), _aligned(v), q_starts,
                    k_starts, bool(causal), scale)
     return (out, lse) if return_lse else out
@@ -352,6 +361,30 @@ def _cache(name, x, dims):
         raise ValueError(f'{name}: rows and heads must start at multiples of 16 bytes, rows less '
                          'than 16 MiB apart.')
     return x
+
+
+def _attend_cached(q, rows, k, v, lengths, prefix_k, prefix_v, scale):
+    """rows: q (requests, tokens, q_heads, dim) as aligned rows."""
+    requests, tokens, q_heads, dim = q.shape
+    capacity, k_heads = k.shape[1:3]
+    prefix = prefix_k.shape[0] if prefix_k is not None else 0
+    out = q.new_empty(q.shape)
+    nbytes = L.library().bevpool_attention_cached_scratch_bytes(
+        requests, tokens, capacity, prefix, q_heads, k_heads, dim)
+    scratch = q.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
+    _run(lambda lib, s: lib.bevpool_attention_cached(
+        *_strides(rows), L.ptr(k), *k.stride()[:3], L.ptr(v), *v.stride()[:3],
+        *_strides(prefix_k), *_strides(prefix_v), L.ptr(lengths), L.DTYPE_CODES[q.dtype],
+        requests, tokens, capacity, prefix, q_heads, k_heads, dim, scale, L.ptr(out),
+        L.ptr(scratch), nbytes, s), q.device, 'bevpool_attention_cached')
+    return out
+
+
+class _AttendCached(torch.autograd.Function):
+    """For tangents and traces alone: there is no gradient."""
+    @staticmethod
+    def forward(ctx, q, rows, k, v, lengths, prefix_k, prefix_v, scale):
+        return _attend_cached(q, rows, k, v, lengths, prefix_k, prefix_v, scale)
 
 
 def attend_cached(q, k, v, lengths, prefix_k=None, prefix_v=None, *, scale=None):
@@ -374,7 +407,6 @@ def attend_cached(q, k, v, lengths, prefix_k=None, prefix_v=None, *, scale=None)
     k, v = _cache('k', k, 4), _cache('v', v, 4)
     _check_heads(q, k, v)
     requests, tokens, q_heads, dim = q.shape
-    capacity, k_heads = k.shape[1:3]
     if k.shape[0] != requests:
         raise ValueError('q and k must have the same number of requests.')
     if tokens < 1:
@@ -400,14 +432,6 @@ def attend_cached(q, k, v, lengths, prefix_k=None, prefix_v=None, *, scale=None)
     rows = _aligned(q.reshape(requests * tokens, q_heads, dim))
     if lengths.dtype != torch.int32 or not lengths.is_contiguous():
         lengths = lengths.to(torch.int32).contiguous()
-    prefix = prefix_k.shape[0] if prefix_k is not None else 0
-    out = q.new_empty(q.shape)
-    nbytes = L.library().bevpool_attention_cached_scratch_bytes(
-        requests, tokens, capacity, prefix, q_heads, k_heads, dim)
-    scratch = q.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
-    _run(lambda lib, s: lib.bevpool_attention_cached(
-        *_strides(rows), L.ptr(k), *k.stride()[:3], L.ptr(v), *v.stride()[:3],
-        *_strides(prefix_k), *_strides(prefix_v), L.ptr(lengths), L.DTYPE_CODES[q.dtype],
-        requests, tokens, capacity, prefix, q_heads, k_heads, dim, scale, L.ptr(out),
-        L.ptr(scratch), nbytes, s), q.device, 'bevpool_attention_cached')
+    run = _AttendCached.apply if _recorded() else _attend_cached
+    out = run(q, rows, k, v, lengths, prefix_k, prefix_v, scale)
     return out[:, 0] if single else out
