@@ -232,7 +232,8 @@ def _aligned(x, group=1):
     if (one == 1 and row % 16 == 0 and head % 16 == 0 and row < 1 << 24
             and head * group < 1 << 30 and x.data_ptr() % 16 == 0):
         return x
-    return x.contiguous() if not x.is_contiguous() else x.clone()
+    # (not contiguous(): a dimension of one keeps whatever stride it has there)
+    return x.clone(memory_format=torch.contiguous_format)
 
 
 def _check_heads(q, k, v):
@@ -352,12 +353,20 @@ def attend_packed(q, k, v, q_starts, k_starts=None, *, causal=False, scale=None,
 
 # ---- new tokens over caches ------------------------------------------------
 
-def _cache(name, x, dims):
-    _check_rows(name, x, dims)
+def _cache_fits(x, strides):
     per = 16 // x.element_size()
-    if x.numel() and (x.stride(-1) != 1 or x.data_ptr() % 16
-                      or any(s % per for s in x.stride()[:-1])
-                      or x.stride(-3) >= per << 20):
+    return (strides[-1] == 1 and x.data_ptr() % 16 == 0 and not any(s % per for s in strides[:-1])
+            and strides[-3] < per << 20)
+
+
+def _cache(name, x, dims):
+    """x, or a view of it in which dimensions of one, whose stride leads
+    nowhere, have a stride that the kernels take."""
+    _check_rows(name, x, dims)
+    if x.numel() and not _cache_fits(x, x.stride()):
+        used = [s if n > 1 else 0 for n, s in zip(x.shape[:-1], x.stride())] + [x.stride(-1)]
+        if _cache_fits(x, used):
+            return x.as_strided(x.shape, used)
         raise ValueError(f'{name}: rows and heads must start at multiples of 16 bytes, rows less '
                          'than 16 MiB apart.')
     return x

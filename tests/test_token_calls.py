@@ -1,5 +1,6 @@
 """The token operators' Python calls where no kernel runs: what follows a call
-besides gradients (tangents, traces) goes through the autograd functions."""
+besides gradients (tangents, traces) goes through the autograd functions, and
+strides that lead nowhere are no reason to refuse."""
 from __future__ import annotations
 
 import warnings
@@ -53,6 +54,52 @@ def test_a_trace_records_the_call(attention, name):
         traced = torch.jit.trace(lambda q: CALLS[name](attention, t, q), (t['q'],),
                                  check_trace=False)
     assert '^_' in str(traced.graph) and 'aten::new_empty' not in str(traced.graph)
+
+
+def odd_units(*shape, dtype=torch.float32):
+    """Dimensions of one with an odd stride, the others dense, from an aligned
+    start."""
+    strides, at = [], 1
+    for n in reversed(shape):
+        strides.append(at if n > 1 else 259)
+        at *= n
+    return torch.zeros(at, dtype=dtype).as_strided(shape, strides[::-1])
+
+
+def test_strides_of_single_entries(attention):
+    """The stride of a dimension of one leads nowhere: no refusal for it, and
+    no copy of a cache."""
+    for shape in ((1, 4, 64), (6, 1, 64), (1, 1, 64)):
+        for dtype in (torch.float32, torch.bfloat16):
+            x = attention._aligned(odd_units(*shape, dtype=dtype))
+            assert not any(s * x.element_size() % 16 for s in x.stride()[:2]), shape
+    for shape in ((1, 9, 2, 64), (3, 1, 2, 64), (3, 9, 1, 64), (1, 1, 1, 64), (1, 2, 64), (5, 1, 64)):
+        x = odd_units(*shape)
+        y = attention._cache('k', x, len(shape))
+        assert y.data_ptr() == x.data_ptr() and y.shape == x.shape
+        assert not any(s % 4 for s in y.stride()[:-1]), shape
+    with pytest.raises(ValueError, match='16 bytes'):
+        attention._cache('k', torch.zeros(9 * 259).as_strided((9, 2, 64), (259, 64, 1)), 3)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('dtype', [torch.bfloat16, torch.float16, torch.float32])
+def test_one_row_of_a_wide_pitch(pkg, cuda, dtype):
+    """Single rows cut from rows of an odd pitch, and a gradient of that kind:
+    the same bits as contiguous ones."""
+    g = torch.Generator().manual_seed(1)
+    rows = [torch.randn((5, 259), generator=g).to(cuda, dtype) for _ in range(4)]
+    starts = torch.tensor([0, 1], device=cuda)
+    odd = [r[:, :256].unflatten(1, (4, 64))[:1] for r in rows]
+    results = []
+    for q, k, v, dout in (odd, [x.clone(memory_format=torch.contiguous_format) for x in odd]):
+        leaves = [x.detach().requires_grad_(True) for x in (q, k, v)]
+        out = pkg.attend_packed(*leaves, starts)
+        results.append((out, *torch.autograd.grad(out, leaves, dout)))
+        with torch.no_grad():
+            results[-1] += (pkg.attend_cached(q, k[None], v[None], starts[1:], k, v),)
+    for a, b in zip(*results):
+        assert torch.equal(a, b)
 
 
 @pytest.mark.gpu
