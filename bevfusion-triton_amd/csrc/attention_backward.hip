@@ -687,9 +687,10 @@ int bevpool_attention_backward(const void *q, int64_t q_row, int64_t q_head, con
   if (!st) st = set_operand(A.dv, "dv", dv, k_dense, dim, elem, k_total);
   if (st) return st;
   if (q_total > 0 && !lse) return fail(BEVPOOL_EINVAL, "lse: null");
-  // (as are those of a tile's rows, heads of a group among them)
-  const int64_t heads = A.group.size < 64 ? A.group.size : 64;
-  if (A.q.head * heads >= (1 << 30) || A.dout.head * heads >= (1 << 30))
+  // (a tile's rows may begin with any head of the group, and their offsets from
+  // the group's first are 32-bit)
+  const int64_t reach = (int64_t(1) << 30) / A.group.size;
+  if (q_total > 0 && (A.q.head >= reach || A.dout.head >= reach))
     return fail(BEVPOOL_EINVAL, "q, dout: the heads of a group must lie within 2^30 bytes");
   const size_t need = bevpool_attention_backward_scratch_bytes(q_total, k_total, q_heads, k_heads,
                                                                dim, dtype, sequences);

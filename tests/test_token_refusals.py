@@ -78,3 +78,27 @@ def test_cached_attention(pkg):
     assert need > 0 and need % ((64 + 2) * 4 * 2 * 4) == 0
     assert call(capacity=5000, scratch=16, nbytes=need - 1) == -3
     assert lib.bevpool_attention_cached_scratch_bytes(2, 1, 64, 0, 4, 2, 64) == 0
+
+
+def test_heads_of_a_group_within_reach(pkg):
+    """Any head of a group may begin a tile of rows, also where there are more
+    than a tile has rows: the strides of all of them count."""
+    lib = pkg.library()
+
+    def backward(group, q_head, dout_head):
+        row = 64 * group
+        return lib.bevpool_attention_backward(
+            16, row, q_head, 16, 64, 64, 16, 64, 64, 16, None, 16, row, dout_head, 16, 2, 4, 4, group,
+            1, 64, 16, 16, 1, 0, 0.125, 16, 16, 16, None, 0, None)
+
+    far = (1 << 23) - 8  # elements: just under 16 MiB
+    for group in (65, 256, 1024):
+        for heads in ((far, 64), (64, far)):
+            assert backward(group, *heads) == -1, (group, heads)
+            assert b'heads of a group' in lib.bevpool_last_error()
+    reach = (1 << 30) // 256 // 2
+    assert backward(256, reach, 64) == -1
+    assert b'heads of a group' in lib.bevpool_last_error()
+    # within reach: the next check (no scratch) answers
+    for group, head in ((256, reach - 8), (4, far), (1024, 64)):
+        assert backward(group, head, head) == -3, (group, head)
