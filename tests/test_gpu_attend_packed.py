@@ -123,6 +123,20 @@ def test_long_walks(pkg, cuda, dim, dtype):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize('dtype', DTYPES)
+@pytest.mark.parametrize('dim', [64, 80, 128])
+def test_long_walks_of_a_full_card(pkg, cuda, dim, dtype):
+    """Many short sequences fill the card with blocks of 128 keys, and the walks
+    of a long one among them are cut in two; the same bits each time."""
+    lengths = [3] * 25 + [1100] + [3] * 35
+    case = make(lengths, lengths, 16, 8, dim, dtype)
+    check(pkg, cuda, case, True)
+    first, again = run(pkg, cuda, case, True), run(pkg, cuda, case, True)
+    for n in first:
+        assert torch.equal(first[n], again[n]), n
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('dtype', DTYPES)
 def test_parts_of_one_projection(pkg, cuda, dtype):
     """Operands as slices of one matrix, aligned and not, and a gradient with
     strides: the same bits as contiguous copies."""
