@@ -128,16 +128,11 @@ class _NormRotate(torch.autograd.Function):
         tokens, q_heads, k_heads, dim, dtype, pairs, eps, interleaved = ctx.call
         dev = positions.device
 
-        def grad_rows(g, heads):
-            if heads == 0:
-                return None
-            if g is None:  # an output that nothing was computed from
-                return torch.zeros((tokens, heads, dim), dtype=dtype, device=dev)
-            return _unit(g if g.dtype == dtype else g.to(dtype))
-
-        dq_out, dk_out = grad_rows(dq_out, q_heads), grad_rows(dk_out, k_heads)
-        dq = dq_out.new_empty(dq_out.shape)
-        dk = dk_out.new_empty(dk_out.shape) if k_heads else None
+        # (None: of a k that is not there; an output that nothing was computed
+        # from has a gradient of zeros)
+        dq_out, dk_out = (g if g is None else _unit(g if g.dtype == dtype else g.to(dtype))
+                          for g in (dq_out, dk_out))
+        dq, dk = (g if g is None else g.new_empty(g.shape) for g in (dq_out, dk_out))
         dqw = torch.empty_like(q_weight) if q_weight is not None else None
         dkw = torch.empty_like(k_weight) if k_weight is not None else None
         lib = L.library()

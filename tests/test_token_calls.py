@@ -82,6 +82,15 @@ def test_strides_of_single_entries(attention):
         attention._cache('k', torch.zeros(9 * 259).as_strided((9, 2, 64), (259, 64, 1)), 3)
 
 
+@pytest.mark.parametrize('heads', [(0, 2), (4, 0), (0, 0)])
+def test_gradients_of_no_heads(attention, heads):
+    t = operands()
+    q, k = (torch.zeros((6, n, 64), requires_grad=True) for n in heads)
+    out = attention.norm_rotate(q, k, t['positions'], t['frequencies'])
+    for x, g in zip((q, k), torch.autograd.grad(out, (q, k), [torch.ones_like(x) for x in out])):
+        assert g.shape == x.shape
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize('dtype', [torch.bfloat16, torch.float16, torch.float32])
 def test_one_row_of_a_wide_pitch(pkg, cuda, dtype):
@@ -114,3 +123,23 @@ def test_a_trace_runs_on_other_inputs(pkg, cuda, name):
     assert not torch.equal(want, CALLS[name](pkg, t, t['q']))
     for _ in range(4):  # (the executor optimises after the first runs)
         assert torch.equal(traced(other), want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('norm', [False, True])
+def test_no_heads_and_no_keys(pkg, cuda, norm):
+    """q without heads, and gradients of one output alone: those of the other
+    operand are what they are without it."""
+    t = {n: x.to(cuda) for n, x in operands().items()}
+    w = torch.linspace(0.5, 1.5, 64, device=cuda, requires_grad=True)
+    weight = {'k_weight': w} if norm else {}
+    args = t['positions'], t['frequencies']
+    k = t['k'].requires_grad_(True)
+    leaves = [k, w] if norm else [k]
+    alone = pkg.norm_rotate(t['k'][:, :0], k, *args, **weight)[1]
+    beside = pkg.norm_rotate(t['q'], k, *args, **weight)[1]
+    assert torch.equal(alone, beside)
+    g = torch.ones_like(alone)
+    for a, b in zip(torch.autograd.grad(alone, leaves, g), torch.autograd.grad(beside, leaves, g)):
+        # (sums of the weights' gradient are cut at other tokens)
+        assert torch.allclose(a, b, rtol=1e-5, atol=1e-6)
