@@ -316,8 +316,8 @@ def attend_packed(q, k, v, q_starts, k_starts=None, *, causal=False, scale=None,
     multiple of k_heads (query head h reads key head h // (q_heads /
     k_heads)), dim a multiple of 8 up to 128.  Sequence i has the queries
     [q_starts[i], q_starts[i + 1]) and the keys [k_starts[i], k_starts[i + 1])
-    (default: as the queries); both are int32 or int64 tensors on the device,
-    ascending from 0, and are never read back.  With ``causal``, query j of a
+    (default: as the queries); both are int32 or int64 tensors on the device
+    (of values that fit 32 bits), ascending from 0, and are never read back.  With ``causal``, query j of a
     sequence sees its keys up to j + (keys - queries): the last query sees
     all.  out = softmax(scale * q k) v (scale: dim ** -0.5); a query that sees
     no key or is in no sequence gives zeros and passes no gradient.  Values of
@@ -398,8 +398,8 @@ def attend_cached(q, k, v, lengths, prefix_k=None, prefix_v=None, *, scale=None)
     q (requests, tokens, q_heads, dim), or (requests, q_heads, dim) for single
     tokens; k, v (requests, capacity, k_heads, dim): each request's own cache,
     its new tokens' keys and values already in it.  lengths (requests,), int32
-    or int64 on the device: the keys in use, the new tokens' among them (taken
-    as within [0, capacity]).  prefix_k, prefix_v (prefix, k_heads, dim) or
+    or int64 on the device (of values that fit 32 bits): the keys in use, the
+    new tokens' among them (taken as within [0, capacity]).  prefix_k, prefix_v (prefix, k_heads, dim) or
     None.  New token i sees the whole prefix and the first lengths - (tokens -
     1 - i) keys of its request's cache; what lies past a length is never read.
     A row that sees nothing gives zeros.  Returns q's shape, contiguous.  Heads
