@@ -44,8 +44,10 @@ class TokenAttention(nn.Module):
         at positions (tokens, axes): (tokens, heads, head_dim) each."""
         rows = self.qkv(x).unflatten(-1, (-1, self.head_dim))
         q, k, v = rows.split((self.q_heads, self.k_heads, self.k_heads), -2)
-        q, k = norm_rotate(q, k, positions, self.frequencies, self.pairs, q_weight=self.q_norm,
-                           k_weight=self.k_norm, eps=self.eps)
+        # (under autocast the projection is 16-bit and the weights are not)
+        q, k = norm_rotate(q, k, positions, self.frequencies, self.pairs,
+                           q_weight=self.q_norm.to(q.dtype), k_weight=self.k_norm.to(k.dtype),
+                           eps=self.eps)
         return q, k, v
 
     def forward(self, x, positions, starts, *, causal=False):

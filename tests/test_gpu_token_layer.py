@@ -51,6 +51,36 @@ def test_training_step(pkg, cuda, causal):
         assert torch.allclose(p.grad.cpu().double(), w[n].grad, rtol=1e-3, atol=1e-4 * scale), n
 
 
+@pytest.mark.parametrize('dtype', [torch.bfloat16, torch.float16])
+def test_autocast(pkg, cuda, dtype):
+    """fp32 parameters under autocast: the training step of a layer in 16 bits
+    with the same values, its gradients in fp32; and single tokens."""
+    torch.manual_seed(3)
+    layer = pkg.TokenAttention(32, 4, 2, 32, (4, 6, 6), device=cuda)
+    with torch.no_grad():
+        for p in layer.parameters():
+            p.copy_((p * 1.25 + 0.01).to(dtype))
+    half = pkg.TokenAttention(32, 4, 2, 32, (4, 6, 6), device=cuda, dtype=dtype)
+    half.load_state_dict(layer.state_dict())
+    x, positions = torch.randn(75, 32, device=cuda), torch.randint(0, 30, (75, 3), device=cuda)
+    starts = torch.tensor([0, 31, 75], device=cuda)
+    with torch.autocast('cuda', dtype):
+        y = layer(x, positions, starts, causal=True)
+    want = half(x.to(dtype), positions, starts, causal=True)
+    assert y.dtype == dtype and torch.equal(y, want)
+    goal = torch.randn_like(want)
+    y.backward(goal)
+    want.backward(goal)
+    for (n, p), h in zip(layer.named_parameters(), half.parameters()):
+        assert p.grad.dtype == torch.float32 and torch.equal(p.grad, h.grad.float()), n
+    cache = [torch.zeros((2, 5, 2, 32), device=cuda, dtype=dtype) for _ in range(4)]
+    lengths = torch.zeros((2, 2), dtype=torch.int32, device=cuda)
+    with torch.autocast('cuda', dtype):
+        y = layer.step(x[:2, None], positions[:2, None], *cache[:2], lengths[0])
+    assert torch.equal(y, half.step(x[:2, None].to(dtype), positions[:2, None], *cache[2:],
+                                    lengths[1]))
+
+
 @pytest.mark.parametrize('new', [1, 3])
 def test_steps_are_the_prompts_rows(pkg, cuda, new):
     """Each answer, `new` tokens at a time over the shared scene and its own
