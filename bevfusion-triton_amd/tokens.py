@@ -31,12 +31,17 @@ class TokenAttention(nn.Module):
         self.out = nn.Linear(q_heads * head_dim, dim, bias=False, **kind)
         self.q_norm = nn.Parameter(torch.ones(head_dim, **kind))
         self.k_norm = nn.Parameter(torch.ones(head_dim, **kind))
+        self.base = base
         # (a plain attribute: fp32 whatever the module is cast to)
         self.frequencies = axis_frequencies(self.pairs, base, device=device)
 
     def _apply(self, fn, *args, **kwargs):
         super()._apply(fn, *args, **kwargs)
-        self.frequencies = self.frequencies.to(self.q_norm.device)
+        device = self.q_norm.device
+        if self.frequencies.is_meta:  # (no values there to move)
+            self.frequencies = axis_frequencies(self.pairs, self.base, device=device)
+        else:
+            self.frequencies = self.frequencies.to(device)
         return self
 
     def project(self, x, positions):

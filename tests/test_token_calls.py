@@ -82,6 +82,17 @@ def test_strides_of_single_entries(attention):
         attention._cache('k', torch.zeros(9 * 259).as_strided((9, 2, 64), (259, 64, 1)), 3)
 
 
+def test_layer_of_the_meta_device(pkg):
+    """A layer made without memory has its frequencies once it is given some."""
+    args = (32, 4, 2, 32, (4, 6, 6))
+    want = pkg.TokenAttention(*args, base=500.0).frequencies
+    layer = pkg.TokenAttention(*args, base=500.0, device='meta').to(torch.bfloat16)
+    assert layer.frequencies.is_meta
+    assert torch.equal(layer.to_empty(device='cpu').frequencies, want)
+    layer = pkg.TokenAttention(*args, base=500.0).to('meta')
+    assert torch.equal(layer.to_empty(device='cpu').double().frequencies, want)
+
+
 @pytest.mark.parametrize('heads', [(0, 2), (4, 0), (0, 0)])
 def test_gradients_of_no_heads(attention, heads):
     t = operands()
