@@ -72,15 +72,22 @@ class TokenAttention(nn.Module):
     def step(self, x, positions, cache_k, cache_v, lengths, prefix=(None, None)):
         """New tokens x (requests, new, dim) at positions (requests, new, axes):
         their keys and values go into the caches (requests, capacity, k_heads,
-        head_dim) behind the ``lengths`` (requests,) that are there, which
-        grow by ``new`` (up to the capacity, which is not checked here); then the tokens attend to ``prefix``, to what their
-        request's cache held and to themselves.  Returns (requests, new, dim)."""
+        head_dim) behind the ``lengths`` (requests,) that are there, which grow
+        by ``new``; then the tokens attend to ``prefix``, to what their
+        request's cache held and to themselves.  The host does not know the
+        lengths: where a cache has no room left, the new tokens take its last
+        slots, and its length stays at the capacity.  Returns (requests, new,
+        dim)."""
         requests, new = x.shape[:2]
+        capacity = cache_k.shape[1]
+        if new > capacity:
+            raise ValueError(f'{new} new tokens do not fit caches of {capacity}.')
         q, k, v = self.project(x.flatten(0, 1), positions.flatten(0, 1))
-        slots = lengths[:, None].long() + torch.arange(new, device=x.device)
+        held = lengths.clamp(0, capacity - new)
+        slots = held[:, None] + torch.arange(new, device=x.device)
         rows = torch.arange(requests, device=x.device)[:, None]
         cache_k[rows, slots] = k.unflatten(0, (requests, new))
         cache_v[rows, slots] = v.unflatten(0, (requests, new))
-        lengths += new
+        torch.add(held, new, out=lengths)
         out = attend_cached(q.unflatten(0, (requests, new)), cache_k, cache_v, lengths, *prefix)
         return self.out(out.flatten(2))

@@ -105,6 +105,24 @@ def test_steps_are_the_prompts_rows(pkg, cuda, new):
         assert torch.allclose(got[b], whole[150:], rtol=1e-4, atol=1e-5)
 
 
+@pytest.mark.parametrize('kind', [torch.int32, torch.int64])
+def test_steps_past_the_capacity_stay_in_the_cache(pkg, cuda, kind):
+    """A full cache takes new tokens in its last slots and no others."""
+    torch.manual_seed(4)
+    layer = pkg.TokenAttention(32, 4, 2, 64, (8, 12, 12), device=cuda)
+    x, at = torch.randn(3, 2, 32, device=cuda), torch.full((3, 2, 3), 7, device=cuda)
+    wide = [torch.zeros((3, 9, 2, 64), device=cuda) for _ in range(2)]
+    cache = [w[:, 2:7] for w in wide]  # 5 slots amid others
+    lengths = torch.tensor([4, 1, 5], device=cuda, dtype=kind)
+    layer.step(x, at, *cache, lengths)
+    assert lengths.tolist() == [5, 3, 5]
+    for w in wide:
+        used = w.flatten(2).abs().sum(-1) > 0
+        assert used.nonzero().tolist() == [[0, 5], [0, 6], [1, 3], [1, 4], [2, 5], [2, 6]]
+    with pytest.raises(ValueError, match='do not fit'):
+        layer.step(torch.randn(3, 6, 32, device=cuda), at, *cache, lengths)
+
+
 def test_example_runs(pkg, cuda, capsys):
     spec = importlib.util.spec_from_file_location('bev_tokens', ROOT / 'examples' /
                                                   'bev_tokens.py')
