@@ -149,7 +149,10 @@ __device__ __forceinline__ void tile_barrier() {
 // writes no register.  The compiler does not see a memory access here, so the
 // block itself keeps the five wait states that one needs behind a vector
 // instruction that wrote its scalar base (a reload of a spilled one, say),
-// and the one behind a write of m0.
+// and the one behind a write of m0.  It cannot be told that m0 is written
+// either (the compiler takes it as reserved); nothing else in these kernels
+// uses it, and no vector register is spilled, whose reloads the hand-counted
+// waits would count too: tests/test_built_kernels.py looks at the built code.
 __device__ __forceinline__ void load_to_lds(const char *base, unsigned offset, unsigned to) {
   asm volatile(
       "s_mov_b32 m0, %0\n\t"
