@@ -12,6 +12,13 @@
 // of all heads of the group, so shared heads' gradients are summed there.
 // P and dS are rounded to the operands' type before their products, as the
 // matrix instructions ask; all else is fp32.
+//
+// dS grows with dout, and fp16 holds only 2^-14 to 2^16 in full: small
+// gradients would be lost in its last bits, large ones past its range.  So in
+// fp16 dS is formed times a power of two that brings dout's largest magnitude
+// to between 4 and 8 (where a dout of order 1 has it already), and the sums,
+// in fp32, are brought back: in dq's kernel by row, in the keys' kernels by the
+// rows that a block walks.
 #include "attention_tiles.h"
 #include "host_calls.h"
 
@@ -27,7 +34,18 @@ struct BackwardArgs : PackedArgs {
   // (tokens, heads): -L / scale, where the sums of q k begin, and -D.  In fp32
   // -L in units of log 2: sums begun so far from zero lose a bit there.
   float2 *stats;
+  // fp16: the largest magnitude of dout in 32 rows, [key head][row tile * tile
+  // rows / 32 + 32 rows], tops_stride for a head
+  float *tops;
+  int tops_stride;
+  int row_tile;  // rows of a tile of the query kernel
 };
+
+// log2 of what dS is formed times, where dout's largest finite magnitude is
+// `top` (0: anything will do).
+__device__ __forceinline__ int raise_of(float top) {
+  return 3 - __builtin_amdgcn_frexp_expf(top);  // top = m 2^e, m in [0.5, 1)
+}
 
 // A lane's part of the dot product of two rows.
 template <typename T, int DP>
@@ -111,6 +129,26 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 4 && DP > 64 ? 1 : 2) void q
   }
   settle(stat);
   const float lse2 = stat[0], delta = stat[1];
+  constexpr bool kRaise = __is_same(T, _Float16);
+  float from = -lse2;  // of the exponents
+  int raise = 0;
+  if constexpr (kRaise) {
+    float top = 0.f;
+#pragma unroll
+    for (int s = 0; s < S::kSteps; ++s)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float size = fabsf(float(g[s][i]));
+        top = fmaxf(top, size < kInf ? size : 0.f);  // (no number: fmaxf's other)
+      }
+    top = max_halves(top);
+    raise = raise_of(top);
+    from += float(raise);
+#pragma unroll
+    for (int m = 1; m < 32; m <<= 1) top = fmaxf(top, __shfl_xor(top, m, 64));
+    if (wave_on && half == 0 && lane == 0)
+      A.tops[int64_t(head) * A.tops_stride + index * (kRows / 32) + wave] = top;
+  }
   if (valid && h == 0 && half == 0) A.stats[stat_at] = make_float2(sizeof(T) == 4 ? -lse2 : -lse2 / A.scale_log2, -delta);
   const char *k_at = A.k.at + seq.k0 * A.k.row + head * A.k.head;
   const char *v_at = A.v.at + seq.k0 * A.v.row + head * A.v.head;
@@ -171,7 +209,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 4 && DP > 64 ? 1 : 2) void q
       float p[16];
 #pragma unroll
       for (int r = 0; r < 16; ++r)
-        p[r] = exp2_fast(fmaf(dots[r], A.scale_log2, -lse2)) * (kBegin ? dp[r] : dp[r] - delta);
+        p[r] = exp2_fast(fmaf(dots[r], A.scale_log2, from)) * (kBegin ? dp[r] : dp[r] - delta);
       if (masked) {
 #pragma unroll
         for (int r = 0; r < 16; ++r)
@@ -203,7 +241,8 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 4 && DP > 64 ? 1 : 2) void q
     if (half == 1) return;
     add_sums<T, DP>(dq, sums);
   }
-  store_row<T, DP>(A.dq.at + token * A.dq.row + q_head * A.dq.head, dq, A.scale, A.dim, valid);
+  const float by = kRaise ? __builtin_amdgcn_ldexpf(A.scale, -raise) : A.scale;
+  store_row<T, DP>(A.dq.at + token * A.dq.row + q_head * A.dq.head, dq, by, A.dim, valid);
 }
 
 // How the keys' kernel keeps a wave's 32 keys: their K and V fragments and
@@ -299,6 +338,25 @@ key_grad_kernel(BackwardArgs A, Splits splits) {
   row_frags<T, DP>(k, A.k.at + k_row * A.k.row + head * A.k.head, A.chunks, true);
   if constexpr (kDk)
     row_frags<T, DP>(v, A.v.at + k_row * A.v.row + head * A.v.head, A.chunks, true);
+  // fp16: dS times 2^raise.  As much of it as P may have for dv as well (2^15 P
+  // fits, and less than P would lose its last bits) is in the exponents; what
+  // is left, of a dout far from 1, is apart with the mask (a product for all
+  // cost 7% of heads of 32).
+  constexpr bool kRaise = __is_same(T, _Float16) && kDk;
+  int raise = 0, raise_p = 0;
+  if constexpr (kRaise) {
+    const int first = sequences::first_tile(A.q_starts, tile.which, A.q_total, heads, A.row_tile);
+    const float *tops = A.tops + int64_t(head) * A.tops_stride + first * (A.row_tile / 32);
+    const int low = begin + (tile.tiles - t_end) * kRows;
+    const int high = min(rows, begin + (tile.tiles - t_begin) * kRows);
+    float top = 0.f;
+    for (int i = low / 32 + lane; i * 32 < high; i += 64) top = fmaxf(top, tops[i]);
+#pragma unroll
+    for (int m = 1; m < 64; m <<= 1) top = fmaxf(top, __shfl_xor(top, m, 64));
+    raise = __builtin_amdgcn_readfirstlane(raise_of(top));
+  }
+  if constexpr (kRaise) raise_p = kDv ? max(0, min(raise, 15)) : raise;
+  const float raise_e = float(raise_p), raise_rest = __builtin_amdgcn_ldexpf(1.f, raise - raise_p);
   const char *q_at = A.q.at + seq.q0 * A.q.row + int64_t(head) * heads * A.q.head;
   const char *g_at = A.dout.at + seq.q0 * A.dout.row + int64_t(head) * heads * A.dout.head;
   const int64_t stat0 = int64_t(seq.q0) * A.q_heads + head * heads;
@@ -357,11 +415,11 @@ key_grad_kernel(BackwardArgs A, Splits splits) {
     const int r0 = begin + (tile.tiles - 1 - t) * kRows;
     const int r_mine = r0 + mine, r_end = r_mine + 32 * kMine;
     if (key0 >= seq.nk || r_end <= from_first || r_mine >= rows) continue;
-    const bool masked = r_mine < from_last || r_end > rows;
+    const bool masked = r_mine < from_last || r_end > rows || raise != raise_p;
     // (hides that the addresses of the reads are the same in every round: kept,
     // they take more registers than there are)
     int at_lane = lane;
-    if constexpr ((kDk && kDv && DP > 80) || (sizeof(T) == 4 && DP > 64))
+    if constexpr ((kDk && kDv && DP >= (kRaise ? 80 : 96)) || (sizeof(T) == 4 && DP > 64))
       asm volatile("" : "+v"(at_lane));
 #pragma unroll
     for (int b = 0; b < kMine; ++b) {
@@ -418,6 +476,7 @@ key_grad_kernel(BackwardArgs A, Splits splits) {
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
         p[r] = exp2_fast(sizeof(T) == 4 ? fmaf(dots[r], A.scale_log2, l[r])
+                         : kRaise       ? fmaf(dots[r], A.scale_log2, raise_e)
                                         : dots[r] * A.scale_log2);
         ds[r] = kDk ? p[r] * dp[r] : 0.f;
       }
@@ -425,6 +484,7 @@ key_grad_kernel(BackwardArgs A, Splits splits) {
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
           const int at = r_mine + 32 * b + c_row(r, h);
+          if (kRaise && kDv) ds[r] *= raise_rest;
           if (at < from || at >= rows) p[r] = ds[r] = 0.f;
         }
       }
@@ -471,6 +531,17 @@ key_grad_kernel(BackwardArgs A, Splits splits) {
       if (half == 0) add_sums<T, DP>(n == 0 ? dk : dv, sums);
     }
     if (half == 1) return;
+  }
+  if constexpr (kRaise) {
+    const float by = __builtin_amdgcn_ldexpf(1.f, -raise);
+    const float by_p = __builtin_amdgcn_ldexpf(1.f, -raise_p);
+#pragma unroll
+    for (int b = 0; b < kBlocks; ++b)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        dk[b][r] *= by;
+        if constexpr (kDv) dv[b][r] *= by_p;
+      }
   }
   if (n_splits > 1) {
     float *put = splits.sums +
@@ -588,6 +659,7 @@ int launch_query(BackwardArgs &A, hipStream_t s) {
   const int64_t blocks = int64_t(A.tiles) * A.k_heads;
   int st = check_grid(blocks, kThreads, "attention query gradient");
   if (st) return st;
+  A.row_tile = kHalves ? 64 : 128;
   LaunchScope scope("attention_query_grad", s);
   hipLaunchKernelGGL((query_grad_kernel<T, DP, kKeys, kHalves>), dim3(unsigned(blocks)),
                      dim3(kThreads), kLds, s, A);
@@ -646,6 +718,23 @@ int launch_backward(BackwardArgs &A, const Splits &splits, hipStream_t s) {
   return launch_keys<T, DP, false>(A, splits, s);
 }
 
+size_t aligned(size_t bytes) { return (bytes + 255) / 256 * 256; }
+
+size_t stats_bytes(int64_t q_total, int q_heads) {
+  return aligned(size_t(q_total) * size_t(q_heads) * sizeof(float2));
+}
+
+// Places for the tops of a key head: 2 of every tile of 64 rows, or 4 of 128.
+int64_t tops_of_head(int64_t q_total, int group, int sequences) {
+  return q_total * group / 32 + 4 * (int64_t(sequences) + 1);
+}
+
+size_t tops_bytes(int64_t q_total, int group, int k_heads, int dtype, int sequences) {
+  return dtype == BEVPOOL_F16
+             ? aligned(size_t(tops_of_head(q_total, group, sequences)) * k_heads * sizeof(float))
+             : 0;
+}
+
 }  // namespace
 
 extern "C" {
@@ -655,10 +744,9 @@ size_t bevpool_attention_backward_scratch_bytes(int64_t q_total, int64_t k_total
                                                 int32_t sequences) {
   if (q_total < 1 || q_heads < 1 || k_heads < 1 || k_total < 0 || sequences < 0) return 0;
   const int elem = dtype == BEVPOOL_F32 ? 4 : 2;
-  const size_t stats = size_t(q_total) * size_t(q_heads) * sizeof(float2);
   const int group = q_heads / k_heads;
   const Splits s = plan_for(q_total, k_total, group, k_heads, dim, elem, sequences, 1);
-  return (stats + 255) / 256 * 256 +
+  return stats_bytes(q_total, q_heads) + tops_bytes(q_total, group, k_heads, dtype, sequences) +
          split_bytes(s, q_total, k_total, group, k_heads, dim, elem, sequences);
 }
 
@@ -704,8 +792,12 @@ int bevpool_attention_backward(const void *q, int64_t q_row, int64_t q_head, con
   A.stats = static_cast<float2 *>(scratch);
   Splits splits =
       plan_for(q_total, k_total, A.group.size, k_heads, dim, elem, sequences, A.causal);
-  const size_t stats_bytes = (size_t(q_total) * q_heads * sizeof(float2) + 255) / 256 * 256;
-  splits.sums = reinterpret_cast<float *>(static_cast<char *>(scratch) + stats_bytes);
+  A.row_tile = 128;  // (no queries, no query kernel to set it)
+  char *at = static_cast<char *>(scratch) + stats_bytes(q_total, q_heads);
+  A.tops = reinterpret_cast<float *>(at);
+  A.tops_stride = int(tops_of_head(q_total, A.group.size, sequences));
+  at += tops_bytes(q_total, A.group.size, k_heads, dtype, sequences);
+  splits.sums = reinterpret_cast<float *>(at);
   hipStream_t s = static_cast<hipStream_t>(stream);
   return dtype == BEVPOOL_BF16  ? (ATTENTION_DIM(__bf16, launch_backward, A, splits, s))
          : dtype == BEVPOOL_F16 ? (ATTENTION_DIM(_Float16, launch_backward, A, splits, s))

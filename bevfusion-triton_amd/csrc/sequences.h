@@ -105,14 +105,14 @@ constexpr RowTile row_tile(const Starts &s, int group, int tile, int index, Wave
 // of them, in `tiles` tiles of tile_rows.
 struct KeyTile {
   Sequence seq;
-  int kb, begin, rows, tiles;
+  int which, kb, begin, rows, tiles;
   bool on;
 };
 template <typename Wave>
 constexpr KeyTile key_tile(const Starts &s, int group, bool causal, int keys, int tile_rows,
                            int index, Wave wave) {
   const int which = find_sequence(s.k, s.n, s.k_total, 1, keys, index, wave);
-  KeyTile t = {sequence_at(s, which), 0, 0, 0, 0, false};
+  KeyTile t = {sequence_at(s, which), which, 0, 0, 0, 0, false};
   if (which == s.n) t.seq.nk = s.k_total - t.seq.k0;  // keys of no sequence: no queries
   t.kb = (index - first_tile(s.k, which, s.k_total, 1, keys)) * keys;
   t.rows = t.seq.nq * group;

@@ -135,6 +135,80 @@ def test_long_walks_of_a_full_card(pkg, cuda, dim, dtype):
         assert torch.equal(first[n], again[n]), n
 
 
+def check_far(pkg, cuda, case, causal, scale=None):
+    """fp16 gradients of a dout far from 1, against the bound of the same dout
+    brought to between 1 and 2: gradients are linear in it, and all that their
+    own size costs is the last rounding."""
+    dtype = case['q'].dtype
+    got = run(pkg, cuda, case, causal, scale)
+    by = 2.0 ** case['dout'].abs().max().double().log2().floor().item()
+    want = ref.attend_packed(case['q'], case['k'], case['v'], case['q_starts'], case['k_starts'],
+                             causal, case['q'].shape[-1] ** -0.5 if scale is None else scale,
+                             case['dout'].double() / by, dtype)
+    tiny = ref.TINY[dtype]
+    for n in ('dq', 'dk', 'dv'):
+        value, bound = want[n]
+        want[n] = value * by, (bound - tiny) * by + tiny
+    compare(got, want)
+    return want
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('small', ['q', 'k'])
+@pytest.mark.parametrize('dim', [32, 80, 128])
+def test_small_gradients_fp16(pkg, cuda, dim, small):
+    """A dout of 1e-5 over hundreds of keys: score gradients far below what the
+    type can hold."""
+    for lengths, heads in ((([300, 9], [700, 30]), (4, 2)),
+                           (([3] * 25 + [1100] + [3] * 35,) * 2, (16, 8))):
+        case = make(*lengths, *heads, dim, torch.float16)
+        case[small] = (case[small].float() * 0.02).half()
+        case['dout'] = (case['dout'].float() * 1e-5).half()
+        check_far(pkg, cuda, case, heads[0] == 16, scale=64.0 * dim ** -0.5)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('dim', [32, 64, 80, 128])
+def test_large_gradients_fp16(pkg, cuda, dim):
+    """Gradients that fp16 can hold where those of the scores pass its range."""
+    case = make([40, 3, 90], [40, 3, 90], 4, 2, dim, torch.float16)
+    case['v'] = case['v'] * 4
+    case['k'] = case['k'] * 0.5
+    case['dout'] = case['dout'] * (5000 if dim < 64 else 4000)
+    want = check_far(pkg, cuda, case, True)
+    assert all(want[n][0].abs().max() < 60000 for n in ('dq', 'dk', 'dv'))
+    a, most = 0, 0.0  # the scores' own
+    for n in (40, 3, 90):
+        for h in range(4):
+            rows = slice(a, a + n)
+            p = ref.attend_rows(case['q'][rows, h].double(), case['k'][rows, h // 2].double(),
+                                case['v'][rows, h // 2].double(), list(range(1, n + 1)),
+                                dim ** -0.5)[0]
+            dp = case['dout'][rows, h].double() @ case['v'][rows, h // 2].double().T
+            most = max(most, (p * (dp - (p * dp).sum(-1, keepdim=True))).abs().max().item())
+        a += n
+    assert most > 66000
+
+
+@pytest.mark.gpu
+def test_rows_of_far_gradients_fp16(pkg, cuda):
+    """Rows whose dout lies 2^20 apart: each row's dq is as good as alone, and
+    zeros, infinities and NaN in dout keep to their row's dq."""
+    case = make([200], [200], 4, 2, 64, torch.float16)
+    case['dout'][::2] = (case['dout'][::2].float() * 2.0 ** -20).half()
+    case['dout'][5] = 0
+    alone = dict(case, dout=case['dout'].clone())
+    alone['dout'][1::2] = 0
+    got, even = run(pkg, cuda, case, False), run(pkg, cuda, alone, False)
+    assert torch.equal(got['dq'][::2], even['dq'][::2])
+    assert not bool(got['dq'][5].any())
+    case['dout'][7, 0, 3], case['dout'][8, 1, 2] = float('inf'), float('nan')
+    far = run(pkg, cuda, case, False)
+    keep = [i for i in range(200) if i not in (7, 8)]
+    assert torch.equal(far['dq'][keep], got['dq'][keep])
+    assert bool(far['dq'][8, 1].isnan().all()) and not bool(far['dq'][7, 0].isfinite().any())
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize('dtype', DTYPES)
 def test_parts_of_one_projection(pkg, cuda, dtype):
