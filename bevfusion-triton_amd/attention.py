@@ -323,7 +323,8 @@ def attend_packed(q, k, v, q_starts, k_starts=None, *, causal=False, scale=None,
     no key or is in no sequence gives zeros and passes no gradient.  Values of
     other sequences and of rows of none never matter, but a key or value that is
     not finite may reach the queries of its own sequence that do not see it
-    (weights of zero times infinity, as where all keys are multiplied).  With
+    (weights of zero times infinity, as where all keys are multiplied), and a
+    query or gradient that is not the keys that it does not see.  With
     ``return_lse`` also the logarithm of each query's sum of exponentials,
     (q_total, q_heads) fp32 (-inf without keys, no gradient)."""
     for name, x in (('q', q), ('k', k), ('v', v)):
@@ -402,7 +403,8 @@ def attend_cached(q, k, v, lengths, prefix_k=None, prefix_v=None, *, scale=None)
     new tokens' among them (taken as within [0, capacity]).  prefix_k, prefix_v (prefix, k_heads, dim) or
     None.  New token i sees the whole prefix and the first lengths - (tokens -
     1 - i) keys of its request's cache; what lies past a length is never read.
-    A row that sees nothing gives zeros.  Returns q's shape, contiguous.  Heads
+    A row that sees nothing gives zeros; a new token's key or value that is not
+    finite may reach the tokens before it.  Returns q's shape, contiguous.  Heads
     and scale are as in :func:`attend_packed`.  No gradient."""
     single = q.dim() == 3
     if single:

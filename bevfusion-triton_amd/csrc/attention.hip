@@ -25,11 +25,11 @@ using bevpool_host::LaunchScope;
 // the matrix instructions bound it (busy in 61% of the cycles at the rate that
 // a large library product reaches, heads of 128).  128 rows a block, so that a wave's query
 // and output rows stay in registers and two blocks a CU hide each other's
-// softmax.  One causal sequence of 32,768 over 8 heads of 128 in bf16: 2.01 ms
+// softmax.  Times by events, steps one after another.  One causal sequence of 32,768 over 8 heads of 128 in bf16: 2.01 ms
 // or 1,090 TFLOP/s, where a library product of 8,192^3 reaches 1,110; 11
-// prompts of up to 4,096, 16 heads over 4: 240 us, 870 TFLOP/s; six cameras of
-// 2,816 tokens, heads of 80 (a sixth of the product is padding to 96): 331 us,
-// 740 TFLOP/s; 9 windows of 900 in fp32, heads of 32: 61 us, 61 TFLOP/s,
+// prompts of up to 4,096, 16 heads over 4: 237 us, 880 TFLOP/s; six cameras of
+// 2,816 tokens, heads of 80 (a sixth of the product is padding to 96): 308 us,
+// 790 TFLOP/s; 9 windows of 900 in fp32, heads of 32: 61 us, 61 TFLOP/s,
 // one wave a SIMD and its walk.
 template <typename T, int DP, int kKeys, bool kHalves>
 __global__ __launch_bounds__(kThreads, sizeof(T) == 4 && DP > 64 ? 1 : 2) void packed_forward_kernel(

@@ -66,10 +66,10 @@ __device__ __forceinline__ float row_dot(const Frags<T, DP> &a, const Frags<T, D
 //
 // Three products of 2 dim operations a pair.  The matrix instructions are busy
 // in half of the cycles: two waves a SIMD, and of each block of 32 keys the
-// exponentials stand between the second product and the third.  In bf16, 11 causal prompts of up to 4,096 over heads of 128: 336 us,
-// 930 TFLOP/s; six cameras of 2,816 tokens, heads of 80: 465 us, 790 TFLOP/s
-// (of 80 of the 96 columns that it computes).  fp32, 9 windows of 900, heads
-// of 32: 81 us.
+// exponentials stand between the second product and the third.  By events, in
+// bf16: 11 causal prompts of up to 4,096 over heads of 128 331 us, 940 TFLOP/s;
+// six cameras of 2,816 tokens, heads of 80, 406 us, 900 TFLOP/s (of 80 of the
+// 96 columns that it computes).  fp32, 9 windows of 900, heads of 32: 81 us.
 template <typename T, int DP, int kKeys, bool kHalves>
 __global__ __launch_bounds__(kThreads, sizeof(T) == 4 && DP > 64 ? 1 : 2) void query_grad_kernel(
     BackwardArgs A) {
@@ -292,11 +292,11 @@ struct Splits {
 // and dout read from LDS twice (as rows for one product, as columns for the
 // next) and a barrier a tile.  The exponentials run beside the products of dP:
 // with the sums of q k begun at -L / scale they wait for no read, and the mask
-// is apart from them, with one branch for all.  In bf16, six cameras of 2,816
-// tokens, heads of 80, dk and dv together: 600 us, 810 TFLOP/s (before, 719);
-// 11 causal prompts of up to 4,096, 16 heads over 4 of 128: dk 375 us, 830
-// TFLOP/s, dv 295 us, 700 TFLOP/s (446 and 351), sums of the cuts 26 us.  fp32,
-// 9 windows of 900, heads of 32: 108 us.
+// is apart from them, with one branch for all (profiled, 719 us became 605).  By
+// events, in bf16: six cameras of 2,816 tokens, heads of 80, dk and dv together
+// 537 us, 910 TFLOP/s; 11 causal prompts of up to 4,096, 16 heads over 4 of
+// 128, dk 369 us, 850 TFLOP/s, dv 281 us, 740 TFLOP/s, sums of the cuts 29 us.
+// fp32, 9 windows of 900, heads of 32: 115 us.
 template <typename T, int DP, bool kHalves, bool kDk, bool kDv>
 __global__ __launch_bounds__(kThreads, (KeyPlan<T, DP, kHalves>::kBlocksPerCu)) void
 key_grad_kernel(BackwardArgs A, Splits splits) {

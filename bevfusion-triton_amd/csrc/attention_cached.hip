@@ -372,6 +372,12 @@ CachedPlan plan_cached(bool f32, int requests, int tokens, int capacity, int pre
     // 27 and 28, 41 and 52.  Float is bound by its matrix instructions, and
     // its tiles by rows hold half the keys: 4 heads of 64, 56 and 31 at 64
     // rows, 94 and 76 at 256, 312 and 264 at 1024.
+    // Parts: by rows one block a CU, by keys two, for a part costs its sums and
+    // the join.  us at half the blocks, as it is, twice and four times: 256
+    // rows by rows, heads of 128, 16,896 keys 74, 55, 57 and 64, 4,096 keys 34,
+    // 33, 40 and 50, heads of 64, 32,768 keys 44, 37, 37 and 46; 1,024 rows
+    // (each tile for 32 parts and more) 241, 156, 142 and 139; by keys in fp32,
+    // 64 rows 40, 31, 37 and 37, 1,024 rows 313, 261, 330 and 226.
     p.by_rows = !f32 && rows > 64;
     p.shared_tiles = int(p.by_rows ? (rows + 127) / 128 : (rows + 31) / 32);
     p.shared_range = range_for(int64_t(k_heads) * p.shared_tiles, prefix, p.by_rows ? 256 : 512,

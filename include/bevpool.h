@@ -606,7 +606,11 @@ int bevpool_attention_forward(const void *q, int64_t q_row, int64_t q_head, cons
  * dk and dv (k_total, k_heads, dim), contiguous, every row written (zeros for
  * queries that see no key and keys that no query sees).  dout has strides of
  * its own, out is contiguous.  No atomics: the same call gives the same bits.
- *   scratch   >= bevpool_attention_backward_scratch_bytes(...)
+ * fp16: dout may be of any size; gradients are as good as their own rounding
+ * while the sums of |v| over a head stay below 2^13.
+ *   scratch   >= bevpool_attention_backward_scratch_bytes(...): 8 bytes a
+ *             query and head, and what the sums of cut walks may need, which
+ *             can be several times dk and dv (the lengths are not known)
  */
 size_t bevpool_attention_backward_scratch_bytes(int64_t q_total, int64_t k_total, int32_t q_heads,
                                                 int32_t k_heads, int32_t dim, int32_t dtype,
