@@ -26,6 +26,8 @@ The directory name is not a Python identifier; load it with
 from . import legacy
 from ._lib import BevPoolError, LibraryNotBuilt, library
 from .attention import attend_cached, attend_packed, axis_frequencies, norm_rotate
+from .block import (CheckpointLinear, Int8Linear, PackedActivations, checkpoint_linear, gated_activation, linear_int8,
+                    pack_activations, quantize_weight, residual_norm)
 from .bev_pool import BevPoolFunction, BevPoolIndexExport, bev_pool, check_errors
 from .tokens import TokenAttention
 from .vtransform import (BevPoolTransform, CameraIndex, LSSIndexExport, create_frustum, gen_dx_bx, host_grid, lss_bev_pool, lss_bev_pool_depth,
@@ -37,21 +39,30 @@ __all__ = [
     'BevPoolIndexExport',
     'BevPoolTransform',
     'CameraIndex',
+    'CheckpointLinear',
+    'Int8Linear',
     'LSSIndexExport',
     'LibraryNotBuilt',
+    'PackedActivations',
     'TokenAttention',
     'attend_cached',
     'attend_packed',
     'axis_frequencies',
     'bev_pool',
     'check_errors',
+    'checkpoint_linear',
     'create_frustum',
+    'gated_activation',
     'gen_dx_bx',
     'host_grid',
     'legacy',
     'library',
+    'linear_int8',
     'lss_bev_pool',
     'lss_bev_pool_depth',
     'lss_index_cameras',
     'norm_rotate',
+    'pack_activations',
+    'quantize_weight',
+    'residual_norm',
 ]

@@ -158,6 +158,33 @@ _SIGNATURES = {
          _vp],
         ctypes.c_int,
     ),
+    'bevpool_checkpoint_pitch': ([_i32], _i64),
+    'bevpool_checkpoint_pack': ([_vp, _i64, _i32, _i64, _i32, _vp, _vp], ctypes.c_int),
+    'bevpool_checkpoint_unpack': ([_vp, _i32, _i64, _i32, _vp, _vp], ctypes.c_int),
+    'bevpool_residual_norm_forward': (
+        [_vp, _i64, _i32, _vp, _i64, _vp, _vp, _vp, _i64, _i64, _vp, _i32, _i64, _i32, _f32, _vp,
+         _vp, _vp, _vp, _vp],
+        ctypes.c_int,
+    ),
+    'bevpool_residual_norm_backward_scratch_bytes': ([_i64, _i32, _i64], _sz),
+    'bevpool_residual_norm_backward': (
+        [_vp, _i64, _i32, _vp, _i64, _vp, _vp, _vp, _i64, _i64, _vp, _i32, _vp, _i64, _vp, _i64,
+         _i32, _i64, _i32, _f32, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp],
+        ctypes.c_int,
+    ),
+    'bevpool_gated_forward': (
+        [_vp, _i64, _i32, _i64, _i32, _i32, _vp, _vp, _vp], ctypes.c_int,
+    ),
+    'bevpool_gated_backward': (
+        [_vp, _i64, _i32, _vp, _i64, _i32, _i64, _i32, _i32, _vp, _vp], ctypes.c_int,
+    ),
+    'bevpool_linear8_pitch': ([_i32], _i64),
+    'bevpool_linear8_codes': ([_vp, _i64, _i32, _i64, _i32, _vp, _vp, _vp], ctypes.c_int),
+    'bevpool_linear8_scratch_bytes': ([_i64, _i32], _sz),
+    'bevpool_linear8': (
+        [_vp, _i64, _i32, _vp, _i64, _vp, _vp, _i64, _i32, _i64, _vp, _vp, _sz, _vp],
+        ctypes.c_int,
+    ),
     'bevpool_timing_enable': ([ctypes.c_int], ctypes.c_int),
     'bevpool_timing_reset': ([], ctypes.c_int),
     'bevpool_timing_read': (

@@ -1,0 +1,492 @@
+"""Operators of the block around the attention on MI355X: what a transformer on
+camera and BEV tokens does between its attention layers, as HIP kernels behind
+the same C ABI (``include/bevpool.h``); the reference has no counterpart.
+
+  * :func:`residual_norm`      norms after and before a block, fused with the
+                               residual, its gate and its scale
+  * :func:`gated_activation`   act(a) b of a projection's two halves
+  * :func:`checkpoint_linear`  a linear layer that keeps its input in 8 bits
+  * :func:`pack_activations`   such an 8-bit checkpoint by itself
+  * :func:`linear_int8`        products in 8-bit integers, for serving, of
+                               weights from :func:`quantize_weight`
+
+The first three have gradients.  With ``checkpoint=8`` the backward pass works
+from 8-bit copies of what the forward read, a little over half of the memory of
+16-bit ones: blocks of 32 values along a row share the least power of two p with
+127 p >= their largest magnitude, and each is rounded to a multiple of p (ties
+to even).  A value that is not finite comes back as NaN, and no other does.
+
+Rows are the leading dimensions; their strides are free, a row's values are
+copied where they are not neighbours.  Calls run on torch's current stream,
+allocate with torch's allocator and never wait for the device.
+"""
+from __future__ import annotations
+
+import torch
+from torch import nn
+from torch.autograd.function import once_differentiable
+
+from . import _lib as L
+from . import _pipeline as P
+from .attention import _recorded, _run, _unit, _wants_grad
+
+ACTIVATIONS = {'silu': 0, 'gelu': 1, 'sigmoid': 2}
+MAX_RESIDUAL_WIDTH = 8192
+MAX_GATED_WIDTH = 1 << 18
+MAX_INT8_WIDTH = 1 << 17
+
+
+def _rows(x):
+    """x as (rows, width) with unit stride along the width."""
+    x = x.unsqueeze(0) if x.dim() == 1 else x.flatten(0, -2)
+    return _unit(x)
+
+
+def _row(x):
+    """(address, row stride) for a call; of nothing: (0, 0)."""
+    return (x.data_ptr(), x.stride(0)) if x is not None else (0, 0)
+
+
+def _check_type(name, x, dtype=None):
+    if x.dtype not in L.DTYPE_CODES:
+        raise TypeError(f'{name} must have dtype torch.float16, torch.float32, or torch.bfloat16.')
+    if dtype is not None and x.dtype != dtype:
+        raise TypeError(f'{name} must have dtype {dtype}.')
+
+
+def _check_device(like, **tensors):
+    for name, t in tensors.items():
+        if t is not None and t.device != like.device:
+            raise ValueError(f'{name} must be on the device of x ({like.device}).')
+
+
+def _check_checkpoint(checkpoint):
+    if checkpoint not in (None, 8):
+        raise ValueError('checkpoint must be None or 8.')
+    return checkpoint is not None
+
+
+def _kept(x, rows, width, copies=1):
+    """Room for an 8-bit checkpoint of rows."""
+    pitch = L.library().bevpool_checkpoint_pitch(width)
+    return x.new_empty((rows, copies * pitch), dtype=torch.uint8)
+
+
+# ---- residual and norms ----------------------------------------------------
+
+def _gate(gate):
+    """(address, row stride, rows) for a call."""
+    return (*_row(gate), gate.shape[0] if gate is not None else 0)
+
+
+def _residual_norm(x, update, update_weight, scale, gate, weight, dtype, eps, keep=False):
+    """(sum, normed, checkpoint of x, of update) of rows."""
+    rows, width = x.shape
+    total = None if update is None else torch.empty_like(x, memory_format=torch.contiguous_format)
+    normed = None if weight is None else x.new_empty(x.shape, dtype=dtype)
+    # (the norm before the next block alone needs x for its gradient)
+    x_kept = _kept(x, rows, width) if keep and weight is not None else None
+    update_kept = _kept(x, rows, width) if keep and update is not None else None
+    _run(lambda lib, s: lib.bevpool_residual_norm_forward(
+        *_row(x), L.DTYPE_CODES[x.dtype], *_row(update), L.ptr(update_weight), L.ptr(scale),
+        *_gate(gate), L.ptr(weight), L.DTYPE_CODES[dtype], rows, width, eps, L.ptr(total),
+        L.ptr(normed), L.ptr(x_kept), L.ptr(update_kept), s), x.device,
+        'bevpool_residual_norm_forward')
+    return total, normed, x_kept, update_kept
+
+
+class _ResidualNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, update, update_weight, scale, gate, weight, dtype, eps, keep):
+        total, normed, x_kept, update_kept = _residual_norm(x, update, update_weight, scale, gate,
+                                                            weight, dtype, eps, keep)
+        if not keep:
+            x_kept, update_kept = x if weight is not None else None, update
+        ctx.save_for_backward(x_kept, update_kept, update_weight, scale, gate, weight)
+        ctx.call = (*x.shape, x.dtype, x.device, dtype, eps, keep, update is not None)
+        ctx.set_materialize_grads(False)
+        return total, normed
+
+    @staticmethod
+    @once_differentiable  # (the gradients are no functions of the graph's)
+    def backward(ctx, dtotal, dnormed):
+        x, update, update_weight, scale, gate, weight = ctx.saved_tensors
+        rows, width, x_dtype, device, dtype, eps, keep, has_update = ctx.call
+        if dtotal is None and dnormed is None:
+            return (None,) * 9
+        with_norm = weight if dnormed is not None else None
+        dtotal, dnormed = (g if g is None else _unit(g if g.dtype == t else g.to(t))
+                           for g, t in ((dtotal, x_dtype), (dnormed, dtype)))
+
+        def room(*shape, kind=dtype):
+            return torch.empty(shape, dtype=kind, device=device)
+
+        dx = room(rows, width, kind=x_dtype)
+        dupdate = room(rows, width) if has_update else None
+        # (no kernel writes the sums of no rows)
+        dgate = None if gate is None else room(*gate.shape) if rows else torch.zeros_like(gate)
+        dupdate_weight, dscale, dweight = (
+            t if t is None else room(width) for t in (update_weight, scale, with_norm))
+        nbytes = L.library().bevpool_residual_norm_backward_scratch_bytes(
+            rows, width, gate.shape[0] if gate is not None else 0)
+        scratch = room(nbytes, kind=torch.uint8)
+        _run(lambda lib, s: lib.bevpool_residual_norm_backward(
+            *_row(x if with_norm is not None else None), L.DTYPE_CODES[x_dtype], *_row(update),
+            L.ptr(update_weight), L.ptr(scale), *_gate(gate), L.ptr(with_norm), int(keep),
+            *_row(dtotal), *_row(dnormed), L.DTYPE_CODES[dtype], rows, width, eps, L.ptr(dx),
+            L.ptr(dupdate), L.ptr(dgate), L.ptr(dupdate_weight), L.ptr(dscale), L.ptr(dweight),
+            L.ptr(scratch), nbytes, s), device, 'bevpool_residual_norm_backward')
+        if weight is not None and with_norm is None:
+            dweight = torch.zeros_like(weight)
+        return dx, dupdate, dupdate_weight, dscale, dgate, dweight, None, None, None
+
+
+def residual_norm(x, update=None, *, update_weight=None, scale=None, gate=None, weight=None,
+                  eps=1e-6, checkpoint=None):
+    """A block's output joins the residual stream, and the next block's input
+    is normed, in one pass; returns (sum, normed).
+
+        n      = update / sqrt(mean(update^2) + eps) * update_weight
+                 (without update_weight: update)
+        sum    = x + scale * gate * n
+        normed = sum / sqrt(mean(sum^2) + eps) * weight
+                 (None without weight; in fp32, of the sum before its rounding)
+
+    x (..., width): the stream, fp32 or the type of the others; update
+    (..., width): the block's output, or None: the norm alone, of x, which is
+    then the sum.  update_weight, scale, weight (width,).  gate: of x's shape,
+    or (groups, width), a row for each of `groups` equal parts of the rows in
+    order, or (width,).  width at most 8192.
+
+    Gradients flow to all of them.  ``checkpoint=8`` keeps 8-bit copies of x
+    and update for them instead of x and update; the gradients are those at
+    the values that the copies stand for."""
+    keep = _check_checkpoint(checkpoint)
+    _check_type('x', x)
+    if x.dim() < 1:
+        raise ValueError('x must have shape [..., width].')
+    width = x.shape[-1]
+    if not 1 <= width <= MAX_RESIDUAL_WIDTH:
+        raise ValueError(f'width must be in [1, {MAX_RESIDUAL_WIDTH}].')
+    if update is None and not (update_weight is scale is gate is None):
+        raise ValueError('update_weight, scale and gate are of an update.')
+    if update is None and weight is None:
+        raise ValueError('neither an update nor a weight: nothing to do.')
+    if not eps >= 0:
+        raise ValueError('eps must not be negative.')
+    dtype = weight.dtype if update is None else update.dtype
+    if update is not None:
+        _check_type('update', update)
+        if update.shape != x.shape:
+            raise ValueError('update must have the shape of x.')
+    for name, t in (('update_weight', update_weight), ('scale', scale), ('weight', weight)):
+        if t is not None:
+            _check_type(name, t, dtype)
+            if tuple(t.shape) != (width,):
+                raise ValueError(f'{name} must have shape [width].')
+    if x.dtype not in (dtype, torch.float32):
+        raise TypeError(f'x must have dtype torch.float32 or that of the others ({dtype}).')
+    rows = x.numel() // width
+    if gate is not None:
+        _check_type('gate', gate, dtype)
+        if gate.shape != x.shape and not (gate.dim() in (1, 2) and gate.shape[-1] == width):
+            raise ValueError('gate must have the shape of x, [groups, width] or [width].')
+        gate = _rows(gate)
+        if gate.shape[0] < min(rows, 1) or gate.shape[0] and rows % gate.shape[0]:
+            raise ValueError('the rows of gate must divide those of x.')
+    P.require_gpu(*[t for t in (x, update, update_weight, scale, gate, weight) if t is not None])
+    _check_device(x, update=update, update_weight=update_weight, scale=scale, gate=gate,
+                  weight=weight)
+    weights = [t if t is None else t.contiguous() for t in (update_weight, scale)]
+    weight = weight if weight is None else weight.contiguous()
+    args = (_rows(x), None if update is None else _rows(update), *weights, gate, weight, dtype,
+            float(eps))
+    if _wants_grad(x, update, *weights, gate, weight) or _recorded():
+        total, normed = _ResidualNorm.apply(*args, keep)
+    else:
+        total, normed = _residual_norm(*args)[:2]
+    return (x if total is None else total.view(x.shape),
+            normed if normed is None else normed.view(x.shape))
+
+
+# ---- gated activation ------------------------------------------------------
+
+def _gated(x, kind, keep=False):
+    rows, width = x.shape[0], x.shape[1] // 2
+    out = x.new_empty((rows, width))
+    kept = _kept(x, rows, width, 2) if keep else None
+    _run(lambda lib, s: lib.bevpool_gated_forward(
+        *_row(x), L.DTYPE_CODES[x.dtype], rows, width, kind, L.ptr(out), L.ptr(kept), s),
+        x.device, 'bevpool_gated_forward')
+    return out, kept
+
+
+class _Gated(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, kind, keep):
+        out, kept = _gated(x, kind, keep)
+        ctx.save_for_backward(kept if keep else x)
+        ctx.call = (x.dtype, kind, keep)
+        return out
+
+    @staticmethod
+    @once_differentiable  # (the gradients are no functions of the graph's)
+    def backward(ctx, dout):
+        x, = ctx.saved_tensors
+        dtype, kind, keep = ctx.call
+        dout = _unit(dout if dout.dtype == dtype else dout.to(dtype))
+        rows, width = dout.shape
+        dx = dout.new_empty((rows, 2 * width))
+        _run(lambda lib, s: lib.bevpool_gated_backward(
+            *_row(x), int(keep), *_row(dout), L.DTYPE_CODES[dtype], rows, width, kind, L.ptr(dx),
+            s), dout.device, 'bevpool_gated_backward')
+        return dx, None, None
+
+
+def gated_activation(x, kind='silu', *, checkpoint=None):
+    """act(a) * b of the two halves a, b of x's rows: x (..., 2 width) ->
+    (..., width).  kind: 'silu' a / (1 + exp(-a)), 'gelu' (of the normal
+    distribution's integral) or 'sigmoid'.  width at most 2^18.  The gradient
+    flows to x; ``checkpoint=8`` keeps an 8-bit copy of x for it instead of x,
+    each half in blocks of its own."""
+    keep = _check_checkpoint(checkpoint)
+    _check_type('x', x)
+    if kind not in ACTIVATIONS:
+        raise ValueError(f'kind must be one of {", ".join(ACTIVATIONS)}.')
+    if x.dim() < 1 or x.shape[-1] % 2 or not 2 <= x.shape[-1] <= 2 * MAX_GATED_WIDTH:
+        raise ValueError(f'x must have shape [..., 2 width], width in [1, {MAX_GATED_WIDTH}].')
+    P.require_gpu(x)
+    rows, kind = _rows(x), ACTIVATIONS[kind]
+    if _wants_grad(x) or _recorded():
+        out = _Gated.apply(rows, kind, keep)
+    else:
+        out = _gated(rows, kind)[0]
+    return out.view(*x.shape[:-1], x.shape[-1] // 2)
+
+
+# ---- 8-bit checkpoints -----------------------------------------------------
+
+class PackedActivations:
+    """An 8-bit checkpoint of a tensor: :meth:`unpack` gives the values that it
+    stands for, in the tensor's type and shape.  33 bytes for 32 values."""
+
+    def __init__(self, data, shape, dtype):
+        self.data, self.shape, self.dtype = data, shape, dtype
+
+    def unpack(self):
+        out = self.data.new_empty(self.shape, dtype=self.dtype)
+        _run(lambda lib, s: lib.bevpool_checkpoint_unpack(
+            L.ptr(self.data), L.DTYPE_CODES[self.dtype], self.data.shape[0], self.shape[-1],
+            L.ptr(out), s), self.data.device, 'bevpool_checkpoint_unpack')
+        return out
+
+
+def _pack(x):
+    rows = _rows(x)
+    data = _kept(rows, *rows.shape)
+    _run(lambda lib, s: lib.bevpool_checkpoint_pack(
+        *_row(rows), L.DTYPE_CODES[x.dtype], *rows.shape, L.ptr(data), s), x.device,
+        'bevpool_checkpoint_pack')
+    return data
+
+
+class _Pack(torch.autograd.Function):
+    """For tangents and traces alone: there is no gradient."""
+    @staticmethod
+    def forward(ctx, x):
+        return _pack(x)
+
+
+def pack_activations(x):
+    """x (..., width) as :class:`PackedActivations`, blocks of 32 values along
+    the width (at most 2^18).  fp16 and bf16 values come back exactly as the
+    type holds them (fp16: the largest at most 65504).  No gradient."""
+    _check_type('x', x)
+    if x.dim() < 1 or not 1 <= x.shape[-1] <= MAX_GATED_WIDTH:
+        raise ValueError(f'x must have shape [..., width], width in [1, {MAX_GATED_WIDTH}].')
+    P.require_gpu(x)
+    if _wants_grad(x):
+        raise RuntimeError('pack_activations has no gradient; call it under torch.no_grad()')
+    data = _Pack.apply(x) if _recorded() else _pack(x)
+    return PackedActivations(data, x.shape, x.dtype)
+
+
+class _CheckpointLinear(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias):
+        # (the weight's gradient alone needs x)
+        data = _pack(x) if ctx.needs_input_grad[1] else None
+        ctx.save_for_backward(data, weight)
+        ctx.call = (x.shape, x.dtype)
+        return nn.functional.linear(x, weight, bias)
+
+    @staticmethod
+    @once_differentiable  # (the gradients are no functions of the graph's)
+    def backward(ctx, dy):
+        data, weight = ctx.saved_tensors
+        dx = dweight = dbias = None
+        if ctx.needs_input_grad[0]:
+            dx = dy @ weight
+        if ctx.needs_input_grad[1]:
+            dweight = dy.t() @ PackedActivations(data, *ctx.call).unpack()
+        if ctx.needs_input_grad[2]:
+            dbias = dy.sum(0)
+        return dx, dweight, dbias
+
+
+def checkpoint_linear(x, weight, bias=None):
+    """x weight^T + bias as torch.nn.functional.linear, x (..., in), weight
+    (out, in), bias (out,), of one type; but what is kept of x for the
+    weight's gradient is an 8-bit copy, and the gradient is that at the values
+    it stands for.  The others are exact.  Follows autocast."""
+    _check_type('x', x)
+    if torch.is_autocast_enabled('cuda'):
+        kind = torch.get_autocast_dtype('cuda')
+        x, weight = x.to(kind), weight.to(kind)
+        bias = bias if bias is None else bias.to(kind)
+    _check_type('weight', weight, x.dtype)
+    if weight.dim() != 2 or x.dim() < 1 or x.shape[-1] != weight.shape[1]:
+        raise ValueError('x must have shape [..., in] and weight [out, in].')
+    if not 1 <= x.shape[-1] <= MAX_GATED_WIDTH:
+        raise ValueError(f'in must be in [1, {MAX_GATED_WIDTH}].')
+    if bias is not None:
+        _check_type('bias', bias, x.dtype)
+        if bias.shape != weight.shape[:1]:
+            raise ValueError('bias must have shape [out].')
+    P.require_gpu(*[t for t in (x, weight, bias) if t is not None])
+    _check_device(x, weight=weight, bias=bias)
+    if not _wants_grad(x, weight, bias) and not _recorded():
+        return nn.functional.linear(x, weight, bias)
+    # (autocast off: the operands have their types)
+    with torch.autocast('cuda', enabled=False):
+        y = _CheckpointLinear.apply(_rows(x), weight, bias)
+    return y.view(*x.shape[:-1], weight.shape[0])
+
+
+class CheckpointLinear(nn.Linear):
+    """A linear layer through :func:`checkpoint_linear`."""
+
+    def forward(self, x):
+        return checkpoint_linear(x, self.weight, self.bias)
+
+
+# ---- products in 8-bit integers --------------------------------------------
+
+def quantize_weight(weight):
+    """(codes, scales) of weight (out, in) for :func:`linear_int8`: each
+    channel's scale is the least number of 8 bits (as bf16 has) with 127 scale
+    >= its largest magnitude, its codes the multiples of the scale next to its
+    values (ties to even).  codes (out, in) int8, rows at multiples of 128 bytes; scales
+    (out,) fp32.  A channel with a value that is not finite has a scale of NaN."""
+    _check_type('weight', weight)
+    if weight.dim() != 2 or not 1 <= weight.shape[1] <= MAX_INT8_WIDTH:
+        raise ValueError(f'weight must have shape [out, in], in in [1, {MAX_INT8_WIDTH}].')
+    P.require_gpu(weight)
+    weight = _unit(weight.detach())
+    out, width = weight.shape
+    codes = weight.new_empty((out, L.library().bevpool_linear8_pitch(width)), dtype=torch.int8)
+    scales = weight.new_empty(out, dtype=torch.float32)
+    _run(lambda lib, s: lib.bevpool_linear8_codes(
+        *_row(weight), L.DTYPE_CODES[weight.dtype], out, width, L.ptr(codes), L.ptr(scales), s),
+        weight.device, 'bevpool_linear8_codes')
+    return codes[:, :width], scales
+
+
+def _code_rows(codes):
+    """(codes, row stride): rows at multiples of 16 bytes that can be read up
+    to one; codes itself, or a copy."""
+    out, width = codes.shape
+    row, one = codes.stride()
+    need = (width + 15) // 16 * 16
+    if out == 1:
+        row = need
+    end = codes.storage_offset() + (out - 1) * row + need
+    if ((one == 1 or width == 1) and need <= row < 1 << 22 and row % 16 == 0
+            and codes.data_ptr() % 16 == 0 and end <= codes.untyped_storage().nbytes()):
+        return codes, row
+    copy = codes.new_zeros((out, need))
+    copy[:, :width] = codes
+    return copy, need
+
+
+def _linear_int8(x, codes, row, scales, bias):
+    (rows, width), channels = x.shape, scales.shape[0]
+    y = x.new_empty((rows, channels))
+    nbytes = L.library().bevpool_linear8_scratch_bytes(rows, width)
+    scratch = x.new_empty(nbytes, dtype=torch.uint8)
+    _run(lambda lib, s: lib.bevpool_linear8(
+        *_row(x), L.DTYPE_CODES[x.dtype], L.ptr(codes), row, L.ptr(scales), L.ptr(bias), rows,
+        width, channels, L.ptr(y), L.ptr(scratch), nbytes, s), x.device, 'bevpool_linear8')
+    return y
+
+
+class _LinearInt8(torch.autograd.Function):
+    """For tangents and traces alone: there is no gradient."""
+    @staticmethod
+    def forward(ctx, x, codes, row, scales, bias):
+        return _linear_int8(x, codes, row, scales, bias)
+
+
+def linear_int8(x, codes, scales, bias=None):
+    """x (codes * scales)^T + bias with products in 8-bit integers: x (..., in)
+    fp32, fp16 or bf16, codes (out, in) int8 and scales (out,) fp32 as
+    :func:`quantize_weight` gives them, bias (out,) of x's type or None ->
+    (..., out).  in is at most 2^17.
+
+    Each token gets a scale (the least number of 8 bits, as bf16 has, with 127 scale >= its
+    largest magnitude) and codes, the nearest multiples of it (ties to even);
+    the sums of products of codes are exact, and are multiplied by both scales
+    in fp32.  A token with a value that is not finite gives NaN.  Rows of codes
+    that do not start at multiples of 16 bytes are copied at each call.  No
+    gradient."""
+    _check_type('x', x)
+    if codes.dim() != 2 or codes.dtype != torch.int8:
+        raise TypeError('codes must have dtype torch.int8 and shape [out, in].')
+    channels, width = codes.shape
+    if not 1 <= width <= MAX_INT8_WIDTH:
+        raise ValueError(f'in must be in [1, {MAX_INT8_WIDTH}].')
+    if x.dim() < 1 or x.shape[-1] != width:
+        raise ValueError('x must have shape [..., in], in as codes have it.')
+    if scales.dtype != torch.float32 or tuple(scales.shape) != (channels,):
+        raise ValueError('scales must have dtype torch.float32 and shape [out].')
+    if bias is not None:
+        _check_type('bias', bias, x.dtype)
+        if tuple(bias.shape) != (channels,):
+            raise ValueError('bias must have shape [out].')
+    P.require_gpu(*[t for t in (x, codes, scales, bias) if t is not None])
+    _check_device(x, codes=codes, scales=scales, bias=bias)
+    if _wants_grad(x, scales, bias):
+        raise RuntimeError('linear_int8 has no gradient; call it under torch.no_grad()')
+    bias = bias if bias is None else bias.contiguous()
+    codes, row = _code_rows(codes) if channels else (codes, 0)
+    run = _LinearInt8.apply if _recorded() else _linear_int8
+    y = run(_rows(x), codes, int(row), scales.contiguous(), bias)  # (a trace has sizes as tensors)
+    return y.view(*x.shape[:-1], channels)
+
+
+class Int8Linear(nn.Module):
+    """A linear layer for serving through :func:`linear_int8`, made of one in
+    another type: ``Int8Linear(nn.Linear(...))``.  Its scales stay fp32
+    whatever the module is cast to."""
+
+    def __init__(self, linear):
+        super().__init__()
+        self.in_features, self.out_features = linear.in_features, linear.out_features
+        codes, scales = quantize_weight(linear.weight)
+        self.register_buffer('codes', codes)
+        self.register_buffer('scales', scales)
+        self.register_buffer('bias', None if linear.bias is None else linear.bias.detach().clone())
+
+    def _apply(self, fn, *args, **kwargs):
+        scales = self.scales
+        super()._apply(fn, *args, **kwargs)
+        if self.scales.dtype != torch.float32:
+            self.scales = scales.to(self.scales.device)
+        return self
+
+    @torch.no_grad()
+    def forward(self, x):
+        if torch.is_autocast_enabled('cuda'):
+            x = x.to(torch.get_autocast_dtype('cuda'))
+        bias = self.bias if self.bias is None else self.bias.to(x.dtype)
+        return linear_int8(x, self.codes, self.scales, bias)

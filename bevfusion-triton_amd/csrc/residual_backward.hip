@@ -1,0 +1,446 @@
+// residual_backward.hip -- gradients of residual.hip's norms, gate and scale
+// (gfx950).  With D the gradient of x', H that of h, r = 1 / sqrt(mean(x'^2) +
+// eps), r_u alike of u (1 without update_weight), c = scale gate
+// update_weight:
+//
+//   G  = D + r (H weight - x' r^2 mean(H weight x'))
+//   dx = G,  dweight = sum over rows of H x' r
+//   du = r_u (G c - n mean(G c n))         (without update_weight: G c)
+//   dgate = G scale update_weight n        (summed over the rows that share it)
+//   Q  = sum over rows of G gate n:  dupdate_weight = scale Q,
+//                                    dscale = update_weight Q
+// So one sum over rows serves three gradients, and with a gate that rows
+// share, its parts (without the gate) serve dgate too.
+//
+// Bound by memory: x, u, D and H (and a gate of each value) read once, dx and
+// du (and dgate) written once.  x' and n are formed again from x and u.
+#include <hip/hip_runtime.h>
+
+#include <stdint.h>
+
+#include "bevpool.h"
+#include "host_calls.h"
+#include "residual.h"
+
+namespace residual {
+
+using bevpool_host::check_launch;
+using bevpool_host::fail;
+using bevpool_host::LaunchScope;
+
+int check(Args &A, int dtype, int x_dtype, int64_t rows, int width, int64_t gate_rows, float eps);
+
+// The groups' sums of a block, added in the groups' order, to `to`.
+template <int kLanes, int kChunks>
+__device__ __forceinline__ void flush(float (&v)[kChunks][8], float *to, int width,
+                                      const Place<kLanes, kChunks> &at, float *lds) {
+  constexpr int kGroups = threads_of(kLanes) / kLanes;
+  if constexpr (kGroups == 1) {
+    store_row<float>(to, 0, width, v, at);
+  } else {
+    __syncthreads();  // what was there has been read
+    store_row<float>(lds, at.group * width, width, v, at);
+    __syncthreads();
+    for (int c = threadIdx.x; c < width; c += threads_of(kLanes)) {
+      float s = 0.f;
+#pragma unroll
+      for (int g = 0; g < kGroups; ++g) s += lds[g * width + c];
+      to[c] = s;
+    }
+  }
+}
+
+// A block walks items, each an equal part of the rows that share a row of
+// gate (without such a gate: of all), and leaves each item's sums.
+template <typename T, typename X, int kLanes, int kChunks, bool kKept>
+__global__ __launch_bounds__(threads_of(kLanes), 1) void residual_backward_kernel(Args A) {
+  constexpr int kGroups = threads_of(kLanes) / kLanes;
+  extern __shared__ float lds[];
+  __shared__ float shared[6][2 * (threads_of(kLanes) / 64)];
+  const Place<kLanes, kChunks> at;
+  const int width = A.width;
+  const int64_t blocks = rows::blocks_of(width), pitch = rows::checkpoint_pitch(width);
+  const bool own_gate = A.gate && A.gate_each == 1;
+  const int64_t part_rows = (A.gate && !own_gate ? A.gate_each : A.rows);
+  const int64_t share = (part_rows + A.parts_each - 1) / A.parts_each;
+  float dweight[kChunks][8] = {};
+  int turn = 0;
+  for (int64_t item = blockIdx.x; item < A.items; item += gridDim.x) {
+    const int64_t owner = item / A.parts_each, part = item % A.parts_each;
+    const int64_t first = owner * part_rows;
+    const int64_t begin = first + part * share;
+    const int64_t end = min(begin + share, first + part_rows);
+    float q[kChunks][8] = {};
+    for (int64_t row = begin + at.group; row < end; row += kGroups, turn = 3 - turn) {
+      const int64_t gate_row = own_gate ? row : owner;
+      float g[kChunks][8], n[kChunks][8], c[kChunks][8], w[kChunks][8];
+      if (A.dsum) {
+        load_row<X>(g, A.dsum, row * A.dsum_row, width, at);
+      } else {
+#pragma unroll
+        for (int j = 0; j < kChunks; ++j)
+#pragma unroll
+          for (int i = 0; i < 8; ++i) g[j][i] = 0.f;
+      }
+      float r_u = 1.f;
+      if (A.update) {
+        if constexpr (kKept) {
+#pragma unroll
+          for (int j = 0; j < kChunks; ++j) {
+            if (at.left(j, width) > 0)
+              rows::load_packed(n[j], A.update_kept + row * pitch, at.chunk(j), blocks);
+            else
+#pragma unroll
+              for (int i = 0; i < 8; ++i) n[j][i] = 0.f;
+          }
+        } else {
+          load_row<T>(n, A.update, row * A.update_row, width, at);
+        }
+#pragma unroll
+        for (int j = 0; j < kChunks; ++j)
+#pragma unroll
+          for (int i = 0; i < 8; ++i) c[j][i] = 1.f;
+        if (A.scale) load_row<T>(c, A.scale, 0, width, at);
+        if (A.update_weight) {
+          float s[1] = {0.f};
+#pragma unroll
+          for (int j = 0; j < kChunks; ++j)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) s[0] += n[j][i] * n[j][i];
+          row_sums<kLanes>(s, shared[turn]);
+          r_u = 1.0f / sqrtf(s[0] * A.inv_width + A.eps);
+          load_row<T>(w, A.update_weight, 0, width, at);
+#pragma unroll
+          for (int j = 0; j < kChunks; ++j)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              n[j][i] *= r_u;
+              c[j][i] *= w[j][i];
+            }
+        }
+      }
+      if (A.weight) {
+        float x[kChunks][8], gate[kChunks][8], h[kChunks][8];
+        if constexpr (kKept) {
+#pragma unroll
+          for (int j = 0; j < kChunks; ++j) {
+            if (at.left(j, width) > 0)
+              rows::load_packed(x[j], A.x_kept + row * pitch, at.chunk(j), blocks);
+            else
+#pragma unroll
+              for (int i = 0; i < 8; ++i) x[j][i] = 0.f;
+          }
+        } else {
+          load_row<X>(x, A.x, row * A.x_row, width, at);
+        }
+        if (A.update) {
+          if (A.gate) {
+            load_row<T>(gate, A.gate, gate_row * A.gate_row, width, at);
+#pragma unroll
+            for (int j = 0; j < kChunks; ++j)
+#pragma unroll
+              for (int i = 0; i < 8; ++i) x[j][i] += n[j][i] * c[j][i] * gate[j][i];
+          } else {
+#pragma unroll
+            for (int j = 0; j < kChunks; ++j)
+#pragma unroll
+              for (int i = 0; i < 8; ++i) x[j][i] += n[j][i] * c[j][i];
+          }
+        }
+        load_row<T>(h, A.dnormed, row * A.dnormed_row, width, at);
+        load_row<T>(w, A.weight, 0, width, at);
+        float s[2] = {0.f, 0.f};
+#pragma unroll
+        for (int j = 0; j < kChunks; ++j)
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            s[0] += x[j][i] * x[j][i];
+            s[1] += h[j][i] * w[j][i] * x[j][i];
+          }
+        row_sums<kLanes>(s, shared[turn + 1]);
+        const float r = 1.0f / sqrtf(s[0] * A.inv_width + A.eps);
+        const float back = s[1] * A.inv_width * r * r;
+#pragma unroll
+        for (int j = 0; j < kChunks; ++j)
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            dweight[j][i] += h[j][i] * (x[j][i] * r);
+            g[j][i] += r * (h[j][i] * w[j][i] - x[j][i] * back);
+          }
+      }
+      store_row<X>(A.dx, row * width, width, g, at);
+      if (!A.update) continue;
+      if (A.gate) {
+        float gate[kChunks][8], dgate[kChunks][8];
+        load_row<T>(gate, A.gate, gate_row * A.gate_row, width, at);
+#pragma unroll
+        for (int j = 0; j < kChunks; ++j)
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const float t = g[j][i] * n[j][i];
+            dgate[j][i] = t * c[j][i];
+            q[j][i] += own_gate ? t * gate[j][i] : t;
+            c[j][i] *= gate[j][i];
+          }
+        if (own_gate) store_row<T>(A.dgate, row * width, width, dgate, at);
+      } else {
+#pragma unroll
+        for (int j = 0; j < kChunks; ++j)
+#pragma unroll
+          for (int i = 0; i < 8; ++i) q[j][i] += g[j][i] * n[j][i];
+      }
+#pragma unroll
+      for (int j = 0; j < kChunks; ++j)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) c[j][i] *= g[j][i];
+      if (A.update_weight) {
+        float s[1] = {0.f};
+#pragma unroll
+        for (int j = 0; j < kChunks; ++j)
+#pragma unroll
+          for (int i = 0; i < 8; ++i) s[0] += c[j][i] * n[j][i];
+        row_sums<kLanes>(s, shared[turn + 2]);
+        const float back = s[0] * A.inv_width;
+#pragma unroll
+        for (int j = 0; j < kChunks; ++j)
+#pragma unroll
+          for (int i = 0; i < 8; ++i) c[j][i] = r_u * (c[j][i] - n[j][i] * back);
+      }
+      store_row<T>(A.dupdate, row * width, width, c, at);
+    }
+    if (A.parts) flush<kLanes, kChunks>(q, A.parts + item * width, width, at, lds);
+  }
+  if (A.weight_parts)
+    flush<kLanes, kChunks>(dweight, A.weight_parts + int64_t(blockIdx.x) * width, width, at, lds);
+}
+
+constexpr int kSumThreads = 1024, kSumColumns = 64, kSlices = kSumThreads / kSumColumns;
+
+// The slices' sums, added in the slices' order; the first slice has them.
+__device__ __forceinline__ float slices_sum(float v, float *lds) {
+  __syncthreads();  // what was there has been read
+  lds[threadIdx.x] = v;
+  __syncthreads();
+  v = 0.f;
+  if (threadIdx.x < kSumColumns)
+#pragma unroll
+    for (int i = 0; i < kSlices; ++i) v += lds[i * kSumColumns + threadIdx.x];
+  return v;
+}
+
+// Sum over `n` rows of `from` of column c, in the first slice.
+__device__ __forceinline__ float column_sum(const float *from, int64_t n, int width, int c,
+                                            float *lds) {
+  float s = 0.f;
+  if (c < width) {
+#pragma unroll 8
+    for (int64_t i = threadIdx.x / kSumColumns; i < n; i += kSlices) s += from[i * width + c];
+  }
+  return slices_sum(s, lds);
+}
+
+// The gradient of a gate that rows share; with several items a row of gate
+// their sum is left in the first's place.
+template <typename T>
+__global__ __launch_bounds__(kSumThreads) void gate_sum_kernel(Args A, T *dgate) {
+  __shared__ float lds[kSumThreads];
+  const int c = blockIdx.x * kSumColumns + int(threadIdx.x) % kSumColumns;
+  for (int64_t owner = blockIdx.y; owner < A.items / A.parts_each; owner += gridDim.y) {
+    float *parts = A.parts + owner * A.parts_each * A.width;
+    const float s = column_sum(parts, A.parts_each, A.width, c, lds);
+    if (threadIdx.x >= kSumColumns || c >= A.width) continue;
+    const float w = A.update_weight ? float(static_cast<const T *>(A.update_weight)[c]) : 1.f;
+    const float scale = A.scale ? float(static_cast<const T *>(A.scale)[c]) : 1.f;
+    dgate[owner * A.width + c] = T(s * w * scale);
+    parts[c] = s;
+  }
+}
+
+// Gradients of the weights and the scale: grid.y 0 those of the update's, 1
+// that of the norm's.
+template <typename T>
+__global__ __launch_bounds__(kSumThreads) void weight_sums_kernel(Args A, int64_t weight_blocks,
+                                                                  T *dupdate_weight, T *dscale,
+                                                                  T *dweight) {
+  __shared__ float lds[kSumThreads];
+  const int c = blockIdx.x * kSumColumns + int(threadIdx.x) % kSumColumns;
+  if (blockIdx.y == 1) {
+    if (!dweight) return;
+    const float s = column_sum(A.weight_parts, weight_blocks, A.width, c, lds);
+    if (threadIdx.x < kSumColumns && c < A.width) dweight[c] = T(s);
+    return;
+  }
+  if (!dupdate_weight && !dscale) return;
+  float s = 0.f;
+  if (A.gate && A.gate_each > 1) {  // (each row of gate's own sum: gate_sum_kernel)
+    if (c < A.width) {
+      const T *gate = static_cast<const T *>(A.gate);
+#pragma unroll 4
+      for (int64_t i = threadIdx.x / kSumColumns; i < A.items / A.parts_each; i += kSlices)
+        s += A.parts[i * A.parts_each * A.width + c] * float(gate[i * A.gate_row + c]);
+    }
+    s = slices_sum(s, lds);
+  } else {
+    s = column_sum(A.parts, A.items, A.width, c, lds);
+  }
+  if (threadIdx.x >= kSumColumns || c >= A.width) return;
+  if (dupdate_weight)
+    dupdate_weight[c] = T(A.scale ? s * float(static_cast<const T *>(A.scale)[c]) : s);
+  if (dscale)
+    dscale[c] =
+        T(A.update_weight ? s * float(static_cast<const T *>(A.update_weight)[c]) : s);
+}
+
+// ---------------------------------------------------------------------------
+// host side
+// ---------------------------------------------------------------------------
+
+// Blocks: as many as the card holds at once (256 CUs, two each), or fewer
+// where there are fewer rows.
+constexpr int kBackwardBlocks = 512;
+
+struct Split {
+  int64_t items, parts_each, blocks;
+};
+Split split_for(int64_t rows, int width, int64_t gate_rows) {
+  const bool shared = gate_rows > 0 && gate_rows < rows;
+  const int64_t owners = shared ? gate_rows : 1, each = rows / owners;
+  const int64_t at_once = rows_at_once(width);
+  int64_t parts = (kBackwardBlocks + owners - 1) / owners;
+  const int64_t most = (each + at_once - 1) / at_once;
+  if (parts > most) parts = most;
+  if (parts < 1) parts = 1;
+  Split s;
+  s.parts_each = parts;
+  s.items = owners * parts;
+  s.blocks = s.items < kBackwardBlocks ? s.items : kBackwardBlocks;
+  return s;
+}
+
+template <typename T, typename X, int kLanes, int kChunks>
+void launch(const Args &A, int64_t blocks, bool kept, hipStream_t s) {
+  constexpr int kGroups = threads_of(kLanes) / kLanes;
+  const size_t lds = kGroups == 1 ? 0 : sizeof(float) * kGroups * size_t(A.width);
+  if (kept)
+    hipLaunchKernelGGL((residual_backward_kernel<T, X, kLanes, kChunks, true>),
+                       dim3(unsigned(blocks)), dim3(threads_of(kLanes)), lds, s, A);
+  else
+    hipLaunchKernelGGL((residual_backward_kernel<T, X, kLanes, kChunks, false>),
+                       dim3(unsigned(blocks)), dim3(threads_of(kLanes)), lds, s, A);
+}
+
+template <typename T, typename X>
+void launch_width(const Args &A, int64_t blocks, bool kept, hipStream_t s) {
+#define RESIDUAL_LAUNCH(kLanes, kChunks, ...) launch<T, X, kLanes, kChunks>(A, blocks, kept, s);
+  RESIDUAL_LAYOUT(RESIDUAL_LAUNCH, A.width)
+#undef RESIDUAL_LAUNCH
+}
+
+template <typename T>
+void launch_sums(const Args &A, int64_t blocks, void *dgate, void *dupdate_weight, void *dscale,
+                 void *dweight, hipStream_t s) {
+  const unsigned columns = unsigned((A.width + kSumColumns - 1) / kSumColumns);
+  const int64_t owners = A.items / A.parts_each;
+  if (A.gate && A.gate_each > 1)
+    hipLaunchKernelGGL((gate_sum_kernel<T>), dim3(columns, unsigned(owners < 4096 ? owners : 4096)),
+                       dim3(kSumThreads), 0, s, A, static_cast<T *>(dgate));
+  if (dupdate_weight || dscale || dweight)
+    hipLaunchKernelGGL((weight_sums_kernel<T>), dim3(columns, 2), dim3(kSumThreads), 0, s, A,
+                       blocks, static_cast<T *>(dupdate_weight), static_cast<T *>(dscale),
+                       static_cast<T *>(dweight));
+}
+
+}  // namespace residual
+
+extern "C" {
+
+size_t bevpool_residual_norm_backward_scratch_bytes(int64_t rows, int32_t width,
+                                                    int64_t gate_rows) {
+  using namespace residual;
+  if (rows < 1 || width < 1 || width > kMaxWidth || gate_rows < 0) return 0;
+  const Split s = split_for(rows, width, gate_rows);
+  return size_t(s.items + s.blocks) * size_t(width) * sizeof(float);
+}
+
+int bevpool_residual_norm_backward(
+    const void *x, int64_t x_row, int32_t x_dtype, const void *update, int64_t update_row,
+    const void *update_weight, const void *scale, const void *gate, int64_t gate_row,
+    int64_t gate_rows, const void *weight, int32_t kept, const void *dsum, int64_t dsum_row,
+    const void *dnormed, int64_t dnormed_row, int32_t dtype, int64_t rows, int32_t width, float eps,
+    void *dx, void *dupdate, void *dgate, void *dupdate_weight, void *dscale, void *dweight,
+    void *scratch, size_t scratch_bytes, void *stream) {
+  using namespace residual;
+  bevpool_host::clear_error();
+  Args A = {};
+  const int st = check(A, dtype, x_dtype, rows, width, gate ? gate_rows : 0, eps);
+  if (st) return st;
+  if ((update_weight && !dupdate_weight) || (scale && !dscale) || (weight && !dweight))
+    return fail(BEVPOOL_EINVAL, "a weight without the place of its gradient");
+  if ((dupdate_weight && !update_weight) || (dscale && !scale) || (dweight && !weight))
+    return fail(BEVPOOL_EINVAL, "a gradient of a weight that is not there");
+  if (rows > 0) {
+    if (gate && gate_rows < 1) return fail(BEVPOOL_EINVAL, "a gate without rows");
+    if (!update && (update_weight || scale || gate))
+      return fail(BEVPOOL_EINVAL, "update_weight, scale and gate are of an update");
+    if (!dx || (update && !dupdate) || (gate && !dgate) || (weight && (!x || !dnormed)))
+      return fail(BEVPOOL_EINVAL, "null rows");
+    if (!scratch ||
+        scratch_bytes < bevpool_residual_norm_backward_scratch_bytes(rows, width, gate_rows))
+      return fail(BEVPOOL_ESPACE, "residual_norm backward scratch too small");
+  }
+  A.x = x;
+  A.x_row = x_row;
+  A.update = update;
+  A.update_row = update_row;
+  if (kept) {
+    A.x_kept = static_cast<uint8_t *>(const_cast<void *>(x));
+    A.update_kept = static_cast<uint8_t *>(const_cast<void *>(update));
+  }
+  A.update_weight = update_weight;
+  A.scale = scale;
+  A.gate = gate;
+  A.gate_row = gate_row;
+  A.weight = weight;
+  A.dsum = dsum;
+  A.dsum_row = dsum_row;
+  A.dnormed = dnormed;
+  A.dnormed_row = dnormed_row;
+  A.dx = dx;
+  A.dupdate = dupdate;
+  A.dgate = dgate;
+  Split split = {0, 1, 0};
+  if (rows > 0) {
+    split = split_for(rows, width, gate ? gate_rows : 0);
+    A.weight_parts = weight ? static_cast<float *>(scratch) : nullptr;
+    const bool shared = gate && gate_rows < rows;
+    if (update && (update_weight || scale || shared))
+      A.parts = static_cast<float *>(scratch) + split.blocks * width;
+  }
+  A.items = split.items;
+  A.parts_each = split.parts_each;
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  if (rows > 0) {
+    LaunchScope scope("residual_norm_backward", s);
+    if (dtype == BEVPOOL_F32)
+      launch_width<float, float>(A, split.blocks, kept != 0, s);
+    else if (dtype == BEVPOOL_F16)
+      x_dtype == BEVPOOL_F32 ? launch_width<_Float16, float>(A, split.blocks, kept != 0, s)
+                             : launch_width<_Float16, _Float16>(A, split.blocks, kept != 0, s);
+    else
+      x_dtype == BEVPOOL_F32 ? launch_width<__bf16, float>(A, split.blocks, kept != 0, s)
+                             : launch_width<__bf16, __bf16>(A, split.blocks, kept != 0, s);
+    const int e = check_launch("residual_norm_backward");
+    if (e) return e;
+  }
+  // (no rows: the sums of nothing, zeros)
+  LaunchScope scope("residual_norm_sums", s);
+  if (dtype == BEVPOOL_F32)
+    launch_sums<float>(A, split.blocks, dgate, dupdate_weight, dscale, dweight, s);
+  else if (dtype == BEVPOOL_F16)
+    launch_sums<_Float16>(A, split.blocks, dgate, dupdate_weight, dscale, dweight, s);
+  else
+    launch_sums<__bf16>(A, split.blocks, dgate, dupdate_weight, dscale, dweight, s);
+  return check_launch("residual_norm_sums");
+}
+
+}  // extern "C"

@@ -1,0 +1,182 @@
+// Rows of values in registers, and their 8-bit checkpoints (gfx950): shared by
+// the kernels of the block around the attention.
+//
+// A lane holds eight neighbouring values of a row (a chunk), four lanes a
+// block of 32.  A checkpoint holds a block as 32 bytes and one for its scale:
+//   scale  2^e, e the least with 127 2^e >= the largest magnitude (e >= -126,
+//          and at most 121, so that nothing comes back infinite)
+//   value  rint(x / 2^e), ties to even, as an unsigned byte 128 higher; 0
+//          stands for a value that is not finite and comes back as NaN
+// The scale is a power of two, so that neither the quotient nor the product
+// is rounded: the byte depends on nothing but x, and what it stands for has 7
+// bits, exact in bf16.  A value is off by at most 2^-7 of its block's largest
+// magnitude, on average over normal values by 0.7% of their deviation (3 bits
+// of mantissa in 8, the other way to spend them, are 2.6%).
+// A row is the bytes of its blocks, then their scales, padded to 16 bytes.
+#pragma once
+
+#include <hip/hip_runtime.h>
+
+#include <stdint.h>
+
+namespace rows {
+
+constexpr int kChunk = 8;   // values of a lane's access
+constexpr int kBlock = 32;  // values that share a scale
+
+__host__ __device__ inline int64_t blocks_of(int64_t width) { return (width + kBlock - 1) / kBlock; }
+__host__ __device__ inline int64_t checkpoint_pitch(int64_t width) {
+  return (blocks_of(width) * (kBlock + 1) + 15) / 16 * 16;
+}
+
+// (loads and stores of 16 bytes need no more than the type's own alignment)
+template <typename T>
+struct __attribute__((packed, aligned(sizeof(T)))) Pack {
+  T v[kChunk];
+};
+
+// Values of a row from `at` on, `left` of them there (zeros behind them).
+template <typename T>
+__device__ __forceinline__ void load(float (&to)[kChunk], const T *at, int left) {
+  if (left >= kChunk) {
+    const Pack<T> p = *reinterpret_cast<const Pack<T> *>(at);
+#pragma unroll
+    for (int i = 0; i < kChunk; ++i) to[i] = float(p.v[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < kChunk; ++i) to[i] = i < left ? float(at[i]) : 0.f;
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ void store(T *at, const float (&from)[kChunk], int left) {
+  if (left >= kChunk) {
+    Pack<T> p;
+#pragma unroll
+    for (int i = 0; i < kChunk; ++i) p.v[i] = T(from[i]);
+    *reinterpret_cast<Pack<T> *>(at) = p;
+  } else {
+#pragma unroll
+    for (int i = 0; i < kChunk; ++i)
+      if (i < left) at[i] = T(from[i]);
+  }
+}
+
+template <int kControl>
+__device__ __forceinline__ unsigned dpp(unsigned v) {
+  return unsigned(__builtin_amdgcn_mov_dpp(int(v), kControl, 0xf, 0xf, true));
+}
+constexpr int kSwap1 = 0xB1, kSwap2 = 0x4E;             // lane ^ 1, lane ^ 2
+constexpr int kMirror8 = 0x141, kMirror16 = 0x140;      // within 8 and 16 lanes
+
+// Sum over kLanes (16, 32 or 64) neighbouring lanes, in all of them.
+template <int kLanes>
+__device__ __forceinline__ float lanes_sum(float v) {
+  auto add = [&](unsigned other) { v += __builtin_bit_cast(float, other); };
+  auto bits = [&] { return __builtin_bit_cast(unsigned, v); };
+  add(dpp<kSwap1>(bits()));
+  add(dpp<kSwap2>(bits()));
+  add(dpp<kMirror8>(bits()));  // (the quads hold their sums: any lane of the other does)
+  add(dpp<kMirror16>(bits()));
+  if constexpr (kLanes >= 32) {
+    const auto x = __builtin_amdgcn_permlane16_swap(bits(), bits(), false, false);
+    const unsigned a = x[0], b = x[1];
+    v = __builtin_bit_cast(float, a) + __builtin_bit_cast(float, b);
+  }
+  if constexpr (kLanes >= 64) {
+    const auto x = __builtin_amdgcn_permlane32_swap(bits(), bits(), false, false);
+    const unsigned a = x[0], b = x[1];
+    v = __builtin_bit_cast(float, a) + __builtin_bit_cast(float, b);
+  }
+  return v;
+}
+
+__device__ __forceinline__ float power(unsigned biased) {
+  return __builtin_bit_cast(float, biased << 23);
+}
+
+// A chunk as bytes, and its block's scale (a biased exponent).  The block's
+// four lanes call it together; values past a row's end are zeros.
+struct Bytes {
+  unsigned low, high;
+};
+__device__ __forceinline__ Bytes pack(const float (&v)[kChunk], unsigned &scale) {
+  constexpr unsigned kInfinite = 0x7f800000u;
+  unsigned top = 0, worst = 0;
+#pragma unroll
+  for (int i = 0; i < kChunk; ++i) {
+    const unsigned m = __builtin_bit_cast(unsigned, v[i]) & 0x7fffffffu;
+    worst = worst > m ? worst : m;
+  }
+  top = worst;
+  if (worst >= kInfinite) {  // (rare: the largest of those that are finite)
+    top = 0;
+#pragma unroll
+    for (int i = 0; i < kChunk; ++i) {
+      const unsigned m = __builtin_bit_cast(unsigned, v[i]) & 0x7fffffffu;
+      top = m < kInfinite && m > top ? m : top;
+    }
+  }
+  unsigned other = dpp<kSwap1>(top);
+  top = top > other ? top : other;
+  other = dpp<kSwap2>(top);
+  top = top > other ? top : other;
+  // 127 = 1.984375 2^6: a mantissa above 0x7E0000 takes the next exponent
+  const int e = int((top + 0x1ffffu) >> 23) - 6;
+  scale = unsigned(e < 1 ? 1 : e > 248 ? 248 : e);
+  const float inverse = power(254 - scale);
+  // Added to 1.5 2^23 a quotient is rounded to a whole number, ties to even,
+  // whose low byte is that of the sum's bits.  (Beyond 127 it gets only where
+  // the scale is at its upper end.)
+  unsigned q[kChunk];
+#pragma unroll
+  for (int i = 0; i < kChunk; ++i) {
+    const float x = __builtin_amdgcn_fmed3f(v[i] * inverse, -127.f, 127.f);
+    q[i] = __builtin_bit_cast(unsigned, x + (12582912.f + 128.f));
+  }
+  if (worst >= kInfinite) {
+#pragma unroll
+    for (int i = 0; i < kChunk; ++i)
+      if ((__builtin_bit_cast(unsigned, v[i]) & 0x7fffffffu) >= kInfinite) q[i] = 0;
+  }
+  // bytes 0 of four words
+  auto four = [](unsigned a, unsigned b, unsigned c, unsigned d) {
+    const unsigned ab = __builtin_amdgcn_perm(b, a, 0x0c0c0400u);
+    const unsigned cd = __builtin_amdgcn_perm(d, c, 0x0c0c0400u);
+    return ab | cd << 16;
+  };
+  return {four(q[0], q[1], q[2], q[3]), four(q[4], q[5], q[6], q[7])};
+}
+
+__device__ __forceinline__ void unpack(float (&v)[kChunk], Bytes b, unsigned scale) {
+  const float by = power(scale);
+#pragma unroll
+  for (int i = 0; i < kChunk; ++i)
+    v[i] = (float(((i < 4 ? b.low : b.high) >> (i % 4 * 8)) & 0xffu) - 128.f) * by;
+  // a byte of zero borrows: one test for four
+  auto zero = [](unsigned x) { return (x - 0x01010101u) & ~x & 0x80808080u; };
+  if ((zero(b.low) | zero(b.high)) != 0) {
+#pragma unroll
+    for (int i = 0; i < kChunk; ++i)
+      if ((((i < 4 ? b.low : b.high) >> (i % 4 * 8)) & 0xffu) == 0) v[i] = __builtin_nanf("");
+  }
+}
+
+// Chunk c of a row of a checkpoint.  (Chunks of the last block behind the
+// row's end are there: zeros.)
+__device__ __forceinline__ void load_packed(float (&v)[kChunk], const uint8_t *row, int c,
+                                            int64_t blocks) {
+  const Bytes b = *reinterpret_cast<const Bytes *>(row + c * int64_t(kChunk));
+  unpack(v, b, row[blocks * kBlock + c / 4]);
+}
+// The block's four lanes call it together.
+__device__ __forceinline__ void store_packed(uint8_t *row, int c, int64_t blocks,
+                                             const float (&v)[kChunk]) {
+  unsigned scale;
+  const Bytes b = pack(v, scale);
+  if (c / 4 >= blocks) return;
+  *reinterpret_cast<Bytes *>(row + c * int64_t(kChunk)) = b;
+  if (c % 4 == 0) row[blocks * kBlock + c / 4] = uint8_t(scale);
+}
+
+}  // namespace rows

@@ -657,6 +657,118 @@ int bevpool_attention_cached(const void *q, int64_t q_row, int64_t q_head, const
                              int32_t k_heads, int32_t dim, float scale, void *out, void *scratch,
                              size_t scratch_bytes, void *stream);
 
+/* -------------------------------------------------------------------------
+ * The block around the attention.  No counterpart in the reference.  Operands
+ * are (rows, width) views with unit stride along width; row strides are
+ * counted in elements.  All sums are held in fp32 (products of 8-bit integers:
+ * exactly); each result is rounded once to its type.
+ * ---------------------------------------------------------------------- */
+
+/*
+ * 8-bit checkpoints of rows: blocks of 32 values along a row share the least
+ * power of two p (2^-126 .. 2^121) with 127 p >= their largest finite
+ * magnitude; a value is held as rint(value / p) + 128, ties to even, in a
+ * byte, 0 where it is not finite (it comes back as NaN).  A row of a
+ * checkpoint is the bytes of its blocks (the last one's filled up with zeros),
+ * then a byte for each block's p (its biased exponent), and
+ * bevpool_checkpoint_pitch(width) bytes long.  width is at most 2^18.
+ *   kept         [rows][bevpool_checkpoint_pitch(width)], from a multiple of 8
+ *   out          (rows, width) contiguous (fp16: at most 65504)
+ */
+int64_t bevpool_checkpoint_pitch(int32_t width);
+
+int bevpool_checkpoint_pack(const void *x, int64_t x_row, int32_t dtype, int64_t rows,
+                            int32_t width, void *kept, void *stream);
+
+int bevpool_checkpoint_unpack(const void *kept, int32_t dtype, int64_t rows, int32_t width,
+                              void *out, void *stream);
+
+/*
+ * Norms after and before a block with the residual between them:
+ *   n      = update / sqrt(mean(update^2) + eps) * update_weight
+ *            (update_weight NULL: n = update)
+ *   sum    = x + scale * gate * n               (scale, gate NULL: 1)
+ *   normed = sum / sqrt(mean(sum^2) + eps) * weight  (weight NULL: not formed)
+ * update NULL: sum is x and is not written.
+ *   x, sum       of x_dtype: fp32 or dtype; all others of dtype
+ *   width        at most 8192
+ *   update_weight, scale, weight   [width]
+ *   gate         [gate_rows][width], gate_rows dividing rows: row i takes
+ *                gate's row i / (rows / gate_rows)
+ *   sum, normed  (rows, width) contiguous
+ *   x_kept, update_kept   8-bit checkpoints of x and update, or NULL
+ */
+int bevpool_residual_norm_forward(const void *x, int64_t x_row, int32_t x_dtype,
+                                  const void *update, int64_t update_row,
+                                  const void *update_weight, const void *scale, const void *gate,
+                                  int64_t gate_row, int64_t gate_rows, const void *weight,
+                                  int32_t dtype, int64_t rows, int32_t width, float eps, void *sum,
+                                  void *normed, void *x_kept, void *update_kept, void *stream);
+
+/*
+ * Its gradients from those of sum (dsum, NULL: zeros) and normed (with
+ * weight): dx (of x_dtype), dupdate, dgate [gate_rows][width], dupdate_weight,
+ * dscale, dweight, contiguous, each where its operand is there; sums over
+ * rows in an order that does not depend on the launch.  Without weight x may
+ * be NULL.  No rows: dgate is not written.
+ *   kept         x and update are their 8-bit checkpoints
+ *   scratch      >= bevpool_residual_norm_backward_scratch_bytes(...)
+ */
+size_t bevpool_residual_norm_backward_scratch_bytes(int64_t rows, int32_t width,
+                                                    int64_t gate_rows);
+
+int bevpool_residual_norm_backward(
+    const void *x, int64_t x_row, int32_t x_dtype, const void *update, int64_t update_row,
+    const void *update_weight, const void *scale, const void *gate, int64_t gate_row,
+    int64_t gate_rows, const void *weight, int32_t kept, const void *dsum, int64_t dsum_row,
+    const void *dnormed, int64_t dnormed_row, int32_t dtype, int64_t rows, int32_t width, float eps,
+    void *dx, void *dupdate, void *dgate, void *dupdate_weight, void *dscale, void *dweight,
+    void *scratch, size_t scratch_bytes, void *stream);
+
+/*
+ * Gated activation: out (rows, width) = act(a) * b, a the first and b the
+ * second half of x (rows, 2 width).  act: 0 a / (1 + exp(-a)), 1 a times the
+ * normal distribution's integral, 2 1 / (1 + exp(-a)).  width is at most 2^18.
+ *   out, dx      contiguous
+ *   kept         forward: 8-bit checkpoints of both halves,
+ *                [rows][2][bevpool_checkpoint_pitch(width)], or NULL;
+ *                backward: whether x is such
+ */
+int bevpool_gated_forward(const void *x, int64_t x_row, int32_t dtype, int64_t rows, int32_t width,
+                          int32_t act, void *out, void *kept, void *stream);
+
+int bevpool_gated_backward(const void *x, int64_t x_row, int32_t kept, const void *dout,
+                           int64_t dout_row, int32_t dtype, int64_t rows, int32_t width,
+                           int32_t act, void *dx, void *stream);
+
+/*
+ * Products in 8-bit integers with a scale for each token and channel:
+ *   y[t][n] = (sum over k of q[t][k] weight[n][k]) * s[t] * weight_scales[n]
+ *             + bias[n]
+ * s[t] is the least bf16 number (2^-126 or more) with 127 s[t] >= the largest
+ * magnitude of x's row t (NaN where one is not finite), q[t][k] = rint(x[t][k]
+ * / s[t]), ties to even.  bevpool_linear8_codes gives these codes, rows of
+ * bevpool_linear8_pitch(width) bytes with zeros behind the last, and scales;
+ * weights are made by it too.
+ *   weight       [channels] rows of int8 at multiples of 16 bytes, weight_row
+ *                bytes apart, readable up to a multiple of 16
+ *   weight_scales   fp32 [channels];  bias [channels] in dtype, or NULL
+ *   width        at most 2^17
+ *   y            (tokens, channels) contiguous, in dtype
+ *   scratch      >= bevpool_linear8_scratch_bytes(...), from a multiple of 16
+ */
+int64_t bevpool_linear8_pitch(int32_t width);
+
+int bevpool_linear8_codes(const void *x, int64_t x_row, int32_t dtype, int64_t rows, int32_t width,
+                          void *codes, void *scales, void *stream);
+
+size_t bevpool_linear8_scratch_bytes(int64_t tokens, int32_t width);
+
+int bevpool_linear8(const void *x, int64_t x_row, int32_t dtype, const void *weight,
+                    int64_t weight_row, const void *weight_scales, const void *bias, int64_t tokens,
+                    int32_t width, int64_t channels, void *y, void *scratch, size_t scratch_bytes,
+                    void *stream);
+
 /*
  * Optional per-kernel timing.  When enabled, every kernel launch is bracketed
  * by HIP events on the launch stream; bevpool_timing_read() synchronises
