@@ -30,7 +30,7 @@ using bevpool_host::LaunchScope;
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 typedef int i32x16 __attribute__((ext_vector_type(16)));
 
-constexpr int kStep = 128;           // bytes of a row that a tile holds
+constexpr int kPitch = 128;          // rows of codes are a multiple of it
 constexpr int kMaxWidth = 1 << 17;   // 2^17 128 127 < 2^31
 
 // ---------------------------------------------------------------------------
@@ -127,39 +127,76 @@ struct ProductArgs {
   int x_tiles, w_tiles;
 };
 
-// Rows of kStep bytes in LDS, 8 chunks of 16: chunk c of row r lies at c ^
-// (r / 2) % 8, so the 16 rows of which a fragment read takes one chunk each
-// use all of the 256 bytes that LDS gives a cycle.
-__device__ __forceinline__ int place(int r, int c) { return c ^ ((r >> 1) & 7); }
+// Four neighbouring channels' results: whole numbers to T, with both scales.
+template <typename T>
+struct __attribute__((packed, aligned(sizeof(T)))) Four {
+  T v[4];
+};
 
-// One block: kX tokens by kW channels, by waves of 32 kTx x 32 kTw.  Channels
+// Rows of kStep bytes in LDS, 4 chunks of 16: chunk c of row r lies at c ^
+// (r / 4) % 4, so the 16 rows of which a fragment read takes one chunk each
+// use all of the 256 bytes that LDS gives a cycle.
+constexpr int kStep = 64;  // bytes of a row that a tile holds
+__device__ __forceinline__ int place(int r, int c) { return c ^ ((r >> 2) & 3); }
+
+// Blocks of one XCD (every eighth) take tiles that lie together: eight tiles of
+// channels by as many of tokens as run at once share what their L2 holds.
+__device__ __forceinline__ bool tile_of(const ProductArgs &A, int &x_tile, int &w_tile) {
+  const int total = A.x_tiles * A.w_tiles, each = (total + 7) / 8;
+  const int i = int(blockIdx.x % 8) * each + int(blockIdx.x / 8);
+  if (int(blockIdx.x / 8) >= each || i >= total) return false;
+  const int group = i / (8 * A.x_tiles), first = group * 8;
+  const int wide = min(8, A.w_tiles - first), in = i - first * A.x_tiles;
+  x_tile = in / wide;
+  w_tile = first + in - x_tile * wide;
+  return true;
+}
+
+// Waits for all but the newest min(kMost, left) steps' loads, kLoads each.
+template <int kLoads, int kMost>
+__device__ __forceinline__ void wait_steps(int left) {
+  if (kMost == 0 || left >= kMost)
+    attention::wait_loads<kLoads * kMost>();
+  else
+    wait_steps<kLoads, (kMost > 0 ? kMost - 1 : 0)>(left);
+}
+
+// One block: kX tokens by kW channels, four waves of 32 kTx x 32 kTw.  Channels
 // are the rows of the matrix instruction's result, tokens its columns: a lane
 // holds one token's channels, four neighbours a register group.
-template <typename T, int kX, int kW, int kTx, int kTw>
-__global__ __launch_bounds__(64 * (kX / (32 * kTx)) * (kW / (32 * kTw))) void product_kernel(
-    ProductArgs A) {
-  constexpr int kThreads = 64 * (kX / (32 * kTx)) * (kW / (32 * kTw));
-  constexpr int kWavesX = kX / (32 * kTx);
-  constexpr int kLoadsX = kX * 8 / kThreads, kLoadsW = kW * 8 / kThreads;
+template <typename T, int kTx, int kTw, int kWavesX, int kBuffers>
+__global__ __launch_bounds__(256, 2) void product_kernel(ProductArgs A) {
+  constexpr int kThreads = 256, kWavesW = 4 / kWavesX;
+  constexpr int kX = 32 * kTx * kWavesX, kW = 32 * kTw * kWavesW;
+  constexpr int kLoadsX = kX * 4 / kThreads, kLoadsW = kW * 4 / kThreads;
   constexpr int kTileX = kX * kStep, kTile = (kX + kW) * kStep;
+  static_assert(kX % 64 == 0 && kW % 64 == 0, "whole rounds of loads");
   extern __shared__ __align__(16) char lds[];
+  float *scales = reinterpret_cast<float *>(lds + kBuffers * kTile), *biases = scales + kW;
+  int x_tile, w_tile;
+  if (!tile_of(A, x_tile, w_tile)) return;
   const int lane = attention::lane_id(), wave = attention::wave_id();
-  const int x0 = int(blockIdx.x % A.x_tiles) * kX, w0 = int(blockIdx.x / A.x_tiles) * kW;
+  const int x0 = x_tile * kX, w0 = w_tile * kW;
+  for (int i = threadIdx.x; i < kW; i += kThreads) {
+    const bool on = w0 + i < A.channels;
+    scales[i] = on ? A.w_scale[w0 + i] : 0.f;
+    biases[i] = on && A.bias ? float(static_cast<const T *>(A.bias)[w0 + i]) : 0.f;
+  }
   const unsigned lds0 = attention::lds_address(lds);
-  // this lane's pieces of the tiles: offsets from the step's first byte
+  // this lane's pieces of the tiles: offsets from a step's first byte
   const char *x_at = reinterpret_cast<const char *>(A.x) + int64_t(x0) * A.x_pitch;
   const char *w_at = reinterpret_cast<const char *>(A.w) + w0 * A.w_row;
   unsigned x_off[kLoadsX], w_off[kLoadsW];
   int w_chunk[kLoadsW];
 #pragma unroll
   for (int i = 0; i < kLoadsX; ++i) {
-    const int slot = i * kThreads + int(threadIdx.x), r = slot / 8, c = place(r, slot % 8);
+    const int slot = i * kThreads + int(threadIdx.x), r = slot / 4, c = place(r, slot % 4);
     x_off[i] = unsigned(min(r, A.tokens - 1 - x0) * A.x_pitch + c * 16);
   }
 #pragma unroll
   for (int i = 0; i < kLoadsW; ++i) {
-    const int slot = i * kThreads + int(threadIdx.x), r = slot / 8;
-    w_chunk[i] = place(r, slot % 8);
+    const int slot = i * kThreads + int(threadIdx.x), r = slot / 4;
+    w_chunk[i] = place(r, slot % 4);
     w_off[i] = unsigned(min(r, A.channels - 1 - w0) * int(A.w_row));
   }
   auto load = [&](int step, int buffer) {
@@ -171,22 +208,28 @@ __global__ __launch_bounds__(64 * (kX / (32 * kTx)) * (kW / (32 * kTw))) void pr
 #pragma unroll
     for (int i = 0; i < kLoadsW; ++i) {
       // (past a row's end: its last chunk once more, which meets zeros)
-      const int c = min(step * 8 + w_chunk[i], A.w_chunks - 1);
+      const int c = min(step * 4 + w_chunk[i], A.w_chunks - 1);
       attention::load_to_lds(w_at, w_off[i] + c * 16, to + kTileX + i * kThreads * 16);
     }
   };
   i32x16 acc[kTw][kTx] = {};
   const int wx = wave % kWavesX * 32 * kTx, ww = wave / kWavesX * 32 * kTw;
   const int c = lane & 31, h = lane >> 5;
-  load(0, 0);
-  int buffer = 0;
-  for (int step = 0; step < A.steps; ++step, buffer ^= 1) {
-    attention::wait_loads<0>();
-    __syncthreads();  // this step's tiles are there, and the last one's have been read
-    if (step + 1 < A.steps) load(step + 1, buffer ^ 1);
-    const char *x_tile = lds + buffer * kTile, *w_tile = x_tile + kTileX;
+  // (the compiler's own loads, of scales, are done: what is counted is the tiles')
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
 #pragma unroll
-    for (int s = 0; s < 4; ++s) {
+  for (int i = 0; i < kBuffers - 1; ++i)
+    if (i < A.steps) load(i, i);
+  int buffer = 0;
+  for (int step = 0; step < A.steps; ++step) {
+    wait_steps<kLoadsX + kLoadsW, kBuffers - 2>(A.steps - 1 - step);
+    attention::tile_barrier();  // this step's tiles are there, and the last one's have been read
+    if (step + kBuffers - 1 < A.steps)
+      load(step + kBuffers - 1, buffer == 0 ? kBuffers - 1 : buffer - 1);
+    const char *x_tile = lds + buffer * kTile, *w_tile = x_tile + kTileX;
+    buffer = buffer == kBuffers - 1 ? 0 : buffer + 1;
+#pragma unroll
+    for (int s = 0; s < kStep / 32; ++s) {
       i32x4 x[kTx], w[kTw];
 #pragma unroll
       for (int i = 0; i < kTx; ++i)
@@ -203,21 +246,129 @@ __global__ __launch_bounds__(64 * (kX / (32 * kTx)) * (kW / (32 * kTw))) void pr
           acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(w[i], x[j], acc[i][j], 0, 0, 0);
     }
   }
-  const T *bias = static_cast<const T *>(A.bias);
 #pragma unroll
   for (int j = 0; j < kTx; ++j) {
     const int token = x0 + wx + 32 * j + c;
-    if (token >= A.tokens) continue;
-    const float by = A.x_scale[token];
+    const bool valid = token < A.tokens;
+    const float by = valid ? A.x_scale[token] : 0.f;
     T *y = static_cast<T *>(A.y) + int64_t(token) * A.channels;
 #pragma unroll
     for (int i = 0; i < kTw; ++i)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const int n = w0 + ww + 32 * i + attention::c_row(r, h);
-        if (n < A.channels)
-          y[n] = T(float(acc[i][j][r]) * by * A.w_scale[n] + (bias ? float(bias[n]) : 0.f));
+      for (int p = 0; p < 2; ++p) {
+        // channels 16 p + 4 h .. + 3 and those 8 further
+        const int n = ww + 32 * i + 16 * p + 4 * h;
+        float v[8];
+#pragma unroll
+        for (int g = 0; g < 2; ++g) {
+          const attention::f32x4 scale = *reinterpret_cast<attention::f32x4 *>(scales + n + 8 * g);
+          const attention::f32x4 bias = *reinterpret_cast<attention::f32x4 *>(biases + n + 8 * g);
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            v[4 * g + r] = float(acc[i][j][8 * p + 4 * g + r]) * by * scale[r] + bias[r];
+        }
+        if constexpr (sizeof(T) == 4) {
+#pragma unroll
+          for (int g = 0; g < 2; ++g) {
+            const int at = w0 + n + 8 * g;
+            if (valid && at + 4 <= A.channels) {
+              *reinterpret_cast<Four<T> *>(y + at) = {v[4 * g], v[4 * g + 1], v[4 * g + 2],
+                                                      v[4 * g + 3]};
+            } else if (valid) {
+#pragma unroll
+              for (int r = 0; r < 4; ++r)
+                if (at + r < A.channels) y[at + r] = v[4 * g + r];
+            }
+          }
+        } else {
+          // the halves trade four channels so that each has eight neighbours
+          typedef T Pair __attribute__((ext_vector_type(2)));
+          unsigned q[4];
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const Pair pair{T(v[2 * r]), T(v[2 * r + 1])};
+            q[r] = __builtin_bit_cast(unsigned, pair);
+          }
+          const auto a = __builtin_amdgcn_permlane32_swap(q[0], q[2], false, false);
+          const auto b = __builtin_amdgcn_permlane32_swap(q[1], q[3], false, false);
+          const attention::u32x4 out{a[0], b[0], a[1], b[1]};
+          rows::Pack<T> eight;
+          __builtin_memcpy(&eight, &out, 16);
+          const int at = w0 + ww + 32 * i + 16 * p + 8 * h;
+          if (valid && at + 8 <= A.channels) {
+            *reinterpret_cast<rows::Pack<T> *>(y + at) = eight;
+          } else if (valid) {
+#pragma unroll
+            for (int r = 0; r < 8; ++r)
+              if (at + r < A.channels) y[at + r] = eight.v[r];
+          }
+        }
       }
+  }
+}
+
+// Few tokens: 16 kTx tokens by 16 kTw channels a block, whose eight waves take
+// every eighth 64 bytes of the rows straight to registers, so that the weights
+// are on their way all at once, and add their sums in LDS.
+constexpr int kFewWaves = 8;
+template <typename T, int kTx, int kTw>
+__global__ __launch_bounds__(64 * kFewWaves) void few_kernel(ProductArgs A) {
+  __shared__ i32x4 sums[kFewWaves][kTw * kTx][64];
+  const int lane = attention::lane_id(), wave = attention::wave_id();
+  const int c = lane & 15, q = lane >> 4;
+  const int w0 = int(blockIdx.x) * 16 * kTw, x0 = int(blockIdx.y) * 16 * kTx;
+  const int8_t *w_at[kTw], *x_at[kTx];
+#pragma unroll
+  for (int i = 0; i < kTw; ++i)
+    w_at[i] = A.w + int64_t(min(w0 + 16 * i + c, A.channels - 1)) * A.w_row;
+#pragma unroll
+  for (int i = 0; i < kTx; ++i)
+    x_at[i] = A.x + int64_t(min(x0 + 16 * i + c, A.tokens - 1)) * A.x_pitch;
+  i32x4 acc[kTw][kTx] = {};
+#pragma unroll 8
+  for (int step = wave; step < A.steps; step += kFewWaves) {
+    i32x4 w[kTw], x[kTx];
+    const int chunk = step * 4 + q;
+#pragma unroll
+    for (int i = 0; i < kTw; ++i)  // (past a row's end: as above)
+      w[i] = *reinterpret_cast<const i32x4 *>(w_at[i] + min(chunk, A.w_chunks - 1) * 16);
+#pragma unroll
+    for (int i = 0; i < kTx; ++i)
+      x[i] = *reinterpret_cast<const i32x4 *>(x_at[i] + chunk * 16);
+#pragma unroll
+    for (int i = 0; i < kTw; ++i)
+#pragma unroll
+      for (int j = 0; j < kTx; ++j)
+        acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(w[i], x[j], acc[i][j], 0, 0, 0);
+  }
+#pragma unroll
+  for (int i = 0; i < kTw; ++i)
+#pragma unroll
+    for (int j = 0; j < kTx; ++j) sums[wave][i * kTx + j][lane] = acc[i][j];
+  __syncthreads();
+  const T *bias = static_cast<const T *>(A.bias);
+  for (int t = wave; t < kTw * kTx; t += kFewWaves) {
+    i32x4 sum = sums[0][t][lane];
+#pragma unroll
+    for (int i = 1; i < kFewWaves; ++i) sum += sums[i][t][lane];
+    // lane 16 q + c: channels 4 q .. + 3 of token c
+    const int token = x0 + t % kTx * 16 + c, n = w0 + t / kTx * 16 + 4 * q;
+    if (token >= A.tokens) continue;
+    const float by = A.x_scale[token];
+    T *y = static_cast<T *>(A.y) + int64_t(token) * A.channels + n;
+    Four<T> four;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int at = min(n + r, A.channels - 1);
+      four.v[r] = T(float(sum[r]) * by * A.w_scale[at] + (bias ? float(bias[at]) : 0.f));
+    }
+    if (n + 4 <= A.channels) {
+      *reinterpret_cast<Four<T> *>(y) = four;
+    } else {
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        if (n + r < A.channels) y[r] = four.v[r];
+    }
   }
 }
 
@@ -225,7 +376,7 @@ __global__ __launch_bounds__(64 * (kX / (32 * kTx)) * (kW / (32 * kTw))) void pr
 // host side
 // ---------------------------------------------------------------------------
 
-int64_t code_pitch(int64_t width) { return (width + kStep - 1) / kStep * kStep; }
+int64_t code_pitch(int64_t width) { return (width + kPitch - 1) / kPitch * kPitch; }
 
 template <typename T>
 void launch_codes(const void *x, int64_t x_row, int64_t n, int width, int pitch, int8_t *codes,
@@ -261,17 +412,53 @@ int codes_for(const void *x, int64_t x_row, int dtype, int64_t n, int width, int
   return check_launch("linear8_codes");
 }
 
-template <typename T>
-int launch_product(ProductArgs &A, hipStream_t s) {
-  constexpr int kX = 128, kW = 128;
+template <typename T, int kTx, int kTw, int kWavesX, int kBuffers>
+int launch_tiles(ProductArgs &A, hipStream_t s) {
+  constexpr int kX = 32 * kTx * kWavesX, kW = 32 * kTw * (4 / kWavesX);
   A.x_tiles = (A.tokens + kX - 1) / kX;
   A.w_tiles = (A.channels + kW - 1) / kW;
-  const int64_t blocks = int64_t(A.x_tiles) * A.w_tiles;
+  const int64_t blocks = (int64_t(A.x_tiles) * A.w_tiles + 7) / 8 * 8;
   const int st = check_grid(blocks, 256, "linear8");
   if (st) return st;
-  hipLaunchKernelGGL((product_kernel<T, kX, kW, 2, 2>), dim3(unsigned(blocks)), dim3(256),
-                     2 * (kX + kW) * kStep, s, A);
+  hipLaunchKernelGGL((product_kernel<T, kTx, kTw, kWavesX, kBuffers>), dim3(unsigned(blocks)), dim3(256),
+                     kBuffers * (kX + kW) * kStep + 2 * kW * sizeof(float), s, A);
   return check_launch("linear8");
+}
+
+template <typename T, int kTx, int kTw>
+int launch_few(const ProductArgs &A, hipStream_t s) {
+  const dim3 grid((A.channels + 16 * kTw - 1) / (16 * kTw), (A.tokens + 16 * kTx - 1) / (16 * kTx));
+  hipLaunchKernelGGL((few_kernel<T, kTx, kTw>), grid, dim3(64 * kFewWaves), 0, s, A);
+  return check_launch("linear8");
+}
+
+template <typename T, int kTw>
+int launch_few_tokens(const ProductArgs &A, hipStream_t s) {
+  if (A.tokens <= 16) return launch_few<T, 1, kTw>(A, s);
+  if (A.tokens <= 32) return launch_few<T, 2, kTw>(A, s);
+  return launch_few<T, 4, kTw>(A, s);
+}
+
+template <typename T>
+int launch_product(ProductArgs &A, hipStream_t s) {
+  // Up to 64 tokens the weights' way to the registers is the time.  32 channels
+  // a block read the tokens half as often as 16, but need enough channels for
+  // the card's CUs: us by 16 and by 32, 16 x 4096 x 6144 12.4 and 10.9, 32 x
+  // 8192 x 8192 32.1 and 24.7; 48 x 4096 x 4096 13.4 and 14.5, 64 x 1280 x 1280
+  // 7.5 and 8.7.
+  if (A.tokens <= 64)
+    return A.channels >= 32 * 160 ? launch_few_tokens<T, 2>(A, s) : launch_few_tokens<T, 1>(A, s);
+  // Tiles of 128 x 256 from one for each CU on (us of these and of 64 x 128:
+  // 1024 x 4096 x 8192 50 and 67, 1500 x 1280 x 10240 33 and 44; 800 x 4096 x
+  // 4096 42 and 31), else of 64 x 128, or 64 x 64 where that is not two for
+  // each (64 x 128 and 64 x 64: 800 x 4096 x 4096 31 and 38, 512 x 4096 x 4096
+  // 24 and 23, 100 x 4096 x 6144 22 and 19).
+  auto tiles = [&](int x, int w) {
+    return int64_t((A.tokens + x - 1) / x) * ((A.channels + w - 1) / w);
+  };
+  if (tiles(128, 256) >= 256) return launch_tiles<T, 2, 4, 2, 3>(A, s);
+  if (tiles(64, 64) > 512) return launch_tiles<T, 1, 2, 2, 6>(A, s);
+  return launch_tiles<T, 1, 1, 2, 8>(A, s);
 }
 
 int check_sizes(int dtype, int64_t tokens, int64_t width, int64_t channels) {

@@ -27,59 +27,146 @@ struct Args {
   int64_t items, parts_each;            // parts_each: items of one row of gate
 };
 
-// Lanes that share a row and chunks that each holds: the fewest lanes for
-// short rows, so that a wave takes several, and no more than three chunks,
-// which leave room for the gradients' values of a row in registers.
+// Lanes that share a row and chunks that each holds: one, so that few registers
+// hold a row's values and several rows' loads are on their way at once (chunks
+// past 4096 values: two), by whole waves, or parts of one for short rows.
 #define RESIDUAL_LAYOUT(FN, width, ...)                                         \
   if ((width) <= 128) FN(16, 1, __VA_ARGS__)                                    \
   else if ((width) <= 256) FN(32, 1, __VA_ARGS__)                               \
   else if ((width) <= 512) FN(64, 1, __VA_ARGS__)                               \
-  else if ((width) <= 1024) FN(64, 2, __VA_ARGS__)                              \
-  else if ((width) <= 1536) FN(64, 3, __VA_ARGS__)                              \
+  else if ((width) <= 1024) FN(128, 1, __VA_ARGS__)                             \
+  else if ((width) <= 1536) FN(192, 1, __VA_ARGS__)                             \
   else if ((width) <= 2048) FN(256, 1, __VA_ARGS__)                             \
-  else if ((width) <= 4096) FN(256, 2, __VA_ARGS__)                             \
+  else if ((width) <= 4096) FN(512, 1, __VA_ARGS__)                             \
   else FN(512, 2, __VA_ARGS__)
 
-constexpr int threads_of(int lanes) { return lanes > 256 ? lanes : 256; }
-inline int lanes_for(int width) {
-  return width <= 128 ? 16 : width <= 256 ? 32 : width <= 1536 ? 64 : width <= 4096 ? 256 : 512;
-}
+// (rows of more than a wave pass barriers: a block of them has one)
+constexpr int threads_of(int lanes) { return lanes > 64 ? lanes : 256; }
 inline int rows_at_once(int width) {
-  const int lanes = lanes_for(width);
-  return threads_of(lanes) / lanes;
+  return width <= 128 ? 16 : width <= 256 ? 8 : width <= 512 ? 4 : 1;
 }
 
-// A lane's place: its row of a block's, and what of it is its own.
-template <int kLanes, int kChunks>
+// A lane's place: its row of a block's, and its chunks.  With kWhole, where the
+// width is no whole number of chunks the last one begins earlier, and shares
+// its first `skip` values with the one before: both form the same of them, and
+// only sums leave them out, so that every access is a whole one (of rows of a
+// chunk at least).  Without, its values past the row's end are zeros.
+template <int kLanes, int kChunks, bool kWhole = true>
 struct Place {
-  int lane, group;
-  __device__ __forceinline__ Place() {
+  int lane, group, width;
+  __device__ __forceinline__ explicit Place(int width) : width(width) {
     lane = int(threadIdx.x) % kLanes;
     group = int(threadIdx.x) / kLanes;
+    if constexpr (kLanes >= 64) group = __builtin_amdgcn_readfirstlane(group);
   }
   __device__ __forceinline__ int chunk(int j) const { return lane + j * kLanes; }
-  __device__ __forceinline__ int left(int j, int width) const {
-    return width - chunk(j) * rows::kChunk;
+  __device__ __forceinline__ bool on(int j) const { return chunk(j) * rows::kChunk < width; }
+  __device__ __forceinline__ int begin(int j) const {
+    const int at = chunk(j) * rows::kChunk;
+    return kWhole ? max(0, min(at, width - rows::kChunk)) : at;
+  }
+  __device__ __forceinline__ int skip(int j) const {
+    return kWhole && on(j) && width >= rows::kChunk ? chunk(j) * rows::kChunk - begin(j) : 0;
+  }
+  __device__ __forceinline__ int left(int j) const { return width - begin(j); }
+};
+
+// A row's values of a lane as they lie in memory, in whole registers.
+template <typename T, int kChunks>
+struct Raw {
+  static constexpr int kWords = rows::kChunk * int(sizeof(T)) / 4;
+  struct __attribute__((packed, aligned(sizeof(T)))) Words {
+    unsigned w[kWords];
+  };
+  Words c[kChunks];
+  template <int kLanes, bool kWhole>
+  __device__ __forceinline__ void load(const void *base, int64_t offset,
+                                       const Place<kLanes, kChunks, kWhole> &at) {
+    const T *row = static_cast<const T *>(base) + offset;
+#pragma unroll
+    for (int j = 0; j < kChunks; ++j) {
+      c[j] = {};
+      if (!at.on(j)) continue;
+      if (at.left(j) >= rows::kChunk) {
+        c[j] = *reinterpret_cast<const Words *>(row + at.begin(j));
+      } else {
+#pragma unroll
+        for (int i = 0; i < rows::kChunk; ++i) {
+          if (i >= at.left(j)) continue;
+          const T v = row[at.begin(j) + i];
+          if constexpr (sizeof(T) == 4)
+            c[j].w[i] = __builtin_bit_cast(unsigned, v);
+          else
+            c[j].w[i / 2] |= unsigned(__builtin_bit_cast(uint16_t, v)) << (i % 2 * 16);
+        }
+      }
+    }
+  }
+  __device__ __forceinline__ float get(int j, int i) const {
+    if constexpr (sizeof(T) == 4) {
+      return __builtin_bit_cast(float, c[j].w[i]);
+    } else {
+      const unsigned w = c[j].w[i / 2];
+      if constexpr (__is_same(T, __bf16))  // (the upper half of the same number in fp32)
+        return __builtin_bit_cast(float, i % 2 ? w & 0xffff0000u : w << 16);
+      else
+        return float(__builtin_bit_cast(T, uint16_t(i % 2 ? w >> 16 : w)));
+    }
   }
 };
 
-template <typename T, int kLanes, int kChunks>
-__device__ __forceinline__ void load_row(float (&v)[kChunks][rows::kChunk], const void *base,
-                                         int64_t offset, int width,
-                                         const Place<kLanes, kChunks> &at) {
-  const T *row = static_cast<const T *>(base) + offset;
+// The same of a row's 8-bit checkpoint.
+template <int kChunks>
+struct Packed {
+  rows::Bytes c[kChunks];
+  unsigned scale[kChunks];
+  template <int kLanes>
+  __device__ __forceinline__ void load(const uint8_t *row,
+                                       const Place<kLanes, kChunks, false> &at) {
+    const uint8_t *scales = row + rows::blocks_of(at.width) * rows::kBlock;
 #pragma unroll
-  for (int j = 0; j < kChunks; ++j)
-    rows::load(v[j], row + at.chunk(j) * rows::kChunk, at.left(j, width));
-}
-template <typename T, int kLanes, int kChunks>
-__device__ __forceinline__ void store_row(void *base, int64_t offset, int width,
+    for (int j = 0; j < kChunks; ++j) {
+      c[j] = {0x80808080u, 0x80808080u};  // zeros
+      scale[j] = 1;
+      if (!at.on(j)) continue;
+      c[j] = *reinterpret_cast<const rows::Bytes *>(row + at.begin(j));
+      scale[j] = scales[at.begin(j) / rows::kBlock];
+    }
+  }
+  __device__ __forceinline__ void get(float (&v)[kChunks][rows::kChunk]) const {
+#pragma unroll
+    for (int j = 0; j < kChunks; ++j) rows::unpack(v[j], c[j], scale[j]);
+  }
+};
+
+template <typename T, int kLanes, int kChunks, bool kWhole>
+__device__ __forceinline__ void store_row(void *base, int64_t offset,
                                           const float (&v)[kChunks][rows::kChunk],
-                                          const Place<kLanes, kChunks> &at) {
+                                          const Place<kLanes, kChunks, kWhole> &at) {
   T *row = static_cast<T *>(base) + offset;
 #pragma unroll
-  for (int j = 0; j < kChunks; ++j)
-    rows::store(row + at.chunk(j) * rows::kChunk, v[j], at.left(j, width));
+  for (int j = 0; j < kChunks; ++j) {
+    if (!at.on(j)) continue;
+    rows::store(row + at.begin(j), v[j], at.left(j));
+  }
+}
+
+// Sum of f(j, i) over a lane's values, none twice.
+template <int kLanes, int kChunks, bool kWhole, typename F>
+__device__ __forceinline__ float own_sum(const Place<kLanes, kChunks, kWhole> &at, F f) {
+  float s = 0.f;
+#pragma unroll
+  for (int j = 0; j < kChunks; ++j) {
+    const int skip = at.skip(j);
+    if (skip == 0) {
+#pragma unroll
+      for (int i = 0; i < rows::kChunk; ++i) s += f(j, i);
+    } else {
+#pragma unroll
+      for (int i = 0; i < rows::kChunk; ++i) s += i >= skip ? f(j, i) : 0.f;
+    }
+  }
+  return s;
 }
 
 // Sums over a row's lanes, kN at once, in all of them.  Rows of more than a

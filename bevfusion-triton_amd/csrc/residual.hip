@@ -24,83 +24,107 @@ using bevpool_host::check_launch;
 using bevpool_host::fail;
 using bevpool_host::LaunchScope;
 
+// What a row's lanes read of it.
+template <typename T, typename X, int kChunks>
+struct Inputs {
+  Raw<X, kChunks> x;
+  Raw<T, kChunks> update, gate;
+  template <int kLanes>
+  __device__ __forceinline__ void load(const Args &A, int64_t row,
+                                       const Place<kLanes, kChunks> &at) {
+    x.load(A.x, row * A.x_row, at);
+    if (A.update) update.load(A.update, row * A.update_row, at);
+    if (A.gate) {
+      const int64_t owner = A.gate_each == 1        ? row
+                            : A.rows < (1LL << 32) ? unsigned(row) / unsigned(A.gate_each)
+                                                   : row / A.gate_each;
+      gate.load(A.gate, owner * A.gate_row, at);
+    }
+  }
+};
+
+// 8-bit checkpoint of a row: of whole chunks of a lane as they are in
+// registers, of the last one from memory, for it begins earlier here.
+template <typename T, int kLanes, int kChunks>
+__device__ __forceinline__ void keep(uint8_t *kept, const Raw<T, kChunks> &raw, const void *base,
+                                     int64_t offset, const Place<kLanes, kChunks> &at) {
+#pragma unroll
+  for (int j = 0; j < kChunks; ++j) {
+    float v[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = raw.get(j, i);
+    if (at.skip(j) > 0) {
+      const int first = at.chunk(j) * 8;
+      rows::load(v, static_cast<const T *>(base) + offset + first, at.width - first);
+    }
+    rows::store_packed(kept, at.chunk(j), rows::blocks_of(at.width), v);
+  }
+}
+
+// A group of lanes takes rows, the next one's loads on their way while one is
+// worked on; weights stay in registers.
 template <typename T, typename X, int kLanes, int kChunks>
 __global__ __launch_bounds__(threads_of(kLanes)) void residual_kernel(Args A) {
   constexpr int kGroups = threads_of(kLanes) / kLanes;
   __shared__ float shared[4][threads_of(kLanes) / 64];
-  const Place<kLanes, kChunks> at;
-  const int width = A.width;
-  const int64_t blocks = rows::blocks_of(width);
-  int turn = 0;
-  for (int64_t row = int64_t(blockIdx.x) * kGroups + at.group; row < A.rows;
-       row += int64_t(gridDim.x) * kGroups, turn ^= 2) {
-    float x[kChunks][8], u[kChunks][8], w[kChunks][8];
-    load_row<X>(x, A.x, row * A.x_row, width, at);
-    if (A.update) {
-      load_row<T>(u, A.update, row * A.update_row, width, at);
-      if (A.update_kept) {
-        uint8_t *kept = A.update_kept + row * rows::checkpoint_pitch(width);
+  const Place<kLanes, kChunks> at(A.width);
+  const int64_t width = A.width, pitch = rows::checkpoint_pitch(width);
+  // scale times the update's weight, and the norm's weight
+  float c[kChunks][8];
+  Raw<T, kChunks> w, weight;
+  if (A.update_weight) w.load(A.update_weight, 0, at);
+  if (A.scale) weight.load(A.scale, 0, at);
 #pragma unroll
-        for (int j = 0; j < kChunks; ++j) rows::store_packed(kept, at.chunk(j), blocks, u[j]);
-      }
-    }
-    if (A.x_kept) {
-      uint8_t *kept = A.x_kept + row * rows::checkpoint_pitch(width);
+  for (int j = 0; j < kChunks; ++j)
 #pragma unroll
-      for (int j = 0; j < kChunks; ++j) rows::store_packed(kept, at.chunk(j), blocks, x[j]);
-    }
+    for (int i = 0; i < 8; ++i)
+      c[j][i] = (A.update_weight ? w.get(j, i) : 1.f) * (A.scale ? weight.get(j, i) : 1.f);
+  if (A.weight) weight.load(A.weight, 0, at);
+  const int64_t step = int64_t(gridDim.x) * kGroups;
+  int64_t row = int64_t(blockIdx.x) * kGroups + at.group;
+  Inputs<T, X, kChunks> next;
+  if (row < A.rows) next.load(A, row, at);
+  for (int turn = 0; row < A.rows; row += step, turn ^= 2) {
+    const Inputs<T, X, kChunks> in = next;
+    if (row + step < A.rows) next.load(A, row + step, at);
+    if (A.x_kept) keep<X>(A.x_kept + row * pitch, in.x, A.x, row * A.x_row, at);
+    float x[kChunks][8];
     if (A.update) {
+      if (A.update_kept)
+        keep<T>(A.update_kept + row * pitch, in.update, A.update, row * A.update_row, at);
+      float r = 1.f;
       if (A.update_weight) {
-        float s[1] = {0.f};
-#pragma unroll
-        for (int j = 0; j < kChunks; ++j)
-#pragma unroll
-          for (int i = 0; i < 8; ++i) s[0] += u[j][i] * u[j][i];
+        float s[1] = {own_sum(at, [&](int j, int i) {
+          const float u = in.update.get(j, i);
+          return u * u;
+        })};
         row_sums<kLanes>(s, shared[turn]);
-        const float r = 1.0f / sqrtf(s[0] * A.inv_width + A.eps);
-        load_row<T>(w, A.update_weight, 0, width, at);
-#pragma unroll
-        for (int j = 0; j < kChunks; ++j)
-#pragma unroll
-          for (int i = 0; i < 8; ++i) u[j][i] *= r * w[j][i];
-      }
-      if (A.scale) {
-        load_row<T>(w, A.scale, 0, width, at);
-#pragma unroll
-        for (int j = 0; j < kChunks; ++j)
-#pragma unroll
-          for (int i = 0; i < 8; ++i) u[j][i] *= w[j][i];
-      }
-      if (A.gate) {
-        const int64_t owner = A.gate_each == 1        ? row
-                              : A.rows < (1LL << 32) ? unsigned(row) / unsigned(A.gate_each)
-                                                     : row / A.gate_each;
-        load_row<T>(w, A.gate, owner * A.gate_row, width, at);
-#pragma unroll
-        for (int j = 0; j < kChunks; ++j)
-#pragma unroll
-          for (int i = 0; i < 8; ++i) u[j][i] *= w[j][i];
+        r = 1.0f / sqrtf(s[0] * A.inv_width + A.eps);
       }
 #pragma unroll
       for (int j = 0; j < kChunks; ++j)
 #pragma unroll
-        for (int i = 0; i < 8; ++i) x[j][i] += u[j][i];
-      store_row<X>(A.sum, row * width, width, x, at);
+        for (int i = 0; i < 8; ++i) {
+          float v = in.update.get(j, i) * r * c[j][i];
+          if (A.gate) v *= in.gate.get(j, i);
+          x[j][i] = in.x.get(j, i) + v;
+        }
+      store_row<X>(A.sum, row * width, x, at);
+    } else {
+#pragma unroll
+      for (int j = 0; j < kChunks; ++j)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[j][i] = in.x.get(j, i);
     }
     if (A.weight) {
-      float s[1] = {0.f};
-#pragma unroll
-      for (int j = 0; j < kChunks; ++j)
-#pragma unroll
-        for (int i = 0; i < 8; ++i) s[0] += x[j][i] * x[j][i];
+      float s[1] = {own_sum(at, [&](int j, int i) { return x[j][i] * x[j][i]; })};
       row_sums<kLanes>(s, shared[turn + 1]);
       const float r = 1.0f / sqrtf(s[0] * A.inv_width + A.eps);
-      load_row<T>(w, A.weight, 0, width, at);
 #pragma unroll
       for (int j = 0; j < kChunks; ++j)
 #pragma unroll
-        for (int i = 0; i < 8; ++i) x[j][i] *= r * w[j][i];
-      store_row<T>(A.normed, row * width, width, x, at);
+        for (int i = 0; i < 8; ++i) x[j][i] *= r * weight.get(j, i);
+      store_row<T>(A.normed, row * width, x, at);
     }
   }
 }

@@ -18,6 +18,8 @@
 
 #include <stdint.h>
 
+#include <type_traits>
+
 #include "bevpool.h"
 #include "host_calls.h"
 #include "residual.h"
@@ -31,15 +33,16 @@ using bevpool_host::LaunchScope;
 int check(Args &A, int dtype, int x_dtype, int64_t rows, int width, int64_t gate_rows, float eps);
 
 // The groups' sums of a block, added in the groups' order, to `to`.
-template <int kLanes, int kChunks>
-__device__ __forceinline__ void flush(float (&v)[kChunks][8], float *to, int width,
-                                      const Place<kLanes, kChunks> &at, float *lds) {
+template <int kLanes, int kChunks, bool kWhole>
+__device__ __forceinline__ void flush(float (&v)[kChunks][8], float *to,
+                                      const Place<kLanes, kChunks, kWhole> &at, float *lds) {
   constexpr int kGroups = threads_of(kLanes) / kLanes;
+  const int width = at.width;
   if constexpr (kGroups == 1) {
-    store_row<float>(to, 0, width, v, at);
+    store_row<float>(to, 0, v, at);
   } else {
     __syncthreads();  // what was there has been read
-    store_row<float>(lds, at.group * width, width, v, at);
+    store_row<float>(lds, at.group * width, v, at);
     __syncthreads();
     for (int c = threadIdx.x; c < width; c += threads_of(kLanes)) {
       float s = 0.f;
@@ -50,20 +53,85 @@ __device__ __forceinline__ void flush(float (&v)[kChunks][8], float *to, int wid
   }
 }
 
+// What a row's lanes read of it; x and update as they were or as checkpoints.
+template <typename T, typename X, int kChunks>
+struct Operands {
+  Raw<X, kChunks> x;
+  Raw<T, kChunks> update;
+  template <int kLanes>
+  __device__ __forceinline__ void load(const Args &A, int64_t row,
+                                       const Place<kLanes, kChunks> &at) {
+    if (A.weight) x.load(A.x, row * A.x_row, at);
+    if (A.update) update.load(A.update, row * A.update_row, at);
+  }
+  __device__ __forceinline__ void get(float (&u)[kChunks][8], float (&v)[kChunks][8]) const {
+#pragma unroll
+    for (int j = 0; j < kChunks; ++j)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        u[j][i] = update.get(j, i);
+        v[j][i] = x.get(j, i);
+      }
+  }
+};
+template <int kChunks>
+struct KeptOperands {
+  Packed<kChunks> x, update;
+  template <int kLanes>
+  __device__ __forceinline__ void load(const Args &A, int64_t row,
+                                       const Place<kLanes, kChunks, false> &at) {
+    const int64_t offset = row * rows::checkpoint_pitch(at.width);
+    if (A.weight) x.load(A.x_kept + offset, at);
+    if (A.update) update.load(A.update_kept + offset, at);
+  }
+  __device__ __forceinline__ void get(float (&u)[kChunks][8], float (&v)[kChunks][8]) const {
+    update.get(u);
+    x.get(v);
+  }
+};
+template <typename Of, typename T, typename X, int kChunks>
+struct Inputs {
+  Of of;
+  Raw<X, kChunks> dsum;
+  Raw<T, kChunks> dnormed, gate;
+  template <int kLanes, bool kWhole>
+  __device__ __forceinline__ void load(const Args &A, int64_t row, bool own_gate,
+                                       const Place<kLanes, kChunks, kWhole> &at) {
+    of.load(A, row, at);
+    if (A.dsum) dsum.load(A.dsum, row * A.dsum_row, at);
+    if (A.weight) dnormed.load(A.dnormed, row * A.dnormed_row, at);
+    if (own_gate) gate.load(A.gate, row * A.gate_row, at);
+  }
+};
+
 // A block walks items, each an equal part of the rows that share a row of
-// gate (without such a gate: of all), and leaves each item's sums.
+// gate (without such a gate: of all), and leaves each item's sums.  Its groups
+// of lanes take rows, the next one's loads on their way while one is worked on.
 template <typename T, typename X, int kLanes, int kChunks, bool kKept>
-__global__ __launch_bounds__(threads_of(kLanes), 1) void residual_backward_kernel(Args A) {
+__global__ __launch_bounds__(threads_of(kLanes), 2) void residual_backward_kernel(Args A) {
   constexpr int kGroups = threads_of(kLanes) / kLanes;
+  typedef std::conditional_t<kKept, KeptOperands<kChunks>, Operands<T, X, kChunks>> Of;
   extern __shared__ float lds[];
   __shared__ float shared[6][2 * (threads_of(kLanes) / 64)];
-  const Place<kLanes, kChunks> at;
-  const int width = A.width;
-  const int64_t blocks = rows::blocks_of(width), pitch = rows::checkpoint_pitch(width);
+  const Place<kLanes, kChunks, !kKept> at(A.width);
+  const int64_t width = A.width;
   const bool own_gate = A.gate && A.gate_each == 1;
   const int64_t part_rows = (A.gate && !own_gate ? A.gate_each : A.rows);
   const int64_t share = (part_rows + A.parts_each - 1) / A.parts_each;
-  float dweight[kChunks][8] = {};
+  // scale times the update's weight, and the norm's weight
+  float c[kChunks][8], dweight[kChunks][8] = {};
+  Raw<T, kChunks> weight;
+  {
+    Raw<T, kChunks> w;
+    if (A.update_weight) w.load(A.update_weight, 0, at);
+    if (A.scale) weight.load(A.scale, 0, at);
+#pragma unroll
+    for (int j = 0; j < kChunks; ++j)
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        c[j][i] = (A.update_weight ? w.get(j, i) : 1.f) * (A.scale ? weight.get(j, i) : 1.f);
+  }
+  if (A.weight) weight.load(A.weight, 0, at);
   int turn = 0;
   for (int64_t item = blockIdx.x; item < A.items; item += gridDim.x) {
     const int64_t owner = item / A.parts_each, part = item % A.parts_each;
@@ -71,92 +139,43 @@ __global__ __launch_bounds__(threads_of(kLanes), 1) void residual_backward_kerne
     const int64_t begin = first + part * share;
     const int64_t end = min(begin + share, first + part_rows);
     float q[kChunks][8] = {};
+    Inputs<Of, T, X, kChunks> next;
+    if (A.gate && !own_gate) next.gate.load(A.gate, owner * A.gate_row, at);
+    if (begin + at.group < end) next.load(A, begin + at.group, own_gate, at);
     for (int64_t row = begin + at.group; row < end; row += kGroups, turn = 3 - turn) {
-      const int64_t gate_row = own_gate ? row : owner;
-      float g[kChunks][8], n[kChunks][8], c[kChunks][8], w[kChunks][8];
-      if (A.dsum) {
-        load_row<X>(g, A.dsum, row * A.dsum_row, width, at);
-      } else {
-#pragma unroll
-        for (int j = 0; j < kChunks; ++j)
-#pragma unroll
-          for (int i = 0; i < 8; ++i) g[j][i] = 0.f;
-      }
+      const Inputs<Of, T, X, kChunks> in = next;
+      if (row + kGroups < end) next.load(A, row + kGroups, own_gate, at);
+      float n[kChunks][8], x[kChunks][8];
+      in.of.get(n, x);
       float r_u = 1.f;
-      if (A.update) {
-        if constexpr (kKept) {
-#pragma unroll
-          for (int j = 0; j < kChunks; ++j) {
-            if (at.left(j, width) > 0)
-              rows::load_packed(n[j], A.update_kept + row * pitch, at.chunk(j), blocks);
-            else
-#pragma unroll
-              for (int i = 0; i < 8; ++i) n[j][i] = 0.f;
-          }
-        } else {
-          load_row<T>(n, A.update, row * A.update_row, width, at);
-        }
+      if (A.update_weight) {
+        float s[1] = {own_sum(at, [&](int j, int i) { return n[j][i] * n[j][i]; })};
+        row_sums<kLanes>(s, shared[turn]);
+        r_u = 1.0f / sqrtf(s[0] * A.inv_width + A.eps);
 #pragma unroll
         for (int j = 0; j < kChunks; ++j)
 #pragma unroll
-          for (int i = 0; i < 8; ++i) c[j][i] = 1.f;
-        if (A.scale) load_row<T>(c, A.scale, 0, width, at);
-        if (A.update_weight) {
-          float s[1] = {0.f};
+          for (int i = 0; i < 8; ++i) n[j][i] *= r_u;
+      }
+      float g[kChunks][8];
 #pragma unroll
-          for (int j = 0; j < kChunks; ++j)
+      for (int j = 0; j < kChunks; ++j)
 #pragma unroll
-            for (int i = 0; i < 8; ++i) s[0] += n[j][i] * n[j][i];
-          row_sums<kLanes>(s, shared[turn]);
-          r_u = 1.0f / sqrtf(s[0] * A.inv_width + A.eps);
-          load_row<T>(w, A.update_weight, 0, width, at);
+        for (int i = 0; i < 8; ++i) g[j][i] = A.dsum ? in.dsum.get(j, i) : 0.f;
+      if (A.weight) {
+        if (A.update) {
 #pragma unroll
           for (int j = 0; j < kChunks; ++j)
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-              n[j][i] *= r_u;
-              c[j][i] *= w[j][i];
+              const float v = n[j][i] * c[j][i];
+              x[j][i] += A.gate ? v * in.gate.get(j, i) : v;
             }
         }
-      }
-      if (A.weight) {
-        float x[kChunks][8], gate[kChunks][8], h[kChunks][8];
-        if constexpr (kKept) {
-#pragma unroll
-          for (int j = 0; j < kChunks; ++j) {
-            if (at.left(j, width) > 0)
-              rows::load_packed(x[j], A.x_kept + row * pitch, at.chunk(j), blocks);
-            else
-#pragma unroll
-              for (int i = 0; i < 8; ++i) x[j][i] = 0.f;
-          }
-        } else {
-          load_row<X>(x, A.x, row * A.x_row, width, at);
-        }
-        if (A.update) {
-          if (A.gate) {
-            load_row<T>(gate, A.gate, gate_row * A.gate_row, width, at);
-#pragma unroll
-            for (int j = 0; j < kChunks; ++j)
-#pragma unroll
-              for (int i = 0; i < 8; ++i) x[j][i] += n[j][i] * c[j][i] * gate[j][i];
-          } else {
-#pragma unroll
-            for (int j = 0; j < kChunks; ++j)
-#pragma unroll
-              for (int i = 0; i < 8; ++i) x[j][i] += n[j][i] * c[j][i];
-          }
-        }
-        load_row<T>(h, A.dnormed, row * A.dnormed_row, width, at);
-        load_row<T>(w, A.weight, 0, width, at);
-        float s[2] = {0.f, 0.f};
-#pragma unroll
-        for (int j = 0; j < kChunks; ++j)
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            s[0] += x[j][i] * x[j][i];
-            s[1] += h[j][i] * w[j][i] * x[j][i];
-          }
+        float s[2] = {own_sum(at, [&](int j, int i) { return x[j][i] * x[j][i]; }),
+                      own_sum(at, [&](int j, int i) {
+                        return in.dnormed.get(j, i) * weight.get(j, i) * x[j][i];
+                      })};
         row_sums<kLanes>(s, shared[turn + 1]);
         const float r = 1.0f / sqrtf(s[0] * A.inv_width + A.eps);
         const float back = s[1] * A.inv_width * r * r;
@@ -164,54 +183,50 @@ __global__ __launch_bounds__(threads_of(kLanes), 1) void residual_backward_kerne
         for (int j = 0; j < kChunks; ++j)
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
-            dweight[j][i] += h[j][i] * (x[j][i] * r);
-            g[j][i] += r * (h[j][i] * w[j][i] - x[j][i] * back);
+            const float h = in.dnormed.get(j, i);
+            dweight[j][i] += h * (x[j][i] * r);
+            g[j][i] += r * (h * weight.get(j, i) - x[j][i] * back);
           }
       }
-      store_row<X>(A.dx, row * width, width, g, at);
+      store_row<X>(A.dx, row * width, g, at);
       if (!A.update) continue;
-      if (A.gate) {
-        float gate[kChunks][8], dgate[kChunks][8];
-        load_row<T>(gate, A.gate, gate_row * A.gate_row, width, at);
+      // g becomes the gradient of n
+      if (own_gate) {
+        float dgate[kChunks][8];
 #pragma unroll
         for (int j = 0; j < kChunks; ++j)
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
-            const float t = g[j][i] * n[j][i];
+            const float t = g[j][i] * n[j][i], gate = in.gate.get(j, i);
             dgate[j][i] = t * c[j][i];
-            q[j][i] += own_gate ? t * gate[j][i] : t;
-            c[j][i] *= gate[j][i];
+            q[j][i] += t * gate;
+            g[j][i] *= c[j][i] * gate;
           }
-        if (own_gate) store_row<T>(A.dgate, row * width, width, dgate, at);
+        store_row<T>(A.dgate, row * width, dgate, at);
       } else {
 #pragma unroll
         for (int j = 0; j < kChunks; ++j)
 #pragma unroll
-          for (int i = 0; i < 8; ++i) q[j][i] += g[j][i] * n[j][i];
+          for (int i = 0; i < 8; ++i) {
+            q[j][i] += g[j][i] * n[j][i];
+            g[j][i] *= A.gate ? c[j][i] * in.gate.get(j, i) : c[j][i];
+          }
       }
-#pragma unroll
-      for (int j = 0; j < kChunks; ++j)
-#pragma unroll
-        for (int i = 0; i < 8; ++i) c[j][i] *= g[j][i];
       if (A.update_weight) {
-        float s[1] = {0.f};
-#pragma unroll
-        for (int j = 0; j < kChunks; ++j)
-#pragma unroll
-          for (int i = 0; i < 8; ++i) s[0] += c[j][i] * n[j][i];
+        float s[1] = {own_sum(at, [&](int j, int i) { return g[j][i] * n[j][i]; })};
         row_sums<kLanes>(s, shared[turn + 2]);
         const float back = s[0] * A.inv_width;
 #pragma unroll
         for (int j = 0; j < kChunks; ++j)
 #pragma unroll
-          for (int i = 0; i < 8; ++i) c[j][i] = r_u * (c[j][i] - n[j][i] * back);
+          for (int i = 0; i < 8; ++i) g[j][i] = r_u * (g[j][i] - n[j][i] * back);
       }
-      store_row<T>(A.dupdate, row * width, width, c, at);
+      store_row<T>(A.dupdate, row * width, g, at);
     }
-    if (A.parts) flush<kLanes, kChunks>(q, A.parts + item * width, width, at, lds);
+    if (A.parts) flush(q, A.parts + item * width, at, lds);
   }
   if (A.weight_parts)
-    flush<kLanes, kChunks>(dweight, A.weight_parts + int64_t(blockIdx.x) * width, width, at, lds);
+    flush(dweight, A.weight_parts + int64_t(blockIdx.x) * width, at, lds);
 }
 
 constexpr int kSumThreads = 1024, kSumColumns = 64, kSlices = kSumThreads / kSumColumns;
@@ -295,9 +310,8 @@ __global__ __launch_bounds__(kSumThreads) void weight_sums_kernel(Args A, int64_
 // host side
 // ---------------------------------------------------------------------------
 
-// Blocks: as many as the card holds at once (256 CUs, two each), or fewer
-// where there are fewer rows.
-constexpr int kBackwardBlocks = 512;
+// Blocks: four for each of 256 CUs, or fewer where there are fewer rows.
+constexpr int kBackwardBlocks = 1024;
 
 struct Split {
   int64_t items, parts_each, blocks;
