@@ -128,7 +128,8 @@ class _ResidualNorm(torch.autograd.Function):
         dupdate_weight, dscale, dweight = (
             t if t is None else room(width) for t in (update_weight, scale, with_norm))
         nbytes = L.library().bevpool_residual_norm_backward_scratch_bytes(
-            rows, width, gate.shape[0] if gate is not None else 0)
+            rows, width, gate.shape[0] if gate is not None else 0, L.DTYPE_CODES[x_dtype],
+            int(keep))
         scratch = room(nbytes, kind=torch.uint8)
         _run(lambda lib, s: lib.bevpool_residual_norm_backward(
             *_row(x if with_norm is not None else None), L.DTYPE_CODES[x_dtype], *_row(update),

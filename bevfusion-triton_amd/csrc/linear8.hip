@@ -291,17 +291,9 @@ __global__ __launch_bounds__(256, 2) void product_kernel(ProductArgs A) {
           }
           const auto a = __builtin_amdgcn_permlane32_swap(q[0], q[2], false, false);
           const auto b = __builtin_amdgcn_permlane32_swap(q[1], q[3], false, false);
-          const attention::u32x4 out{a[0], b[0], a[1], b[1]};
-          rows::Pack<T> eight;
-          __builtin_memcpy(&eight, &out, 16);
+          const rows::Words<T> out{{a[0], b[0], a[1], b[1]}};
           const int at = w0 + ww + 32 * i + 16 * p + 8 * h;
-          if (valid && at + 8 <= A.channels) {
-            *reinterpret_cast<rows::Pack<T> *>(y + at) = eight;
-          } else if (valid) {
-#pragma unroll
-            for (int r = 0; r < 8; ++r)
-              if (at + r < A.channels) y[at + r] = eight.v[r];
-          }
+          out.store(y + at, valid ? A.channels - at : 0);
         }
       }
   }
@@ -314,6 +306,7 @@ constexpr int kFewWaves = 8;
 template <typename T, int kTx, int kTw>
 __global__ __launch_bounds__(64 * kFewWaves) void few_kernel(ProductArgs A) {
   __shared__ i32x4 sums[kFewWaves][kTw * kTx][64];
+  constexpr int kDeep = kTx > 2 ? 4 : 8;  // steps whose loads are on their way together
   const int lane = attention::lane_id(), wave = attention::wave_id();
   const int c = lane & 15, q = lane >> 4;
   const int w0 = int(blockIdx.x) * 16 * kTw, x0 = int(blockIdx.y) * 16 * kTx;
@@ -325,21 +318,27 @@ __global__ __launch_bounds__(64 * kFewWaves) void few_kernel(ProductArgs A) {
   for (int i = 0; i < kTx; ++i)
     x_at[i] = A.x + int64_t(min(x0 + 16 * i + c, A.tokens - 1)) * A.x_pitch;
   i32x4 acc[kTw][kTx] = {};
-#pragma unroll 8
-  for (int step = wave; step < A.steps; step += kFewWaves) {
-    i32x4 w[kTw], x[kTx];
-    const int chunk = step * 4 + q;
+  for (int first = wave; first < A.steps; first += kFewWaves * kDeep) {
+    i32x4 w[kDeep][kTw], x[kDeep][kTx];
 #pragma unroll
-    for (int i = 0; i < kTw; ++i)  // (past a row's end: as above)
-      w[i] = *reinterpret_cast<const i32x4 *>(w_at[i] + min(chunk, A.w_chunks - 1) * 16);
+    for (int d = 0; d < kDeep; ++d) {
+      const int step = first + d * kFewWaves, chunk = min(step, A.steps - 1) * 4 + q;
 #pragma unroll
-    for (int i = 0; i < kTx; ++i)
-      x[i] = *reinterpret_cast<const i32x4 *>(x_at[i] + chunk * 16);
+      for (int i = 0; i < kTw; ++i)  // (past a row's end: as above)
+        w[d][i] = *reinterpret_cast<const i32x4 *>(w_at[i] + min(chunk, A.w_chunks - 1) * 16);
 #pragma unroll
-    for (int i = 0; i < kTw; ++i)
+      for (int i = 0; i < kTx; ++i) {
+        x[d][i] = *reinterpret_cast<const i32x4 *>(x_at[i] + chunk * 16);
+        if (step >= A.steps) x[d][i] = i32x4{0, 0, 0, 0};
+      }
+    }
 #pragma unroll
-      for (int j = 0; j < kTx; ++j)
-        acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(w[i], x[j], acc[i][j], 0, 0, 0);
+    for (int d = 0; d < kDeep; ++d)
+#pragma unroll
+      for (int i = 0; i < kTw; ++i)
+#pragma unroll
+        for (int j = 0; j < kTx; ++j)
+          acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(w[d][i], x[d][j], acc[i][j], 0, 0, 0);
   }
 #pragma unroll
   for (int i = 0; i < kTw; ++i)

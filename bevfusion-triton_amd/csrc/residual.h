@@ -42,8 +42,18 @@ struct Args {
 
 // (rows of more than a wave pass barriers: a block of them has one)
 constexpr int threads_of(int lanes) { return lanes > 64 ? lanes : 256; }
-inline int rows_at_once(int width) {
-  return width <= 128 ? 16 : width <= 256 ? 8 : width <= 512 ? 4 : 1;
+// Waves of a SIMD that the registers of a kernel leave room for (they are
+// compiled to), and the blocks of the whole card: the kernels walk rows by as
+// many as are there at once.  More only begin later: backward of 200,000 rows of
+// 80 by three blocks a CU, as many as there is room for, 57 us, by four 71; one
+// block a row instead, forward of 16,896 rows of 1,280 63 us for 43.
+constexpr int forward_waves(int chunks) { return chunks > 1 ? 3 : 4; }
+constexpr int backward_waves(int lanes, int chunks, bool kept, bool wide) {
+  return chunks > 1 ? 2 : kept || lanes < 64 || wide ? 3 : 4;  // (wide: a stream in fp32)
+}
+constexpr int blocks_for(int lanes, int waves) {
+  const int each = 4 * waves * 64 / threads_of(lanes);
+  return 256 * (each > 1 ? each : 1);
 }
 
 // A lane's place: its row of a block's, and its chunks.  With kWhole, where the
@@ -71,71 +81,34 @@ struct Place {
   __device__ __forceinline__ int left(int j) const { return width - begin(j); }
 };
 
-// A row's values of a lane as they lie in memory, in whole registers.
+// A row's values of a lane, and those of its 8-bit checkpoint, as they lie in
+// memory.
 template <typename T, int kChunks>
 struct Raw {
-  static constexpr int kWords = rows::kChunk * int(sizeof(T)) / 4;
-  struct __attribute__((packed, aligned(sizeof(T)))) Words {
-    unsigned w[kWords];
-  };
-  Words c[kChunks];
+  rows::Words<T> c[kChunks];
   template <int kLanes, bool kWhole>
   __device__ __forceinline__ void load(const void *base, int64_t offset,
                                        const Place<kLanes, kChunks, kWhole> &at) {
     const T *row = static_cast<const T *>(base) + offset;
 #pragma unroll
-    for (int j = 0; j < kChunks; ++j) {
-      c[j] = {};
-      if (!at.on(j)) continue;
-      if (at.left(j) >= rows::kChunk) {
-        c[j] = *reinterpret_cast<const Words *>(row + at.begin(j));
-      } else {
-#pragma unroll
-        for (int i = 0; i < rows::kChunk; ++i) {
-          if (i >= at.left(j)) continue;
-          const T v = row[at.begin(j) + i];
-          if constexpr (sizeof(T) == 4)
-            c[j].w[i] = __builtin_bit_cast(unsigned, v);
-          else
-            c[j].w[i / 2] |= unsigned(__builtin_bit_cast(uint16_t, v)) << (i % 2 * 16);
-        }
-      }
-    }
+    for (int j = 0; j < kChunks; ++j)
+      c[j].load(row + at.begin(j), at.on(j) ? at.left(j) : 0);
   }
-  __device__ __forceinline__ float get(int j, int i) const {
-    if constexpr (sizeof(T) == 4) {
-      return __builtin_bit_cast(float, c[j].w[i]);
-    } else {
-      const unsigned w = c[j].w[i / 2];
-      if constexpr (__is_same(T, __bf16))  // (the upper half of the same number in fp32)
-        return __builtin_bit_cast(float, i % 2 ? w & 0xffff0000u : w << 16);
-      else
-        return float(__builtin_bit_cast(T, uint16_t(i % 2 ? w >> 16 : w)));
-    }
-  }
+  __device__ __forceinline__ float get(int j, int i) const { return c[j].get(i); }
 };
-
-// The same of a row's 8-bit checkpoint.
 template <int kChunks>
 struct Packed {
-  rows::Bytes c[kChunks];
-  unsigned scale[kChunks];
+  rows::PackedChunk c[kChunks];
   template <int kLanes>
   __device__ __forceinline__ void load(const uint8_t *row,
                                        const Place<kLanes, kChunks, false> &at) {
-    const uint8_t *scales = row + rows::blocks_of(at.width) * rows::kBlock;
 #pragma unroll
-    for (int j = 0; j < kChunks; ++j) {
-      c[j] = {0x80808080u, 0x80808080u};  // zeros
-      scale[j] = 1;
-      if (!at.on(j)) continue;
-      c[j] = *reinterpret_cast<const rows::Bytes *>(row + at.begin(j));
-      scale[j] = scales[at.begin(j) / rows::kBlock];
-    }
+    for (int j = 0; j < kChunks; ++j)
+      if (at.on(j)) c[j].load(row, at.chunk(j), rows::blocks_of(at.width));
   }
   __device__ __forceinline__ void get(float (&v)[kChunks][rows::kChunk]) const {
 #pragma unroll
-    for (int j = 0; j < kChunks; ++j) rows::unpack(v[j], c[j], scale[j]);
+    for (int j = 0; j < kChunks; ++j) c[j].get(v[j]);
   }
 };
 

@@ -64,7 +64,7 @@ __device__ __forceinline__ void keep(uint8_t *kept, const Raw<T, kChunks> &raw, 
 // A group of lanes takes rows, the next one's loads on their way while one is
 // worked on; weights stay in registers.
 template <typename T, typename X, int kLanes, int kChunks>
-__global__ __launch_bounds__(threads_of(kLanes)) void residual_kernel(Args A) {
+__global__ __launch_bounds__(threads_of(kLanes), forward_waves(kChunks)) void residual_kernel(Args A) {
   constexpr int kGroups = threads_of(kLanes) / kLanes;
   __shared__ float shared[4][threads_of(kLanes) / 64];
   const Place<kLanes, kChunks> at(A.width);
@@ -129,15 +129,13 @@ __global__ __launch_bounds__(threads_of(kLanes)) void residual_kernel(Args A) {
   }
 }
 
-// Blocks: as many as the card holds at once, or as there are rows.
-constexpr int kForwardBlocks = 2048;
-
 template <typename T, typename X, int kLanes, int kChunks>
 void launch(const Args &A, hipStream_t s) {
   constexpr int kGroups = threads_of(kLanes) / kLanes;
+  constexpr int kBlocks = blocks_for(kLanes, forward_waves(kChunks));
   const int64_t blocks = (A.rows + kGroups - 1) / kGroups;
   hipLaunchKernelGGL((residual_kernel<T, X, kLanes, kChunks>),
-                     dim3(unsigned(blocks < kForwardBlocks ? blocks : kForwardBlocks)),
+                     dim3(unsigned(blocks < kBlocks ? blocks : kBlocks)),
                      dim3(threads_of(kLanes)), 0, s, A);
 }
 

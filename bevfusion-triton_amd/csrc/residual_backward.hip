@@ -108,7 +108,7 @@ struct Inputs {
 // gate (without such a gate: of all), and leaves each item's sums.  Its groups
 // of lanes take rows, the next one's loads on their way while one is worked on.
 template <typename T, typename X, int kLanes, int kChunks, bool kKept>
-__global__ __launch_bounds__(threads_of(kLanes), 2) void residual_backward_kernel(Args A) {
+__global__ __launch_bounds__(threads_of(kLanes), backward_waves(kLanes, kChunks, kKept, sizeof(X) == 4)) void residual_backward_kernel(Args A) {
   constexpr int kGroups = threads_of(kLanes) / kLanes;
   typedef std::conditional_t<kKept, KeptOperands<kChunks>, Operands<T, X, kChunks>> Of;
   extern __shared__ float lds[];
@@ -229,7 +229,7 @@ __global__ __launch_bounds__(threads_of(kLanes), 2) void residual_backward_kerne
     flush(dweight, A.weight_parts + int64_t(blockIdx.x) * width, at, lds);
 }
 
-constexpr int kSumThreads = 1024, kSumColumns = 64, kSlices = kSumThreads / kSumColumns;
+constexpr int kSumThreads = 1024, kSumColumns = 32, kSlices = kSumThreads / kSumColumns;
 
 // The slices' sums, added in the slices' order; the first slice has them.
 __device__ __forceinline__ float slices_sum(float v, float *lds) {
@@ -310,24 +310,28 @@ __global__ __launch_bounds__(kSumThreads) void weight_sums_kernel(Args A, int64_
 // host side
 // ---------------------------------------------------------------------------
 
-// Blocks: four for each of 256 CUs, or fewer where there are fewer rows.
-constexpr int kBackwardBlocks = 1024;
-
 struct Split {
   int64_t items, parts_each, blocks;
 };
-Split split_for(int64_t rows, int width, int64_t gate_rows) {
+Split split_for(int64_t rows, int width, int64_t gate_rows, bool kept, bool wide) {
+  int64_t most_blocks = 0, at_once = 0;
+#define RESIDUAL_BLOCKS(kLanes, kChunks, ...)                                   \
+  {                                                                             \
+    most_blocks = blocks_for(kLanes, backward_waves(kLanes, kChunks, kept, wide));    \
+    at_once = threads_of(kLanes) / kLanes;                                      \
+  }
+  RESIDUAL_LAYOUT(RESIDUAL_BLOCKS, width)
+#undef RESIDUAL_BLOCKS
   const bool shared = gate_rows > 0 && gate_rows < rows;
   const int64_t owners = shared ? gate_rows : 1, each = rows / owners;
-  const int64_t at_once = rows_at_once(width);
-  int64_t parts = (kBackwardBlocks + owners - 1) / owners;
+  int64_t parts = (most_blocks + owners - 1) / owners;
   const int64_t most = (each + at_once - 1) / at_once;
   if (parts > most) parts = most;
   if (parts < 1) parts = 1;
   Split s;
   s.parts_each = parts;
   s.items = owners * parts;
-  s.blocks = s.items < kBackwardBlocks ? s.items : kBackwardBlocks;
+  s.blocks = s.items < most_blocks ? s.items : most_blocks;
   return s;
 }
 
@@ -369,10 +373,11 @@ void launch_sums(const Args &A, int64_t blocks, void *dgate, void *dupdate_weigh
 extern "C" {
 
 size_t bevpool_residual_norm_backward_scratch_bytes(int64_t rows, int32_t width,
-                                                    int64_t gate_rows) {
+                                                    int64_t gate_rows, int32_t x_dtype,
+                                                    int32_t kept) {
   using namespace residual;
   if (rows < 1 || width < 1 || width > kMaxWidth || gate_rows < 0) return 0;
-  const Split s = split_for(rows, width, gate_rows);
+  const Split s = split_for(rows, width, gate_rows, kept != 0, x_dtype == BEVPOOL_F32);
   return size_t(s.items + s.blocks) * size_t(width) * sizeof(float);
 }
 
@@ -399,7 +404,8 @@ int bevpool_residual_norm_backward(
     if (!dx || (update && !dupdate) || (gate && !dgate) || (weight && (!x || !dnormed)))
       return fail(BEVPOOL_EINVAL, "null rows");
     if (!scratch ||
-        scratch_bytes < bevpool_residual_norm_backward_scratch_bytes(rows, width, gate_rows))
+        scratch_bytes < bevpool_residual_norm_backward_scratch_bytes(
+                            rows, width, gate ? gate_rows : 0, x_dtype, kept))
       return fail(BEVPOOL_ESPACE, "residual_norm backward scratch too small");
   }
   A.x = x;
@@ -424,7 +430,7 @@ int bevpool_residual_norm_backward(
   A.dgate = dgate;
   Split split = {0, 1, 0};
   if (rows > 0) {
-    split = split_for(rows, width, gate ? gate_rows : 0);
+    split = split_for(rows, width, gate ? gate_rows : 0, kept != 0, x_dtype == BEVPOOL_F32);
     A.weight_parts = weight ? static_cast<float *>(scratch) : nullptr;
     const bool shared = gate && gate_rows < rows;
     if (update && (update_weight || scale || shared))

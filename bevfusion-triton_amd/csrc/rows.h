@@ -29,37 +29,81 @@ __host__ __device__ inline int64_t checkpoint_pitch(int64_t width) {
   return (blocks_of(width) * (kBlock + 1) + 15) / 16 * 16;
 }
 
-// (loads and stores of 16 bytes need no more than the type's own alignment)
+// A chunk as it lies in memory, in whole registers: what reads it is apart from
+// what converts it, so that the loads of several are on their way together.
+// (Accesses of 16 bytes need no more than the type's own alignment.)
 template <typename T>
-struct __attribute__((packed, aligned(sizeof(T)))) Pack {
-  T v[kChunk];
+struct __attribute__((packed, aligned(sizeof(T)))) Words {
+  static constexpr int kWords = kChunk * int(sizeof(T)) / 4;
+  unsigned w[kWords];
+  // `left` values are there (the others: zeros)
+  __device__ __forceinline__ void load(const T *at, int left) {
+#pragma unroll
+    for (int i = 0; i < kWords; ++i) w[i] = 0;
+    if (left >= kChunk) {
+      *this = *reinterpret_cast<const Words *>(at);
+    } else if (left > 0) {
+#pragma unroll
+      for (int i = 0; i < kChunk; ++i) {
+        if (i >= left) continue;
+        const T v = at[i];
+        if constexpr (sizeof(T) == 4)
+          w[i] = __builtin_bit_cast(unsigned, v);
+        else
+          w[i / 2] |= unsigned(__builtin_bit_cast(uint16_t, v)) << (i % 2 * 16);
+      }
+    }
+  }
+  __device__ __forceinline__ float get(int i) const {
+    if constexpr (sizeof(T) == 4) {
+      return __builtin_bit_cast(float, w[i]);
+    } else if constexpr (__is_same(T, __bf16)) {  // (the upper half of the same number in fp32)
+      return __builtin_bit_cast(float, i % 2 ? w[i / 2] & 0xffff0000u : w[i / 2] << 16);
+    } else {
+      return float(__builtin_bit_cast(T, uint16_t(i % 2 ? w[i / 2] >> 16 : w[i / 2])));
+    }
+  }
+  __device__ __forceinline__ void set(const float (&v)[kChunk]) {
+#pragma unroll
+    for (int i = 0; i < kWords; ++i) {
+      if constexpr (sizeof(T) == 4) {
+        w[i] = __builtin_bit_cast(unsigned, v[i]);
+      } else {
+        typedef T Pair __attribute__((ext_vector_type(2)));
+        const Pair pair{T(v[2 * i]), T(v[2 * i + 1])};
+        w[i] = __builtin_bit_cast(unsigned, pair);
+      }
+    }
+  }
+  __device__ __forceinline__ void store(T *at, int left) const {
+    if (left >= kChunk) {
+      *reinterpret_cast<Words *>(at) = *this;
+    } else if (left > 0) {
+#pragma unroll
+      for (int i = 0; i < kChunk; ++i) {
+        if (i >= left) continue;
+        if constexpr (sizeof(T) == 4)
+          at[i] = __builtin_bit_cast(T, w[i]);
+        else
+          at[i] = __builtin_bit_cast(T, uint16_t(w[i / 2] >> (i % 2 * 16)));
+      }
+    }
+  }
 };
 
-// Values of a row from `at` on, `left` of them there (zeros behind them).
+// The same at once.
 template <typename T>
 __device__ __forceinline__ void load(float (&to)[kChunk], const T *at, int left) {
-  if (left >= kChunk) {
-    const Pack<T> p = *reinterpret_cast<const Pack<T> *>(at);
+  Words<T> words;
+  words.load(at, left);
 #pragma unroll
-    for (int i = 0; i < kChunk; ++i) to[i] = float(p.v[i]);
-  } else {
-#pragma unroll
-    for (int i = 0; i < kChunk; ++i) to[i] = i < left ? float(at[i]) : 0.f;
-  }
+  for (int i = 0; i < kChunk; ++i) to[i] = words.get(i);
 }
-
 template <typename T>
 __device__ __forceinline__ void store(T *at, const float (&from)[kChunk], int left) {
-  if (left >= kChunk) {
-    Pack<T> p;
-#pragma unroll
-    for (int i = 0; i < kChunk; ++i) p.v[i] = T(from[i]);
-    *reinterpret_cast<Pack<T> *>(at) = p;
-  } else {
-#pragma unroll
-    for (int i = 0; i < kChunk; ++i)
-      if (i < left) at[i] = T(from[i]);
-  }
+  Words<T> words;
+  words.set(from);
+  words.store(at, left);
 }
 
 template <int kControl>
@@ -162,13 +206,17 @@ __device__ __forceinline__ void unpack(float (&v)[kChunk], Bytes b, unsigned sca
   }
 }
 
-// Chunk c of a row of a checkpoint.  (Chunks of the last block behind the
-// row's end are there: zeros.)
-__device__ __forceinline__ void load_packed(float (&v)[kChunk], const uint8_t *row, int c,
-                                            int64_t blocks) {
-  const Bytes b = *reinterpret_cast<const Bytes *>(row + c * int64_t(kChunk));
-  unpack(v, b, row[blocks * kBlock + c / 4]);
-}
+// Chunk c of a row of a checkpoint as it lies there.  (Chunks of the last block
+// behind the row's end are there: zeros.)
+struct PackedChunk {
+  Bytes bytes = {0x80808080u, 0x80808080u};  // zeros
+  unsigned scale = 1;
+  __device__ __forceinline__ void load(const uint8_t *row, int c, int64_t blocks) {
+    bytes = *reinterpret_cast<const Bytes *>(row + c * int64_t(kChunk));
+    scale = row[blocks * kBlock + c / 4];
+  }
+  __device__ __forceinline__ void get(float (&v)[kChunk]) const { unpack(v, bytes, scale); }
+};
 // The block's four lanes call it together.
 __device__ __forceinline__ void store_packed(uint8_t *row, int c, int64_t blocks,
                                              const float (&v)[kChunk]) {

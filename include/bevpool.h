@@ -715,7 +715,8 @@ int bevpool_residual_norm_forward(const void *x, int64_t x_row, int32_t x_dtype,
  *   scratch      >= bevpool_residual_norm_backward_scratch_bytes(...)
  */
 size_t bevpool_residual_norm_backward_scratch_bytes(int64_t rows, int32_t width,
-                                                    int64_t gate_rows);
+                                                    int64_t gate_rows, int32_t x_dtype,
+                                                    int32_t kept);
 
 int bevpool_residual_norm_backward(
     const void *x, int64_t x_row, int32_t x_dtype, const void *update, int64_t update_row,

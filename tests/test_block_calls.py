@@ -53,7 +53,7 @@ def test_residual_norm_entries(pkg):
             x, 64, 2, update, 64, uw, None, gate, 64, gate_rows, weight, 0, None, 0, dnormed, 64, 2,
             rows, 64, 1e-6, dx, dupdate, dgate, duw, dscale, dweight, scratch, nbytes, None)
 
-    need = lib.bevpool_residual_norm_backward_scratch_bytes(8, 64, 4)
+    need = lib.bevpool_residual_norm_backward_scratch_bytes(8, 64, 4, 2, 0)
     refused(lib, backward, (
         (dict(gate_rows=3), -1, b'divide'), (dict(x=None), -1, b'null'), (dict(dx=None), -1, b'null'),
         (dict(dupdate=None), -1, b'null'), (dict(dgate=None), -1, b'null'),
@@ -61,7 +61,7 @@ def test_residual_norm_entries(pkg):
         (dict(dweight=None), -1, b'place'), (dict(dscale=16), -1, b'not there'),
         (dict(update=None), -1, b'of an update'), (dict(scratch=None), -3, b'scratch'),
         (dict(nbytes=need - 1), -3, b'scratch')))
-    assert need > 0 and lib.bevpool_residual_norm_backward_scratch_bytes(0, 64, 0) == 0
+    assert need > 0 and lib.bevpool_residual_norm_backward_scratch_bytes(0, 64, 0, 2, 0) == 0
 
 
 def test_gated_and_checkpoint_entries(pkg):
