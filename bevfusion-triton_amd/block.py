@@ -22,6 +22,8 @@ allocate with torch's allocator and never wait for the device.
 """
 from __future__ import annotations
 
+import functools
+
 import torch
 from torch import nn
 from torch.autograd.function import once_differentiable
@@ -38,7 +40,8 @@ MAX_INT8_WIDTH = 1 << 17
 
 def _rows(x):
     """x as (rows, width) with unit stride along the width."""
-    x = x.unsqueeze(0) if x.dim() == 1 else x.flatten(0, -2)
+    if x.dim() != 2:
+        x = x.unsqueeze(0) if x.dim() == 1 else x.flatten(0, -2)
     return _unit(x)
 
 
@@ -47,17 +50,26 @@ def _row(x):
     return (x.data_ptr(), x.stride(0)) if x is not None else (0, 0)
 
 
-def _check_type(name, x, dtype=None):
+def _check_type(name, x):
     if x.dtype not in L.DTYPE_CODES:
         raise TypeError(f'{name} must have dtype torch.float16, torch.float32, or torch.bfloat16.')
-    if dtype is not None and x.dtype != dtype:
+
+
+def _check_beside(name, t, dtype, device):
+    if t.dtype != dtype:
         raise TypeError(f'{name} must have dtype {dtype}.')
+    if t.device != device:
+        raise ValueError(f'{name} must be on the device of x ({device}).')
 
 
-def _check_device(like, **tensors):
-    for name, t in tensors.items():
-        if t is not None and t.device != like.device:
-            raise ValueError(f'{name} must be on the device of x ({like.device}).')
+def _vector(name, t, size, dtype, device, shape='width'):
+    """t (size,), contiguous; None is None."""
+    if t is None:
+        return None
+    _check_beside(name, t, dtype, device)
+    if t.shape != (size,):
+        raise ValueError(f'{name} must have shape [{shape}].')
+    return t if t.is_contiguous() else t.contiguous()
 
 
 def _check_checkpoint(checkpoint):
@@ -74,11 +86,6 @@ def _kept(x, rows, width, copies=1):
 
 # ---- residual and norms ----------------------------------------------------
 
-def _gate(gate):
-    """(address, row stride, rows) for a call."""
-    return (*_row(gate), gate.shape[0] if gate is not None else 0)
-
-
 def _residual_norm(x, update, update_weight, scale, gate, weight, dtype, eps, keep=False):
     """(sum, normed, checkpoint of x, of update) of rows."""
     rows, width = x.shape
@@ -89,7 +96,8 @@ def _residual_norm(x, update, update_weight, scale, gate, weight, dtype, eps, ke
     update_kept = _kept(x, rows, width) if keep and update is not None else None
     _run(lambda lib, s: lib.bevpool_residual_norm_forward(
         *_row(x), L.DTYPE_CODES[x.dtype], *_row(update), L.ptr(update_weight), L.ptr(scale),
-        *_gate(gate), L.ptr(weight), L.DTYPE_CODES[dtype], rows, width, eps, L.ptr(total),
+        *_row(gate), 0 if gate is None else gate.shape[0], L.ptr(weight), L.DTYPE_CODES[dtype], rows,
+        width, eps, L.ptr(total),
         L.ptr(normed), L.ptr(x_kept), L.ptr(update_kept), s), x.device,
         'bevpool_residual_norm_forward')
     return total, normed, x_kept, update_kept
@@ -114,32 +122,43 @@ class _ResidualNorm(torch.autograd.Function):
         rows, width, x_dtype, device, dtype, eps, keep, has_update = ctx.call
         if dtotal is None and dnormed is None:
             return (None,) * 9
-        with_norm = weight if dnormed is not None else None
-        dtotal, dnormed = (g if g is None else _unit(g if g.dtype == t else g.to(t))
-                           for g, t in ((dtotal, x_dtype), (dnormed, dtype)))
-
-        def room(*shape, kind=dtype):
-            return torch.empty(shape, dtype=kind, device=device)
-
-        dx = room(rows, width, kind=x_dtype)
-        dupdate = room(rows, width) if has_update else None
-        # (no kernel writes the sums of no rows)
-        dgate = None if gate is None else room(*gate.shape) if rows else torch.zeros_like(gate)
-        dupdate_weight, dscale, dweight = (
-            t if t is None else room(width) for t in (update_weight, scale, with_norm))
-        nbytes = L.library().bevpool_residual_norm_backward_scratch_bytes(
-            rows, width, gate.shape[0] if gate is not None else 0, L.DTYPE_CODES[x_dtype],
-            int(keep))
-        scratch = room(nbytes, kind=torch.uint8)
+        dweight = None
+        if dnormed is None:
+            if weight is not None:
+                dweight, weight = torch.zeros_like(weight), None
+            x = None
+        elif dnormed.dtype != dtype or dnormed.stride(1) != 1:
+            dnormed = _unit(dnormed.to(dtype))
+        if dtotal is not None and (dtotal.dtype != x_dtype or dtotal.stride(1) != 1):
+            dtotal = _unit(dtotal.to(x_dtype))
+        new = (dtotal if dnormed is None else dnormed).new_empty
+        dx = new((rows, width), dtype=x_dtype)
+        dupdate = new((rows, width), dtype=dtype) if has_update else None
+        dupdate_weight = None if update_weight is None else new(width, dtype=dtype)
+        dscale = None if scale is None else new(width, dtype=dtype)
+        if weight is not None:
+            dweight = new(width, dtype=dtype)
+        gate_rows, dgate = 0, None
+        if gate is not None:
+            gate_rows = gate.shape[0]
+            # (no kernel writes the sums of no rows)
+            dgate = new((gate_rows, width), dtype=dtype) if rows else torch.zeros_like(gate)
+        x_code = L.DTYPE_CODES[x_dtype]
+        nbytes = _backward_scratch(rows, width, gate_rows, x_code, keep)
+        scratch = new(nbytes, dtype=torch.uint8)
+        ptr = L.ptr
         _run(lambda lib, s: lib.bevpool_residual_norm_backward(
-            *_row(x if with_norm is not None else None), L.DTYPE_CODES[x_dtype], *_row(update),
-            L.ptr(update_weight), L.ptr(scale), *_gate(gate), L.ptr(with_norm), int(keep),
-            *_row(dtotal), *_row(dnormed), L.DTYPE_CODES[dtype], rows, width, eps, L.ptr(dx),
-            L.ptr(dupdate), L.ptr(dgate), L.ptr(dupdate_weight), L.ptr(dscale), L.ptr(dweight),
-            L.ptr(scratch), nbytes, s), device, 'bevpool_residual_norm_backward')
-        if weight is not None and with_norm is None:
-            dweight = torch.zeros_like(weight)
+            *_row(x), x_code, *_row(update), ptr(update_weight), ptr(scale), *_row(gate), gate_rows,
+            ptr(weight), keep, *_row(dtotal), *_row(dnormed), L.DTYPE_CODES[dtype], rows, width, eps,
+            ptr(dx), ptr(dupdate), ptr(dgate), ptr(dupdate_weight), ptr(dscale),
+            0 if weight is None else ptr(dweight), ptr(scratch), nbytes, s), device,
+            'bevpool_residual_norm_backward')
         return dx, dupdate, dupdate_weight, dscale, dgate, dweight, None, None, None
+
+
+@functools.lru_cache(maxsize=256)
+def _backward_scratch(*sizes):
+    return L.library().bevpool_residual_norm_backward_scratch_bytes(*sizes)
 
 
 def residual_norm(x, update=None, *, update_weight=None, scale=None, gate=None, weight=None,
@@ -164,50 +183,51 @@ def residual_norm(x, update=None, *, update_weight=None, scale=None, gate=None, 
     the values that the copies stand for."""
     keep = _check_checkpoint(checkpoint)
     _check_type('x', x)
+    P.require_gpu(x)
     if x.dim() < 1:
         raise ValueError('x must have shape [..., width].')
-    width = x.shape[-1]
+    shape, device = x.shape, x.device
+    width = shape[-1]
     if not 1 <= width <= MAX_RESIDUAL_WIDTH:
         raise ValueError(f'width must be in [1, {MAX_RESIDUAL_WIDTH}].')
-    if update is None and not (update_weight is scale is gate is None):
-        raise ValueError('update_weight, scale and gate are of an update.')
-    if update is None and weight is None:
-        raise ValueError('neither an update nor a weight: nothing to do.')
-    if not eps >= 0:
-        raise ValueError('eps must not be negative.')
-    dtype = weight.dtype if update is None else update.dtype
-    if update is not None:
+    if update is None:
+        if not (update_weight is scale is gate is None):
+            raise ValueError('update_weight, scale and gate are of an update.')
+        if weight is None:
+            raise ValueError('neither an update nor a weight: nothing to do.')
+        _check_type('weight', weight)
+        dtype = weight.dtype
+    else:
         _check_type('update', update)
-        if update.shape != x.shape:
+        dtype = update.dtype
+        _check_beside('update', update, dtype, device)
+        if update.shape != shape:
             raise ValueError('update must have the shape of x.')
-    for name, t in (('update_weight', update_weight), ('scale', scale), ('weight', weight)):
-        if t is not None:
-            _check_type(name, t, dtype)
-            if tuple(t.shape) != (width,):
-                raise ValueError(f'{name} must have shape [width].')
     if x.dtype not in (dtype, torch.float32):
         raise TypeError(f'x must have dtype torch.float32 or that of the others ({dtype}).')
-    rows = x.numel() // width
+    if not eps >= 0:
+        raise ValueError('eps must not be negative.')
+    update_weight = _vector('update_weight', update_weight, width, dtype, device)
+    scale = _vector('scale', scale, width, dtype, device)
+    weight = _vector('weight', weight, width, dtype, device)
     if gate is not None:
-        _check_type('gate', gate, dtype)
-        if gate.shape != x.shape and not (gate.dim() in (1, 2) and gate.shape[-1] == width):
+        _check_beside('gate', gate, dtype, device)
+        if gate.shape != shape and not (gate.dim() in (1, 2) and gate.shape[-1] == width):
             raise ValueError('gate must have the shape of x, [groups, width] or [width].')
         gate = _rows(gate)
-        if gate.shape[0] < min(rows, 1) or gate.shape[0] and rows % gate.shape[0]:
+        rows, groups = x.numel() // width, gate.shape[0]
+        if groups < min(rows, 1) or groups and rows % groups:
             raise ValueError('the rows of gate must divide those of x.')
-    P.require_gpu(*[t for t in (x, update, update_weight, scale, gate, weight) if t is not None])
-    _check_device(x, update=update, update_weight=update_weight, scale=scale, gate=gate,
-                  weight=weight)
-    weights = [t if t is None else t.contiguous() for t in (update_weight, scale)]
-    weight = weight if weight is None else weight.contiguous()
-    args = (_rows(x), None if update is None else _rows(update), *weights, gate, weight, dtype,
-            float(eps))
-    if _wants_grad(x, update, *weights, gate, weight) or _recorded():
+    args = (_rows(x), None if update is None else _rows(update), update_weight, scale, gate, weight,
+            dtype, float(eps))
+    if _wants_grad(x, update, update_weight, scale, gate, weight) or _recorded():
         total, normed = _ResidualNorm.apply(*args, keep)
     else:
         total, normed = _residual_norm(*args)[:2]
-    return (x if total is None else total.view(x.shape),
-            normed if normed is None else normed.view(x.shape))
+    if len(shape) == 2:
+        return x if total is None else total, normed
+    return (x if total is None else total.view(shape),
+            normed if normed is None else normed.view(shape))
 
 
 # ---- gated activation ------------------------------------------------------
@@ -262,7 +282,7 @@ def gated_activation(x, kind='silu', *, checkpoint=None):
         out = _Gated.apply(rows, kind, keep)
     else:
         out = _gated(rows, kind)[0]
-    return out.view(*x.shape[:-1], x.shape[-1] // 2)
+    return out if x.dim() == 2 else out.view(*x.shape[:-1], x.shape[-1] // 2)
 
 
 # ---- 8-bit checkpoints -----------------------------------------------------
@@ -341,27 +361,26 @@ def checkpoint_linear(x, weight, bias=None):
     weight's gradient is an 8-bit copy, and the gradient is that at the values
     it stands for.  The others are exact.  Follows autocast."""
     _check_type('x', x)
-    if torch.is_autocast_enabled('cuda'):
+    P.require_gpu(x)
+    autocast = torch.is_autocast_enabled('cuda')
+    if autocast:
         kind = torch.get_autocast_dtype('cuda')
         x, weight = x.to(kind), weight.to(kind)
         bias = bias if bias is None else bias.to(kind)
-    _check_type('weight', weight, x.dtype)
+    _check_beside('weight', weight, x.dtype, x.device)
     if weight.dim() != 2 or x.dim() < 1 or x.shape[-1] != weight.shape[1]:
         raise ValueError('x must have shape [..., in] and weight [out, in].')
     if not 1 <= x.shape[-1] <= MAX_GATED_WIDTH:
         raise ValueError(f'in must be in [1, {MAX_GATED_WIDTH}].')
-    if bias is not None:
-        _check_type('bias', bias, x.dtype)
-        if bias.shape != weight.shape[:1]:
-            raise ValueError('bias must have shape [out].')
-    P.require_gpu(*[t for t in (x, weight, bias) if t is not None])
-    _check_device(x, weight=weight, bias=bias)
+    bias = _vector('bias', bias, weight.shape[0], x.dtype, x.device, 'out')
     if not _wants_grad(x, weight, bias) and not _recorded():
         return nn.functional.linear(x, weight, bias)
-    # (autocast off: the operands have their types)
-    with torch.autocast('cuda', enabled=False):
+    if autocast:  # (the operands have their types)
+        with torch.autocast('cuda', enabled=False):
+            y = _CheckpointLinear.apply(_rows(x), weight, bias)
+    else:
         y = _CheckpointLinear.apply(_rows(x), weight, bias)
-    return y.view(*x.shape[:-1], weight.shape[0])
+    return y if x.dim() == 2 else y.view(*x.shape[:-1], weight.shape[0])
 
 
 class CheckpointLinear(nn.Linear):
@@ -441,6 +460,7 @@ def linear_int8(x, codes, scales, bias=None):
     that do not start at multiples of 16 bytes are copied at each call.  No
     gradient."""
     _check_type('x', x)
+    P.require_gpu(x)
     if codes.dim() != 2 or codes.dtype != torch.int8:
         raise TypeError('codes must have dtype torch.int8 and shape [out, in].')
     channels, width = codes.shape
@@ -448,21 +468,17 @@ def linear_int8(x, codes, scales, bias=None):
         raise ValueError(f'in must be in [1, {MAX_INT8_WIDTH}].')
     if x.dim() < 1 or x.shape[-1] != width:
         raise ValueError('x must have shape [..., in], in as codes have it.')
-    if scales.dtype != torch.float32 or tuple(scales.shape) != (channels,):
-        raise ValueError('scales must have dtype torch.float32 and shape [out].')
-    if bias is not None:
-        _check_type('bias', bias, x.dtype)
-        if tuple(bias.shape) != (channels,):
-            raise ValueError('bias must have shape [out].')
-    P.require_gpu(*[t for t in (x, codes, scales, bias) if t is not None])
-    _check_device(x, codes=codes, scales=scales, bias=bias)
+    device = x.device
+    if codes.device != device:
+        raise ValueError(f'codes must be on the device of x ({device}).')
+    scales = _vector('scales', scales, channels, torch.float32, device, 'out')
+    bias = _vector('bias', bias, channels, x.dtype, device, 'out')
     if _wants_grad(x, scales, bias):
         raise RuntimeError('linear_int8 has no gradient; call it under torch.no_grad()')
-    bias = bias if bias is None else bias.contiguous()
     codes, row = _code_rows(codes) if channels else (codes, 0)
     run = _LinearInt8.apply if _recorded() else _linear_int8
-    y = run(_rows(x), codes, int(row), scales.contiguous(), bias)  # (a trace has sizes as tensors)
-    return y.view(*x.shape[:-1], channels)
+    y = run(_rows(x), codes, int(row), scales, bias)  # (a trace has sizes as tensors)
+    return y if x.dim() == 2 else y.view(*x.shape[:-1], channels)
 
 
 class Int8Linear(nn.Module):

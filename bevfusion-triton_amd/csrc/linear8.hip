@@ -48,15 +48,43 @@ __device__ __forceinline__ float scale_of(float top) {
   return top < __builtin_inff() ? s : __builtin_nanf("");
 }
 
-// rint(x / s), ties to even, for |x| <= 127 s: the product with the rounded
-// 1 / s is off by less than 2^-15, so k is right or one off where x is next to
-// a border; x - k s is exact.
-__device__ __forceinline__ int code_of(float x, float s, float inverse) {
-  const float k = rintf(x * inverse);
-  const float d = 2.f * fmaf(-k, s, x);
-  const int q = int(k);
-  if (fabsf(d) > s || (fabsf(d) == s && (q & 1))) return d > 0.f ? q + 1 : q - 1;
-  return q;
+// rint(x / s), ties to even, for |x| <= 127 s, as the low byte of a word.  The
+// quotient comes from 1 / s with one correction, which makes it exact where it
+// has few enough bits, as halves of whole numbers have.  Quotients of a number
+// of at most 11 bits (fp16, bf16) by one of 8 are such a half or 2^-12 away from
+// it, far more than the 2^-16 that they may be off.  In fp32 they can be nearer:
+// there x is compared with the border itself; x - k s is exact.
+template <typename T>
+__device__ __forceinline__ unsigned code_of(float x, float s, float inverse) {
+  float q = x * inverse;
+  q = fmaf(fmaf(-q, s, x), inverse, q);
+  if constexpr (sizeof(T) == 4) {
+    const float k = rintf(q), d = 2.f * fmaf(-k, s, x);
+    q = fabsf(d) > s ? k + copysignf(1.f, d) : k;
+    // (an exact tie went to the even one: its quotient is exact)
+  }
+  // added to 1.5 2^23 a number is rounded to a whole one, ties to even
+  return __builtin_bit_cast(unsigned, q + 12582912.f);
+}
+
+// The largest magnitude of a chunk, as the bits of an fp32 number (those of
+// infinities and NaN are the largest).
+template <typename T>
+__device__ __forceinline__ unsigned top_of(const rows::Words<T> &c) {
+  unsigned top = 0;
+  if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) top = max(top, c.w[i] & 0x7fffffffu);
+    return top;
+  } else {
+    typedef unsigned short Pair __attribute__((ext_vector_type(2)));
+    Pair most = {0, 0};
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      most = __builtin_elementwise_max(most, __builtin_bit_cast(Pair, c.w[i] & 0x7fff7fffu));
+    top = max(unsigned(most[0]), unsigned(most[1]));
+    return __builtin_bit_cast(unsigned, float(__builtin_bit_cast(T, uint16_t(top)))) & 0x7fffffffu;
+  }
 }
 
 // A row of codes by kLanes lanes that hold it (kChunks chunks each), or, with
@@ -64,49 +92,55 @@ __device__ __forceinline__ int code_of(float x, float s, float inverse) {
 template <typename T, int kLanes, int kChunks>
 __global__ __launch_bounds__(256) void codes_kernel(const T *x, int64_t x_row, int64_t n, int width,
                                                     int pitch, int8_t *codes, float *scales) {
-  __shared__ float shared[4];
+  __shared__ unsigned shared[4];
   constexpr int kHold = kChunks > 0 ? kChunks : 1;
   const int lane = int(threadIdx.x) % kLanes;
   const int64_t row = int64_t(blockIdx.x) * (256 / kLanes) + int(threadIdx.x) / kLanes;
   const bool on = row < n;  // (the same for a row's lanes)
   const T *at = x + (on ? row : 0) * x_row;
-  const int chunks = kChunks > 0 ? kChunks : (pitch / 8 + kLanes - 1) / kLanes;
-  float v[kHold][8], top = 0.f;
-  bool finite = true;
-  auto look = [&](const float (&c)[8]) {
+  rows::Words<T> c[kHold];
+  unsigned top = 0;
+  if constexpr (kChunks > 0) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      top = fmaxf(top, fabsf(c[i]));  // (passes over NaN)
-      finite = finite && c[i] == c[i];
+    for (int j = 0; j < kChunks; ++j) {
+      const int d = (lane + j * kLanes) * 8;
+      c[j].load(at + d, width - d);
     }
-  };
-  for (int j = 0; j < chunks; ++j) {
-    float(&c)[8] = v[kChunks > 0 ? j : 0];
-    const int d = (lane + j * kLanes) * 8;
-    rows::load(c, at + d, width - d);
-    look(c);
-  }
-  if (!finite) top = __builtin_inff();
 #pragma unroll
-  for (int m = 1; m < (kLanes < 64 ? kLanes : 64); m <<= 1) top = fmaxf(top, __shfl_xor(top, m, 64));
-  if (kLanes > 64) {
+    for (int j = 0; j < kChunks; ++j) top = max(top, top_of(c[j]));
+  } else {
+    for (int d = lane * 8; d < width; d += kLanes * 8) {
+      c[0].load(at + d, width - d);
+      top = max(top, top_of(c[0]));
+    }
+  }
+#pragma unroll
+  for (int m = 1; m < 64; m <<= 1) top = max(top, unsigned(__shfl_xor(int(top), m, 64)));
+  if constexpr (kLanes > 64) {
     if (threadIdx.x % 64 == 0) shared[threadIdx.x / 64] = top;
     __syncthreads();
-    top = fmaxf(fmaxf(shared[0], shared[1]), fmaxf(shared[2], shared[3]));
+    top = max(max(shared[0], shared[1]), max(shared[2], shared[3]));
   }
   if (!on) return;
-  const float s = scale_of(top), inverse = 1.f / s;
+  const float s = scale_of(__builtin_bit_cast(float, top)), inverse = 1.f / s;
   if (lane == 0) scales[row] = s;
-  for (int j = 0; j < chunks; ++j) {
-    float(&c)[8] = v[kChunks > 0 ? j : 0];
-    const int d = (lane + j * kLanes) * 8;
-    if (d >= pitch) continue;
-    if (kChunks == 0) rows::load(c, at + d, width - d);
-    unsigned q[2] = {0, 0};
+  auto put = [&](const rows::Words<T> &words, int d) {
+    unsigned q[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-      q[i / 4] |= (unsigned(code_of(c[i], s, inverse)) & 0xffu) << (i % 4 * 8);
-    *reinterpret_cast<rows::Bytes *>(codes + row * pitch + d) = {q[0], q[1]};
+    for (int i = 0; i < 8; ++i) q[i] = code_of<T>(words.get(i), s, inverse);
+    *reinterpret_cast<rows::Bytes *>(codes + row * pitch + d) = rows::low_bytes(q);
+  };
+  if constexpr (kChunks > 0) {
+#pragma unroll
+    for (int j = 0; j < kChunks; ++j) {
+      const int d = (lane + j * kLanes) * 8;
+      if (d < pitch) put(c[j], d);
+    }
+  } else {
+    for (int d = lane * 8; d < pitch; d += kLanes * 8) {
+      c[0].load(at + d, width - d);
+      put(c[0], d);
+    }
   }
 }
 
@@ -304,9 +338,9 @@ __global__ __launch_bounds__(256, 2) void product_kernel(ProductArgs A) {
 // are on their way all at once, and add their sums in LDS.
 constexpr int kFewWaves = 8;
 template <typename T, int kTx, int kTw>
-__global__ __launch_bounds__(64 * kFewWaves) void few_kernel(ProductArgs A) {
+__global__ __launch_bounds__(64 * kFewWaves, kTx * kTw > 4 ? 2 : 4) void few_kernel(ProductArgs A) {
   __shared__ i32x4 sums[kFewWaves][kTw * kTx][64];
-  constexpr int kDeep = kTx > 2 ? 4 : 8;  // steps whose loads are on their way together
+  constexpr int kDeep = 4;  // steps whose loads are on their way together
   const int lane = attention::lane_id(), wave = attention::wave_id();
   const int c = lane & 15, q = lane >> 4;
   const int w0 = int(blockIdx.x) * 16 * kTw, x0 = int(blockIdx.y) * 16 * kTx;
@@ -322,16 +356,20 @@ __global__ __launch_bounds__(64 * kFewWaves) void few_kernel(ProductArgs A) {
     i32x4 w[kDeep][kTw], x[kDeep][kTx];
 #pragma unroll
     for (int d = 0; d < kDeep; ++d) {
-      const int step = first + d * kFewWaves, chunk = min(step, A.steps - 1) * 4 + q;
+      const int step = first + d * kFewWaves, chunk = step * 4 + q;
+#pragma unroll
+      for (int i = 0; i < kTw; ++i) w[d][i] = i32x4{0, 0, 0, 0};
+#pragma unroll
+      for (int i = 0; i < kTx; ++i) x[d][i] = i32x4{0, 0, 0, 0};
+      if (step >= A.steps) continue;
 #pragma unroll
       for (int i = 0; i < kTw; ++i)  // (past a row's end: as above)
         w[d][i] = *reinterpret_cast<const i32x4 *>(w_at[i] + min(chunk, A.w_chunks - 1) * 16);
 #pragma unroll
-      for (int i = 0; i < kTx; ++i) {
+      for (int i = 0; i < kTx; ++i)
         x[d][i] = *reinterpret_cast<const i32x4 *>(x_at[i] + chunk * 16);
-        if (step >= A.steps) x[d][i] = i32x4{0, 0, 0, 0};
-      }
     }
+    __builtin_amdgcn_sched_barrier(0);  // (else the compiler takes loads to their products)
 #pragma unroll
     for (int d = 0; d < kDeep; ++d)
 #pragma unroll

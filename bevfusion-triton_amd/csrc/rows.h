@@ -139,11 +139,21 @@ __device__ __forceinline__ float power(unsigned biased) {
   return __builtin_bit_cast(float, biased << 23);
 }
 
-// A chunk as bytes, and its block's scale (a biased exponent).  The block's
-// four lanes call it together; values past a row's end are zeros.
 struct Bytes {
   unsigned low, high;
 };
+// The low bytes of eight words.
+__device__ __forceinline__ Bytes low_bytes(const unsigned (&q)[kChunk]) {
+  auto four = [](unsigned a, unsigned b, unsigned c, unsigned d) {
+    const unsigned ab = __builtin_amdgcn_perm(b, a, 0x0c0c0400u);
+    const unsigned cd = __builtin_amdgcn_perm(d, c, 0x0c0c0400u);
+    return ab | cd << 16;
+  };
+  return {four(q[0], q[1], q[2], q[3]), four(q[4], q[5], q[6], q[7])};
+}
+
+// A chunk as bytes, and its block's scale (a biased exponent).  The block's
+// four lanes call it together; values past a row's end are zeros.
 __device__ __forceinline__ Bytes pack(const float (&v)[kChunk], unsigned &scale) {
   constexpr unsigned kInfinite = 0x7f800000u;
   unsigned top = 0, worst = 0;
@@ -183,13 +193,7 @@ __device__ __forceinline__ Bytes pack(const float (&v)[kChunk], unsigned &scale)
     for (int i = 0; i < kChunk; ++i)
       if ((__builtin_bit_cast(unsigned, v[i]) & 0x7fffffffu) >= kInfinite) q[i] = 0;
   }
-  // bytes 0 of four words
-  auto four = [](unsigned a, unsigned b, unsigned c, unsigned d) {
-    const unsigned ab = __builtin_amdgcn_perm(b, a, 0x0c0c0400u);
-    const unsigned cd = __builtin_amdgcn_perm(d, c, 0x0c0c0400u);
-    return ab | cd << 16;
-  };
-  return {four(q[0], q[1], q[2], q[3]), four(q[4], q[5], q[6], q[7])};
+  return low_bytes(q);
 }
 
 __device__ __forceinline__ void unpack(float (&v)[kChunk], Bytes b, unsigned scale) {
