@@ -15,6 +15,10 @@ ziyangyeh/bevfusion-triton behind the reference's own Python surface:
   norm_rotate, attend_packed, attend_cached  operators of a transformer over camera and BEV
                                             tokens, and TokenAttention, the layer that
                                             runs them (no counterpart in the reference)
+  residual_norm, gated_activation,          operators of the block around it: norms fused
+  checkpoint_linear, pack_activations,      with gate and residual, 8-bit checkpoints,
+  linear_int8, quantize_weight              8-bit integer products, and TokenBlock, which
+                                            runs them (no counterpart)
 
 The kernels live in ``csrc/`` and are reached through the C ABI of
 ``include/bevpool.h`` (``libbevpool_amd.so``, loaded by ``_lib``).  There is no
@@ -29,7 +33,7 @@ from .attention import attend_cached, attend_packed, axis_frequencies, norm_rota
 from .block import (CheckpointLinear, Int8Linear, PackedActivations, checkpoint_linear, gated_activation, linear_int8,
                     pack_activations, quantize_weight, residual_norm)
 from .bev_pool import BevPoolFunction, BevPoolIndexExport, bev_pool, check_errors
-from .tokens import TokenAttention
+from .tokens import TokenAttention, TokenBlock
 from .vtransform import (BevPoolTransform, CameraIndex, LSSIndexExport, create_frustum, gen_dx_bx, host_grid, lss_bev_pool, lss_bev_pool_depth,
                          lss_index_cameras)
 
@@ -45,6 +49,7 @@ __all__ = [
     'LibraryNotBuilt',
     'PackedActivations',
     'TokenAttention',
+    'TokenBlock',
     'attend_cached',
     'attend_packed',
     'axis_frequencies',

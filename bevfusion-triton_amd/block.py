@@ -501,7 +501,6 @@ class Int8Linear(nn.Module):
             self.scales = scales.to(self.scales.device)
         return self
 
-    @torch.no_grad()
     def forward(self, x):
         if torch.is_autocast_enabled('cuda'):
             x = x.to(torch.get_autocast_dtype('cuda'))

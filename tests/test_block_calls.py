@@ -20,6 +20,14 @@ def block(pkg, monkeypatch):
     return block
 
 
+@pytest.fixture(autouse=True)
+def no_error_left(pkg):
+    """The thread's error text is as other tests expect it: a call of nothing
+    clears it."""
+    yield
+    assert pkg.library().bevpool_gated_forward(None, 0, 0, 0, 1, 0, None, None, None) == 0
+
+
 # ---- the C entries: they return before any HIP call ------------------------
 
 def refused(lib, call, cases):
