@@ -161,6 +161,12 @@ _SIGNATURES = {
     'bevpool_checkpoint_pitch': ([_i32], _i64),
     'bevpool_checkpoint_pack': ([_vp, _i64, _i32, _i64, _i32, _vp, _vp], ctypes.c_int),
     'bevpool_checkpoint_unpack': ([_vp, _i32, _i64, _i32, _vp, _vp], ctypes.c_int),
+    'bevpool_checkpoint_weight_grad_scratch_bytes': ([_i64, _i32, _i32], _sz),
+    'bevpool_checkpoint_weight_grad': (
+        [_vp, _i64, _vp, _i32, _i64, _i32, _i32, _vp, _vp, _sz, _vp], ctypes.c_int,
+    ),
+    'bevpool_column_sums_scratch_bytes': ([_i32], _sz),
+    'bevpool_column_sums': ([_vp, _i64, _i32, _i64, _i32, _vp, _vp, _sz, _vp], ctypes.c_int),
     'bevpool_residual_norm_forward': (
         [_vp, _i64, _i32, _vp, _i64, _vp, _vp, _vp, _i64, _i64, _vp, _i32, _i64, _i32, _f32, _vp,
          _vp, _vp, _vp, _vp],

@@ -332,6 +332,34 @@ def pack_activations(x):
     return PackedActivations(data, x.shape, x.dtype)
 
 
+def _weight_grad(dy, data, x_shape):
+    """dy^T x of the checkpoint of x."""
+    n, k = dy.shape[1], x_shape[1]
+    dweight = dy.new_empty((n, k))
+    nbytes = _weight_grad_scratch(dy.shape[0], n, k)
+    scratch = dy.new_empty(nbytes, dtype=torch.uint8)
+    _run(lambda lib, s: lib.bevpool_checkpoint_weight_grad(
+        *_row(dy), L.ptr(data), L.DTYPE_CODES[dy.dtype], dy.shape[0], n, k, L.ptr(dweight),
+        L.ptr(scratch), nbytes, s), dy.device, 'bevpool_checkpoint_weight_grad')
+    return dweight
+
+
+@functools.lru_cache(maxsize=256)
+def _weight_grad_scratch(*sizes):
+    return L.library().bevpool_checkpoint_weight_grad_scratch_bytes(*sizes)
+
+
+def _column_sums(x):
+    dy = _unit(x)
+    out = dy.new_empty(dy.shape[1])
+    nbytes = L.library().bevpool_column_sums_scratch_bytes(dy.shape[1])
+    scratch = dy.new_empty(nbytes, dtype=torch.uint8)
+    _run(lambda lib, s: lib.bevpool_column_sums(
+        *_row(dy), L.DTYPE_CODES[dy.dtype], *dy.shape, L.ptr(out), L.ptr(scratch), nbytes, s),
+        dy.device, 'bevpool_column_sums')
+    return out
+
+
 class _CheckpointLinear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias):
@@ -345,13 +373,20 @@ class _CheckpointLinear(torch.autograd.Function):
     @once_differentiable  # (the gradients are no functions of the graph's)
     def backward(ctx, dy):
         data, weight = ctx.saved_tensors
+        x_shape, dtype = ctx.call
         dx = dweight = dbias = None
         if ctx.needs_input_grad[0]:
             dx = dy @ weight
         if ctx.needs_input_grad[1]:
-            dweight = dy.t() @ PackedActivations(data, *ctx.call).unpack()
+            tokens, n = dy.shape
+            if dtype != torch.float32 and tokens and n and n % 8 == 0:
+                if dy.stride(1) != 1 or dy.stride(0) % 8 or dy.data_ptr() % 16 or dy.stride(0) >= 1 << 24:
+                    dy = dy.clone(memory_format=torch.contiguous_format)
+                dweight = _weight_grad(dy, data, x_shape)
+            else:
+                dweight = dy.t() @ PackedActivations(data, x_shape, dtype).unpack()
         if ctx.needs_input_grad[2]:
-            dbias = dy.sum(0)
+            dbias = _column_sums(dy)
         return dx, dweight, dbias
 
 

@@ -684,6 +684,30 @@ int bevpool_checkpoint_unpack(const void *kept, int32_t dtype, int64_t rows, int
                               void *out, void *stream);
 
 /*
+ * The gradient of a linear layer's weight from the checkpoint of its input:
+ * dweight[i][j] = sum over tokens t of dy[t][i] x[t][j], x being what the
+ * checkpoint stands for.  Sums in fp32, in an order that the sizes alone set.
+ *   dy           (tokens, n), fp16 or bf16, n a multiple of 8, rows from
+ *                multiples of 16 bytes; tokens at least 1
+ *   kept         checkpoint of (tokens, k), from a multiple of 16 bytes
+ *   dweight      (n, k) contiguous, in dtype
+ *   scratch      >= bevpool_checkpoint_weight_grad_scratch_bytes(...): sums of
+ *                parts of the tokens, up to 512 x 256 x 128 numbers and more
+ *                only where dweight has more
+ * And that of its bias, the sums of columns: out [width] of x (rows, width).
+ */
+size_t bevpool_checkpoint_weight_grad_scratch_bytes(int64_t tokens, int32_t n, int32_t k);
+
+int bevpool_checkpoint_weight_grad(const void *dy, int64_t dy_row, const void *kept, int32_t dtype,
+                                   int64_t tokens, int32_t n, int32_t k, void *dweight,
+                                   void *scratch, size_t scratch_bytes, void *stream);
+
+size_t bevpool_column_sums_scratch_bytes(int32_t width);
+
+int bevpool_column_sums(const void *x, int64_t x_row, int32_t dtype, int64_t rows, int32_t width,
+                        void *out, void *scratch, size_t scratch_bytes, void *stream);
+
+/*
  * Norms after and before a block with the residual between them:
  *   n      = update / sqrt(mean(update^2) + eps) * update_weight
  *            (update_weight NULL: n = update)

@@ -99,6 +99,33 @@ def test_gated_and_checkpoint_entries(pkg):
     assert [pitch(w) for w in (0, 1, 32, 33, 1280)] == [0, 48, 48, 80, 1328]
 
 
+def test_weight_gradient_entries(pkg):
+    lib = pkg.library()
+
+    def grad(dy=16, row=64, kept=16, dtype=2, tokens=100, n=64, k=40, dw=16, scratch=16, nbytes=1 << 30):
+        return lib.bevpool_checkpoint_weight_grad(dy, row, kept, dtype, tokens, n, k, dw, scratch,
+                                                  nbytes, None)
+
+    need = lib.bevpool_checkpoint_weight_grad_scratch_bytes(100, 64, 40)
+    refused(lib, grad, (
+        (dict(dtype=0), -1, b'16-bit'), (dict(tokens=0), -1, b'tokens'), (dict(n=60), -1, b'multiple of 8'),
+        (dict(n=0), -1, b'multiple of 8'), (dict(k=0), -1, b'2^18'), (dict(k=(1 << 18) + 1), -1, b'2^18'),
+        (dict(dy=None), -1, b'null'), (dict(kept=None), -1, b'null'), (dict(dw=None), -1, b'null'),
+        (dict(dy=8), -1, b'16 bytes'), (dict(row=60), -1, b'16 bytes'), (dict(row=1 << 24), -1, b'16 bytes'),
+        (dict(kept=8), -1, b'16 bytes'), (dict(scratch=None), -3, b'scratch'),
+        (dict(nbytes=need - 1), -3, b'scratch')))
+    assert need == 64 * 40 * 4
+
+    def sums(x=16, dtype=2, rows=9, width=5, out=16, scratch=16, nbytes=1 << 20):
+        return lib.bevpool_column_sums(x, 5, dtype, rows, width, out, scratch, nbytes, None)
+
+    need = lib.bevpool_column_sums_scratch_bytes(5)
+    refused(lib, sums, (
+        (dict(dtype=3), -1, b'dtype'), (dict(rows=-1), -1, b'rows'), (dict(width=0), -1, b'width'),
+        (dict(x=None), -1, b'null'), (dict(out=None), -1, b'null'), (dict(scratch=None), -3, b'scratch'),
+        (dict(nbytes=need - 1), -3, b'scratch')))
+
+
 def test_linear8_entries(pkg):
     lib = pkg.library()
 
@@ -233,17 +260,18 @@ def operands(cuda, rows=37, width=120, dtype=torch.bfloat16):
     g = torch.Generator().manual_seed(rows)
     n = lambda *s: torch.randn(s, generator=g).to(cuda, dtype)
     return {'x': n(rows, width), 'update': n(rows, width), 'w': 1 + 0.2 * n(width), 'gate': n(1, width),
-            'linear': n(64, width), 'dx': n(rows, width), 'dhalf': n(rows, width // 2), 'dy': n(rows, 64)}
+            'linear': n(64, width), 'bias': n(64), 'dx': n(rows, width), 'dhalf': n(rows, width // 2), 'dy': n(rows, 64)}
 
 
 def steps(pkg, t, codes, checkpoint):
     """One pass through each operator with its gradients."""
-    leaves = [t[n].detach().requires_grad_(True) for n in ('x', 'update', 'w', 'gate', 'linear')]
-    x, update, w, gate, linear = leaves
+    leaves = [t[n].detach().requires_grad_(True)
+              for n in ('x', 'update', 'w', 'gate', 'linear', 'bias')]
+    x, update, w, gate, linear, bias = leaves
     total, normed = pkg.residual_norm(x, update, update_weight=w, scale=w, gate=gate, weight=w,
                                       checkpoint=checkpoint)
     half = pkg.gated_activation(x, 'gelu', checkpoint=checkpoint)
-    y = pkg.checkpoint_linear(x, linear)
+    y = pkg.checkpoint_linear(x, linear, bias)
     with torch.no_grad():
         z = pkg.linear_int8(t['x'], *codes)
     grads = torch.autograd.grad((total, normed, half, y), leaves, (t['dx'], t['dx'], t['dhalf'], t['dy']))

@@ -179,6 +179,53 @@ def test_checkpoint_linear(pkg, cuda, dtype, rows, width, out, bias):
     assert torch.equal(y, torch.nn.functional.linear(*leaves))
 
 
+@pytest.mark.parametrize('dtype', [torch.float16, torch.bfloat16], ids=str)
+@pytest.mark.parametrize('rows,width,out', [
+    (1, 1, 8), (31, 40, 16), (32, 128, 256), (33, 129, 264), (64, 33, 512), (255, 300, 8),
+    (257, 127, 248), (1000, 260, 520), (5003, 96, 40), (9001, 257, 300 * 8)])
+def test_weight_gradients(pkg, cuda, dtype, rows, width, out):
+    """The weight's gradient from the checkpoint itself: sizes on both sides of
+    steps, tiles and parts of the tokens; gradients of wide pitches."""
+    g = torch.Generator().manual_seed(rows)
+    x = (torch.randn((rows, width), generator=g) * 2 ** torch.randint(-6, 6, (rows, 1), generator=g)
+         ).to(dtype)
+    dy = torch.randn((rows, out), generator=g).to(dtype)
+    w = torch.randn((out, width), generator=g).to(dtype)
+    X, D, kept = x.to(cuda), dy.double(), ref.kept(x)
+    leaf = w.to(cuda).requires_grad_(True)
+    wide, odd = (torch.full((rows, out + 24), math.nan, dtype=dtype, device=cuda) for _ in range(2))
+    results = []
+    for grad in (dy.to(cuda), wide[:, 8:out + 8].copy_(dy), odd[:, 3:out + 3].copy_(dy)):
+        results.append(torch.autograd.grad(pkg.checkpoint_linear(X, leaf), leaf, grad)[0])
+    close(results[0], D.T @ kept, (rows + 8) * ref.F * (D.abs().T @ kept.abs()), 'dweight')
+    for r in results[1:]:
+        assert torch.equal(r, results[0])
+
+
+@pytest.mark.parametrize('dtype', DTYPES, ids=str)
+def test_bias_gradients(pkg, cuda, dtype):
+    for rows, out in ((1, 1), (3, 65), (300, 7), (5001, 130)):
+        g = torch.Generator().manual_seed(rows)
+        dy = torch.randn((rows, out), generator=g).to(dtype)
+        x, w = torch.zeros((rows, 8), device=cuda, dtype=dtype), torch.zeros((out, 8), device=cuda, dtype=dtype)
+        b = torch.zeros(out, device=cuda, dtype=dtype, requires_grad=True)
+        for grad in (dy.to(cuda), dy.t().contiguous().t().to(cuda)):
+            d, = torch.autograd.grad(pkg.checkpoint_linear(x, w, b), b, grad)
+            close(d, dy.double().sum(0), (rows + 8) * ref.F * dy.double().abs().sum(0), 'dbias')
+
+
+def test_values_that_are_not_finite_in_gradients(pkg, cuda):
+    """One gradient and one input: their row and column of the weight's gradient."""
+    x, dy = torch.randn(70, 40, device=cuda).bfloat16(), torch.randn(70, 24, device=cuda).bfloat16()
+    w = torch.zeros(24, 40, device=cuda, dtype=torch.bfloat16, requires_grad=True)
+    x[69, 5], dy[69, 9] = math.nan, math.inf
+    d, = torch.autograd.grad(pkg.checkpoint_linear(x, w), w, dy)
+    bad = ~d.isfinite()
+    want = torch.zeros_like(bad)
+    want[:, 5] = want[9] = True
+    assert torch.equal(bad, want)
+
+
 def test_checkpoint_linear_layer(pkg, cuda):
     """Leading dimensions, autocast, and what needs no gradient."""
     torch.manual_seed(0)
