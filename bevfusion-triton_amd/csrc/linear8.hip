@@ -195,16 +195,16 @@ __device__ __forceinline__ void wait_steps(int left) {
     wait_steps<kLoads, (kMost > 0 ? kMost - 1 : 0)>(left);
 }
 
-// One block: kX tokens by kW channels, four waves of 32 kTx x 32 kTw.  Channels
+// One block: kX tokens by kW channels, kWavesX x kWavesW waves of 32 kTx x 32 kTw.  Channels
 // are the rows of the matrix instruction's result, tokens its columns: a lane
 // holds one token's channels, four neighbours a register group.
-template <typename T, int kTx, int kTw, int kWavesX, int kBuffers>
-__global__ __launch_bounds__(256, 2) void product_kernel(ProductArgs A) {
-  constexpr int kThreads = 256, kWavesW = 4 / kWavesX;
+template <typename T, int kTx, int kTw, int kWavesX, int kWavesW, int kBuffers>
+__global__ __launch_bounds__(64 * kWavesX * kWavesW, 2) void product_kernel(ProductArgs A) {
+  constexpr int kThreads = 64 * kWavesX * kWavesW;
   constexpr int kX = 32 * kTx * kWavesX, kW = 32 * kTw * kWavesW;
   constexpr int kLoadsX = kX * 4 / kThreads, kLoadsW = kW * 4 / kThreads;
   constexpr int kTileX = kX * kStep, kTile = (kX + kW) * kStep;
-  static_assert(kX % 64 == 0 && kW % 64 == 0, "whole rounds of loads");
+  static_assert(kX * 4 % kThreads == 0 && kW * 4 % kThreads == 0, "whole rounds of loads");
   extern __shared__ __align__(16) char lds[];
   float *scales = reinterpret_cast<float *>(lds + kBuffers * kTile), *biases = scales + kW;
   int x_tile, w_tile;
@@ -449,15 +449,16 @@ int codes_for(const void *x, int64_t x_row, int dtype, int64_t n, int width, int
   return check_launch("linear8_codes");
 }
 
-template <typename T, int kTx, int kTw, int kWavesX, int kBuffers>
+template <typename T, int kTx, int kTw, int kWavesX, int kWavesW, int kBuffers>
 int launch_tiles(ProductArgs &A, hipStream_t s) {
-  constexpr int kX = 32 * kTx * kWavesX, kW = 32 * kTw * (4 / kWavesX);
+  constexpr int kThreads = 64 * kWavesX * kWavesW, kX = 32 * kTx * kWavesX, kW = 32 * kTw * kWavesW;
   A.x_tiles = (A.tokens + kX - 1) / kX;
   A.w_tiles = (A.channels + kW - 1) / kW;
   const int64_t blocks = (int64_t(A.x_tiles) * A.w_tiles + 7) / 8 * 8;
-  const int st = check_grid(blocks, 256, "linear8");
+  const int st = check_grid(blocks, kThreads, "linear8");
   if (st) return st;
-  hipLaunchKernelGGL((product_kernel<T, kTx, kTw, kWavesX, kBuffers>), dim3(unsigned(blocks)), dim3(256),
+  hipLaunchKernelGGL((product_kernel<T, kTx, kTw, kWavesX, kWavesW, kBuffers>),
+                     dim3(unsigned(blocks)), dim3(kThreads),
                      kBuffers * (kX + kW) * kStep + 2 * kW * sizeof(float), s, A);
   return check_launch("linear8");
 }
@@ -485,17 +486,25 @@ int launch_product(ProductArgs &A, hipStream_t s) {
   // 7.5 and 8.7.
   if (A.tokens <= 64)
     return A.channels >= 32 * 160 ? launch_few_tokens<T, 2>(A, s) : launch_few_tokens<T, 1>(A, s);
-  // Tiles of 128 x 256 from one for each CU on (us of these and of 64 x 128:
-  // 1024 x 4096 x 8192 50 and 67, 1500 x 1280 x 10240 33 and 44; 800 x 4096 x
-  // 4096 42 and 31), else of 64 x 128, or 64 x 64 where that is not two for
-  // each (64 x 128 and 64 x 64: 800 x 4096 x 4096 31 and 38, 512 x 4096 x 4096
-  // 24 and 23, 100 x 4096 x 6144 22 and 19).
   auto tiles = [&](int x, int w) {
     return int64_t((A.tokens + x - 1) / x) * ((A.channels + w - 1) / w);
   };
-  if (tiles(128, 256) >= 256) return launch_tiles<T, 2, 4, 2, 3>(A, s);
-  if (tiles(64, 64) > 512) return launch_tiles<T, 1, 2, 2, 6>(A, s);
-  return launch_tiles<T, 1, 1, 2, 8>(A, s);
+  // Tiles of 256 x 256, one a CU, read each operand least often: a round of 256
+  // takes 0.88 of the time of 512 of 128 x 256, two a CU (8192 x 8192 x 8192 519
+  // and 590 us), but a last round of up to 256 of these, one a CU, 0.6 of it.  So
+  // us by 256 x 256 and 128 x 256: 16896 x 1280 x 10240 323 and 336, 1500 x 1280 x
+  // 10240 29 and 33; 16896 x 5120 x 1280 148 and 143, 1024 x 4096 x 8192 60 and 48.
+  const int64_t wide = tiles(256, 256), half = tiles(128, 256), rest = half % 512;
+  if (wide >= 128 &&
+      (wide + 255) / 256 * 88 < half / 512 * 100 + (rest > 256 ? 100 : rest > 0 ? 60 : 0))
+    return launch_tiles<T, 4, 2, 2, 4, 4>(A, s);
+  // From one for each CU on 128 x 256 (us of these and of 64 x 128: 1024 x 4096 x
+  // 8192 50 and 67; 800 x 4096 x 4096 42 and 31), else 64 x 128, or 64 x 64 where
+  // that is not two for each (64 x 128 and 64 x 64: 800 x 4096 x 4096 31 and 38,
+  // 512 x 4096 x 4096 24 and 23, 100 x 4096 x 6144 22 and 19).
+  if (half >= 256) return launch_tiles<T, 2, 4, 2, 2, 3>(A, s);
+  if (tiles(64, 64) > 512) return launch_tiles<T, 1, 2, 2, 2, 6>(A, s);
+  return launch_tiles<T, 1, 1, 2, 2, 8>(A, s);
 }
 
 int check_sizes(int dtype, int64_t tokens, int64_t width, int64_t channels) {

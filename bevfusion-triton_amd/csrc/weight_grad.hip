@@ -6,7 +6,7 @@
 // exact in the operands' type, so the products are those of the type's matrix
 // instructions and only their sums are rounded, in fp32.
 //
-// A block takes 256 x 128 of dW and a part of the tokens, 32 at a time: rows of
+// A block takes 256 x 256 of dW and a part of the tokens, 32 at a time: rows of
 // dy go to LDS as they are, bytes of x through LDS and registers, where they
 // become numbers of the type, to a tile of their own.  Both tiles have tokens as
 // rows and are read transposed.  The parts' sums are joined in their order.
@@ -26,12 +26,15 @@ using bevpool_host::check_launch;
 using bevpool_host::fail;
 using bevpool_host::LaunchScope;
 
-constexpr int kThreads = 256;
-constexpr int kN = 256, kK = 128;  // a block's part of dW
-constexpr int kTokens = 32;        // of a step
-constexpr int kHalfTile = kTokens * 256;       // bytes of 128 columns
-constexpr int kRaw = kTokens * kK + kTokens * 4;  // bytes of x, then its scales
-constexpr int kLds = 3 * 2 * kHalfTile + 2 * kHalfTile + 2 * kRaw;
+constexpr int kThreads = 256;            // (join and sums)
+constexpr int kGradThreads = 512;        // eight waves of 128 x 64
+constexpr int kSide = 256;               // a block's part of dW, both ways
+constexpr int kTokens = 32;              // of a step
+constexpr int kHalf = kTokens * 256;     // bytes of 128 columns
+constexpr int kTile = 2 * kHalf;         // of 256
+constexpr int kScales = kTokens * kSide; // where the scales of x's bytes begin
+constexpr int kRaw = kScales + kTokens * 8;
+constexpr int kLds = 4 * kTile + 2 * kTile + 3 * kRaw;
 
 struct GradArgs {
   const char *dy;
@@ -45,125 +48,174 @@ struct GradArgs {
 };
 
 template <typename T>
-__global__ __launch_bounds__(kThreads, 2) void weight_grad_kernel(GradArgs A) {
+__global__ __launch_bounds__(kGradThreads, 2) void weight_grad_kernel(GradArgs A) {
   extern __shared__ __align__(16) char lds[];
-  char *const x_lds = lds + 3 * 2 * kHalfTile, *const raw_lds = x_lds + 2 * kHalfTile;
+  char *const x_lds = lds + 4 * kTile, *const raw_lds = x_lds + 2 * kTile;
   // blocks of one XCD (every eighth) take parts of the tokens that lie together,
   // all tiles of one part before the next: they read the same rows at the same time
   const int tiles = A.n_tiles * A.k_tiles, total = tiles * A.n_parts, each = (total + 7) / 8;
   const int id = int(blockIdx.x % 8) * each + int(blockIdx.x / 8);
   if (int(blockIdx.x / 8) >= each || id >= total) return;
   const int part = id / tiles, tile = id - part * tiles;
-  const int n0 = tile / A.k_tiles * kN, k0 = tile % A.k_tiles * kK;
+  const int n0 = tile / A.k_tiles * kSide, k0 = tile % A.k_tiles * kSide;
   const int64_t begin = part * A.share, end = min(begin + A.share, A.tokens);
   const int steps = int((end - begin + kTokens - 1) / kTokens);
   const int lane = attention::lane_id(), wave = attention::wave_id();
   const unsigned lds0 = attention::lds_address(lds), raw0 = attention::lds_address(raw_lds);
 
-  // this lane's pieces of a step: four chunks of dy, one of x's bytes and, for
-  // eight lanes of a wave, the scales of the rows that the wave converts
-  int dy_r[4];
-  unsigned dy_off[4];
+  // this lane's pieces of a step: two chunks of dy, one of x's bytes and, for
+  // eight lanes of a wave, the scales of the four rows that the wave converts
+  int dy_r[2];
+  unsigned dy_off[2];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int slot = i * kThreads + int(threadIdx.x), in = slot % 512;
+  for (int i = 0; i < 2; ++i) {
+    const int in = int(threadIdx.x);  // (the tile's half i)
     dy_r[i] = in / 16;
     const int chunk = in % 16 ^ attention::swizzle<T, 128>(dy_r[i]);
-    const int col = min(n0 + slot / 512 * 128 + chunk * 8, A.n - 8);  // (past n: not stored)
+    const int col = min(n0 + i * 128 + chunk * 8, A.n - 8);  // (past n: not stored)
     dy_off[i] = unsigned(dy_r[i] * int(A.dy_row) + col * 2);
   }
-  const int raw_r = int(threadIdx.x) / 8, raw_c = int(threadIdx.x) % 8;
+  const int raw_r = int(threadIdx.x) / 16, raw_c = int(threadIdx.x) % 16;
   const unsigned raw_off = unsigned(raw_r * int(A.pitch) + min(k0 + raw_c * 16, A.blocks * 32 - 16));
-  const int scale_r = wave * 8 + (lane & 7);
-  const unsigned scale_off = unsigned(scale_r * int(A.pitch) + A.blocks * 32 + k0 / 32);
+  const int scale_r = wave * 4 + (lane & 7) / 2;
+  const unsigned scale_off =
+      unsigned(scale_r * int(A.pitch) + A.blocks * 32 + k0 / 32 + lane % 2 * 4);
 
   auto load = [&](int step) {
     const int64_t t0 = begin + int64_t(step) * kTokens;
     const int rows = int(min(int64_t(kTokens), end - t0));
     const char *dy = A.dy + t0 * A.dy_row;
     const char *kept = reinterpret_cast<const char *>(A.kept) + t0 * A.pitch;
-    const unsigned to = lds0 + step % 3 * 2 * kHalfTile, raw = raw0 + step % 2 * kRaw;
+    const unsigned to = lds0 + step % 4 * kTile + wave * 1024, raw = raw0 + step % 3 * kRaw;
     if (rows == kTokens) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        attention::load_to_lds(dy, dy_off[i], to + i * kThreads * 16 + wave * 1024);
+      attention::load_to_lds(dy, dy_off[0], to);
+      attention::load_to_lds(dy, dy_off[1], to + kHalf);
       attention::load_to_lds(kept, raw_off, raw + wave * 1024);
-      if (lane < 8) attention::load_to_lds4(kept, scale_off, raw + kTokens * kK + wave * 32);
+      if (lane < 8) attention::load_to_lds4(kept, scale_off, raw + kScales + wave * 32);
     } else {  // (rows past the part: zeros)
-      char *at = lds + step % 3 * 2 * kHalfTile, *raw_at = raw_lds + step % 2 * kRaw;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        if (dy_r[i] < rows)
-          attention::load_to_lds(dy, dy_off[i], to + i * kThreads * 16 + wave * 1024);
-        else
-          *reinterpret_cast<attention::u32x4 *>(at + (i * kThreads + int(threadIdx.x)) * 16) =
-              attention::u32x4{0, 0, 0, 0};
-      }
-      if (raw_r < rows)
+      const attention::u32x4 zero = {0, 0, 0, 0};
+      const unsigned none = 0x80808080u;
+      char *at = lds + step % 4 * kTile + int(threadIdx.x) * 16, *raw_at = raw_lds + step % 3 * kRaw;
+      if (raw_r < rows) {  // (dy's row of a lane is that of its bytes)
+        attention::load_to_lds(dy, dy_off[0], to);
+        attention::load_to_lds(dy, dy_off[1], to + kHalf);
         attention::load_to_lds(kept, raw_off, raw + wave * 1024);
-      else
+      } else {
+        *reinterpret_cast<attention::u32x4 *>(at) = zero;
+        *reinterpret_cast<attention::u32x4 *>(at + kHalf) = zero;
         *reinterpret_cast<attention::u32x4 *>(raw_at + int(threadIdx.x) * 16) =
-            attention::u32x4{0x80808080u, 0x80808080u, 0x80808080u, 0x80808080u};
+            attention::u32x4{none, none, none, none};
+      }
       if (lane < 8) {
         if (scale_r < rows)
-          attention::load_to_lds4(kept, scale_off, raw + kTokens * kK + wave * 32);
+          attention::load_to_lds4(kept, scale_off, raw + kScales + wave * 32);
         else
-          *reinterpret_cast<unsigned *>(raw_at + kTokens * kK + scale_r * 4) = 0x01010101u;
+          *reinterpret_cast<unsigned *>(raw_at + kScales + wave * 32 + lane * 4) = 0x01010101u;
       }
     }
   };
-  // bytes of x (of this lane's own load) to a tile of numbers
-  auto convert = [&](int step) {
-    const char *raw = raw_lds + step % 2 * kRaw;
-    const attention::u32x4 bytes =
-        *reinterpret_cast<const attention::u32x4 *>(raw + int(threadIdx.x) * 16);
-    const unsigned scales = *reinterpret_cast<const unsigned *>(raw + kTokens * kK + raw_r * 4);
-    const unsigned scale = scales >> (raw_c / 2 * 8) & 0xffu;
-    char *to = x_lds + step % 2 * kHalfTile + raw_r * 256;
+  // bytes of x (of this lane's own load) as numbers.  Without a branch, so that
+  // it runs beside the products: what is not finite, and the largest scale, whose
+  // 128 times is infinite, are left to mend().
+  struct Numbers {
+    attention::u32x4 bytes;
+    unsigned scale;
+    rows::Words<T> words[2];
+  };
+  auto fetch = [&](int step, Numbers &x) {
+    const char *raw = raw_lds + step % 3 * kRaw;
+    x.bytes = *reinterpret_cast<const attention::u32x4 *>(raw + int(threadIdx.x) * 16);
+    const unsigned scales =
+        *reinterpret_cast<const unsigned *>(raw + kScales + (raw_r * 2 + raw_c / 8) * 4);
+    x.scale = scales >> (raw_c % 8 / 2 * 8) & 0xffu;
+  };
+  auto convert = [&](Numbers &x) {
+    const float by = rows::power(x.scale), less = -128.f * by;
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       float v[8];
-      rows::unpack(v, rows::Bytes{bytes[2 * i], bytes[2 * i + 1]}, scale);
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        v[j] = fmaf(float(x.bytes[2 * i + j / 4] >> (j % 4 * 8) & 0xffu), by, less);
+      // (64 2^10 stands for the largest numbers of fp16, and is none)
       if constexpr (__is_same(T, _Float16))
 #pragma unroll
-        for (int j = 0; j < 8; ++j)  // (64 2^10 stands for the largest numbers, and is none)
-          if (fabsf(v[j]) > 65504.f) v[j] = copysignf(65504.f, v[j]);
-      rows::Words<T> words;
-      words.set(v);
-      *reinterpret_cast<rows::Words<T> *>(
-          to + ((2 * raw_c + i) ^ attention::swizzle<T, 128>(raw_r)) * 16) = words;
+        for (int j = 0; j < 8; ++j) v[j] = __builtin_amdgcn_fmed3f(v[j], -65504.f, 65504.f);
+      x.words[i].set(v);
     }
   };
+  auto mend = [&](Numbers &x) {
+    auto zero = [](unsigned b) { return (b - 0x01010101u) & ~b & 0x80808080u; };
+    if ((zero(x.bytes[0]) | zero(x.bytes[1]) | zero(x.bytes[2]) | zero(x.bytes[3])) == 0 &&
+        x.scale < 248)
+      return;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      float v[8];
+      rows::unpack(v, rows::Bytes{x.bytes[2 * i], x.bytes[2 * i + 1]}, x.scale);
+      if constexpr (__is_same(T, _Float16))
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          if (fabsf(v[j]) > 65504.f) v[j] = copysignf(65504.f, v[j]);
+      x.words[i].set(v);
+    }
+  };
+  auto put = [&](int step, const Numbers &x) {
+    char *to = x_lds + step % 2 * kTile + raw_c / 8 * kHalf + raw_r * 256;
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      *reinterpret_cast<rows::Words<T> *>(
+          to + ((2 * (raw_c % 8) + i) ^ attention::swizzle<T, 128>(raw_r)) * 16) = x.words[i];
+  };
 
-  const int wn = wave / 2, wk = wave % 2;
+  const int wn = wave / 4, wk = wave % 4;
   attention::f32x16 acc[4][2] = {};
+  Numbers x;
   load(0);
   if (steps > 1) load(1);
+  if (steps > 2) load(2);
   attention::wait_loads<0>();
-  convert(0);
+  fetch(0, x);
+  convert(x);
+  mend(x);
+  put(0, x);
   attention::tile_barrier();
   for (int step = 0; step < steps; ++step) {
-    if (step + 2 < steps) load(step + 2);
-    attention::Columns<T, 128> a;
-    attention::Piece<T> b;
-    a.read(lds + step % 3 * 2 * kHalfTile + wn * kHalfTile, 0);
-    attention::read_column_piece<T, 128>(b, x_lds + step % 2 * kHalfTile, 0, 2 * wk, lane);
-    attention::pin_reads();
+    // there: both tiles of this step, this wave's bytes of the next
+    if (step + 3 < steps) load(step + 3);
+    attention::Piece<T> b, a0, a1;
+    attention::read_column_piece<T, 128>(b, x_lds + step % 2 * kTile + wk / 2 * kHalf, 0,
+                                         2 * (wk % 2), lane);
+    const char *dy_tile = lds + step % 4 * kTile + wn * kHalf;
+    attention::read_column_piece<T, 128>(a0, dy_tile, 0, 0, lane);
+    attention::read_column_piece<T, 128>(a1, dy_tile, 0, 2, lane);
+    fetch(step + 1, x);  // (behind the last step: what is there, which nothing reads)
+    __builtin_amdgcn_sched_barrier(0);
+    convert(x);
 #pragma unroll
     for (int j = 0; j < 2; ++j)
 #pragma unroll
       for (int p = 0; p < 4; ++p)
 #pragma unroll
         for (int q = 0; q < 2; ++q)
-          acc[p][q] = attention::Mat<T>::mma(a.f[p][j], b[2 * q + j], acc[p][q]);
+          acc[p][q] = attention::Mat<T>::mma(p < 2 ? a0[2 * p + j] : a1[2 * p - 4 + j],
+                                             b[2 * q + j], acc[p][q]);
+    // a few of the conversion's instructions behind each product
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+      __builtin_amdgcn_sched_group_barrier(0x002, 5, 0);
+    }
+    __builtin_amdgcn_sched_barrier(0);
     if (step + 1 < steps) {
-      // the next step's loads have arrived: all but the six behind them (the
-      // last step's may be fewer)
-      if (step + 2 < steps - 1)
-        attention::wait_loads<6>();
+      mend(x);
+      put(step + 1, x);
+      // the loads of the step behind it have arrived: all but those of the third
+      // (the last step's may be fewer)
+      if (step + 3 < steps - 1)
+        attention::wait_loads<4>();
       else
         attention::wait_loads<0>();
-      convert(step + 1);
     }
     attention::tile_barrier();  // tiles of the next step are there, this one's have been read
   }
@@ -236,14 +288,14 @@ struct Split {
   int parts, n_tiles, k_tiles;
 };
 
-// Parts of the tokens: two blocks a CU together, each of eight steps at least.
+// Parts of the tokens: one block a CU together, each of eight steps at least.
 Split split_for(int64_t tokens, int n, int k) {
   Split s;
-  s.n_tiles = (n + kN - 1) / kN;
-  s.k_tiles = (k + kK - 1) / kK;
+  s.n_tiles = (n + kSide - 1) / kSide;
+  s.k_tiles = (k + kSide - 1) / kSide;
   const int64_t tiles = int64_t(s.n_tiles) * s.k_tiles;
   const int64_t steps = (tokens + kTokens - 1) / kTokens;
-  int64_t parts = 512 / tiles;
+  int64_t parts = 256 / tiles;
   if (parts > steps / 8) parts = steps / 8;
   if (parts < 1) parts = 1;
   const int64_t each = (steps + parts - 1) / parts;
@@ -257,12 +309,12 @@ int launch(const GradArgs &A, T *dweight, hipStream_t s) {
   const int64_t total = int64_t(A.n_tiles) * A.k_tiles * A.n_parts;
   const int64_t grid = (total + 7) / 8 * 8, values = int64_t(A.n) * A.k;
   const int64_t join = (values / rows::kChunk + kThreads - 1) / kThreads;
-  int st = check_grid(grid, kThreads, "weight_grad");
+  int st = check_grid(grid, kGradThreads, "weight_grad");
   if (!st) st = check_grid(join, kThreads, "weight_grad");
   if (st) return st;
   {
     LaunchScope scope("weight_grad", s);
-    hipLaunchKernelGGL((weight_grad_kernel<T>), dim3(unsigned(grid)), dim3(kThreads), kLds, s, A);
+    hipLaunchKernelGGL((weight_grad_kernel<T>), dim3(unsigned(grid)), dim3(kGradThreads), kLds, s, A);
     st = check_launch("weight_grad");
     if (st) return st;
   }

@@ -362,17 +362,57 @@ def test_a_second_derivative_is_refused(pkg, cuda):
 
 
 @pytest.mark.gpu
+def test_more_than_2_31_values(pkg, cuda):
+    """Offsets past 32 bits: the last rows are those of a call of their own."""
+    rows, width = 270_000, 8192  # 2.2 G values
+    x = torch.empty((rows, width), device=cuda, dtype=torch.bfloat16)
+    x[:] = torch.randn(width, device=cuda).bfloat16()
+    x[-3:] = torch.randn((3, width), device=cuda).bfloat16()
+    w = torch.ones(width, device=cuda, dtype=torch.bfloat16)
+    total, normed = pkg.residual_norm(x, x, update_weight=w, weight=w)
+    small = pkg.residual_norm(x[-3:], x[-3:], update_weight=w, weight=w)
+    assert torch.equal(total[-3:], small[0]) and torch.equal(normed[-3:], small[1])
+    del total, normed
+    assert torch.equal(pkg.gated_activation(x)[-3:], pkg.gated_activation(x[-3:]))
+    packed = pkg.pack_activations(x)
+    assert torch.equal(packed.unpack()[-3:], pkg.pack_activations(x[-3:]).unpack())
+    del packed
+    leaf = x.requires_grad_(True)
+    dy = torch.ones((rows, width // 2), device=cuda, dtype=torch.bfloat16)
+    d, = torch.autograd.grad(pkg.gated_activation(leaf, checkpoint=8), leaf, dy)
+    tail = x.detach()[-3:].clone().requires_grad_(True)
+    e, = torch.autograd.grad(pkg.gated_activation(tail, checkpoint=8), tail, dy[-3:])
+    assert torch.equal(d[-3:], e)
+    del d, dy
+    dy = torch.ones((rows, width), device=cuda, dtype=torch.bfloat16)
+    d, = torch.autograd.grad(pkg.residual_norm(leaf, leaf, weight=w, checkpoint=8), leaf, (dy, dy))
+    e, = torch.autograd.grad(pkg.residual_norm(tail, tail, weight=w, checkpoint=8), tail,
+                             (dy[-3:], dy[-3:]))
+    assert torch.equal(d[-3:], e)
+    del d, dy, leaf, x
+    x = torch.randn((70_000, 96), device=cuda).bfloat16()
+    codes, scales = pkg.quantize_weight(torch.randn((40_000, 96), device=cuda))
+    with torch.no_grad():
+        y = pkg.linear_int8(x, codes, scales)
+        assert torch.equal(y[-300:], pkg.linear_int8(x[-300:], codes, scales))
+
+
+@pytest.mark.gpu
 def test_what_is_kept(pkg, cuda):
     """A checkpoint is what the backward pass holds on to: 33 bytes for 32
     values, and the operands themselves are free."""
     x = torch.randn(4096, 1280, device=cuda, dtype=torch.bfloat16)
     held = {}
+
+    def requested():  # (allocated blocks may be larger)
+        return torch.cuda.memory_stats()['requested_bytes.all.current']
+
     for checkpoint in (None, 8):
         leaf = x.clone().requires_grad_(True)
         torch.cuda.synchronize()
-        before = torch.cuda.memory_allocated()
+        before = requested()
         out = pkg.gated_activation(leaf * 1.0, 'silu', checkpoint=checkpoint)
-        held[checkpoint] = torch.cuda.memory_allocated() - before - out.numel() * 2
+        held[checkpoint] = requested() - before - out.numel() * 2
         del out
     assert held[None] == 4096 * 1280 * 2
     assert held[8] == 4096 * 2 * 672  # (rows of 640 codes and 20 scales, at 16 bytes)
