@@ -157,7 +157,7 @@ struct ProductArgs {
   int64_t w_row;
   int x_pitch, w_chunks;  // 16-byte chunks of a row of w that are there
   int tokens, channels;
-  int steps;              // of kStep bytes
+  int steps;              // of 64 bytes
   int x_tiles, w_tiles;
 };
 
@@ -167,11 +167,13 @@ struct __attribute__((packed, aligned(sizeof(T)))) Four {
   T v[4];
 };
 
-// Rows of kStep bytes in LDS, 4 chunks of 16: chunk c of row r lies at c ^
-// (r / 4) % 4, so the 16 rows of which a fragment read takes one chunk each
-// use all of the 256 bytes that LDS gives a cycle.
-constexpr int kStep = 64;  // bytes of a row that a tile holds
-__device__ __forceinline__ int place(int r, int c) { return c ^ ((r >> 2) & 3); }
+// Rows of 64 or 128 bytes in LDS, kChunks of 16: chunk c of row r lies at c ^
+// (r / 4) % 4, or c ^ (r / 2) % 8, so the 16 rows of which a fragment read takes
+// one chunk each use all of the 256 bytes that LDS gives a cycle.
+template <int kChunks>
+__device__ __forceinline__ int place(int r, int c) {
+  return kChunks == 4 ? c ^ ((r >> 2) & 3) : c ^ ((r >> 1) & 7);
+}
 
 // Blocks of one XCD (every eighth) take tiles that lie together: eight tiles of
 // channels by as many of tokens as run at once share what their L2 holds.
@@ -197,40 +199,52 @@ __device__ __forceinline__ void wait_steps(int left) {
 
 // One block: kX tokens by kW channels, kWavesX x kWavesW waves of 32 kTx x 32 kTw.  Channels
 // are the rows of the matrix instruction's result, tokens its columns: a lane
-// holds one token's channels, four neighbours a register group.
-template <typename T, int kTx, int kTw, int kWavesX, int kWavesW, int kBuffers>
-__global__ __launch_bounds__(64 * kWavesX * kWavesW, 2) void product_kernel(ProductArgs A) {
-  constexpr int kThreads = 64 * kWavesX * kWavesW;
+// holds one token's channels, four neighbours a register group.  kGroups such
+// groups of waves take equal parts of the rows' length, each with tiles of its
+// own, and the first adds their sums.
+template <typename T, int kTx, int kTw, int kWavesX, int kWavesW, int kStep, int kBuffers,
+          int kGroups>
+__global__ __launch_bounds__(64 * kWavesX * kWavesW * kGroups, kGroups > 2 ? kGroups : 2)
+void product_kernel(ProductArgs A) {
+  constexpr int kThreads = 64 * kWavesX * kWavesW;  // of a group
   constexpr int kX = 32 * kTx * kWavesX, kW = 32 * kTw * kWavesW;
-  constexpr int kLoadsX = kX * 4 / kThreads, kLoadsW = kW * 4 / kThreads;
+  constexpr int kChunks = kStep / 16;
+  constexpr int kLoadsX = kX * kChunks / kThreads, kLoadsW = kW * kChunks / kThreads;
   constexpr int kTileX = kX * kStep, kTile = (kX + kW) * kStep;
-  static_assert(kX * 4 % kThreads == 0 && kW * 4 % kThreads == 0, "whole rounds of loads");
+  static_assert(kX * kChunks % kThreads == 0 && kW * kChunks % kThreads == 0, "whole rounds");
   extern __shared__ __align__(16) char lds[];
-  float *scales = reinterpret_cast<float *>(lds + kBuffers * kTile), *biases = scales + kW;
+  float *scales = reinterpret_cast<float *>(lds + kGroups * kBuffers * kTile);
+  float *biases = scales + kW;
   int x_tile, w_tile;
   if (!tile_of(A, x_tile, w_tile)) return;
-  const int lane = attention::lane_id(), wave = attention::wave_id();
+  const int lane = attention::lane_id(), group = attention::wave_id() / (kThreads / 64);
+  const int wave = attention::wave_id() % (kThreads / 64), thread = int(threadIdx.x) % kThreads;
   const int x0 = x_tile * kX, w0 = w_tile * kW;
-  for (int i = threadIdx.x; i < kW; i += kThreads) {
+  for (int i = threadIdx.x; i < kW; i += kThreads * kGroups) {
     const bool on = w0 + i < A.channels;
     scales[i] = on ? A.w_scale[w0 + i] : 0.f;
     biases[i] = on && A.bias ? float(static_cast<const T *>(A.bias)[w0 + i]) : 0.f;
   }
-  const unsigned lds0 = attention::lds_address(lds);
+  const unsigned lds0 = attention::lds_address(lds) + group * kBuffers * kTile;
+  char *const tiles = lds + group * kBuffers * kTile;
+  // this group's steps
+  const int all = A.x_pitch / kStep, most = (all + kGroups - 1) / kGroups, first = group * most;
+  const int steps = min(most, all - first);
   // this lane's pieces of the tiles: offsets from a step's first byte
-  const char *x_at = reinterpret_cast<const char *>(A.x) + int64_t(x0) * A.x_pitch;
+  const char *x_at =
+      reinterpret_cast<const char *>(A.x) + int64_t(x0) * A.x_pitch + int64_t(first) * kStep;
   const char *w_at = reinterpret_cast<const char *>(A.w) + w0 * A.w_row;
   unsigned x_off[kLoadsX], w_off[kLoadsW];
   int w_chunk[kLoadsW];
 #pragma unroll
   for (int i = 0; i < kLoadsX; ++i) {
-    const int slot = i * kThreads + int(threadIdx.x), r = slot / 4, c = place(r, slot % 4);
+    const int slot = i * kThreads + thread, r = slot / kChunks, c = place<kChunks>(r, slot % kChunks);
     x_off[i] = unsigned(min(r, A.tokens - 1 - x0) * A.x_pitch + c * 16);
   }
 #pragma unroll
   for (int i = 0; i < kLoadsW; ++i) {
-    const int slot = i * kThreads + int(threadIdx.x), r = slot / 4;
-    w_chunk[i] = place(r, slot % 4);
+    const int slot = i * kThreads + thread, r = slot / kChunks;
+    w_chunk[i] = first * kChunks + place<kChunks>(r, slot % kChunks);
     w_off[i] = unsigned(min(r, A.channels - 1 - w0) * int(A.w_row));
   }
   auto load = [&](int step, int buffer) {
@@ -242,7 +256,7 @@ __global__ __launch_bounds__(64 * kWavesX * kWavesW, 2) void product_kernel(Prod
 #pragma unroll
     for (int i = 0; i < kLoadsW; ++i) {
       // (past a row's end: its last chunk once more, which meets zeros)
-      const int c = min(step * 4 + w_chunk[i], A.w_chunks - 1);
+      const int c = min(step * kChunks + w_chunk[i], A.w_chunks - 1);
       attention::load_to_lds(w_at, w_off[i] + c * 16, to + kTileX + i * kThreads * 16);
     }
   };
@@ -253,14 +267,15 @@ __global__ __launch_bounds__(64 * kWavesX * kWavesW, 2) void product_kernel(Prod
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
 #pragma unroll
   for (int i = 0; i < kBuffers - 1; ++i)
-    if (i < A.steps) load(i, i);
+    if (i < steps) load(i, i);
   int buffer = 0;
-  for (int step = 0; step < A.steps; ++step) {
-    wait_steps<kLoadsX + kLoadsW, kBuffers - 2>(A.steps - 1 - step);
+  for (int step = 0; step < most; ++step) {  // (as many barriers for every group)
+    wait_steps<kLoadsX + kLoadsW, kBuffers - 2>(steps - 1 - step);
     attention::tile_barrier();  // this step's tiles are there, and the last one's have been read
-    if (step + kBuffers - 1 < A.steps)
+    if (kGroups > 1 && step >= steps) continue;
+    if (step + kBuffers - 1 < steps)
       load(step + kBuffers - 1, buffer == 0 ? kBuffers - 1 : buffer - 1);
-    const char *x_tile = lds + buffer * kTile, *w_tile = x_tile + kTileX;
+    const char *x_tile = tiles + buffer * kTile, *w_tile = x_tile + kTileX;
     buffer = buffer == kBuffers - 1 ? 0 : buffer + 1;
 #pragma unroll
     for (int s = 0; s < kStep / 32; ++s) {
@@ -268,16 +283,35 @@ __global__ __launch_bounds__(64 * kWavesX * kWavesW, 2) void product_kernel(Prod
 #pragma unroll
       for (int i = 0; i < kTx; ++i)
         x[i] = *reinterpret_cast<const i32x4 *>(x_tile + (wx + 32 * i + c) * kStep +
-                                                place(c, 2 * s + h) * 16);
+                                                place<kChunks>(c, 2 * s + h) * 16);
 #pragma unroll
       for (int i = 0; i < kTw; ++i)
         w[i] = *reinterpret_cast<const i32x4 *>(w_tile + (ww + 32 * i + c) * kStep +
-                                                place(c, 2 * s + h) * 16);
+                                                place<kChunks>(c, 2 * s + h) * 16);
 #pragma unroll
       for (int i = 0; i < kTw; ++i)
 #pragma unroll
         for (int j = 0; j < kTx; ++j)
           acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(w[i], x[j], acc[i][j], 0, 0, 0);
+    }
+  }
+  if constexpr (kGroups > 1) {
+    // the groups' sums, each in the place of tiles of its own (all read by now)
+    static_assert(kBuffers * kTile >= kX * kW * 4, "a group's sums fit its tiles");
+    __syncthreads();
+    if (group > 0) {
+      int *to = reinterpret_cast<int *>(tiles) + wave * (kTw * kTx * 1024) + lane;
+#pragma unroll
+      for (int i = 0; i < kTw * kTx * 16; ++i) to[i * 64] = acc[i / 16 / kTx][i / 16 % kTx][i % 16];
+    }
+    __syncthreads();
+    if (group > 0) return;
+#pragma unroll
+    for (int g = 1; g < kGroups; ++g) {
+      const int *from = reinterpret_cast<const int *>(lds + g * kBuffers * kTile) +
+                        wave * (kTw * kTx * 1024) + lane;
+#pragma unroll
+      for (int i = 0; i < kTw * kTx * 16; ++i) acc[i / 16 / kTx][i / 16 % kTx][i % 16] += from[i * 64];
     }
   }
 #pragma unroll
@@ -449,17 +483,18 @@ int codes_for(const void *x, int64_t x_row, int dtype, int64_t n, int width, int
   return check_launch("linear8_codes");
 }
 
-template <typename T, int kTx, int kTw, int kWavesX, int kWavesW, int kBuffers>
+template <typename T, int kTx, int kTw, int kWavesX, int kWavesW, int kStep, int kBuffers,
+          int kGroups = 1>
 int launch_tiles(ProductArgs &A, hipStream_t s) {
-  constexpr int kThreads = 64 * kWavesX * kWavesW, kX = 32 * kTx * kWavesX, kW = 32 * kTw * kWavesW;
+  constexpr int kThreads = 64 * kWavesX * kWavesW * kGroups, kX = 32 * kTx * kWavesX, kW = 32 * kTw * kWavesW;
   A.x_tiles = (A.tokens + kX - 1) / kX;
   A.w_tiles = (A.channels + kW - 1) / kW;
   const int64_t blocks = (int64_t(A.x_tiles) * A.w_tiles + 7) / 8 * 8;
   const int st = check_grid(blocks, kThreads, "linear8");
   if (st) return st;
-  hipLaunchKernelGGL((product_kernel<T, kTx, kTw, kWavesX, kWavesW, kBuffers>),
+  hipLaunchKernelGGL((product_kernel<T, kTx, kTw, kWavesX, kWavesW, kStep, kBuffers, kGroups>),
                      dim3(unsigned(blocks)), dim3(kThreads),
-                     kBuffers * (kX + kW) * kStep + 2 * kW * sizeof(float), s, A);
+                     kGroups * kBuffers * (kX + kW) * kStep + 2 * kW * sizeof(float), s, A);
   return check_launch("linear8");
 }
 
@@ -470,41 +505,42 @@ int launch_few(const ProductArgs &A, hipStream_t s) {
   return check_launch("linear8");
 }
 
-template <typename T, int kTw>
-int launch_few_tokens(const ProductArgs &A, hipStream_t s) {
-  if (A.tokens <= 16) return launch_few<T, 1, kTw>(A, s);
-  if (A.tokens <= 32) return launch_few<T, 2, kTw>(A, s);
-  return launch_few<T, 4, kTw>(A, s);
-}
-
 template <typename T>
 int launch_product(ProductArgs &A, hipStream_t s) {
-  // Up to 64 tokens the weights' way to the registers is the time.  32 channels
+  // Up to 32 tokens the weights' way to the registers is the time.  32 channels
   // a block read the tokens half as often as 16, but need enough channels for
   // the card's CUs: us by 16 and by 32, 16 x 4096 x 6144 12.4 and 10.9, 32 x
-  // 8192 x 8192 32.1 and 24.7; 48 x 4096 x 4096 13.4 and 14.5, 64 x 1280 x 1280
-  // 7.5 and 8.7.
-  if (A.tokens <= 64)
-    return A.channels >= 32 * 160 ? launch_few_tokens<T, 2>(A, s) : launch_few_tokens<T, 1>(A, s);
+  // 8192 x 8192 32.1 and 24.7; 8 x 1280 x 10240 7.7 and 8.1, 32 x 1280 x 1280 6.2
+  // and 7.1.
+  if (A.tokens <= 32) {
+    const bool wide = A.channels >= 32 * 160;
+    if (A.tokens <= 16) return wide ? launch_few<T, 1, 2>(A, s) : launch_few<T, 1, 1>(A, s);
+    return wide ? launch_few<T, 2, 2>(A, s) : launch_few<T, 2, 1>(A, s);
+  }
   auto tiles = [&](int x, int w) {
     return int64_t((A.tokens + x - 1) / x) * ((A.channels + w - 1) / w);
   };
+  // Small tiles where few of larger ones would leave CUs idle, and while there
+  // are no more than CUs the rows' length in two parts: us by 64 x 64 in two
+  // parts, 64 x 64 and 64 x 128, 67 x 5000 x 4099 14.0, 17.1 and 22.1, 200 x 4096
+  // x 4096 12.8, 15.0 and 18.5; 512 x 4096 x 4096 21.6, 18.7 and 20.3, 1024 x 1280
+  // x 1280 12.1, 9.2 and 10.8; 800 x 4096 x 4096 37.4, 30.3 and 24.0.
+  const int64_t small = tiles(64, 64);
+  if (small <= 256) return launch_tiles<T, 1, 1, 2, 2, 128, 4, 2>(A, s);
+  if (small <= 512) return launch_tiles<T, 1, 1, 2, 2, 128, 4>(A, s);
   // Tiles of 256 x 256, one a CU, read each operand least often: a round of 256
-  // takes 0.88 of the time of 512 of 128 x 256, two a CU (8192 x 8192 x 8192 519
+  // takes 0.83 of the time of 512 of 128 x 256, two a CU (8192 x 8192 x 8192 487
   // and 590 us), but a last round of up to 256 of these, one a CU, 0.6 of it.  So
-  // us by 256 x 256 and 128 x 256: 16896 x 1280 x 10240 323 and 336, 1500 x 1280 x
-  // 10240 29 and 33; 16896 x 5120 x 1280 148 and 143, 1024 x 4096 x 8192 60 and 48.
+  // us by 256 x 256 and 128 x 256: 16896 x 1280 x 10240 304 and 336, 1500 x 1280 x
+  // 10240 29 and 33; 16896 x 5120 x 1280 148 and 139, 1024 x 4096 x 8192 57 and 48.
   const int64_t wide = tiles(256, 256), half = tiles(128, 256), rest = half % 512;
   if (wide >= 128 &&
-      (wide + 255) / 256 * 88 < half / 512 * 100 + (rest > 256 ? 100 : rest > 0 ? 60 : 0))
-    return launch_tiles<T, 4, 2, 2, 4, 4>(A, s);
-  // From one for each CU on 128 x 256 (us of these and of 64 x 128: 1024 x 4096 x
-  // 8192 50 and 67; 800 x 4096 x 4096 42 and 31), else 64 x 128, or 64 x 64 where
-  // that is not two for each (64 x 128 and 64 x 64: 800 x 4096 x 4096 31 and 38,
-  // 512 x 4096 x 4096 24 and 23, 100 x 4096 x 6144 22 and 19).
-  if (half >= 256) return launch_tiles<T, 2, 4, 2, 2, 3>(A, s);
-  if (tiles(64, 64) > 512) return launch_tiles<T, 1, 2, 2, 2, 6>(A, s);
-  return launch_tiles<T, 1, 1, 2, 2, 8>(A, s);
+      (wide + 255) / 256 * 83 < half / 512 * 100 + (rest > 256 ? 100 : rest > 0 ? 60 : 0))
+    return launch_tiles<T, 4, 2, 2, 4, 128, 2>(A, s);
+  // 128 x 256 from one for each CU on (us of these and of 64 x 128: 1024 x 4096 x
+  // 8192 48 and 53; 800 x 4096 x 4096 42 and 24).
+  if (half >= 256) return launch_tiles<T, 2, 4, 2, 2, 64, 3>(A, s);
+  return launch_tiles<T, 1, 2, 2, 2, 128, 3>(A, s);
 }
 
 int check_sizes(int dtype, int64_t tokens, int64_t width, int64_t channels) {
@@ -574,7 +610,7 @@ int bevpool_linear8(const void *x, int64_t x_row, int32_t dtype, const void *wei
   A.w_chunks = (width + 15) / 16;
   A.tokens = int(tokens);
   A.channels = int(channels);
-  A.steps = pitch / kStep;
+  A.steps = pitch / 64;
   LaunchScope scope("linear8", s);
   if (dtype == BEVPOOL_F32) return launch_product<float>(A, s);
   if (dtype == BEVPOOL_F16) return launch_product<_Float16>(A, s);

@@ -53,7 +53,9 @@ def test_channels(pkg, cuda, out, tokens):
         check(pkg, cuda, *make(tokens, 160, out, dtype, out, bias=out % 2 == 1))
 
 
-@pytest.mark.parametrize('tokens,width,out', [(1000, 700, 2100), (2049, 256, 1025), (4100, 130, 600)])
+@pytest.mark.parametrize('tokens,width,out', [
+    (1000, 700, 2100), (2049, 256, 1025), (4100, 130, 600), (512, 300, 3001), (2000, 140, 8003),
+    (4100, 130, 2100)])
 def test_large(pkg, cuda, tokens, width, out):
     """More tiles than the card has CUs, and ends of tiles both ways."""
     check(pkg, cuda, *make(tokens, width, out, torch.bfloat16, 1))
