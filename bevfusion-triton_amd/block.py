@@ -535,7 +535,9 @@ class Int8Linear(nn.Module):
         super().__init__()
         self.in_features, self.out_features = linear.in_features, linear.out_features
         codes, scales = quantize_weight(linear.weight)
-        self.register_buffer('codes', codes)
+        # (whole rows, which stay where they begin when the module is moved)
+        self.register_buffer('codes', codes.as_strided((codes.shape[0], codes.stride(0)),
+                                                       codes.stride()))
         self.register_buffer('scales', scales)
         self.register_buffer('bias', None if linear.bias is None else linear.bias.detach().clone())
 
@@ -550,4 +552,4 @@ class Int8Linear(nn.Module):
         if torch.is_autocast_enabled('cuda'):
             x = x.to(torch.get_autocast_dtype('cuda'))
         bias = self.bias if self.bias is None else self.bias.to(x.dtype)
-        return linear_int8(x, self.codes, self.scales, bias)
+        return linear_int8(x, self.codes[:, :self.in_features], self.scales, bias)

@@ -377,14 +377,14 @@ __global__ __launch_bounds__(64 * kFewWaves, kTx * kTw > 4 ? 2 : 4) void few_ker
   constexpr int kDeep = 4;  // steps whose loads are on their way together
   const int lane = attention::lane_id(), wave = attention::wave_id();
   const int c = lane & 15, q = lane >> 4;
-  const int w0 = int(blockIdx.x) * 16 * kTw, x0 = int(blockIdx.y) * 16 * kTx;
+  const int w0 = int(blockIdx.x) * 16 * kTw;
   const int8_t *w_at[kTw], *x_at[kTx];
 #pragma unroll
   for (int i = 0; i < kTw; ++i)
     w_at[i] = A.w + int64_t(min(w0 + 16 * i + c, A.channels - 1)) * A.w_row;
 #pragma unroll
   for (int i = 0; i < kTx; ++i)
-    x_at[i] = A.x + int64_t(min(x0 + 16 * i + c, A.tokens - 1)) * A.x_pitch;
+    x_at[i] = A.x + int64_t(min(16 * i + c, A.tokens - 1)) * A.x_pitch;
   i32x4 acc[kTw][kTx] = {};
   for (int first = wave; first < A.steps; first += kFewWaves * kDeep) {
     i32x4 w[kDeep][kTw], x[kDeep][kTx];
@@ -423,7 +423,7 @@ __global__ __launch_bounds__(64 * kFewWaves, kTx * kTw > 4 ? 2 : 4) void few_ker
 #pragma unroll
     for (int i = 1; i < kFewWaves; ++i) sum += sums[i][t][lane];
     // lane 16 q + c: channels 4 q .. + 3 of token c
-    const int token = x0 + t % kTx * 16 + c, n = w0 + t / kTx * 16 + 4 * q;
+    const int token = t % kTx * 16 + c, n = w0 + t / kTx * 16 + 4 * q;
     if (token >= A.tokens) continue;
     const float by = A.x_scale[token];
     T *y = static_cast<T *>(A.y) + int64_t(token) * A.channels + n;
@@ -471,6 +471,9 @@ void launch_codes(const void *x, int64_t x_row, int64_t n, int width, int pitch,
 
 int codes_for(const void *x, int64_t x_row, int dtype, int64_t n, int width, int pitch, void *codes,
               void *scales, hipStream_t s) {
+  // (a block takes four rows at most, and one at least)
+  const int st = check_grid(pitch > 2048 ? n : (n + 3) / 4, 256, "linear8 codes");
+  if (st) return st;
   LaunchScope scope("linear8_codes", s);
   int8_t *to = static_cast<int8_t *>(codes);
   float *scale = static_cast<float *>(scales);
@@ -500,8 +503,10 @@ int launch_tiles(ProductArgs &A, hipStream_t s) {
 
 template <typename T, int kTx, int kTw>
 int launch_few(const ProductArgs &A, hipStream_t s) {
-  const dim3 grid((A.channels + 16 * kTw - 1) / (16 * kTw), (A.tokens + 16 * kTx - 1) / (16 * kTx));
-  hipLaunchKernelGGL((few_kernel<T, kTx, kTw>), grid, dim3(64 * kFewWaves), 0, s, A);
+  const int blocks = (A.channels + 16 * kTw - 1) / (16 * kTw);
+  const int st = check_grid(blocks, 64 * kFewWaves, "linear8");
+  if (st) return st;
+  hipLaunchKernelGGL((few_kernel<T, kTx, kTw>), dim3(blocks), dim3(64 * kFewWaves), 0, s, A);
   return check_launch("linear8");
 }
 
@@ -592,6 +597,10 @@ int bevpool_linear8(const void *x, int64_t x_row, int32_t dtype, const void *wei
   if (!scratch || scratch_bytes < bevpool_linear8_scratch_bytes(tokens, width) ||
       reinterpret_cast<uintptr_t>(scratch) % 16)
     return fail(BEVPOOL_ESPACE, "linear8 scratch too small, or not at a multiple of 16 bytes");
+  // (before anything is launched: the blocks of any plan of launch_product)
+  st = tokens <= 32 ? check_grid((channels + 15) / 16, 64 * kFewWaves, "linear8")
+                    : check_grid(((tokens + 255) / 256) * ((channels + 255) / 256), 512, "linear8");
+  if (st) return st;
   hipStream_t s = static_cast<hipStream_t>(stream);
   const int pitch = int(code_pitch(width));
   int8_t *codes = static_cast<int8_t *>(scratch);

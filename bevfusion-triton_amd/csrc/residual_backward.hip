@@ -254,56 +254,60 @@ __device__ __forceinline__ float column_sum(const float *from, int64_t n, int wi
   return slices_sum(s, lds);
 }
 
-// The gradient of a gate that rows share; with several items a row of gate
-// their sum is left in the first's place.
+// The gradients that are sums over rows, from the items' and the blocks' sums:
+// grid.y 0 those of the update's weight and of the scale, 1 that of the norm's
+// weight, from 2 on that of a gate that rows share, by its rows.
 template <typename T>
-__global__ __launch_bounds__(kSumThreads) void gate_sum_kernel(Args A, T *dgate) {
+__global__ __launch_bounds__(kSumThreads) void sums_kernel(Args A, int64_t weight_blocks, T *dgate,
+                                                           T *dupdate_weight, T *dscale,
+                                                           T *dweight) {
   __shared__ float lds[kSumThreads];
   const int c = blockIdx.x * kSumColumns + int(threadIdx.x) % kSumColumns;
-  for (int64_t owner = blockIdx.y; owner < A.items / A.parts_each; owner += gridDim.y) {
-    float *parts = A.parts + owner * A.parts_each * A.width;
-    const float s = column_sum(parts, A.parts_each, A.width, c, lds);
-    if (threadIdx.x >= kSumColumns || c >= A.width) continue;
-    const float w = A.update_weight ? float(static_cast<const T *>(A.update_weight)[c]) : 1.f;
-    const float scale = A.scale ? float(static_cast<const T *>(A.scale)[c]) : 1.f;
-    dgate[owner * A.width + c] = T(s * w * scale);
-    parts[c] = s;
-  }
-}
-
-// Gradients of the weights and the scale: grid.y 0 those of the update's, 1
-// that of the norm's.
-template <typename T>
-__global__ __launch_bounds__(kSumThreads) void weight_sums_kernel(Args A, int64_t weight_blocks,
-                                                                  T *dupdate_weight, T *dscale,
-                                                                  T *dweight) {
-  __shared__ float lds[kSumThreads];
-  const int c = blockIdx.x * kSumColumns + int(threadIdx.x) % kSumColumns;
+  const bool writes = threadIdx.x < kSumColumns && c < A.width;
   if (blockIdx.y == 1) {
     if (!dweight) return;
     const float s = column_sum(A.weight_parts, weight_blocks, A.width, c, lds);
-    if (threadIdx.x < kSumColumns && c < A.width) dweight[c] = T(s);
+    if (writes) dweight[c] = T(s);
     return;
   }
-  if (!dupdate_weight && !dscale) return;
-  float s = 0.f;
-  if (A.gate && A.gate_each > 1) {  // (each row of gate's own sum: gate_sum_kernel)
-    if (c < A.width) {
-      const T *gate = static_cast<const T *>(A.gate);
+  if (blockIdx.y == 0 && !dupdate_weight && !dscale) return;
+  float w = 1.f, scale = 1.f;
+  if (c < A.width && A.update_weight) w = float(static_cast<const T *>(A.update_weight)[c]);
+  if (c < A.width && A.scale) scale = float(static_cast<const T *>(A.scale)[c]);
+  if (blockIdx.y == 0) {
+    float s = 0.f;
+    if (A.gate && A.gate_each > 1) {  // (the items' sums are without the gate)
+      if (c < A.width) {
+        const T *gate = static_cast<const T *>(A.gate) + c;
+        const float *parts = A.parts + c;
+        const int slice = threadIdx.x / kSumColumns;
+        if (A.parts_each >= kSlices) {
+          for (int64_t owner = 0; owner < A.items / A.parts_each; ++owner) {
+            float t = 0.f;
+#pragma unroll 8
+            for (int64_t i = slice; i < A.parts_each; i += kSlices)
+              t += parts[(owner * A.parts_each + i) * A.width];
+            s += t * float(gate[owner * A.gate_row]);
+          }
+        } else {
 #pragma unroll 4
-      for (int64_t i = threadIdx.x / kSumColumns; i < A.items / A.parts_each; i += kSlices)
-        s += A.parts[i * A.parts_each * A.width + c] * float(gate[i * A.gate_row + c]);
+          for (int64_t i = slice; i < A.items; i += kSlices)
+            s += parts[i * A.width] * float(gate[i / A.parts_each * A.gate_row]);
+        }
+      }
+      s = slices_sum(s, lds);
+    } else {
+      s = column_sum(A.parts, A.items, A.width, c, lds);
     }
-    s = slices_sum(s, lds);
-  } else {
-    s = column_sum(A.parts, A.items, A.width, c, lds);
+    if (writes && dupdate_weight) dupdate_weight[c] = T(s * scale);
+    if (writes && dscale) dscale[c] = T(s * w);
+    return;
   }
-  if (threadIdx.x >= kSumColumns || c >= A.width) return;
-  if (dupdate_weight)
-    dupdate_weight[c] = T(A.scale ? s * float(static_cast<const T *>(A.scale)[c]) : s);
-  if (dscale)
-    dscale[c] =
-        T(A.update_weight ? s * float(static_cast<const T *>(A.update_weight)[c]) : s);
+  for (int64_t owner = blockIdx.y - 2; owner < A.items / A.parts_each; owner += gridDim.y - 2) {
+    const float s =
+        column_sum(A.parts + owner * A.parts_each * A.width, A.parts_each, A.width, c, lds);
+    if (writes) dgate[owner * A.width + c] = T(s * w * scale);
+  }
 }
 
 // ---------------------------------------------------------------------------
@@ -357,15 +361,13 @@ void launch_width(const Args &A, int64_t blocks, bool kept, hipStream_t s) {
 template <typename T>
 void launch_sums(const Args &A, int64_t blocks, void *dgate, void *dupdate_weight, void *dscale,
                  void *dweight, hipStream_t s) {
-  const unsigned columns = unsigned((A.width + kSumColumns - 1) / kSumColumns);
-  const int64_t owners = A.items / A.parts_each;
-  if (A.gate && A.gate_each > 1)
-    hipLaunchKernelGGL((gate_sum_kernel<T>), dim3(columns, unsigned(owners < 4096 ? owners : 4096)),
-                       dim3(kSumThreads), 0, s, A, static_cast<T *>(dgate));
-  if (dupdate_weight || dscale || dweight)
-    hipLaunchKernelGGL((weight_sums_kernel<T>), dim3(columns, 2), dim3(kSumThreads), 0, s, A,
-                       blocks, static_cast<T *>(dupdate_weight), static_cast<T *>(dscale),
-                       static_cast<T *>(dweight));
+  const int64_t owners = A.gate && A.gate_each > 1 ? A.items / A.parts_each : 0;
+  if (!owners && !dupdate_weight && !dscale && !dweight) return;
+  const dim3 grid((A.width + kSumColumns - 1) / kSumColumns,
+                  unsigned(2 + (owners < 4096 ? owners : 4096)));
+  hipLaunchKernelGGL((sums_kernel<T>), grid, dim3(kSumThreads), 0, s, A, blocks,
+                     static_cast<T *>(dgate), static_cast<T *>(dupdate_weight),
+                     static_cast<T *>(dscale), static_cast<T *>(dweight));
 }
 
 }  // namespace residual

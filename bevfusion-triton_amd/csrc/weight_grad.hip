@@ -328,6 +328,8 @@ template <typename T>
 int launch_columns(const void *x, int64_t x_row, int64_t n_rows, int width, void *out,
                    float *scratch, hipStream_t s) {
   const dim3 grid((width + kColumns - 1) / kColumns, kColumnParts);
+  const int st = check_grid(int64_t(grid.x) * kColumnParts, kThreads, "column_sums");
+  if (st) return st;
   LaunchScope scope("column_sums", s);
   hipLaunchKernelGGL((column_sum_kernel<T, float>), grid, dim3(kThreads), 0, s,
                      static_cast<const T *>(x), x_row, n_rows, width, scratch);

@@ -124,6 +124,7 @@ def test_weight_gradient_entries(pkg):
         (dict(dtype=3), -1, b'dtype'), (dict(rows=-1), -1, b'rows'), (dict(width=0), -1, b'width'),
         (dict(x=None), -1, b'null'), (dict(out=None), -1, b'null'), (dict(scratch=None), -3, b'scratch'),
         (dict(nbytes=need - 1), -3, b'scratch')))
+    assert sums(width=1 << 27, nbytes=1 << 60) == -1 and b'grid' in lib.bevpool_last_error()
 
 
 def test_linear8_entries(pkg):
@@ -143,6 +144,10 @@ def test_linear8_entries(pkg):
         (dict(row=96), -1, b'16 bytes'), (dict(row=1 << 22), -1, b'16 bytes'),
         (dict(scratch=None), -3, b'scratch'), (dict(scratch=8), -3, b'scratch'),
         (dict(nbytes=3 * 132 - 1), -3, b'scratch')))
+    assert product(tokens=1, width=1, row=16, channels=1 << 30, nbytes=1 << 20) == -1
+    assert b'grid' in lib.bevpool_last_error()
+    assert lib.bevpool_linear8_codes(16, 1, 2, 1 << 30, 1, 16, 16, None) == -1
+    assert b'grid' in lib.bevpool_last_error()
     assert lib.bevpool_linear8_scratch_bytes(3, 100) == 3 * 132
     assert product(tokens=0, x=None) == 0 and product(channels=0, weight=None) == 0
     assert lib.bevpool_linear8_codes(16, 100, 2, 3, 100, None, 16, None) == -1
