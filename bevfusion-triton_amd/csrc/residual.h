@@ -8,8 +8,11 @@ namespace residual {
 constexpr int kMaxWidth = 8192;
 
 struct Args {
-  // inputs (null: not there)
+  // inputs.  Weights that are not there are null; rows that are not there are
+  // other rows, read all the same and not used (see the flags), so that no load
+  // is behind a condition.
   const void *x, *update, *gate, *update_weight, *scale, *weight;
+  bool has_update, has_gate, has_dsum, keeps;
   int64_t x_row, update_row, gate_row;  // strides in values
   uint8_t *x_kept, *update_kept;        // 8-bit checkpoints
   int64_t rows;
@@ -31,14 +34,15 @@ struct Args {
 // hold a row's values and several rows' loads are on their way at once (chunks
 // past 4096 values: two), by whole waves, or parts of one for short rows.
 #define RESIDUAL_LAYOUT(FN, width, ...)                                         \
-  if ((width) <= 128) FN(16, 1, __VA_ARGS__)                                    \
-  else if ((width) <= 256) FN(32, 1, __VA_ARGS__)                               \
-  else if ((width) <= 512) FN(64, 1, __VA_ARGS__)                               \
-  else if ((width) <= 1024) FN(128, 1, __VA_ARGS__)                             \
-  else if ((width) <= 1536) FN(192, 1, __VA_ARGS__)                             \
-  else if ((width) <= 2048) FN(256, 1, __VA_ARGS__)                             \
-  else if ((width) <= 4096) FN(512, 1, __VA_ARGS__)                             \
-  else FN(512, 2, __VA_ARGS__)
+  if ((width) < 8) FN(16, 1, false, __VA_ARGS__)                                \
+  else if ((width) <= 128) FN(16, 1, true, __VA_ARGS__)                         \
+  else if ((width) <= 256) FN(32, 1, true, __VA_ARGS__)                         \
+  else if ((width) <= 512) FN(64, 1, true, __VA_ARGS__)                         \
+  else if ((width) <= 1024) FN(128, 1, true, __VA_ARGS__)                       \
+  else if ((width) <= 1536) FN(192, 1, true, __VA_ARGS__)                       \
+  else if ((width) <= 2048) FN(256, 1, true, __VA_ARGS__)                       \
+  else if ((width) <= 4096) FN(512, 1, true, __VA_ARGS__)                       \
+  else FN(512, 2, true, __VA_ARGS__)
 
 // (rows of more than a wave pass barriers: a block of them has one)
 constexpr int threads_of(int lanes) { return lanes > 64 ? lanes : 256; }
@@ -56,12 +60,14 @@ constexpr int blocks_for(int lanes, int waves) {
   return 256 * (each > 1 ? each : 1);
 }
 
-// A lane's place: its row of a block's, and its chunks.  With kWhole, where the
-// width is no whole number of chunks the last one begins earlier, and shares
-// its first `skip` values with the one before: both form the same of them, and
-// only sums leave them out, so that every access is a whole one (of rows of a
-// chunk at least).  Without, its values past the row's end are zeros.
-template <int kLanes, int kChunks, bool kWhole = true>
+// A lane's place: its row of a block's, and its chunks.  With kWhole (rows of a
+// chunk at least) every lane reads and writes whole chunks, whatever the width:
+// where it is no whole number of chunks the last one begins earlier, and lanes
+// past it have the last one too.  So the first `skip` values of a chunk are
+// another lane's as well; all form the same of them, and only sums leave them
+// out.  No access is behind a condition, so the compiler can count them, and a
+// row's loads wait for no store of the row before.
+template <int kLanes, int kChunks, bool kWhole>
 struct Place {
   int lane, group, width;
   __device__ __forceinline__ explicit Place(int width) : width(width) {
@@ -70,15 +76,15 @@ struct Place {
     if constexpr (kLanes >= 64) group = __builtin_amdgcn_readfirstlane(group);
   }
   __device__ __forceinline__ int chunk(int j) const { return lane + j * kLanes; }
-  __device__ __forceinline__ bool on(int j) const { return chunk(j) * rows::kChunk < width; }
   __device__ __forceinline__ int begin(int j) const {
     const int at = chunk(j) * rows::kChunk;
-    return kWhole ? max(0, min(at, width - rows::kChunk)) : at;
+    return kWhole ? min(at, width - rows::kChunk) : at;
   }
   __device__ __forceinline__ int skip(int j) const {
-    return kWhole && on(j) && width >= rows::kChunk ? chunk(j) * rows::kChunk - begin(j) : 0;
+    return kWhole ? min(rows::kChunk, chunk(j) * rows::kChunk - begin(j)) : 0;
   }
-  __device__ __forceinline__ int left(int j) const { return width - begin(j); }
+  // values from the chunk's place (not its begin) to the row's end
+  __device__ __forceinline__ int left(int j) const { return width - chunk(j) * rows::kChunk; }
 };
 
 // A row's values of a lane, and those of its 8-bit checkpoint, as they lie in
@@ -91,24 +97,59 @@ struct Raw {
                                        const Place<kLanes, kChunks, kWhole> &at) {
     const T *row = static_cast<const T *>(base) + offset;
 #pragma unroll
-    for (int j = 0; j < kChunks; ++j)
-      c[j].load(row + at.begin(j), at.on(j) ? at.left(j) : 0);
+    for (int j = 0; j < kChunks; ++j) {
+      if constexpr (kWhole)
+        c[j] = *reinterpret_cast<const rows::Words<T> *>(row + at.begin(j));
+      else
+        c[j].load(row + at.begin(j), at.left(j));
+    }
   }
   __device__ __forceinline__ float get(int j, int i) const { return c[j].get(i); }
+  // has arrived here
+  __device__ __forceinline__ void settle() {
+#pragma unroll
+    for (int j = 0; j < kChunks; ++j)
+#pragma unroll
+      for (int i = 0; i < rows::Words<T>::kWords; ++i) asm volatile("" : "+v"(c[j].w[i]));
+  }
 };
 template <int kChunks>
 struct Packed {
-  rows::PackedChunk c[kChunks];
-  template <int kLanes>
+  rows::Bytes c[kChunks];
+  unsigned first[kChunks], last[kChunks];  // scales of a chunk's ends
+  template <int kLanes, bool kWhole>
   __device__ __forceinline__ void load(const uint8_t *row,
-                                       const Place<kLanes, kChunks, false> &at) {
+                                       const Place<kLanes, kChunks, kWhole> &at) {
+    struct __attribute__((packed, aligned(1))) Eight {
+      rows::Bytes b;
+    };
+    const uint8_t *scales = row + rows::blocks_of(at.width) * rows::kBlock;
 #pragma unroll
-    for (int j = 0; j < kChunks; ++j)
-      if (at.on(j)) c[j].load(row, at.chunk(j), rows::blocks_of(at.width));
+    for (int j = 0; j < kChunks; ++j) {
+      // (without kWhole rows are one block, whose bytes are all there)
+      const int begin = kWhole ? at.begin(j) : min(at.begin(j), rows::kBlock - rows::kChunk);
+      c[j] = reinterpret_cast<const Eight *>(row + begin)->b;
+      first[j] = scales[begin / rows::kBlock];
+      last[j] = scales[(begin + rows::kChunk - 1) / rows::kBlock];
+    }
   }
-  __device__ __forceinline__ void get(float (&v)[kChunks][rows::kChunk]) const {
+  template <int kLanes, bool kWhole>
+  __device__ __forceinline__ void get(float (&v)[kChunks][rows::kChunk],
+                                      const Place<kLanes, kChunks, kWhole> &at) const {
 #pragma unroll
-    for (int j = 0; j < kChunks; ++j) c[j].get(v[j]);
+    for (int j = 0; j < kChunks; ++j) {
+      rows::unpack(v[j], c[j], first[j]);
+      if (at.width % rows::kChunk != 0) {  // (two blocks' values may lie in it)
+        float w[rows::kChunk];
+        rows::unpack(w, c[j], last[j]);
+        const int begin = at.begin(j);
+#pragma unroll
+        for (int i = 0; i < rows::kChunk; ++i) {
+          if ((begin + i) / rows::kBlock != begin / rows::kBlock) v[j][i] = w[i];
+          if (!kWhole && i >= at.left(j)) v[j][i] = 0.f;
+        }
+      }
+    }
   }
 };
 
@@ -119,8 +160,12 @@ __device__ __forceinline__ void store_row(void *base, int64_t offset,
   T *row = static_cast<T *>(base) + offset;
 #pragma unroll
   for (int j = 0; j < kChunks; ++j) {
-    if (!at.on(j)) continue;
-    rows::store(row + at.begin(j), v[j], at.left(j));
+    rows::Words<T> words;
+    words.set(v[j]);
+    if constexpr (kWhole)
+      *reinterpret_cast<rows::Words<T> *>(row + at.begin(j)) = words;
+    else
+      words.store(row + at.begin(j), at.left(j));
   }
 }
 

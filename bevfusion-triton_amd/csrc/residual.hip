@@ -32,45 +32,47 @@ template <typename T, typename X, int kChunks>
 struct Inputs {
   Raw<X, kChunks> x;
   Raw<T, kChunks> update, gate;
-  template <int kLanes>
+  template <int kLanes, bool kWhole>
   __device__ __forceinline__ void load(const Args &A, int64_t row,
-                                       const Place<kLanes, kChunks> &at) {
+                                       const Place<kLanes, kChunks, kWhole> &at) {
     x.load(A.x, row * A.x_row, at);
-    if (A.update) update.load(A.update, row * A.update_row, at);
-    if (A.gate) {
-      const int64_t owner = A.gate_each == 1        ? row
-                            : A.rows < (1LL << 32) ? unsigned(row) / unsigned(A.gate_each)
-                                                   : row / A.gate_each;
-      gate.load(A.gate, owner * A.gate_row, at);
-    }
+    update.load(A.update, row * A.update_row, at);
+    const int64_t owner = A.gate_each == 1        ? row
+                          : A.rows < (1LL << 32) ? unsigned(row) / unsigned(A.gate_each)
+                                                 : row / A.gate_each;
+    gate.load(A.gate, owner * A.gate_row, at);
+  }
+  __device__ __forceinline__ void settle() {
+    x.settle();
+    update.settle();
+    gate.settle();
   }
 };
 
-// 8-bit checkpoint of a row: of whole chunks of a lane as they are in
-// registers, of the last one from memory, for it begins earlier here.
-template <typename T, int kLanes, int kChunks>
+// 8-bit checkpoint of a row: of chunks in their place as they are in registers,
+// of the last one from memory, for it begins earlier there.
+template <typename T, int kLanes, int kChunks, bool kWhole>
 __device__ __forceinline__ void keep(uint8_t *kept, const Raw<T, kChunks> &raw, const void *base,
-                                     int64_t offset, const Place<kLanes, kChunks> &at) {
+                                     int64_t offset, const Place<kLanes, kChunks, kWhole> &at) {
 #pragma unroll
   for (int j = 0; j < kChunks; ++j) {
     float v[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] = raw.get(j, i);
-    if (at.skip(j) > 0) {
-      const int first = at.chunk(j) * 8;
-      rows::load(v, static_cast<const T *>(base) + offset + first, at.width - first);
-    }
+    if (at.skip(j) > 0)
+      rows::load(v, static_cast<const T *>(base) + offset + at.chunk(j) * 8, at.left(j));
     rows::store_packed(kept, at.chunk(j), rows::blocks_of(at.width), v);
   }
 }
 
 // A group of lanes takes rows, the next one's loads on their way while one is
 // worked on; weights stay in registers.
-template <typename T, typename X, int kLanes, int kChunks>
-__global__ __launch_bounds__(threads_of(kLanes), forward_waves(kChunks)) void residual_kernel(Args A) {
+template <typename T, typename X, int kLanes, int kChunks, bool kWhole>
+__global__ __launch_bounds__(threads_of(kLanes), forward_waves(kChunks)) void residual_kernel(
+    Args A) {
   constexpr int kGroups = threads_of(kLanes) / kLanes;
   __shared__ float shared[4][threads_of(kLanes) / 64];
-  const Place<kLanes, kChunks> at(A.width);
+  const Place<kLanes, kChunks, kWhole> at(A.width);
   const int64_t width = A.width, pitch = rows::checkpoint_pitch(width);
   // scale times the update's weight, and the norm's weight
   float c[kChunks][8];
@@ -85,16 +87,13 @@ __global__ __launch_bounds__(threads_of(kLanes), forward_waves(kChunks)) void re
   if (A.weight) weight.load(A.weight, 0, at);
   const int64_t step = int64_t(gridDim.x) * kGroups;
   int64_t row = int64_t(blockIdx.x) * kGroups + at.group;
-  Inputs<T, X, kChunks> next;
-  if (row < A.rows) next.load(A, row, at);
+  if (row >= A.rows) return;  // (all of a block whose rows pass barriers)
+  Inputs<T, X, kChunks> in, next;
+  in.load(A, row, at);
   for (int turn = 0; row < A.rows; row += step, turn ^= 2) {
-    const Inputs<T, X, kChunks> in = next;
-    if (row + step < A.rows) next.load(A, row + step, at);
-    if (A.x_kept) keep<X>(A.x_kept + row * pitch, in.x, A.x, row * A.x_row, at);
+    next.load(A, row + step < A.rows ? row + step : row, at);
     float x[kChunks][8];
-    if (A.update) {
-      if (A.update_kept)
-        keep<T>(A.update_kept + row * pitch, in.update, A.update, row * A.update_row, at);
+    if (A.has_update) {
       float r = 1.f;
       if (A.update_weight) {
         float s[1] = {own_sum(at, [&](int j, int i) {
@@ -109,42 +108,52 @@ __global__ __launch_bounds__(threads_of(kLanes), forward_waves(kChunks)) void re
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
           float v = in.update.get(j, i) * r * c[j][i];
-          if (A.gate) v *= in.gate.get(j, i);
+          if (A.has_gate) v *= in.gate.get(j, i);
           x[j][i] = in.x.get(j, i) + v;
         }
-      store_row<X>(A.sum, row * width, x, at);
     } else {
 #pragma unroll
       for (int j = 0; j < kChunks; ++j)
 #pragma unroll
         for (int i = 0; i < 8; ++i) x[j][i] = in.x.get(j, i);
     }
+    float r = 0.f;
     if (A.weight) {
       float s[1] = {own_sum(at, [&](int j, int i) { return x[j][i] * x[j][i]; })};
       row_sums<kLanes>(s, shared[turn + 1]);
-      const float r = 1.0f / sqrtf(s[0] * A.inv_width + A.eps);
+      r = 1.0f / sqrtf(s[0] * A.inv_width + A.eps);
+    }
+    next.settle();  // (before the stores, for which it would wait behind them)
+    if (A.keeps) {
+      if (A.x_kept) keep<X>(A.x_kept + row * pitch, in.x, A.x, row * A.x_row, at);
+      if (A.update_kept)
+        keep<T>(A.update_kept + row * pitch, in.update, A.update, row * A.update_row, at);
+    }
+    if (A.has_update) store_row<X>(A.sum, row * width, x, at);
+    if (A.weight) {
 #pragma unroll
       for (int j = 0; j < kChunks; ++j)
 #pragma unroll
         for (int i = 0; i < 8; ++i) x[j][i] *= r * weight.get(j, i);
       store_row<T>(A.normed, row * width, x, at);
     }
+    in = next;
   }
 }
 
-template <typename T, typename X, int kLanes, int kChunks>
+template <typename T, typename X, int kLanes, int kChunks, bool kWhole>
 void launch(const Args &A, hipStream_t s) {
   constexpr int kGroups = threads_of(kLanes) / kLanes;
   constexpr int kBlocks = blocks_for(kLanes, forward_waves(kChunks));
   const int64_t blocks = (A.rows + kGroups - 1) / kGroups;
-  hipLaunchKernelGGL((residual_kernel<T, X, kLanes, kChunks>),
+  hipLaunchKernelGGL((residual_kernel<T, X, kLanes, kChunks, kWhole>),
                      dim3(unsigned(blocks < kBlocks ? blocks : kBlocks)),
                      dim3(threads_of(kLanes)), 0, s, A);
 }
 
 template <typename T, typename X>
 void launch_width(const Args &A, hipStream_t s) {
-#define RESIDUAL_LAUNCH(kLanes, kChunks, ...) launch<T, X, kLanes, kChunks>(A, s);
+#define RESIDUAL_LAUNCH(kLanes, kChunks, kWhole, ...) launch<T, X, kLanes, kChunks, kWhole>(A, s);
   RESIDUAL_LAYOUT(RESIDUAL_LAUNCH, A.width)
 #undef RESIDUAL_LAUNCH
 }
@@ -208,6 +217,18 @@ int bevpool_residual_norm_forward(const void *x, int64_t x_row, int32_t x_dtype,
   A.normed = normed;
   A.x_kept = static_cast<uint8_t *>(x_kept);
   A.update_kept = static_cast<uint8_t *>(update_kept);
+  A.keeps = x_kept || update_kept;
+  A.has_update = update != nullptr;
+  A.has_gate = gate != nullptr;
+  // (read and not used: x's first row, which is no shorter than one of theirs)
+  if (!update) {
+    A.update = x;
+    A.update_row = 0;
+  }
+  if (!gate) {
+    A.gate = x;
+    A.gate_row = 0;
+  }
   hipStream_t s = static_cast<hipStream_t>(stream);
   LaunchScope scope("residual_norm", s);
   if (dtype == BEVPOOL_F32)

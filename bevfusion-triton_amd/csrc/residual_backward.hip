@@ -60,13 +60,15 @@ template <typename T, typename X, int kChunks>
 struct Operands {
   Raw<X, kChunks> x;
   Raw<T, kChunks> update;
-  template <int kLanes>
+  template <int kLanes, bool kWhole>
   __device__ __forceinline__ void load(const Args &A, int64_t row,
-                                       const Place<kLanes, kChunks> &at) {
-    if (A.weight) x.load(A.x, row * A.x_row, at);
-    if (A.update) update.load(A.update, row * A.update_row, at);
+                                       const Place<kLanes, kChunks, kWhole> &at) {
+    x.load(A.x, row * A.x_row, at);
+    update.load(A.update, row * A.update_row, at);
   }
-  __device__ __forceinline__ void get(float (&u)[kChunks][8], float (&v)[kChunks][8]) const {
+  template <int kLanes, bool kWhole>
+  __device__ __forceinline__ void get(float (&u)[kChunks][8], float (&v)[kChunks][8],
+                                      const Place<kLanes, kChunks, kWhole> &) const {
 #pragma unroll
     for (int j = 0; j < kChunks; ++j)
 #pragma unroll
@@ -79,16 +81,18 @@ struct Operands {
 template <int kChunks>
 struct KeptOperands {
   Packed<kChunks> x, update;
-  template <int kLanes>
+  template <int kLanes, bool kWhole>
   __device__ __forceinline__ void load(const Args &A, int64_t row,
-                                       const Place<kLanes, kChunks, false> &at) {
+                                       const Place<kLanes, kChunks, kWhole> &at) {
     const int64_t offset = row * rows::checkpoint_pitch(at.width);
-    if (A.weight) x.load(A.x_kept + offset, at);
-    if (A.update) update.load(A.update_kept + offset, at);
+    x.load(A.x_kept + offset, at);
+    update.load(A.update_kept + offset, at);
   }
-  __device__ __forceinline__ void get(float (&u)[kChunks][8], float (&v)[kChunks][8]) const {
-    update.get(u);
-    x.get(v);
+  template <int kLanes, bool kWhole>
+  __device__ __forceinline__ void get(float (&u)[kChunks][8], float (&v)[kChunks][8],
+                                      const Place<kLanes, kChunks, kWhole> &at) const {
+    update.get(u, at);
+    x.get(v, at);
   }
 };
 template <typename Of, typename T, typename X, int kChunks>
@@ -100,8 +104,8 @@ struct Inputs {
   __device__ __forceinline__ void load(const Args &A, int64_t row, bool own_gate,
                                        const Place<kLanes, kChunks, kWhole> &at) {
     of.load(A, row, at);
-    if (A.dsum) dsum.load(A.dsum, row * A.dsum_row, at);
-    if (A.weight) dnormed.load(A.dnormed, row * A.dnormed_row, at);
+    dsum.load(A.dsum, row * A.dsum_row, at);
+    dnormed.load(A.dnormed, row * A.dnormed_row, at);
     if (own_gate) gate.load(A.gate, row * A.gate_row, at);
   }
 };
@@ -109,16 +113,18 @@ struct Inputs {
 // A block walks items, each an equal part of the rows that share a row of
 // gate (without such a gate: of all), and leaves each item's sums.  Its groups
 // of lanes take rows, the next one's loads on their way while one is worked on.
-template <typename T, typename X, int kLanes, int kChunks, bool kKept>
-__global__ __launch_bounds__(threads_of(kLanes), backward_waves(kLanes, kChunks, kKept, sizeof(X) == 4)) void residual_backward_kernel(Args A) {
+template <typename T, typename X, int kLanes, int kChunks, bool kWhole, bool kKept>
+__global__ __launch_bounds__(threads_of(kLanes),
+                             backward_waves(kLanes, kChunks, kKept, sizeof(X) == 4))
+void residual_backward_kernel(Args A) {
   constexpr int kGroups = threads_of(kLanes) / kLanes;
   typedef std::conditional_t<kKept, KeptOperands<kChunks>, Operands<T, X, kChunks>> Of;
   extern __shared__ float lds[];
   __shared__ float shared[6][2 * (threads_of(kLanes) / 64)];
-  const Place<kLanes, kChunks, !kKept> at(A.width);
+  const Place<kLanes, kChunks, kWhole> at(A.width);
   const int64_t width = A.width;
-  const bool own_gate = A.gate && A.gate_each == 1;
-  const int64_t part_rows = (A.gate && !own_gate ? A.gate_each : A.rows);
+  const bool own_gate = A.has_gate && A.gate_each == 1;
+  const int64_t part_rows = (A.has_gate && !own_gate ? A.gate_each : A.rows);
   const int64_t share = (part_rows + A.parts_each - 1) / A.parts_each;
   // scale times the update's weight, and the norm's weight
   float c[kChunks][8], dweight[kChunks][8] = {};
@@ -141,14 +147,15 @@ __global__ __launch_bounds__(threads_of(kLanes), backward_waves(kLanes, kChunks,
     const int64_t begin = first + part * share;
     const int64_t end = min(begin + share, first + part_rows);
     float q[kChunks][8] = {};
-    Inputs<Of, T, X, kChunks> next;
-    if (A.gate && !own_gate) next.gate.load(A.gate, owner * A.gate_row, at);
-    if (begin + at.group < end) next.load(A, begin + at.group, own_gate, at);
-    for (int64_t row = begin + at.group; row < end; row += kGroups, turn = 3 - turn) {
-      const Inputs<Of, T, X, kChunks> in = next;
-      if (row + kGroups < end) next.load(A, row + kGroups, own_gate, at);
+    Inputs<Of, T, X, kChunks> in, next;
+    int64_t row = begin + at.group;
+    if (A.has_gate && !own_gate) next.gate.load(A.gate, owner * A.gate_row, at);
+    if (row < end) next.load(A, row, own_gate, at);
+    for (; row < end; row += kGroups, turn = 3 - turn) {
+      in = next;
+      next.load(A, row + kGroups < end ? row + kGroups : row, own_gate, at);
       float n[kChunks][8], x[kChunks][8];
-      in.of.get(n, x);
+      in.of.get(n, x, at);
       float r_u = 1.f;
       if (A.update_weight) {
         float s[1] = {own_sum(at, [&](int j, int i) { return n[j][i] * n[j][i]; })};
@@ -163,15 +170,15 @@ __global__ __launch_bounds__(threads_of(kLanes), backward_waves(kLanes, kChunks,
 #pragma unroll
       for (int j = 0; j < kChunks; ++j)
 #pragma unroll
-        for (int i = 0; i < 8; ++i) g[j][i] = A.dsum ? in.dsum.get(j, i) : 0.f;
+        for (int i = 0; i < 8; ++i) g[j][i] = A.has_dsum ? in.dsum.get(j, i) : 0.f;
       if (A.weight) {
-        if (A.update) {
+        if (A.has_update) {
 #pragma unroll
           for (int j = 0; j < kChunks; ++j)
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
               const float v = n[j][i] * c[j][i];
-              x[j][i] += A.gate ? v * in.gate.get(j, i) : v;
+              x[j][i] += A.has_gate ? v * in.gate.get(j, i) : v;
             }
         }
         float s[2] = {own_sum(at, [&](int j, int i) { return x[j][i] * x[j][i]; }),
@@ -190,40 +197,39 @@ __global__ __launch_bounds__(threads_of(kLanes), backward_waves(kLanes, kChunks,
             g[j][i] += r * (h * weight.get(j, i) - x[j][i] * back);
           }
       }
-      store_row<X>(A.dx, row * width, g, at);
-      if (!A.update) continue;
-      // g becomes the gradient of n
-      if (own_gate) {
-        float dgate[kChunks][8];
-#pragma unroll
-        for (int j = 0; j < kChunks; ++j)
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const float t = g[j][i] * n[j][i], gate = in.gate.get(j, i);
-            dgate[j][i] = t * c[j][i];
-            q[j][i] += t * gate;
-            g[j][i] *= c[j][i] * gate;
-          }
-        store_row<T>(A.dgate, row * width, dgate, at);
-      } else {
-#pragma unroll
-        for (int j = 0; j < kChunks; ++j)
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            q[j][i] += g[j][i] * n[j][i];
-            g[j][i] *= A.gate ? c[j][i] * in.gate.get(j, i) : c[j][i];
-          }
+      if (!A.has_update) {
+        store_row<X>(A.dx, row * width, g, at);
+        continue;
       }
+      // dn: the gradient of n, with gate and weights
+      float dn[kChunks][8];
+#pragma unroll
+      for (int j = 0; j < kChunks; ++j)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const float t = g[j][i] * n[j][i], gate = A.has_gate ? in.gate.get(j, i) : 1.f;
+          q[j][i] += own_gate ? t * gate : t;
+          dn[j][i] = g[j][i] * (c[j][i] * gate);
+        }
+      float back = 0.f;
       if (A.update_weight) {
-        float s[1] = {own_sum(at, [&](int j, int i) { return g[j][i] * n[j][i]; })};
+        float s[1] = {own_sum(at, [&](int j, int i) { return dn[j][i] * n[j][i]; })};
         row_sums<kLanes>(s, shared[turn + 2]);
-        const float back = s[0] * A.inv_width;
+        back = s[0] * A.inv_width;
+      }
+      store_row<X>(A.dx, row * width, g, at);
+      if (own_gate) {
 #pragma unroll
         for (int j = 0; j < kChunks; ++j)
 #pragma unroll
-          for (int i = 0; i < 8; ++i) g[j][i] = r_u * (g[j][i] - n[j][i] * back);
+          for (int i = 0; i < 8; ++i) g[j][i] *= n[j][i] * c[j][i];
+        store_row<T>(A.dgate, row * width, g, at);
       }
-      store_row<T>(A.dupdate, row * width, g, at);
+#pragma unroll
+      for (int j = 0; j < kChunks; ++j)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) dn[j][i] = r_u * (dn[j][i] - n[j][i] * back);
+      store_row<T>(A.dupdate, row * width, dn, at);
     }
     if (A.parts) flush(q, A.parts + item * width, at, lds);
   }
@@ -278,7 +284,7 @@ __global__ __launch_bounds__(kSumThreads) void sums_kernel(Args A, int64_t weigh
   if (c < A.width && A.scale) scale = float(static_cast<const T *>(A.scale)[c]);
   if (blockIdx.y == 0) {
     float s = 0.f;
-    if (A.gate && A.gate_each > 1) {  // (the items' sums are without the gate)
+    if (A.has_gate && A.gate_each > 1) {  // (the items' sums are without the gate)
       if (c < A.width) {
         const T *gate = static_cast<const T *>(A.gate) + c;
         const float *parts = A.parts + c;
@@ -321,7 +327,7 @@ struct Split {
 };
 Split split_for(int64_t rows, int width, int64_t gate_rows, bool kept, bool wide) {
   int64_t most_blocks = 0, at_once = 0;
-#define RESIDUAL_BLOCKS(kLanes, kChunks, ...)                                   \
+#define RESIDUAL_BLOCKS(kLanes, kChunks, kWhole, ...)                                   \
   {                                                                             \
     most_blocks = blocks_for(kLanes, backward_waves(kLanes, kChunks, kept, wide));    \
     at_once = threads_of(kLanes) / kLanes;                                      \
@@ -341,21 +347,22 @@ Split split_for(int64_t rows, int width, int64_t gate_rows, bool kept, bool wide
   return s;
 }
 
-template <typename T, typename X, int kLanes, int kChunks>
+template <typename T, typename X, int kLanes, int kChunks, bool kWhole>
 void launch(const Args &A, int64_t blocks, bool kept, hipStream_t s) {
   constexpr int kGroups = threads_of(kLanes) / kLanes;
   const size_t lds = kGroups == 1 ? 0 : sizeof(float) * kGroups * size_t(A.width);
   if (kept)
-    hipLaunchKernelGGL((residual_backward_kernel<T, X, kLanes, kChunks, true>),
+    hipLaunchKernelGGL((residual_backward_kernel<T, X, kLanes, kChunks, kWhole, true>),
                        dim3(unsigned(blocks)), dim3(threads_of(kLanes)), lds, s, A);
   else
-    hipLaunchKernelGGL((residual_backward_kernel<T, X, kLanes, kChunks, false>),
+    hipLaunchKernelGGL((residual_backward_kernel<T, X, kLanes, kChunks, kWhole, false>),
                        dim3(unsigned(blocks)), dim3(threads_of(kLanes)), lds, s, A);
 }
 
 template <typename T, typename X>
 void launch_width(const Args &A, int64_t blocks, bool kept, hipStream_t s) {
-#define RESIDUAL_LAUNCH(kLanes, kChunks, ...) launch<T, X, kLanes, kChunks>(A, blocks, kept, s);
+#define RESIDUAL_LAUNCH(kLanes, kChunks, kWhole, ...) \
+  launch<T, X, kLanes, kChunks, kWhole>(A, blocks, kept, s);
   RESIDUAL_LAYOUT(RESIDUAL_LAUNCH, A.width)
 #undef RESIDUAL_LAUNCH
 }
@@ -363,7 +370,7 @@ void launch_width(const Args &A, int64_t blocks, bool kept, hipStream_t s) {
 template <typename T>
 void launch_sums(const Args &A, int64_t blocks, void *dgate, void *dupdate_weight, void *dscale,
                  void *dweight, hipStream_t s) {
-  const int64_t owners = A.gate && A.gate_each > 1 ? A.items / A.parts_each : 0;
+  const int64_t owners = A.has_gate && A.gate_each > 1 ? A.items / A.parts_each : 0;
   if (!owners && !dupdate_weight && !dscale && !dweight) return;
   const dim3 grid((A.width + kSumColumns - 1) / kSumColumns,
                   unsigned(2 + (owners < 4096 ? owners : 4096)));
@@ -402,6 +409,7 @@ int bevpool_residual_norm_backward(
   if ((dupdate_weight && !update_weight) || (dscale && !scale) || (dweight && !weight))
     return fail(BEVPOOL_EINVAL, "a gradient of a weight that is not there");
   if (rows > 0) {
+    if (!update && !weight) return fail(BEVPOOL_EINVAL, "neither an update nor a norm");
     if (gate && gate_rows < 1) return fail(BEVPOOL_EINVAL, "a gate without rows");
     if (!update && (update_weight || scale || gate))
       return fail(BEVPOOL_EINVAL, "update_weight, scale and gate are of an update");
@@ -432,6 +440,27 @@ int bevpool_residual_norm_backward(
   A.dx = dx;
   A.dupdate = dupdate;
   A.dgate = dgate;
+  A.has_update = update != nullptr;
+  A.has_gate = gate != nullptr;
+  A.has_dsum = dsum != nullptr;
+  // What is read and not used: rows that are there and no shorter.  (dx is read
+  // by the lanes that write it, before they do.)
+  if (!dsum) {
+    A.dsum = dx;
+    A.dsum_row = width;
+  }
+  if (!weight) {
+    A.x = A.dsum;
+    A.x_row = A.dsum_row;
+    A.x_kept = A.update_kept;
+    A.dnormed = A.dsum;
+    A.dnormed_row = 0;
+  }
+  if (!update) {
+    A.update = A.dnormed;
+    A.update_row = 0;
+    A.update_kept = A.x_kept;
+  }
   Split split = {0, 1, 0};
   if (rows > 0) {
     split = split_for(rows, width, gate ? gate_rows : 0, kept != 0, x_dtype == BEVPOOL_F32);
