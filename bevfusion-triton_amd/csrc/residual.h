@@ -10,7 +10,7 @@ constexpr int kMaxWidth = 8192;
 struct Args {
   // inputs.  Weights that are not there are null; rows that are not there are
   // other rows, read all the same and not used (see the flags), so that no load
-  // is behind a condition.
+  // of a row in turn is behind a condition (but a gate's of its own).
   const void *x, *update, *gate, *update_weight, *scale, *weight;
   bool has_update, has_gate, has_dsum, keeps;
   int64_t x_row, update_row, gate_row;  // strides in values
@@ -49,8 +49,9 @@ constexpr int threads_of(int lanes) { return lanes > 64 ? lanes : 256; }
 // Waves of a SIMD that the registers of a kernel leave room for (they are
 // compiled to), and the blocks of the whole card: the kernels walk rows by as
 // many as are there at once.  More only begin later: backward of 200,000 rows of
-// 80 by three blocks a CU, as many as there is room for, 57 us, by four 71; one
-// block a row instead, forward of 16,896 rows of 1,280 63 us for 43.
+// 80 by three blocks a CU, as many as there is room for, 48 us, by four 50, 80,000
+// of 256 49 and 54; one block a row instead, forward of 16,896 rows of 1,280 45 us
+// for 35.
 constexpr int forward_waves(int chunks) { return chunks > 1 ? 3 : 4; }
 constexpr int backward_waves(int lanes, int chunks, bool kept, bool wide) {
   return chunks > 1 ? 2 : kept || lanes < 64 || wide ? 3 : 4;  // (wide: a stream in fp32)
@@ -66,7 +67,8 @@ constexpr int blocks_for(int lanes, int waves) {
 // past it have the last one too.  So the first `skip` values of a chunk are
 // another lane's as well; all form the same of them, and only sums leave them
 // out.  No access is behind a condition, so the compiler can count them, and a
-// row's loads wait for no store of the row before.
+// row's loads wait for no store of the row before (16,896 rows of 1,280: forward
+// 35 us for 39, backward 56 for 65).
 template <int kLanes, int kChunks, bool kWhole>
 struct Place {
   int lane, group, width;

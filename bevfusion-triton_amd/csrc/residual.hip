@@ -9,7 +9,7 @@
 //
 // Bound by memory: x and u (and a gate of each value) read once, x' and h
 // written once.  A row stays in the registers of its lanes from the first sum
-// to the last store.  16,896 rows of 1,280 in bf16 39 us (4.4 TB/s of what has
+// to the last store.  16,896 rows of 1,280 in bf16 35 us (4.9 TB/s of what has
 // to move; a large copy reaches 5.1), with an fp32 stream and the checkpoints
 // 62 us (4.9 TB/s); 30,011 rows of 1,283 in fp16 with a gate of each value, rows
 // that begin at any address, 89 us (4.3 TB/s).

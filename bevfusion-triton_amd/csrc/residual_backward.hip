@@ -14,8 +14,8 @@
 //
 // Bound by memory: x, u, D and H (and a gate of each value) read once, dx and
 // du (and dgate) written once.  x' and n are formed again from x and u.  16,896
-// rows of 1,280 in bf16 65 us (4.0 TB/s) and 10 for the sums of six rows of gate;
-// from checkpoints, with an fp32 stream, 79 us (3.8 TB/s) and 5.
+// rows of 1,280 in bf16 56 us (4.6 TB/s) and 10 for the sums of six rows of gate;
+// from checkpoints, with an fp32 stream, 71 us (4.3 TB/s) and 5.
 #include <hip/hip_runtime.h>
 
 #include <stdint.h>
