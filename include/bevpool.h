@@ -692,7 +692,7 @@ int bevpool_checkpoint_unpack(const void *kept, int32_t dtype, int64_t rows, int
  *   kept         checkpoint of (tokens, k), from a multiple of 16 bytes
  *   dweight      (n, k) contiguous, in dtype
  *   scratch      >= bevpool_checkpoint_weight_grad_scratch_bytes(...): sums of
- *                parts of the tokens, up to 512 x 256 x 128 numbers and more
+ *                parts of the tokens, up to 256 x 256 x 256 numbers and more
  *                only where dweight has more
  * And that of its bias, the sums of columns: out [width] of x (rows, width).
  */
@@ -713,7 +713,8 @@ int bevpool_column_sums(const void *x, int64_t x_row, int32_t dtype, int64_t row
  *            (update_weight NULL: n = update)
  *   sum    = x + scale * gate * n               (scale, gate NULL: 1)
  *   normed = sum / sqrt(mean(sum^2) + eps) * weight  (weight NULL: not formed)
- * update NULL: sum is x and is not written.
+ * update NULL: sum is x and is not written (without weight there is nothing
+ * to do: refused, as in the backward).
  *   x, sum       of x_dtype: fp32 or dtype; all others of dtype
  *   width        at most 8192
  *   update_weight, scale, weight   [width]

@@ -68,7 +68,8 @@ def test_residual_norm_entries(pkg):
         (dict(dnormed=None), -1, b'null'), (dict(duw=None), -1, b'place'),
         (dict(dweight=None), -1, b'place'), (dict(dscale=16), -1, b'not there'),
         (dict(update=None), -1, b'of an update'), (dict(scratch=None), -3, b'scratch'),
-        (dict(nbytes=need - 1), -3, b'scratch')))
+        (dict(nbytes=need - 1), -3, b'scratch'),
+        (dict(update=None, uw=None, duw=None, gate=None, weight=None, dweight=None), -1, b'neither')))
     assert need > 0 and lib.bevpool_residual_norm_backward_scratch_bytes(0, 64, 0, 2, 0) == 0
 
 

@@ -136,6 +136,15 @@ def test_gradient_of_one_output(pkg, cuda, only):
     check(pkg, cuda, case, {only: grads[only]})
 
 
+@pytest.mark.parametrize('only', ['sum', 'normed'])
+@pytest.mark.parametrize('gate', [None, 5])
+@pytest.mark.parametrize('width', [5, 1283])
+def test_gradient_of_one_output_from_checkpoints(pkg, cuda, width, gate, only):
+    """Rows, of gradients or of a gate, that are not there."""
+    case, grads = make(10, width, torch.float32, torch.float16, seed=width, gate=gate)
+    check(pkg, cuda, case, {only: grads[only]}, 8)
+
+
 @pytest.mark.parametrize('types', TYPES, ids=str)
 @pytest.mark.parametrize('width', [1, 31, 80, 1283, 2056, 5000])
 def test_checkpoints(pkg, cuda, width, types):
