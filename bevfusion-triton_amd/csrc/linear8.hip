@@ -16,7 +16,7 @@
 // card's power leaves (busy in 47% of the cycles): 8192 x 8192 x 8192 487 us,
 // 2,260 TOPS (a library's product to 32-bit sums 2,050), 16,896 x 1,280 x 10,240
 // 255 us, 1,740 TOPS, and 15 for the codes; a few tokens by the weights' bytes:
-// one of 4,096 x 6,144 6.4 us (3.9 TB/s) and 2.5, 67 of 5,000 x 4,099 12.8 and 4.
+// one of 4,096 x 6,144 8.1 us, codes and all, 67 of 5,000 x 4,099 12.8 and 4.
 #include <hip/hip_runtime.h>
 
 #include <stdint.h>
@@ -376,9 +376,47 @@ void product_kernel(ProductArgs A) {
 // Few tokens: 16 kTx tokens by 16 kTw channels a block, whose eight waves take
 // every eighth 64 bytes of the rows straight to registers, so that the weights
 // are on their way all at once, and add their sums in LDS.
-constexpr int kFewWaves = 8;
+constexpr int kFewWaves = 8, kFewThreads = 64 * kFewWaves;
+
+// The waves' sums of a block to its results.
 template <typename T, int kTx, int kTw>
-__global__ __launch_bounds__(64 * kFewWaves, kTx * kTw > 4 ? 2 : 4) void few_kernel(ProductArgs A) {
+__device__ __forceinline__ void finish_few(const ProductArgs &A, i32x4 (&sums)[kFewWaves][kTw * kTx][64],
+                                           const i32x4 (&acc)[kTw][kTx], const float *x_scale, int w0,
+                                           int lane, int wave) {
+  const int c = lane & 15, q = lane >> 4;
+#pragma unroll
+  for (int i = 0; i < kTw; ++i)
+#pragma unroll
+    for (int j = 0; j < kTx; ++j) sums[wave][i * kTx + j][lane] = acc[i][j];
+  __syncthreads();
+  const T *bias = static_cast<const T *>(A.bias);
+  for (int t = wave; t < kTw * kTx; t += kFewWaves) {
+    i32x4 sum = sums[0][t][lane];
+#pragma unroll
+    for (int i = 1; i < kFewWaves; ++i) sum += sums[i][t][lane];
+    // lane 16 q + c: channels 4 q .. + 3 of token c
+    const int token = t % kTx * 16 + c, n = w0 + t / kTx * 16 + 4 * q;
+    if (token >= A.tokens) continue;
+    const float by = x_scale[token];
+    T *y = static_cast<T *>(A.y) + int64_t(token) * A.channels + n;
+    Four<T> four;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int at = min(n + r, A.channels - 1);
+      four.v[r] = T(float(sum[r]) * by * A.w_scale[at] + (bias ? float(bias[at]) : 0.f));
+    }
+    if (n + 4 <= A.channels) {
+      *reinterpret_cast<Four<T> *>(y) = four;
+    } else {
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        if (n + r < A.channels) y[r] = four.v[r];
+    }
+  }
+}
+
+template <typename T, int kTx, int kTw>
+__global__ __launch_bounds__(kFewThreads, kTx * kTw > 4 ? 2 : 4) void few_kernel(ProductArgs A) {
   __shared__ i32x4 sums[kFewWaves][kTw * kTx][64];
   constexpr int kDeep = 4;  // steps whose loads are on their way together
   const int lane = attention::lane_id(), wave = attention::wave_id();
@@ -418,35 +456,87 @@ __global__ __launch_bounds__(64 * kFewWaves, kTx * kTw > 4 ? 2 : 4) void few_ker
         for (int j = 0; j < kTx; ++j)
           acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(w[d][i], x[d][j], acc[i][j], 0, 0, 0);
   }
+  finish_few<T, kTx, kTw>(A, sums, acc, A.x_scale, w0, lane, wave);
+}
+
+// Up to eight short tokens: every block forms their codes itself, beside its
+// weights' way, instead of a launch before.  Tokens' values go to registers
+// first, so that what waits for them does not wait for the weights; a token has
+// 512, 256, 128 or 64 of the block's lanes, codes lie in LDS.  us by events, in
+// one launch and in two: 1 x 4096 x 6144 10.3, 6.2 + 9.8; 1 x 8192 x 8192 16.6,
+// 6.5 + 22.3; 4 x 1280 x 10240 8.9, 6.2 + 7.9; 8 x 2048 x 8192 9.9, 6.6 + 8.0.
+// Weights of eight steps are on their way together, of short rows four (1 x 1280
+// x 10240 8.6, by eight 11.2; 1 x 4096 x 4096 8.2, by four 11.1).
+constexpr int kOwnTokens = 8;
+constexpr int kOwnBytes = 16384;  // of codes, tokens rounded up to a power of two
+template <typename T, int kDeep>
+__global__ __launch_bounds__(kFewThreads, 4) void token_kernel(ProductArgs A, const T *x, int64_t x_row,
+                                                               int width, int row_lanes) {
+  constexpr int kHold = kOwnBytes / kFewThreads / rows::kChunk;
+  __shared__ i32x4 sums[kFewWaves][1][64];
+  __shared__ __align__(16) int8_t codes[kOwnBytes + kOwnTokens * 16];  // (16 bytes between rows: banks)
+  __shared__ float scales[kOwnTokens];
+  __shared__ unsigned tops[kFewWaves];
+  const int lane = attention::lane_id(), wave = attention::wave_id();
+  const int c = lane & 15, q = lane >> 4;
+  const int w0 = int(blockIdx.x) * 16, code_row = A.x_pitch + 16;
+  const int token = int(threadIdx.x) / row_lanes, own = int(threadIdx.x) % row_lanes;
+  const T *at = x + min(token, A.tokens - 1) * x_row;
+  rows::Words<T> words[kHold];
 #pragma unroll
-  for (int i = 0; i < kTw; ++i)
+  for (int j = 0; j < kHold; ++j) {
+    const int d = (own + j * row_lanes) * rows::kChunk;
+    words[j].load(at + d, width - d);
+  }
+  __builtin_amdgcn_sched_barrier(0);
+  const int8_t *w_at = A.w + int64_t(min(w0 + c, A.channels - 1)) * A.w_row;
+  i32x4 w[kDeep];
+  auto fetch = [&](int first) {
 #pragma unroll
-    for (int j = 0; j < kTx; ++j) sums[wave][i * kTx + j][lane] = acc[i][j];
-  __syncthreads();
-  const T *bias = static_cast<const T *>(A.bias);
-  for (int t = wave; t < kTw * kTx; t += kFewWaves) {
-    i32x4 sum = sums[0][t][lane];
-#pragma unroll
-    for (int i = 1; i < kFewWaves; ++i) sum += sums[i][t][lane];
-    // lane 16 q + c: channels 4 q .. + 3 of token c
-    const int token = t % kTx * 16 + c, n = w0 + t / kTx * 16 + 4 * q;
-    if (token >= A.tokens) continue;
-    const float by = A.x_scale[token];
-    T *y = static_cast<T *>(A.y) + int64_t(token) * A.channels + n;
-    Four<T> four;
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const int at = min(n + r, A.channels - 1);
-      four.v[r] = T(float(sum[r]) * by * A.w_scale[at] + (bias ? float(bias[at]) : 0.f));
+    for (int d = 0; d < kDeep; ++d) {
+      // (past a row's end, and behind the last step: as above)
+      const int chunk = min((first + d * kFewWaves) * 4 + q, A.w_chunks - 1);
+      w[d] = *reinterpret_cast<const i32x4 *>(w_at + chunk * 16);
     }
-    if (n + 4 <= A.channels) {
-      *reinterpret_cast<Four<T> *>(y) = four;
-    } else {
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  fetch(wave);
+  unsigned top = 0;
 #pragma unroll
-      for (int r = 0; r < 4; ++r)
-        if (n + r < A.channels) y[r] = four.v[r];
+  for (int j = 0; j < kHold; ++j) top = max(top, top_of(words[j]));
+#pragma unroll
+  for (int m = 1; m < 64; m <<= 1) top = max(top, unsigned(__shfl_xor(int(top), m, 64)));
+  if (lane == 0) tops[wave] = top;
+  attention::tile_barrier();
+  const int first_wave = token * row_lanes / 64;
+  for (int i = 0; i < row_lanes / 64; ++i) top = max(top, tops[first_wave + i]);
+  const float s = scale_of(__builtin_bit_cast(float, top)), inverse = 1.f / s;
+  if (token < A.tokens) {
+    if (own == 0) scales[token] = s;
+#pragma unroll
+    for (int j = 0; j < kHold; ++j) {
+      const int d = (own + j * row_lanes) * rows::kChunk;
+      if (d >= A.x_pitch) continue;
+      unsigned code[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) code[i] = code_of<T>(words[j].get(i), s, inverse);
+      *reinterpret_cast<rows::Bytes *>(codes + token * code_row + d) = rows::low_bytes(code);
     }
   }
+  attention::tile_barrier();
+  const int8_t *x_at = codes + min(c, A.tokens - 1) * code_row;
+  i32x4 acc[1][1] = {};
+  for (int first = wave; first < A.steps; first += kFewWaves * kDeep) {
+    if (first != wave) fetch(first);
+#pragma unroll
+    for (int d = 0; d < kDeep; ++d) {
+      const int step = first + d * kFewWaves;
+      i32x4 x = {0, 0, 0, 0};
+      if (step < A.steps) x = *reinterpret_cast<const i32x4 *>(x_at + (step * 4 + q) * 16);
+      acc[0][0] = __builtin_amdgcn_mfma_i32_16x16x64_i8(w[d], x, acc[0][0], 0, 0, 0);
+    }
+  }
+  finish_few<T, 1, 1>(A, sums, acc, scales, w0, lane, wave);
 }
 
 // ---------------------------------------------------------------------------
@@ -507,6 +597,27 @@ int launch_tiles(ProductArgs &A, hipStream_t s) {
   return check_launch("linear8");
 }
 
+// Lanes of a token where every block forms the codes itself; else 0.
+int own_lanes(int64_t tokens, int pitch) {
+  if (tokens > kOwnTokens) return 0;
+  const int places = tokens > 4 ? 8 : tokens > 2 ? 4 : int(tokens);
+  return places * pitch <= kOwnBytes ? kFewThreads / places : 0;
+}
+
+template <typename T, int kDeep>
+int launch_token(const ProductArgs &A, const void *x, int64_t x_row, int width, int row_lanes,
+                 hipStream_t s) {
+  hipLaunchKernelGGL((token_kernel<T, kDeep>), dim3((A.channels + 15) / 16), dim3(kFewThreads), 0, s,
+                     A, static_cast<const T *>(x), x_row, width, row_lanes);
+  return check_launch("linear8");
+}
+template <typename T>
+int launch_own(const ProductArgs &A, const void *x, int64_t x_row, int width, int row_lanes,
+               hipStream_t s) {
+  return A.steps > 4 * kFewWaves ? launch_token<T, 8>(A, x, x_row, width, row_lanes, s)
+                                 : launch_token<T, 4>(A, x, x_row, width, row_lanes, s);
+}
+
 template <typename T, int kTx, int kTw>
 int launch_few(const ProductArgs &A, hipStream_t s) {
   const int blocks = (A.channels + 16 * kTw - 1) / (16 * kTw);
@@ -521,8 +632,7 @@ int launch_product(ProductArgs &A, hipStream_t s) {
   // Up to 32 tokens the weights' way to the registers is the time.  32 channels
   // a block read the tokens half as often as 16, but need enough channels for
   // the card's CUs: us by 16 and by 32, 16 x 4096 x 6144 12.4 and 10.9, 32 x
-  // 8192 x 8192 32.1 and 24.7; 8 x 1280 x 10240 7.7 and 8.1, 32 x 1280 x 1280 6.2
-  // and 7.1.
+  // 8192 x 8192 32.1 and 24.7; 32 x 1280 x 1280 6.2 and 7.1.
   if (A.tokens <= 32) {
     const bool wide = A.channels >= 32 * 160;
     if (A.tokens <= 16) return wide ? launch_few<T, 1, 2>(A, s) : launch_few<T, 1, 1>(A, s);
@@ -611,8 +721,11 @@ int bevpool_linear8(const void *x, int64_t x_row, int32_t dtype, const void *wei
   const int pitch = int(code_pitch(width));
   int8_t *codes = static_cast<int8_t *>(scratch);
   float *scales = reinterpret_cast<float *>(codes + tokens * pitch);
-  st = codes_for(x, x_row, dtype, tokens, width, pitch, codes, scales, s);
-  if (st) return st;
+  const int row_lanes = own_lanes(tokens, pitch);
+  if (!row_lanes) {
+    st = codes_for(x, x_row, dtype, tokens, width, pitch, codes, scales, s);
+    if (st) return st;
+  }
   ProductArgs A = {};
   A.x = codes;
   A.w = static_cast<const int8_t *>(weight);
@@ -627,6 +740,10 @@ int bevpool_linear8(const void *x, int64_t x_row, int32_t dtype, const void *wei
   A.channels = int(channels);
   A.steps = pitch / 64;
   LaunchScope scope("linear8", s);
+  if (row_lanes && dtype == BEVPOOL_F32) return launch_own<float>(A, x, x_row, width, row_lanes, s);
+  if (row_lanes && dtype == BEVPOOL_F16)
+    return launch_own<_Float16>(A, x, x_row, width, row_lanes, s);
+  if (row_lanes) return launch_own<__bf16>(A, x, x_row, width, row_lanes, s);
   if (dtype == BEVPOOL_F32) return launch_product<float>(A, s);
   if (dtype == BEVPOOL_F16) return launch_product<_Float16>(A, s);
   return launch_product<__bf16>(A, s);

@@ -46,6 +46,25 @@ def test_widths(pkg, cuda, width, tokens):
     check(pkg, cuda, *make(tokens, width, 37, torch.bfloat16, width))
 
 
+@pytest.mark.parametrize('dtype', DTYPES, ids=str)
+@pytest.mark.parametrize('tokens,width', [
+    (1, 2048), (1, 2049), (1, 16384), (1, 16385), (2, 8192), (2, 8193), (3, 4096), (4, 4097),
+    (5, 2048), (8, 2048), (8, 2049), (9, 100)])
+def test_few_tokens(pkg, cuda, dtype, tokens, width):
+    """Both sides of where every block forms the codes itself; rows that begin
+    at any address, and one that is not finite."""
+    x, *rest = make(tokens, width, 41, dtype, width)
+    wide = torch.zeros((tokens, width + 3), dtype=dtype, device=cuda)
+    wide[:, 1:-2] = x.to(cuda)
+    check(pkg, cuda, x, *rest, got=pkg.linear_int8(wide[:, 1:-2], *(t.to(cuda) for t in rest)))
+    if tokens > 1:
+        wide[1, width // 2] = float('inf')
+        got = pkg.linear_int8(wide[:, 1:-2], *(t.to(cuda) for t in rest))
+        assert bool(got[1].isnan().all())
+        keep = [i for i in range(tokens) if i != 1]
+        check(pkg, cuda, x[keep], *rest, got=got[keep])
+
+
 @pytest.mark.parametrize('out', [1, 3, 4, 7, 8, 31, 32, 33, 127, 129, 1030])
 @pytest.mark.parametrize('tokens', [1, 40])
 def test_channels(pkg, cuda, out, tokens):
