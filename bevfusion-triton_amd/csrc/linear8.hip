@@ -642,10 +642,14 @@ int launch_product(ProductArgs &A, hipStream_t s) {
     return int64_t((A.tokens + x - 1) / x) * ((A.channels + w - 1) / w);
   };
   // Small tiles where few of larger ones would leave CUs idle, and while there
-  // are no more than CUs the rows' length in two parts: us by 64 x 64 in two
+  // are no more than CUs the rows' length in parts, four of 64 x 32 and two of 64
+  // x 64.  us by 64 x 32 in four and 64 x 64 in two: 33 x 8192 x 8192 18.0 and
+  // 22.9, 64 x 4096 x 4096 9.9 and 12.0, 500 x 4096 x 1024 10.6 and 12.8; 128 x
+  // 4096 x 6144 17.5 and 13.2.  By 64 x 64 in two
   // parts, 64 x 64 and 64 x 128, 67 x 5000 x 4099 14.0, 17.1 and 22.1, 200 x 4096
   // x 4096 12.8, 15.0 and 18.5; 512 x 4096 x 4096 21.6, 18.7 and 20.3, 1024 x 1280
   // x 1280 12.1, 9.2 and 10.8; 800 x 4096 x 4096 37.4, 30.3 and 24.0.
+  if (tiles(64, 32) <= 256) return launch_tiles<T, 1, 1, 2, 1, 128, 3, 4>(A, s);
   const int64_t small = tiles(64, 64);
   if (small <= 256) return launch_tiles<T, 1, 1, 2, 2, 128, 4, 2>(A, s);
   if (small <= 512) return launch_tiles<T, 1, 1, 2, 2, 128, 4>(A, s);

@@ -46,6 +46,15 @@ def test_widths(pkg, cuda, width, tokens):
     check(pkg, cuda, *make(tokens, width, 37, torch.bfloat16, width))
 
 
+@pytest.mark.parametrize('tokens,width,out', [
+    (33, 128, 8191), (70, 129, 4097), (300, 333, 2000), (64, 640, 8193), (40, 2050, 50),
+    (257, 1100, 1601)])
+def test_parts_of_rows(pkg, cuda, tokens, width, out):
+    """Rows whose length is divided: evenly, unevenly and with parts that are
+    left with nothing; both sides of where tiles grow."""
+    check(pkg, cuda, *make(tokens, width, out, torch.float16, width))
+
+
 @pytest.mark.parametrize('dtype', DTYPES, ids=str)
 @pytest.mark.parametrize('tokens,width', [
     (1, 2048), (1, 2049), (1, 16384), (1, 16385), (2, 8192), (2, 8193), (3, 4096), (4, 4097),
