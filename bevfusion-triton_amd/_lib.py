@@ -12,11 +12,14 @@ already loaded; device pointers and streams are then shared with torch.
 from __future__ import annotations
 
 import ctypes
+import importlib.machinery
+import importlib.util
 from pathlib import Path
 
 import torch  # noqa: F401  (loads the HIP runtime first; see module docstring)
 
 LIB_PATH = Path(__file__).resolve().parent / 'libbevpool_amd.so'
+GRADIENTS_PATH = LIB_PATH.with_name('_autograd.so')
 ABI_VERSION = 4
 
 F32, F16, BF16 = 0, 1, 2
@@ -203,6 +206,7 @@ _SIGNATURES = {
 EXPORTED_SYMBOLS = tuple(_SIGNATURES)
 
 _lib = None
+_gradients = None
 
 
 def library():
@@ -228,6 +232,27 @@ def library():
         raise LibraryNotBuilt(f'{LIB_PATH} has ABI version {version}, expected {ABI_VERSION}')
     _lib = lib
     return lib
+
+
+def gradients():
+    """The autograd nodes of csrc/autograd.cpp (loaded once)."""
+    global _gradients
+    if _gradients is None:
+        library()
+        if not GRADIENTS_PATH.exists():
+            raise LibraryNotBuilt(
+                f'{GRADIENTS_PATH} is missing: build it with `python -c "import __graft_entry__ as g; '
+                f'g.build()"` (or `make -C bevfusion-triton_amd/csrc`)'
+            )
+        loader = importlib.machinery.ExtensionFileLoader('_autograd', str(GRADIENTS_PATH))
+        spec = importlib.util.spec_from_loader('_autograd', loader)
+        try:
+            module = importlib.util.module_from_spec(spec)
+            loader.exec_module(module)
+        except ImportError as exc:  # (another torch than it was built with)
+            raise LibraryNotBuilt(f'cannot load {GRADIENTS_PATH}: {exc}') from exc
+        _gradients = module
+    return _gradients
 
 
 def check(status: int, what: str) -> None:

@@ -22,8 +22,6 @@ allocate with torch's allocator and never wait for the device.
 """
 from __future__ import annotations
 
-import functools
-
 import torch
 from torch import nn
 from torch.autograd.function import once_differentiable
@@ -104,6 +102,8 @@ def _residual_norm(x, update, update_weight, scale, gate, weight, dtype, eps, ke
 
 
 class _ResidualNorm(torch.autograd.Function):
+    """For traces, and to refuse tangents; csrc/autograd.cpp has the node that
+    follows other calls."""
     @staticmethod
     def forward(ctx, x, update, update_weight, scale, gate, weight, dtype, eps, keep):
         total, normed, x_kept, update_kept = _residual_norm(x, update, update_weight, scale, gate,
@@ -111,54 +111,15 @@ class _ResidualNorm(torch.autograd.Function):
         if not keep:
             x_kept, update_kept = x if weight is not None else None, update
         ctx.save_for_backward(x_kept, update_kept, update_weight, scale, gate, weight)
-        ctx.call = (*x.shape, x.dtype, x.device, dtype, eps, keep, update is not None)
+        ctx.call = (*x.shape, x.dtype, dtype, eps, keep, update is not None)
         ctx.set_materialize_grads(False)
         return total, normed
 
     @staticmethod
-    @once_differentiable  # (the gradients are no functions of the graph's)
+    @once_differentiable
     def backward(ctx, dtotal, dnormed):
-        x, update, update_weight, scale, gate, weight = ctx.saved_tensors
-        rows, width, x_dtype, device, dtype, eps, keep, has_update = ctx.call
-        if dtotal is None and dnormed is None:
-            return (None,) * 9
-        dweight = None
-        if dnormed is None:
-            if weight is not None:
-                dweight, weight = torch.zeros_like(weight), None
-            x = None
-        elif dnormed.dtype != dtype or dnormed.stride(1) != 1:
-            dnormed = _unit(dnormed.to(dtype))
-        if dtotal is not None and (dtotal.dtype != x_dtype or dtotal.stride(1) != 1):
-            dtotal = _unit(dtotal.to(x_dtype))
-        new = (dtotal if dnormed is None else dnormed).new_empty
-        dx = new((rows, width), dtype=x_dtype)
-        dupdate = new((rows, width), dtype=dtype) if has_update else None
-        dupdate_weight = None if update_weight is None else new(width, dtype=dtype)
-        dscale = None if scale is None else new(width, dtype=dtype)
-        if weight is not None:
-            dweight = new(width, dtype=dtype)
-        gate_rows, dgate = 0, None
-        if gate is not None:
-            gate_rows = gate.shape[0]
-            # (no kernel writes the sums of no rows)
-            dgate = new((gate_rows, width), dtype=dtype) if rows else torch.zeros_like(gate)
-        x_code = L.DTYPE_CODES[x_dtype]
-        nbytes = _backward_scratch(rows, width, gate_rows, x_code, keep)
-        scratch = new(nbytes, dtype=torch.uint8)
-        ptr = L.ptr
-        _run(lambda lib, s: lib.bevpool_residual_norm_backward(
-            *_row(x), x_code, *_row(update), ptr(update_weight), ptr(scale), *_row(gate), gate_rows,
-            ptr(weight), keep, *_row(dtotal), *_row(dnormed), L.DTYPE_CODES[dtype], rows, width, eps,
-            ptr(dx), ptr(dupdate), ptr(dgate), ptr(dupdate_weight), ptr(dscale),
-            0 if weight is None else ptr(dweight), ptr(scratch), nbytes, s), device,
-            'bevpool_residual_norm_backward')
-        return dx, dupdate, dupdate_weight, dscale, dgate, dweight, None, None, None
-
-
-@functools.lru_cache(maxsize=256)
-def _backward_scratch(*sizes):
-    return L.library().bevpool_residual_norm_backward_scratch_bytes(*sizes)
+        return (*L.gradients().residual_norm_backward(dtotal, dnormed, *ctx.saved_tensors, *ctx.call),
+                None, None, None)
 
 
 def residual_norm(x, update=None, *, update_weight=None, scale=None, gate=None, weight=None,
@@ -218,12 +179,15 @@ def residual_norm(x, update=None, *, update_weight=None, scale=None, gate=None, 
         rows, groups = x.numel() // width, gate.shape[0]
         if groups < min(rows, 1) or groups and rows % groups:
             raise ValueError('the rows of gate must divide those of x.')
-    args = (_rows(x), None if update is None else _rows(update), update_weight, scale, gate, weight,
-            dtype, float(eps))
-    if _wants_grad(x, update, update_weight, scale, gate, weight) or _recorded():
-        total, normed = _ResidualNorm.apply(*args, keep)
+    args = (_rows(x), None if update is None else _rows(update), update_weight, scale, gate, weight)
+    eps = float(eps)
+    if _recorded():
+        total, normed = _ResidualNorm.apply(*args, dtype, eps, keep)
+    elif _wants_grad(*args):
+        total, normed, *kept = _residual_norm(*args, dtype, eps, keep)
+        L.gradients().record_residual_norm(total, normed, *args, *kept, dtype, eps, keep)
     else:
-        total, normed = _residual_norm(*args)[:2]
+        total, normed = _residual_norm(*args, dtype, eps)[:2]
     if len(shape) == 2:
         return x if total is None else total, normed
     return (x if total is None else total.view(shape),
@@ -243,6 +207,7 @@ def _gated(x, kind, keep=False):
 
 
 class _Gated(torch.autograd.Function):
+    """As _ResidualNorm."""
     @staticmethod
     def forward(ctx, x, kind, keep):
         out, kept = _gated(x, kind, keep)
@@ -251,17 +216,9 @@ class _Gated(torch.autograd.Function):
         return out
 
     @staticmethod
-    @once_differentiable  # (the gradients are no functions of the graph's)
+    @once_differentiable
     def backward(ctx, dout):
-        x, = ctx.saved_tensors
-        dtype, kind, keep = ctx.call
-        dout = _unit(dout if dout.dtype == dtype else dout.to(dtype))
-        rows, width = dout.shape
-        dx = dout.new_empty((rows, 2 * width))
-        _run(lambda lib, s: lib.bevpool_gated_backward(
-            *_row(x), int(keep), *_row(dout), L.DTYPE_CODES[dtype], rows, width, kind, L.ptr(dx),
-            s), dout.device, 'bevpool_gated_backward')
-        return dx, None, None
+        return *L.gradients().gated_activation_backward(dout, *ctx.saved_tensors, *ctx.call), None, None
 
 
 def gated_activation(x, kind='silu', *, checkpoint=None):
@@ -278,8 +235,11 @@ def gated_activation(x, kind='silu', *, checkpoint=None):
         raise ValueError(f'x must have shape [..., 2 width], width in [1, {MAX_GATED_WIDTH}].')
     P.require_gpu(x)
     rows, kind = _rows(x), ACTIVATIONS[kind]
-    if _wants_grad(x) or _recorded():
+    if _recorded():
         out = _Gated.apply(rows, kind, keep)
+    elif _wants_grad(x):
+        out, kept = _gated(rows, kind, keep)
+        L.gradients().record_gated_activation(out, rows, kept, kind)
     else:
         out = _gated(rows, kind)[0]
     return out if x.dim() == 2 else out.view(*x.shape[:-1], x.shape[-1] // 2)
@@ -332,23 +292,6 @@ def pack_activations(x):
     return PackedActivations(data, x.shape, x.dtype)
 
 
-def _weight_grad(dy, data, x_shape):
-    """dy^T x of the checkpoint of x."""
-    n, k = dy.shape[1], x_shape[1]
-    dweight = dy.new_empty((n, k))
-    nbytes = _weight_grad_scratch(dy.shape[0], n, k)
-    scratch = dy.new_empty(nbytes, dtype=torch.uint8)
-    _run(lambda lib, s: lib.bevpool_checkpoint_weight_grad(
-        *_row(dy), L.ptr(data), L.DTYPE_CODES[dy.dtype], dy.shape[0], n, k, L.ptr(dweight),
-        L.ptr(scratch), nbytes, s), dy.device, 'bevpool_checkpoint_weight_grad')
-    return dweight
-
-
-@functools.lru_cache(maxsize=256)
-def _weight_grad_scratch(*sizes):
-    return L.library().bevpool_checkpoint_weight_grad_scratch_bytes(*sizes)
-
-
 def _from_checkpoint(dtype, n, k):
     """Whether the gradient of a weight (n, k) is formed from the checkpoint
     itself: where it is so small that the tokens have to be divided over the
@@ -360,44 +303,31 @@ def _from_checkpoint(dtype, n, k):
             and -(-n // 256) * -(-k // 256) <= 128)
 
 
-def _column_sums(x):
-    dy = _unit(x)
-    out = dy.new_empty(dy.shape[1])
-    nbytes = L.library().bevpool_column_sums_scratch_bytes(dy.shape[1])
-    scratch = dy.new_empty(nbytes, dtype=torch.uint8)
-    _run(lambda lib, s: lib.bevpool_column_sums(
-        *_row(dy), L.DTYPE_CODES[dy.dtype], *dy.shape, L.ptr(out), L.ptr(scratch), nbytes, s),
-        dy.device, 'bevpool_column_sums')
-    return out
-
-
 class _CheckpointLinear(torch.autograd.Function):
+    """As _ResidualNorm."""
     @staticmethod
-    def forward(ctx, x, weight, bias):
+    def forward(ctx, x, weight, bias, direct):
         # (the weight's gradient alone needs x)
-        data = _pack(x) if ctx.needs_input_grad[1] else None
-        ctx.save_for_backward(data, weight)
-        ctx.call = (x.shape, x.dtype)
+        ctx.save_for_backward(_pack(x) if ctx.needs_input_grad[1] else None, weight)
+        ctx.call = (*x.shape, x.dtype, direct)
         return nn.functional.linear(x, weight, bias)
 
     @staticmethod
-    @once_differentiable  # (the gradients are no functions of the graph's)
+    @once_differentiable
     def backward(ctx, dy):
-        data, weight = ctx.saved_tensors
-        x_shape, dtype = ctx.call
-        dx = dweight = dbias = None
-        if ctx.needs_input_grad[0]:
-            dx = dy @ weight
-        if ctx.needs_input_grad[1]:
-            if dy.shape[0] and _from_checkpoint(dtype, dy.shape[1], x_shape[1]):
-                if dy.stride(1) != 1 or dy.stride(0) % 8 or dy.data_ptr() % 16 or dy.stride(0) >= 1 << 24:
-                    dy = dy.clone(memory_format=torch.contiguous_format)
-                dweight = _weight_grad(dy, data, x_shape)
-            else:
-                dweight = dy.t() @ PackedActivations(data, x_shape, dtype).unpack()
-        if ctx.needs_input_grad[2]:
-            dbias = _column_sums(dy)
-        return dx, dweight, dbias
+        return *L.gradients().checkpoint_linear_backward(dy, *ctx.saved_tensors, *ctx.call,
+                                                         *ctx.needs_input_grad[:3]), None
+
+
+def _checkpoint_linear(x, weight, bias):
+    direct = _from_checkpoint(x.dtype, *weight.shape)
+    if _recorded():
+        return _CheckpointLinear.apply(x, weight, bias, direct)
+    with torch.no_grad():
+        kept = _pack(x) if weight.requires_grad else None
+        y = nn.functional.linear(x, weight, bias)
+    L.gradients().record_checkpoint_linear(y, x, kept, weight, bias, direct)
+    return y
 
 
 def checkpoint_linear(x, weight, bias=None):
@@ -422,9 +352,9 @@ def checkpoint_linear(x, weight, bias=None):
         return nn.functional.linear(x, weight, bias)
     if autocast:  # (the operands have their types)
         with torch.autocast('cuda', enabled=False):
-            y = _CheckpointLinear.apply(_rows(x), weight, bias)
+            y = _checkpoint_linear(_rows(x), weight, bias)
     else:
-        y = _CheckpointLinear.apply(_rows(x), weight, bias)
+        y = _checkpoint_linear(_rows(x), weight, bias)
     return y if x.dim() == 2 else y.view(*x.shape[:-1], weight.shape[0])
 
 

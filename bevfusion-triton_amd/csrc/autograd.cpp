@@ -1,0 +1,298 @@
+// autograd.cpp -- the gradients of the block operators as nodes of torch's
+// autograd graph, in C++ beside the C ABI that they call.
+//
+// A training step on a few thousand tokens is bound by the host: the backward
+// pass runs on the autograd engine's thread, and in Python the interpreter's
+// objects go back and forth between two cores.  us of a step on a few tokens by
+// Python functions and by these nodes: residual_norm with all its operands 143
+// and 98, gated_activation 85 and 49, checkpoint_linear 165 and 115 (torch's own
+// linear 109).  The forward passes stay in Python; record_* hangs a node on their
+// results.  The *_backward functions are the nodes' bodies, for where Python
+// functions follow a call (traces).
+#include <ATen/ATen.h>
+#include <c10/hip/HIPStream.h>
+#include <torch/csrc/autograd/function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/functions/utils.h>
+#include <torch/csrc/autograd/saved_variable.h>
+#include <torch/csrc/utils/pybind.h>
+
+#include <mutex>
+#include <optional>
+#include <stdexcept>
+#include <string>
+
+#include "bevpool.h"
+
+namespace {
+
+using at::Tensor;
+using torch::autograd::Node;
+using torch::autograd::SavedVariable;
+using torch::autograd::variable_list;
+typedef std::optional<Tensor> Maybe;
+
+// ---- calls -----------------------------------------------------------------
+
+void check(int status, const char *what) {
+  if (status != BEVPOOL_OK)
+    throw std::runtime_error(std::string(what) + " failed (status " + std::to_string(status) +
+                             "): " + bevpool_last_error());
+}
+int code_of(at::ScalarType type) {
+  return type == at::kFloat ? BEVPOOL_F32 : type == at::kHalf ? BEVPOOL_F16 : BEVPOOL_BF16;
+}
+void *stream() { return c10::hip::getCurrentHIPStream().stream(); }
+void *at_of(const Tensor &t) { return t.defined() ? t.data_ptr() : nullptr; }
+int64_t row_of(const Tensor &t) { return t.defined() ? t.stride(0) : 0; }
+Tensor given(const Maybe &t) { return t.has_value() ? *t : Tensor(); }
+// rows of this type with unit stride along them
+Tensor rows_of(const Tensor &t, at::ScalarType type) {
+  Tensor r = t.scalar_type() == type ? t : t.to(type);
+  return r.stride(1) == 1 || r.size(1) == 1 ? r : r.contiguous();
+}
+Tensor bytes(const Tensor &like, size_t n) {
+  return at::empty({int64_t(n)}, like.options().dtype(at::kByte));
+}
+
+struct Residual {
+  int64_t rows, width;
+  at::ScalarType x_type, type;
+  double eps;
+  bool kept, has_update;
+};
+// Gradients of x, update, update_weight, scale, gate and weight.
+variable_list residual_backward(const Residual &R, Tensor dsum, Tensor dnormed, Tensor x,
+                                const Tensor &update, const Tensor &update_weight,
+                                const Tensor &scale, const Tensor &gate, Tensor weight) {
+  if (!dsum.defined() && !dnormed.defined()) return variable_list(6);
+  const auto options = (dsum.defined() ? dsum : dnormed).options();
+  const auto wide = options.dtype(R.x_type), own = options.dtype(R.type);
+  Tensor dweight;
+  if (weight.defined()) dweight = dnormed.defined() ? at::empty({R.width}, own) : at::zeros_like(weight);
+  if (dnormed.defined()) {
+    dnormed = rows_of(dnormed, R.type);
+  } else {
+    weight = Tensor();
+    x = Tensor();
+  }
+  if (dsum.defined()) dsum = rows_of(dsum, R.x_type);
+  Tensor dx = at::empty({R.rows, R.width}, wide), dupdate, dupdate_weight, dscale, dgate;
+  if (R.has_update) dupdate = at::empty({R.rows, R.width}, own);
+  if (update_weight.defined()) dupdate_weight = at::empty({R.width}, own);
+  if (scale.defined()) dscale = at::empty({R.width}, own);
+  const int64_t gate_rows = gate.defined() ? gate.size(0) : 0;
+  // (no kernel writes the sums of no rows)
+  if (gate.defined()) dgate = R.rows ? at::empty({gate_rows, R.width}, own) : at::zeros_like(gate);
+  const int width = int(R.width), x_code = code_of(R.x_type);
+  const size_t need =
+      bevpool_residual_norm_backward_scratch_bytes(R.rows, width, gate_rows, x_code, R.kept);
+  const Tensor scratch = bytes(dx, need);
+  check(bevpool_residual_norm_backward(
+            at_of(x), row_of(x), x_code, at_of(update), row_of(update), at_of(update_weight),
+            at_of(scale), at_of(gate), row_of(gate), gate_rows, at_of(weight), R.kept, at_of(dsum),
+            row_of(dsum), at_of(dnormed), row_of(dnormed), code_of(R.type), R.rows, width,
+            float(R.eps), at_of(dx), at_of(dupdate), at_of(dgate), at_of(dupdate_weight),
+            at_of(dscale), weight.defined() ? at_of(dweight) : nullptr, at_of(scratch), need,
+            stream()),
+        "bevpool_residual_norm_backward");
+  return {dx, dupdate, dupdate_weight, dscale, dgate, dweight};
+}
+
+struct Gated {
+  at::ScalarType type;
+  int kind;
+  bool kept;
+};
+variable_list gated_backward(const Gated &G, Tensor dout, const Tensor &x) {
+  if (!dout.defined()) return variable_list(1);
+  dout = rows_of(dout, G.type);
+  const int64_t rows = dout.size(0), width = dout.size(1);
+  const Tensor dx = at::empty({rows, 2 * width}, dout.options());
+  check(bevpool_gated_backward(at_of(x), row_of(x), G.kept, at_of(dout), row_of(dout),
+                               code_of(G.type), rows, int(width), G.kind, at_of(dx), stream()),
+        "bevpool_gated_backward");
+  return {dx};
+}
+
+struct Linear {
+  int64_t rows, width;
+  at::ScalarType type;
+  bool direct;  // the weight's gradient from the checkpoint itself
+};
+// Gradients of x, weight and bias, those that are needed.
+variable_list linear_backward(const Linear &A, const Tensor &dy, const Tensor &kept,
+                              const Tensor &weight, bool need_x, bool need_weight, bool need_bias) {
+  variable_list grads(3);
+  if (!dy.defined()) return grads;
+  const int n = int(weight.size(0)), k = int(A.width), code = code_of(A.type);
+  if (need_x) grads[0] = dy.mm(weight);
+  if (need_weight && A.direct && A.rows) {
+    Tensor rows = dy;
+    if (dy.stride(1) != 1 || dy.stride(0) % 8 || reinterpret_cast<uintptr_t>(dy.data_ptr()) % 16 ||
+        dy.stride(0) >= (1 << 24))
+      rows = dy.clone(at::MemoryFormat::Contiguous);
+    grads[1] = at::empty({n, k}, dy.options());
+    const size_t need = bevpool_checkpoint_weight_grad_scratch_bytes(A.rows, n, k);
+    const Tensor scratch = bytes(dy, need);
+    check(bevpool_checkpoint_weight_grad(at_of(rows), row_of(rows), at_of(kept), code, A.rows, n, k,
+                                         at_of(grads[1]), at_of(scratch), need, stream()),
+          "bevpool_checkpoint_weight_grad");
+  } else if (need_weight) {
+    const Tensor x = at::empty({A.rows, A.width}, dy.options());
+    check(bevpool_checkpoint_unpack(at_of(kept), code, A.rows, k, at_of(x), stream()),
+          "bevpool_checkpoint_unpack");
+    grads[1] = dy.t().mm(x);
+  }
+  if (need_bias) {
+    const Tensor rows = rows_of(dy, A.type);
+    grads[2] = at::empty({n}, dy.options());
+    const size_t need = bevpool_column_sums_scratch_bytes(n);
+    const Tensor scratch = bytes(dy, need);
+    check(bevpool_column_sums(at_of(rows), row_of(rows), code, A.rows, n, at_of(grads[2]),
+                              at_of(scratch), need, stream()),
+          "bevpool_column_sums");
+  }
+  return grads;
+}
+
+// ---- nodes -----------------------------------------------------------------
+
+// A node keeps tensors; its body gets them back.  Gradients are no functions of
+// the graph's: a second derivative is refused.
+template <int kSaved>
+struct Recorded : public Node {
+  SavedVariable saved[kSaved];
+  void release_variables() override {
+    std::lock_guard<std::mutex> lock(mutex_);
+    for (SavedVariable &s : saved) s.reset_data();
+  }
+  virtual variable_list body(variable_list &&grads, const variable_list &kept) = 0;
+  variable_list apply(variable_list &&grads) override {
+    std::lock_guard<std::mutex> lock(mutex_);
+    variable_list kept;
+    kept.reserve(kSaved);
+    for (const SavedVariable &s : saved) kept.push_back(s.unpack());
+    const bool followed = at::GradMode::is_enabled();
+    variable_list out;
+    {
+      const at::NoGradGuard none;
+      out = body(std::move(grads), kept);
+    }
+    if (!followed) return out;
+    for (Tensor &t : out)
+      if (t.defined()) t = t.detach().set_requires_grad(true);
+    torch::autograd::DelayedError refusal(
+        "a second derivative of " + name() + " was asked for, which it does not have",
+        int64_t(out.size()));
+    return refusal.apply(std::move(out));
+  }
+};
+template <typename N, typename... Inputs>
+std::shared_ptr<N> node_of(const Inputs &...inputs) {
+  std::shared_ptr<N> node(new N(), torch::autograd::deleteNode);
+  node->set_next_edges(torch::autograd::collect_next_edges(inputs...));
+  return node;
+}
+
+struct ResidualNode : public Recorded<6> {
+  Residual call;
+  std::string name() const override { return "residual_norm"; }
+  variable_list body(variable_list &&g, const variable_list &s) override {
+    return residual_backward(call, g[0], g[1], s[0], s[1], s[2], s[3], s[4], s[5]);
+  }
+};
+struct GatedNode : public Recorded<1> {
+  Gated call;
+  std::string name() const override { return "gated_activation"; }
+  variable_list body(variable_list &&g, const variable_list &s) override {
+    return gated_backward(call, g[0], s[0]);
+  }
+};
+struct LinearNode : public Recorded<2> {
+  Linear call;
+  std::string name() const override { return "checkpoint_linear"; }
+  variable_list body(variable_list &&g, const variable_list &s) override {
+    return linear_backward(call, g[0], s[0], s[1], task_should_compute_output(0),
+                           task_should_compute_output(1), task_should_compute_output(2));
+  }
+};
+
+// ---- for Python ------------------------------------------------------------
+
+Residual residual_call(int64_t rows, int64_t width, at::ScalarType x_type, at::ScalarType type,
+                       double eps, bool kept, bool has_update) {
+  return {rows, width, x_type, type, eps, kept, has_update};
+}
+
+void record_residual_norm(const Maybe &sum, const Maybe &normed, const Tensor &x, const Maybe &update,
+                          const Maybe &update_weight, const Maybe &scale, const Maybe &gate,
+                          const Maybe &weight, const Maybe &x_kept, const Maybe &update_kept,
+                          at::ScalarType type, double eps, bool kept) {
+  const Tensor u = given(update), uw = given(update_weight), s = given(scale), g = given(gate),
+               w = given(weight);
+  auto node = node_of<ResidualNode>(x, u, uw, s, g, w);
+  node->call = residual_call(x.size(0), x.size(1), x.scalar_type(), type, eps, kept, u.defined());
+  // (without weight x is not needed)
+  const Tensor saved[6] = {!w.defined() ? Tensor() : kept ? given(x_kept) : x,
+                           kept ? given(update_kept) : u, uw, s, g, w};
+  for (int i = 0; i < 6; ++i) node->saved[i] = SavedVariable(saved[i], false);
+  torch::autograd::set_history(given(sum), node);
+  torch::autograd::set_history(given(normed), node);
+}
+
+void record_gated_activation(const Tensor &out, const Tensor &x, const Maybe &kept, int kind) {
+  auto node = node_of<GatedNode>(x);
+  node->call = {x.scalar_type(), kind, kept.has_value()};
+  node->saved[0] = SavedVariable(kept.has_value() ? *kept : x, false);
+  torch::autograd::set_history(out, node);
+}
+
+void record_checkpoint_linear(const Tensor &out, const Tensor &x, const Maybe &kept,
+                              const Tensor &weight, const Maybe &bias, bool direct) {
+  const Tensor b = given(bias);
+  auto node = node_of<LinearNode>(x, weight, b);
+  node->call = {x.size(0), x.size(1), x.scalar_type(), direct};
+  node->saved[0] = SavedVariable(given(kept), false);
+  node->saved[1] = SavedVariable(weight, false);
+  torch::autograd::set_history(out, node);
+}
+
+std::vector<Maybe> maybe(const variable_list &grads) {
+  std::vector<Maybe> out;
+  for (const Tensor &t : grads) out.push_back(t.defined() ? Maybe(t) : std::nullopt);
+  return out;
+}
+
+}  // namespace
+
+PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
+  namespace py = pybind11;
+  typedef py::call_guard<py::gil_scoped_release> Free;
+  m.def("record_residual_norm", &record_residual_norm, Free());
+  m.def("record_gated_activation", &record_gated_activation, Free());
+  m.def("record_checkpoint_linear", &record_checkpoint_linear, Free());
+  m.def("residual_norm_backward",
+        [](const Maybe &dsum, const Maybe &dnormed, const Maybe &x, const Maybe &update,
+           const Maybe &update_weight, const Maybe &scale, const Maybe &gate, const Maybe &weight,
+           int64_t rows, int64_t width, at::ScalarType x_type, at::ScalarType type, double eps,
+           bool kept, bool has_update) {
+          return maybe(residual_backward(
+              residual_call(rows, width, x_type, type, eps, kept, has_update), given(dsum),
+              given(dnormed), given(x), given(update), given(update_weight), given(scale),
+              given(gate), given(weight)));
+        },
+        Free());
+  m.def("gated_activation_backward",
+        [](const Tensor &dout, const Tensor &x, at::ScalarType type, int kind, bool kept) {
+          return maybe(gated_backward({type, kind, kept}, dout, x));
+        },
+        Free());
+  m.def("checkpoint_linear_backward",
+        [](const Tensor &dy, const Maybe &kept, const Tensor &weight, int64_t rows, int64_t width,
+           at::ScalarType type, bool direct, bool need_x, bool need_weight, bool need_bias) {
+          return maybe(linear_backward({rows, width, type, direct}, dy, given(kept), weight, need_x,
+                                       need_weight, need_bias));
+        },
+        Free());
+}
