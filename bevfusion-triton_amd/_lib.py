@@ -19,7 +19,7 @@ from pathlib import Path
 import torch  # noqa: F401  (loads the HIP runtime first; see module docstring)
 
 LIB_PATH = Path(__file__).resolve().parent / 'libbevpool_amd.so'
-GRADIENTS_PATH = LIB_PATH.with_name('_autograd.so')
+BLOCK_CALLS_PATH = LIB_PATH.with_name('_block_calls.so')
 ABI_VERSION = 4
 
 F32, F16, BF16 = 0, 1, 2
@@ -206,7 +206,7 @@ _SIGNATURES = {
 EXPORTED_SYMBOLS = tuple(_SIGNATURES)
 
 _lib = None
-_gradients = None
+_block_module = None
 
 
 def library():
@@ -234,25 +234,27 @@ def library():
     return lib
 
 
-def gradients():
-    """The autograd nodes of csrc/autograd.cpp (loaded once)."""
-    global _gradients
-    if _gradients is None:
+def block_calls():
+    """The block operators on tensors, with the nodes of their gradients
+    (csrc/block_calls.cpp; loaded once)."""
+    global _block_module
+    if _block_module is None:
         library()
-        if not GRADIENTS_PATH.exists():
+        if not BLOCK_CALLS_PATH.exists():
             raise LibraryNotBuilt(
-                f'{GRADIENTS_PATH} is missing: build it with `python -c "import __graft_entry__ as g; '
+                f'{BLOCK_CALLS_PATH} is missing: build it with `python -c "import __graft_entry__ as g; '
                 f'g.build()"` (or `make -C bevfusion-triton_amd/csrc`)'
             )
-        loader = importlib.machinery.ExtensionFileLoader('_autograd', str(GRADIENTS_PATH))
-        spec = importlib.util.spec_from_loader('_autograd', loader)
+        loader = importlib.machinery.ExtensionFileLoader('_block_calls', str(BLOCK_CALLS_PATH))
+        spec = importlib.util.spec_from_loader('_block_calls', loader)
         try:
             module = importlib.util.module_from_spec(spec)
             loader.exec_module(module)
         except ImportError as exc:  # (another torch than it was built with)
-            raise LibraryNotBuilt(f'cannot load {GRADIENTS_PATH}: {exc}') from exc
-        _gradients = module
-    return _gradients
+            raise LibraryNotBuilt(f'cannot load {BLOCK_CALLS_PATH}: {exc}') from exc
+        module.errors_are(BevPoolError)
+        _block_module = module
+    return _block_module
 
 
 def check(status: int, what: str) -> None:

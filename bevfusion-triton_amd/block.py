@@ -76,38 +76,15 @@ def _check_checkpoint(checkpoint):
     return checkpoint is not None
 
 
-def _kept(x, rows, width, copies=1):
-    """Room for an 8-bit checkpoint of rows."""
-    pitch = L.library().bevpool_checkpoint_pitch(width)
-    return x.new_empty((rows, copies * pitch), dtype=torch.uint8)
-
-
 # ---- residual and norms ----------------------------------------------------
 
-def _residual_norm(x, update, update_weight, scale, gate, weight, dtype, eps, keep=False):
-    """(sum, normed, checkpoint of x, of update) of rows."""
-    rows, width = x.shape
-    total = None if update is None else torch.empty_like(x, memory_format=torch.contiguous_format)
-    normed = None if weight is None else x.new_empty(x.shape, dtype=dtype)
-    # (the norm before the next block alone needs x for its gradient)
-    x_kept = _kept(x, rows, width) if keep and weight is not None else None
-    update_kept = _kept(x, rows, width) if keep and update is not None else None
-    _run(lambda lib, s: lib.bevpool_residual_norm_forward(
-        *_row(x), L.DTYPE_CODES[x.dtype], *_row(update), L.ptr(update_weight), L.ptr(scale),
-        *_row(gate), 0 if gate is None else gate.shape[0], L.ptr(weight), L.DTYPE_CODES[dtype], rows,
-        width, eps, L.ptr(total),
-        L.ptr(normed), L.ptr(x_kept), L.ptr(update_kept), s), x.device,
-        'bevpool_residual_norm_forward')
-    return total, normed, x_kept, update_kept
-
-
 class _ResidualNorm(torch.autograd.Function):
-    """For traces, and to refuse tangents; csrc/autograd.cpp has the node that
+    """For traces, and to refuse tangents; csrc/block_calls.cpp has the node that
     follows other calls."""
     @staticmethod
     def forward(ctx, x, update, update_weight, scale, gate, weight, dtype, eps, keep):
-        total, normed, x_kept, update_kept = _residual_norm(x, update, update_weight, scale, gate,
-                                                            weight, dtype, eps, keep)
+        total, normed, x_kept, update_kept = L.block_calls().residual_norm_forward(
+            x, update, update_weight, scale, gate, weight, dtype, eps, keep)
         if not keep:
             x_kept, update_kept = x if weight is not None else None, update
         ctx.save_for_backward(x_kept, update_kept, update_weight, scale, gate, weight)
@@ -118,7 +95,7 @@ class _ResidualNorm(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, dtotal, dnormed):
-        return (*L.gradients().residual_norm_backward(dtotal, dnormed, *ctx.saved_tensors, *ctx.call),
+        return (*L.block_calls().residual_norm_backward(dtotal, dnormed, *ctx.saved_tensors, *ctx.call),
                 None, None, None)
 
 
@@ -179,15 +156,12 @@ def residual_norm(x, update=None, *, update_weight=None, scale=None, gate=None, 
         rows, groups = x.numel() // width, gate.shape[0]
         if groups < min(rows, 1) or groups and rows % groups:
             raise ValueError('the rows of gate must divide those of x.')
-    args = (_rows(x), None if update is None else _rows(update), update_weight, scale, gate, weight)
-    eps = float(eps)
+    args = (_rows(x), None if update is None else _rows(update), update_weight, scale, gate, weight,
+            dtype, float(eps))
     if _recorded():
-        total, normed = _ResidualNorm.apply(*args, dtype, eps, keep)
-    elif _wants_grad(*args):
-        total, normed, *kept = _residual_norm(*args, dtype, eps, keep)
-        L.gradients().record_residual_norm(total, normed, *args, *kept, dtype, eps, keep)
+        total, normed = _ResidualNorm.apply(*args, keep)
     else:
-        total, normed = _residual_norm(*args, dtype, eps)[:2]
+        total, normed = L.block_calls().residual_norm(*args, keep, _wants_grad(*args[:6]))
     if len(shape) == 2:
         return x if total is None else total, normed
     return (x if total is None else total.view(shape),
@@ -196,21 +170,11 @@ def residual_norm(x, update=None, *, update_weight=None, scale=None, gate=None, 
 
 # ---- gated activation ------------------------------------------------------
 
-def _gated(x, kind, keep=False):
-    rows, width = x.shape[0], x.shape[1] // 2
-    out = x.new_empty((rows, width))
-    kept = _kept(x, rows, width, 2) if keep else None
-    _run(lambda lib, s: lib.bevpool_gated_forward(
-        *_row(x), L.DTYPE_CODES[x.dtype], rows, width, kind, L.ptr(out), L.ptr(kept), s),
-        x.device, 'bevpool_gated_forward')
-    return out, kept
-
-
 class _Gated(torch.autograd.Function):
     """As _ResidualNorm."""
     @staticmethod
     def forward(ctx, x, kind, keep):
-        out, kept = _gated(x, kind, keep)
+        out, kept = L.block_calls().gated_activation_forward(x, kind, keep)
         ctx.save_for_backward(kept if keep else x)
         ctx.call = (x.dtype, kind, keep)
         return out
@@ -218,7 +182,7 @@ class _Gated(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, dout):
-        return *L.gradients().gated_activation_backward(dout, *ctx.saved_tensors, *ctx.call), None, None
+        return *L.block_calls().gated_activation_backward(dout, *ctx.saved_tensors, *ctx.call), None, None
 
 
 def gated_activation(x, kind='silu', *, checkpoint=None):
@@ -237,11 +201,8 @@ def gated_activation(x, kind='silu', *, checkpoint=None):
     rows, kind = _rows(x), ACTIVATIONS[kind]
     if _recorded():
         out = _Gated.apply(rows, kind, keep)
-    elif _wants_grad(x):
-        out, kept = _gated(rows, kind, keep)
-        L.gradients().record_gated_activation(out, rows, kept, kind)
     else:
-        out = _gated(rows, kind)[0]
+        out = L.block_calls().gated_activation(rows, kind, keep, _wants_grad(x))
     return out if x.dim() == 2 else out.view(*x.shape[:-1], x.shape[-1] // 2)
 
 
@@ -263,12 +224,7 @@ class PackedActivations:
 
 
 def _pack(x):
-    rows = _rows(x)
-    data = _kept(rows, *rows.shape)
-    _run(lambda lib, s: lib.bevpool_checkpoint_pack(
-        *_row(rows), L.DTYPE_CODES[x.dtype], *rows.shape, L.ptr(data), s), x.device,
-        'bevpool_checkpoint_pack')
-    return data
+    return L.block_calls().pack(_rows(x))
 
 
 class _Pack(torch.autograd.Function):
@@ -315,7 +271,7 @@ class _CheckpointLinear(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
-        return *L.gradients().checkpoint_linear_backward(dy, *ctx.saved_tensors, *ctx.call,
+        return *L.block_calls().checkpoint_linear_backward(dy, *ctx.saved_tensors, *ctx.call,
                                                          *ctx.needs_input_grad[:3]), None
 
 
@@ -323,11 +279,7 @@ def _checkpoint_linear(x, weight, bias):
     direct = _from_checkpoint(x.dtype, *weight.shape)
     if _recorded():
         return _CheckpointLinear.apply(x, weight, bias, direct)
-    with torch.no_grad():
-        kept = _pack(x) if weight.requires_grad else None
-        y = nn.functional.linear(x, weight, bias)
-    L.gradients().record_checkpoint_linear(y, x, kept, weight, bias, direct)
-    return y
+    return L.block_calls().checkpoint_linear(x, weight, bias, direct)
 
 
 def checkpoint_linear(x, weight, bias=None):
@@ -404,22 +356,11 @@ def _code_rows(codes):
     return copy, need
 
 
-def _linear_int8(x, codes, row, scales, bias):
-    (rows, width), channels = x.shape, scales.shape[0]
-    y = x.new_empty((rows, channels))
-    nbytes = L.library().bevpool_linear8_scratch_bytes(rows, width)
-    scratch = x.new_empty(nbytes, dtype=torch.uint8)
-    _run(lambda lib, s: lib.bevpool_linear8(
-        *_row(x), L.DTYPE_CODES[x.dtype], L.ptr(codes), row, L.ptr(scales), L.ptr(bias), rows,
-        width, channels, L.ptr(y), L.ptr(scratch), nbytes, s), x.device, 'bevpool_linear8')
-    return y
-
-
 class _LinearInt8(torch.autograd.Function):
     """For tangents and traces alone: there is no gradient."""
     @staticmethod
     def forward(ctx, x, codes, row, scales, bias):
-        return _linear_int8(x, codes, row, scales, bias)
+        return L.block_calls().linear_int8(x, codes, row, scales, bias)
 
 
 def linear_int8(x, codes, scales, bias=None):
@@ -451,7 +392,7 @@ def linear_int8(x, codes, scales, bias=None):
     if _wants_grad(x, scales, bias):
         raise RuntimeError('linear_int8 has no gradient; call it under torch.no_grad()')
     codes, row = _code_rows(codes) if channels else (codes, 0)
-    run = _LinearInt8.apply if _recorded() else _linear_int8
+    run = _LinearInt8.apply if _recorded() else L.block_calls().linear_int8
     y = run(_rows(x), codes, int(row), scales, bias)  # (a trace has sizes as tensors)
     return y if x.dim() == 2 else y.view(*x.shape[:-1], channels)
 

@@ -1,15 +1,19 @@
-// autograd.cpp -- the gradients of the block operators as nodes of torch's
-// autograd graph, in C++ beside the C ABI that they call.
+// block_calls.cpp -- the block operators as functions of tensors, and their
+// gradients as nodes of torch's autograd graph, in C++ beside the C ABI that
+// they call.  Arguments are checked in Python (block.py).
 //
-// A training step on a few thousand tokens is bound by the host: the backward
-// pass runs on the autograd engine's thread, and in Python the interpreter's
-// objects go back and forth between two cores.  us of a step on a few tokens by
-// Python functions and by these nodes: residual_norm with all its operands 143
-// and 98, gated_activation 85 and 49, checkpoint_linear 165 and 115 (torch's own
-// linear 109).  The forward passes stay in Python; record_* hangs a node on their
-// results.  The *_backward functions are the nodes' bodies, for where Python
-// functions follow a call (traces).
+// A call on a few tokens is bound by the host, and so is a training step on a
+// few thousand: the backward pass runs on the autograd engine's thread, and in
+// Python the interpreter's objects go back and forth between two cores.  us of a
+// step on a few tokens by Python functions over ctypes and by this: residual_norm
+// with all its operands 143 and 87, gated_activation 85 and 44, checkpoint_linear
+// 165 and 98 (torch's own linear 102); of a call without gradients 12.5 and 9.1,
+// 7.7 and 5.8, linear_int8 10.7 and 7.6.
+//
+// What is not followed by a gradient's node is followed by a Python function
+// (traces, tangents), which calls the *_forward and *_backward here.
 #include <ATen/ATen.h>
+#include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
@@ -34,18 +38,28 @@ typedef std::optional<Tensor> Maybe;
 
 // ---- calls -----------------------------------------------------------------
 
+struct CallError : public std::runtime_error {
+  using std::runtime_error::runtime_error;
+};
+PyObject *call_error = nullptr;  // what Python sees of it
 void check(int status, const char *what) {
   if (status != BEVPOOL_OK)
-    throw std::runtime_error(std::string(what) + " failed (status " + std::to_string(status) +
+    throw CallError(std::string(what) + " failed (status " + std::to_string(status) +
                              "): " + bevpool_last_error());
 }
 int code_of(at::ScalarType type) {
   return type == at::kFloat ? BEVPOOL_F32 : type == at::kHalf ? BEVPOOL_F16 : BEVPOOL_BF16;
 }
-void *stream() { return c10::hip::getCurrentHIPStream().stream(); }
+void *stream() { return c10::hip::getCurrentHIPStream().stream(); }  // of the current device
 void *at_of(const Tensor &t) { return t.defined() ? t.data_ptr() : nullptr; }
 int64_t row_of(const Tensor &t) { return t.defined() ? t.stride(0) : 0; }
 Tensor given(const Maybe &t) { return t.has_value() ? *t : Tensor(); }
+Maybe maybe(const Tensor &t) { return t.defined() ? Maybe(t) : std::nullopt; }
+std::vector<Maybe> maybe(const variable_list &tensors) {
+  std::vector<Maybe> out;
+  for (const Tensor &t : tensors) out.push_back(maybe(t));
+  return out;
+}
 // rows of this type with unit stride along them
 Tensor rows_of(const Tensor &t, at::ScalarType type) {
   Tensor r = t.scalar_type() == type ? t : t.to(type);
@@ -53,6 +67,33 @@ Tensor rows_of(const Tensor &t, at::ScalarType type) {
 }
 Tensor bytes(const Tensor &like, size_t n) {
   return at::empty({int64_t(n)}, like.options().dtype(at::kByte));
+}
+
+// room for an 8-bit checkpoint of rows
+Tensor kept_rows(const Tensor &x, int64_t rows, int64_t width, int copies = 1) {
+  return at::empty({rows, copies * bevpool_checkpoint_pitch(int(width))},
+                   x.options().dtype(at::kByte));
+}
+
+// Sum and normed of rows, and the checkpoints of x and update.
+variable_list residual_forward(const Tensor &x, const Tensor &update, const Tensor &update_weight,
+                               const Tensor &scale, const Tensor &gate, const Tensor &weight,
+                               at::ScalarType type, double eps, bool keep) {
+  const c10::DeviceGuard device(x.device());
+  const int64_t rows = x.size(0), width = x.size(1);
+  Tensor sum, normed, x_kept, update_kept;
+  if (update.defined()) sum = at::empty({rows, width}, x.options());
+  if (weight.defined()) normed = at::empty({rows, width}, x.options().dtype(type));
+  // (the norm before the next block alone needs x for its gradient)
+  if (keep && weight.defined()) x_kept = kept_rows(x, rows, width);
+  if (keep && update.defined()) update_kept = kept_rows(x, rows, width);
+  check(bevpool_residual_norm_forward(
+            at_of(x), row_of(x), code_of(x.scalar_type()), at_of(update), row_of(update),
+            at_of(update_weight), at_of(scale), at_of(gate), row_of(gate),
+            gate.defined() ? gate.size(0) : 0, at_of(weight), code_of(type), rows, int(width),
+            float(eps), at_of(sum), at_of(normed), at_of(x_kept), at_of(update_kept), stream()),
+        "bevpool_residual_norm_forward");
+  return {sum, normed, x_kept, update_kept};
 }
 
 struct Residual {
@@ -99,6 +140,19 @@ variable_list residual_backward(const Residual &R, Tensor dsum, Tensor dnormed, 
   return {dx, dupdate, dupdate_weight, dscale, dgate, dweight};
 }
 
+// The activation and the checkpoint.
+variable_list gated_forward(const Tensor &x, int kind, bool keep) {
+  const c10::DeviceGuard device(x.device());
+  const int64_t rows = x.size(0), width = x.size(1) / 2;
+  const Tensor out = at::empty({rows, width}, x.options());
+  Tensor kept;
+  if (keep) kept = kept_rows(x, rows, width, 2);
+  check(bevpool_gated_forward(at_of(x), row_of(x), code_of(x.scalar_type()), rows, int(width), kind,
+                              at_of(out), at_of(kept), stream()),
+        "bevpool_gated_forward");
+  return {out, kept};
+}
+
 struct Gated {
   at::ScalarType type;
   int kind;
@@ -113,6 +167,30 @@ variable_list gated_backward(const Gated &G, Tensor dout, const Tensor &x) {
                                code_of(G.type), rows, int(width), G.kind, at_of(dx), stream()),
         "bevpool_gated_backward");
   return {dx};
+}
+
+Tensor pack(const Tensor &x) {
+  const c10::DeviceGuard device(x.device());
+  const Tensor kept = kept_rows(x, x.size(0), x.size(1));
+  check(bevpool_checkpoint_pack(at_of(x), row_of(x), code_of(x.scalar_type()), x.size(0),
+                                int(x.size(1)), at_of(kept), stream()),
+        "bevpool_checkpoint_pack");
+  return kept;
+}
+
+Tensor linear8(const Tensor &x, const Tensor &codes, int64_t row, const Tensor &scales,
+               const Tensor &bias) {
+  const c10::DeviceGuard device(x.device());
+  const int64_t rows = x.size(0), channels = scales.size(0);
+  const int width = int(x.size(1));
+  const Tensor y = at::empty({rows, channels}, x.options());
+  const size_t need = bevpool_linear8_scratch_bytes(rows, width);
+  const Tensor scratch = bytes(x, need);
+  check(bevpool_linear8(at_of(x), row_of(x), code_of(x.scalar_type()), at_of(codes), row,
+                        at_of(scales), at_of(bias), rows, width, channels, at_of(y), at_of(scratch),
+                        need, stream()),
+        "bevpool_linear8");
+  return y;
 }
 
 struct Linear {
@@ -218,49 +296,51 @@ struct LinearNode : public Recorded<2> {
   }
 };
 
-// ---- for Python ------------------------------------------------------------
+// ---- calls with their nodes, and what Python calls ------------------------------------------------------------
 
-Residual residual_call(int64_t rows, int64_t width, at::ScalarType x_type, at::ScalarType type,
-                       double eps, bool kept, bool has_update) {
-  return {rows, width, x_type, type, eps, kept, has_update};
-}
-
-void record_residual_norm(const Maybe &sum, const Maybe &normed, const Tensor &x, const Maybe &update,
-                          const Maybe &update_weight, const Maybe &scale, const Maybe &gate,
-                          const Maybe &weight, const Maybe &x_kept, const Maybe &update_kept,
-                          at::ScalarType type, double eps, bool kept) {
+std::pair<Maybe, Maybe> residual_norm(const Tensor &x, const Maybe &update, const Maybe &update_weight,
+                                      const Maybe &scale, const Maybe &gate, const Maybe &weight,
+                                      at::ScalarType type, double eps, bool keep, bool follow) {
   const Tensor u = given(update), uw = given(update_weight), s = given(scale), g = given(gate),
                w = given(weight);
-  auto node = node_of<ResidualNode>(x, u, uw, s, g, w);
-  node->call = residual_call(x.size(0), x.size(1), x.scalar_type(), type, eps, kept, u.defined());
-  // (without weight x is not needed)
-  const Tensor saved[6] = {!w.defined() ? Tensor() : kept ? given(x_kept) : x,
-                           kept ? given(update_kept) : u, uw, s, g, w};
-  for (int i = 0; i < 6; ++i) node->saved[i] = SavedVariable(saved[i], false);
-  torch::autograd::set_history(given(sum), node);
-  torch::autograd::set_history(given(normed), node);
+  const variable_list out = residual_forward(x, u, uw, s, g, w, type, eps, keep && follow);
+  if (follow) {
+    auto node = node_of<ResidualNode>(x, u, uw, s, g, w);
+    node->call = {x.size(0), x.size(1), x.scalar_type(), type, eps, keep, u.defined()};
+    // (without weight x is not needed)
+    const Tensor saved[6] = {!w.defined() ? Tensor() : keep ? out[2] : x, keep ? out[3] : u,
+                             uw, s, g, w};
+    for (int i = 0; i < 6; ++i) node->saved[i] = SavedVariable(saved[i], false);
+    torch::autograd::set_history(out[0], node);
+    torch::autograd::set_history(out[1], node);
+  }
+  return {maybe(out[0]), maybe(out[1])};
 }
 
-void record_gated_activation(const Tensor &out, const Tensor &x, const Maybe &kept, int kind) {
-  auto node = node_of<GatedNode>(x);
-  node->call = {x.scalar_type(), kind, kept.has_value()};
-  node->saved[0] = SavedVariable(kept.has_value() ? *kept : x, false);
-  torch::autograd::set_history(out, node);
+Tensor gated_activation(const Tensor &x, int kind, bool keep, bool follow) {
+  const variable_list out = gated_forward(x, kind, keep && follow);
+  if (follow) {
+    auto node = node_of<GatedNode>(x);
+    node->call = {x.scalar_type(), kind, keep};
+    node->saved[0] = SavedVariable(keep ? out[1] : x, false);
+    torch::autograd::set_history(out[0], node);
+  }
+  return out[0];
 }
 
-void record_checkpoint_linear(const Tensor &out, const Tensor &x, const Maybe &kept,
-                              const Tensor &weight, const Maybe &bias, bool direct) {
+Tensor checkpoint_linear(const Tensor &x, const Tensor &weight, const Maybe &bias, bool direct) {
   const Tensor b = given(bias);
   auto node = node_of<LinearNode>(x, weight, b);
   node->call = {x.size(0), x.size(1), x.scalar_type(), direct};
-  node->saved[0] = SavedVariable(given(kept), false);
+  // (the weight's gradient alone needs x)
+  node->saved[0] = SavedVariable(weight.requires_grad() ? pack(x) : Tensor(), false);
   node->saved[1] = SavedVariable(weight, false);
+  Tensor out;
+  {
+    const at::NoGradGuard none;
+    out = at::linear(x, weight, bias);
+  }
   torch::autograd::set_history(out, node);
-}
-
-std::vector<Maybe> maybe(const variable_list &grads) {
-  std::vector<Maybe> out;
-  for (const Tensor &t : grads) out.push_back(t.defined() ? Maybe(t) : std::nullopt);
   return out;
 }
 
@@ -269,18 +349,41 @@ std::vector<Maybe> maybe(const variable_list &grads) {
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   namespace py = pybind11;
   typedef py::call_guard<py::gil_scoped_release> Free;
-  m.def("record_residual_norm", &record_residual_norm, Free());
-  m.def("record_gated_activation", &record_gated_activation, Free());
-  m.def("record_checkpoint_linear", &record_checkpoint_linear, Free());
+  m.def("errors_are", [](py::object type) { call_error = type.release().ptr(); });
+  py::register_exception_translator([](std::exception_ptr e) {
+    try {
+      if (e) std::rethrow_exception(e);
+    } catch (const CallError &error) {
+      PyErr_SetString(call_error ? call_error : PyExc_RuntimeError, error.what());
+    }
+  });
+  m.def("residual_norm", &residual_norm, Free());
+  m.def("gated_activation", &gated_activation, Free());
+  m.def("checkpoint_linear", &checkpoint_linear, Free());
+  m.def("pack", &pack, Free());
+  m.def("linear_int8",
+        [](const Tensor &x, const Tensor &codes, int64_t row, const Tensor &scales,
+           const Maybe &bias) { return linear8(x, codes, row, scales, given(bias)); },
+        Free());
+  m.def("residual_norm_forward",
+        [](const Tensor &x, const Maybe &update, const Maybe &update_weight, const Maybe &scale,
+           const Maybe &gate, const Maybe &weight, at::ScalarType type, double eps, bool keep) {
+          return maybe(residual_forward(x, given(update), given(update_weight), given(scale),
+                                        given(gate), given(weight), type, eps, keep));
+        },
+        Free());
+  m.def("gated_activation_forward",
+        [](const Tensor &x, int kind, bool keep) { return maybe(gated_forward(x, kind, keep)); },
+        Free());
   m.def("residual_norm_backward",
         [](const Maybe &dsum, const Maybe &dnormed, const Maybe &x, const Maybe &update,
            const Maybe &update_weight, const Maybe &scale, const Maybe &gate, const Maybe &weight,
            int64_t rows, int64_t width, at::ScalarType x_type, at::ScalarType type, double eps,
            bool kept, bool has_update) {
-          return maybe(residual_backward(
-              residual_call(rows, width, x_type, type, eps, kept, has_update), given(dsum),
-              given(dnormed), given(x), given(update), given(update_weight), given(scale),
-              given(gate), given(weight)));
+          return maybe(residual_backward({rows, width, x_type, type, eps, kept, has_update},
+                                         given(dsum), given(dnormed), given(x), given(update),
+                                         given(update_weight), given(scale), given(gate),
+                                         given(weight)));
         },
         Free());
   m.def("gated_activation_backward",

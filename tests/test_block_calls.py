@@ -10,13 +10,37 @@ import torch
 from torch.autograd import forward_ad
 
 
+class NoLaunches:
+    """Results of the right shapes, and no gradients."""
+
+    @staticmethod
+    def residual_norm_forward(x, *args):
+        return torch.empty_like(x), torch.empty_like(x), None, None
+
+    @staticmethod
+    def residual_norm(x, *args):
+        return torch.empty_like(x), torch.empty_like(x)
+
+    @staticmethod
+    def gated_activation_forward(x, *args):
+        return x.new_empty((x.shape[0], x.shape[1] // 2)), None
+
+    @staticmethod
+    def gated_activation(x, *args):
+        return x.new_empty((x.shape[0], x.shape[1] // 2))
+
+    @staticmethod
+    def linear_int8(x, codes, row, scales, bias):
+        return x.new_empty((x.shape[0], scales.shape[0]))
+
+
 @pytest.fixture
 def block(pkg, monkeypatch):
     """The module with its launches and the check for a GPU left out."""
     from bevfusion_triton_amd import block
 
     monkeypatch.setattr(block.P, 'require_gpu', lambda *t: None)
-    monkeypatch.setattr(block, '_run', lambda call, device, what: None)
+    monkeypatch.setattr(block.L, 'block_calls', lambda: NoLaunches)
     return block
 
 

@@ -29,14 +29,26 @@ every = pytest.mark.parametrize('name', CALLS)
 def test_a_missing_library_is_an_error(pkg, monkeypatch, tmp_path):
     from bevfusion_triton_amd import _lib
 
-    assert _lib.gradients() is _lib.gradients()
-    monkeypatch.setattr(_lib, '_gradients', None)
-    monkeypatch.setattr(_lib, 'GRADIENTS_PATH', tmp_path / '_autograd.so')
+    assert _lib.block_calls() is _lib.block_calls()
+    monkeypatch.setattr(_lib, '_block_module', None)
+    monkeypatch.setattr(_lib, 'BLOCK_CALLS_PATH', tmp_path / '_block_calls.so')
     with pytest.raises(_lib.LibraryNotBuilt, match='missing'):
-        _lib.gradients()
-    (tmp_path / '_autograd.so').write_bytes(b'no library')
+        _lib.block_calls()
+    (tmp_path / '_block_calls.so').write_bytes(b'no library')
     with pytest.raises(_lib.LibraryNotBuilt, match='cannot load'):
-        _lib.gradients()
+        _lib.block_calls()
+
+
+@pytest.mark.gpu
+def test_a_refusal_below_is_the_package_s_error(pkg, cuda):
+    """Of what the Python call has checked before."""
+    from bevfusion_triton_amd import _lib
+
+    x = torch.zeros(4, 8, device=cuda)
+    with pytest.raises(_lib.BevPoolError, match='unknown activation 7'):
+        _lib.block_calls().gated_activation(x, 7, False, False)
+    with pytest.raises(_lib.BevPoolError, match='neither'):
+        _lib.block_calls().residual_norm(x, None, None, None, None, None, x.dtype, 0.0, False, False)
 
 
 def grads(pkg, name, t, kept=None, douts=None, **more):
