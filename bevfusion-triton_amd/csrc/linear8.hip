@@ -16,7 +16,7 @@
 // card's power leaves (busy in 47% of the cycles): 8192 x 8192 x 8192 487 us,
 // 2,260 TOPS (a library's product to 32-bit sums 2,050), 16,896 x 1,280 x 10,240
 // 255 us, 1,740 TOPS, and 15 for the codes; a few tokens by the weights' bytes:
-// one of 4,096 x 6,144 8.1 us, codes and all, 67 of 5,000 x 4,099 12.8 and 4.
+// one of 4,096 x 6,144 8.1 us, codes and all, 67 of 5,000 x 4,099 10.5 and 4.
 #include <hip/hip_runtime.h>
 
 #include <stdint.h>
@@ -373,76 +373,68 @@ void product_kernel(ProductArgs A) {
   }
 }
 
-// Few tokens: 16 kTx tokens by 16 kTw channels a block, whose eight waves take
-// every eighth 64 bytes of the rows straight to registers, so that the weights
-// are on their way all at once, and add their sums in LDS.
+// Few tokens and channels: 16 kTx tokens by 16 channels a block, whose eight waves
+// take every eighth 64 bytes of the rows straight to registers, so that the
+// weights are on their way all at once, and add their sums in LDS.
 constexpr int kFewWaves = 8, kFewThreads = 64 * kFewWaves;
 
 // The waves' sums of a block to its results.
-template <typename T, int kTx, int kTw>
-__device__ __forceinline__ void finish_few(const ProductArgs &A, i32x4 (&sums)[kFewWaves][kTw * kTx][64],
-                                           const i32x4 (&acc)[kTw][kTx], const float *x_scale, int w0,
+template <typename T, int kTx>
+__device__ __forceinline__ void finish_few(const ProductArgs &A, i32x4 (&sums)[kFewWaves][kTx][64],
+                                           const i32x4 (&acc)[kTx], const float *x_scale, int w0,
                                            int lane, int wave) {
   const int c = lane & 15, q = lane >> 4;
 #pragma unroll
-  for (int i = 0; i < kTw; ++i)
-#pragma unroll
-    for (int j = 0; j < kTx; ++j) sums[wave][i * kTx + j][lane] = acc[i][j];
+  for (int j = 0; j < kTx; ++j) sums[wave][j][lane] = acc[j];
   __syncthreads();
+  if (wave >= kTx) return;
+  i32x4 sum = sums[0][wave][lane];
+#pragma unroll
+  for (int i = 1; i < kFewWaves; ++i) sum += sums[i][wave][lane];
+  // lane 16 q + c: channels 4 q .. + 3 of token c
   const T *bias = static_cast<const T *>(A.bias);
-  for (int t = wave; t < kTw * kTx; t += kFewWaves) {
-    i32x4 sum = sums[0][t][lane];
+  const int token = wave * 16 + c, n = w0 + 4 * q;
+  if (token >= A.tokens) return;
+  const float by = x_scale[token];
+  T *y = static_cast<T *>(A.y) + int64_t(token) * A.channels + n;
+  Four<T> four;
 #pragma unroll
-    for (int i = 1; i < kFewWaves; ++i) sum += sums[i][t][lane];
-    // lane 16 q + c: channels 4 q .. + 3 of token c
-    const int token = t % kTx * 16 + c, n = w0 + t / kTx * 16 + 4 * q;
-    if (token >= A.tokens) continue;
-    const float by = x_scale[token];
-    T *y = static_cast<T *>(A.y) + int64_t(token) * A.channels + n;
-    Four<T> four;
+  for (int r = 0; r < 4; ++r) {
+    const int at = min(n + r, A.channels - 1);
+    four.v[r] = T(float(sum[r]) * by * A.w_scale[at] + (bias ? float(bias[at]) : 0.f));
+  }
+  if (n + 4 <= A.channels) {
+    *reinterpret_cast<Four<T> *>(y) = four;
+  } else {
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const int at = min(n + r, A.channels - 1);
-      four.v[r] = T(float(sum[r]) * by * A.w_scale[at] + (bias ? float(bias[at]) : 0.f));
-    }
-    if (n + 4 <= A.channels) {
-      *reinterpret_cast<Four<T> *>(y) = four;
-    } else {
-#pragma unroll
-      for (int r = 0; r < 4; ++r)
-        if (n + r < A.channels) y[r] = four.v[r];
-    }
+    for (int r = 0; r < 4; ++r)
+      if (n + r < A.channels) y[r] = four.v[r];
   }
 }
 
-template <typename T, int kTx, int kTw>
-__global__ __launch_bounds__(kFewThreads, kTx * kTw > 4 ? 2 : 4) void few_kernel(ProductArgs A) {
-  __shared__ i32x4 sums[kFewWaves][kTw * kTx][64];
+template <typename T, int kTx>
+__global__ __launch_bounds__(kFewThreads, 4) void few_kernel(ProductArgs A) {
+  __shared__ i32x4 sums[kFewWaves][kTx][64];
   constexpr int kDeep = 4;  // steps whose loads are on their way together
   const int lane = attention::lane_id(), wave = attention::wave_id();
   const int c = lane & 15, q = lane >> 4;
-  const int w0 = int(blockIdx.x) * 16 * kTw;
-  const int8_t *w_at[kTw], *x_at[kTx];
-#pragma unroll
-  for (int i = 0; i < kTw; ++i)
-    w_at[i] = A.w + int64_t(min(w0 + 16 * i + c, A.channels - 1)) * A.w_row;
+  const int w0 = int(blockIdx.x) * 16;
+  const int8_t *w_at = A.w + int64_t(min(w0 + c, A.channels - 1)) * A.w_row, *x_at[kTx];
 #pragma unroll
   for (int i = 0; i < kTx; ++i)
     x_at[i] = A.x + int64_t(min(16 * i + c, A.tokens - 1)) * A.x_pitch;
-  i32x4 acc[kTw][kTx] = {};
+  i32x4 acc[kTx] = {};
   for (int first = wave; first < A.steps; first += kFewWaves * kDeep) {
-    i32x4 w[kDeep][kTw], x[kDeep][kTx];
+    i32x4 w[kDeep], x[kDeep][kTx];
 #pragma unroll
     for (int d = 0; d < kDeep; ++d) {
       const int step = first + d * kFewWaves, chunk = step * 4 + q;
-#pragma unroll
-      for (int i = 0; i < kTw; ++i) w[d][i] = i32x4{0, 0, 0, 0};
+      w[d] = i32x4{0, 0, 0, 0};
 #pragma unroll
       for (int i = 0; i < kTx; ++i) x[d][i] = i32x4{0, 0, 0, 0};
       if (step >= A.steps) continue;
-#pragma unroll
-      for (int i = 0; i < kTw; ++i)  // (past a row's end: as above)
-        w[d][i] = *reinterpret_cast<const i32x4 *>(w_at[i] + min(chunk, A.w_chunks - 1) * 16);
+      // (past a row's end: as above)
+      w[d] = *reinterpret_cast<const i32x4 *>(w_at + min(chunk, A.w_chunks - 1) * 16);
 #pragma unroll
       for (int i = 0; i < kTx; ++i)
         x[d][i] = *reinterpret_cast<const i32x4 *>(x_at[i] + chunk * 16);
@@ -451,12 +443,10 @@ __global__ __launch_bounds__(kFewThreads, kTx * kTw > 4 ? 2 : 4) void few_kernel
 #pragma unroll
     for (int d = 0; d < kDeep; ++d)
 #pragma unroll
-      for (int i = 0; i < kTw; ++i)
-#pragma unroll
-        for (int j = 0; j < kTx; ++j)
-          acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(w[d][i], x[d][j], acc[i][j], 0, 0, 0);
+      for (int j = 0; j < kTx; ++j)
+        acc[j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(w[d], x[d][j], acc[j], 0, 0, 0);
   }
-  finish_few<T, kTx, kTw>(A, sums, acc, A.x_scale, w0, lane, wave);
+  finish_few<T, kTx>(A, sums, acc, A.x_scale, w0, lane, wave);
 }
 
 // Up to eight short tokens: every block forms their codes itself, beside its
@@ -525,7 +515,7 @@ __global__ __launch_bounds__(kFewThreads, 4) void token_kernel(ProductArgs A, co
   }
   attention::tile_barrier();
   const int8_t *x_at = codes + min(c, A.tokens - 1) * code_row;
-  i32x4 acc[1][1] = {};
+  i32x4 acc[1] = {};
   for (int first = wave; first < A.steps; first += kFewWaves * kDeep) {
     if (first != wave) fetch(first);
 #pragma unroll
@@ -533,10 +523,10 @@ __global__ __launch_bounds__(kFewThreads, 4) void token_kernel(ProductArgs A, co
       const int step = first + d * kFewWaves;
       i32x4 x = {0, 0, 0, 0};
       if (step < A.steps) x = *reinterpret_cast<const i32x4 *>(x_at + (step * 4 + q) * 16);
-      acc[0][0] = __builtin_amdgcn_mfma_i32_16x16x64_i8(w[d], x, acc[0][0], 0, 0, 0);
+      acc[0] = __builtin_amdgcn_mfma_i32_16x16x64_i8(w[d], x, acc[0], 0, 0, 0);
     }
   }
-  finish_few<T, 1, 1>(A, sums, acc, scales, w0, lane, wave);
+  finish_few<T, 1>(A, sums, acc, scales, w0, lane, wave);
 }
 
 // ---------------------------------------------------------------------------
@@ -618,38 +608,37 @@ int launch_own(const ProductArgs &A, const void *x, int64_t x_row, int width, in
                                  : launch_token<T, 4>(A, x, x_row, width, row_lanes, s);
 }
 
-template <typename T, int kTx, int kTw>
+template <typename T, int kTx>
 int launch_few(const ProductArgs &A, hipStream_t s) {
-  const int blocks = (A.channels + 16 * kTw - 1) / (16 * kTw);
-  const int st = check_grid(blocks, 64 * kFewWaves, "linear8");
-  if (st) return st;
-  hipLaunchKernelGGL((few_kernel<T, kTx, kTw>), dim3(blocks), dim3(64 * kFewWaves), 0, s, A);
+  hipLaunchKernelGGL((few_kernel<T, kTx>), dim3((A.channels + 15) / 16), dim3(kFewThreads), 0, s, A);
   return check_launch("linear8");
 }
 
 template <typename T>
 int launch_product(ProductArgs &A, hipStream_t s) {
-  // Up to 32 tokens the weights' way to the registers is the time.  32 channels
-  // a block read the tokens half as often as 16, but need enough channels for
-  // the card's CUs: us by 16 and by 32, 16 x 4096 x 6144 12.4 and 10.9, 32 x
-  // 8192 x 8192 32.1 and 24.7; 32 x 1280 x 1280 6.2 and 7.1.
-  if (A.tokens <= 32) {
-    const bool wide = A.channels >= 32 * 160;
-    if (A.tokens <= 16) return wide ? launch_few<T, 1, 2>(A, s) : launch_few<T, 1, 1>(A, s);
-    return wide ? launch_few<T, 2, 2>(A, s) : launch_few<T, 2, 1>(A, s);
-  }
   auto tiles = [&](int x, int w) {
     return int64_t((A.tokens + x - 1) / x) * ((A.channels + w - 1) / w);
   };
-  // Small tiles where few of larger ones would leave CUs idle, and while there
-  // are no more than CUs the rows' length in parts, four of 64 x 32 and two of 64
-  // x 64.  us by 64 x 32 in four and 64 x 64 in two: 33 x 8192 x 8192 18.0 and
-  // 22.9, 64 x 4096 x 4096 9.9 and 12.0, 500 x 4096 x 1024 10.6 and 12.8; 128 x
-  // 4096 x 6144 17.5 and 13.2.  By 64 x 64 in two
-  // parts, 64 x 64 and 64 x 128, 67 x 5000 x 4099 14.0, 17.1 and 22.1, 200 x 4096
-  // x 4096 12.8, 15.0 and 18.5; 512 x 4096 x 4096 21.6, 18.7 and 20.3, 1024 x 1280
-  // x 1280 12.1, 9.2 and 10.8; 800 x 4096 x 4096 37.4, 30.3 and 24.0.
+  // Small tiles where few of larger ones would leave CUs idle, and the rows' length
+  // in parts.  us of products by events:
+  //   few tokens and channels: blocks of 16 channels; 1 x 32768 x 4096 34.5, by 32 x
+  //   32 in four parts 37.2, 5 x 5000 x 300 7.6 and 8.7, but 24 x 4096 x 4096 (128
+  //   tiles) 10.2 and 8.8, 32 x 8192 x 8192 25.2 and 17.0
+  const int64_t least = tiles(32, 32);
+  if (A.tokens <= 32 && least < 128)
+    return A.tokens <= 16 ? launch_few<T, 1>(A, s) : launch_few<T, 2>(A, s);
+  //   no more than CUs: 32 x 32 in four parts, then 64 x 32; 64 x 4096 x 4096 9.2 and
+  //   9.9; 33 x 8192 x 8192 (512 and 256) 24.5 and 18.3, by 64 x 64 in two 22.9
+  if (least <= 256) return launch_tiles<T, 1, 1, 1, 1, 128, 4, 4>(A, s);
   if (tiles(64, 32) <= 256) return launch_tiles<T, 1, 1, 2, 1, 128, 3, 4>(A, s);
+  //   twice as many: 32 x 32 in three parts, two blocks a CU; 67 x 5000 x 4099 12.6, by
+  //   64 x 64 in two 14.8, 33 x 8192 x 8192 20.3; always for up to 32 tokens, 32 x 4096
+  //   x 20000 24.3 and by blocks of 32 channels as above 30.2; 48 x 1280 x 10240 10.4,
+  //   by 64 x 64 in two 8.0
+  if (A.tokens <= 32 || least <= 512) return launch_tiles<T, 1, 1, 1, 1, 128, 3, 3>(A, s);
+  //   64 x 64 in two parts, 64 x 64 and 64 x 128: 200 x 4096 x 4096 12.8, 15.0 and 18.5;
+  //   512 x 4096 x 4096 21.6, 18.7 and 20.3, 1024 x 1280 x 1280 12.1, 9.2 and 10.8; 800
+  //   x 4096 x 4096 37.4, 30.3 and 24.0
   const int64_t small = tiles(64, 64);
   if (small <= 256) return launch_tiles<T, 1, 1, 2, 2, 128, 4, 2>(A, s);
   if (small <= 512) return launch_tiles<T, 1, 1, 2, 2, 128, 4>(A, s);

@@ -47,6 +47,7 @@ def test_widths(pkg, cuda, width, tokens):
 
 
 @pytest.mark.parametrize('tokens,width,out', [
+    (9, 128, 4064), (16, 3000, 4100), (32, 200, 8193), (20, 300, 20001), (32, 129, 4000),
     (33, 128, 8191), (70, 129, 4097), (300, 333, 2000), (64, 640, 8193), (40, 2050, 50),
     (257, 1100, 1601)])
 def test_parts_of_rows(pkg, cuda, tokens, width, out):
