@@ -14,7 +14,7 @@
 //
 // Bound by memory: x, u, D and H (and a gate of each value) read once, dx and
 // du (and dgate) written once.  x' and n are formed again from x and u.  16,896
-// rows of 1,280 in bf16 56 us (4.6 TB/s) and 10 for the sums of six rows of gate;
+// rows of 1,280 in bf16 56 us (4.6 TB/s) and 9 for the sums of six rows of gate;
 // from checkpoints, with an fp32 stream, 71 us (4.3 TB/s) and 5.
 #include <hip/hip_runtime.h>
 
@@ -251,69 +251,85 @@ __device__ __forceinline__ float slices_sum(float v, float *lds) {
   return v;
 }
 
-// Sum over `n` rows of `from` of column c, in the first slice.
-__device__ __forceinline__ float column_sum(const float *from, int64_t n, int width, int c,
-                                            float *lds) {
+// Sum of rows first, first + step, .. below n of a column.
+__device__ __forceinline__ float strided_sum(const float *from, int64_t first, int64_t n, int step,
+                                             int width) {
   float s = 0.f;
-  if (c < width) {
 #pragma unroll 8
-    for (int64_t i = threadIdx.x / kSumColumns; i < n; i += kSlices) s += from[i * width + c];
-  }
-  return slices_sum(s, lds);
+  for (int64_t i = first; i < n; i += step) s += from[i * width];
+  return s;
 }
 
 // The gradients that are sums over rows, from the items' and the blocks' sums:
 // grid.y 0 those of the update's weight and of the scale, 1 that of the norm's
-// weight, from 2 on that of a gate that rows share, by its rows.
+// weight, from 2 on that of a gate that rows share, by its rows, or, where these
+// have so few parts that a slice sums them, by kSlices of them (us of all sums of
+// 16,896 rows of 1,280, by events: 40 rows of gate 10, by a block each 22; 1,000 11
+// and 119).
+constexpr int kFewParts = kSlices;
 template <typename T>
 __global__ __launch_bounds__(kSumThreads) void sums_kernel(Args A, int64_t weight_blocks, T *dgate,
                                                            T *dupdate_weight, T *dscale,
                                                            T *dweight) {
   __shared__ float lds[kSumThreads];
+  const int slice = int(threadIdx.x) / kSumColumns;
   const int c = blockIdx.x * kSumColumns + int(threadIdx.x) % kSumColumns;
-  const bool writes = threadIdx.x < kSumColumns && c < A.width;
+  const bool on = c < A.width, writes = slice == 0 && on;
   if (blockIdx.y == 1) {
     if (!dweight) return;
-    const float s = column_sum(A.weight_parts, weight_blocks, A.width, c, lds);
+    float s = on ? strided_sum(A.weight_parts + c, slice, weight_blocks, kSlices, A.width) : 0.f;
+    s = slices_sum(s, lds);
     if (writes) dweight[c] = T(s);
     return;
   }
   if (blockIdx.y == 0 && !dupdate_weight && !dscale) return;
   float w = 1.f, scale = 1.f;
-  if (c < A.width && A.update_weight) w = float(static_cast<const T *>(A.update_weight)[c]);
-  if (c < A.width && A.scale) scale = float(static_cast<const T *>(A.scale)[c]);
+  if (on && A.update_weight) w = float(static_cast<const T *>(A.update_weight)[c]);
+  if (on && A.scale) scale = float(static_cast<const T *>(A.scale)[c]);
+  const float *parts = A.parts + c;
+  const bool shared = A.has_gate && A.gate_each > 1;  // (the items' sums are without the gate)
+  const int64_t owners = A.items / A.parts_each;
   if (blockIdx.y == 0) {
     float s = 0.f;
-    if (A.has_gate && A.gate_each > 1) {  // (the items' sums are without the gate)
-      if (c < A.width) {
-        const T *gate = static_cast<const T *>(A.gate) + c;
-        const float *parts = A.parts + c;
-        const int slice = threadIdx.x / kSumColumns;
-        if (A.parts_each >= kSlices) {
-          for (int64_t owner = 0; owner < A.items / A.parts_each; ++owner) {
-            float t = 0.f;
+    if (on && shared && owners > 1) {
+      const T *gate = static_cast<const T *>(A.gate) + c;
+      // (item, its owner and its place among the owner's parts)
+      const int each = int(A.parts_each), owners_on = kSlices / each, places_on = kSlices % each;
+      int64_t owner = slice / each;
+      int place = slice % each;
 #pragma unroll 8
-            for (int64_t i = slice; i < A.parts_each; i += kSlices)
-              t += parts[(owner * A.parts_each + i) * A.width];
-            s += t * float(gate[owner * A.gate_row]);
-          }
-        } else {
-#pragma unroll 4
-          for (int64_t i = slice; i < A.items; i += kSlices)
-            s += parts[i * A.width] * float(gate[i / A.parts_each * A.gate_row]);
+      for (int64_t i = slice; i < A.items; i += kSlices) {
+        s += parts[i * A.width] * float(gate[owner * A.gate_row]);
+        owner += owners_on;
+        place += places_on;
+        if (place >= each) {
+          place -= each;
+          ++owner;
         }
       }
-      s = slices_sum(s, lds);
-    } else {
-      s = column_sum(A.parts, A.items, A.width, c, lds);
+    } else if (on) {
+      s = strided_sum(parts, slice, A.items, kSlices, A.width);
+      if (shared) s *= float(static_cast<const T *>(A.gate)[c]);
     }
+    s = slices_sum(s, lds);
     if (writes && dupdate_weight) dupdate_weight[c] = T(s * scale);
     if (writes && dscale) dscale[c] = T(s * w);
     return;
   }
-  for (int64_t owner = blockIdx.y - 2; owner < A.items / A.parts_each; owner += gridDim.y - 2) {
-    const float s =
-        column_sum(A.parts + owner * A.parts_each * A.width, A.parts_each, A.width, c, lds);
+  const int64_t first = blockIdx.y - 2, step = gridDim.y - 2;
+  if (A.parts_each <= kFewParts) {
+    if (on)
+      for (int64_t owner = first * kSlices + slice; owner < owners; owner += step * kSlices) {
+        const int64_t at = owner * A.parts_each;
+        const float s = strided_sum(parts, at, at + A.parts_each, 1, A.width);
+        dgate[owner * A.width + c] = T(s * w * scale);
+      }
+    return;
+  }
+  for (int64_t owner = first; owner < owners; owner += step) {
+    const int64_t at = owner * A.parts_each;
+    float s = on ? strided_sum(parts, at + slice, at + A.parts_each, kSlices, A.width) : 0.f;
+    s = slices_sum(s, lds);
     if (writes) dgate[owner * A.width + c] = T(s * w * scale);
   }
 }
@@ -336,10 +352,19 @@ Split split_for(int64_t rows, int width, int64_t gate_rows, bool kept, bool wide
 #undef RESIDUAL_BLOCKS
   const bool shared = gate_rows > 0 && gate_rows < rows;
   const int64_t owners = shared ? gate_rows : 1, each = rows / owners;
-  int64_t parts = (most_blocks + owners - 1) / owners;
   const int64_t most = (each + at_once - 1) / at_once;
+  // As many parts of each owner's rows as give every block an item, or one more,
+  // whichever leaves a block fewer rows at most: 16,896 rows of 1,280 of six owners,
+  // 1,278 items on 1,280 blocks in place of 1,284, four of them with two; 16,800 of
+  // 600 owners 56.7 us for 59.5.
+  auto load = [&](int64_t parts) {
+    const int64_t items = owners * parts, blocks = items < most_blocks ? items : most_blocks;
+    return (items + blocks - 1) / blocks * ((each + parts - 1) / parts);
+  };
+  int64_t parts = most_blocks / owners;
   if (parts > most) parts = most;
   if (parts < 1) parts = 1;
+  if (parts < most && load(parts + 1) < load(parts)) ++parts;
   Split s;
   s.parts_each = parts;
   s.items = owners * parts;
@@ -372,8 +397,9 @@ void launch_sums(const Args &A, int64_t blocks, void *dgate, void *dupdate_weigh
                  void *dweight, hipStream_t s) {
   const int64_t owners = A.has_gate && A.gate_each > 1 ? A.items / A.parts_each : 0;
   if (!owners && !dupdate_weight && !dscale && !dweight) return;
+  const int64_t sums = A.parts_each <= kFewParts ? (owners + kSlices - 1) / kSlices : owners;
   const dim3 grid((A.width + kSumColumns - 1) / kSumColumns,
-                  unsigned(2 + (owners < 4096 ? owners : 4096)));
+                  unsigned(2 + (sums < 4096 ? sums : 4096)));
   hipLaunchKernelGGL((sums_kernel<T>), grid, dim3(kSumThreads), 0, s, A, blocks,
                      static_cast<T *>(dgate), static_cast<T *>(dupdate_weight),
                      static_cast<T *>(dscale), static_cast<T *>(dweight));

@@ -119,6 +119,14 @@ def test_rows(pkg, cuda, rows, gate):
     check(pkg, cuda, *make(rows, 40, torch.float32, torch.float32, seed=rows, gate=gate))
 
 
+@pytest.mark.parametrize('rows,width,gate', [
+    (1200, 200, 40), (4000, 1030, 40), (2600, 600, 20), (3200, 1283, 800), (8000, 40, 1000),
+    (6000, 2048, 3)])
+def test_shared_gates(pkg, cuda, rows, width, gate):
+    """Parts of a gate's rows that a slice of the sums takes alone, or all do."""
+    check(pkg, cuda, *make(rows, width, torch.float32, torch.float16, seed=gate, gate=gate))
+
+
 @pytest.mark.parametrize('parts', [
     ('x', 'weight'), ('x', 'update'), ('x', 'update', 'weight'), ('x', 'update', 'update_weight'),
     ('x', 'update', 'scale'), ('x', 'update', 'gate', 'weight'),
