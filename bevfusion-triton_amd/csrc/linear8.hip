@@ -642,18 +642,20 @@ int launch_product(ProductArgs &A, hipStream_t s) {
   const int64_t small = tiles(64, 64);
   if (small <= 256) return launch_tiles<T, 1, 1, 2, 2, 128, 4, 2>(A, s);
   if (small <= 512) return launch_tiles<T, 1, 1, 2, 2, 128, 4>(A, s);
-  // Tiles of 256 x 256, one a CU, read each operand least often: a round of 256
-  // takes 0.83 of the time of 512 of 128 x 256, two a CU (8192 x 8192 x 8192 487
-  // and 590 us), but a last round of up to 256 of these, one a CU, 0.6 of it.  So
-  // us by 256 x 256 and 128 x 256: 16896 x 1280 x 10240 304 and 336, 1500 x 1280 x
-  // 10240 29 and 33; 16896 x 5120 x 1280 148 and 139, 1024 x 4096 x 8192 57 and 48.
-  const int64_t wide = tiles(256, 256), half = tiles(128, 256), rest = half % 512;
-  if (wide >= 128 &&
-      (wide + 255) / 256 * 83 < half / 512 * 100 + (rest > 256 ? 100 : rest > 0 ? 60 : 0))
-    return launch_tiles<T, 4, 2, 2, 4, 128, 2>(A, s);
-  // 128 x 256 from one for each CU on (us of these and of 64 x 128: 1024 x 4096 x
-  // 8192 48 and 53; 800 x 4096 x 4096 42 and 24).
-  if (half >= 256) return launch_tiles<T, 2, 4, 2, 2, 64, 3>(A, s);
+  // Larger tiles read operands less often, smaller ones leave less of a last round
+  // and of a tile's edge empty: by what a round takes, 100 being 512 tiles of 128 x
+  // 256, two a CU, and a last one of up to 256, one a CU, less.  us by 256 x 256, 128
+  // x 256 and 64 x 128: 8192 x 8192 x 8192 487, 590; 1500 x 1280 x 10240 29, 33, 38;
+  // 4000 x 4096 x 2500 59, 66, 66; 1024 x 4096 x 8192 56, 48, 53; 10325 x 1787 x 624
+  // 33, 27, 29; 17223 x 5288 x 288 78, 83, 66; 7000 x 2560 x 1100 40, 43, 36.
+  auto rounds = [&](int x, int w, int64_t each, int64_t full, int64_t last) {
+    const int64_t n = tiles(x, w), rest = n % each;
+    return n / each * full + (rest > 256 ? full : rest > 0 ? last : 0);
+  };
+  const int64_t large = rounds(256, 256, 256, 83, 83), middle = rounds(128, 256, 512, 100, 63);
+  const int64_t little = rounds(64, 128, 512, 33, 29);
+  if (large <= middle && large <= little) return launch_tiles<T, 4, 2, 2, 4, 128, 2>(A, s);
+  if (middle <= little) return launch_tiles<T, 2, 4, 2, 2, 64, 3>(A, s);
   return launch_tiles<T, 1, 2, 2, 2, 128, 3>(A, s);
 }
 
@@ -708,7 +710,7 @@ int bevpool_linear8(const void *x, int64_t x_row, int32_t dtype, const void *wei
     return fail(BEVPOOL_ESPACE, "linear8 scratch too small, or not at a multiple of 16 bytes");
   // (before anything is launched: the blocks of any plan of launch_product)
   st = tokens <= 32 ? check_grid((channels + 15) / 16, 64 * kFewWaves, "linear8")
-                    : check_grid(((tokens + 255) / 256) * ((channels + 255) / 256), 512, "linear8");
+                    : check_grid(((tokens + 63) / 64) * ((channels + 127) / 128), 256, "linear8");
   if (st) return st;
   hipStream_t s = static_cast<hipStream_t>(stream);
   const int pitch = int(code_pitch(width));
