@@ -333,14 +333,18 @@ int launch(const GradArgs &A, T *dweight, hipStream_t s) {
 template <typename T>
 int launch_columns(const void *x, int64_t x_row, int64_t n_rows, int width, void *out,
                    float *scratch, hipStream_t s) {
-  const dim3 grid((width + kColumns - 1) / kColumns, kColumnParts);
+  // Parts of 32 rows at least: us of both by events, 300 x 1280 9.3, by 256 parts
+  // 11 to 16, 86 x 3577 9.0 and 15.
+  const int64_t some = (n_rows + 31) / 32;
+  const int64_t parts = some < 1 ? 1 : some < kColumnParts ? some : kColumnParts;
+  const dim3 grid((width + kColumns - 1) / kColumns, unsigned(parts));
   const int st = check_grid(int64_t(grid.x) * kColumnParts, kThreads, "column_sums");
   if (st) return st;
   LaunchScope scope("column_sums", s);
   hipLaunchKernelGGL((column_sum_kernel<T, float>), grid, dim3(kThreads), 0, s,
                      static_cast<const T *>(x), x_row, n_rows, width, scratch);
   hipLaunchKernelGGL((column_sum_kernel<float, T>), dim3(grid.x, 1), dim3(kThreads), 0, s, scratch,
-                     int64_t(width), int64_t(kColumnParts), width, static_cast<T *>(out));
+                     int64_t(width), parts, width, static_cast<T *>(out));
   return check_launch("column_sums");
 }
 
