@@ -5,6 +5,9 @@ The library is built in-tree by ``csrc/Makefile`` next to this file.  There is
 no fallback: when the library is missing or fails to load, every entry point
 raises :class:`LibraryNotBuilt`.
 
+The block operators go through ``_block_calls.so`` beside it, which calls the
+same C ABI and holds the nodes of their gradients.
+
 torch is imported before the library is loaded so that the HIP runtime the
 library links against (``libamdhip64.so.7``) resolves to the instance torch
 already loaded; device pointers and streams are then shared with torch.
