@@ -178,3 +178,29 @@ def test_a_trace_has_gradients(pkg, cuda, name):
     out = CALLS[name](pkg, dict(t, x=y), 8)[-1]
     want, = torch.autograd.grad(out, y, torch.ones_like(out))
     assert torch.equal(got, want)
+
+
+@pytest.mark.gpu
+def test_two_threads(pkg, cuda):
+    """Steps of two threads at once, each on a stream of its own."""
+    from concurrent.futures import ThreadPoolExecutor
+
+    t = leaves(cuda, 3000, 512)
+    want = {n: grads(pkg, n, t, 8) for n in CALLS}
+    codes = pkg.quantize_weight(t['linear'])
+    product = pkg.linear_int8(t['x'], *codes)
+    torch.cuda.synchronize()
+
+    def work(_):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(10):
+                got = {n: grads(pkg, n, t, 8) for n in CALLS}
+                y = pkg.linear_int8(t['x'], *codes)
+            torch.cuda.current_stream().synchronize()
+        return got, y
+
+    with ThreadPoolExecutor(2) as pool:
+        for got, y in pool.map(work, range(2)):
+            assert torch.equal(y, product)
+            for n in CALLS:
+                same(got[n], want[n])
