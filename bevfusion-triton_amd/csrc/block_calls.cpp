@@ -222,9 +222,9 @@ variable_list linear_backward(const Linear &A, const Tensor &dy, const Tensor &k
           "bevpool_checkpoint_unpack");
     grads[1] = dy.t().mm(x);
   }
-  if (need_bias) {
+  if (need_bias) grads[2] = at::empty({n}, dy.options());
+  if (need_bias && n > 0) {  // (the sums refuse rows of nothing)
     const Tensor rows = rows_of(dy, A.type);
-    grads[2] = at::empty({n}, dy.options());
     const size_t need = bevpool_column_sums_scratch_bytes(n);
     const Tensor scratch = bytes(dy, need);
     check(bevpool_column_sums(at_of(rows), row_of(rows), code, A.rows, n, at_of(grads[2]),

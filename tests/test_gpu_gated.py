@@ -247,3 +247,15 @@ def test_checkpoint_linear_layer(pkg, cuda):
                        torch.autograd.grad(plain(x).sum(), x)[0])
     with torch.no_grad():
         assert not layer(x).requires_grad
+
+
+@pytest.mark.parametrize('dtype', DTYPES, ids=str)
+@pytest.mark.parametrize('rows', [0, 5])
+def test_no_outputs(pkg, cuda, dtype, rows):
+    """A layer of no channels, as torch's own: empty gradients, and zeros for x."""
+    leaves = [torch.ones(s, device=cuda, dtype=dtype, requires_grad=True)
+              for s in ((rows, 16), (0, 16), (0,))]
+    y = pkg.checkpoint_linear(*leaves)
+    assert y.shape == (rows, 0)
+    for t, d in zip(leaves, torch.autograd.grad(y, leaves, y.detach())):
+        assert d.shape == t.shape and d.dtype == dtype and not d.any()
