@@ -164,8 +164,8 @@ __global__ __launch_bounds__(kThreads) void gated_backward_kernel(GatedArgs A) {
       ap.load(kept, at.chunk, blocks);
       bp.load(kept + pitch, at.chunk, blocks);
     }
-    ap.get(a);
-    bp.get(b);
+    ap.template get<T>(a);
+    bp.template get<T>(b);
   } else {
     const T *x = static_cast<const T *>(A.x) + at.row * A.x_row + begin;
     rows::Words<T> aw, bw;
@@ -208,12 +208,7 @@ __global__ __launch_bounds__(kThreads) void unpack_kernel(Chunks C, const uint8_
   rows::PackedChunk chunk;
   chunk.load(kept + at.row * rows::checkpoint_pitch(C.width), at.chunk, rows::blocks_of(C.width));
   float v[8];
-  chunk.get(v);
-  // (64 2^10, which stands for fp16 values from 65,024 on, is none itself)
-  if constexpr (__is_same(T, _Float16))
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (fabsf(v[i]) > 65504.f) v[i] = copysignf(65504.f, v[i]);
+  chunk.template get<T>(v);
   rows::store(out + at.row * C.width + at.chunk * rows::kChunk, v, at.left);
 }
 

@@ -115,7 +115,7 @@ struct Raw {
       for (int i = 0; i < rows::Words<T>::kWords; ++i) asm volatile("" : "+v"(c[j].w[i]));
   }
 };
-template <int kChunks>
+template <typename T, int kChunks>
 struct Packed {
   rows::Bytes c[kChunks];
   unsigned first[kChunks], last[kChunks];  // scales of a chunk's ends
@@ -140,10 +140,10 @@ struct Packed {
                                       const Place<kLanes, kChunks, kWhole> &at) const {
 #pragma unroll
     for (int j = 0; j < kChunks; ++j) {
-      rows::unpack(v[j], c[j], first[j]);
+      rows::unpack<T>(v[j], c[j], first[j]);
       if (at.width % rows::kChunk != 0) {  // (two blocks' values may lie in it)
         float w[rows::kChunk];
-        rows::unpack(w, c[j], last[j]);
+        rows::unpack<T>(w, c[j], last[j]);
         const int begin = at.begin(j);
 #pragma unroll
         for (int i = 0; i < rows::kChunk; ++i) {

@@ -78,9 +78,10 @@ struct Operands {
       }
   }
 };
-template <int kChunks>
+template <typename T, typename X, int kChunks>
 struct KeptOperands {
-  Packed<kChunks> x, update;
+  Packed<X, kChunks> x;
+  Packed<T, kChunks> update;
   template <int kLanes, bool kWhole>
   __device__ __forceinline__ void load(const Args &A, int64_t row,
                                        const Place<kLanes, kChunks, kWhole> &at) {
@@ -118,7 +119,7 @@ __global__ __launch_bounds__(threads_of(kLanes),
                              backward_waves(kLanes, kChunks, kKept, sizeof(X) == 4))
 void residual_backward_kernel(Args A) {
   constexpr int kGroups = threads_of(kLanes) / kLanes;
-  typedef std::conditional_t<kKept, KeptOperands<kChunks>, Operands<T, X, kChunks>> Of;
+  typedef std::conditional_t<kKept, KeptOperands<T, X, kChunks>, Operands<T, X, kChunks>> Of;
   extern __shared__ float lds[];
   __shared__ float shared[6][2 * (threads_of(kLanes) / 64)];
   const Place<kLanes, kChunks, kWhole> at(A.width);

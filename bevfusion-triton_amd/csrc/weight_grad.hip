@@ -158,11 +158,7 @@ __global__ __launch_bounds__(kGradThreads, 2) void weight_grad_kernel(GradArgs A
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       float v[8];
-      rows::unpack(v, rows::Bytes{x.bytes[2 * i], x.bytes[2 * i + 1]}, x.scale);
-      if constexpr (__is_same(T, _Float16))
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-          if (fabsf(v[j]) > 65504.f) v[j] = copysignf(65504.f, v[j]);
+      rows::unpack<T>(v, rows::Bytes{x.bytes[2 * i], x.bytes[2 * i + 1]}, x.scale);
       x.words[i].set(v);
     }
   };

@@ -259,3 +259,19 @@ def test_no_outputs(pkg, cuda, dtype, rows):
     assert y.shape == (rows, 0)
     for t, d in zip(leaves, torch.autograd.grad(y, leaves, y.detach())):
         assert d.shape == t.shape and d.dtype == dtype and not d.any()
+
+
+def test_largest_halves(pkg, cuda):
+    """fp16's largest numbers come back from a checkpoint as its largest, not as
+    the power of two above it: gradients of silu, whose slope is one there."""
+    half = torch.float16
+    g = torch.Generator().manual_seed(9)
+    x = torch.linspace(64000, 65504, 400).to(half).repeat(3, 2)
+    dout = (torch.randn((3, 400), generator=g) / 64).to(half)
+    leaf = x.to(cuda).requires_grad_(True)
+    out = pkg.gated_activation(leaf, 'silu', checkpoint=8)
+    got, = torch.autograd.grad(out, leaf, dout.to(cuda))
+    a, b = ref.kept(x.unflatten(-1, (2, -1))).unbind(-2)
+    assert a.max() == 65504
+    want = torch.cat((dout.double() * b, dout.double() * a), -1).to(half)  # (exact products)
+    assert torch.equal(got.cpu(), want)

@@ -262,3 +262,17 @@ def test_zero_rows_and_no_eps(pkg, cuda):
         assert torch.equal(dx, torch.full_like(dx, 1 + 1000.0)) or torch.allclose(
             dx, torch.full_like(dx, 1001.0), rtol=1e-6)
         assert not dw.any()
+
+
+def test_largest_halves(pkg, cuda):
+    """fp16's largest numbers come back from a checkpoint as its largest, not as
+    the power of two above it."""
+    half = torch.float16
+    g = torch.Generator().manual_seed(6)
+    case, grads = make(12, 64, torch.float32, half, seed=6, parts=('x', 'update', 'weight'))
+    at = torch.randint(0, 64, (12,), generator=g)
+    case['update'][torch.arange(12), at] = torch.linspace(64900, 65504, 12).to(half)
+    check(pkg, cuda, case, grads, 8)
+    case, grads = make(12, 64, half, half, seed=7, parts=('x', 'weight'))
+    case['x'][torch.arange(12), at] = torch.linspace(65504, 64900, 12).to(half)
+    check(pkg, cuda, case, {'normed': 64 * grads['normed']}, 8)
