@@ -173,6 +173,19 @@ struct __attribute__((packed, aligned(sizeof(T)))) Four {
   T v[4];
 };
 
+// A token's scale around the channel's: ahead of it where it makes a sum smaller,
+// behind it where larger.  So nothing on the way passes fp32's range where the
+// result does not, whatever the channel's scale.  (One multiplication more:
+// 16,896 x 1,280 x 10,240 takes 0.5% longer, with a choice for each value 1.3%.)
+struct TokenScale {
+  float ahead, behind;
+  __device__ __forceinline__ explicit TokenScale(float s)
+      : ahead(s >= 1.f ? 1.f : s), behind(s >= 1.f ? s : 1.f) {}
+  __device__ __forceinline__ float of(int sum, float channel) const {
+    return float(sum) * ahead * channel * behind;
+  }
+};
+
 // Rows of 64 or 128 bytes in LDS, kChunks of 16: chunk c of row r lies at c ^
 // (r / 4) % 4, or c ^ (r / 2) % 8, so the 16 rows of which a fragment read takes
 // one chunk each use all of the 256 bytes that LDS gives a cycle.
@@ -324,7 +337,7 @@ void product_kernel(ProductArgs A) {
   for (int j = 0; j < kTx; ++j) {
     const int token = x0 + wx + 32 * j + c;
     const bool valid = token < A.tokens;
-    const float by = valid ? A.x_scale[token] : 0.f;
+    const TokenScale by(valid ? A.x_scale[token] : 0.f);
     T *y = static_cast<T *>(A.y) + int64_t(token) * A.channels;
 #pragma unroll
     for (int i = 0; i < kTw; ++i)
@@ -339,7 +352,7 @@ void product_kernel(ProductArgs A) {
           const attention::f32x4 bias = *reinterpret_cast<attention::f32x4 *>(biases + n + 8 * g);
 #pragma unroll
           for (int r = 0; r < 4; ++r)
-            v[4 * g + r] = float(acc[i][j][8 * p + 4 * g + r]) * by * scale[r] + bias[r];
+            v[4 * g + r] = by.of(acc[i][j][8 * p + 4 * g + r], scale[r]) + bias[r];
         }
         if constexpr (sizeof(T) == 4) {
 #pragma unroll
@@ -395,13 +408,13 @@ __device__ __forceinline__ void finish_few(const ProductArgs &A, i32x4 (&sums)[k
   const T *bias = static_cast<const T *>(A.bias);
   const int token = wave * 16 + c, n = w0 + 4 * q;
   if (token >= A.tokens) return;
-  const float by = x_scale[token];
+  const TokenScale by(x_scale[token]);
   T *y = static_cast<T *>(A.y) + int64_t(token) * A.channels + n;
   Four<T> four;
 #pragma unroll
   for (int r = 0; r < 4; ++r) {
     const int at = min(n + r, A.channels - 1);
-    four.v[r] = T(float(sum[r]) * by * A.w_scale[at] + (bias ? float(bias[at]) : 0.f));
+    four.v[r] = T(by.of(sum[r], A.w_scale[at]) + (bias ? float(bias[at]) : 0.f));
   }
   if (n + 4 <= A.channels) {
     *reinterpret_cast<Four<T> *>(y) = four;

@@ -204,3 +204,20 @@ def test_layer(pkg, cuda):
     other = pkg.Int8Linear(torch.nn.Linear(200, 90, device=cuda))
     other.load_state_dict(layer.state_dict())
     assert torch.equal(other(x), y)
+
+
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16], ids=str)
+@pytest.mark.parametrize('tokens', [1, 9, 20, 100])
+@pytest.mark.parametrize('size,scale', [(1e33, 1e-4), (1e-4, 1e33), (1e-33, 1e-3), (1e33, 1e-36),
+                                        (1e-36, 1e33)])
+def test_far_scales(pkg, cuda, dtype, tokens, size, scale):
+    """The largest and the smallest tokens and channels: nothing on the way leaves
+    the range in which the result is, and a scale of zero gives zeros."""
+    g = torch.Generator().manual_seed(tokens)
+    x = ((0.5 + torch.rand((tokens, 8192), generator=g)) * size).to(dtype)
+    codes = torch.randint(100, 128, (70, 8192), generator=g).to(torch.int8)
+    scales = scale * (0.5 + torch.rand(70, generator=g))
+    scales[5], scales[6] = 0, -scales[6]
+    want, _ = ref.linear_int8(x, codes, scales, None)
+    assert want.abs().max() < 1e36 and want[:, 0].abs().min() > 1e-33
+    check(pkg, cuda, x, codes, scales, None)
