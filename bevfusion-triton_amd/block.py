@@ -176,7 +176,7 @@ class _Gated(torch.autograd.Function):
     def forward(ctx, x, kind, keep):
         out, kept = L.block_calls().gated_activation_forward(x, kind, keep)
         ctx.save_for_backward(kept if keep else x)
-        ctx.call = (x.dtype, kind, keep)
+        ctx.call = (*out.shape, x.dtype, kind, keep)
         return out
 
     @staticmethod

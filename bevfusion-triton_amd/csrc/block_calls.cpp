@@ -60,11 +60,6 @@ std::vector<Maybe> maybe(const variable_list &tensors) {
   for (const Tensor &t : tensors) out.push_back(maybe(t));
   return out;
 }
-// rows of this type with unit stride along them
-Tensor rows_of(const Tensor &t, at::ScalarType type) {
-  Tensor r = t.scalar_type() == type ? t : t.to(type);
-  return r.stride(1) == 1 || r.size(1) == 1 ? r : r.contiguous();
-}
 Tensor bytes(const Tensor &like, size_t n) {
   return at::empty({int64_t(n)}, like.options().dtype(at::kByte));
 }
@@ -74,6 +69,43 @@ Tensor kept_rows(const Tensor &x, int64_t rows, int64_t width, int copies = 1) {
   return at::empty({rows, copies * bevpool_checkpoint_pitch(int(width))},
                    x.options().dtype(at::kByte));
 }
+
+// What a backward pass reads.  Saved tensors come back by way of hooks, and
+// gradients from whoever calls a node: of another size, type or place than the
+// forward's they are refused, before a kernel reads past them; in another layout
+// they are copied.
+struct Given {
+  at::Device device;  // that of the gradients
+  explicit Given(const Tensor &grad) : device(grad.device()) {
+    TORCH_CHECK(grad.is_cuda(), "a gradient is not on the GPU");
+  }
+  Tensor fits(const Tensor &t, at::ScalarType type, at::IntArrayRef sizes, const char *what) const {
+    TORCH_CHECK(t.device() == device && t.scalar_type() == type && t.sizes() == sizes, what,
+                " of a backward pass is not the forward's: ", t.scalar_type(), " ", t.sizes(),
+                " on ", t.device(), " for ", type, " ", sizes, " on ", device);
+    return t;
+  }
+  // (rows have unit stride along them)
+  Tensor rows(const Tensor &t, at::ScalarType type, int64_t n, int64_t width, const char *what) const {
+    if (!t.defined()) return t;
+    fits(t, type, {n, width}, what);
+    return t.stride(1) == 1 || width == 1 ? t : t.contiguous();
+  }
+  Tensor grad(const Tensor &t, at::ScalarType type, int64_t n, int64_t width) const {
+    return t.defined() && t.scalar_type() != type ? rows(t.to(type), type, n, width, "a gradient")
+                                                  : rows(t, type, n, width, "a gradient");
+  }
+  Tensor vector(const Tensor &t, at::ScalarType type, int64_t width, const char *what) const {
+    return t.defined() ? fits(t, type, {width}, what).contiguous() : t;
+  }
+  // (from a multiple of 16 bytes, as an allocation is)
+  Tensor kept(const Tensor &t, int64_t n, int64_t width, int copies = 1) const {
+    if (!t.defined()) return t;
+    fits(t, at::kByte, {n, copies * bevpool_checkpoint_pitch(int(width))}, "a checkpoint");
+    const bool lies = t.is_contiguous() && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
+    return lies ? t : t.clone(at::MemoryFormat::Contiguous);
+  }
+};
 
 // Sum and normed of rows, and the checkpoints of x and update.
 variable_list residual_forward(const Tensor &x, const Tensor &update, const Tensor &update_weight,
@@ -104,20 +136,28 @@ struct Residual {
 };
 // Gradients of x, update, update_weight, scale, gate and weight.
 variable_list residual_backward(const Residual &R, Tensor dsum, Tensor dnormed, Tensor x,
-                                const Tensor &update, const Tensor &update_weight,
-                                const Tensor &scale, const Tensor &gate, Tensor weight) {
+                                Tensor update, Tensor update_weight, Tensor scale, Tensor gate,
+                                Tensor weight) {
   if (!dsum.defined() && !dnormed.defined()) return variable_list(6);
+  const Given in(dsum.defined() ? dsum : dnormed);
+  const c10::DeviceGuard device(in.device);
   const auto options = (dsum.defined() ? dsum : dnormed).options();
+  dsum = in.grad(dsum, R.x_type, R.rows, R.width);
+  dnormed = in.grad(dnormed, R.type, R.rows, R.width);
+  x = R.kept ? in.kept(x, R.rows, R.width) : in.rows(x, R.x_type, R.rows, R.width, "x");
+  update = R.kept ? in.kept(update, R.rows, R.width)
+                  : in.rows(update, R.type, R.rows, R.width, "update");
+  update_weight = in.vector(update_weight, R.type, R.width, "update_weight");
+  scale = in.vector(scale, R.type, R.width, "scale");
+  weight = in.vector(weight, R.type, R.width, "weight");
+  if (gate.defined()) gate = in.rows(gate, R.type, gate.size(0), R.width, "gate");
   const auto wide = options.dtype(R.x_type), own = options.dtype(R.type);
   Tensor dweight;
   if (weight.defined()) dweight = dnormed.defined() ? at::empty({R.width}, own) : at::zeros_like(weight);
-  if (dnormed.defined()) {
-    dnormed = rows_of(dnormed, R.type);
-  } else {
+  if (!dnormed.defined()) {
     weight = Tensor();
     x = Tensor();
   }
-  if (dsum.defined()) dsum = rows_of(dsum, R.x_type);
   Tensor dx = at::empty({R.rows, R.width}, wide), dupdate, dupdate_weight, dscale, dgate;
   if (R.has_update) dupdate = at::empty({R.rows, R.width}, own);
   if (update_weight.defined()) dupdate_weight = at::empty({R.width}, own);
@@ -154,17 +194,21 @@ variable_list gated_forward(const Tensor &x, int kind, bool keep) {
 }
 
 struct Gated {
+  int64_t rows, width;
   at::ScalarType type;
   int kind;
   bool kept;
 };
-variable_list gated_backward(const Gated &G, Tensor dout, const Tensor &x) {
+variable_list gated_backward(const Gated &G, Tensor dout, Tensor x) {
   if (!dout.defined()) return variable_list(1);
-  dout = rows_of(dout, G.type);
-  const int64_t rows = dout.size(0), width = dout.size(1);
-  const Tensor dx = at::empty({rows, 2 * width}, dout.options());
+  const Given in(dout);
+  const c10::DeviceGuard device(in.device);
+  dout = in.grad(dout, G.type, G.rows, G.width);
+  x = G.kept ? in.kept(x, G.rows, G.width, 2)
+             : in.rows(x, G.type, G.rows, 2 * G.width, "x");
+  const Tensor dx = at::empty({G.rows, 2 * G.width}, dout.options());
   check(bevpool_gated_backward(at_of(x), row_of(x), G.kept, at_of(dout), row_of(dout),
-                               code_of(G.type), rows, int(width), G.kind, at_of(dx), stream()),
+                               code_of(G.type), G.rows, int(G.width), G.kind, at_of(dx), stream()),
         "bevpool_gated_backward");
   return {dx};
 }
@@ -199,15 +243,20 @@ struct Linear {
   bool direct;  // the weight's gradient from the checkpoint itself
 };
 // Gradients of x, weight and bias, those that are needed.
-variable_list linear_backward(const Linear &A, const Tensor &dy, const Tensor &kept,
-                              const Tensor &weight, bool need_x, bool need_weight, bool need_bias) {
+variable_list linear_backward(const Linear &A, Tensor dy, Tensor kept, const Tensor &weight,
+                              bool need_x, bool need_weight, bool need_bias) {
   variable_list grads(3);
   if (!dy.defined()) return grads;
+  const Given in(dy);
+  const c10::DeviceGuard device(in.device);
+  in.fits(weight, A.type, {weight.dim() ? weight.size(0) : 0, A.width}, "weight");
   const int n = int(weight.size(0)), k = int(A.width), code = code_of(A.type);
+  dy = in.grad(dy, A.type, A.rows, n);
+  kept = in.kept(kept, A.rows, A.width);
   if (need_x) grads[0] = dy.mm(weight);
   if (need_weight && A.direct && A.rows) {
     Tensor rows = dy;
-    if (dy.stride(1) != 1 || dy.stride(0) % 8 || reinterpret_cast<uintptr_t>(dy.data_ptr()) % 16 ||
+    if (dy.stride(0) % 8 || reinterpret_cast<uintptr_t>(dy.data_ptr()) % 16 ||
         dy.stride(0) >= (1 << 24))
       rows = dy.clone(at::MemoryFormat::Contiguous);
     grads[1] = at::empty({n, k}, dy.options());
@@ -224,10 +273,9 @@ variable_list linear_backward(const Linear &A, const Tensor &dy, const Tensor &k
   }
   if (need_bias) grads[2] = at::empty({n}, dy.options());
   if (need_bias && n > 0) {  // (the sums refuse rows of nothing)
-    const Tensor rows = rows_of(dy, A.type);
     const size_t need = bevpool_column_sums_scratch_bytes(n);
     const Tensor scratch = bytes(dy, need);
-    check(bevpool_column_sums(at_of(rows), row_of(rows), code, A.rows, n, at_of(grads[2]),
+    check(bevpool_column_sums(at_of(dy), row_of(dy), code, A.rows, n, at_of(grads[2]),
                               at_of(scratch), need, stream()),
           "bevpool_column_sums");
   }
@@ -321,7 +369,7 @@ Tensor gated_activation(const Tensor &x, int kind, bool keep, bool follow) {
   const variable_list out = gated_forward(x, kind, keep && follow);
   if (follow) {
     auto node = node_of<GatedNode>(x);
-    node->call = {x.scalar_type(), kind, keep};
+    node->call = {x.size(0), x.size(1) / 2, x.scalar_type(), kind, keep};
     node->saved[0] = SavedVariable(keep ? out[1] : x, false);
     torch::autograd::set_history(out[0], node);
   }
@@ -387,8 +435,9 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         },
         Free());
   m.def("gated_activation_backward",
-        [](const Tensor &dout, const Tensor &x, at::ScalarType type, int kind, bool kept) {
-          return maybe(gated_backward({type, kind, kept}, dout, x));
+        [](const Tensor &dout, const Tensor &x, int64_t rows, int64_t width, at::ScalarType type,
+           int kind, bool kept) {
+          return maybe(gated_backward({rows, width, type, kind, kept}, dout, x));
         },
         Free());
   m.def("checkpoint_linear_backward",

@@ -204,3 +204,49 @@ def test_two_threads(pkg, cuda):
             assert torch.equal(y, product)
             for n in CALLS:
                 same(got[n], want[n])
+
+
+@pytest.mark.gpu
+@every
+@pytest.mark.parametrize('kept', [None, 8])
+def test_saved_tensors_in_another_layout(pkg, cuda, name, kept):
+    """A hook may give a saved tensor back as it likes it laid out."""
+    def lay(t):
+        if t.dim() == 2:
+            return t.t().contiguous().t()
+        return torch.stack((t, torch.zeros_like(t)), 1)[:, 0]
+
+    t = leaves(cuda)
+    want = grads(pkg, name, t, kept)
+    with torch.autograd.graph.saved_tensors_hooks(lambda s: s, lay):
+        got = grads(pkg, name, t, kept)
+    same(got, want)
+
+
+@pytest.mark.gpu
+@every
+@pytest.mark.parametrize('kept', [None, 8])
+def test_what_does_not_fit_is_refused(pkg, cuda, name, kept):
+    """Saved tensors of another size, type or place, and gradients that a caller
+    of a node gives: before any kernel reads them."""
+    t = leaves(cuda)
+    for change in (lambda s: s[..., :-1], lambda s: s[:-1], lambda s: s.double(), lambda s: s.cpu()):
+        u = {n: v.detach().requires_grad_(True) for n, v in t.items()}
+        with torch.autograd.graph.saved_tensors_hooks(lambda s: s, change):
+            outs = CALLS[name](pkg, u, kept)
+            with pytest.raises(RuntimeError):
+                torch.autograd.grad(outs, list(u.values()), [torch.ones_like(o) for o in outs],
+                                    allow_unused=True)
+    for n in t:
+        t[n].requires_grad_(True)
+    out = CALLS[name](pkg, t, kept)[-1]
+    node, nothing = out.grad_fn, [None] * (name in ('residual_norm', 'norm'))
+    for d in (torch.ones_like(out)[:-1], torch.ones_like(out)[:, :-1], torch.ones_like(out).cpu(),
+              torch.ones_like(out)[0]):
+        with pytest.raises(RuntimeError):
+            node(*nothing, d)
+    torch.cuda.synchronize()
+    douts = [torch.zeros_like(o) for o in CALLS[name](pkg, t, kept)[:-1]] + [torch.ones_like(out)]
+    got = node(*nothing, douts[-1])
+    got = got if isinstance(got, torch.Tensor) else got[0]  # (a node of one input)
+    assert torch.equal(got, grads(pkg, name, t, kept, douts)[0])
