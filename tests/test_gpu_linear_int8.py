@@ -221,3 +221,18 @@ def test_far_scales(pkg, cuda, dtype, tokens, size, scale):
     want, _ = ref.linear_int8(x, codes, scales, None)
     assert want.abs().max() < 1e36 and want[:, 0].abs().min() > 1e-33
     check(pkg, cuda, x, codes, scales, None)
+
+
+@pytest.mark.parametrize('dtype,tokens,width,out', [
+    (torch.bfloat16, 4100, 1290, 2100), (torch.float32, 2600, 650, 3333),    # 256 x 256
+    (torch.float16, 1024, 600, 8192), (torch.bfloat16, 1100, 513, 7100),     # 128 x 256
+    (torch.bfloat16, 1000, 1000, 2100), (torch.float32, 700, 1150, 4099),    # 64 x 128
+    (torch.float16, 512, 1300, 3001), (torch.float32, 1030, 1190, 1800),     # 64 x 64
+    (torch.bfloat16, 200, 2310, 4090), (torch.float16, 300, 2600, 2000),     # in two parts
+    (torch.float16, 67, 5000, 4099), (torch.bfloat16, 67, 2800, 4099),       # 32 x 32 in three
+    (torch.bfloat16, 64, 3700, 8001), (torch.float32, 257, 3300, 1601),      # 64 x 32 in four
+    (torch.float32, 40, 4700, 201), (torch.float16, 31, 8100, 5003)])        # 32 x 32 in four
+def test_long_walks(pkg, cuda, dtype, tokens, width, out):
+    """Rows so long that every tile's ring of buffers goes round twice and more,
+    with ends of tiles and of rows, on each kind of tile."""
+    check(pkg, cuda, *make(tokens, width, out, dtype, width))

@@ -276,3 +276,34 @@ def test_largest_halves(pkg, cuda):
     case, grads = make(12, 64, half, half, seed=7, parts=('x', 'weight'))
     case['x'][torch.arange(12), at] = torch.linspace(65504, 64900, 12).to(half)
     check(pkg, cuda, case, {'normed': 64 * grads['normed']}, 8)
+
+
+@pytest.mark.parametrize('rows,width,types,gate', [
+    (4002, 1283, TYPES[4], 6), (4002, 1280, TYPES[2], 6), (3000, 2056, TYPES[3], 3),
+    (2000, 5000, TYPES[0], None), (1500, 8191, TYPES[4], 'element'), (6000, 640, TYPES[1], 2)])
+@pytest.mark.parametrize('checkpoint', [None, 8])
+def test_many_rows(pkg, cuda, rows, width, types, gate, checkpoint):
+    """Rows of several waves, and many of them for each block: the next row's
+    loads, the places of the sums and what is summed over rows."""
+    check(pkg, cuda, *make(rows, width, *types, seed=rows, gate=gate), checkpoint)
+
+
+def test_no_eps(pkg, cuda):
+    """eps of zero: the formula, and for a row of zeros its quotient of zeros in
+    that row and in the sums over rows, and nowhere else."""
+    case, _ = make(9, 72, torch.float32, torch.float32, seed=8, parts=('x', 'weight'))
+    dev = {n: t.to(cuda).requires_grad_(True) for n, t in case.items()}
+    _, normed = pkg.residual_norm(dev['x'], weight=dev['weight'], eps=0.0)
+    x, w = (case[n].double() for n in ('x', 'weight'))
+    _, want = ref.residual_norm(x, None, None, None, None, w, 0.0)
+    bounds = ref.residual_bounds(x, None, None, None, None, w, 0.0, torch.float32, torch.float32)
+    close(normed, want, bounds['normed'], 'normed')
+    zeros = case['x'].clone()
+    zeros[4] = 0
+    leaf = zeros.to(cuda).requires_grad_(True)
+    for checkpoint in (None, 8):
+        _, y = pkg.residual_norm(leaf, weight=dev['weight'], eps=0.0, checkpoint=checkpoint)
+        dx, dw = torch.autograd.grad(y, (leaf, dev['weight']), torch.ones_like(y))
+        rest = [i for i in range(9) if i != 4]
+        assert y[4].isnan().all() and torch.equal(y[rest], normed[rest])
+        assert dx[4].isnan().all() and dx[rest].isfinite().all() and dw.isnan().all()
