@@ -11,10 +11,12 @@ the same C ABI (``include/bevpool.h``); the reference has no counterpart.
                                weights from :func:`quantize_weight`
 
 The first three have gradients.  With ``checkpoint=8`` the backward pass works
-from 8-bit copies of what the forward read, a little over half of the memory of
-16-bit ones: blocks of 32 values along a row share the least power of two p with
-127 p >= their largest magnitude, and each is rounded to a multiple of p (ties
-to even).  A value that is not finite comes back as NaN, and no other does.
+from 8-bit copies of what the forward read, for wide rows a little over half of
+the memory of 16-bit ones (33 bytes for 32 values, a row's rounded up to whole
+blocks and then to 16 bytes: narrow rows gain less or nothing).  Blocks of 32 values along
+a row share the least power of two p with 127 p >= their largest magnitude, and
+each is rounded to a multiple of p (ties to even; in fp16 at most to its largest
+number).  A value that is not finite comes back as NaN, and no other does.
 
 Rows are the leading dimensions; their strides are free, a row's values are
 copied where they are not neighbours.  Calls run on torch's current stream,
@@ -116,6 +118,8 @@ def residual_norm(x, update=None, *, update_weight=None, scale=None, gate=None, 
     or (groups, width), a row for each of `groups` equal parts of the rows in
     order, or (width,).  width at most 8192.
 
+    With eps of 0 a row of zeros is NaN, as the formula has it.
+
     Gradients flow to all of them.  ``checkpoint=8`` keeps 8-bit copies of x
     and update for them instead of x and update; the gradients are those at
     the values that the copies stand for."""
@@ -210,7 +214,8 @@ def gated_activation(x, kind='silu', *, checkpoint=None):
 
 class PackedActivations:
     """An 8-bit checkpoint of a tensor: :meth:`unpack` gives the values that it
-    stands for, in the tensor's type and shape.  33 bytes for 32 values."""
+    stands for, in the tensor's type and shape.  ``data``: a row of bytes for each
+    row, 33 for 32 values, rounded up to 16 (48 at least)."""
 
     def __init__(self, data, shape, dtype):
         self.data, self.shape, self.dtype = data, shape, dtype
@@ -236,8 +241,9 @@ class _Pack(torch.autograd.Function):
 
 def pack_activations(x):
     """x (..., width) as :class:`PackedActivations`, blocks of 32 values along
-    the width (at most 2^18).  fp16 and bf16 values come back exactly as the
-    type holds them (fp16: the largest at most 65504).  No gradient."""
+    the width (at most 2^18).  Values are rounded to 7 bits of their block's
+    largest; what they stand for fp16 and bf16 hold exactly, so unpacking rounds
+    no more (fp16: 65,536 is 65,504).  No gradient."""
     _check_type('x', x)
     if x.dim() < 1 or not 1 <= x.shape[-1] <= MAX_GATED_WIDTH:
         raise ValueError(f'x must have shape [..., width], width in [1, {MAX_GATED_WIDTH}].')
@@ -254,7 +260,10 @@ def _from_checkpoint(dtype, n, k):
     card's CUs, up to half a tile of 256 x 256 for each.  Above, what the
     checkpoint stands for and a library product are faster.  us of the one and
     of the other: 16,896 tokens of 1280 x 1280 84 and 220, of 1280 x 5120 278 and
-    322, of 10240 x 1280 584 and 522; 4,096 of 4096 x 4096 166 and 137."""
+    322, of 10240 x 1280 584 and 522; 4,096 of 4096 x 4096 166 and 137.  For fewer
+    tokens the one is slower too, and keeps no 16-bit copy: 300, 2,048 and 4,096 of
+    1280 x 1280 27 and 19, 37 and 31, 45 and 47; 512 and 4,096 of 2048 x 4096 41 and
+    27, 96 and 84; 300 and 4,096 of 256 x 256 24 and 28, 25 and 37."""
     return (dtype != torch.float32 and 0 < n <= 1 << 20 and n % 8 == 0
             and -(-n // 256) * -(-k // 256) <= 128)
 

@@ -32,7 +32,17 @@ struct Args {
 
 // Lanes that share a row and chunks that each holds: one, so that few registers
 // hold a row's values and several rows' loads are on their way at once (chunks
-// past 4096 values: two), by whole waves, or parts of one for short rows.
+// past 4096 values: two), by whole waves, or parts of one for short rows.  More
+// lanes hold the last chunk again: us of forward and backward, 43 MB of rows in
+// bf16, by these lanes and by the next layout,
+//   128 values 28 and 51, 38 and 72      512 values 27 and 51, 38 and 72
+//   768 29 and 57, 43 and 78             1024 27 and 56, 32 and 63
+//   1280 30 and 57, 33 and 62            1536 28 and 54, 29 and 55
+//   2048 28 and 55, 42 and 72
+// So rows just past a step lose: 2,304 values 43 and 72, 4,096 35 and 64, 5,120 43
+// and 75 (other data than the above, none of it in the cache).  In fp32 two chunks
+// do not fit the registers beside two rows (14 to 19 are spilled): 43 MB of rows of
+// 4,096 38 and 62 us, of 8,192 63 and 86.
 #define RESIDUAL_LAYOUT(FN, width, ...)                                         \
   if ((width) < 8) FN(16, 1, false, __VA_ARGS__)                                \
   else if ((width) <= 128) FN(16, 1, true, __VA_ARGS__)                         \

@@ -9,10 +9,11 @@
 //          stands for a value that is not finite and comes back as NaN
 // The scale is a power of two, so that neither the quotient nor the product
 // is rounded: the byte depends on nothing but x, and what it stands for has 7
-// bits, exact in bf16.  A value is off by at most 2^-7 of its block's largest
-// magnitude, on average over normal values by 0.7% of their deviation (3 bits
-// of mantissa in 8, the other way to spend them, are 2.6%).
-// A row is the bytes of its blocks, then their scales, padded to 16 bytes.
+// bits, exact in bf16.  A value is off by half a scale at most, which is less than
+// 1/127 of its block's largest magnitude, on average over normal values by 0.7% of
+// their deviation (3 bits of mantissa in 8, the other way to spend them, are 2.6%).
+// A row is the bytes of its blocks, then their scales, padded to 16 bytes: 33
+// bytes for 32 values of wide rows, 48 at least (8 values in 16 bits are 16).
 #pragma once
 
 #include <hip/hip_runtime.h>

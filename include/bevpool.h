@@ -673,7 +673,8 @@ int bevpool_attention_cached(const void *q, int64_t q_row, int64_t q_head, const
  * then a byte for each block's p (its biased exponent), and
  * bevpool_checkpoint_pitch(width) bytes long.  width is at most 2^18.
  *   kept         [rows][bevpool_checkpoint_pitch(width)], from a multiple of 8
- *   out          (rows, width) contiguous (fp16: at most 65504)
+ *   out          (rows, width) contiguous
+ * What stands for 65,536 in fp16 is 65,504 here and in all gradients below.
  */
 int64_t bevpool_checkpoint_pitch(int32_t width);
 
