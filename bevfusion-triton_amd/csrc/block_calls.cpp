@@ -15,6 +15,7 @@
 #include <ATen/ATen.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
+#include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/functions/utils.h>
@@ -284,6 +285,16 @@ variable_list linear_backward(const Linear &A, Tensor dy, Tensor kept, const Ten
 
 // ---- nodes -----------------------------------------------------------------
 
+// A refusal as Python's own error: the only ones whose type the engine carries to
+// the thread that waits for it.
+[[noreturn]] void raise(const CallError &refusal) {
+  const pybind11::gil_scoped_acquire held;
+  PyErr_SetString(call_error ? call_error : PyExc_RuntimeError, refusal.what());
+  python_error error;
+  error.persist();
+  throw error;
+}
+
 // A node keeps tensors; its body gets them back.  Gradients are no functions of
 // the graph's: a second derivative is refused.
 template <int kSaved>
@@ -301,9 +312,11 @@ struct Recorded : public Node {
     for (const SavedVariable &s : saved) kept.push_back(s.unpack());
     const bool followed = at::GradMode::is_enabled();
     variable_list out;
-    {
+    try {
       const at::NoGradGuard none;
       out = body(std::move(grads), kept);
+    } catch (const CallError &refusal) {
+      raise(refusal);
     }
     if (!followed) return out;
     for (Tensor &t : out)

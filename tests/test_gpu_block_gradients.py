@@ -250,3 +250,18 @@ def test_what_does_not_fit_is_refused(pkg, cuda, name, kept):
     got = node(*nothing, douts[-1])
     got = got if isinstance(got, torch.Tensor) else got[0]  # (a node of one input)
     assert torch.equal(got, grads(pkg, name, t, kept, douts)[0])
+
+
+@pytest.mark.gpu
+def test_a_refusal_in_a_backward_pass_is_the_package_s_error(pkg, cuda):
+    """As in the forward, through the autograd engine and from the node."""
+    from bevfusion_triton_amd import _lib
+
+    t = {n: v.requires_grad_(True) for n, v in leaves(cuda).items()}
+    more = lambda s: s[:1].repeat(5, 1) if s.shape == t['gate'].shape else s
+    with torch.autograd.graph.saved_tensors_hooks(lambda s: s, more):
+        out = CALLS['residual_norm'](pkg, t, None)[0]
+        with pytest.raises(_lib.BevPoolError, match='do not divide'):
+            out.grad_fn(torch.ones_like(out), None)
+        with pytest.raises(_lib.BevPoolError, match='do not divide'):
+            out.sum().backward()
