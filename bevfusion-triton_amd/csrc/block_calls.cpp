@@ -252,12 +252,13 @@ variable_list linear_backward(const Linear &A, Tensor dy, Tensor kept, const Ten
   const c10::DeviceGuard device(in.device);
   in.fits(weight, A.type, {weight.dim() ? weight.size(0) : 0, A.width}, "weight");
   const int n = int(weight.size(0)), k = int(A.width), code = code_of(A.type);
-  dy = in.grad(dy, A.type, A.rows, n);
+  if (dy.scalar_type() != A.type) dy = dy.to(A.type);
+  in.fits(dy, A.type, {A.rows, n}, "a gradient");  // (the library takes any layout)
   kept = in.kept(kept, A.rows, A.width);
   if (need_x) grads[0] = dy.mm(weight);
   if (need_weight && A.direct && A.rows) {
     Tensor rows = dy;
-    if (dy.stride(0) % 8 || reinterpret_cast<uintptr_t>(dy.data_ptr()) % 16 ||
+    if (dy.stride(1) != 1 || dy.stride(0) % 8 || reinterpret_cast<uintptr_t>(dy.data_ptr()) % 16 ||
         dy.stride(0) >= (1 << 24))
       rows = dy.clone(at::MemoryFormat::Contiguous);
     grads[1] = at::empty({n, k}, dy.options());
@@ -274,9 +275,10 @@ variable_list linear_backward(const Linear &A, Tensor dy, Tensor kept, const Ten
   }
   if (need_bias) grads[2] = at::empty({n}, dy.options());
   if (need_bias && n > 0) {  // (the sums refuse rows of nothing)
+    const Tensor rows = in.rows(dy, A.type, A.rows, n, "a gradient");
     const size_t need = bevpool_column_sums_scratch_bytes(n);
     const Tensor scratch = bytes(dy, need);
-    check(bevpool_column_sums(at_of(dy), row_of(dy), code, A.rows, n, at_of(grads[2]),
+    check(bevpool_column_sums(at_of(rows), row_of(rows), code, A.rows, n, at_of(grads[2]),
                               at_of(scratch), need, stream()),
           "bevpool_column_sums");
   }
