@@ -24,6 +24,8 @@ allocate with torch's allocator and never wait for the device.
 """
 from __future__ import annotations
 
+import math
+
 import torch
 from torch import nn
 from torch.autograd.function import once_differentiable
@@ -221,10 +223,21 @@ class PackedActivations:
         self.data, self.shape, self.dtype = data, shape, dtype
 
     def unpack(self):
-        out = self.data.new_empty(self.shape, dtype=self.dtype)
+        data, shape = self.data, tuple(self.shape)
+        P.require_gpu(data)
+        if data.dtype != torch.uint8 or self.dtype not in L.DTYPE_CODES:
+            raise TypeError('a checkpoint has bytes of dtype torch.uint8, of values of dtype '
+                            'torch.float16, torch.float32, or torch.bfloat16.')
+        width = shape[-1] if shape else 0
+        pitch = L.library().bevpool_checkpoint_pitch(width)
+        if not 1 <= width <= MAX_GATED_WIDTH or data.shape != (math.prod(shape[:-1]), pitch):
+            raise ValueError(f'data must have shape [rows, {pitch}] for a checkpoint of {shape}.')
+        if not data.is_contiguous() or data.data_ptr() % 16:
+            data = data.clone(memory_format=torch.contiguous_format)
+        out = data.new_empty(shape, dtype=self.dtype)
         _run(lambda lib, s: lib.bevpool_checkpoint_unpack(
-            L.ptr(self.data), L.DTYPE_CODES[self.dtype], self.data.shape[0], self.shape[-1],
-            L.ptr(out), s), self.data.device, 'bevpool_checkpoint_unpack')
+            L.ptr(data), L.DTYPE_CODES[self.dtype], data.shape[0], width, L.ptr(out), s),
+            data.device, 'bevpool_checkpoint_unpack')
         return out
 
 

@@ -446,3 +446,21 @@ def test_what_is_kept(pkg, cuda):
         del out
     assert held[None] == 4096 * 1280 * 2
     assert held[8] == 4096 * 2 * 672  # (rows of 640 codes and 20 scales, at 16 bytes)
+
+
+def test_checkpoints_that_do_not_fit_are_refused(block):
+    """Before any kernel reads them: rows of another length, number or type."""
+    data = torch.zeros((3, 48), dtype=torch.uint8)  # (of rows of 1 to 32 values)
+    for bad, shape in ((data[:, :47], (3, 8)), (data[:2], (3, 8)), (data, (4, 8)), (data, (3, 33)),
+                       (data, (3, 2, 8)), (data[0], (8,)), (data, (0, 8)), (data, (3, 0))):
+        with pytest.raises(ValueError, match='checkpoint'):
+            block.PackedActivations(bad, torch.Size(shape), torch.bfloat16).unpack()
+    for bad, dtype in ((data.to(torch.int8), torch.bfloat16), (data, torch.float64)):
+        with pytest.raises(TypeError, match='dtype'):
+            block.PackedActivations(bad, torch.Size((3, 8)), dtype).unpack()
+
+
+def test_checkpoints_on_the_host_are_refused(pkg):
+    with pytest.raises(RuntimeError, match='ROCm GPU only'):
+        pkg.PackedActivations(torch.zeros((3, 48), dtype=torch.uint8), torch.Size((3, 8)),
+                              torch.bfloat16).unpack()

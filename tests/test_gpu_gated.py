@@ -275,3 +275,14 @@ def test_largest_halves(pkg, cuda):
     assert a.max() == 65504
     want = torch.cat((dout.double() * b, dout.double() * a), -1).to(half)  # (exact products)
     assert torch.equal(got.cpu(), want)
+
+
+def test_checkpoints_laid_out_otherwise(pkg, cuda):
+    """Bytes that have been moved are the same checkpoint wherever they lie."""
+    x = torch.randn((6, 3, 70), device=cuda).bfloat16()
+    packed = pkg.pack_activations(x)
+    want, data = packed.unpack(), packed.data
+    shifted = torch.zeros(data.numel() + 1, dtype=torch.uint8, device=cuda)[1:].view(data.shape)
+    for other in (data.t().contiguous().t(), data.cpu().to(cuda), shifted.copy_(data),
+                  torch.stack((data, data), 1)[:, 0]):
+        assert torch.equal(pkg.PackedActivations(other, packed.shape, packed.dtype).unpack(), want)
